@@ -350,6 +350,98 @@ size_t rosa_hip_router_workspace_bytes(const rosa_router_update* update);
 int rosa_hip_router_update(const rosa_router_update* update, void* stream);
 
 /*
+ * Mixers that stand beside the operator in a model's blocks (no counterpart in the reference):
+ * linear attention with a decay for each head, and attention with a sliding window and sinks.
+ *
+ * Token t of a sequence, query head h, key and value head g = h / (H / Hkv):
+ *   decay:   S_t = exp(log_decay[h]) S_{t-1} + k_t v_t^T,  o_t = scale q_t^T S_t,  S_{-1} = 0 or
+ *            the slot's state;
+ *   window:  o_t = sum_s p_s v_s, p = softmax of scale q_t . k_s over the tokens s <= t with
+ *            t - s < window or s < sinks (0 <= sinks <= 64).
+ *
+ * Layouts as for rosa_problem: dense (B sequences of T tokens, N = B T, S = 0, cu_seqlens NULL) or
+ * packed (N tokens cut by cu_seqlens into S sequences, B = T = 0).  query [.., H, D], key
+ * [.., Hkv, D], value [.., Hkv, Dv]; D and Dv in [1, 128].  Inputs are described by strides in
+ * elements, with neighbouring elements inside a head; outputs and gradients are contiguous
+ * [N, heads, width] in the problem's dtype and fully overwritten.  Sums, states and softmax
+ * statistics are float32.  Results do not depend on the order in which blocks run.  Invalid device
+ * offsets make every output and gradient NaN and leave states and caches as they were.
+ */
+typedef struct rosa_mixer_problem {
+  int dtype;
+  int B, T;      /* dense only */
+  int N, S;
+  int H, Hkv;
+  int D, Dv;
+  float scale;
+  const int32_t* cu_seqlens; /* device, packed layout only */
+} rosa_mixer_problem;
+
+typedef struct rosa_mixer_tensor {
+  const void* data;
+  int64_t batch_stride;  /* dense layout only */
+  int64_t token_stride, head_stride;
+} rosa_mixer_tensor;
+
+/* Workspace of a call: 0 forward, 1 backward, 2 update.  Host arithmetic only; 0 is an error. */
+size_t rosa_hip_decay_workspace_bytes(const rosa_mixer_problem* problem, int call);
+
+/* `log_decay` float32 [H].  The backward writes the gradients whose pointers are not NULL. */
+int rosa_hip_decay_forward(const rosa_mixer_problem* problem, const rosa_mixer_tensor* query,
+                           const rosa_mixer_tensor* key, const rosa_mixer_tensor* value,
+                           const float* log_decay, void* output, void* workspace,
+                           size_t workspace_bytes, void* stream);
+int rosa_hip_decay_backward(const rosa_mixer_problem* problem, const rosa_mixer_tensor* query,
+                            const rosa_mixer_tensor* key, const rosa_mixer_tensor* value,
+                            const rosa_mixer_tensor* grad_output, const float* log_decay,
+                            void* grad_query, void* grad_key, void* grad_value, void* workspace,
+                            size_t workspace_bytes, void* stream);
+
+/*
+ * Serving: the sequences are slots, whose states float32 [slots, H, D, Dv] are read from
+ * `state_in` and left, advanced by the new tokens, in `state_out` (the same array, or one that
+ * does not overlap it).  One token per slot (dense, T = 1) is one launch without a workspace.
+ */
+int rosa_hip_decay_update(const rosa_mixer_problem* problem, const rosa_mixer_tensor* query,
+                          const rosa_mixer_tensor* key, const rosa_mixer_tensor* value,
+                          const float* log_decay, const float* state_in, float* state_out,
+                          void* output, void* workspace, size_t workspace_bytes, void* stream);
+
+/* Workspace of the backward (capacity 0) or of an update of caches of `capacity` rows. */
+size_t rosa_hip_window_workspace_bytes(const rosa_mixer_problem* problem, int window, int sinks,
+                                       int64_t capacity);
+
+/*
+ * `log_sum` (optional) float32 [H, N]: the base-two logarithm of every token's softmax sum, which
+ * the backward takes together with the forward's output.
+ */
+int rosa_hip_window_forward(const rosa_mixer_problem* problem, int window, int sinks,
+                            const rosa_mixer_tensor* query, const rosa_mixer_tensor* key,
+                            const rosa_mixer_tensor* value, void* output, float* log_sum,
+                            void* stream);
+int rosa_hip_window_backward(const rosa_mixer_problem* problem, int window, int sinks,
+                             const rosa_mixer_tensor* query, const rosa_mixer_tensor* key,
+                             const rosa_mixer_tensor* value, const void* output,
+                             const float* log_sum, const rosa_mixer_tensor* grad_output,
+                             void* grad_query, void* grad_key, void* grad_value, void* workspace,
+                             size_t workspace_bytes, void* stream);
+
+/*
+ * Serving: the sequences are slots with caches [slots, Hkv, capacity, D] and [.., Dv] of the
+ * problem's dtype, contiguous, capacity >= sinks + window.  Position p lies on row p for
+ * p < sinks and on row sinks + (p - sinks) mod (capacity - sinks) otherwise.  `lengths` int32
+ * [slots] (device): the tokens that each slot has seen, which the call reads and leaves to the
+ * caller to advance (the layers of a model share them); below 2^31 - 1024 together with the new
+ * tokens, negative ones count as 0.  The new tokens attend to what their
+ * slot holds and to each other and are then put on their rows.
+ */
+int rosa_hip_window_update(const rosa_mixer_problem* problem, int window, int sinks,
+                           const rosa_mixer_tensor* query, const rosa_mixer_tensor* key,
+                           const rosa_mixer_tensor* value, void* key_cache, void* value_cache,
+                           int64_t capacity, const int32_t* lengths, void* output, void* workspace,
+                           size_t workspace_bytes, void* stream);
+
+/*
  * Invalid device cu_seqlens values (not starting at 0, decreasing, or not ending
  * at N) cannot be seen by the host without a synchronisation.  The reference
  * aborts the process with a device assert (rosa_soft_kernels.cu:287-308); here no

@@ -31,6 +31,14 @@ _OPERATORS = (
     "hard_forward_varlen",
     "surrogate_vjp_masked",
     "surrogate_vjp_varlen_masked",
+    # rosa_soft_amd.mixers
+    "decay_attention",
+    "decay_attention_vjp",
+    "decay_attention_update",
+    "decay_attention_update_out",
+    "window_attention",
+    "window_attention_vjp",
+    "window_attention_update",
 )
 
 

@@ -29,11 +29,17 @@ HIP_SOURCE = os.path.join(HERE, "csrc", "rosa_kernels.hip")
 INSTANCES_SOURCE = os.path.join(HERE, "csrc", "rosa_vjp_instances.hip")
 TILE_FAMILIES = [(1, 8, 1), (1, 8, 2), (1, 16, 1), (1, 16, 2), (1, 32, 1), (1, 32, 2),
                  (2, 64, 1), (2, 64, 2)]
+# the mixers: checks and work division in one unit, kernels once per element type and operator
+MIXER_SOURCE = os.path.join(HERE, "csrc", "mixers.hip")
+MIXER_INSTANCES_SOURCE = os.path.join(HERE, "csrc", "mixer_instances.hip")
+MIXER_TYPES = [("float", "float32"), ("_Float16", "float16"), ("__bf16", "bfloat16")]
 HIP_HEADERS = [os.path.join(HERE, "csrc", name)
-               for name in ("rosa_device_common.hpp", "rosa_vjp_bands.hpp")]
+               for name in ("rosa_device_common.hpp", "rosa_vjp_bands.hpp", "mixer_calls.hpp",
+                            "mixer_device.hpp", "decay_attention.hpp", "window_attention.hpp")]
 OBJECT_DIR = os.path.join(HERE, "build_objects")
 HIP_LIBRARY = os.path.join(HERE, "librosa_soft_hip.so")
-DISPATCH_SOURCE = os.path.join(HERE, "csrc", "rosa_dispatch.cpp")
+DISPATCH_SOURCES = [os.path.join(HERE, "csrc", name)
+                    for name in ("rosa_dispatch.cpp", "mixer_dispatch.cpp")]
 # registers, spills, scratch and LDS of every kernel, as the compiler reported them
 RESOURCE_REPORT = os.path.join(HERE, "kernel_resources.json")
 
@@ -110,7 +116,7 @@ def source_digest() -> str:
     resource report or a counter summary must name to speak for the library in the tree."""
 
     digest = hashlib.sha256()
-    for path in (HIP_SOURCE, INSTANCES_SOURCE, *HIP_HEADERS):
+    for path in (HIP_SOURCE, INSTANCES_SOURCE, MIXER_SOURCE, MIXER_INSTANCES_SOURCE, *HIP_HEADERS):
         with open(path, "rb") as handle:
             digest.update(handle.read())
     digest.update(" ".join(HIPCC_FLAGS).encode())
@@ -118,10 +124,10 @@ def source_digest() -> str:
 
 
 def build_hip_library() -> str:
-    """Compile the main translation unit and the eight tile families side by side, then link.
+    """Compile the translation units (main, eight tile families, mixers) side by side, then link.
 
     One compiler process per translation unit; the families take one to two minutes each,
-    which is also the build's wall time on eight cores."""
+    which is also most of the build's wall time on eight cores."""
 
     from concurrent.futures import ThreadPoolExecutor
 
@@ -135,6 +141,13 @@ def build_hip_library() -> str:
                       f"-DROSA_FAMILY_NVW={nvw}", f"-DROSA_FAMILY_DVP={dvp}",
                       f"-DROSA_FAMILY_DT={symbol_tiles}", "-c", INSTANCES_SOURCE],
                      os.path.join(OBJECT_DIR, f"rosa_vjp_{nvw}_{dvp}_{symbol_tiles}.o")))
+    jobs.append(([hipcc, *HIPCC_FLAGS, "-c", MIXER_SOURCE], os.path.join(OBJECT_DIR, "mixers.o")))
+    for element, name in MIXER_TYPES:
+        for window, operator in ((0, "decay"), (1, "window")):
+            jobs.append(([hipcc, *HIPCC_FLAGS, "-Rpass-analysis=kernel-resource-usage",
+                          f"-DROSA_MIXER_TYPE={element}", f"-DROSA_MIXER_NAME={name}",
+                          f"-DROSA_MIXER_WINDOW={window}", "-c", MIXER_INSTANCES_SOURCE],
+                         os.path.join(OBJECT_DIR, f"mixer_{operator}_{name}.o")))
 
     def compile_one(job):
         command = [*job[0], "-o", job[1]]
@@ -170,7 +183,7 @@ def build_dispatcher() -> str:
         "g++", "-O2", "-std=c++17", "-fPIC", "-shared",
         "-D__HIP_PLATFORM_AMD__=1", "-DUSE_ROCM=1", "-DTORCH_EXTENSION_NAME=_C",
         "-D_GLIBCXX_USE_CXX11_ABI=1",
-        *include_flags, DISPATCH_SOURCE, "-o", output,
+        *include_flags, *DISPATCH_SOURCES, "-o", output,
         *library_flags, f"-L{HERE}", "-lrosa_soft_hip",
         "-lc10", "-lc10_hip", "-ltorch_cpu", "-ltorch_hip", "-ltorch",
         f"-L{ROCM_HOME}/lib", "-lamdhip64",

@@ -47,6 +47,14 @@ EXPORTED_SYMBOLS = (
     "rosa_hip_surrogate_vjp",
     "rosa_hip_router_update",
     "rosa_hip_router_workspace_bytes",
+    "rosa_hip_decay_workspace_bytes",
+    "rosa_hip_decay_forward",
+    "rosa_hip_decay_backward",
+    "rosa_hip_decay_update",
+    "rosa_hip_window_workspace_bytes",
+    "rosa_hip_window_forward",
+    "rosa_hip_window_backward",
+    "rosa_hip_window_update",
     "rosa_hip_read_offset_error",
     "rosa_hip_stage_timing",
     "rosa_hip_stage_count",
@@ -102,6 +110,35 @@ class RosaRouterUpdate(ctypes.Structure):
         ("workspace", ctypes.c_void_p),
         ("workspace_bytes", ctypes.c_size_t),
         ("history_lengths_out", ctypes.c_void_p),
+    ]
+
+
+class RosaMixerProblem(ctypes.Structure):
+    """``rosa_mixer_problem`` of ``include/rosa_soft_hip.h``."""
+
+    _fields_ = [
+        ("dtype", ctypes.c_int),
+        ("B", ctypes.c_int),
+        ("T", ctypes.c_int),
+        ("N", ctypes.c_int),
+        ("S", ctypes.c_int),
+        ("H", ctypes.c_int),
+        ("Hkv", ctypes.c_int),
+        ("D", ctypes.c_int),
+        ("Dv", ctypes.c_int),
+        ("scale", ctypes.c_float),
+        ("cu_seqlens", ctypes.c_void_p),
+    ]
+
+
+class RosaMixerTensor(ctypes.Structure):
+    """``rosa_mixer_tensor`` of ``include/rosa_soft_hip.h``."""
+
+    _fields_ = [
+        ("data", ctypes.c_void_p),
+        ("batch_stride", ctypes.c_int64),
+        ("token_stride", ctypes.c_int64),
+        ("head_stride", ctypes.c_int64),
     ]
 
 
@@ -195,6 +232,31 @@ def load() -> ctypes.CDLL:
         problem_p, vp, vp, vp, vp, vp, vp, vp,
         ctypes.c_float, ctypes.c_float, ctypes.c_float, ctypes.c_float, ctypes.c_int,
         vp, vp, vp, vp, ctypes.c_size_t, vp,
+    ]
+    mixer_p, tensor_p = ctypes.POINTER(RosaMixerProblem), ctypes.POINTER(RosaMixerTensor)
+    sized = [vp, ctypes.c_size_t, vp]  # workspace, its bytes, stream
+    library.rosa_hip_decay_workspace_bytes.restype = ctypes.c_size_t
+    library.rosa_hip_decay_workspace_bytes.argtypes = [mixer_p, ctypes.c_int]
+    library.rosa_hip_decay_forward.restype = ctypes.c_int
+    library.rosa_hip_decay_forward.argtypes = [mixer_p, *[tensor_p] * 3, vp, vp, *sized]
+    library.rosa_hip_decay_backward.restype = ctypes.c_int
+    library.rosa_hip_decay_backward.argtypes = [mixer_p, *[tensor_p] * 4, vp, vp, vp, vp, *sized]
+    library.rosa_hip_decay_update.restype = ctypes.c_int
+    library.rosa_hip_decay_update.argtypes = [mixer_p, *[tensor_p] * 3, vp, vp, vp, vp, *sized]
+    library.rosa_hip_window_workspace_bytes.restype = ctypes.c_size_t
+    library.rosa_hip_window_workspace_bytes.argtypes = [
+        mixer_p, ctypes.c_int, ctypes.c_int, ctypes.c_int64,
+    ]
+    masked = [mixer_p, ctypes.c_int, ctypes.c_int]  # problem, window, sinks
+    library.rosa_hip_window_forward.restype = ctypes.c_int
+    library.rosa_hip_window_forward.argtypes = [*masked, *[tensor_p] * 3, vp, vp, vp]
+    library.rosa_hip_window_backward.restype = ctypes.c_int
+    library.rosa_hip_window_backward.argtypes = [
+        *masked, *[tensor_p] * 3, vp, vp, tensor_p, vp, vp, vp, *sized,
+    ]
+    library.rosa_hip_window_update.restype = ctypes.c_int
+    library.rosa_hip_window_update.argtypes = [
+        *masked, *[tensor_p] * 3, vp, vp, ctypes.c_int64, vp, vp, *sized,
     ]
     library.rosa_hip_read_offset_error.restype = ctypes.c_int
     library.rosa_hip_read_offset_error.argtypes = [vp, vp]

@@ -1,0 +1,639 @@
+// Linear attention with a decay for each head.
+//
+//   S_t = lambda S_{t-1} + k_t v_t^T,   o_t = scale q_t^T S_t
+//
+// A chunk of 64 tokens that starts from the state S is three products (i, j inside the chunk):
+//   o_i = scale (lambda^(i+1) q_i^T S + sum_{j<=i} lambda^(i-j) (q_i . k_j) v_j)
+//   S'  = lambda^64 S + sum_j lambda^(63-j) k_j v_j^T
+// so a block walks its sequence chunk by chunk with the state in the registers of its four
+// waves: one pass over the data, no state in memory.
+//
+// The gradients are the same operator on other operands, two of them from the last token to the
+// first:  dq = F(dO, v, k),  dv = F_reversed(k, q, dO),  dk = F_reversed(v, dO, q).
+#pragma once
+
+#include "mixer_calls.hpp"
+#include "mixer_device.hpp"
+
+namespace rosa_mixer {
+
+constexpr int kChunk = 64;
+
+template <typename T>
+struct DecayPass {
+  View<const T> query, key, value;
+  int query_share, key_share, value_share;  // heads of the call to one head of the tensor
+  int key_width, value_width;
+  T* out;                                    // [tokens][H][value_width]
+  float* partial;                            // instead of it: before the sum over shared heads
+  bool reverse, whole;
+};
+
+template <typename T>
+struct DecayArgs {
+  DecayPass<T> pass[3];
+  int passes, heads, slices, segment;
+  int64_t slots, items;
+  Sequences sequences;
+  const float* log_decay;
+  float scale;
+  float* segment_states;                     // [pass][slot][head][key_width][value_width] or null
+  const float* state_in;                     // [sequence][head][key_width][value_width] or null
+  float* state_out;
+};
+
+// Terms of a value times its weight in the state's sum.  The state is a float32 sum, so its
+// bfloat16 operands are split: three terms where the state itself is an answer (2^-25 relative),
+// fewer where it is only read again through 16-bit operands.
+template <typename T>
+using StateType = std::conditional_t<sizeof(T) == 4, float, __bf16>;
+
+template <typename T, int WIDTH, int SLICE, int TERMS, bool STATE_ONLY>
+__global__ __launch_bounds__(kThreads) void decay_chunks_kernel(DecayArgs<T> a) {
+  using ST = StateType<T>;
+  constexpr int kColTiles = SLICE / 16;
+  constexpr int kTiles = WIDTH / 16 * kColTiles / 4;   // state tiles of a wave
+  constexpr int kWaveCols = kTiles < kColTiles ? kTiles : kColTiles;
+  constexpr int kWaveRows = kTiles / kWaveCols;
+  constexpr int kSteps = WIDTH / 32;
+
+  __shared__ __attribute__((aligned(16))) T keys[kChunk * kPitch<T, WIDTH>];
+  __shared__ __attribute__((aligned(16))) T values[STATE_ONLY ? 16 : kChunk * kPitch<T, SLICE>];
+  __shared__ __attribute__((aligned(16))) ST weighted[TERMS * kChunk * kPitch<ST, SLICE>];
+  __shared__ __attribute__((aligned(16))) T state_rows[STATE_ONLY ? 16 : SLICE * kPitch<T, WIDTH>];
+  __shared__ float largest[4];
+
+  const int64_t item = item_of_block(a.items);
+  if (item >= a.items) return;
+  const int tid = threadIdx.x, lane = tid & 63, group = lane >> 4, column = lane & 15;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int slice = static_cast<int>(item % a.slices);
+  const int64_t slot = item / a.slices % a.slots;
+  const int head = static_cast<int>(item / a.slices / a.slots % a.heads);
+  const int pass_index = static_cast<int>(item / a.slices / a.slots / a.heads);
+  const DecayPass<T>& p = a.pass[pass_index];
+  const int col0 = slice * SLICE;
+  if (col0 >= p.value_width) return;
+
+  Run run;
+  const Found found = find_run(a.sequences, slot, a.segment, tid, &run);
+  const int64_t state_size = static_cast<int64_t>(p.key_width) * p.value_width;
+  if (found != Found::kRun) {
+    if constexpr (!STATE_ONLY) {
+      if (found == Found::kInvalid) {  // no offset can be relied on: everything is NaN
+        const int64_t first = slot * a.segment;
+        const int64_t last = min(first + a.segment, static_cast<int64_t>(a.sequences.tokens));
+        if (slice == 0) {
+          fill_nan(p.partial ? nullptr : p.out, first, last, a.heads, head, p.value_width, tid);
+          fill_nan(p.partial, first, last, a.heads, head, p.value_width, tid);
+        }
+      }
+      // a slot without new tokens keeps its state
+      const int64_t kept = found == Found::kInvalid ? slot : run.length == 0 ? run.sequence : -1;
+      if (slice == 0 && a.state_out != a.state_in && kept >= 0 && kept < a.sequences.count &&
+          (found == Found::kInvalid || run.tile == 0)) {
+        const int64_t at = (kept * a.heads + head) * state_size;
+        for (int64_t e = tid; e < state_size; e += kThreads) a.state_out[at + e] = a.state_in[at + e];
+      }
+    }
+    return;
+  }
+  const int start = run.tile * a.segment;                       // in the order of the walk
+  const int stop = min(start + a.segment, run.length);
+  if (STATE_ONLY && stop == run.length) return;                 // nothing follows this segment
+  const float rate = a.log_decay[head] * 1.4426950408889634f;
+
+  // the walk's token i of this sequence
+  const auto token = [&](int i) { return run.begin + (p.reverse ? run.length - 1 - i : i); };
+  const int query_head = head / p.query_share, key_head = head / p.key_share,
+            value_head = head / p.value_share;
+
+  // state rows (key columns) and columns (value columns) of this wave's tiles
+  const int row_tile = wave * kTiles / kColTiles, col_tile = wave * kTiles % kColTiles;
+  f32x4 state[kWaveRows][kWaveCols];
+  {
+    const float* from = nullptr;
+    if (!STATE_ONLY && a.segment_states != nullptr)
+      from = a.segment_states + ((pass_index * a.slots + slot) * a.heads + head) * state_size;
+    else if (!STATE_ONLY && a.state_in != nullptr)
+      from = a.state_in + (static_cast<int64_t>(run.sequence) * a.heads + head) * state_size;
+#pragma unroll
+    for (int i = 0; i < kWaveRows; ++i)
+#pragma unroll
+      for (int j = 0; j < kWaveCols; ++j)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          const int row = (row_tile + i) * 16 + 4 * group + r, col = col0 + (col_tile + j) * 16 + column;
+          state[i][j][r] = from != nullptr && row < p.key_width && col < p.value_width
+                               ? from[static_cast<int64_t>(row) * p.value_width + col]
+                               : 0.0f;
+        }
+  }
+
+  float weight[4][4];  // lambda^(i - j) of this lane's query row i and key rows j, 0 for j > i
+  const int own = wave * 16 + column;
+  if constexpr (!STATE_ONLY) {
+#pragma unroll
+    for (int t = 0; t < 4; ++t)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        const int apart = own - (t * 16 + 4 * group + r);
+        weight[t][r] = apart >= 0 ? power_of(rate, apart) : 0.0f;
+      }
+  }
+
+  TileMove<T, kChunk, WIDTH> key_move;
+  TileMove<T, kChunk, SLICE> value_move;
+  Frag<T> next_query[kSteps];
+  const auto fetch = [&](int at) {
+    key_move.fetch(
+        [&](int i) -> const T* {
+          return at + i < stop ? p.key.row(run.batch, token(at + i), key_head) : nullptr;
+        },
+        p.key_width, p.whole, tid);
+    value_move.fetch(
+        [&](int i) -> const T* {
+          return at + i < stop ? p.value.row(run.batch, token(at + i), value_head) + col0 : nullptr;
+        },
+        p.value_width - col0, p.whole, tid);
+    if constexpr (!STATE_ONLY) {
+      const T* row = at + own < stop ? p.query.row(run.batch, token(at + own), query_head) : nullptr;
+#pragma unroll
+      for (int s = 0; s < kSteps; ++s)
+        next_query[s] = memory_operand(row, s * 32 + 8 * group, p.key_width, p.whole);
+    }
+  };
+  fetch(start);
+
+  float unit = 1.0f;  // float16: brings the rounded state into range
+  if constexpr (kNarrow<T> && !STATE_ONLY) {
+    float most = 0.0f;
+#pragma unroll
+    for (int i = 0; i < kWaveRows; ++i)
+#pragma unroll
+      for (int j = 0; j < kWaveCols; ++j)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) most = fmaxf(most, fabsf(state[i][j][r]));
+    for (int apart = 1; apart < 64; apart *= 2) most = fmaxf(most, __shfl_xor(most, apart));
+    if (lane == 0) largest[wave] = most;
+    __syncthreads();
+  }
+
+  for (int at = start; at < stop; at += kChunk) {
+    const int fill = min(kChunk, stop - at);
+    // what this chunk reads goes to LDS: keys, values, weighted values, the state before it
+    key_move.store(keys, tid);
+    if constexpr (!STATE_ONLY) value_move.store(values, tid);
+#pragma unroll
+    for (int i = 0; i < value_move.kPieces; ++i) {
+      constexpr int kElements = value_move.kElements, kPerRow = value_move.kPerRow;
+      const int piece = i * kThreads + tid, row = piece / kPerRow;
+      const float by = row < fill ? power_of(rate, fill - 1 - row) : 0.0f;
+      float left[kElements];
+#pragma unroll
+      for (int e = 0; e < kElements; ++e) left[e] = static_cast<float>(value_move.held[i][e]) * by;
+#pragma unroll
+      for (int t = 0; t < TERMS; ++t) {
+        typedef ST Piece __attribute__((ext_vector_type(kElements)));
+        Piece term;
+#pragma unroll
+        for (int e = 0; e < kElements; ++e) {
+          term[e] = static_cast<ST>(left[e]);
+          left[e] -= static_cast<float>(term[e]);
+        }
+        *reinterpret_cast<Piece*>(weighted + (t * kChunk + row) * kPitch<ST, SLICE> +
+                                  piece % kPerRow * kElements) = term;
+      }
+    }
+    if constexpr (!STATE_ONLY) {
+      if constexpr (kNarrow<T>) {
+        const float most = fmaxf(fmaxf(largest[0], largest[1]), fmaxf(largest[2], largest[3]));
+        unit = lift_of(most);
+      }
+#pragma unroll
+      for (int i = 0; i < kWaveRows; ++i)
+#pragma unroll
+        for (int j = 0; j < kWaveCols; ++j) {
+          Quad<T> rounded;
+#pragma unroll
+          for (int r = 0; r < 4; ++r) rounded[r] = static_cast<T>(state[i][j][r] * unit);
+          *reinterpret_cast<Quad<T>*>(state_rows +
+                                      ((col_tile + j) * 16 + column) * kPitch<T, WIDTH> +
+                                      (row_tile + i) * 16 + 4 * group) = rounded;
+        }
+    }
+    Frag<T> query[kSteps];
+    if constexpr (!STATE_ONLY) {
+#pragma unroll
+      for (int s = 0; s < kSteps; ++s) query[s] = next_query[s];
+    }
+    __syncthreads();
+    if (at + kChunk < stop) fetch(at + kChunk);
+
+    if constexpr (!STATE_ONLY) {
+      if (wave * 16 < fill) {
+        // outputs transposed: rows are value columns, columns are this wave's 16 tokens
+        f32x4 out[kColTiles];
+#pragma unroll
+        for (int t = 0; t < kColTiles; ++t) out[t] = f32x4(0.0f);
+#pragma unroll
+        for (int s = 0; s < kSteps; ++s)
+#pragma unroll
+          for (int t = 0; t < kColTiles; ++t)
+            out[t] = mma(row_operand<T, WIDTH>(state_rows, t * 16, s * 32, lane), query[s], out[t]);
+        float carried = power_of(rate, own + 1);
+        f32x4 score[4];
+#pragma unroll
+        for (int t = 0; t < 4; ++t) {
+          score[t] = f32x4(0.0f);
+          if (t <= wave) {
+#pragma unroll
+            for (int s = 0; s < kSteps; ++s)
+              score[t] = mma(row_operand<T, WIDTH>(keys, t * 16, s * 32, lane), query[s], score[t]);
+#pragma unroll
+            for (int r = 0; r < 4; ++r)  // (a select, so that keys behind a token never reach it)
+              score[t][r] = weight[t][r] == 0.0f ? 0.0f : score[t][r] * weight[t][r];
+          }
+        }
+        float range = 1.0f;  // float16: the same for the scores of a token
+        if constexpr (kNarrow<T>) {
+          carried /= unit;
+          float most = 0.0f;
+#pragma unroll
+          for (int t = 0; t < 4; ++t)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) most = fmaxf(most, fabsf(score[t][r]));
+          range = lift_of(over_groups_max(most));
+#pragma unroll
+          for (int t = 0; t < 4; ++t) score[t] *= range;
+          carried *= range;
+        }
+#pragma unroll
+        for (int t = 0; t < kColTiles; ++t) out[t] *= carried;
+#pragma unroll
+        for (int half = 0; half < 2; ++half) {
+          if (2 * half <= wave) {
+            const Frag<T> scores = operand_of<T>(score[2 * half], score[2 * half + 1]);
+#pragma unroll
+            for (int t = 0; t < kColTiles; ++t)
+              out[t] = mma(column_operand<T, SLICE>(values, half * 32, t * 16, lane), scores, out[t]);
+          }
+        }
+        if (own < fill) {
+          const int64_t row =
+              ((run.first + token(at + own) - run.begin) * a.heads + head) * p.value_width + col0;
+          const bool quads = p.value_width % 4 == 0;
+          const float by = a.scale / range;
+#pragma unroll
+          for (int t = 0; t < kColTiles; ++t) {
+            if (p.partial != nullptr)
+              store4(p.partial + row, t * 16 + 4 * group, out[t] * by, p.value_width - col0, quads);
+            else
+              store4(p.out + row, t * 16 + 4 * group, out[t] * by, p.value_width - col0, quads);
+          }
+        }
+      }
+    }
+
+    // the state behind the chunk
+    const float decay = power_of(rate, fill);
+#pragma unroll
+    for (int i = 0; i < kWaveRows; ++i)
+#pragma unroll
+      for (int j = 0; j < kWaveCols; ++j) state[i][j] *= decay;
+#pragma unroll
+    for (int half = 0; half < 2; ++half) {
+      if (half * 32 >= fill) break;
+      Frag<ST> value[TERMS][kWaveCols];
+#pragma unroll
+      for (int t = 0; t < TERMS; ++t)
+#pragma unroll
+        for (int j = 0; j < kWaveCols; ++j)
+          value[t][j] = column_operand<ST, SLICE>(weighted + t * kChunk * kPitch<ST, SLICE>, half * 32,
+                                                  (col_tile + j) * 16, lane);
+#pragma unroll
+      for (int i = 0; i < kWaveRows; ++i) {
+        const Frag<T> key = column_operand<T, WIDTH>(keys, half * 32, (row_tile + i) * 16, lane);
+        if constexpr (std::is_same_v<T, _Float16>) {
+          // a float16 is the sum of two bfloat16
+          Frag<__bf16> high, low;
+#pragma unroll
+          for (int e = 0; e < 8; ++e) {
+            high[e] = static_cast<__bf16>(static_cast<float>(key[e]));
+            low[e] = static_cast<__bf16>(static_cast<float>(key[e]) - static_cast<float>(high[e]));
+          }
+#pragma unroll
+          for (int t = 0; t < TERMS; ++t)
+#pragma unroll
+            for (int j = 0; j < kWaveCols; ++j) {
+              state[i][j] = mma(high, value[t][j], state[i][j]);
+              if (t == 0 || t + 1 < TERMS) state[i][j] = mma(low, value[t][j], state[i][j]);
+            }
+        } else {
+#pragma unroll
+          for (int t = 0; t < TERMS; ++t)
+#pragma unroll
+            for (int j = 0; j < kWaveCols; ++j) state[i][j] = mma(key, value[t][j], state[i][j]);
+        }
+      }
+    }
+    if constexpr (kNarrow<T> && !STATE_ONLY) {
+      float most = 0.0f;
+#pragma unroll
+      for (int i = 0; i < kWaveRows; ++i)
+#pragma unroll
+        for (int j = 0; j < kWaveCols; ++j)
+#pragma unroll
+          for (int r = 0; r < 4; ++r) most = fmaxf(most, fabsf(state[i][j][r]));
+      for (int apart = 1; apart < 64; apart *= 2) most = fmaxf(most, __shfl_xor(most, apart));
+      if (lane == 0) largest[wave] = most;
+    }
+    __syncthreads();
+  }
+
+  float* to = nullptr;
+  if (STATE_ONLY)
+    to = a.segment_states + ((pass_index * a.slots + slot) * a.heads + head) * state_size;
+  else if (a.state_out != nullptr && stop == run.length)
+    to = a.state_out + (static_cast<int64_t>(run.sequence) * a.heads + head) * state_size;
+  if (to != nullptr) {
+#pragma unroll
+    for (int i = 0; i < kWaveRows; ++i)
+#pragma unroll
+      for (int j = 0; j < kWaveCols; ++j)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          const int row = (row_tile + i) * 16 + 4 * group + r, col = col0 + (col_tile + j) * 16 + column;
+          if (row < p.key_width && col < p.value_width)
+            to[static_cast<int64_t>(row) * p.value_width + col] = state[i][j][r];
+        }
+  }
+}
+
+// What every segment starts from: the segments' own sums, in their place, become the states before
+// them.  One thread per element of a state, in the order of the segments.
+template <typename T>
+__global__ __launch_bounds__(kThreads) void decay_join_kernel(DecayArgs<T> a, int64_t state_size) {
+  const int tid = threadIdx.x;
+  const int64_t pieces = (state_size + kThreads - 1) / kThreads, row = blockIdx.x / pieces;
+  const int head = static_cast<int>(row % a.heads);
+  const int pass_index = static_cast<int>(row / a.heads % a.passes);
+  const int sequence = static_cast<int>(row / a.heads / a.passes);
+  Run run;
+  if (a.sequences.offsets == nullptr) {
+    run.sequence = sequence;
+    run.begin = 0;
+    run.length = a.sequences.length;
+  } else {
+    int bad = 0;
+    for (int s = tid; s < a.sequences.count; s += kThreads)
+      bad |= a.sequences.offsets[s] > a.sequences.offsets[s + 1] ||
+             (s == 0 && a.sequences.offsets[0] != 0) ||
+             (s == a.sequences.count - 1 && a.sequences.offsets[s + 1] != a.sequences.tokens);
+    if (__syncthreads_or(bad)) return;
+    run.sequence = sequence;
+    run.begin = a.sequences.offsets[sequence];
+    run.length = a.sequences.offsets[sequence + 1] - static_cast<int>(run.begin);
+  }
+  const int64_t slot = first_slot(a.sequences, run, a.segment);
+  const int64_t e = blockIdx.x % pieces * kThreads + tid;
+  if (e >= state_size) return;
+  const int segments = (run.length + a.segment - 1) / a.segment;
+  const float decay = power_of(a.log_decay[head] * 1.4426950408889634f, a.segment);
+  float state = a.state_in == nullptr
+                    ? 0.0f
+                    : a.state_in[(static_cast<int64_t>(sequence) * a.heads + head) * state_size + e];
+  float* at = a.segment_states + ((pass_index * a.slots + slot) * a.heads + head) * state_size + e;
+  const int64_t step = a.heads * state_size;
+  for (int s = 0; s < segments; ++s) {
+    const float own = s + 1 < segments ? at[s * step] : 0.0f;
+    at[s * step] = state;
+    state = decay * state + own;
+  }
+}
+
+// Gradients of a head of keys or values shared by `share` query heads: their sum, in order.
+template <typename T>
+__global__ __launch_bounds__(kThreads) void sum_shared_kernel(const float* partial, T* out,
+                                                              int64_t rows, int share, int width) {
+  const int64_t e = static_cast<int64_t>(blockIdx.x) * kThreads + threadIdx.x;
+  if (e >= rows * width) return;
+  const int64_t row = e / width, col = e % width;
+  float sum = 0.0f;
+  for (int s = 0; s < share; ++s) sum += partial[(row * share + s) * width + col];
+  out[e] = static_cast<T>(sum);
+}
+
+// ---------------------------------------------------------------------------
+// one token: the state is read, advanced, applied and written, once
+// ---------------------------------------------------------------------------
+
+template <typename T>
+struct DecayTokenArgs {
+  View<const T> query, key, value;
+  const float* log_decay;
+  const float* state_in;
+  float* state_out;
+  T* out;
+  int heads, share, key_width, value_width, slice;  // value columns of a block
+  float scale;
+};
+
+// VEC neighbouring columns per thread, the rows dealt out to the threads that are left.
+template <typename T, int VEC>
+__global__ __launch_bounds__(kThreads) void decay_token_kernel(DecayTokenArgs<T> a) {
+  __shared__ float query[kMostWidth], key[kMostWidth];
+  __shared__ float sums[kThreads * VEC];
+  const int tid = threadIdx.x;
+  const int slices = (a.value_width + a.slice - 1) / a.slice;
+  const int col0 = blockIdx.x % slices * a.slice;
+  const int head = blockIdx.x / slices % a.heads, batch = blockIdx.x / slices / a.heads;
+  const int columns = min(a.slice, a.value_width - col0);
+  if (tid < a.key_width) {
+    query[tid] = static_cast<float>(a.query.row(batch, 0, head)[tid]);
+    key[tid] = static_cast<float>(a.key.row(batch, 0, head / a.share)[tid]);
+  }
+  const int across = a.slice / VEC, rows = kThreads / across;
+  const int col = tid % across * VEC, row0 = tid / across;
+  const bool there = col < columns && row0 < rows;
+  float value[VEC], sum[VEC];
+#pragma unroll
+  for (int e = 0; e < VEC; ++e) {
+    value[e] = there ? static_cast<float>(a.value.row(batch, 0, head / a.share)[col0 + col + e]) : 0.0f;
+    sum[e] = 0.0f;
+  }
+  const float decay = power_of(a.log_decay[head] * 1.4426950408889634f, 1);
+  __syncthreads();
+  typedef float Piece __attribute__((ext_vector_type(VEC)));
+  const int64_t at = (static_cast<int64_t>(batch) * a.heads + head) * a.key_width * a.value_width +
+                     col0 + col;
+  if (there) {
+#pragma unroll 4
+    for (int d = row0; d < a.key_width; d += rows) {
+      const int64_t place = at + static_cast<int64_t>(d) * a.value_width;
+      Piece state = *reinterpret_cast<const Piece*>(a.state_in + place);
+#pragma unroll
+      for (int e = 0; e < VEC; ++e) {
+        state[e] = decay * state[e] + key[d] * value[e];
+        sum[e] += query[d] * state[e];
+      }
+      *reinterpret_cast<Piece*>(a.state_out + place) = state;
+    }
+  }
+#pragma unroll
+  for (int e = 0; e < VEC; ++e) sums[tid * VEC + e] = sum[e];
+  __syncthreads();
+  for (int c = tid; c < columns; c += kThreads) {
+    float total = 0.0f;
+    for (int r = 0; r < rows; ++r) total += sums[r * across * VEC + c];
+    a.out[(static_cast<int64_t>(batch) * a.heads + head) * a.value_width + col0 + c] =
+        static_cast<T>(total * a.scale);
+  }
+}
+
+// ---------------------------------------------------------------------------
+// launches
+// ---------------------------------------------------------------------------
+
+template <typename T, int WIDTH, int TERMS>
+void decay_walk(DecayArgs<T>& args, const DecayPlan& plan, hipStream_t stream) {
+  constexpr int kSlice = WIDTH < 64 ? WIDTH : 64;
+  int widest = 0;
+  for (int i = 0; i < args.passes; ++i)
+    widest = args.pass[i].value_width > widest ? args.pass[i].value_width : widest;
+  args.slices = (widest + kSlice - 1) / kSlice;
+  args.segment = plan.segment;
+  args.slots = plan.slots;
+  args.items = args.passes * plan.slots * args.heads * args.slices;
+  const dim3 grid(static_cast<unsigned>(grid_of(args.items)));
+  if (plan.segmented) {
+    decay_chunks_kernel<T, WIDTH, kSlice, TERMS, true><<<grid, kThreads, 0, stream>>>(args);
+    const int64_t size = static_cast<int64_t>(args.pass[0].key_width) * args.pass[0].value_width;
+    const dim3 join(static_cast<unsigned>((size + kThreads - 1) / kThreads * args.heads *
+                                          args.passes * args.sequences.count));
+    decay_join_kernel<T><<<join, kThreads, 0, stream>>>(args, size);
+  } else {
+    args.segment_states = nullptr;
+  }
+  decay_chunks_kernel<T, WIDTH, kSlice, TERMS, false><<<grid, kThreads, 0, stream>>>(args);
+}
+
+template <typename T, int TERMS>
+void decay_walk_width(DecayArgs<T>& args, const DecayPlan& plan, const rosa_mixer_problem& p,
+                      hipStream_t stream) {
+  switch (padded_width(p.D > p.Dv ? p.D : p.Dv)) {
+    case 32: return decay_walk<T, 32, TERMS>(args, plan, stream);
+    case 64: return decay_walk<T, 64, TERMS>(args, plan, stream);
+    default: return decay_walk<T, 128, TERMS>(args, plan, stream);
+  }
+}
+
+template <typename T>
+DecayArgs<T> decay_args(const DecayCall& call) {
+  DecayArgs<T> args{};
+  args.heads = call.problem->H;
+  args.sequences = sequences_of(*call.problem);
+  args.log_decay = call.log_decay;
+  args.scale = call.problem->scale;
+  return args;
+}
+
+template <typename T>
+DecayPass<T> decay_forward_pass(const DecayCall& call) {
+  const rosa_mixer_problem& p = *call.problem;
+  const int share = p.H / p.Hkv;
+  return {view_of<T>(*call.query), view_of<T>(*call.key), view_of<T>(*call.value), 1, share, share,
+          p.D, p.Dv, static_cast<T*>(call.out), nullptr, false,
+          whole_pieces<T>(*call.query, p.D) && whole_pieces<T>(*call.key, p.D) &&
+              whole_pieces<T>(*call.value, p.Dv)};
+}
+
+// One term of a weighted value is enough where the state is read through the same 16 bits;
+// float16 has more of them than bfloat16 and takes two.
+template <typename T> constexpr int kTrainTerms = std::is_same_v<T, _Float16> ? 2 : 1;
+template <typename T> constexpr int kUpdateTerms = sizeof(T) == 4 ? 1 : 3;
+
+template <typename T>
+void decay_forward(const DecayCall& call) {
+  DecayArgs<T> args = decay_args<T>(call);
+  const DecayPlan plan = decay_plan(*call.problem, 1, false);
+  args.passes = 1;
+  args.pass[0] = decay_forward_pass<T>(call);
+  args.segment_states = reinterpret_cast<float*>(call.workspace);
+  decay_walk_width<T, kTrainTerms<T>>(args, plan, *call.problem, call.stream);
+}
+
+template <typename T>
+void decay_backward(const DecayCall& call) {
+  const rosa_mixer_problem& p = *call.problem;
+  const int share = p.H / p.Hkv;
+  const DecayPlan plan = decay_plan(p, 3, false);
+  DecayArgs<T> args = decay_args<T>(call);
+  args.segment_states = reinterpret_cast<float*>(call.workspace);
+  float* partial = reinterpret_cast<float*>(call.workspace + plan.state_bytes);
+  const View<const T> q = view_of<T>(*call.query), k = view_of<T>(*call.key),
+                      v = view_of<T>(*call.value), go = view_of<T>(*call.grad_output);
+  const bool whole = whole_pieces<T>(*call.query, p.D) && whole_pieces<T>(*call.key, p.D) &&
+                     whole_pieces<T>(*call.value, p.Dv) && whole_pieces<T>(*call.grad_output, p.Dv);
+  float *key_partial = nullptr, *value_partial = nullptr;
+  args.passes = 0;
+  if (call.grad_query)
+    args.pass[args.passes++] = {go, v, k, 1, share, share, p.Dv, p.D,
+                                static_cast<T*>(call.grad_query), nullptr, false, whole};
+  if (call.grad_key) {
+    if (share > 1) {
+      key_partial = partial;
+      partial += static_cast<int64_t>(p.N) * p.H * p.D;
+    }
+    args.pass[args.passes++] = {v, go, q, share, 1, 1, p.Dv, p.D,
+                                static_cast<T*>(call.grad_key), key_partial, true, whole};
+  }
+  if (call.grad_value) {
+    if (share > 1) value_partial = partial;
+    args.pass[args.passes++] = {k, q, go, share, 1, 1, p.D, p.Dv,
+                                static_cast<T*>(call.grad_value), value_partial, true, whole};
+  }
+  decay_walk_width<T, kTrainTerms<T>>(args, plan, p, call.stream);
+  const int64_t rows = static_cast<int64_t>(p.N) * p.Hkv;
+  const auto blocks = [&](int width) {
+    return dim3(static_cast<unsigned>((rows * width + kThreads - 1) / kThreads));
+  };
+  if (key_partial != nullptr)
+    sum_shared_kernel<T><<<blocks(p.D), kThreads, 0, call.stream>>>(
+        key_partial, static_cast<T*>(call.grad_key), rows, share, p.D);
+  if (value_partial != nullptr)
+    sum_shared_kernel<T><<<blocks(p.Dv), kThreads, 0, call.stream>>>(
+        value_partial, static_cast<T*>(call.grad_value), rows, share, p.Dv);
+}
+
+template <typename T>
+void decay_update(const DecayCall& call) {
+  const rosa_mixer_problem& p = *call.problem;
+  if (p.cu_seqlens == nullptr && p.T == 1) {
+    DecayTokenArgs<T> args{view_of<T>(*call.query), view_of<T>(*call.key), view_of<T>(*call.value),
+                           call.log_decay, call.state_in, call.state_out,
+                           static_cast<T*>(call.out), p.H, p.H / p.Hkv, p.D, p.Dv, 0, p.scale};
+    const bool quads = p.Dv % 4 == 0 && reinterpret_cast<uintptr_t>(call.state_in) % 16 == 0 &&
+                       reinterpret_cast<uintptr_t>(call.state_out) % 16 == 0;
+    // whole rows of a state per block, or narrower slices until there are blocks for the chip
+    args.slice = padded_width(p.Dv);
+    while (args.slice > 16 && static_cast<int64_t>(p.B) * p.H * (p.Dv / args.slice + 1) < 512)
+      args.slice /= 2;
+    const dim3 grid(static_cast<unsigned>((p.Dv + args.slice - 1) / args.slice) * p.H * p.B);
+    if (quads)
+      decay_token_kernel<T, 4><<<grid, kThreads, 0, call.stream>>>(args);
+    else
+      decay_token_kernel<T, 1><<<grid, kThreads, 0, call.stream>>>(args);
+    return;
+  }
+  DecayArgs<T> args = decay_args<T>(call);
+  const DecayPlan plan = decay_plan(p, 1, true);
+  args.passes = 1;
+  args.pass[0] = decay_forward_pass<T>(call);
+  args.segment_states = reinterpret_cast<float*>(call.workspace);
+  args.state_in = call.state_in;
+  args.state_out = call.state_out;
+  decay_walk_width<T, kUpdateTerms<T>>(args, plan, p, call.stream);
+}
+
+}  // namespace rosa_mixer

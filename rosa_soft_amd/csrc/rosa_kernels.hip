@@ -45,6 +45,18 @@ int fail_hip(hipError_t status, const char* what) {
   return 100 + static_cast<int>(status);
 }
 
+}  // namespace
+
+// the same for the library's other translation units
+__attribute__((visibility("hidden"))) int rosa_fail(int code, const char* message) {
+  return fail(code, message);
+}
+__attribute__((visibility("hidden"))) int rosa_fail_hip(hipError_t status, const char* what) {
+  return fail_hip(status, what);
+}
+
+namespace {
+
 // Optional stage timing: when enabled, every launch sequence brackets its
 // stages with HIP events recorded on the caller's stream.  Nothing is read
 // back, and the host waits for nothing, until rosa_hip_stage_times() or

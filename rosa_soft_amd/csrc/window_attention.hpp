@@ -1,0 +1,1004 @@
+// Attention with a sliding window and sinks: token t sees token s <= t of its sequence when
+// t - s < window or s < sinks.
+//
+//   p = softmax_s(scale q_t . k_s),  o_t = sum_s p_s v_s
+//   backward: P again from the saved log-sum, dS = P (dO . v - dO . o),
+//             dq = scale dS k, dk = scale dS^T q, dv = P^T dO
+//
+// Scores are formed transposed, keys down and the tokens of a wave across: the weights of a token
+// then lie in the four lanes of its column, its maximum and sum are two lane exchanges away, and
+// the weights are an operand of the product with the values as they stand.
+#pragma once
+
+#include "mixer_calls.hpp"
+#include "mixer_device.hpp"
+
+namespace rosa_mixer {
+
+constexpr int kKeys = 64;  // keys of a tile
+constexpr float kLog2e = 1.4426950408889634f;
+
+// Weights are formed as 2^kLift p and rounded so: float16 would lose bits of a weight below 2^-14,
+// which a long window's are.
+template <typename T> constexpr float kLift = kNarrow<T> ? 14.0f : 0.0f;
+template <typename T> constexpr float kUnlift = kNarrow<T> ? 1.0f / 16384.0f : 1.0f;
+
+template <typename T>
+struct WindowArgs {
+  View<const T> query, key, value, grad_output;
+  const T* output;           // [tokens][heads][value_width]
+  T* out;
+  float *log_sum, *delta;    // [heads][tokens]
+  T *grad_query, *grad_key, *grad_value;
+  float* sink_sums;          // [sink slot][kv head][sink][key_width + value_width]
+  const T *key_cache, *value_cache;
+  const int32_t* lengths;
+  int64_t capacity;
+  Sequences sequences;
+  int64_t slots, sink_slots, items;
+  int heads, kv_heads, share, key_width, value_width, window, sinks;
+  int key_block;             // keys of a block of window_grad_key_kernel
+  float scale;
+  bool whole;
+};
+
+// Positions of a slot's cache: the sinks on rows of their own, the others in a ring behind them.
+struct CacheRows {
+  int sinks, ring;
+  __device__ __forceinline__ int row(int position) const {
+    return position < sinks ? position : sinks + (position - sinks) % ring;
+  }
+};
+
+__device__ __forceinline__ bool visible(int t, int s, int window, int sinks) {
+  return s <= t && (t - s < window || s < sinks);
+}
+
+// The rows of keys and values by position: those before `past` in the cache, the others among the
+// new tokens.
+template <typename T, bool CACHED>
+struct KeyRows {
+  const T *key, *value;                 // of position 0, or of the first new token
+  int64_t key_stride, value_stride;
+  const T *key_cache, *value_cache;     // of row 0
+  int key_width, value_width, past;
+  CacheRows rows;
+  __device__ __forceinline__ const T* key_row(int s) const {
+    if (CACHED && s < past) return key_cache + static_cast<int64_t>(rows.row(s)) * key_width;
+    return key + (CACHED ? s - past : s) * key_stride;
+  }
+  __device__ __forceinline__ const T* value_row(int s) const {
+    if (CACHED && s < past) return value_cache + static_cast<int64_t>(rows.row(s)) * value_width;
+    return value + (CACHED ? s - past : s) * value_stride;
+  }
+};
+
+template <bool CACHED, typename T>
+__device__ __forceinline__ int tokens_before(const WindowArgs<T>& a, const Run& run) {
+  if constexpr (!CACHED) return 0;
+  return max(0, min(a.lengths[run.sequence], 0x7fffffff - run.length - 1024));
+}
+
+template <bool CACHED, typename T>
+__device__ __forceinline__ KeyRows<T, CACHED> key_rows(const WindowArgs<T>& a, const Run& run,
+                                                       int kv_head, int past) {
+  KeyRows<T, CACHED> rows{};
+  rows.key = a.key.row(run.batch, run.begin, kv_head);
+  rows.value = a.value.row(run.batch, run.begin, kv_head);
+  rows.key_stride = a.key.token_stride;
+  rows.value_stride = a.value.token_stride;
+  rows.past = past;
+  if constexpr (CACHED) {
+    const int64_t at = (static_cast<int64_t>(run.sequence) * a.kv_heads + kv_head) * a.capacity;
+    rows.key_cache = a.key_cache + at * a.key_width;
+    rows.value_cache = a.value_cache + at * a.value_width;
+    rows.key_width = a.key_width;
+    rows.value_width = a.value_width;
+    rows.rows = {a.sinks, static_cast<int>(a.capacity) - a.sinks};
+  }
+  return rows;
+}
+
+// The key tiles of the tokens [first, last]: the sinks in front of the window, then the window.
+struct KeyTiles {
+  int window_begin, sinks_end, at, last;
+  __device__ __forceinline__ KeyTiles(int first, int last_, int window, int sinks)
+      : window_begin(max(0, first - window + 1)), sinks_end(min(sinks, window_begin)),
+        at(sinks_end > 0 ? -1 : window_begin), last(last_) {}
+  __device__ __forceinline__ bool more() const { return at <= last; }
+  __device__ __forceinline__ int begin() const { return at < 0 ? 0 : at; }
+  __device__ __forceinline__ int end() const { return at < 0 ? sinks_end : min(at + kKeys, last + 1); }
+  __device__ __forceinline__ void next() { at = at < 0 ? window_begin : at + kKeys; }
+};
+
+template <typename T, int WIDTH, int QUERIES, bool CACHED>
+__global__ __launch_bounds__(kThreads) void window_forward_kernel(WindowArgs<T> a) {
+  constexpr int kSteps = WIDTH / 32, kRows = 64 * QUERIES, kCols = WIDTH / 16;
+  __shared__ __attribute__((aligned(16))) T keys[kKeys * kPitch<T, WIDTH>];
+  __shared__ __attribute__((aligned(16))) T values[kKeys * kPitch<T, WIDTH>];
+
+  const int64_t item = item_of_block(a.items);
+  if (item >= a.items) return;
+  const int tid = threadIdx.x, lane = tid & 63, group = lane >> 4, column = lane & 15;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  // the query heads that share keys and values are neighbours; late tiles, which see most, first
+  const int64_t slot = a.slots - 1 - item / a.share % a.slots;
+  const int kv_head = static_cast<int>(item / a.share / a.slots);
+  const int head = kv_head * a.share + static_cast<int>(item % a.share);
+  Run run;
+  const Found found = find_run(a.sequences, slot, kRows, tid, &run);
+  if (found != Found::kRun) {
+    if (found == Found::kInvalid)
+      fill_nan(a.out, slot * kRows, min((slot + 1) * kRows, static_cast<int64_t>(a.sequences.tokens)),
+               a.heads, head, a.value_width, tid);
+    return;
+  }
+  const int past = tokens_before<CACHED>(a, run);
+  const int first = past + run.tile * kRows, last = min(first + kRows, past + run.length) - 1;
+  const KeyRows<T, CACHED> rows = key_rows<CACHED>(a, run, kv_head, past);
+
+  // this wave's tokens, as the columns of operands
+  const int wave_first = first + wave * 16 * QUERIES, wave_last = wave_first + 16 * QUERIES - 1;
+  Frag<T> query[QUERIES][kSteps];
+#pragma unroll
+  for (int i = 0; i < QUERIES; ++i) {
+    const int t = wave_first + i * 16 + column;
+    const T* row = t <= last ? a.query.row(run.batch, run.begin + t - past, head) : nullptr;
+#pragma unroll
+    for (int s = 0; s < kSteps; ++s)
+      query[i][s] = memory_operand(row, s * 32 + 8 * group, a.key_width, a.whole);
+  }
+  f32x4 out[QUERIES][kCols];
+  float most[QUERIES], sum[QUERIES];
+#pragma unroll
+  for (int i = 0; i < QUERIES; ++i) {
+    most[i] = -__builtin_inff();
+    sum[i] = 0.0f;
+#pragma unroll
+    for (int d = 0; d < kCols; ++d) out[i][d] = f32x4(0.0f);
+  }
+  const float factor = a.scale * kLog2e;
+
+  TileMove<T, kKeys, WIDTH> key_move, value_move;
+  KeyTiles tiles(first, last, a.window, a.sinks);
+  const auto fetch = [&] {
+    const int begin = tiles.begin(), end = tiles.end();
+    key_move.fetch([&](int i) { return begin + i < end ? rows.key_row(begin + i) : nullptr; },
+                   a.key_width, a.whole, tid);
+    value_move.fetch([&](int i) { return begin + i < end ? rows.value_row(begin + i) : nullptr; },
+                     a.value_width, a.whole, tid);
+  };
+  fetch();
+  while (tiles.more()) {
+    const int begin = tiles.begin(), end = tiles.end();
+    tiles.next();
+    key_move.store(keys, tid);
+    value_move.store(values, tid);
+    __syncthreads();
+    if (tiles.more()) fetch();
+    // nothing of this tile is visible to the wave: behind it, or before its windows and no sink
+    const bool none = begin > min(wave_last, last) || wave_first > last ||
+                      (end - 1 <= wave_first - a.window && begin >= a.sinks);
+    if (!none) {
+      const bool all = end - begin == kKeys && end - 1 <= wave_first && wave_last - begin < a.window;
+      f32x4 score[QUERIES][4];
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+#pragma unroll
+        for (int i = 0; i < QUERIES; ++i) score[i][k] = f32x4(0.0f);
+#pragma unroll
+        for (int s = 0; s < kSteps; ++s) {
+          const Frag<T> key = row_operand<T, WIDTH>(keys, k * 16, s * 32, lane);
+#pragma unroll
+          for (int i = 0; i < QUERIES; ++i) score[i][k] = mma(key, query[i][s], score[i][k]);
+        }
+      }
+      Frag<T> weights[QUERIES][2];
+#pragma unroll
+      for (int i = 0; i < QUERIES; ++i) {
+        if (!all) {
+          const int t = wave_first + i * 16 + column;
+#pragma unroll
+          for (int k = 0; k < 4; ++k)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+              const int s = begin + k * 16 + 4 * group + r;
+              if (s >= end || !visible(t, s, a.window, a.sinks)) score[i][k][r] = -__builtin_inff();
+            }
+        }
+        float here = score[i][0][0];
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+#pragma unroll
+          for (int r = 0; r < 4; ++r) here = fmaxf(here, score[i][k][r]);
+        here = over_groups_max(here) * factor;
+        if (__any(here > most[i])) {
+          const float larger = fmaxf(here, most[i]);
+          const float shrink = larger == -__builtin_inff() ? 1.0f : exp2_of(most[i] - larger);
+          sum[i] *= shrink;
+#pragma unroll
+          for (int d = 0; d < kCols; ++d) out[i][d] *= shrink;
+          most[i] = larger;
+        }
+        const float base = (most[i] == -__builtin_inff() ? 0.0f : most[i]) - kLift<T>;
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+#pragma unroll
+          for (int r = 0; r < 4; ++r) {
+            score[i][k][r] = exp2_of(score[i][k][r] * factor - base);
+            sum[i] += score[i][k][r];
+          }
+#pragma unroll
+        for (int half = 0; half < 2; ++half)
+          weights[i][half] = operand_of<T>(score[i][2 * half], score[i][2 * half + 1]);
+      }
+#pragma unroll
+      for (int half = 0; half < 2; ++half)
+#pragma unroll
+        for (int d = 0; d < kCols; ++d) {
+          const Frag<T> value = column_operand<T, WIDTH>(values, half * 32, d * 16, lane);
+#pragma unroll
+          for (int i = 0; i < QUERIES; ++i) out[i][d] = mma(value, weights[i][half], out[i][d]);
+        }
+    }
+    __syncthreads();
+  }
+
+  const bool quads = a.value_width % 4 == 0;
+#pragma unroll
+  for (int i = 0; i < QUERIES; ++i) {
+    const int t = wave_first + i * 16 + column;
+    const float total = over_groups_sum(sum[i]);
+    if (t > last) continue;
+    const int64_t token = run.first + t - past;
+    T* to = a.out + (token * a.heads + head) * a.value_width;
+    const float by = 1.0f / total;
+#pragma unroll
+    for (int d = 0; d < kCols; ++d) store4(to, d * 16 + 4 * group, out[i][d] * by, a.value_width, quads);
+    if (a.log_sum != nullptr && group == 0)
+      a.log_sum[static_cast<int64_t>(head) * a.sequences.tokens + token] = most[i] + log2_of(total) - kLift<T>;
+  }
+}
+
+// dq, and the sums dO . o that the gradients of keys need too.  The walk of the forward pass.
+template <typename T, int WIDTH, int QUERIES>
+__global__ __launch_bounds__(kThreads) void window_grad_query_kernel(WindowArgs<T> a) {
+  constexpr int kSteps = WIDTH / 32, kRows = 64 * QUERIES, kCols = WIDTH / 16;
+  __shared__ __attribute__((aligned(16))) T keys[kKeys * kPitch<T, WIDTH>];
+  __shared__ __attribute__((aligned(16))) T values[kKeys * kPitch<T, WIDTH>];
+
+  const int64_t item = item_of_block(a.items);
+  if (item >= a.items) return;
+  const int tid = threadIdx.x, lane = tid & 63, group = lane >> 4, column = lane & 15;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int64_t slot = a.slots - 1 - item / a.share % a.slots;
+  const int kv_head = static_cast<int>(item / a.share / a.slots);
+  const int head = kv_head * a.share + static_cast<int>(item % a.share);
+  Run run;
+  const Found found = find_run(a.sequences, slot, kRows, tid, &run);
+  if (found != Found::kRun) {
+    if (found == Found::kInvalid)
+      fill_nan(a.grad_query, slot * kRows,
+               min((slot + 1) * kRows, static_cast<int64_t>(a.sequences.tokens)), a.heads, head,
+               a.key_width, tid);
+    return;
+  }
+  const int first = run.tile * kRows, last = min(first + kRows, run.length) - 1;
+  const KeyRows<T, false> rows = key_rows<false>(a, run, kv_head, 0);
+  const int wave_first = first + wave * 16 * QUERIES, wave_last = wave_first + 16 * QUERIES - 1;
+
+  Frag<T> query[QUERIES][kSteps], grad[QUERIES][kSteps];
+  float log_sum[QUERIES], delta[QUERIES], unit[QUERIES];
+#pragma unroll
+  for (int i = 0; i < QUERIES; ++i) {
+    const int t = wave_first + i * 16 + column;
+    const bool there = t <= last;
+    const T* row = there ? a.query.row(run.batch, run.begin + t, head) : nullptr;
+    const T* grad_row = there ? a.grad_output.row(run.batch, run.begin + t, head) : nullptr;
+    const T* out_row =
+        there ? a.output + ((run.first + t) * a.heads + head) * a.value_width : nullptr;
+    float dot = 0.0f;
+#pragma unroll
+    for (int s = 0; s < kSteps; ++s) {
+      query[i][s] = memory_operand(row, s * 32 + 8 * group, a.key_width, a.whole);
+      grad[i][s] = memory_operand(grad_row, s * 32 + 8 * group, a.value_width, a.whole);
+      const Frag<T> out = memory_operand(out_row, s * 32 + 8 * group, a.value_width, a.whole);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) dot += static_cast<float>(grad[i][s][e]) * static_cast<float>(out[e]);
+    }
+    delta[i] = over_groups_sum(dot);
+    const int64_t at = static_cast<int64_t>(head) * a.sequences.tokens + run.first + t;
+    log_sum[i] = there ? a.log_sum[at] : __builtin_inff();
+    if (there && group == 0) a.delta[at] = delta[i];
+    unit[i] = kNarrow<T> ? 0.0f : 1.0f;
+  }
+  if (a.grad_query == nullptr) return;
+  f32x4 out[QUERIES][kCols];
+#pragma unroll
+  for (int i = 0; i < QUERIES; ++i)
+#pragma unroll
+    for (int d = 0; d < kCols; ++d) out[i][d] = f32x4(0.0f);
+  const float factor = a.scale * kLog2e;
+
+  TileMove<T, kKeys, WIDTH> key_move, value_move;
+  KeyTiles tiles(first, last, a.window, a.sinks);
+  const auto fetch = [&] {
+    const int begin = tiles.begin(), end = tiles.end();
+    key_move.fetch([&](int i) { return begin + i < end ? rows.key_row(begin + i) : nullptr; },
+                   a.key_width, a.whole, tid);
+    value_move.fetch([&](int i) { return begin + i < end ? rows.value_row(begin + i) : nullptr; },
+                     a.value_width, a.whole, tid);
+  };
+  fetch();
+  while (tiles.more()) {
+    const int begin = tiles.begin(), end = tiles.end();
+    tiles.next();
+    key_move.store(keys, tid);
+    value_move.store(values, tid);
+    __syncthreads();
+    if (tiles.more()) fetch();
+    const bool none = begin > min(wave_last, last) || wave_first > last ||
+                      (end - 1 <= wave_first - a.window && begin >= a.sinks);
+    if (!none) {
+      const bool all = end - begin == kKeys && end - 1 <= wave_first && wave_last - begin < a.window;
+#pragma unroll
+      for (int half = 0; half < 2; ++half) {
+        f32x4 slope[QUERIES][2];
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+          f32x4 score[QUERIES];
+#pragma unroll
+          for (int i = 0; i < QUERIES; ++i) score[i] = slope[i][k] = f32x4(0.0f);
+#pragma unroll
+          for (int s = 0; s < kSteps; ++s) {
+            const Frag<T> key = row_operand<T, WIDTH>(keys, half * 32 + k * 16, s * 32, lane);
+            const Frag<T> value = row_operand<T, WIDTH>(values, half * 32 + k * 16, s * 32, lane);
+#pragma unroll
+            for (int i = 0; i < QUERIES; ++i) {
+              score[i] = mma(key, query[i][s], score[i]);
+              slope[i][k] = mma(value, grad[i][s], slope[i][k]);
+            }
+          }
+#pragma unroll
+          for (int i = 0; i < QUERIES; ++i) {
+            const int t = wave_first + i * 16 + column;
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+              const int s = begin + half * 32 + k * 16 + 4 * group + r;
+              const bool seen = all || (s < end && visible(t, s, a.window, a.sinks));
+              const float p = exp2_of(score[i][r] * factor - log_sum[i]);
+              slope[i][k][r] = seen ? p * (slope[i][k][r] - delta[i]) : 0.0f;
+            }
+          }
+        }
+        Frag<T> operand[QUERIES];
+#pragma unroll
+        for (int i = 0; i < QUERIES; ++i) {
+          if constexpr (kNarrow<T>) {
+            float most = 0.0f;
+#pragma unroll
+            for (int k = 0; k < 2; ++k)
+#pragma unroll
+              for (int r = 0; r < 4; ++r) most = fmaxf(most, fabsf(slope[i][k][r]));
+            const float by = follow_range(&unit[i], over_groups_max(most));
+            if (__any(by != 1.0f)) {
+#pragma unroll
+              for (int d = 0; d < kCols; ++d) out[i][d] *= by;
+            }
+            slope[i][0] *= unit[i];
+            slope[i][1] *= unit[i];
+          }
+          operand[i] = operand_of<T>(slope[i][0], slope[i][1]);
+        }
+#pragma unroll
+        for (int d = 0; d < kCols; ++d) {
+          const Frag<T> key = column_operand<T, WIDTH>(keys, half * 32, d * 16, lane);
+#pragma unroll
+          for (int i = 0; i < QUERIES; ++i) out[i][d] = mma(key, operand[i], out[i][d]);
+        }
+      }
+    }
+    __syncthreads();
+  }
+  const bool quads = a.key_width % 4 == 0;
+#pragma unroll
+  for (int i = 0; i < QUERIES; ++i) {
+    const int t = wave_first + i * 16 + column;
+    if (t > last) continue;
+    T* to = a.grad_query + ((run.first + t) * a.heads + head) * a.key_width;
+    const float by = unit[i] == 0.0f ? a.scale : a.scale / unit[i];
+#pragma unroll
+    for (int d = 0; d < kCols; ++d) store4(to, d * 16 + 4 * group, out[i][d] * by, a.key_width, quads);
+  }
+}
+
+// dk and dv of the keys of a block, 16 KEYS to a wave, over the tokens that see them: scores have
+// the tokens down and the wave's keys across.  The tokens beyond the window of the sinks are a
+// walk of their own (SINKS): pieces of kSinkRows tokens, each with a sum of its own in memory,
+// which the block of the sequence's first keys starts from.
+template <typename T, int WIDTH, int KEYS, bool SINKS>
+__global__ __launch_bounds__(kThreads) void window_grad_key_kernel(WindowArgs<T> a) {
+  constexpr int kSteps = WIDTH / 32, kRows = SINKS ? kSinkRows : 64 * KEYS, kCols = WIDTH / 16;
+  constexpr int kQueries = sizeof(T) == 4 && WIDTH == 128 ? 32 : 64;  // (registers)
+  __shared__ __attribute__((aligned(16))) T queries[kQueries * kPitch<T, WIDTH>];
+  __shared__ __attribute__((aligned(16))) T grads[kQueries * kPitch<T, WIDTH>];
+  __shared__ __attribute__((aligned(16))) float log_sums[kQueries], deltas[kQueries];
+
+  const int64_t item = item_of_block(a.items);
+  if (item >= a.items) return;
+  const int tid = threadIdx.x, lane = tid & 63, group = lane >> 4, column = lane & 15;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int64_t slots = SINKS ? a.sink_slots : a.slots;
+  const int64_t slot = item % slots;
+  const int kv_head = static_cast<int>(item / slots);
+  Run run;
+  const Found found = find_run(a.sequences, slot, kRows, tid, &run);
+  if (found != Found::kRun) {
+    if (!SINKS && found == Found::kInvalid) {
+      const int64_t first = slot * kRows;
+      const int64_t last = min(first + kRows, static_cast<int64_t>(a.sequences.tokens));
+      fill_nan(a.grad_key, first, last, a.kv_heads, kv_head, a.key_width, tid);
+      fill_nan(a.grad_value, first, last, a.kv_heads, kv_head, a.value_width, tid);
+    }
+    return;
+  }
+  // keys of the block; the tokens [from, to) walked for them
+  const int first = SINKS ? 0 : run.tile * kRows;
+  const int behind = SINKS ? min(a.sinks, run.length) : min(first + kRows, run.length);
+  // the tokens that see the keys of the first block in their window end here, in whole tiles
+  const auto window_end = [&](int block_first, int rows) {
+    const int64_t end = static_cast<int64_t>(block_first) + rows - 1 + a.window;
+    return static_cast<int>(min(static_cast<int64_t>(run.length), (end + kQueries - 1) / kQueries * kQueries));
+  };
+  const int sink_begin = window_end(0, a.key_block);
+  const int from = SINKS ? max(sink_begin, run.tile * kRows) : first;
+  const int to = SINKS ? min(run.length, (run.tile + 1) * kRows) : window_end(first, kRows);
+  const int sums = a.key_width + a.value_width;
+  if (SINKS && from >= to) return;  // (nor are its sums read)
+
+  const int wave_first = first + wave * 16 * KEYS;
+  Frag<T> key[KEYS][kSteps], value[KEYS][kSteps];
+  f32x4 grad_key[KEYS][kCols], grad_value[KEYS][kCols];
+#pragma unroll
+  for (int i = 0; i < KEYS; ++i) {
+    const int s = wave_first + i * 16 + column;
+    const T* row = s < behind ? a.key.row(run.batch, run.begin + s, kv_head) : nullptr;
+    const T* value_row = s < behind ? a.value.row(run.batch, run.begin + s, kv_head) : nullptr;
+#pragma unroll
+    for (int step = 0; step < kSteps; ++step) {
+      key[i][step] = memory_operand(row, step * 32 + 8 * group, a.key_width, a.whole);
+      value[i][step] = memory_operand(value_row, step * 32 + 8 * group, a.value_width, a.whole);
+    }
+#pragma unroll
+    for (int d = 0; d < kCols; ++d) grad_key[i][d] = grad_value[i][d] = f32x4(0.0f);
+  }
+  float unit[KEYS];
+#pragma unroll
+  for (int i = 0; i < KEYS; ++i) unit[i] = kNarrow<T> ? 0.0f : 1.0f;
+  if (!SINKS && run.tile == 0 && a.sink_sums != nullptr && sink_begin < run.length) {
+    const int64_t slot0 = first_slot(a.sequences, run, kSinkRows);
+    for (int piece = sink_begin / kSinkRows; piece * kSinkRows < run.length; ++piece) {
+      const float* from_piece = a.sink_sums + ((slot0 + piece) * a.kv_heads + kv_head) * a.sinks * sums;
+#pragma unroll
+      for (int i = 0; i < KEYS; ++i) {
+        const int s = wave_first + i * 16 + column;
+        if (s >= behind || s >= a.sinks) continue;
+#pragma unroll
+        for (int d = 0; d < kCols; ++d)
+#pragma unroll
+          for (int r = 0; r < 4; ++r) {
+            const int col = d * 16 + 4 * group + r;
+            if (col < a.key_width) grad_key[i][d][r] += from_piece[s * sums + col];
+            if (col < a.value_width) grad_value[i][d][r] += from_piece[s * sums + a.key_width + col];
+          }
+      }
+    }
+  }
+  const float factor = a.scale * kLog2e;
+  const bool idle = wave_first >= behind;
+
+  TileMove<T, kQueries, WIDTH> query_move, grad_move;
+  float next_log_sum = 0.0f, next_delta = 0.0f;
+  const int rows_here = to - from;
+  const int walk = (rows_here + kQueries - 1) / kQueries;
+  const auto fetch = [&](int step) {
+    const int head = kv_head * a.share + step / walk, begin = from + step % walk * kQueries;
+    query_move.fetch(
+        [&](int i) -> const T* {
+          return begin + i < to ? a.query.row(run.batch, run.begin + begin + i, head) : nullptr;
+        },
+        a.key_width, a.whole, tid);
+    grad_move.fetch(
+        [&](int i) -> const T* {
+          return begin + i < to ? a.grad_output.row(run.batch, run.begin + begin + i, head) : nullptr;
+        },
+        a.value_width, a.whole, tid);
+    if (tid < kQueries) {
+      const bool there = begin + tid < to;
+      const int64_t at = static_cast<int64_t>(head) * a.sequences.tokens + run.first + begin + tid;
+      next_log_sum = there ? a.log_sum[at] - kLift<T> : __builtin_inff();
+      next_delta = there ? a.delta[at] : 0.0f;
+    }
+  };
+  fetch(0);
+  for (int step = 0; step < walk * a.share; ++step) {
+    const int begin = from + step % walk * kQueries;
+    query_move.store(queries, tid);
+    grad_move.store(grads, tid);
+    if (tid < kQueries) {
+      log_sums[tid] = next_log_sum;
+      deltas[tid] = next_delta;
+    }
+    __syncthreads();
+    if (step + 1 < walk * a.share) fetch(step + 1);
+    const int wave_last = min(wave_first + 16 * KEYS, behind) - 1;
+    const bool none = idle || begin + kQueries - 1 < wave_first ||
+                      (!SINKS && begin - wave_last >= a.window && wave_first >= a.sinks);
+    if (!none) {
+      const bool all = wave_last - wave_first + 1 == 16 * KEYS && wave_last <= begin &&
+                       begin + kQueries <= to && begin + kQueries - 1 - wave_first < a.window;
+#pragma unroll
+      for (int half = 0; half < kQueries / 32; ++half) {
+        f32x4 weight[KEYS][2], slope[KEYS][2];
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+          const int row0 = half * 32 + k * 16;
+#pragma unroll
+          for (int i = 0; i < KEYS; ++i) weight[i][k] = slope[i][k] = f32x4(0.0f);
+#pragma unroll
+          for (int s = 0; s < kSteps; ++s) {
+            const Frag<T> query = row_operand<T, WIDTH>(queries, row0, s * 32, lane);
+            const Frag<T> grad = row_operand<T, WIDTH>(grads, row0, s * 32, lane);
+#pragma unroll
+            for (int i = 0; i < KEYS; ++i) {
+              weight[i][k] = mma(query, key[i][s], weight[i][k]);
+              slope[i][k] = mma(grad, value[i][s], slope[i][k]);
+            }
+          }
+          const f32x4 log_sum = *reinterpret_cast<const f32x4*>(log_sums + row0 + 4 * group);
+          const f32x4 delta = *reinterpret_cast<const f32x4*>(deltas + row0 + 4 * group);
+#pragma unroll
+          for (int i = 0; i < KEYS; ++i) {
+            const int s = wave_first + i * 16 + column;
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+              const int t = begin + row0 + 4 * group + r;
+              const bool seen = all || (s < behind && t < to && visible(t, s, a.window, a.sinks));
+              const float p = seen ? exp2_of(weight[i][k][r] * factor - log_sum[r]) : 0.0f;  // (lifted)
+              weight[i][k][r] = p;
+              slope[i][k][r] = seen ? p * (slope[i][k][r] - delta[r]) : 0.0f;
+            }
+          }
+        }
+        Frag<T> weights[KEYS], slopes[KEYS];
+#pragma unroll
+        for (int i = 0; i < KEYS; ++i) {
+          if constexpr (kNarrow<T>) {
+            float most = 0.0f;
+#pragma unroll
+            for (int k = 0; k < 2; ++k)
+#pragma unroll
+              for (int r = 0; r < 4; ++r) most = fmaxf(most, fabsf(slope[i][k][r]));
+            const float by = follow_range(&unit[i], over_groups_max(most));
+            if (__any(by != 1.0f)) {
+#pragma unroll
+              for (int d = 0; d < kCols; ++d) grad_key[i][d] *= by;
+            }
+            slope[i][0] *= unit[i];
+            slope[i][1] *= unit[i];
+          }
+          weights[i] = operand_of<T>(weight[i][0], weight[i][1]);
+          slopes[i] = operand_of<T>(slope[i][0], slope[i][1]);
+        }
+#pragma unroll
+        for (int d = 0; d < kCols; ++d) {
+          const Frag<T> grad = column_operand<T, WIDTH>(grads, half * 32, d * 16, lane);
+          const Frag<T> query = column_operand<T, WIDTH>(queries, half * 32, d * 16, lane);
+#pragma unroll
+          for (int i = 0; i < KEYS; ++i) {
+            grad_value[i][d] = mma(grad, weights[i], grad_value[i][d]);
+            grad_key[i][d] = mma(query, slopes[i], grad_key[i][d]);
+          }
+        }
+      }
+    }
+    __syncthreads();
+  }
+
+#pragma unroll
+  for (int i = 0; i < KEYS; ++i) {
+    const int s = wave_first + i * 16 + column;
+    if (s >= behind) continue;
+    const float back = unit[i] == 0.0f ? 1.0f : 1.0f / unit[i];
+    if constexpr (SINKS) {
+      float* piece = a.sink_sums + ((slot * a.kv_heads + kv_head) * a.sinks + s) * sums;
+#pragma unroll
+      for (int d = 0; d < kCols; ++d) {
+        store4(piece, d * 16 + 4 * group, grad_key[i][d] * back, a.key_width, false);
+        store4(piece + a.key_width, d * 16 + 4 * group, grad_value[i][d], a.value_width, false);
+      }
+    } else {
+      const int64_t row = (run.first + s) * a.kv_heads + kv_head;
+#pragma unroll
+      for (int d = 0; d < kCols; ++d) {
+        if (a.grad_key != nullptr)
+          store4(a.grad_key + row * a.key_width, d * 16 + 4 * group, grad_key[i][d] * (a.scale * back * kUnlift<T>),
+                 a.key_width, a.key_width % 4 == 0);
+        if (a.grad_value != nullptr)
+          store4(a.grad_value + row * a.value_width, d * 16 + 4 * group, grad_value[i][d] * kUnlift<T>,
+                 a.value_width, a.value_width % 4 == 0);
+      }
+    }
+  }
+}
+
+// ---------------------------------------------------------------------------
+// serving
+// ---------------------------------------------------------------------------
+
+// The new tokens that a cache keeps, each on its row: the sinks and the newest `ring` others.
+// Blocks of 64 tokens of one head of keys.
+template <typename T>
+__global__ __launch_bounds__(kThreads) void window_append_kernel(WindowArgs<T> a, T* key_cache,
+                                                                 T* value_cache) {
+  const int tid = threadIdx.x;
+  const int64_t slot = blockIdx.x / a.kv_heads;
+  const int kv_head = static_cast<int>(blockIdx.x % a.kv_heads);
+  Run run;
+  if (find_run(a.sequences, slot, 64, tid, &run) != Found::kRun) return;
+  const int past = tokens_before<true>(a, run);
+  const KeyRows<T, true> rows = key_rows<true>(a, run, kv_head, past);
+  const int begin = past + run.tile * 64, end = min(begin + 64, past + run.length);
+  const int64_t oldest = static_cast<int64_t>(past) + run.length - rows.rows.ring;
+  const int64_t at = (static_cast<int64_t>(run.sequence) * a.kv_heads + kv_head) * a.capacity;
+  const auto copy = [&](T* cache, int width, auto&& from) {
+    constexpr int kElements = 16 / static_cast<int>(sizeof(T));
+    typedef T Piece __attribute__((ext_vector_type(kElements)));
+    const int pieces = (width + kElements - 1) / kElements;
+    for (int e = tid; e < (end - begin) * pieces; e += kThreads) {
+      const int s = begin + e / pieces, col = e % pieces * kElements;
+      if (s >= a.sinks && s < oldest) continue;
+      T* to = cache + (at + rows.rows.row(s)) * width + col;
+      const T* source = from(s) + col;
+      if (a.whole)
+        *reinterpret_cast<Piece*>(to) = *reinterpret_cast<const Piece*>(source);
+      else
+        for (int i = 0; i < kElements && col + i < width; ++i) to[i] = source[i];
+    }
+  };
+  copy(key_cache, a.key_width, [&](int s) { return rows.key_row(s); });
+  copy(value_cache, a.value_width, [&](int s) { return rows.value_row(s); });
+}
+
+// One new token of every slot against its cache, which is shared out to the blocks of a head of
+// keys and, in tiles of 32 keys, to their waves: every wave has a softmax of its own over its
+// tiles, with the query heads of the group (up to 16) across; the waves are joined at the end and
+// the blocks by window_token_join_kernel.
+template <typename T>
+struct TokenArgs {
+  WindowArgs<T> window;
+  T *key_cache, *value_cache;
+  int splits, head_blocks;
+  float* partial;   // [slot][head][split][2 + value_width]: maximum, sum, outputs
+};
+
+template <typename T, int WIDTH>
+__global__ __launch_bounds__(kThreads) void window_token_kernel(TokenArgs<T> args) {
+  constexpr int kSteps = WIDTH / 32, kCols = WIDTH / 16, kTile = 32;
+  constexpr int kElements = 16 / static_cast<int>(sizeof(T)), kPerRow = WIDTH / kElements;
+  constexpr int kPieces = kTile * kPerRow / 64;
+  typedef T Piece __attribute__((ext_vector_type(kElements)));
+  const WindowArgs<T>& a = args.window;
+  constexpr size_t kTileBytes = sizeof(T) * kTile * kPitch<T, WIDTH>;
+  constexpr size_t kJoinBytes = sizeof(float) * 16 * (WIDTH + 4);
+  __shared__ __attribute__((aligned(16))) char shared[4 * (kTileBytes > kJoinBytes ? kTileBytes : kJoinBytes)];
+  __shared__ float tops[4][16], totals[4][16];
+
+  const int tid = threadIdx.x, lane = tid & 63, group = lane >> 4, column = lane & 15;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  T* values = reinterpret_cast<T*>(shared) + wave * kTile * kPitch<T, WIDTH>;
+  const int split = blockIdx.x % args.splits;
+  const int head_block = blockIdx.x / args.splits % args.head_blocks;
+  const int kv_head = blockIdx.x / args.splits / args.head_blocks % a.kv_heads;
+  const int slot = blockIdx.x / args.splits / args.head_blocks / a.kv_heads;
+  const Run run{slot, 1, 0, slot, 0, slot};
+  const int past = tokens_before<true>(a, run);
+  const KeyRows<T, true> rows = key_rows<true>(a, run, kv_head, past);
+
+  if (split == 0 && head_block == 0) {  // (the row that it takes is one that nobody sees any more)
+    const int64_t at = (static_cast<int64_t>(slot) * a.kv_heads + kv_head) * a.capacity + rows.rows.row(past);
+    for (int d = tid; d < a.key_width; d += kThreads) args.key_cache[at * a.key_width + d] = rows.key[d];
+    for (int d = tid; d < a.value_width; d += kThreads)
+      args.value_cache[at * a.value_width + d] = rows.value[d];
+  }
+  // what the token sees, in order: sinks, window, itself
+  const int window_begin = max(0, past - a.window + 1), sinks_end = min(a.sinks, window_begin);
+  const int seen = sinks_end + past - window_begin + 1;
+  const int tiles = (seen + kTile - 1) / kTile;
+  const int share = (tiles + args.splits - 1) / args.splits;
+  const int tile_end = min(tiles, (split + 1) * share);
+  const auto position = [&](int u) { return u < sinks_end ? u : window_begin + u - sinks_end; };
+
+  const int member = head_block * 16 + column;      // of the group of query heads
+  const int head = kv_head * a.share + member;
+  const T* query_row = member < a.share ? a.query.row(slot, 0, head) : nullptr;
+  Frag<T> query[kSteps];
+#pragma unroll
+  for (int s = 0; s < kSteps; ++s)
+    query[s] = memory_operand(query_row, s * 32 + 8 * group, a.key_width, a.whole);
+  f32x4 out[kCols];
+#pragma unroll
+  for (int d = 0; d < kCols; ++d) out[d] = f32x4(0.0f);
+  float most = -__builtin_inff(), sum = 0.0f;
+  const float factor = a.scale * kLog2e;
+
+  Frag<T> key[2][kSteps];
+  Piece held[kPieces];
+  const auto fetch = [&](int tile) {
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+      const int u = tile * kTile + k * 16 + column;
+      const T* row = u < seen ? rows.key_row(position(u)) : nullptr;
+#pragma unroll
+      for (int s = 0; s < kSteps; ++s)
+        key[k][s] = memory_operand(row, s * 32 + 8 * group, a.key_width, a.whole);
+    }
+#pragma unroll
+    for (int i = 0; i < kPieces; ++i) {
+      const int piece = i * 64 + lane, u = tile * kTile + piece / kPerRow, col = piece % kPerRow * kElements;
+      const T* row = u < seen ? rows.value_row(position(u)) : nullptr;
+      held[i] = Piece(static_cast<T>(0.0f));
+      if (row != nullptr) {
+        if (a.whole) {
+          if (col < a.value_width) held[i] = *reinterpret_cast<const Piece*>(row + col);
+        } else {
+#pragma unroll
+          for (int e = 0; e < kElements; ++e)
+            if (col + e < a.value_width) held[i][e] = row[col + e];
+        }
+      }
+    }
+  };
+  int tile = split * share + wave;
+  if (tile < tile_end) fetch(tile);
+  for (; tile < tile_end; tile += 4) {
+    f32x4 score[2];
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+      score[k] = f32x4(0.0f);
+#pragma unroll
+      for (int s = 0; s < kSteps; ++s) score[k] = mma(key[k][s], query[s], score[k]);
+    }
+    // (LDS accesses of one wave are carried out in order: its tile needs no barrier)
+#pragma unroll
+    for (int i = 0; i < kPieces; ++i) {
+      const int piece = i * 64 + lane;
+      *reinterpret_cast<Piece*>(values + piece / kPerRow * kPitch<T, WIDTH> +
+                                piece % kPerRow * kElements) = held[i];
+    }
+    asm volatile("" ::: "memory");
+    if (tile + 4 < tile_end) fetch(tile + 4);
+    float here = -__builtin_inff();
+#pragma unroll
+    for (int k = 0; k < 2; ++k)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        if (tile * kTile + k * 16 + 4 * group + r >= seen) score[k][r] = -__builtin_inff();
+        here = fmaxf(here, score[k][r]);
+      }
+    here = over_groups_max(here) * factor;
+    if (__any(here > most)) {
+      const float larger = fmaxf(here, most);
+      const float shrink = larger == -__builtin_inff() ? 1.0f : exp2_of(most - larger);
+      sum *= shrink;
+#pragma unroll
+      for (int d = 0; d < kCols; ++d) out[d] *= shrink;
+      most = larger;
+    }
+    const float base = (most == -__builtin_inff() ? 0.0f : most) - kLift<T>;
+#pragma unroll
+    for (int k = 0; k < 2; ++k)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        score[k][r] = exp2_of(score[k][r] * factor - base);
+        sum += score[k][r];
+      }
+    const Frag<T> weights = operand_of<T>(score[0], score[1]);
+#pragma unroll
+    for (int d = 0; d < kCols; ++d)
+      out[d] = mma(column_operand<T, WIDTH>(values, 0, d * 16, lane), weights, out[d]);
+    asm volatile("" ::: "memory");
+  }
+  sum = over_groups_sum(sum);
+
+  // the waves of the block
+  __syncthreads();
+  float* outs = reinterpret_cast<float*>(shared) + wave * 16 * (WIDTH + 4);
+#pragma unroll
+  for (int d = 0; d < kCols; ++d)
+    *reinterpret_cast<f32x4*>(outs + column * (WIDTH + 4) + d * 16 + 4 * group) = out[d];
+  if (group == 0) {
+    tops[wave][column] = most;
+    totals[wave][column] = sum;
+  }
+  __syncthreads();
+  const int members = min(16, a.share - head_block * 16);
+  for (int e = tid; e < members * a.value_width; e += kThreads) {
+    const int m = e / a.value_width, d = e % a.value_width;
+    const float top = fmaxf(fmaxf(tops[0][m], tops[1][m]), fmaxf(tops[2][m], tops[3][m]));
+    float total = 0.0f, value = 0.0f;
+#pragma unroll
+    for (int w = 0; w < 4; ++w) {
+      const float by = top == -__builtin_inff() ? 1.0f : exp2_of(tops[w][m] - top);
+      total += by * totals[w][m];
+      value += by * (reinterpret_cast<float*>(shared) + w * 16 * (WIDTH + 4))[m * (WIDTH + 4) + d];
+    }
+    const int64_t row = static_cast<int64_t>(slot) * a.heads + kv_head * a.share + head_block * 16 + m;
+    if (args.splits == 1) {
+      a.out[row * a.value_width + d] = static_cast<T>(value / total);
+    } else {
+      float* to = args.partial + (row * args.splits + split) * (2 + a.value_width);
+      if (d == 0) {
+        to[0] = top;
+        to[1] = total;
+      }
+      to[2 + d] = value;
+    }
+  }
+}
+
+// One block per slot and head: the parts of window_token_kernel, in their order.
+template <typename T>
+__global__ __launch_bounds__(kMostWidth) void window_token_join_kernel(const float* partial, T* out,
+                                                                       int splits, int width) {
+  const int64_t row = blockIdx.x;
+  const float* parts = partial + row * splits * (2 + width);
+  float top = -__builtin_inff();
+  for (int s = 0; s < splits; ++s) top = fmaxf(top, parts[s * (2 + width)]);
+  const int d = threadIdx.x;
+  if (d >= width) return;
+  float total = 0.0f, value = 0.0f;
+  for (int s = 0; s < splits; ++s) {
+    const float* part = parts + s * (2 + width);
+    const float by = top == -__builtin_inff() ? 1.0f : exp2_of(part[0] - top);
+    total += by * part[1];
+    value += by * part[2 + d];
+  }
+  out[row * width + d] = static_cast<T>(value / total);
+}
+
+// ---------------------------------------------------------------------------
+// launches
+// ---------------------------------------------------------------------------
+
+template <typename T>
+WindowArgs<T> window_args(const WindowCall& call) {
+  const rosa_mixer_problem& p = *call.problem;
+  WindowArgs<T> args{};
+  args.query = view_of<T>(*call.query);
+  args.key = view_of<T>(*call.key);
+  args.value = view_of<T>(*call.value);
+  args.whole = whole_pieces<T>(*call.query, p.D) && whole_pieces<T>(*call.key, p.D) &&
+               whole_pieces<T>(*call.value, p.Dv);
+  args.sequences = sequences_of(p);
+  args.heads = p.H;
+  args.kv_heads = p.Hkv;
+  args.share = p.H / p.Hkv;
+  args.key_width = p.D;
+  args.value_width = p.Dv;
+  args.window = call.window;
+  args.sinks = call.sinks;
+  args.scale = p.scale;
+  args.out = static_cast<T*>(call.out);
+  args.log_sum = call.log_sum;
+  return args;
+}
+
+// Tokens (in sixteens) of a wave.
+template <typename T, int WIDTH> constexpr int kForwardQueries = sizeof(T) == 4 && WIDTH == 128 ? 1 : 2;
+template <typename T, int WIDTH> constexpr int kGradQueries = sizeof(T) == 4 && WIDTH == 128 ? 1 : 2;
+template <typename T, int WIDTH> constexpr int kGradKeys = sizeof(T) == 4 && WIDTH == 128 ? 1 : 2;
+
+template <typename T, int WIDTH, bool CACHED>
+void window_forward_launch(WindowArgs<T>& args, hipStream_t stream) {
+  constexpr int kQueries = kForwardQueries<T, WIDTH>;
+  args.slots = slots_of(args.sequences, 64 * kQueries);
+  args.items = args.slots * args.heads;
+  window_forward_kernel<T, WIDTH, kQueries, CACHED>
+      <<<dim3(static_cast<unsigned>(grid_of(args.items))), kThreads, 0, stream>>>(args);
+}
+
+template <typename T>
+void window_forward(const WindowCall& call) {
+  WindowArgs<T> args = window_args<T>(call);
+  const rosa_mixer_problem& p = *call.problem;
+  switch (padded_width(p.D > p.Dv ? p.D : p.Dv)) {
+    case 32: return window_forward_launch<T, 32, false>(args, call.stream);
+    case 64: return window_forward_launch<T, 64, false>(args, call.stream);
+    default: return window_forward_launch<T, 128, false>(args, call.stream);
+  }
+}
+
+template <typename T, int WIDTH>
+void window_backward_launch(WindowArgs<T>& args, hipStream_t stream) {
+  constexpr int kQueries = kGradQueries<T, WIDTH>, kWaveKeys = kGradKeys<T, WIDTH>;
+  args.slots = slots_of(args.sequences, 64 * kQueries);
+  args.items = args.slots * args.heads;
+  window_grad_query_kernel<T, WIDTH, kQueries>
+      <<<dim3(static_cast<unsigned>(grid_of(args.items))), kThreads, 0, stream>>>(args);
+  if (args.grad_key == nullptr && args.grad_value == nullptr) return;
+  args.key_block = 64 * kWaveKeys;
+  if (args.sink_slots > 0) {
+    args.items = args.sink_slots * args.kv_heads;
+    window_grad_key_kernel<T, WIDTH, 1, true>  // (64 keys hold all sinks)
+        <<<dim3(static_cast<unsigned>(grid_of(args.items))), kThreads, 0, stream>>>(args);
+  }
+  args.slots = slots_of(args.sequences, 64 * kWaveKeys);
+  args.items = args.slots * args.kv_heads;
+  window_grad_key_kernel<T, WIDTH, kWaveKeys, false>
+      <<<dim3(static_cast<unsigned>(grid_of(args.items))), kThreads, 0, stream>>>(args);
+}
+
+template <typename T>
+void window_backward(const WindowCall& call) {
+  WindowArgs<T> args = window_args<T>(call);
+  const rosa_mixer_problem& p = *call.problem;
+  const WindowPlan plan = window_plan(p, call.window, call.sinks);
+  args.grad_output = view_of<T>(*call.grad_output);
+  args.output = static_cast<const T*>(call.output);
+  args.whole = args.whole && whole_pieces<T>(*call.grad_output, p.Dv) &&
+               reinterpret_cast<uintptr_t>(call.output) % 16 == 0;
+  args.delta = reinterpret_cast<float*>(call.workspace);
+  args.grad_query = static_cast<T*>(call.grad_query);
+  args.grad_key = static_cast<T*>(call.grad_key);
+  args.grad_value = static_cast<T*>(call.grad_value);
+  args.sink_slots = plan.sink_slots;
+  args.sink_sums =
+      plan.sink_slots > 0 ? reinterpret_cast<float*>(call.workspace + plan.delta_bytes) : nullptr;
+  switch (padded_width(p.D > p.Dv ? p.D : p.Dv)) {
+    case 32: return window_backward_launch<T, 32>(args, call.stream);
+    case 64: return window_backward_launch<T, 64>(args, call.stream);
+    default: return window_backward_launch<T, 128>(args, call.stream);
+  }
+}
+
+template <typename T, int WIDTH>
+void window_update_launch(WindowArgs<T>& args, const WindowCall& call) {
+  const rosa_mixer_problem& p = *call.problem;
+  T* key_cache = static_cast<T*>(call.key_cache);
+  T* value_cache = static_cast<T*>(call.value_cache);
+  if (p.cu_seqlens == nullptr && p.T == 1) {
+    const TokenPlan plan = token_plan(p, call.capacity);
+    TokenArgs<T> token{args, key_cache, value_cache, plan.splits, plan.head_blocks,
+                       reinterpret_cast<float*>(call.workspace)};
+    const unsigned blocks = static_cast<unsigned>(p.B) * p.Hkv * plan.head_blocks * plan.splits;
+    window_token_kernel<T, WIDTH><<<dim3(blocks), kThreads, 0, call.stream>>>(token);
+    if (plan.splits > 1)
+      window_token_join_kernel<T><<<dim3(static_cast<unsigned>(p.B) * p.H), kMostWidth, 0, call.stream>>>(
+          token.partial, args.out, plan.splits, p.Dv);
+    return;
+  }
+  window_forward_launch<T, WIDTH, true>(args, call.stream);
+  const int64_t blocks = slots_of(args.sequences, 64) * p.Hkv;
+  window_append_kernel<T>
+      <<<dim3(static_cast<unsigned>(blocks)), kThreads, 0, call.stream>>>(args, key_cache, value_cache);
+}
+
+template <typename T>
+void window_update(const WindowCall& call) {
+  WindowArgs<T> args = window_args<T>(call);
+  const rosa_mixer_problem& p = *call.problem;
+  args.key_cache = static_cast<const T*>(call.key_cache);
+  args.value_cache = static_cast<const T*>(call.value_cache);
+  args.lengths = call.lengths;
+  args.capacity = call.capacity;
+  args.whole = args.whole && reinterpret_cast<uintptr_t>(call.key_cache) % 16 == 0 &&
+               reinterpret_cast<uintptr_t>(call.value_cache) % 16 == 0;
+  switch (padded_width(p.D > p.Dv ? p.D : p.Dv)) {
+    case 32: return window_update_launch<T, 32>(args, call);
+    case 64: return window_update_launch<T, 64>(args, call);
+    default: return window_update_launch<T, 128>(args, call);
+  }
+}
+
+}  // namespace rosa_mixer

@@ -26,7 +26,7 @@ struct DecayPass {
   int key_width, value_width;
   T* out;                                    // [tokens][H][value_width]
   float* partial;                            // instead of it: before the sum over shared heads
-  bool reverse, whole;
+  bool reverse;
 };
 
 template <typename T>
@@ -48,8 +48,10 @@ struct DecayArgs {
 template <typename T>
 using StateType = std::conditional_t<sizeof(T) == 4, float, __bf16>;
 
-template <typename T, int WIDTH, int SLICE, int TERMS, bool STATE_ONLY>
-__global__ __launch_bounds__(kThreads) void decay_chunks_kernel(DecayArgs<T> a) {
+// (two waves per SIMD: with one the accumulators would be kept apart from the other registers and
+// every use of them outside a product would be a move)
+template <typename T, int WIDTH, int SLICE, int TERMS, bool STATE_ONLY, bool WHOLE>
+__global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2))) void decay_chunks_kernel(DecayArgs<T> a) {
   using ST = StateType<T>;
   constexpr int kColTiles = SLICE / 16;
   constexpr int kTiles = WIDTH / 16 * kColTiles / 4;   // state tiles of a wave
@@ -142,25 +144,19 @@ __global__ __launch_bounds__(kThreads) void decay_chunks_kernel(DecayArgs<T> a) 
       }
   }
 
-  TileMove<T, kChunk, WIDTH> key_move;
-  TileMove<T, kChunk, SLICE> value_move;
+  TileMove<T, kChunk, WIDTH, WHOLE> key_move;
+  TileMove<T, kChunk, SLICE, WHOLE> value_move;
   Frag<T> next_query[kSteps];
   const auto fetch = [&](int at) {
-    key_move.fetch(
-        [&](int i) -> const T* {
-          return at + i < stop ? p.key.row(run.batch, token(at + i), key_head) : nullptr;
-        },
-        p.key_width, p.whole, tid);
-    value_move.fetch(
-        [&](int i) -> const T* {
-          return at + i < stop ? p.value.row(run.batch, token(at + i), value_head) + col0 : nullptr;
-        },
-        p.value_width - col0, p.whole, tid);
+    const auto place = [&](int i) { return token(min(at + i, stop - 1)); };
+    key_move.fetch([&](int i) { return p.key.row(run.batch, place(i), key_head); }, p.key_width, tid);
+    value_move.fetch([&](int i) { return p.value.row(run.batch, place(i), value_head) + col0; },
+                     p.value_width - col0, tid);
     if constexpr (!STATE_ONLY) {
-      const T* row = at + own < stop ? p.query.row(run.batch, token(at + own), query_head) : nullptr;
+      const T* row = p.query.row(run.batch, place(own), query_head);
 #pragma unroll
       for (int s = 0; s < kSteps; ++s)
-        next_query[s] = memory_operand(row, s * 32 + 8 * group, p.key_width, p.whole);
+        next_query[s] = memory_operand<WHOLE>(row, s * 32 + 8 * group, p.key_width);
     }
   };
   fetch(start);
@@ -495,7 +491,7 @@ __global__ __launch_bounds__(kThreads) void decay_token_kernel(DecayTokenArgs<T>
 // launches
 // ---------------------------------------------------------------------------
 
-template <typename T, int WIDTH, int TERMS>
+template <typename T, int WIDTH, int TERMS, bool WHOLE>
 void decay_walk(DecayArgs<T>& args, const DecayPlan& plan, hipStream_t stream) {
   constexpr int kSlice = WIDTH < 64 ? WIDTH : 64;
   int widest = 0;
@@ -507,7 +503,7 @@ void decay_walk(DecayArgs<T>& args, const DecayPlan& plan, hipStream_t stream) {
   args.items = args.passes * plan.slots * args.heads * args.slices;
   const dim3 grid(static_cast<unsigned>(grid_of(args.items)));
   if (plan.segmented) {
-    decay_chunks_kernel<T, WIDTH, kSlice, TERMS, true><<<grid, kThreads, 0, stream>>>(args);
+    decay_chunks_kernel<T, WIDTH, kSlice, TERMS, true, WHOLE><<<grid, kThreads, 0, stream>>>(args);
     const int64_t size = static_cast<int64_t>(args.pass[0].key_width) * args.pass[0].value_width;
     const dim3 join(static_cast<unsigned>((size + kThreads - 1) / kThreads * args.heads *
                                           args.passes * args.sequences.count));
@@ -515,17 +511,34 @@ void decay_walk(DecayArgs<T>& args, const DecayPlan& plan, hipStream_t stream) {
   } else {
     args.segment_states = nullptr;
   }
-  decay_chunks_kernel<T, WIDTH, kSlice, TERMS, false><<<grid, kThreads, 0, stream>>>(args);
+  decay_chunks_kernel<T, WIDTH, kSlice, TERMS, false, WHOLE><<<grid, kThreads, 0, stream>>>(args);
 }
 
-template <typename T, int TERMS>
+template <typename T, int TERMS, bool WHOLE>
 void decay_walk_width(DecayArgs<T>& args, const DecayPlan& plan, const rosa_mixer_problem& p,
                       hipStream_t stream) {
   switch (padded_width(p.D > p.Dv ? p.D : p.Dv)) {
-    case 32: return decay_walk<T, 32, TERMS>(args, plan, stream);
-    case 64: return decay_walk<T, 64, TERMS>(args, plan, stream);
-    default: return decay_walk<T, 128, TERMS>(args, plan, stream);
+    case 32: return decay_walk<T, 32, TERMS, WHOLE>(args, plan, stream);
+    case 64: return decay_walk<T, 64, TERMS, WHOLE>(args, plan, stream);
+    default: return decay_walk<T, 128, TERMS, WHOLE>(args, plan, stream);
   }
+}
+
+template <typename T, int TERMS>
+void decay_walk_any(DecayArgs<T>& args, const DecayPlan& plan, const rosa_mixer_problem& p, bool whole,
+                    hipStream_t stream) {
+  if (whole)
+    decay_walk_width<T, TERMS, true>(args, plan, p, stream);
+  else
+    decay_walk_width<T, TERMS, false>(args, plan, p, stream);
+}
+
+template <typename T>
+bool whole_inputs(const DecayCall& call) {
+  const rosa_mixer_problem& p = *call.problem;
+  return whole_pieces<T>(*call.query, p.D) && whole_pieces<T>(*call.key, p.D) &&
+         whole_pieces<T>(*call.value, p.Dv) &&
+         (call.grad_output == nullptr || whole_pieces<T>(*call.grad_output, p.Dv));
 }
 
 template <typename T>
@@ -543,14 +556,11 @@ DecayPass<T> decay_forward_pass(const DecayCall& call) {
   const rosa_mixer_problem& p = *call.problem;
   const int share = p.H / p.Hkv;
   return {view_of<T>(*call.query), view_of<T>(*call.key), view_of<T>(*call.value), 1, share, share,
-          p.D, p.Dv, static_cast<T*>(call.out), nullptr, false,
-          whole_pieces<T>(*call.query, p.D) && whole_pieces<T>(*call.key, p.D) &&
-              whole_pieces<T>(*call.value, p.Dv)};
+          p.D, p.Dv, static_cast<T*>(call.out), nullptr, false};
 }
 
-// One term of a weighted value is enough where the state is read through the same 16 bits;
-// float16 has more of them than bfloat16 and takes two.
-template <typename T> constexpr int kTrainTerms = std::is_same_v<T, _Float16> ? 2 : 1;
+// Two terms of a weighted value (2^-16) are enough where the state is only read through 16 bits.
+template <typename T> constexpr int kTrainTerms = sizeof(T) == 4 ? 1 : 2;
 template <typename T> constexpr int kUpdateTerms = sizeof(T) == 4 ? 1 : 3;
 
 template <typename T>
@@ -560,7 +570,7 @@ void decay_forward(const DecayCall& call) {
   args.passes = 1;
   args.pass[0] = decay_forward_pass<T>(call);
   args.segment_states = reinterpret_cast<float*>(call.workspace);
-  decay_walk_width<T, kTrainTerms<T>>(args, plan, *call.problem, call.stream);
+  decay_walk_any<T, kTrainTerms<T>>(args, plan, *call.problem, whole_inputs<T>(call), call.stream);
 }
 
 template <typename T>
@@ -573,27 +583,25 @@ void decay_backward(const DecayCall& call) {
   float* partial = reinterpret_cast<float*>(call.workspace + plan.state_bytes);
   const View<const T> q = view_of<T>(*call.query), k = view_of<T>(*call.key),
                       v = view_of<T>(*call.value), go = view_of<T>(*call.grad_output);
-  const bool whole = whole_pieces<T>(*call.query, p.D) && whole_pieces<T>(*call.key, p.D) &&
-                     whole_pieces<T>(*call.value, p.Dv) && whole_pieces<T>(*call.grad_output, p.Dv);
   float *key_partial = nullptr, *value_partial = nullptr;
   args.passes = 0;
   if (call.grad_query)
     args.pass[args.passes++] = {go, v, k, 1, share, share, p.Dv, p.D,
-                                static_cast<T*>(call.grad_query), nullptr, false, whole};
+                                static_cast<T*>(call.grad_query), nullptr, false};
   if (call.grad_key) {
     if (share > 1) {
       key_partial = partial;
       partial += static_cast<int64_t>(p.N) * p.H * p.D;
     }
     args.pass[args.passes++] = {v, go, q, share, 1, 1, p.Dv, p.D,
-                                static_cast<T*>(call.grad_key), key_partial, true, whole};
+                                static_cast<T*>(call.grad_key), key_partial, true};
   }
   if (call.grad_value) {
     if (share > 1) value_partial = partial;
     args.pass[args.passes++] = {k, q, go, share, 1, 1, p.D, p.Dv,
-                                static_cast<T*>(call.grad_value), value_partial, true, whole};
+                                static_cast<T*>(call.grad_value), value_partial, true};
   }
-  decay_walk_width<T, kTrainTerms<T>>(args, plan, p, call.stream);
+  decay_walk_any<T, kTrainTerms<T>>(args, plan, p, whole_inputs<T>(call), call.stream);
   const int64_t rows = static_cast<int64_t>(p.N) * p.Hkv;
   const auto blocks = [&](int width) {
     return dim3(static_cast<unsigned>((rows * width + kThreads - 1) / kThreads));
@@ -633,7 +641,7 @@ void decay_update(const DecayCall& call) {
   args.segment_states = reinterpret_cast<float*>(call.workspace);
   args.state_in = call.state_in;
   args.state_out = call.state_out;
-  decay_walk_width<T, kUpdateTerms<T>>(args, plan, p, call.stream);
+  decay_walk_any<T, kUpdateTerms<T>>(args, plan, p, whole_inputs<T>(call), call.stream);
 }
 
 }  // namespace rosa_mixer

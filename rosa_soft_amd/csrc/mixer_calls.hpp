@@ -16,6 +16,7 @@ namespace rosa_mixer {
 constexpr int kWidths[] = {32, 64, 128};  // padded head widths that kernels exist for
 constexpr int kMostWidth = 128;
 constexpr int kMostSinks = 64;
+constexpr int kMostSplits = 512;
 
 constexpr int padded_width(int widest) { return widest <= 32 ? 32 : widest <= 64 ? 64 : 128; }
 

@@ -53,13 +53,21 @@ __device__ __forceinline__ float power_of(float log2_rate, int n) {
   return n == 0 ? 1.0f : exp2_of(log2_rate * static_cast<float>(n));
 }
 
+// Over the four lanes of a column.  The exchanges of gfx950 swap half of one register with the
+// other half of another: of two copies of x they leave x of this half and of the other one.
+template <typename Join>
+__device__ __forceinline__ float over_groups(float x, Join&& join) {
+  const int bits = __float_as_int(x);
+  const auto rows = __builtin_amdgcn_permlane16_swap(bits, bits, false, false);
+  const int pair = __float_as_int(join(__int_as_float(rows[0]), __int_as_float(rows[1])));
+  const auto halves = __builtin_amdgcn_permlane32_swap(pair, pair, false, false);
+  return join(__int_as_float(halves[0]), __int_as_float(halves[1]));
+}
 __device__ __forceinline__ float over_groups_max(float x) {
-  x = fmaxf(x, __shfl_xor(x, 16));
-  return fmaxf(x, __shfl_xor(x, 32));
+  return over_groups(x, [](float a, float b) { return fmaxf(a, b); });
 }
 __device__ __forceinline__ float over_groups_sum(float x) {
-  x += __shfl_xor(x, 16);
-  return x + __shfl_xor(x, 32);
+  return over_groups(x, [](float a, float b) { return a + b; });
 }
 
 // ---------------------------------------------------------------------------
@@ -117,10 +125,11 @@ __device__ __forceinline__ Frag<T> operand_of(f32x4 low, f32x4 high) {
   return out;
 }
 
-// A tile of ROWS x WIDTH on its way from memory to LDS through the registers of the block.  Rows
-// that do not exist (a null row pointer) and columns from `width` on are zeros.  `whole`: rows
-// are whole 16-byte pieces at 16-byte addresses.
-template <typename T, int ROWS, int WIDTH>
+// A tile of ROWS x WIDTH on its way from memory to LDS through the registers of the block.
+// `row_pointer` gives an existing row for every row of the tile (a caller repeats its last one and
+// masks what comes of it), so that loads are never predicated; columns from `width` on are zeros.
+// WHOLE: rows are whole 16-byte pieces at 16-byte addresses.
+template <typename T, int ROWS, int WIDTH, bool WHOLE>
 struct TileMove {
   static constexpr int kElements = 16 / static_cast<int>(sizeof(T));
   static constexpr int kPerRow = WIDTH / kElements;
@@ -131,24 +140,25 @@ struct TileMove {
   Piece held[kPieces];
 
   template <typename RowPointer>
-  __device__ __forceinline__ void fetch(RowPointer&& row_pointer, int width, bool whole, int tid) {
-    if (whole) {
+  __device__ __forceinline__ void fetch(RowPointer&& row_pointer, int width, int tid) {
 #pragma unroll
-      for (int i = 0; i < kPieces; ++i) {
-        const int piece = i * kThreads + tid, col = piece % kPerRow * kElements;
-        const T* row = row_pointer(piece / kPerRow);
-        held[i] = Piece(static_cast<T>(0.0f));
-        if (row != nullptr && col < width) held[i] = *reinterpret_cast<const Piece*>(row + col);
+    for (int i = 0; i < kPieces; ++i) {
+      const int piece = i * kThreads + tid, col = piece % kPerRow * kElements;
+      const T* row = row_pointer(piece / kPerRow);
+      if constexpr (WHOLE) {
+        held[i] = *reinterpret_cast<const Piece*>(row + min(col, width - kElements));
+      } else {
+#pragma unroll
+        for (int e = 0; e < kElements; ++e) held[i][e] = row[min(col + e, width - 1)];
       }
-    } else {
+    }
+    if (width < WIDTH) {
 #pragma unroll
       for (int i = 0; i < kPieces; ++i) {
-        const int piece = i * kThreads + tid, col = piece % kPerRow * kElements;
-        const T* row = row_pointer(piece / kPerRow);
-        held[i] = Piece(static_cast<T>(0.0f));
+        const int col = (i * kThreads + tid) % kPerRow * kElements;
 #pragma unroll
         for (int e = 0; e < kElements; ++e)
-          if (row != nullptr && col + e < width) held[i][e] = row[col + e];
+          held[i][e] = col + e < width ? held[i][e] : static_cast<T>(0.0f);
       }
     }
   }
@@ -161,46 +171,29 @@ struct TileMove {
                                 piece % kPerRow * kElements) = held[i];
     }
   }
-
-  // the same rows times a factor of each row
-  template <typename Factor>
-  __device__ __forceinline__ void store_scaled(T* tile, Factor&& factor, int tid) const {
-#pragma unroll
-    for (int i = 0; i < kPieces; ++i) {
-      const int piece = i * kThreads + tid;
-      const float by = factor(piece / kPerRow);
-      Piece scaled;
-#pragma unroll
-      for (int e = 0; e < kElements; ++e)
-        scaled[e] = static_cast<T>(static_cast<float>(held[i][e]) * by);
-      *reinterpret_cast<Piece*>(tile + piece / kPerRow * kPitch<T, WIDTH> +
-                                piece % kPerRow * kElements) = scaled;
-    }
-  }
 };
 
-// row-wise operand straight from memory: `row` is the lane's own row or null
-template <typename T>
-__device__ __forceinline__ Frag<T> memory_operand(const T* row, int col, int width, bool whole) {
-  Frag<T> out = Frag<T>(static_cast<T>(0.0f));
-  if (row == nullptr) return out;
-  if (whole) {
-    if constexpr (sizeof(T) == 2) {
-      if (col < width) out = load8(row + col);
-    } else {  // pieces of four
+// row-wise operand straight from memory: `row` is the lane's own row
+template <bool WHOLE, typename T>
+__device__ __forceinline__ Frag<T> memory_operand(const T* row, int col, int width) {
+  Frag<T> out;
+  if constexpr (WHOLE && sizeof(T) == 2) {
+    out = load8(row + min(col, width - 8));
+    if (col >= width) out = Frag<T>(static_cast<T>(0.0f));
+  } else if constexpr (WHOLE) {
 #pragma unroll
-      for (int half = 0; half < 2; ++half) {
-        if (col + 4 * half < width) {
-          const f32x4 part = *reinterpret_cast<const f32x4*>(row + col + 4 * half);
+    for (int half = 0; half < 2; ++half) {
+      f32x4 part = *reinterpret_cast<const f32x4*>(row + min(col + 4 * half, width - 4));
+      if (col + 4 * half >= width) part = f32x4(0.0f);
 #pragma unroll
-          for (int e = 0; e < 4; ++e) out[4 * half + e] = part[e];
-        }
-      }
+      for (int e = 0; e < 4; ++e) out[4 * half + e] = part[e];
     }
   } else {
 #pragma unroll
-    for (int e = 0; e < 8; ++e)
-      if (col + e < width) out[e] = row[col + e];
+    for (int e = 0; e < 8; ++e) {
+      const T element = row[min(col + e, width - 1)];
+      out[e] = col + e < width ? element : static_cast<T>(0.0f);
+    }
   }
   return out;
 }

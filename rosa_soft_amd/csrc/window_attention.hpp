@@ -16,6 +16,13 @@
 namespace rosa_mixer {
 
 constexpr int kKeys = 64;  // keys of a tile
+
+// Waves per SIMD that a kernel is compiled for: two, so that products of one overlap the softmax
+// of the other and accumulators share the registers that the rest can use directly; float32 tiles
+// of 128 columns leave room in LDS for one block, and moving 128 columns element by element takes
+// more registers.
+template <typename T, int WIDTH, bool WHOLE>
+constexpr int kWaves = WIDTH == 128 && (sizeof(T) == 4 || !WHOLE) ? 1 : 2;
 constexpr float kLog2e = 1.4426950408889634f;
 
 // Weights are formed as 2^kLift p and rounded so: float16 would lose bits of a weight below 2^-14,
@@ -39,7 +46,6 @@ struct WindowArgs {
   int heads, kv_heads, share, key_width, value_width, window, sinks;
   int key_block;             // keys of a block of window_grad_key_kernel
   float scale;
-  bool whole;
 };
 
 // Positions of a slot's cache: the sinks on rows of their own, the others in a ring behind them.
@@ -50,8 +56,18 @@ struct CacheRows {
   }
 };
 
-__device__ __forceinline__ bool visible(int t, int s, int window, int sinks) {
-  return s <= t && (t - s < window || s < sinks);
+// Which elements of a column of scores are seen: e up to `last`, and from `first` on or below
+// `sinks`; e counts from the lane's first row.  (Bitwise: no branch per element.)
+struct Seen {
+  int first, last, sinks;
+  __device__ __forceinline__ bool operator()(int e) const {
+    return (e <= last) & ((e >= first) | (e < sinks));
+  }
+};
+
+// of token t, keys from `row` on (the lane's first of a tile) that end before `end`
+__device__ __forceinline__ Seen seen_keys(int t, int row, int end, int window, int sinks) {
+  return {t - window + 1 - row, min(t, end - 1) - row, sinks - row};
 }
 
 // The rows of keys and values by position: those before `past` in the cache, the others among the
@@ -111,8 +127,9 @@ struct KeyTiles {
   __device__ __forceinline__ void next() { at = at < 0 ? window_begin : at + kKeys; }
 };
 
-template <typename T, int WIDTH, int QUERIES, bool CACHED>
-__global__ __launch_bounds__(kThreads) void window_forward_kernel(WindowArgs<T> a) {
+template <typename T, int WIDTH, int QUERIES, bool CACHED, bool WHOLE>
+__global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(kWaves<T, WIDTH, WHOLE>))) void
+window_forward_kernel(WindowArgs<T> a) {
   constexpr int kSteps = WIDTH / 32, kRows = 64 * QUERIES, kCols = WIDTH / 16;
   __shared__ __attribute__((aligned(16))) T keys[kKeys * kPitch<T, WIDTH>];
   __shared__ __attribute__((aligned(16))) T values[kKeys * kPitch<T, WIDTH>];
@@ -143,10 +160,10 @@ __global__ __launch_bounds__(kThreads) void window_forward_kernel(WindowArgs<T> 
 #pragma unroll
   for (int i = 0; i < QUERIES; ++i) {
     const int t = wave_first + i * 16 + column;
-    const T* row = t <= last ? a.query.row(run.batch, run.begin + t - past, head) : nullptr;
+    const T* row = a.query.row(run.batch, run.begin + min(t, last) - past, head);
 #pragma unroll
     for (int s = 0; s < kSteps; ++s)
-      query[i][s] = memory_operand(row, s * 32 + 8 * group, a.key_width, a.whole);
+      query[i][s] = memory_operand<WHOLE>(row, s * 32 + 8 * group, a.key_width);
   }
   f32x4 out[QUERIES][kCols];
   float most[QUERIES], sum[QUERIES];
@@ -159,14 +176,12 @@ __global__ __launch_bounds__(kThreads) void window_forward_kernel(WindowArgs<T> 
   }
   const float factor = a.scale * kLog2e;
 
-  TileMove<T, kKeys, WIDTH> key_move, value_move;
+  TileMove<T, kKeys, WIDTH, WHOLE> key_move, value_move;
   KeyTiles tiles(first, last, a.window, a.sinks);
   const auto fetch = [&] {
     const int begin = tiles.begin(), end = tiles.end();
-    key_move.fetch([&](int i) { return begin + i < end ? rows.key_row(begin + i) : nullptr; },
-                   a.key_width, a.whole, tid);
-    value_move.fetch([&](int i) { return begin + i < end ? rows.value_row(begin + i) : nullptr; },
-                     a.value_width, a.whole, tid);
+    key_move.fetch([&](int i) { return rows.key_row(min(begin + i, end - 1)); }, a.key_width, tid);
+    value_move.fetch([&](int i) { return rows.value_row(min(begin + i, end - 1)); }, a.value_width, tid);
   };
   fetch();
   while (tiles.more()) {
@@ -197,14 +212,13 @@ __global__ __launch_bounds__(kThreads) void window_forward_kernel(WindowArgs<T> 
 #pragma unroll
       for (int i = 0; i < QUERIES; ++i) {
         if (!all) {
-          const int t = wave_first + i * 16 + column;
+          const Seen seen = seen_keys(wave_first + i * 16 + column, begin + 4 * group, end, a.window,
+                                      a.sinks);
 #pragma unroll
           for (int k = 0; k < 4; ++k)
 #pragma unroll
-            for (int r = 0; r < 4; ++r) {
-              const int s = begin + k * 16 + 4 * group + r;
-              if (s >= end || !visible(t, s, a.window, a.sinks)) score[i][k][r] = -__builtin_inff();
-            }
+            for (int r = 0; r < 4; ++r)
+              score[i][k][r] = seen(k * 16 + r) ? score[i][k][r] : -__builtin_inff();
         }
         float here = score[i][0][0];
 #pragma unroll
@@ -261,8 +275,9 @@ __global__ __launch_bounds__(kThreads) void window_forward_kernel(WindowArgs<T> 
 }
 
 // dq, and the sums dO . o that the gradients of keys need too.  The walk of the forward pass.
-template <typename T, int WIDTH, int QUERIES>
-__global__ __launch_bounds__(kThreads) void window_grad_query_kernel(WindowArgs<T> a) {
+template <typename T, int WIDTH, int QUERIES, bool WHOLE>
+__global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(kWaves<T, WIDTH, WHOLE>))) void
+window_grad_query_kernel(WindowArgs<T> a) {
   constexpr int kSteps = WIDTH / 32, kRows = 64 * QUERIES, kCols = WIDTH / 16;
   __shared__ __attribute__((aligned(16))) T keys[kKeys * kPitch<T, WIDTH>];
   __shared__ __attribute__((aligned(16))) T values[kKeys * kPitch<T, WIDTH>];
@@ -293,22 +308,22 @@ __global__ __launch_bounds__(kThreads) void window_grad_query_kernel(WindowArgs<
   for (int i = 0; i < QUERIES; ++i) {
     const int t = wave_first + i * 16 + column;
     const bool there = t <= last;
-    const T* row = there ? a.query.row(run.batch, run.begin + t, head) : nullptr;
-    const T* grad_row = there ? a.grad_output.row(run.batch, run.begin + t, head) : nullptr;
-    const T* out_row =
-        there ? a.output + ((run.first + t) * a.heads + head) * a.value_width : nullptr;
+    const int row_t = min(t, last);
+    const T* row = a.query.row(run.batch, run.begin + row_t, head);
+    const T* grad_row = a.grad_output.row(run.batch, run.begin + row_t, head);
+    const T* out_row = a.output + ((run.first + row_t) * a.heads + head) * a.value_width;
     float dot = 0.0f;
 #pragma unroll
     for (int s = 0; s < kSteps; ++s) {
-      query[i][s] = memory_operand(row, s * 32 + 8 * group, a.key_width, a.whole);
-      grad[i][s] = memory_operand(grad_row, s * 32 + 8 * group, a.value_width, a.whole);
-      const Frag<T> out = memory_operand(out_row, s * 32 + 8 * group, a.value_width, a.whole);
+      query[i][s] = memory_operand<WHOLE>(row, s * 32 + 8 * group, a.key_width);
+      grad[i][s] = memory_operand<WHOLE>(grad_row, s * 32 + 8 * group, a.value_width);
+      const Frag<T> out = memory_operand<WHOLE>(out_row, s * 32 + 8 * group, a.value_width);
 #pragma unroll
       for (int e = 0; e < 8; ++e) dot += static_cast<float>(grad[i][s][e]) * static_cast<float>(out[e]);
     }
     delta[i] = over_groups_sum(dot);
-    const int64_t at = static_cast<int64_t>(head) * a.sequences.tokens + run.first + t;
-    log_sum[i] = there ? a.log_sum[at] : __builtin_inff();
+    const int64_t at = static_cast<int64_t>(head) * a.sequences.tokens + run.first + row_t;
+    log_sum[i] = a.log_sum[at];
     if (there && group == 0) a.delta[at] = delta[i];
     unit[i] = kNarrow<T> ? 0.0f : 1.0f;
   }
@@ -320,14 +335,12 @@ __global__ __launch_bounds__(kThreads) void window_grad_query_kernel(WindowArgs<
     for (int d = 0; d < kCols; ++d) out[i][d] = f32x4(0.0f);
   const float factor = a.scale * kLog2e;
 
-  TileMove<T, kKeys, WIDTH> key_move, value_move;
+  TileMove<T, kKeys, WIDTH, WHOLE> key_move, value_move;
   KeyTiles tiles(first, last, a.window, a.sinks);
   const auto fetch = [&] {
     const int begin = tiles.begin(), end = tiles.end();
-    key_move.fetch([&](int i) { return begin + i < end ? rows.key_row(begin + i) : nullptr; },
-                   a.key_width, a.whole, tid);
-    value_move.fetch([&](int i) { return begin + i < end ? rows.value_row(begin + i) : nullptr; },
-                     a.value_width, a.whole, tid);
+    key_move.fetch([&](int i) { return rows.key_row(min(begin + i, end - 1)); }, a.key_width, tid);
+    value_move.fetch([&](int i) { return rows.value_row(min(begin + i, end - 1)); }, a.value_width, tid);
   };
   fetch();
   while (tiles.more()) {
@@ -361,13 +374,16 @@ __global__ __launch_bounds__(kThreads) void window_grad_query_kernel(WindowArgs<
           }
 #pragma unroll
           for (int i = 0; i < QUERIES; ++i) {
-            const int t = wave_first + i * 16 + column;
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
-              const int s = begin + half * 32 + k * 16 + 4 * group + r;
-              const bool seen = all || (s < end && visible(t, s, a.window, a.sinks));
               const float p = exp2_of(score[i][r] * factor - log_sum[i]);
-              slope[i][k][r] = seen ? p * (slope[i][k][r] - delta[i]) : 0.0f;
+              slope[i][k][r] = p * (slope[i][k][r] - delta[i]);
+            }
+            if (!all) {
+              const Seen seen = seen_keys(wave_first + i * 16 + column,
+                                          begin + half * 32 + k * 16 + 4 * group, end, a.window, a.sinks);
+#pragma unroll
+              for (int r = 0; r < 4; ++r) slope[i][k][r] = seen(r) ? slope[i][k][r] : 0.0f;
             }
           }
         }
@@ -416,8 +432,9 @@ __global__ __launch_bounds__(kThreads) void window_grad_query_kernel(WindowArgs<
 // the tokens down and the wave's keys across.  The tokens beyond the window of the sinks are a
 // walk of their own (SINKS): pieces of kSinkRows tokens, each with a sum of its own in memory,
 // which the block of the sequence's first keys starts from.
-template <typename T, int WIDTH, int KEYS, bool SINKS>
-__global__ __launch_bounds__(kThreads) void window_grad_key_kernel(WindowArgs<T> a) {
+template <typename T, int WIDTH, int KEYS, bool SINKS, bool WHOLE>
+__global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(WIDTH * sizeof(T) > 128 ? 1 : 2))) void
+window_grad_key_kernel(WindowArgs<T> a) {
   constexpr int kSteps = WIDTH / 32, kRows = SINKS ? kSinkRows : 64 * KEYS, kCols = WIDTH / 16;
   constexpr int kQueries = sizeof(T) == 4 && WIDTH == 128 ? 32 : 64;  // (registers)
   __shared__ __attribute__((aligned(16))) T queries[kQueries * kPitch<T, WIDTH>];
@@ -462,12 +479,12 @@ __global__ __launch_bounds__(kThreads) void window_grad_key_kernel(WindowArgs<T>
 #pragma unroll
   for (int i = 0; i < KEYS; ++i) {
     const int s = wave_first + i * 16 + column;
-    const T* row = s < behind ? a.key.row(run.batch, run.begin + s, kv_head) : nullptr;
-    const T* value_row = s < behind ? a.value.row(run.batch, run.begin + s, kv_head) : nullptr;
+    const T* row = a.key.row(run.batch, run.begin + min(s, behind - 1), kv_head);
+    const T* value_row = a.value.row(run.batch, run.begin + min(s, behind - 1), kv_head);
 #pragma unroll
     for (int step = 0; step < kSteps; ++step) {
-      key[i][step] = memory_operand(row, step * 32 + 8 * group, a.key_width, a.whole);
-      value[i][step] = memory_operand(value_row, step * 32 + 8 * group, a.value_width, a.whole);
+      key[i][step] = memory_operand<WHOLE>(row, step * 32 + 8 * group, a.key_width);
+      value[i][step] = memory_operand<WHOLE>(value_row, step * 32 + 8 * group, a.value_width);
     }
 #pragma unroll
     for (int d = 0; d < kCols; ++d) grad_key[i][d] = grad_value[i][d] = f32x4(0.0f);
@@ -497,27 +514,20 @@ __global__ __launch_bounds__(kThreads) void window_grad_key_kernel(WindowArgs<T>
   const float factor = a.scale * kLog2e;
   const bool idle = wave_first >= behind;
 
-  TileMove<T, kQueries, WIDTH> query_move, grad_move;
+  TileMove<T, kQueries, WIDTH, WHOLE> query_move, grad_move;
   float next_log_sum = 0.0f, next_delta = 0.0f;
   const int rows_here = to - from;
   const int walk = (rows_here + kQueries - 1) / kQueries;
   const auto fetch = [&](int step) {
     const int head = kv_head * a.share + step / walk, begin = from + step % walk * kQueries;
-    query_move.fetch(
-        [&](int i) -> const T* {
-          return begin + i < to ? a.query.row(run.batch, run.begin + begin + i, head) : nullptr;
-        },
-        a.key_width, a.whole, tid);
-    grad_move.fetch(
-        [&](int i) -> const T* {
-          return begin + i < to ? a.grad_output.row(run.batch, run.begin + begin + i, head) : nullptr;
-        },
-        a.value_width, a.whole, tid);
+    const auto token = [&](int i) { return run.begin + min(begin + i, to - 1); };
+    query_move.fetch([&](int i) { return a.query.row(run.batch, token(i), head); }, a.key_width, tid);
+    grad_move.fetch([&](int i) { return a.grad_output.row(run.batch, token(i), head); }, a.value_width,
+                    tid);
     if (tid < kQueries) {
-      const bool there = begin + tid < to;
-      const int64_t at = static_cast<int64_t>(head) * a.sequences.tokens + run.first + begin + tid;
-      next_log_sum = there ? a.log_sum[at] - kLift<T> : __builtin_inff();
-      next_delta = there ? a.delta[at] : 0.0f;
+      const int64_t at = static_cast<int64_t>(head) * a.sequences.tokens + run.first - run.begin + token(tid);
+      next_log_sum = a.log_sum[at] - kLift<T>;
+      next_delta = a.delta[at];
     }
   };
   fetch(0);
@@ -559,14 +569,21 @@ __global__ __launch_bounds__(kThreads) void window_grad_key_kernel(WindowArgs<T>
           const f32x4 delta = *reinterpret_cast<const f32x4*>(deltas + row0 + 4 * group);
 #pragma unroll
           for (int i = 0; i < KEYS; ++i) {
-            const int s = wave_first + i * 16 + column;
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
-              const int t = begin + row0 + 4 * group + r;
-              const bool seen = all || (s < behind && t < to && visible(t, s, a.window, a.sinks));
-              const float p = seen ? exp2_of(weight[i][k][r] * factor - log_sum[r]) : 0.0f;  // (lifted)
-              weight[i][k][r] = p;
-              slope[i][k][r] = seen ? p * (slope[i][k][r] - delta[r]) : 0.0f;
+              weight[i][k][r] = exp2_of(weight[i][k][r] * factor - log_sum[r]);  // (lifted)
+              slope[i][k][r] = weight[i][k][r] * (slope[i][k][r] - delta[r]);
+            }
+            if (!all) {  // tokens t from this row on that see key s: s <= t < to, t - s < window
+              const int s = wave_first + i * 16 + column, row = begin + row0 + 4 * group;
+              const int64_t end = s >= behind ? 0 : s < a.sinks ? to : min<int64_t>(to, int64_t{s} + a.window);
+              const int first_seen = s - row, last_seen = static_cast<int>(end) - 1 - row;
+#pragma unroll
+              for (int r = 0; r < 4; ++r) {
+                const bool seen = (r >= first_seen) & (r <= last_seen);
+                weight[i][k][r] = seen ? weight[i][k][r] : 0.0f;
+                slope[i][k][r] = seen ? slope[i][k][r] : 0.0f;
+              }
             }
           }
         }
@@ -638,7 +655,7 @@ __global__ __launch_bounds__(kThreads) void window_grad_key_kernel(WindowArgs<T>
 
 // The new tokens that a cache keeps, each on its row: the sinks and the newest `ring` others.
 // Blocks of 64 tokens of one head of keys.
-template <typename T>
+template <typename T, bool WHOLE>
 __global__ __launch_bounds__(kThreads) void window_append_kernel(WindowArgs<T> a, T* key_cache,
                                                                  T* value_cache) {
   const int tid = threadIdx.x;
@@ -660,7 +677,7 @@ __global__ __launch_bounds__(kThreads) void window_append_kernel(WindowArgs<T> a
       if (s >= a.sinks && s < oldest) continue;
       T* to = cache + (at + rows.rows.row(s)) * width + col;
       const T* source = from(s) + col;
-      if (a.whole)
+      if constexpr (WHOLE)
         *reinterpret_cast<Piece*>(to) = *reinterpret_cast<const Piece*>(source);
       else
         for (int i = 0; i < kElements && col + i < width; ++i) to[i] = source[i];
@@ -682,8 +699,9 @@ struct TokenArgs {
   float* partial;   // [slot][head][split][2 + value_width]: maximum, sum, outputs
 };
 
-template <typename T, int WIDTH>
-__global__ __launch_bounds__(kThreads) void window_token_kernel(TokenArgs<T> args) {
+template <typename T, int WIDTH, bool WHOLE>
+__global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(kWaves<T, WIDTH, WHOLE>))) void
+window_token_kernel(TokenArgs<T> args) {
   constexpr int kSteps = WIDTH / 32, kCols = WIDTH / 16, kTile = 32;
   constexpr int kElements = 16 / static_cast<int>(sizeof(T)), kPerRow = WIDTH / kElements;
   constexpr int kPieces = kTile * kPerRow / 64;
@@ -719,13 +737,13 @@ __global__ __launch_bounds__(kThreads) void window_token_kernel(TokenArgs<T> arg
   const int tile_end = min(tiles, (split + 1) * share);
   const auto position = [&](int u) { return u < sinks_end ? u : window_begin + u - sinks_end; };
 
-  const int member = head_block * 16 + column;      // of the group of query heads
-  const int head = kv_head * a.share + member;
-  const T* query_row = member < a.share ? a.query.row(slot, 0, head) : nullptr;
+  // this column's member of the group of query heads (the last one again beyond it)
+  const int head = kv_head * a.share + min(head_block * 16 + column, a.share - 1);
+  const T* query_row = a.query.row(slot, 0, head);
   Frag<T> query[kSteps];
 #pragma unroll
   for (int s = 0; s < kSteps; ++s)
-    query[s] = memory_operand(query_row, s * 32 + 8 * group, a.key_width, a.whole);
+    query[s] = memory_operand<WHOLE>(query_row, s * 32 + 8 * group, a.key_width);
   f32x4 out[kCols];
 #pragma unroll
   for (int d = 0; d < kCols; ++d) out[d] = f32x4(0.0f);
@@ -737,25 +755,20 @@ __global__ __launch_bounds__(kThreads) void window_token_kernel(TokenArgs<T> arg
   const auto fetch = [&](int tile) {
 #pragma unroll
     for (int k = 0; k < 2; ++k) {
-      const int u = tile * kTile + k * 16 + column;
-      const T* row = u < seen ? rows.key_row(position(u)) : nullptr;
+      const T* row = rows.key_row(position(min(tile * kTile + k * 16 + column, seen - 1)));
 #pragma unroll
       for (int s = 0; s < kSteps; ++s)
-        key[k][s] = memory_operand(row, s * 32 + 8 * group, a.key_width, a.whole);
+        key[k][s] = memory_operand<WHOLE>(row, s * 32 + 8 * group, a.key_width);
     }
 #pragma unroll
     for (int i = 0; i < kPieces; ++i) {
-      const int piece = i * 64 + lane, u = tile * kTile + piece / kPerRow, col = piece % kPerRow * kElements;
-      const T* row = u < seen ? rows.value_row(position(u)) : nullptr;
-      held[i] = Piece(static_cast<T>(0.0f));
-      if (row != nullptr) {
-        if (a.whole) {
-          if (col < a.value_width) held[i] = *reinterpret_cast<const Piece*>(row + col);
-        } else {
+      const int piece = i * 64 + lane, col = piece % kPerRow * kElements;
+      const T* row = rows.value_row(position(min(tile * kTile + piece / kPerRow, seen - 1)));
+      if constexpr (WHOLE) {
+        held[i] = *reinterpret_cast<const Piece*>(row + min(col, a.value_width - kElements));
+      } else {
 #pragma unroll
-          for (int e = 0; e < kElements; ++e)
-            if (col + e < a.value_width) held[i][e] = row[col + e];
-        }
+        for (int e = 0; e < kElements; ++e) held[i][e] = row[min(col + e, a.value_width - 1)];
       }
     }
   };
@@ -847,24 +860,49 @@ __global__ __launch_bounds__(kThreads) void window_token_kernel(TokenArgs<T> arg
   }
 }
 
-// One block per slot and head: the parts of window_token_kernel, in their order.
+// One block per slot and head: the parts of window_token_kernel, whose weights a thread each forms
+// and whose outputs the waves add up in turn.
 template <typename T>
-__global__ __launch_bounds__(kMostWidth) void window_token_join_kernel(const float* partial, T* out,
-                                                                       int splits, int width) {
+__global__ __launch_bounds__(kThreads) void window_token_join_kernel(const float* partial, T* out,
+                                                                     int splits, int width) {
+  __shared__ float weights[kMostSplits], sums[kThreads], tops[4], totals[4];
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const int64_t row = blockIdx.x;
   const float* parts = partial + row * splits * (2 + width);
   float top = -__builtin_inff();
-  for (int s = 0; s < splits; ++s) top = fmaxf(top, parts[s * (2 + width)]);
-  const int d = threadIdx.x;
-  if (d >= width) return;
-  float total = 0.0f, value = 0.0f;
-  for (int s = 0; s < splits; ++s) {
-    const float* part = parts + s * (2 + width);
-    const float by = top == -__builtin_inff() ? 1.0f : exp2_of(part[0] - top);
-    total += by * part[1];
-    value += by * part[2 + d];
+  for (int s = tid; s < splits; s += kThreads) {
+    weights[s] = parts[static_cast<int64_t>(s) * (2 + width)];
+    top = fmaxf(top, weights[s]);
   }
-  out[row * width + d] = static_cast<T>(value / total);
+  for (int apart = 1; apart < 64; apart *= 2) top = fmaxf(top, __shfl_xor(top, apart));
+  if (lane == 0) tops[wave] = top;
+  __syncthreads();
+  top = fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3]));
+  float total = 0.0f;
+  for (int s = tid; s < splits; s += kThreads) {
+    const float by = top == -__builtin_inff() ? 1.0f : exp2_of(weights[s] - top);
+    weights[s] = by;
+    total += by * parts[static_cast<int64_t>(s) * (2 + width) + 1];
+  }
+  for (int apart = 1; apart < 64; apart *= 2) total += __shfl_xor(total, apart);
+  if (lane == 0) totals[wave] = total;
+  __syncthreads();
+  total = totals[0] + totals[1] + totals[2] + totals[3];
+  for (int col0 = 0; col0 < width; col0 += 64) {
+    const int col = col0 + lane;
+    float value = 0.0f;
+    if (col < width) {
+#pragma unroll 8
+      for (int s = wave; s < splits; s += 4)
+        value += weights[s] * parts[static_cast<int64_t>(s) * (2 + width) + 2 + col];
+    }
+    sums[tid] = value;
+    __syncthreads();
+    if (wave == 0 && col < width)
+      out[row * width + col] = static_cast<T>((sums[lane] + sums[64 + lane] + sums[128 + lane] +
+                                               sums[192 + lane]) / total);
+    __syncthreads();
+  }
 }
 
 // ---------------------------------------------------------------------------
@@ -878,8 +916,6 @@ WindowArgs<T> window_args(const WindowCall& call) {
   args.query = view_of<T>(*call.query);
   args.key = view_of<T>(*call.key);
   args.value = view_of<T>(*call.value);
-  args.whole = whole_pieces<T>(*call.query, p.D) && whole_pieces<T>(*call.key, p.D) &&
-               whole_pieces<T>(*call.value, p.Dv);
   args.sequences = sequences_of(p);
   args.heads = p.H;
   args.kv_heads = p.Hkv;
@@ -899,55 +935,71 @@ template <typename T, int WIDTH> constexpr int kForwardQueries = sizeof(T) == 4 
 template <typename T, int WIDTH> constexpr int kGradQueries = sizeof(T) == 4 && WIDTH == 128 ? 1 : 2;
 template <typename T, int WIDTH> constexpr int kGradKeys = sizeof(T) == 4 && WIDTH == 128 ? 1 : 2;
 
-template <typename T, int WIDTH, bool CACHED>
+template <typename T>
+bool whole_inputs(const WindowCall& call) {
+  const rosa_mixer_problem& p = *call.problem;
+  const auto aligned = [](const void* data) { return reinterpret_cast<uintptr_t>(data) % 16 == 0; };
+  return whole_pieces<T>(*call.query, p.D) && whole_pieces<T>(*call.key, p.D) &&
+         whole_pieces<T>(*call.value, p.Dv) &&
+         (call.grad_output == nullptr || whole_pieces<T>(*call.grad_output, p.Dv)) &&
+         aligned(call.output) && aligned(call.key_cache) && aligned(call.value_cache);
+}
+
+template <typename T, int WIDTH, bool CACHED, bool WHOLE>
 void window_forward_launch(WindowArgs<T>& args, hipStream_t stream) {
   constexpr int kQueries = kForwardQueries<T, WIDTH>;
   args.slots = slots_of(args.sequences, 64 * kQueries);
   args.items = args.slots * args.heads;
-  window_forward_kernel<T, WIDTH, kQueries, CACHED>
+  window_forward_kernel<T, WIDTH, kQueries, CACHED, WHOLE>
       <<<dim3(static_cast<unsigned>(grid_of(args.items))), kThreads, 0, stream>>>(args);
+}
+
+template <typename T, bool WHOLE>
+void window_forward_width(const WindowCall& call) {
+  WindowArgs<T> args = window_args<T>(call);
+  const rosa_mixer_problem& p = *call.problem;
+  switch (padded_width(p.D > p.Dv ? p.D : p.Dv)) {
+    case 32: return window_forward_launch<T, 32, false, WHOLE>(args, call.stream);
+    case 64: return window_forward_launch<T, 64, false, WHOLE>(args, call.stream);
+    default: return window_forward_launch<T, 128, false, WHOLE>(args, call.stream);
+  }
 }
 
 template <typename T>
 void window_forward(const WindowCall& call) {
-  WindowArgs<T> args = window_args<T>(call);
-  const rosa_mixer_problem& p = *call.problem;
-  switch (padded_width(p.D > p.Dv ? p.D : p.Dv)) {
-    case 32: return window_forward_launch<T, 32, false>(args, call.stream);
-    case 64: return window_forward_launch<T, 64, false>(args, call.stream);
-    default: return window_forward_launch<T, 128, false>(args, call.stream);
-  }
+  if (whole_inputs<T>(call))
+    window_forward_width<T, true>(call);
+  else
+    window_forward_width<T, false>(call);
 }
 
-template <typename T, int WIDTH>
+template <typename T, int WIDTH, bool WHOLE>
 void window_backward_launch(WindowArgs<T>& args, hipStream_t stream) {
   constexpr int kQueries = kGradQueries<T, WIDTH>, kWaveKeys = kGradKeys<T, WIDTH>;
   args.slots = slots_of(args.sequences, 64 * kQueries);
   args.items = args.slots * args.heads;
-  window_grad_query_kernel<T, WIDTH, kQueries>
+  window_grad_query_kernel<T, WIDTH, kQueries, WHOLE>
       <<<dim3(static_cast<unsigned>(grid_of(args.items))), kThreads, 0, stream>>>(args);
   if (args.grad_key == nullptr && args.grad_value == nullptr) return;
   args.key_block = 64 * kWaveKeys;
   if (args.sink_slots > 0) {
     args.items = args.sink_slots * args.kv_heads;
-    window_grad_key_kernel<T, WIDTH, 1, true>  // (64 keys hold all sinks)
+    window_grad_key_kernel<T, WIDTH, 1, true, WHOLE>  // (64 keys hold all sinks)
         <<<dim3(static_cast<unsigned>(grid_of(args.items))), kThreads, 0, stream>>>(args);
   }
   args.slots = slots_of(args.sequences, 64 * kWaveKeys);
   args.items = args.slots * args.kv_heads;
-  window_grad_key_kernel<T, WIDTH, kWaveKeys, false>
+  window_grad_key_kernel<T, WIDTH, kWaveKeys, false, WHOLE>
       <<<dim3(static_cast<unsigned>(grid_of(args.items))), kThreads, 0, stream>>>(args);
 }
 
-template <typename T>
-void window_backward(const WindowCall& call) {
+template <typename T, bool WHOLE>
+void window_backward_width(const WindowCall& call) {
   WindowArgs<T> args = window_args<T>(call);
   const rosa_mixer_problem& p = *call.problem;
   const WindowPlan plan = window_plan(p, call.window, call.sinks);
   args.grad_output = view_of<T>(*call.grad_output);
   args.output = static_cast<const T*>(call.output);
-  args.whole = args.whole && whole_pieces<T>(*call.grad_output, p.Dv) &&
-               reinterpret_cast<uintptr_t>(call.output) % 16 == 0;
   args.delta = reinterpret_cast<float*>(call.workspace);
   args.grad_query = static_cast<T*>(call.grad_query);
   args.grad_key = static_cast<T*>(call.grad_key);
@@ -956,13 +1008,21 @@ void window_backward(const WindowCall& call) {
   args.sink_sums =
       plan.sink_slots > 0 ? reinterpret_cast<float*>(call.workspace + plan.delta_bytes) : nullptr;
   switch (padded_width(p.D > p.Dv ? p.D : p.Dv)) {
-    case 32: return window_backward_launch<T, 32>(args, call.stream);
-    case 64: return window_backward_launch<T, 64>(args, call.stream);
-    default: return window_backward_launch<T, 128>(args, call.stream);
+    case 32: return window_backward_launch<T, 32, WHOLE>(args, call.stream);
+    case 64: return window_backward_launch<T, 64, WHOLE>(args, call.stream);
+    default: return window_backward_launch<T, 128, WHOLE>(args, call.stream);
   }
 }
 
-template <typename T, int WIDTH>
+template <typename T>
+void window_backward(const WindowCall& call) {
+  if (whole_inputs<T>(call))
+    window_backward_width<T, true>(call);
+  else
+    window_backward_width<T, false>(call);
+}
+
+template <typename T, int WIDTH, bool WHOLE>
 void window_update_launch(WindowArgs<T>& args, const WindowCall& call) {
   const rosa_mixer_problem& p = *call.problem;
   T* key_cache = static_cast<T*>(call.key_cache);
@@ -972,33 +1032,39 @@ void window_update_launch(WindowArgs<T>& args, const WindowCall& call) {
     TokenArgs<T> token{args, key_cache, value_cache, plan.splits, plan.head_blocks,
                        reinterpret_cast<float*>(call.workspace)};
     const unsigned blocks = static_cast<unsigned>(p.B) * p.Hkv * plan.head_blocks * plan.splits;
-    window_token_kernel<T, WIDTH><<<dim3(blocks), kThreads, 0, call.stream>>>(token);
+    window_token_kernel<T, WIDTH, WHOLE><<<dim3(blocks), kThreads, 0, call.stream>>>(token);
     if (plan.splits > 1)
-      window_token_join_kernel<T><<<dim3(static_cast<unsigned>(p.B) * p.H), kMostWidth, 0, call.stream>>>(
+      window_token_join_kernel<T><<<dim3(static_cast<unsigned>(p.B) * p.H), kThreads, 0, call.stream>>>(
           token.partial, args.out, plan.splits, p.Dv);
     return;
   }
-  window_forward_launch<T, WIDTH, true>(args, call.stream);
+  window_forward_launch<T, WIDTH, true, WHOLE>(args, call.stream);
   const int64_t blocks = slots_of(args.sequences, 64) * p.Hkv;
-  window_append_kernel<T>
+  window_append_kernel<T, WHOLE>
       <<<dim3(static_cast<unsigned>(blocks)), kThreads, 0, call.stream>>>(args, key_cache, value_cache);
 }
 
-template <typename T>
-void window_update(const WindowCall& call) {
+template <typename T, bool WHOLE>
+void window_update_width(const WindowCall& call) {
   WindowArgs<T> args = window_args<T>(call);
   const rosa_mixer_problem& p = *call.problem;
   args.key_cache = static_cast<const T*>(call.key_cache);
   args.value_cache = static_cast<const T*>(call.value_cache);
   args.lengths = call.lengths;
   args.capacity = call.capacity;
-  args.whole = args.whole && reinterpret_cast<uintptr_t>(call.key_cache) % 16 == 0 &&
-               reinterpret_cast<uintptr_t>(call.value_cache) % 16 == 0;
   switch (padded_width(p.D > p.Dv ? p.D : p.Dv)) {
-    case 32: return window_update_launch<T, 32>(args, call);
-    case 64: return window_update_launch<T, 64>(args, call);
-    default: return window_update_launch<T, 128>(args, call);
+    case 32: return window_update_launch<T, 32, WHOLE>(args, call);
+    case 64: return window_update_launch<T, 64, WHOLE>(args, call);
+    default: return window_update_launch<T, 128, WHOLE>(args, call);
   }
+}
+
+template <typename T>
+void window_update(const WindowCall& call) {
+  if (whole_inputs<T>(call))
+    window_update_width<T, true>(call);
+  else
+    window_update_width<T, false>(call);
 }
 
 }  // namespace rosa_mixer

@@ -132,34 +132,63 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2))) v
         }
   }
 
-  float weight[4][4];  // lambda^(i - j) of this lane's query row i and key rows j, 0 for j > i
+  // Weights of a token's scores, scale lambda^(i - j): of the tile of 16 keys that its own tile is,
+  // and of the tile before it, from which the ones before that are powers of lambda^16 away.
   const int own = wave * 16 + column;
+  float diagonal[4], before[4];
   if constexpr (!STATE_ONLY) {
 #pragma unroll
-    for (int t = 0; t < 4; ++t)
-#pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        const int apart = own - (t * 16 + 4 * group + r);
-        weight[t][r] = apart >= 0 ? power_of(rate, apart) : 0.0f;
-      }
+    for (int r = 0; r < 4; ++r) {
+      const int apart = column - 4 * group - r;
+      diagonal[r] = apart >= 0 ? a.scale * power_of(rate, apart) : 0.0f;
+      before[r] = a.scale * power_of(rate, 16 + apart);
+    }
   }
+  const float carry = a.scale * power_of(rate, own + 1);
 
   TileMove<T, kChunk, WIDTH, WHOLE> key_move;
   TileMove<T, kChunk, SLICE, WHOLE> value_move;
   Frag<T> next_query[kSteps];
   const auto fetch = [&](int at) {
-    const auto place = [&](int i) { return token(min(at + i, stop - 1)); };
-    key_move.fetch([&](int i) { return p.key.row(run.batch, place(i), key_head); }, p.key_width, tid);
-    value_move.fetch([&](int i) { return p.value.row(run.batch, place(i), value_head) + col0; },
-                     p.value_width - col0, tid);
+    // the chunk's tokens as they lie in memory
+    const int fill = min(kChunk, stop - at);
+    const int64_t first = run.begin + (p.reverse ? run.length - at - fill : at);
+    key_move.fetch(p.key.rows(run.batch, first, key_head, fill), p.key_width, tid);
+    Rows<T> values_here = p.value.rows(run.batch, first, value_head, fill);
+    values_here.base += col0;
+    value_move.fetch(values_here, p.value_width - col0, tid);
     if constexpr (!STATE_ONLY) {
-      const T* row = p.query.row(run.batch, place(own), query_head);
+      const Rows<T> queries = p.query.rows(run.batch, first, query_head, fill);
+      const int row = p.reverse ? max(fill - 1 - own, 0) : own;
 #pragma unroll
       for (int s = 0; s < kSteps; ++s)
-        next_query[s] = memory_operand<WHOLE>(row, s * 32 + 8 * group, p.key_width);
+        next_query[s] = memory_operand<WHOLE>(queries, row, s * 32 + 8 * group, p.key_width);
     }
   };
   fetch(start);
+  // what a row of values counts for in the state behind a whole chunk
+  float whole_chunk[value_move.kPieces];
+#pragma unroll
+  for (int i = 0; i < value_move.kPieces; ++i)
+    whole_chunk[i] = power_of(
+        rate, kChunk - 1 - value_move.walk_row(value_move.row_of(i, tid), p.reverse ? kChunk : 0));
+
+  // Outputs of a chunk are stored when the next one has begun: loads retire in order with the
+  // stores issued before them, and the wait for a chunk's tiles would be one for them as well.
+  f32x4 ready[kColTiles];
+  int ready_at = -1;
+  const auto store_ready = [&] {
+    if (ready_at < 0 || ready_at + own >= stop) return;
+    const int64_t row = ((run.first + token(ready_at + own) - run.begin) * a.heads + head) * p.value_width + col0;
+    const bool quads = WHOLE || p.value_width % 4 == 0;
+#pragma unroll
+    for (int t = 0; t < kColTiles; ++t) {
+      if (p.partial != nullptr)
+        store4(p.partial + row, t * 16 + 4 * group, ready[t], p.value_width - col0, quads);
+      else
+        store4(p.out + row, t * 16 + 4 * group, ready[t], p.value_width - col0, quads);
+    }
+  };
 
   float unit = 1.0f;  // float16: brings the rounded state into range
   if constexpr (kNarrow<T> && !STATE_ONLY) {
@@ -178,13 +207,18 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2))) v
   for (int at = start; at < stop; at += kChunk) {
     const int fill = min(kChunk, stop - at);
     // what this chunk reads goes to LDS: keys, values, weighted values, the state before it
-    key_move.store(keys, tid);
-    if constexpr (!STATE_ONLY) value_move.store(values, tid);
+    const int flip = p.reverse ? fill : 0;
+    key_move.store(keys, p.key_width, tid, flip);
+    if constexpr (!STATE_ONLY)
+      value_move.store(values, p.value_width - col0, tid, flip);
+    else
+      value_move.clear_padding(p.value_width - col0, tid);
 #pragma unroll
     for (int i = 0; i < value_move.kPieces; ++i) {
-      constexpr int kElements = value_move.kElements, kPerRow = value_move.kPerRow;
-      const int piece = i * kThreads + tid, row = piece / kPerRow;
-      const float by = row < fill ? power_of(rate, fill - 1 - row) : 0.0f;
+      constexpr int kElements = value_move.kElements;
+      const int row = value_move.walk_row(value_move.row_of(i, tid), flip);
+      float by = whole_chunk[i];
+      if (fill < kChunk) by = row < fill ? power_of(rate, fill - 1 - row) : 0.0f;
       float left[kElements];
 #pragma unroll
       for (int e = 0; e < kElements; ++e) left[e] = static_cast<float>(value_move.held[i][e]) * by;
@@ -198,7 +232,7 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2))) v
           left[e] -= static_cast<float>(term[e]);
         }
         *reinterpret_cast<Piece*>(weighted + (t * kChunk + row) * kPitch<ST, SLICE> +
-                                  piece % kPerRow * kElements) = term;
+                                  value_move.col_of(tid)) = term;
       }
     }
     if constexpr (!STATE_ONLY) {
@@ -221,12 +255,17 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2))) v
     Frag<T> query[kSteps];
     if constexpr (!STATE_ONLY) {
 #pragma unroll
-      for (int s = 0; s < kSteps; ++s) query[s] = next_query[s];
+      for (int s = 0; s < kSteps; ++s) {
+        query[s] = next_query[s];
+        clear_operand<WHOLE>(query[s], s * 32 + 8 * group, p.key_width);
+      }
     }
     __syncthreads();
+    if constexpr (!STATE_ONLY) store_ready();
     if (at + kChunk < stop) fetch(at + kChunk);
 
     if constexpr (!STATE_ONLY) {
+      ready_at = -1;
       if (wave * 16 < fill) {
         // outputs transposed: rows are value columns, columns are this wave's 16 tokens
         f32x4 out[kColTiles];
@@ -237,23 +276,30 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2))) v
 #pragma unroll
           for (int t = 0; t < kColTiles; ++t)
             out[t] = mma(row_operand<T, WIDTH>(state_rows, t * 16, s * 32, lane), query[s], out[t]);
-        float carried = power_of(rate, own + 1);
         f32x4 score[4];
+        float step = 1.0f;  // lambda^16 for every tile further back
+        const float tile_rate = power_of(rate, 16);
 #pragma unroll
-        for (int t = 0; t < 4; ++t) {
+        for (int t = 3; t >= 0; --t) {
           score[t] = f32x4(0.0f);
           if (t <= wave) {
 #pragma unroll
             for (int s = 0; s < kSteps; ++s)
               score[t] = mma(row_operand<T, WIDTH>(keys, t * 16, s * 32, lane), query[s], score[t]);
+            if (t == wave) {
 #pragma unroll
-            for (int r = 0; r < 4; ++r)  // (a select, so that keys behind a token never reach it)
-              score[t][r] = weight[t][r] == 0.0f ? 0.0f : score[t][r] * weight[t][r];
+              for (int r = 0; r < 4; ++r)  // (a select, so that later keys never reach a token)
+                score[t][r] = 4 * group + r <= column ? score[t][r] * diagonal[r] : 0.0f;
+            } else {
+#pragma unroll
+              for (int r = 0; r < 4; ++r) score[t][r] *= before[r] * step;
+              step *= tile_rate;
+            }
           }
         }
+        float carried = carry;
         float range = 1.0f;  // float16: the same for the scores of a token
         if constexpr (kNarrow<T>) {
-          carried /= unit;
           float most = 0.0f;
 #pragma unroll
           for (int t = 0; t < 4; ++t)
@@ -262,7 +308,7 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2))) v
           range = lift_of(over_groups_max(most));
 #pragma unroll
           for (int t = 0; t < 4; ++t) score[t] *= range;
-          carried *= range;
+          carried *= range / unit;
         }
 #pragma unroll
         for (int t = 0; t < kColTiles; ++t) out[t] *= carried;
@@ -275,18 +321,11 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2))) v
               out[t] = mma(column_operand<T, SLICE>(values, half * 32, t * 16, lane), scores, out[t]);
           }
         }
-        if (own < fill) {
-          const int64_t row =
-              ((run.first + token(at + own) - run.begin) * a.heads + head) * p.value_width + col0;
-          const bool quads = p.value_width % 4 == 0;
-          const float by = a.scale / range;
+        ready_at = at;
 #pragma unroll
-          for (int t = 0; t < kColTiles; ++t) {
-            if (p.partial != nullptr)
-              store4(p.partial + row, t * 16 + 4 * group, out[t] * by, p.value_width - col0, quads);
-            else
-              store4(p.out + row, t * 16 + 4 * group, out[t] * by, p.value_width - col0, quads);
-          }
+        for (int t = 0; t < kColTiles; ++t) {
+          ready[t] = out[t];
+          if constexpr (kNarrow<T>) ready[t] *= 1.0f / range;
         }
       }
     }
@@ -347,6 +386,7 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2))) v
     __syncthreads();
   }
 
+  if constexpr (!STATE_ONLY) store_ready();
   float* to = nullptr;
   if (STATE_ONLY)
     to = a.segment_states + ((pass_index * a.slots + slot) * a.heads + head) * state_size;
@@ -375,22 +415,8 @@ __global__ __launch_bounds__(kThreads) void decay_join_kernel(DecayArgs<T> a, in
   const int head = static_cast<int>(row % a.heads);
   const int pass_index = static_cast<int>(row / a.heads % a.passes);
   const int sequence = static_cast<int>(row / a.heads / a.passes);
-  Run run;
-  if (a.sequences.offsets == nullptr) {
-    run.sequence = sequence;
-    run.begin = 0;
-    run.length = a.sequences.length;
-  } else {
-    int bad = 0;
-    for (int s = tid; s < a.sequences.count; s += kThreads)
-      bad |= a.sequences.offsets[s] > a.sequences.offsets[s + 1] ||
-             (s == 0 && a.sequences.offsets[0] != 0) ||
-             (s == a.sequences.count - 1 && a.sequences.offsets[s + 1] != a.sequences.tokens);
-    if (__syncthreads_or(bad)) return;
-    run.sequence = sequence;
-    run.begin = a.sequences.offsets[sequence];
-    run.length = a.sequences.offsets[sequence + 1] - static_cast<int>(run.begin);
-  }
+  const Run run = run_of_sequence(a.sequences, sequence, tid);
+  if (run.length < 0) return;
   const int64_t slot = first_slot(a.sequences, run, a.segment);
   const int64_t e = blockIdx.x % pieces * kThreads + tid;
   if (e >= state_size) return;
@@ -566,7 +592,7 @@ template <typename T> constexpr int kUpdateTerms = sizeof(T) == 4 ? 1 : 3;
 template <typename T>
 void decay_forward(const DecayCall& call) {
   DecayArgs<T> args = decay_args<T>(call);
-  const DecayPlan plan = decay_plan(*call.problem, 1, false);
+  const DecayPlan plan = decay_plan(*call.problem, 1);
   args.passes = 1;
   args.pass[0] = decay_forward_pass<T>(call);
   args.segment_states = reinterpret_cast<float*>(call.workspace);
@@ -577,7 +603,7 @@ template <typename T>
 void decay_backward(const DecayCall& call) {
   const rosa_mixer_problem& p = *call.problem;
   const int share = p.H / p.Hkv;
-  const DecayPlan plan = decay_plan(p, 3, false);
+  const DecayPlan plan = decay_plan(p, 3);
   DecayArgs<T> args = decay_args<T>(call);
   args.segment_states = reinterpret_cast<float*>(call.workspace);
   float* partial = reinterpret_cast<float*>(call.workspace + plan.state_bytes);
@@ -635,7 +661,7 @@ void decay_update(const DecayCall& call) {
     return;
   }
   DecayArgs<T> args = decay_args<T>(call);
-  const DecayPlan plan = decay_plan(p, 1, true);
+  const DecayPlan plan = decay_plan(p, 1);
   args.passes = 1;
   args.pass[0] = decay_forward_pass<T>(call);
   args.segment_states = reinterpret_cast<float*>(call.workspace);

@@ -53,11 +53,12 @@ struct DecayPlan {
   size_t state_bytes;   // incoming states of all segments, all passes
   size_t partial_bytes; // one gradient of a shared head before the sum over its group
 };
-DecayPlan decay_plan(const rosa_mixer_problem& p, int passes, bool update);
+DecayPlan decay_plan(const rosa_mixer_problem& p, int passes);
 
 struct WindowPlan {
-  int64_t sink_slots;   // pieces of the rows that see sinks beyond their window
-  size_t delta_bytes, sink_bytes;
+  int64_t sink_slots;   // pieces of the tokens that see sinks beyond their window
+  size_t delta_bytes, sink_bytes, sink_part_bytes;
+  size_t bytes() const { return delta_bytes + sink_bytes + sink_part_bytes; }
 };
 WindowPlan window_plan(const rosa_mixer_problem& p, int window, int sinks);
 
@@ -67,7 +68,7 @@ struct TokenPlan {
 };
 TokenPlan token_plan(const rosa_mixer_problem& p, int64_t capacity);
 
-constexpr int kSinkRows = 1024;   // query rows of a piece
+constexpr int kSinkRows = 256;    // tokens of a piece
 
 #define ROSA_MIXER_LAUNCHERS(NAME)                                     \
   void window_forward_##NAME(const WindowCall& call);                  \

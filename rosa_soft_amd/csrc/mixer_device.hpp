@@ -113,6 +113,11 @@ __device__ __forceinline__ Frag<T> column_operand(const T* tile, int row0, int c
   return out;
 }
 
+// LDS reads and products stay on their side of this point.  Left alone, the compiler puts every
+// read directly in front of its use and the wave waits for LDS each time; the kernels read the
+// operands of one batch of products ahead of the products of the batch before it.
+__device__ __forceinline__ void in_order() { __builtin_amdgcn_sched_barrier(0x476); }
+
 // two results, rows [0, 16) and [16, 32) of the summed index, as the operand of the next product
 template <typename T>
 __device__ __forceinline__ Frag<T> operand_of(f32x4 low, f32x4 high) {
@@ -125,10 +130,31 @@ __device__ __forceinline__ Frag<T> operand_of(f32x4 low, f32x4 high) {
   return out;
 }
 
-// A tile of ROWS x WIDTH on its way from memory to LDS through the registers of the block.
-// `row_pointer` gives an existing row for every row of the tile (a caller repeats its last one and
-// masks what comes of it), so that loads are never predicated; columns from `width` on are zeros.
-// WHOLE: rows are whole 16-byte pieces at 16-byte addresses.
+// Rows of a head in memory: `stride` elements apart from `base` on, the last of them number `last`.
+template <typename T>
+struct Rows {
+  const T* base;
+  int64_t stride;
+  int last;
+};
+
+// Where element `col` of a row lies.  WHOLE: the stride is below 2^24 bytes, so that a 32-bit
+// offset from a base that the whole block shares is enough: no 64-bit arithmetic per load.
+template <bool WHOLE, typename T>
+__device__ __forceinline__ const T* place_of(const Rows<T>& rows, int row, int col) {
+  if constexpr (WHOLE) {
+    const uint32_t offset = __umul24(static_cast<uint32_t>(row),
+                                     static_cast<uint32_t>(rows.stride) * static_cast<uint32_t>(sizeof(T))) +
+                            static_cast<uint32_t>(col) * static_cast<uint32_t>(sizeof(T));
+    return reinterpret_cast<const T*>(reinterpret_cast<const char*>(rows.base) + offset);
+  } else {
+    return rows.base + row * rows.stride + col;
+  }
+}
+
+// A tile of ROWS x WIDTH on its way from memory to LDS through the registers of the block.  Rows
+// that do not exist are the last one again (a caller masks what comes of it), so that loads are
+// never predicated.  WHOLE: rows are whole 16-byte pieces at 16-byte addresses.
 template <typename T, int ROWS, int WIDTH, bool WHOLE>
 struct TileMove {
   static constexpr int kElements = 16 / static_cast<int>(sizeof(T));
@@ -139,66 +165,97 @@ struct TileMove {
 
   Piece held[kPieces];
 
-  template <typename RowPointer>
-  __device__ __forceinline__ void fetch(RowPointer&& row_pointer, int width, int tid) {
+  static __device__ __forceinline__ int row_of(int i, int tid) {
+    return i * (kThreads / kPerRow) + tid / kPerRow;
+  }
+  static __device__ __forceinline__ int col_of(int tid) { return tid % kPerRow * kElements; }
+
+  // `place(row, col)`: the address of an element
+  template <typename Place>
+  __device__ __forceinline__ void fetch_from(Place&& place, int width, int tid) {
+    const int col = col_of(tid);
 #pragma unroll
     for (int i = 0; i < kPieces; ++i) {
-      const int piece = i * kThreads + tid, col = piece % kPerRow * kElements;
-      const T* row = row_pointer(piece / kPerRow);
+      const int row = row_of(i, tid);
       if constexpr (WHOLE) {
-        held[i] = *reinterpret_cast<const Piece*>(row + min(col, width - kElements));
+        held[i] = *reinterpret_cast<const Piece*>(place(row, min(col, width - kElements)));
       } else {
+        const T* from = place(row, 0);
 #pragma unroll
-        for (int e = 0; e < kElements; ++e) held[i][e] = row[min(col + e, width - 1)];
+        for (int e = 0; e < kElements; ++e) held[i][e] = from[min(col + e, width - 1)];
       }
     }
-    if (width < WIDTH) {
+  }
+
+  __device__ __forceinline__ void fetch(const Rows<T>& rows, int width, int tid) {
+    fetch_from([&](int row, int col) { return place_of<WHOLE>(rows, min(row, rows.last), col); }, width,
+               tid);
+  }
+
+  // Columns from `width` on become zeros here, not where the loads were issued: touching a loaded
+  // register there would wait for it.
+  __device__ __forceinline__ void clear_padding(int width, int tid) {
+    const int col = col_of(tid);
+    if constexpr (WHOLE) {  // (all of a piece or nothing)
+      if (col >= width) {
 #pragma unroll
-      for (int i = 0; i < kPieces; ++i) {
-        const int col = (i * kThreads + tid) % kPerRow * kElements;
+        for (int i = 0; i < kPieces; ++i) held[i] = Piece(static_cast<T>(0.0f));
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < kPieces; ++i)
 #pragma unroll
         for (int e = 0; e < kElements; ++e)
           held[i][e] = col + e < width ? held[i][e] : static_cast<T>(0.0f);
-      }
     }
   }
 
-  __device__ __forceinline__ void store(T* tile, int tid) const {
+  // row r of a walk that runs backwards over `flip` rows of memory
+  static __device__ __forceinline__ int walk_row(int row, int flip) {
+    return row < flip ? flip - 1 - row : row;
+  }
+
+  __device__ __forceinline__ void store(T* tile, int width, int tid, int flip = 0) {
+    clear_padding(width, tid);
 #pragma unroll
-    for (int i = 0; i < kPieces; ++i) {
-      const int piece = i * kThreads + tid;
-      *reinterpret_cast<Piece*>(tile + piece / kPerRow * kPitch<T, WIDTH> +
-                                piece % kPerRow * kElements) = held[i];
-    }
+    for (int i = 0; i < kPieces; ++i)
+      *reinterpret_cast<Piece*>(tile + walk_row(row_of(i, tid), flip) * kPitch<T, WIDTH> +
+                                col_of(tid)) = held[i];
   }
 };
 
-// row-wise operand straight from memory: `row` is the lane's own row
+// row-wise operand straight from memory, of the lane's own row; columns from `width` on are some
+// other elements of it until clear_operand
 template <bool WHOLE, typename T>
-__device__ __forceinline__ Frag<T> memory_operand(const T* row, int col, int width) {
+__device__ __forceinline__ Frag<T> memory_operand(const Rows<T>& rows, int row, int col, int width) {
   Frag<T> out;
+  row = min(row, rows.last);
   if constexpr (WHOLE && sizeof(T) == 2) {
-    out = load8(row + min(col, width - 8));
-    if (col >= width) out = Frag<T>(static_cast<T>(0.0f));
+    out = load8(place_of<WHOLE>(rows, row, min(col, width - 8)));
   } else if constexpr (WHOLE) {
 #pragma unroll
     for (int half = 0; half < 2; ++half) {
-      f32x4 part = *reinterpret_cast<const f32x4*>(row + min(col + 4 * half, width - 4));
-      if (col + 4 * half >= width) part = f32x4(0.0f);
+      const f32x4 part =
+          *reinterpret_cast<const f32x4*>(place_of<WHOLE>(rows, row, min(col + 4 * half, width - 4)));
 #pragma unroll
       for (int e = 0; e < 4; ++e) out[4 * half + e] = part[e];
     }
   } else {
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      const T element = row[min(col + e, width - 1)];
-      out[e] = col + e < width ? element : static_cast<T>(0.0f);
-    }
+    for (int e = 0; e < 8; ++e) out[e] = *place_of<WHOLE>(rows, row, min(col + e, width - 1));
   }
   return out;
 }
 
-// four neighbouring elements of a contiguous output row
+template <bool WHOLE, typename T>
+__device__ __forceinline__ void clear_operand(Frag<T>& operand, int col, int width) {
+  constexpr int kPiece = WHOLE ? 16 / static_cast<int>(sizeof(T)) : 1;  // all or nothing
+#pragma unroll
+  for (int e = 0; e < 8; ++e)
+    operand[e] = col + e / kPiece * kPiece < width ? operand[e] : static_cast<T>(0.0f);
+}
+
+// four neighbouring elements of a contiguous output row; `quads`: rows are whole quads
 template <typename T>
 __device__ __forceinline__ void store4(T* row, int col, f32x4 value, int width, bool quads) {
   if (quads) {
@@ -245,6 +302,11 @@ struct View {
   int64_t batch_stride, token_stride, head_stride;
   __device__ __forceinline__ T* row(int64_t batch, int64_t token, int head) const {
     return data + batch * batch_stride + token * token_stride + head * head_stride;
+  }
+  // `count` tokens from `token` on
+  __device__ __forceinline__ Rows<std::remove_const_t<T>> rows(int64_t batch, int64_t token, int head,
+                                                               int count) const {
+    return {row(batch, token, head), token_stride, count - 1};
   }
 };
 
@@ -308,6 +370,18 @@ __device__ __forceinline__ Found find_run(const Sequences& q, int64_t slot, int 
   return static_cast<int64_t>(run->tile) * rows < run->length ? Found::kRun : Found::kNothing;
 }
 
+// The whole of a sequence, for a whole block; of length -1 where the offsets are invalid.
+__device__ __forceinline__ Run run_of_sequence(const Sequences& q, int sequence, int tid) {
+  if (q.offsets == nullptr)
+    return {sequence, q.length, 0, sequence, 0, static_cast<int64_t>(sequence) * q.length};
+  int bad = 0;
+  for (int s = tid; s < q.count; s += kThreads)
+    bad |= q.offsets[s] > q.offsets[s + 1] || (s == 0 && q.offsets[0] != 0) ||
+           (s == q.count - 1 && q.offsets[s + 1] != q.tokens);
+  const int begin = q.offsets[sequence], length = q.offsets[sequence + 1] - begin;
+  return {sequence, __syncthreads_or(bad) ? -1 : length, 0, 0, begin, begin};
+}
+
 // The slot of a sequence's first tile.
 __device__ __forceinline__ int64_t first_slot(const Sequences& q, const Run& run, int rows) {
   return q.offsets == nullptr ? static_cast<int64_t>(run.sequence) * ((q.length + rows - 1) / rows)
@@ -348,12 +422,13 @@ View<const T> view_of(const rosa_mixer_tensor& t) {
   return {static_cast<const T*>(t.data), t.batch_stride, t.token_stride, t.head_stride};
 }
 
-// rows of whole 16-byte pieces at 16-byte addresses
+// rows of whole 16-byte pieces at 16-byte addresses, less than 2^24 bytes apart
 template <typename T>
 bool whole_pieces(const rosa_mixer_tensor& t, int width) {
   const int64_t piece = 16 / sizeof(T);
   return reinterpret_cast<uintptr_t>(t.data) % 16 == 0 && width % piece == 0 &&
-         t.batch_stride % piece == 0 && t.token_stride % piece == 0 && t.head_stride % piece == 0;
+         t.batch_stride % piece == 0 && t.token_stride % piece == 0 && t.head_stride % piece == 0 &&
+         t.token_stride >= 0 && t.token_stride < (1 << 24) / static_cast<int64_t>(sizeof(T));
 }
 
 }  // namespace rosa_mixer

@@ -24,31 +24,45 @@ int64_t tile_slots(const rosa_mixer_problem& p, int64_t rows) {
 
 }  // namespace
 
-// A sequence is walked by one block per head and slice of 64 value columns; where that leaves
-// compute units idle it is cut into segments, whose states are summed by a walk of their own over
-// keys and values.  Segments are as long as leaves two blocks for a compute unit, and at least
-// four chunks.
-DecayPlan decay_plan(const rosa_mixer_problem& p, int passes, bool update) {
-  (void)update;
+// A sequence is walked by one block per head and slice of 64 value columns, chunk after chunk; where
+// that leaves compute units idle it is cut into segments, whose states are summed by a walk of
+// their own over keys and values and joined.  The number of segments is the one with the least
+// time by this count, in chunks: rounds of kBlocks resident blocks, 0.45 of a chunk for one that
+// is only summed (38 against 84 us at 2 x 4096 tokens, 32 heads of 128), the states' traffic and
+// the two more launches at 5 us a chunk.  Segments have at least two chunks.
+DecayPlan decay_plan(const rosa_mixer_problem& p, int passes) {
   const int width = padded_width(std::max(p.D, p.Dv));
   const int slices = width == 128 ? 2 : 1;
-  const int64_t per_token = static_cast<int64_t>(p.H) * slices * passes;
   const int64_t longest = p.cu_seqlens == nullptr ? p.T : p.N;
-  const int64_t sequences = p.cu_seqlens == nullptr ? p.B : p.S;
+  const int64_t walks = static_cast<int64_t>(p.H) * slices * passes;  // of every slot
   const int64_t state = static_cast<int64_t>(passes) * p.H * p.D * p.Dv * 4;
-  int64_t segment = p.N * per_token / (2 * kBlocks);
-  segment = std::max<int64_t>((segment + kDecayChunk - 1) / kDecayChunk * kDecayChunk, 4 * kDecayChunk);
-  const int64_t room = kMostStateBytes / state - sequences;  // segments beyond one per sequence
+  const int64_t chunks = (longest + kDecayChunk - 1) / kDecayChunk;
   DecayPlan plan{};
-  plan.segmented = segment < longest && room > 0 &&
-                   (p.cu_seqlens != nullptr || sequences * per_token < kBlocks);
-  if (plan.segmented) {
-    const int64_t least = (p.N / room + kDecayChunk) / kDecayChunk * kDecayChunk;
-    segment = std::max(segment, least);
-    plan.segmented = segment < longest;
+  int64_t best_segment = chunks;
+  double best = -1.0;
+  for (int64_t cuts = 1; cuts <= std::min<int64_t>(chunks, 256); ++cuts) {
+    const int64_t segment = (chunks + cuts - 1) / cuts;
+    if (cuts > 1 && segment < 2) break;
+    const int64_t slots = tile_slots(p, segment * kDecayChunk);
+    // (packed: how many slots hold tokens is not known here; as many as the tokens fill)
+    const int64_t filled = p.cu_seqlens == nullptr
+                               ? slots
+                               : std::max<int64_t>(1, p.N / (segment * kDecayChunk));
+    const double rounds = static_cast<double>((filled * walks + kBlocks - 1) / kBlocks);
+    double cost = rounds * segment;
+    if (cuts > 1) {
+      if (slots * state > kMostStateBytes) break;
+      const double summed = static_cast<double>((filled * walks * (cuts - 1) / cuts + kBlocks - 1) / kBlocks);
+      const double joined = 2.0 * static_cast<double>(filled * state) / 4.5e6 + 8.0;  // us
+      cost += 0.45 * summed * segment + joined / 5.0;
+    }
+    if (best < 0.0 || cost < best) {
+      best = cost;
+      best_segment = segment;
+      plan.segmented = cuts > 1;
+    }
   }
-  if (!plan.segmented) segment = (longest + kDecayChunk - 1) / kDecayChunk * kDecayChunk;
-  plan.segment = static_cast<int>(std::min<int64_t>(segment, 0x7fffffff / kDecayChunk * kDecayChunk));
+  plan.segment = static_cast<int>(std::min<int64_t>(best_segment, 0x7fffffff / kDecayChunk)) * kDecayChunk;
   plan.slots = tile_slots(p, plan.segment);
   plan.state_bytes = plan.segmented ? aligned(static_cast<size_t>(plan.slots) * state) : 0;
   if (passes > 1 && p.H > p.Hkv)
@@ -61,9 +75,10 @@ WindowPlan window_plan(const rosa_mixer_problem& p, int window, int sinks) {
   plan.delta_bytes = aligned(static_cast<size_t>(p.H) * p.N * 4);
   const int longest = p.cu_seqlens == nullptr ? p.T : p.N;
   if (sinks > 0 && window < longest) {
+    const size_t size = static_cast<size_t>(sinks) * (p.D + p.Dv) * 4;
     plan.sink_slots = tile_slots(p, kSinkRows);
-    plan.sink_bytes =
-        aligned(static_cast<size_t>(plan.sink_slots) * p.Hkv * sinks * (p.D + p.Dv) * 4);
+    plan.sink_bytes = aligned((p.cu_seqlens == nullptr ? p.B : p.S) * p.Hkv * size);
+    plan.sink_part_bytes = aligned(static_cast<size_t>(plan.sink_slots) * p.H * size);
   }
   return plan;
 }
@@ -136,7 +151,7 @@ bool is_token(const rosa_mixer_problem& p) { return p.cu_seqlens == nullptr && p
 
 size_t decay_bytes(const rosa_mixer_problem& p, int backward) {
   if (backward == 2 && is_token(p)) return 0;
-  const DecayPlan plan = decay_plan(p, backward == 1 ? 3 : 1, backward == 2);
+  const DecayPlan plan = decay_plan(p, backward == 1 ? 3 : 1);
   return plan.state_bytes + plan.partial_bytes;
 }
 
@@ -240,7 +255,7 @@ size_t rosa_hip_window_workspace_bytes(const rosa_mixer_problem* problem, int wi
   if (check(problem, capacity > 0) != 0 || check_window(window, sinks) != 0) return 0;
   if (capacity > 0) return std::max<size_t>(window_update_bytes(*problem, capacity), 256);
   const WindowPlan plan = window_plan(*problem, window, sinks);
-  return plan.delta_bytes + plan.sink_bytes;
+  return plan.bytes();
 }
 
 int rosa_hip_window_forward(const rosa_mixer_problem* problem, int window, int sinks,
@@ -277,7 +292,7 @@ int rosa_hip_window_backward(const rosa_mixer_problem* problem, int window, int 
     return bad;
   if (!output || !log_sum || !workspace) return rosa_fail(2, "window_backward: NULL pointer");
   const WindowPlan plan = window_plan(*problem, window, sinks);
-  if (workspace_bytes < plan.delta_bytes + plan.sink_bytes)
+  if (workspace_bytes < plan.bytes())
     return rosa_fail(3, "window_backward: workspace too small");
   if (!grad_query && !grad_key && !grad_value) return 0;
   WindowCall call{};

@@ -27,8 +27,13 @@ constexpr float kLog2e = 1.4426950408889634f;
 
 // Weights are formed as 2^kLift p and rounded so: float16 would lose bits of a weight below 2^-14,
 // which a long window's are.
-template <typename T> constexpr float kLift = kNarrow<T> ? 14.0f : 0.0f;
-template <typename T> constexpr float kUnlift = kNarrow<T> ? 1.0f / 16384.0f : 1.0f;
+template <typename T> constexpr float kLift = kNarrow<T> ? 8.0f : 0.0f;
+template <typename T> constexpr float kUnlift = kNarrow<T> ? 1.0f / 256.0f : 1.0f;
+
+// How far, in exponents of two, a score may pass the reference of its softmax before the sums so
+// far are scaled to a new one: weights up to 2^kSlack (with kLift below float16's largest) are as
+// exact, and most tiles leave the sums alone.
+constexpr float kSlack = 6.0f;
 
 template <typename T>
 struct WindowArgs {
@@ -37,7 +42,8 @@ struct WindowArgs {
   T* out;
   float *log_sum, *delta;    // [heads][tokens]
   T *grad_query, *grad_key, *grad_value;
-  float* sink_sums;          // [sink slot][kv head][sink][key_width + value_width]
+  float* sink_sums;          // [sequence][kv head][sink][key_width + value_width]
+  float* sink_parts;         // [sink slot][head][sink][key_width + value_width]
   const T *key_cache, *value_cache;
   const int32_t* lengths;
   int64_t capacity;
@@ -67,25 +73,39 @@ struct Seen {
 
 // of token t, keys from `row` on (the lane's first of a tile) that end before `end`
 __device__ __forceinline__ Seen seen_keys(int t, int row, int end, int window, int sinks) {
+  asm volatile("" : "+v"(row));  // (stays on the path of the tiles that need it)
   return {t - window + 1 - row, min(t, end - 1) - row, sinks - row};
 }
 
-// The rows of keys and values by position: those before `past` in the cache, the others among the
-// new tokens.
+// The rows of keys or values of a head by position: those before `past` in the cache, the others
+// among the new tokens.
 template <typename T, bool CACHED>
-struct KeyRows {
-  const T *key, *value;                 // of position 0, or of the first new token
-  int64_t key_stride, value_stride;
-  const T *key_cache, *value_cache;     // of row 0
-  int key_width, value_width, past;
+struct History {
+  const T* fresh;               // of the first new token
+  int64_t stride;
+  const T* cache;               // of row 0
+  int width, past;
   CacheRows rows;
-  __device__ __forceinline__ const T* key_row(int s) const {
-    if (CACHED && s < past) return key_cache + static_cast<int64_t>(rows.row(s)) * key_width;
-    return key + (CACHED ? s - past : s) * key_stride;
+  __device__ __forceinline__ const T* row(int s) const {
+    if (CACHED && s < past) return cache + static_cast<int64_t>(rows.row(s)) * width;
+    return fresh + (CACHED ? s - past : s) * stride;
   }
-  __device__ __forceinline__ const T* value_row(int s) const {
-    if (CACHED && s < past) return value_cache + static_cast<int64_t>(rows.row(s)) * value_width;
-    return value + (CACHED ? s - past : s) * value_stride;
+  // Positions [begin, end), as rows that lie one behind the other.  Those of a cache do not where
+  // the ring closes, nor where they end and the new tokens begin.
+  __device__ __forceinline__ bool in_order(int begin, int end) const {
+    if (!CACHED || begin >= past) return true;
+    return end <= past && (begin < rows.sinks ? end <= rows.sinks
+                                              : rows.row(begin) + (end - 1 - begin) < rows.sinks + rows.ring);
+  }
+  __device__ __forceinline__ Rows<T> span(int begin, int end) const {
+    return {row(begin), CACHED && begin < past ? width : stride, end - 1 - begin};
+  }
+  template <typename Move>
+  __device__ __forceinline__ void fetch(Move& move, int begin, int end, int tid) const {
+    if (in_order(begin, end))
+      move.fetch(span(begin, end), width, tid);
+    else
+      move.fetch_from([&](int i, int col) { return row(min(begin + i, end - 1)) + col; }, width, tid);
   }
 };
 
@@ -96,20 +116,16 @@ __device__ __forceinline__ int tokens_before(const WindowArgs<T>& a, const Run& 
 }
 
 template <bool CACHED, typename T>
-__device__ __forceinline__ KeyRows<T, CACHED> key_rows(const WindowArgs<T>& a, const Run& run,
-                                                       int kv_head, int past) {
-  KeyRows<T, CACHED> rows{};
-  rows.key = a.key.row(run.batch, run.begin, kv_head);
-  rows.value = a.value.row(run.batch, run.begin, kv_head);
-  rows.key_stride = a.key.token_stride;
-  rows.value_stride = a.value.token_stride;
+__device__ __forceinline__ History<T, CACHED> history_of(const WindowArgs<T>& a, const View<const T>& view,
+                                                         const T* cache, int width, const Run& run,
+                                                         int kv_head, int past) {
+  History<T, CACHED> rows{};
+  rows.fresh = view.row(run.batch, run.begin, kv_head);
+  rows.stride = view.token_stride;
+  rows.width = width;
   rows.past = past;
   if constexpr (CACHED) {
-    const int64_t at = (static_cast<int64_t>(run.sequence) * a.kv_heads + kv_head) * a.capacity;
-    rows.key_cache = a.key_cache + at * a.key_width;
-    rows.value_cache = a.value_cache + at * a.value_width;
-    rows.key_width = a.key_width;
-    rows.value_width = a.value_width;
+    rows.cache = cache + (static_cast<int64_t>(run.sequence) * a.kv_heads + kv_head) * a.capacity * width;
     rows.rows = {a.sinks, static_cast<int>(a.capacity) - a.sinks};
   }
   return rows;
@@ -152,25 +168,32 @@ window_forward_kernel(WindowArgs<T> a) {
   }
   const int past = tokens_before<CACHED>(a, run);
   const int first = past + run.tile * kRows, last = min(first + kRows, past + run.length) - 1;
-  const KeyRows<T, CACHED> rows = key_rows<CACHED>(a, run, kv_head, past);
+  const History<T, CACHED> key_rows = history_of<CACHED>(a, a.key, a.key_cache, a.key_width, run, kv_head, past);
+  const History<T, CACHED> value_rows =
+      history_of<CACHED>(a, a.value, a.value_cache, a.value_width, run, kv_head, past);
 
   // this wave's tokens, as the columns of operands
   const int wave_first = first + wave * 16 * QUERIES, wave_last = wave_first + 16 * QUERIES - 1;
   Frag<T> query[QUERIES][kSteps];
+  const Rows<T> query_rows = a.query.rows(run.batch, run.begin + first - past, head, last - first + 1);
 #pragma unroll
   for (int i = 0; i < QUERIES; ++i) {
-    const int t = wave_first + i * 16 + column;
-    const T* row = a.query.row(run.batch, run.begin + min(t, last) - past, head);
+    const int row = wave * 16 * QUERIES + i * 16 + column;
 #pragma unroll
-    for (int s = 0; s < kSteps; ++s)
-      query[i][s] = memory_operand<WHOLE>(row, s * 32 + 8 * group, a.key_width);
+    for (int s = 0; s < kSteps; ++s) {
+      query[i][s] = memory_operand<WHOLE>(query_rows, row, s * 32 + 8 * group, a.key_width);
+      clear_operand<WHOLE>(query[i][s], s * 32 + 8 * group, a.key_width);
+    }
   }
   f32x4 out[QUERIES][kCols];
-  float most[QUERIES], sum[QUERIES];
+  float most[QUERIES];
+  // The sums of the weights: for the 16-bit types a product with ones, which adds what is rounded
+  // and takes no vector instructions (every row of the result is the sum).
+  f32x4 sum[QUERIES];
 #pragma unroll
   for (int i = 0; i < QUERIES; ++i) {
     most[i] = -__builtin_inff();
-    sum[i] = 0.0f;
+    sum[i] = f32x4(0.0f);
 #pragma unroll
     for (int d = 0; d < kCols; ++d) out[i][d] = f32x4(0.0f);
   }
@@ -180,15 +203,15 @@ window_forward_kernel(WindowArgs<T> a) {
   KeyTiles tiles(first, last, a.window, a.sinks);
   const auto fetch = [&] {
     const int begin = tiles.begin(), end = tiles.end();
-    key_move.fetch([&](int i) { return rows.key_row(min(begin + i, end - 1)); }, a.key_width, tid);
-    value_move.fetch([&](int i) { return rows.value_row(min(begin + i, end - 1)); }, a.value_width, tid);
+    key_rows.fetch(key_move, begin, end, tid);
+    value_rows.fetch(value_move, begin, end, tid);
   };
   fetch();
   while (tiles.more()) {
     const int begin = tiles.begin(), end = tiles.end();
     tiles.next();
-    key_move.store(keys, tid);
-    value_move.store(values, tid);
+    key_move.store(keys, a.key_width, tid);
+    value_move.store(values, a.value_width, tid);
     __syncthreads();
     if (tiles.more()) fetch();
     // nothing of this tile is visible to the wave: behind it, or before its windows and no sink
@@ -197,21 +220,40 @@ window_forward_kernel(WindowArgs<T> a) {
     if (!none) {
       const bool all = end - begin == kKeys && end - 1 <= wave_first && wave_last - begin < a.window;
       f32x4 score[QUERIES][4];
+      Frag<T> key[2][kSteps];
+      const auto read_keys = [&](int k) {
+#pragma unroll
+        for (int s = 0; s < kSteps; ++s)
+          key[k & 1][s] = row_operand<T, WIDTH>(keys, k * 16, s * 32, lane);
+      };
+      read_keys(0);
 #pragma unroll
       for (int k = 0; k < 4; ++k) {
+        if (k + 1 < 4) read_keys(k + 1);
+        in_order();
 #pragma unroll
         for (int i = 0; i < QUERIES; ++i) score[i][k] = f32x4(0.0f);
 #pragma unroll
-        for (int s = 0; s < kSteps; ++s) {
-          const Frag<T> key = row_operand<T, WIDTH>(keys, k * 16, s * 32, lane);
+        for (int s = 0; s < kSteps; ++s)
 #pragma unroll
-          for (int i = 0; i < QUERIES; ++i) score[i][k] = mma(key, query[i][s], score[i][k]);
-        }
+          for (int i = 0; i < QUERIES; ++i) score[i][k] = mma(key[k & 1][s], query[i][s], score[i][k]);
+        in_order();
       }
-      Frag<T> weights[QUERIES][2];
+      // (the first values, for when the weights are there)
+      Frag<T> value[2][2][2];
+      const auto read_values = [&](int d) {
 #pragma unroll
-      for (int i = 0; i < QUERIES; ++i) {
-        if (!all) {
+        for (int half = 0; half < 2; ++half)
+#pragma unroll
+          for (int e = 0; e < 2; ++e)
+            value[d / 2 & 1][half][e] = column_operand<T, WIDTH>(values, half * 32, (d + e) * 16, lane);
+      };
+      read_values(0);
+      in_order();
+      Frag<T> weights[QUERIES][2];
+      if (!all) {
+#pragma unroll
+        for (int i = 0; i < QUERIES; ++i) {
           const Seen seen = seen_keys(wave_first + i * 16 + column, begin + 4 * group, end, a.window,
                                       a.sinks);
 #pragma unroll
@@ -220,13 +262,16 @@ window_forward_kernel(WindowArgs<T> a) {
             for (int r = 0; r < 4; ++r)
               score[i][k][r] = seen(k * 16 + r) ? score[i][k][r] : -__builtin_inff();
         }
+      }
+#pragma unroll
+      for (int i = 0; i < QUERIES; ++i) {
         float here = score[i][0][0];
 #pragma unroll
         for (int k = 0; k < 4; ++k)
 #pragma unroll
           for (int r = 0; r < 4; ++r) here = fmaxf(here, score[i][k][r]);
         here = over_groups_max(here) * factor;
-        if (__any(here > most[i])) {
+        if (__any(here > most[i] + kSlack)) {
           const float larger = fmaxf(here, most[i]);
           const float shrink = larger == -__builtin_inff() ? 1.0f : exp2_of(most[i] - larger);
           sum[i] *= shrink;
@@ -240,29 +285,38 @@ window_forward_kernel(WindowArgs<T> a) {
 #pragma unroll
           for (int r = 0; r < 4; ++r) {
             score[i][k][r] = exp2_of(score[i][k][r] * factor - base);
-            sum[i] += score[i][k][r];
+            if constexpr (sizeof(T) == 4) sum[i][r] += score[i][k][r];
           }
 #pragma unroll
-        for (int half = 0; half < 2; ++half)
+        for (int half = 0; half < 2; ++half) {
           weights[i][half] = operand_of<T>(score[i][2 * half], score[i][2 * half + 1]);
+          if constexpr (sizeof(T) == 2)
+            sum[i] = mma(Frag<T>(static_cast<T>(1.0f)), weights[i][half], sum[i]);
+        }
       }
 #pragma unroll
-      for (int half = 0; half < 2; ++half)
+      for (int d = 0; d < kCols; d += 2) {
+        if (d + 2 < kCols) read_values(d + 2);
+        in_order();
 #pragma unroll
-        for (int d = 0; d < kCols; ++d) {
-          const Frag<T> value = column_operand<T, WIDTH>(values, half * 32, d * 16, lane);
+        for (int half = 0; half < 2; ++half)
 #pragma unroll
-          for (int i = 0; i < QUERIES; ++i) out[i][d] = mma(value, weights[i][half], out[i][d]);
-        }
+          for (int e = 0; e < 2; ++e)
+#pragma unroll
+            for (int i = 0; i < QUERIES; ++i)
+              out[i][d + e] = mma(value[d / 2 & 1][half][e], weights[i][half], out[i][d + e]);
+        in_order();
+      }
     }
     __syncthreads();
   }
 
-  const bool quads = a.value_width % 4 == 0;
+  const bool quads = WHOLE || a.value_width % 4 == 0;
 #pragma unroll
   for (int i = 0; i < QUERIES; ++i) {
     const int t = wave_first + i * 16 + column;
-    const float total = over_groups_sum(sum[i]);
+    float total = sum[i][0];
+    if constexpr (sizeof(T) == 4) total = over_groups_sum(sum[i][0] + sum[i][1] + sum[i][2] + sum[i][3]);
     if (t > last) continue;
     const int64_t token = run.first + t - past;
     T* to = a.out + (token * a.heads + head) * a.value_width;
@@ -299,30 +353,36 @@ window_grad_query_kernel(WindowArgs<T> a) {
     return;
   }
   const int first = run.tile * kRows, last = min(first + kRows, run.length) - 1;
-  const KeyRows<T, false> rows = key_rows<false>(a, run, kv_head, 0);
+  const History<T, false> key_rows = history_of<false>(a, a.key, a.key_cache, a.key_width, run, kv_head, 0);
+  const History<T, false> value_rows =
+      history_of<false>(a, a.value, a.value_cache, a.value_width, run, kv_head, 0);
   const int wave_first = first + wave * 16 * QUERIES, wave_last = wave_first + 16 * QUERIES - 1;
 
   Frag<T> query[QUERIES][kSteps], grad[QUERIES][kSteps];
   float log_sum[QUERIES], delta[QUERIES], unit[QUERIES];
+  const int count = last - first + 1;
+  const Rows<T> query_rows = a.query.rows(run.batch, run.begin + first, head, count);
+  const Rows<T> grad_rows = a.grad_output.rows(run.batch, run.begin + first, head, count);
+  const Rows<T> out_rows{a.output + ((run.first + first) * a.heads + head) * a.value_width,
+                         static_cast<int64_t>(a.heads) * a.value_width, count - 1};
 #pragma unroll
   for (int i = 0; i < QUERIES; ++i) {
-    const int t = wave_first + i * 16 + column;
-    const bool there = t <= last;
-    const int row_t = min(t, last);
-    const T* row = a.query.row(run.batch, run.begin + row_t, head);
-    const T* grad_row = a.grad_output.row(run.batch, run.begin + row_t, head);
-    const T* out_row = a.output + ((run.first + row_t) * a.heads + head) * a.value_width;
+    const int row = wave * 16 * QUERIES + i * 16 + column;
+    const bool there = row < count;
     float dot = 0.0f;
 #pragma unroll
     for (int s = 0; s < kSteps; ++s) {
-      query[i][s] = memory_operand<WHOLE>(row, s * 32 + 8 * group, a.key_width);
-      grad[i][s] = memory_operand<WHOLE>(grad_row, s * 32 + 8 * group, a.value_width);
-      const Frag<T> out = memory_operand<WHOLE>(out_row, s * 32 + 8 * group, a.value_width);
+      query[i][s] = memory_operand<WHOLE>(query_rows, row, s * 32 + 8 * group, a.key_width);
+      grad[i][s] = memory_operand<WHOLE>(grad_rows, row, s * 32 + 8 * group, a.value_width);
+      Frag<T> out = memory_operand<WHOLE>(out_rows, row, s * 32 + 8 * group, a.value_width);
+      clear_operand<WHOLE>(query[i][s], s * 32 + 8 * group, a.key_width);
+      clear_operand<WHOLE>(grad[i][s], s * 32 + 8 * group, a.value_width);
+      clear_operand<WHOLE>(out, s * 32 + 8 * group, a.value_width);
 #pragma unroll
       for (int e = 0; e < 8; ++e) dot += static_cast<float>(grad[i][s][e]) * static_cast<float>(out[e]);
     }
     delta[i] = over_groups_sum(dot);
-    const int64_t at = static_cast<int64_t>(head) * a.sequences.tokens + run.first + row_t;
+    const int64_t at = static_cast<int64_t>(head) * a.sequences.tokens + run.first + first + min(row, count - 1);
     log_sum[i] = a.log_sum[at];
     if (there && group == 0) a.delta[at] = delta[i];
     unit[i] = kNarrow<T> ? 0.0f : 1.0f;
@@ -339,15 +399,15 @@ window_grad_query_kernel(WindowArgs<T> a) {
   KeyTiles tiles(first, last, a.window, a.sinks);
   const auto fetch = [&] {
     const int begin = tiles.begin(), end = tiles.end();
-    key_move.fetch([&](int i) { return rows.key_row(min(begin + i, end - 1)); }, a.key_width, tid);
-    value_move.fetch([&](int i) { return rows.value_row(min(begin + i, end - 1)); }, a.value_width, tid);
+    key_rows.fetch(key_move, begin, end, tid);
+    value_rows.fetch(value_move, begin, end, tid);
   };
   fetch();
   while (tiles.more()) {
     const int begin = tiles.begin(), end = tiles.end();
     tiles.next();
-    key_move.store(keys, tid);
-    value_move.store(values, tid);
+    key_move.store(keys, a.key_width, tid);
+    value_move.store(values, a.value_width, tid);
     __syncthreads();
     if (tiles.more()) fetch();
     const bool none = begin > min(wave_last, last) || wave_first > last ||
@@ -416,7 +476,7 @@ window_grad_query_kernel(WindowArgs<T> a) {
     }
     __syncthreads();
   }
-  const bool quads = a.key_width % 4 == 0;
+  const bool quads = WHOLE || a.key_width % 4 == 0;
 #pragma unroll
   for (int i = 0; i < QUERIES; ++i) {
     const int t = wave_first + i * 16 + column;
@@ -428,14 +488,18 @@ window_grad_query_kernel(WindowArgs<T> a) {
   }
 }
 
+// The tokens from here on see the sinks beyond their window: the first block of keys of a sequence
+// walks the tokens before it, window_grad_sinks_kernel the others.
+__device__ __forceinline__ int64_t walk_end(int first, int keys, int window) {
+  return static_cast<int64_t>(first) + keys - 1 + window;
+}
+
 // dk and dv of the keys of a block, 16 KEYS to a wave, over the tokens that see them: scores have
-// the tokens down and the wave's keys across.  The tokens beyond the window of the sinks are a
-// walk of their own (SINKS): pieces of kSinkRows tokens, each with a sum of its own in memory,
-// which the block of the sequence's first keys starts from.
-template <typename T, int WIDTH, int KEYS, bool SINKS, bool WHOLE>
+// the tokens down and the wave's keys across.
+template <typename T, int WIDTH, int KEYS, bool WHOLE>
 __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(WIDTH * sizeof(T) > 128 ? 1 : 2))) void
 window_grad_key_kernel(WindowArgs<T> a) {
-  constexpr int kSteps = WIDTH / 32, kRows = SINKS ? kSinkRows : 64 * KEYS, kCols = WIDTH / 16;
+  constexpr int kSteps = WIDTH / 32, kRows = 64 * KEYS, kCols = WIDTH / 16;
   constexpr int kQueries = sizeof(T) == 4 && WIDTH == 128 ? 32 : 64;  // (registers)
   __shared__ __attribute__((aligned(16))) T queries[kQueries * kPitch<T, WIDTH>];
   __shared__ __attribute__((aligned(16))) T grads[kQueries * kPitch<T, WIDTH>];
@@ -445,13 +509,12 @@ window_grad_key_kernel(WindowArgs<T> a) {
   if (item >= a.items) return;
   const int tid = threadIdx.x, lane = tid & 63, group = lane >> 4, column = lane & 15;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int64_t slots = SINKS ? a.sink_slots : a.slots;
-  const int64_t slot = item % slots;
-  const int kv_head = static_cast<int>(item / slots);
+  const int64_t slot = item % a.slots;
+  const int kv_head = static_cast<int>(item / a.slots);
   Run run;
   const Found found = find_run(a.sequences, slot, kRows, tid, &run);
   if (found != Found::kRun) {
-    if (!SINKS && found == Found::kInvalid) {
+    if (found == Found::kInvalid) {
       const int64_t first = slot * kRows;
       const int64_t last = min(first + kRows, static_cast<int64_t>(a.sequences.tokens));
       fill_nan(a.grad_key, first, last, a.kv_heads, kv_head, a.key_width, tid);
@@ -459,32 +522,25 @@ window_grad_key_kernel(WindowArgs<T> a) {
     }
     return;
   }
-  // keys of the block; the tokens [from, to) walked for them
-  const int first = SINKS ? 0 : run.tile * kRows;
-  const int behind = SINKS ? min(a.sinks, run.length) : min(first + kRows, run.length);
-  // the tokens that see the keys of the first block in their window end here, in whole tiles
-  const auto window_end = [&](int block_first, int rows) {
-    const int64_t end = static_cast<int64_t>(block_first) + rows - 1 + a.window;
-    return static_cast<int>(min(static_cast<int64_t>(run.length), (end + kQueries - 1) / kQueries * kQueries));
-  };
-  const int sink_begin = window_end(0, a.key_block);
-  const int from = SINKS ? max(sink_begin, run.tile * kRows) : first;
-  const int to = SINKS ? min(run.length, (run.tile + 1) * kRows) : window_end(first, kRows);
+  // keys of the block; the tokens [first, to) walked for them
+  const int first = run.tile * kRows, behind = min(first + kRows, run.length);
+  const int to = static_cast<int>(min<int64_t>(run.length, walk_end(first, kRows, a.window)));
   const int sums = a.key_width + a.value_width;
-  if (SINKS && from >= to) return;  // (nor are its sums read)
 
   const int wave_first = first + wave * 16 * KEYS;
+  const Rows<T> key_rows = a.key.rows(run.batch, run.begin + first, kv_head, behind - first);
+  const Rows<T> value_rows = a.value.rows(run.batch, run.begin + first, kv_head, behind - first);
   Frag<T> key[KEYS][kSteps], value[KEYS][kSteps];
   f32x4 grad_key[KEYS][kCols], grad_value[KEYS][kCols];
 #pragma unroll
   for (int i = 0; i < KEYS; ++i) {
-    const int s = wave_first + i * 16 + column;
-    const T* row = a.key.row(run.batch, run.begin + min(s, behind - 1), kv_head);
-    const T* value_row = a.value.row(run.batch, run.begin + min(s, behind - 1), kv_head);
+    const int row = wave * 16 * KEYS + i * 16 + column;
 #pragma unroll
     for (int step = 0; step < kSteps; ++step) {
-      key[i][step] = memory_operand<WHOLE>(row, step * 32 + 8 * group, a.key_width);
-      value[i][step] = memory_operand<WHOLE>(value_row, step * 32 + 8 * group, a.value_width);
+      key[i][step] = memory_operand<WHOLE>(key_rows, row, step * 32 + 8 * group, a.key_width);
+      value[i][step] = memory_operand<WHOLE>(value_rows, row, step * 32 + 8 * group, a.value_width);
+      clear_operand<WHOLE>(key[i][step], step * 32 + 8 * group, a.key_width);
+      clear_operand<WHOLE>(value[i][step], step * 32 + 8 * group, a.value_width);
     }
 #pragma unroll
     for (int d = 0; d < kCols; ++d) grad_key[i][d] = grad_value[i][d] = f32x4(0.0f);
@@ -492,23 +548,20 @@ window_grad_key_kernel(WindowArgs<T> a) {
   float unit[KEYS];
 #pragma unroll
   for (int i = 0; i < KEYS; ++i) unit[i] = kNarrow<T> ? 0.0f : 1.0f;
-  if (!SINKS && run.tile == 0 && a.sink_sums != nullptr && sink_begin < run.length) {
-    const int64_t slot0 = first_slot(a.sequences, run, kSinkRows);
-    for (int piece = sink_begin / kSinkRows; piece * kSinkRows < run.length; ++piece) {
-      const float* from_piece = a.sink_sums + ((slot0 + piece) * a.kv_heads + kv_head) * a.sinks * sums;
+  if (run.tile == 0 && a.sink_sums != nullptr && to < run.length) {
+    const float* sinks = a.sink_sums + (static_cast<int64_t>(run.sequence) * a.kv_heads + kv_head) * a.sinks * sums;
 #pragma unroll
-      for (int i = 0; i < KEYS; ++i) {
-        const int s = wave_first + i * 16 + column;
-        if (s >= behind || s >= a.sinks) continue;
+    for (int i = 0; i < KEYS; ++i) {
+      const int s = wave_first + i * 16 + column;
+      if (s >= a.sinks) continue;
 #pragma unroll
-        for (int d = 0; d < kCols; ++d)
+      for (int d = 0; d < kCols; ++d)
 #pragma unroll
-          for (int r = 0; r < 4; ++r) {
-            const int col = d * 16 + 4 * group + r;
-            if (col < a.key_width) grad_key[i][d][r] += from_piece[s * sums + col];
-            if (col < a.value_width) grad_value[i][d][r] += from_piece[s * sums + a.key_width + col];
-          }
-      }
+        for (int r = 0; r < 4; ++r) {
+          const int col = d * 16 + 4 * group + r;
+          if (col < a.key_width) grad_key[i][d][r] = sinks[s * sums + col];
+          if (col < a.value_width) grad_value[i][d][r] = sinks[s * sums + a.key_width + col];
+        }
     }
   }
   const float factor = a.scale * kLog2e;
@@ -516,25 +569,24 @@ window_grad_key_kernel(WindowArgs<T> a) {
 
   TileMove<T, kQueries, WIDTH, WHOLE> query_move, grad_move;
   float next_log_sum = 0.0f, next_delta = 0.0f;
-  const int rows_here = to - from;
-  const int walk = (rows_here + kQueries - 1) / kQueries;
+  const int walk = (to - first + kQueries - 1) / kQueries;
   const auto fetch = [&](int step) {
-    const int head = kv_head * a.share + step / walk, begin = from + step % walk * kQueries;
-    const auto token = [&](int i) { return run.begin + min(begin + i, to - 1); };
-    query_move.fetch([&](int i) { return a.query.row(run.batch, token(i), head); }, a.key_width, tid);
-    grad_move.fetch([&](int i) { return a.grad_output.row(run.batch, token(i), head); }, a.value_width,
-                    tid);
+    const int head = kv_head * a.share + step / walk, begin = first + step % walk * kQueries;
+    const int count = min(kQueries, to - begin);
+    query_move.fetch(a.query.rows(run.batch, run.begin + begin, head, count), a.key_width, tid);
+    grad_move.fetch(a.grad_output.rows(run.batch, run.begin + begin, head, count), a.value_width, tid);
     if (tid < kQueries) {
-      const int64_t at = static_cast<int64_t>(head) * a.sequences.tokens + run.first - run.begin + token(tid);
+      const int64_t at =
+          static_cast<int64_t>(head) * a.sequences.tokens + run.first + begin + min(tid, count - 1);
       next_log_sum = a.log_sum[at] - kLift<T>;
       next_delta = a.delta[at];
     }
   };
   fetch(0);
   for (int step = 0; step < walk * a.share; ++step) {
-    const int begin = from + step % walk * kQueries;
-    query_move.store(queries, tid);
-    grad_move.store(grads, tid);
+    const int begin = first + step % walk * kQueries;
+    query_move.store(queries, a.key_width, tid);
+    grad_move.store(grads, a.value_width, tid);
     if (tid < kQueries) {
       log_sums[tid] = next_log_sum;
       deltas[tid] = next_delta;
@@ -543,7 +595,7 @@ window_grad_key_kernel(WindowArgs<T> a) {
     if (step + 1 < walk * a.share) fetch(step + 1);
     const int wave_last = min(wave_first + 16 * KEYS, behind) - 1;
     const bool none = idle || begin + kQueries - 1 < wave_first ||
-                      (!SINKS && begin - wave_last >= a.window && wave_first >= a.sinks);
+                      (begin - wave_last >= a.window && wave_first >= a.sinks);
     if (!none) {
       const bool all = wave_last - wave_first + 1 == 16 * KEYS && wave_last <= begin &&
                        begin + kQueries <= to && begin + kQueries - 1 - wave_first < a.window;
@@ -574,17 +626,22 @@ window_grad_key_kernel(WindowArgs<T> a) {
               weight[i][k][r] = exp2_of(weight[i][k][r] * factor - log_sum[r]);  // (lifted)
               slope[i][k][r] = weight[i][k][r] * (slope[i][k][r] - delta[r]);
             }
-            if (!all) {  // tokens t from this row on that see key s: s <= t < to, t - s < window
-              const int s = wave_first + i * 16 + column, row = begin + row0 + 4 * group;
-              const int64_t end = s >= behind ? 0 : s < a.sinks ? to : min<int64_t>(to, int64_t{s} + a.window);
-              const int first_seen = s - row, last_seen = static_cast<int>(end) - 1 - row;
+          }
+        }
+        if (!all) {  // tokens t from this row on that see key s: s <= t < to, t - s < window
+#pragma unroll
+          for (int i = 0; i < KEYS; ++i) {
+            const int s = wave_first + i * 16 + column, row = begin + half * 32 + 4 * group;
+            const int64_t end = s >= behind ? 0 : s < a.sinks ? to : min<int64_t>(to, int64_t{s} + a.window);
+            const int first_seen = s - row, last_seen = static_cast<int>(end) - 1 - row;
+#pragma unroll
+            for (int k = 0; k < 2; ++k)
 #pragma unroll
               for (int r = 0; r < 4; ++r) {
-                const bool seen = (r >= first_seen) & (r <= last_seen);
+                const bool seen = (k * 16 + r >= first_seen) & (k * 16 + r <= last_seen);
                 weight[i][k][r] = seen ? weight[i][k][r] : 0.0f;
                 slope[i][k][r] = seen ? slope[i][k][r] : 0.0f;
               }
-            }
           }
         }
         Frag<T> weights[KEYS], slopes[KEYS];
@@ -627,26 +684,170 @@ window_grad_key_kernel(WindowArgs<T> a) {
     const int s = wave_first + i * 16 + column;
     if (s >= behind) continue;
     const float back = unit[i] == 0.0f ? 1.0f : 1.0f / unit[i];
-    if constexpr (SINKS) {
-      float* piece = a.sink_sums + ((slot * a.kv_heads + kv_head) * a.sinks + s) * sums;
+    const int64_t row = (run.first + s) * a.kv_heads + kv_head;
 #pragma unroll
-      for (int d = 0; d < kCols; ++d) {
-        store4(piece, d * 16 + 4 * group, grad_key[i][d] * back, a.key_width, false);
-        store4(piece + a.key_width, d * 16 + 4 * group, grad_value[i][d], a.value_width, false);
-      }
-    } else {
-      const int64_t row = (run.first + s) * a.kv_heads + kv_head;
-#pragma unroll
-      for (int d = 0; d < kCols; ++d) {
-        if (a.grad_key != nullptr)
-          store4(a.grad_key + row * a.key_width, d * 16 + 4 * group, grad_key[i][d] * (a.scale * back * kUnlift<T>),
-                 a.key_width, a.key_width % 4 == 0);
-        if (a.grad_value != nullptr)
-          store4(a.grad_value + row * a.value_width, d * 16 + 4 * group, grad_value[i][d] * kUnlift<T>,
-                 a.value_width, a.value_width % 4 == 0);
-      }
+    for (int d = 0; d < kCols; ++d) {
+      if (a.grad_key != nullptr)
+        store4(a.grad_key + row * a.key_width, d * 16 + 4 * group,
+               grad_key[i][d] * (a.scale * back * kUnlift<T>), a.key_width, WHOLE || a.key_width % 4 == 0);
+      if (a.grad_value != nullptr)
+        store4(a.grad_value + row * a.value_width, d * 16 + 4 * group, grad_value[i][d] * kUnlift<T>,
+               a.value_width, WHOLE || a.value_width % 4 == 0);
     }
   }
+}
+
+// The gradients of the sinks from the tokens beyond the first block's walk: every block takes a
+// piece of kSinkRows tokens of one query head and 16 sinks, every wave 32 tokens of a tile.  (One
+// block walking all of them would be the last to finish by far.)
+template <typename T, int WIDTH, bool WHOLE>
+__global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(1))) void
+window_grad_sinks_kernel(WindowArgs<T> a) {
+  constexpr int kSteps = WIDTH / 32, kCols = WIDTH / 16;
+  constexpr int kRows = sizeof(T) == 4 ? 64 : 128, kTeams = kRows / 32;  // waves with tokens
+  constexpr int kSumPitch = WIDTH + 4;
+  constexpr size_t kTileBytes = sizeof(T) * kRows * kPitch<T, WIDTH>;
+  static_assert(2 * kTileBytes >= sizeof(float) * kTeams * 2 * 16 * kSumPitch, "sums lie over the tiles");
+  __shared__ __attribute__((aligned(16))) char shared[2 * kTileBytes];
+  __shared__ __attribute__((aligned(16))) float log_sums[kRows], deltas[kRows];
+  T* queries = reinterpret_cast<T*>(shared);
+  T* grads = reinterpret_cast<T*>(shared + kTileBytes);
+
+  const int64_t item = item_of_block(a.items);
+  if (item >= a.items) return;
+  const int tid = threadIdx.x, lane = tid & 63, group = lane >> 4, column = lane & 15;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int parts = (a.sinks + 15) / 16;
+  const int first = static_cast<int>(item % parts) * 16;
+  const int head = static_cast<int>(item / parts % a.heads), kv_head = head / a.share;
+  const int64_t slot = item / parts / a.heads;
+  Run run;
+  if (find_run(a.sequences, slot, kSinkRows, tid, &run) != Found::kRun) return;
+  const int from = static_cast<int>(
+      max<int64_t>(run.tile * kSinkRows, min<int64_t>(run.length, walk_end(0, a.key_block, a.window))));
+  const int to = min(run.length, (run.tile + 1) * kSinkRows);
+  if (from >= to) return;  // (nor are its sums read)
+
+  // these tokens see all sinks
+  Frag<T> key[kSteps], value[kSteps];
+  f32x4 grad_key[kCols], grad_value[kCols];
+  const Rows<T> key_rows = a.key.rows(run.batch, run.begin + first, kv_head, a.sinks - first);
+  const Rows<T> value_rows = a.value.rows(run.batch, run.begin + first, kv_head, a.sinks - first);
+#pragma unroll
+  for (int step = 0; step < kSteps; ++step) {
+    key[step] = memory_operand<WHOLE>(key_rows, column, step * 32 + 8 * group, a.key_width);
+    value[step] = memory_operand<WHOLE>(value_rows, column, step * 32 + 8 * group, a.value_width);
+    clear_operand<WHOLE>(key[step], step * 32 + 8 * group, a.key_width);
+    clear_operand<WHOLE>(value[step], step * 32 + 8 * group, a.value_width);
+  }
+#pragma unroll
+  for (int d = 0; d < kCols; ++d) grad_key[d] = grad_value[d] = f32x4(0.0f);
+  float unit = kNarrow<T> ? 0.0f : 1.0f;
+  const float factor = a.scale * kLog2e;
+
+  TileMove<T, kRows, WIDTH, WHOLE> query_move, grad_move;
+  for (int begin = from; begin < to; begin += kRows) {
+    const int count = min(kRows, to - begin);
+    query_move.fetch(a.query.rows(run.batch, run.begin + begin, head, count), a.key_width, tid);
+    grad_move.fetch(a.grad_output.rows(run.batch, run.begin + begin, head, count), a.value_width, tid);
+    __syncthreads();
+    if (tid < kRows) {
+      const int64_t at =
+          static_cast<int64_t>(head) * a.sequences.tokens + run.first + begin + min(tid, count - 1);
+      log_sums[tid] = a.log_sum[at] - kLift<T>;
+      deltas[tid] = a.delta[at];
+    }
+    query_move.store(queries, a.key_width, tid);
+    grad_move.store(grads, a.value_width, tid);
+    __syncthreads();
+    const int row0 = wave * 32;
+    if (wave >= kTeams || row0 >= count) continue;
+    f32x4 weight[2], slope[2];
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+      weight[k] = slope[k] = f32x4(0.0f);
+#pragma unroll
+      for (int s = 0; s < kSteps; ++s) {
+        weight[k] = mma(row_operand<T, WIDTH>(queries, row0 + k * 16, s * 32, lane), key[s], weight[k]);
+        slope[k] = mma(row_operand<T, WIDTH>(grads, row0 + k * 16, s * 32, lane), value[s], slope[k]);
+      }
+      const int row = row0 + k * 16 + 4 * group;
+      const f32x4 log_sum = *reinterpret_cast<const f32x4*>(log_sums + row);
+      const f32x4 delta = *reinterpret_cast<const f32x4*>(deltas + row);
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        const bool there = row + r < count;
+        weight[k][r] = there ? exp2_of(weight[k][r] * factor - log_sum[r]) : 0.0f;
+        slope[k][r] = there ? weight[k][r] * (slope[k][r] - delta[r]) : 0.0f;
+      }
+    }
+    if constexpr (kNarrow<T>) {
+      float most = 0.0f;
+#pragma unroll
+      for (int k = 0; k < 2; ++k)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) most = fmaxf(most, fabsf(slope[k][r]));
+      const float by = follow_range(&unit, over_groups_max(most));
+#pragma unroll
+      for (int d = 0; d < kCols; ++d) grad_key[d] *= by;
+      slope[0] *= unit;
+      slope[1] *= unit;
+    }
+    const Frag<T> weights = operand_of<T>(weight[0], weight[1]), slopes = operand_of<T>(slope[0], slope[1]);
+#pragma unroll
+    for (int d = 0; d < kCols; ++d) {
+      grad_value[d] = mma(column_operand<T, WIDTH>(grads, row0, d * 16, lane), weights, grad_value[d]);
+      grad_key[d] = mma(column_operand<T, WIDTH>(queries, row0, d * 16, lane), slopes, grad_key[d]);
+    }
+  }
+
+  // the waves' sums, in their order
+  __syncthreads();
+  float* sums = reinterpret_cast<float*>(shared);
+  const float back = unit == 0.0f ? 1.0f : 1.0f / unit;
+  if (wave < kTeams) {
+#pragma unroll
+    for (int d = 0; d < kCols; ++d) {
+      float* at = sums + (wave * 32 + column) * kSumPitch + d * 16 + 4 * group;
+      *reinterpret_cast<f32x4*>(at) = grad_key[d] * back;
+      *reinterpret_cast<f32x4*>(at + 16 * kSumPitch) = grad_value[d];
+    }
+  }
+  __syncthreads();
+  const int columns = a.key_width + a.value_width, there = min(16, a.sinks - first);
+  float* piece = a.sink_parts + ((slot * a.heads + head) * a.sinks + first) * columns;
+  for (int e = tid; e < there * columns; e += kThreads) {
+    const int s = e / columns, col = e % columns;
+    const int at = col < a.key_width ? s * kSumPitch + col : (16 + s) * kSumPitch + col - a.key_width;
+    float sum = 0.0f;
+#pragma unroll
+    for (int w = 0; w < kTeams; ++w) sum += sums[w * 32 * kSumPitch + at];
+    piece[e] = sum;
+  }
+}
+
+// The pieces of window_grad_sinks_kernel, and the query heads of a group, added up in their order:
+// [sequence][kv head][sink][key_width + value_width].
+template <typename T>
+__global__ __launch_bounds__(kThreads) void window_join_sinks_kernel(WindowArgs<T> a) {
+  const int tid = threadIdx.x, size = a.sinks * (a.key_width + a.value_width);
+  const int blocks = (size + kThreads - 1) / kThreads;
+  const int sequence = static_cast<int>(blockIdx.x / blocks / a.kv_heads);
+  const int kv_head = static_cast<int>(blockIdx.x / blocks % a.kv_heads);
+  const Run run = run_of_sequence(a.sequences, sequence, tid);
+  if (run.length < 0) return;
+  const int e = static_cast<int>(blockIdx.x % blocks) * kThreads + tid;
+  if (e >= size) return;
+  const int64_t begin = walk_end(0, a.key_block, a.window);
+  if (begin >= run.length) return;
+  const int first = static_cast<int>(begin) / kSinkRows, pieces = (run.length + kSinkRows - 1) / kSinkRows;
+  const int64_t slot = first_slot(a.sequences, run, kSinkRows) + first;
+  const float* part = a.sink_parts + (slot * a.heads + kv_head * a.share) * size + e;
+  float sum = 0.0f;
+#pragma unroll 4
+  for (int i = 0; i < (pieces - first) * a.share; ++i)
+    sum += part[(static_cast<int64_t>(i / a.share) * a.heads + i % a.share) * size];
+  a.sink_sums[(static_cast<int64_t>(sequence) * a.kv_heads + kv_head) * size + e] = sum;
 }
 
 // ---------------------------------------------------------------------------
@@ -664,9 +865,11 @@ __global__ __launch_bounds__(kThreads) void window_append_kernel(WindowArgs<T> a
   Run run;
   if (find_run(a.sequences, slot, 64, tid, &run) != Found::kRun) return;
   const int past = tokens_before<true>(a, run);
-  const KeyRows<T, true> rows = key_rows<true>(a, run, kv_head, past);
+  const History<T, true> key_rows = history_of<true>(a, a.key, a.key_cache, a.key_width, run, kv_head, past);
+  const History<T, true> value_rows =
+      history_of<true>(a, a.value, a.value_cache, a.value_width, run, kv_head, past);
   const int begin = past + run.tile * 64, end = min(begin + 64, past + run.length);
-  const int64_t oldest = static_cast<int64_t>(past) + run.length - rows.rows.ring;
+  const int64_t oldest = static_cast<int64_t>(past) + run.length - key_rows.rows.ring;
   const int64_t at = (static_cast<int64_t>(run.sequence) * a.kv_heads + kv_head) * a.capacity;
   const auto copy = [&](T* cache, int width, auto&& from) {
     constexpr int kElements = 16 / static_cast<int>(sizeof(T));
@@ -675,7 +878,7 @@ __global__ __launch_bounds__(kThreads) void window_append_kernel(WindowArgs<T> a
     for (int e = tid; e < (end - begin) * pieces; e += kThreads) {
       const int s = begin + e / pieces, col = e % pieces * kElements;
       if (s >= a.sinks && s < oldest) continue;
-      T* to = cache + (at + rows.rows.row(s)) * width + col;
+      T* to = cache + (at + key_rows.rows.row(s)) * width + col;
       const T* source = from(s) + col;
       if constexpr (WHOLE)
         *reinterpret_cast<Piece*>(to) = *reinterpret_cast<const Piece*>(source);
@@ -683,8 +886,8 @@ __global__ __launch_bounds__(kThreads) void window_append_kernel(WindowArgs<T> a
         for (int i = 0; i < kElements && col + i < width; ++i) to[i] = source[i];
     }
   };
-  copy(key_cache, a.key_width, [&](int s) { return rows.key_row(s); });
-  copy(value_cache, a.value_width, [&](int s) { return rows.value_row(s); });
+  copy(key_cache, a.key_width, [&](int s) { return key_rows.row(s); });
+  copy(value_cache, a.value_width, [&](int s) { return value_rows.row(s); });
 }
 
 // One new token of every slot against its cache, which is shared out to the blocks of a head of
@@ -721,13 +924,15 @@ window_token_kernel(TokenArgs<T> args) {
   const int slot = blockIdx.x / args.splits / args.head_blocks / a.kv_heads;
   const Run run{slot, 1, 0, slot, 0, slot};
   const int past = tokens_before<true>(a, run);
-  const KeyRows<T, true> rows = key_rows<true>(a, run, kv_head, past);
+  const History<T, true> key_rows = history_of<true>(a, a.key, a.key_cache, a.key_width, run, kv_head, past);
+  const History<T, true> value_rows =
+      history_of<true>(a, a.value, a.value_cache, a.value_width, run, kv_head, past);
 
   if (split == 0 && head_block == 0) {  // (the row that it takes is one that nobody sees any more)
-    const int64_t at = (static_cast<int64_t>(slot) * a.kv_heads + kv_head) * a.capacity + rows.rows.row(past);
-    for (int d = tid; d < a.key_width; d += kThreads) args.key_cache[at * a.key_width + d] = rows.key[d];
+    const int64_t at = (static_cast<int64_t>(slot) * a.kv_heads + kv_head) * a.capacity + key_rows.rows.row(past);
+    for (int d = tid; d < a.key_width; d += kThreads) args.key_cache[at * a.key_width + d] = key_rows.fresh[d];
     for (int d = tid; d < a.value_width; d += kThreads)
-      args.value_cache[at * a.value_width + d] = rows.value[d];
+      args.value_cache[at * a.value_width + d] = value_rows.fresh[d];
   }
   // what the token sees, in order: sinks, window, itself
   const int window_begin = max(0, past - a.window + 1), sinks_end = min(a.sinks, window_begin);
@@ -739,11 +944,13 @@ window_token_kernel(TokenArgs<T> args) {
 
   // this column's member of the group of query heads (the last one again beyond it)
   const int head = kv_head * a.share + min(head_block * 16 + column, a.share - 1);
-  const T* query_row = a.query.row(slot, 0, head);
+  const Rows<T> query_row = {a.query.row(slot, 0, head), 0, 0};
   Frag<T> query[kSteps];
 #pragma unroll
-  for (int s = 0; s < kSteps; ++s)
-    query[s] = memory_operand<WHOLE>(query_row, s * 32 + 8 * group, a.key_width);
+  for (int s = 0; s < kSteps; ++s) {
+    query[s] = memory_operand<WHOLE>(query_row, 0, s * 32 + 8 * group, a.key_width);
+    clear_operand<WHOLE>(query[s], s * 32 + 8 * group, a.key_width);
+  }
   f32x4 out[kCols];
 #pragma unroll
   for (int d = 0; d < kCols; ++d) out[d] = f32x4(0.0f);
@@ -755,15 +962,15 @@ window_token_kernel(TokenArgs<T> args) {
   const auto fetch = [&](int tile) {
 #pragma unroll
     for (int k = 0; k < 2; ++k) {
-      const T* row = rows.key_row(position(min(tile * kTile + k * 16 + column, seen - 1)));
+      const Rows<T> row = {key_rows.row(position(min(tile * kTile + k * 16 + column, seen - 1))), 0, 0};
 #pragma unroll
       for (int s = 0; s < kSteps; ++s)
-        key[k][s] = memory_operand<WHOLE>(row, s * 32 + 8 * group, a.key_width);
+        key[k][s] = memory_operand<WHOLE>(row, 0, s * 32 + 8 * group, a.key_width);
     }
 #pragma unroll
     for (int i = 0; i < kPieces; ++i) {
       const int piece = i * 64 + lane, col = piece % kPerRow * kElements;
-      const T* row = rows.value_row(position(min(tile * kTile + piece / kPerRow, seen - 1)));
+      const T* row = value_rows.row(position(min(tile * kTile + piece / kPerRow, seen - 1)));
       if constexpr (WHOLE) {
         held[i] = *reinterpret_cast<const Piece*>(row + min(col, a.value_width - kElements));
       } else {
@@ -780,7 +987,10 @@ window_token_kernel(TokenArgs<T> args) {
     for (int k = 0; k < 2; ++k) {
       score[k] = f32x4(0.0f);
 #pragma unroll
-      for (int s = 0; s < kSteps; ++s) score[k] = mma(key[k][s], query[s], score[k]);
+      for (int s = 0; s < kSteps; ++s) {
+        clear_operand<WHOLE>(key[k][s], s * 32 + 8 * group, a.key_width);
+        score[k] = mma(key[k][s], query[s], score[k]);
+      }
     }
     // (LDS accesses of one wave are carried out in order: its tile needs no barrier)
 #pragma unroll
@@ -983,13 +1193,17 @@ void window_backward_launch(WindowArgs<T>& args, hipStream_t stream) {
   if (args.grad_key == nullptr && args.grad_value == nullptr) return;
   args.key_block = 64 * kWaveKeys;
   if (args.sink_slots > 0) {
-    args.items = args.sink_slots * args.kv_heads;
-    window_grad_key_kernel<T, WIDTH, 1, true, WHOLE>  // (64 keys hold all sinks)
+    args.items = args.sink_slots * args.heads * ((args.sinks + 15) / 16);
+    window_grad_sinks_kernel<T, WIDTH, WHOLE>
         <<<dim3(static_cast<unsigned>(grid_of(args.items))), kThreads, 0, stream>>>(args);
+    const int size = args.sinks * (args.key_width + args.value_width);
+    window_join_sinks_kernel<T>
+        <<<dim3(static_cast<unsigned>((size + kThreads - 1) / kThreads * args.kv_heads * args.sequences.count)),
+           kThreads, 0, stream>>>(args);
   }
   args.slots = slots_of(args.sequences, 64 * kWaveKeys);
   args.items = args.slots * args.kv_heads;
-  window_grad_key_kernel<T, WIDTH, kWaveKeys, false, WHOLE>
+  window_grad_key_kernel<T, WIDTH, kWaveKeys, WHOLE>
       <<<dim3(static_cast<unsigned>(grid_of(args.items))), kThreads, 0, stream>>>(args);
 }
 
@@ -1005,8 +1219,10 @@ void window_backward_width(const WindowCall& call) {
   args.grad_key = static_cast<T*>(call.grad_key);
   args.grad_value = static_cast<T*>(call.grad_value);
   args.sink_slots = plan.sink_slots;
-  args.sink_sums =
-      plan.sink_slots > 0 ? reinterpret_cast<float*>(call.workspace + plan.delta_bytes) : nullptr;
+  if (plan.sink_slots > 0) {
+    args.sink_sums = reinterpret_cast<float*>(call.workspace + plan.delta_bytes);
+    args.sink_parts = reinterpret_cast<float*>(call.workspace + plan.delta_bytes + plan.sink_bytes);
+  }
   switch (padded_width(p.D > p.Dv ? p.D : p.Dv)) {
     case 32: return window_backward_launch<T, 32, WHOLE>(args, call.stream);
     case 64: return window_backward_launch<T, 64, WHOLE>(args, call.stream);

@@ -1,12 +1,14 @@
 // Dispatcher layer of the mixers (module rosa_soft_amd._C, beside rosa_dispatch.cpp): schemas,
 // validation, allocation and stream of decayed linear attention and window attention.  Inputs are
 // taken with their strides as long as the elements of a head are neighbours; outputs are
-// contiguous and of the inputs' dtype.  No device code lives in this file.
+// contiguous and of the inputs' dtype.  All checks are made here, whatever the inputs' device, so
+// that a call costs the interpreter nothing but the call; the autograd nodes are here as well, so
+// that a backward does not wait for the interpreter.  No device code lives in this file.
 
 #include <ATen/Context.h>
-#include <ATen/MemoryOverlap.h>
 #include <ATen/hip/impl/HIPGuardImplMasqueradingAsCUDA.h>
 #include <ATen/hip/impl/HIPStreamMasqueradingAsCUDA.h>
+#include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/extension.h>
 
 #include <hip/hip_runtime_api.h>
@@ -46,15 +48,22 @@ void raise_on_failure(int status, const char* what) {
   TORCH_CHECK(status == 0, what, " failed (", status, "): ", rosa_hip_last_error());
 }
 
-// The backward of this build is not recorded into HIP graphs, however it is reached.
-void refuse_capture(const char* what) {
+bool is_capturing(const Tensor& on) {
+  // (tracing: nothing is being launched)
+  if (!on.is_cuda() || on.key_set().has(c10::DispatchKey::Python)) return false;
+  const Guard guard(on.device());
   hipStreamCaptureStatus capture = hipStreamCaptureStatusNone;
   const hipError_t queried = hipStreamIsCapturing(
       c10::hip::getCurrentHIPStreamMasqueradingAsCUDA().stream(), &capture);
-  TORCH_CHECK(queried == hipSuccess, what, ": hipStreamIsCapturing failed: ",
-              hipGetErrorString(queried));
-  TORCH_CHECK(capture == hipStreamCaptureStatusNone, what,
-              ": the backward cannot be recorded into a HIP graph in this build; run it eagerly");
+  TORCH_CHECK(queried == hipSuccess, "hipStreamIsCapturing failed: ", hipGetErrorString(queried));
+  return capture != hipStreamCaptureStatusNone;
+}
+
+// The backward of this build is not recorded into HIP graphs, however it is reached.
+void refuse_capture(const char* what, const Tensor& on) {
+  TORCH_CHECK(!is_capturing(on), what,
+              ": the backward cannot be recorded into a HIP graph in this build; capture the "
+              "forward under torch.no_grad() or run the training step eagerly");
 }
 
 // elements of a head next to each other; everything else by strides
@@ -75,46 +84,64 @@ struct Call {
   rosa_mixer_tensor q, k, v;
 };
 
-void check_call(const Tensor& query, const Tensor& key, const Tensor& value,
-                const OptionalTensor& cu_seqlens, double scale) {
+#define REQUIRE TORCH_CHECK_VALUE
+
+// Shapes, dtypes, devices and scale; returns the scale.  `empty`: calls without tokens are meant.
+double check_call(const Tensor& query, const Tensor& key, const Tensor& value,
+                  const OptionalTensor& cu_seqlens, const std::optional<double>& scale, bool empty) {
   const int64_t rank = cu_seqlens ? 3 : 4;
-  TORCH_CHECK(query.is_cuda() && key.is_cuda() && value.is_cuda(),
-              "query, key and value must be CUDA tensors");
-  TORCH_CHECK(query.device() == key.device() && query.device() == value.device(),
-              "query, key and value must be on the same CUDA device");
-  TORCH_CHECK(dtype_code(query.scalar_type()) >= 0,
-              "query must be float32, float16, or bfloat16");
-  TORCH_CHECK(query.scalar_type() == key.scalar_type() &&
-                  query.scalar_type() == value.scalar_type(),
-              "query, key and value must have the same dtype");
-  TORCH_CHECK(query.dim() == rank && key.dim() == rank && value.dim() == rank,
-              "query, key and value must have shape ",
-              cu_seqlens ? "(N, heads, width)" : "(B, T, heads, width)");
-  for (int64_t axis = 0; axis + 2 < rank; ++axis)
-    TORCH_CHECK(query.size(axis) == key.size(axis) && query.size(axis) == value.size(axis),
-                "query, key and value must share their token dimensions");
-  TORCH_CHECK(key.size(-2) == value.size(-2), "key and value head counts must match");
-  TORCH_CHECK(key.size(-2) > 0 && query.size(-2) > 0 && query.size(-2) % key.size(-2) == 0,
-              "query heads must be a positive multiple of key heads");
-  TORCH_CHECK(query.size(-1) == key.size(-1), "query and key widths must match");
-  TORCH_CHECK(query.size(-1) >= 1 && query.size(-1) <= kMostWidth && value.size(-1) >= 1 &&
-                  value.size(-1) <= kMostWidth,
-              "head widths must be in [1, 128]");
-  const int64_t tokens = query.numel() / (query.size(-2) * query.size(-1));
-  TORCH_CHECK(tokens <= kIntMax && tokens * query.size(-2) <= kIntMax,
-              "tokens times heads must fit in int32");
-  const float narrowed = static_cast<float>(scale);
-  TORCH_CHECK(std::isnormal(narrowed) && narrowed > 0.0f,
-              "scale must be representable as a positive normal float32 value");
-  if (cu_seqlens) {
-    TORCH_CHECK(cu_seqlens->is_cuda() && cu_seqlens->device() == query.device(),
-                "cu_seqlens must be on the CUDA device of the inputs");
-    TORCH_CHECK(cu_seqlens->scalar_type() == torch::kInt32, "cu_seqlens must be int32");
-    TORCH_CHECK(cu_seqlens->dim() == 1 && cu_seqlens->numel() >= 2,
-                "cu_seqlens must be one-dimensional with at least two entries");
-    TORCH_CHECK(cu_seqlens->numel() - 1 <= kIntMax, "too many packed sequences");
+  REQUIRE(query.dim() == rank && key.dim() == rank && value.dim() == rank,
+          "query, key, and value must have shape ",
+          cu_seqlens ? "(N, heads, width)" : "(B, T, heads, width)");
+  int64_t tokens = 1;
+  for (int64_t axis = 0; axis + 2 < rank; ++axis) {
+    REQUIRE(query.size(axis) == key.size(axis) && query.size(axis) == value.size(axis),
+            "all inputs must share their token dimensions");
+    tokens *= query.size(axis);
   }
+  const int64_t heads = query.size(-2), shared = key.size(-2), width = query.size(-1);
+  REQUIRE(shared == value.size(-2), "key and value head counts must match");
+  REQUIRE(heads >= 1 && shared >= 1, "query and key must have at least one head");
+  REQUIRE(heads % shared == 0, "query heads must be divisible by key heads");
+  REQUIRE(width == key.size(-1), "query and key widths must match");
+  REQUIRE(width >= 1 && width <= kMostWidth && value.size(-1) >= 1 && value.size(-1) <= kMostWidth,
+          "head widths must be in [1, 128]");
+  REQUIRE(empty || tokens >= 1, "batch and sequence dimensions must be >= 1");
+  REQUIRE(tokens <= kIntMax && tokens * heads <= kIntMax, "tokens times heads must fit in int32");
+  REQUIRE(query.device() == key.device() && query.device() == value.device(),
+          "all inputs must be on the same device");
+  REQUIRE(query.scalar_type() == key.scalar_type() && query.scalar_type() == value.scalar_type(),
+          "all inputs must have the same dtype");
+  REQUIRE(dtype_code(query.scalar_type()) >= 0, "the mixers support float32, float16, and bfloat16");
+  if (cu_seqlens) {
+    REQUIRE(cu_seqlens->device() == query.device(),
+            "all inputs and cu_seqlens must be on the same device");
+    REQUIRE(cu_seqlens->scalar_type() == torch::kInt32, "cu_seqlens must have dtype int32");
+    REQUIRE(cu_seqlens->dim() == 1 && cu_seqlens->numel() >= 2,
+            "cu_seqlens must be a one-dimensional int32 tensor");
+    REQUIRE(cu_seqlens->numel() - 1 <= kIntMax, "too many packed sequences");
+  }
+  const double given = scale ? *scale : 1.0 / std::sqrt(static_cast<double>(width));
+  const float narrowed = static_cast<float>(given);
+  REQUIRE(std::isnormal(narrowed) && narrowed > 0.0f,
+          "scale must be representable as a positive normal float32 value");
+  return given;
 }
+
+// Whether the spans of memory that two tensors' elements lie in meet.
+bool overlap(const Tensor& a, const Tensor& b) {
+  if (a.numel() == 0 || b.numel() == 0) return false;
+  const auto end = [](const Tensor& t) {
+    int64_t last = 0;
+    for (int64_t axis = 0; axis < t.dim(); ++axis) last += (t.size(axis) - 1) * t.stride(axis);
+    return reinterpret_cast<uintptr_t>(t.const_data_ptr()) + (last + 1) * t.element_size();
+  };
+  return reinterpret_cast<uintptr_t>(a.const_data_ptr()) < end(b) &&
+         reinterpret_cast<uintptr_t>(b.const_data_ptr()) < end(a);
+}
+
+// (after every other check)
+void check_device(const Tensor& query) { REQUIRE(query.is_cuda(), "the mixers require CUDA tensors"); }
 
 Call make_call(const Tensor& query, const Tensor& key, const Tensor& value,
                const OptionalTensor& cu_seqlens, double scale) {
@@ -157,38 +184,33 @@ Tensor new_workspace(size_t bytes, const Tensor& like) {
   return torch::empty({static_cast<int64_t>(bytes)}, like.options().dtype(torch::kUInt8));
 }
 
-Tensor check_log_decay(const Tensor& log_decay, const Tensor& query) {
-  TORCH_CHECK(log_decay.is_cuda() && log_decay.device() == query.device(),
-              "log_decay must be on the CUDA device of the inputs");
-  TORCH_CHECK(log_decay.scalar_type() == torch::kFloat32, "log_decay must be float32");
-  TORCH_CHECK(log_decay.dim() == 1 && log_decay.size(0) == query.size(-2),
-              "log_decay must have one entry per query head");
-  return log_decay.contiguous();
+void check_log_decay(const Tensor& log_decay, const Tensor& query) {
+  REQUIRE(log_decay.dim() == 1 && log_decay.size(0) == query.size(-2),
+          "log_decay must have one entry per query head");
+  REQUIRE(log_decay.scalar_type() == torch::kFloat32, "log_decay must have dtype float32");
+  REQUIRE(log_decay.device() == query.device(),
+          "all inputs and log_decay must be on the same device");
 }
 
 void check_grad_output(const Tensor& grad_output, const Tensor& query, const Tensor& value) {
   auto sizes = query.sizes().vec();
   sizes.back() = value.size(-1);
-  TORCH_CHECK(grad_output.device() == query.device(),
-              "grad_output must be on the CUDA device of the inputs");
-  TORCH_CHECK(grad_output.scalar_type() == query.scalar_type(), "grad_output dtype mismatch");
-  TORCH_CHECK(grad_output.sizes() == torch::IntArrayRef(sizes), "grad_output shape mismatch");
-}
-
-void check_training(const Tensor& query) {
-  TORCH_CHECK(query.numel() > 0, "batch and sequence dimensions must be >= 1");
+  REQUIRE(grad_output.device() == query.device(),
+          "grad_output must be on the device of the inputs");
+  REQUIRE(grad_output.scalar_type() == query.scalar_type(), "grad_output dtype mismatch");
+  REQUIRE(grad_output.sizes() == torch::IntArrayRef(sizes), "grad_output shape mismatch");
 }
 
 void check_window(int64_t window, int64_t sinks) {
-  TORCH_CHECK(window >= 1, "window must be >= 1");
-  TORCH_CHECK(sinks >= 0 && sinks <= kMostSinks, "sinks must be in [0, 64]");
+  REQUIRE(window >= 1, "window must be >= 1");
+  REQUIRE(sinks >= 0 && sinks <= kMostSinks, "sinks must be in [0, 64]");
 }
 
 int narrow_window(int64_t window) { return static_cast<int>(std::min(window, kIntMax)); }
 
 void check_mask(int64_t gradient_mask) {
-  TORCH_CHECK(gradient_mask >= 1 && gradient_mask <= 7,
-              "gradient_mask must be an integer bit mask in [1, 7]");
+  REQUIRE(gradient_mask >= 1 && gradient_mask <= 7,
+          "gradient_mask must be an integer bit mask in [1, 7]");
 }
 
 // the requested gradients, each in the layout and dtype of its input
@@ -212,13 +234,17 @@ struct Gradients {
 // decayed linear attention
 // ---------------------------------------------------------------------------
 
+using Scale = std::optional<double>;
+using Triple = std::tuple<Tensor, Tensor, Tensor>;
+
 Tensor decay_attention_op(const Tensor& query, const Tensor& key, const Tensor& value,
-                          const OptionalTensor& cu_seqlens, const Tensor& log_decay, double scale) {
-  check_call(query, key, value, cu_seqlens, scale);
-  check_training(query);
-  const Tensor rates = check_log_decay(log_decay, query);
+                          const OptionalTensor& cu_seqlens, const Tensor& log_decay, Scale scale) {
+  const double factor = check_call(query, key, value, cu_seqlens, scale, false);
+  check_log_decay(log_decay, query);
+  check_device(query);
   const Guard guard(query.device());
-  const Call call = make_call(query, key, value, cu_seqlens, scale);
+  const Tensor rates = log_decay.contiguous();
+  const Call call = make_call(query, key, value, cu_seqlens, factor);
   const Tensor output = new_output(call);
   const size_t bytes = rosa_hip_decay_workspace_bytes(&call.problem, 0);
   const Tensor workspace = new_workspace(bytes, query);
@@ -229,17 +255,18 @@ Tensor decay_attention_op(const Tensor& query, const Tensor& key, const Tensor& 
   return output;
 }
 
-std::tuple<Tensor, Tensor, Tensor> decay_attention_vjp_op(
-    const Tensor& query, const Tensor& key, const Tensor& value, const OptionalTensor& cu_seqlens,
-    const Tensor& log_decay, const Tensor& grad_output, double scale, int64_t gradient_mask) {
-  check_call(query, key, value, cu_seqlens, scale);
-  check_training(query);
-  const Tensor rates = check_log_decay(log_decay, query);
+Triple decay_attention_vjp_op(const Tensor& query, const Tensor& key, const Tensor& value,
+                              const OptionalTensor& cu_seqlens, const Tensor& log_decay,
+                              const Tensor& grad_output, Scale scale, int64_t gradient_mask) {
+  const double factor = check_call(query, key, value, cu_seqlens, scale, false);
+  check_log_decay(log_decay, query);
   check_grad_output(grad_output, query, value);
   check_mask(gradient_mask);
+  check_device(query);
   const Guard guard(query.device());
-  refuse_capture("decay_attention_vjp");
-  const Call call = make_call(query, key, value, cu_seqlens, scale);
+  refuse_capture("decay_attention_vjp", query);
+  const Tensor rates = log_decay.contiguous();
+  const Call call = make_call(query, key, value, cu_seqlens, factor);
   const Tensor grad = readable(grad_output);
   const rosa_mixer_tensor go = describe(grad);
   const Gradients gradients(call, gradient_mask);
@@ -255,34 +282,38 @@ std::tuple<Tensor, Tensor, Tensor> decay_attention_vjp_op(
   return {gradients.query, gradients.key, gradients.value};
 }
 
-int64_t slot_count(const Tensor& query, const OptionalTensor& cu_seqlens) {
-  return cu_seqlens ? cu_seqlens->numel() - 1 : query.size(0);
+int64_t check_slots(const Tensor& query, const OptionalTensor& cu_seqlens) {
+  const int64_t slots = cu_seqlens ? cu_seqlens->numel() - 1 : query.size(0);
+  REQUIRE(slots >= 1, "an update needs at least one slot");
+  return slots;
 }
 
 Tensor decay_attention_update_out_op(const Tensor& query, const Tensor& key, const Tensor& value,
                                      const OptionalTensor& cu_seqlens, const Tensor& log_decay,
-                                     const Tensor& state, Tensor state_out, double scale) {
-  check_call(query, key, value, cu_seqlens, scale);
-  const Tensor rates = check_log_decay(log_decay, query);
-  const int64_t slots = slot_count(query, cu_seqlens);
+                                     const Tensor& state, Tensor state_out, Scale scale) {
+  const double factor = check_call(query, key, value, cu_seqlens, scale, true);
+  check_log_decay(log_decay, query);
+  const int64_t slots = check_slots(query, cu_seqlens);
   for (const Tensor* tensor : {&state, const_cast<const Tensor*>(&state_out)}) {
-    TORCH_CHECK(tensor->device() == query.device(),
-                "state must be on the CUDA device of the inputs");
-    TORCH_CHECK(tensor->scalar_type() == torch::kFloat32, "state must be float32");
-    TORCH_CHECK(tensor->sizes() == torch::IntArrayRef({slots, query.size(-2), query.size(-1),
-                                                       value.size(-1)}),
-                "state must have shape (slots, heads, key width, value width)");
-    TORCH_CHECK(tensor->is_contiguous(), "state must be contiguous");
+    REQUIRE(tensor->sizes() ==
+                torch::IntArrayRef({slots, query.size(-2), query.size(-1), value.size(-1)}),
+            "state must have shape (slots, heads, key width, value width)");
+    REQUIRE(tensor->scalar_type() == torch::kFloat32, "state must have dtype float32");
+    REQUIRE(tensor->device() == query.device(), "all inputs and state must be on the same device");
+    REQUIRE(tensor->is_contiguous(), "state must be contiguous");
+    if (state_out.is_same(state)) break;
   }
-  TORCH_CHECK(slots >= 1, "an update needs at least one slot");
-  at::assert_no_partial_overlap(state_out, state);
+  REQUIRE(state_out.const_data_ptr() == state.const_data_ptr() || !overlap(state_out, state),
+          "state_out must be state or share no memory with it");
+  check_device(query);
   const Guard guard(query.device());
-  const Call call = make_call(query, key, value, cu_seqlens, scale);
+  const Call call = make_call(query, key, value, cu_seqlens, factor);
   const Tensor output = new_output(call);
   if (query.numel() == 0) {  // nobody brings a token
     if (!state_out.is_same(state)) state_out.copy_(state);
     return output;
   }
+  const Tensor rates = log_decay.contiguous();
   const size_t bytes = rosa_hip_decay_workspace_bytes(&call.problem, 2);
   const Tensor workspace = new_workspace(bytes, query);
   raise_on_failure(rosa_hip_decay_update(&call.problem, &call.q, &call.k, &call.v,
@@ -295,7 +326,7 @@ Tensor decay_attention_update_out_op(const Tensor& query, const Tensor& key, con
 
 Tensor decay_attention_update_op(const Tensor& query, const Tensor& key, const Tensor& value,
                                  const OptionalTensor& cu_seqlens, const Tensor& log_decay,
-                                 Tensor state, double scale) {
+                                 Tensor state, Scale scale) {
   return decay_attention_update_out_op(query, key, value, cu_seqlens, log_decay, state, state,
                                        scale);
 }
@@ -307,12 +338,12 @@ Tensor decay_attention_update_op(const Tensor& query, const Tensor& key, const T
 std::tuple<Tensor, Tensor> window_attention_op(const Tensor& query, const Tensor& key,
                                                const Tensor& value,
                                                const OptionalTensor& cu_seqlens, int64_t window,
-                                               int64_t sinks, double scale, bool want_log_sum) {
-  check_call(query, key, value, cu_seqlens, scale);
-  check_training(query);
+                                               int64_t sinks, Scale scale, bool want_log_sum) {
+  const double factor = check_call(query, key, value, cu_seqlens, scale, false);
   check_window(window, sinks);
+  check_device(query);
   const Guard guard(query.device());
-  const Call call = make_call(query, key, value, cu_seqlens, scale);
+  const Call call = make_call(query, key, value, cu_seqlens, factor);
   const Tensor output = new_output(call);
   const auto options = query.options().dtype(torch::kFloat32);
   const Tensor log_sum = want_log_sum ? torch::empty({call.problem.H, call.problem.N}, options)
@@ -326,26 +357,26 @@ std::tuple<Tensor, Tensor> window_attention_op(const Tensor& query, const Tensor
   return {output, log_sum};
 }
 
-std::tuple<Tensor, Tensor, Tensor> window_attention_vjp_op(
-    const Tensor& query, const Tensor& key, const Tensor& value, const OptionalTensor& cu_seqlens,
-    const Tensor& output, const Tensor& log_sum, const Tensor& grad_output, int64_t window,
-    int64_t sinks, double scale, int64_t gradient_mask) {
-  check_call(query, key, value, cu_seqlens, scale);
-  check_training(query);
+Triple window_attention_vjp_op(const Tensor& query, const Tensor& key, const Tensor& value,
+                               const OptionalTensor& cu_seqlens, const Tensor& output,
+                               const Tensor& log_sum, const Tensor& grad_output, int64_t window,
+                               int64_t sinks, Scale scale, int64_t gradient_mask) {
+  const double factor = check_call(query, key, value, cu_seqlens, scale, false);
   check_window(window, sinks);
   check_grad_output(grad_output, query, value);
   check_mask(gradient_mask);
-  TORCH_CHECK(output.device() == query.device() && output.scalar_type() == query.scalar_type() &&
-                  output.sizes() == grad_output.sizes(),
-              "output must be the forward's");
-  TORCH_CHECK(log_sum.device() == query.device() && log_sum.scalar_type() == torch::kFloat32 &&
-                  log_sum.sizes() == torch::IntArrayRef({query.size(-2),
-                                                         query.numel() / (query.size(-2) *
-                                                                          query.size(-1))}),
-              "log_sum must be the forward's");
+  REQUIRE(output.device() == query.device() && output.scalar_type() == query.scalar_type() &&
+              output.sizes() == grad_output.sizes(),
+          "output must be the forward's");
+  REQUIRE(log_sum.device() == query.device() && log_sum.scalar_type() == torch::kFloat32 &&
+              log_sum.sizes() == torch::IntArrayRef({query.size(-2),
+                                                     query.numel() / (query.size(-2) *
+                                                                      query.size(-1))}),
+          "log_sum must be the forward's");
+  check_device(query);
   const Guard guard(query.device());
-  refuse_capture("window_attention_vjp");
-  const Call call = make_call(query, key, value, cu_seqlens, scale);
+  refuse_capture("window_attention_vjp", query);
+  const Call call = make_call(query, key, value, cu_seqlens, factor);
   const Tensor grad = readable(grad_output);
   const Tensor out = output.contiguous(), sums = log_sum.contiguous();
   const rosa_mixer_tensor go = describe(grad);
@@ -367,37 +398,35 @@ std::tuple<Tensor, Tensor, Tensor> window_attention_vjp_op(
 Tensor window_attention_update_op(const Tensor& query, const Tensor& key, const Tensor& value,
                                   Tensor key_cache, Tensor value_cache, const Tensor& lengths,
                                   const OptionalTensor& cu_seqlens, int64_t window, int64_t sinks,
-                                  double scale) {
-  check_call(query, key, value, cu_seqlens, scale);
+                                  Scale scale) {
+  const double factor = check_call(query, key, value, cu_seqlens, scale, true);
   check_window(window, sinks);
-  const int64_t slots = slot_count(query, cu_seqlens);
-  TORCH_CHECK(slots >= 1, "an update needs at least one slot");
-  TORCH_CHECK(key_cache.dim() == 4 && value_cache.dim() == 4,
-              "caches must have shape (slots, key heads, capacity, width)");
+  const int64_t slots = check_slots(query, cu_seqlens);
+  REQUIRE(key_cache.dim() == 4 && value_cache.dim() == 4,
+          "caches must have shape (slots, key heads, capacity, width)");
   const int64_t capacity = key_cache.size(2);
-  TORCH_CHECK(key_cache.sizes() ==
-                      torch::IntArrayRef({slots, key.size(-2), capacity, key.size(-1)}) &&
-                  value_cache.sizes() ==
-                      torch::IntArrayRef({slots, key.size(-2), capacity, value.size(-1)}),
-              "caches must have shape (slots, key heads, capacity, width)");
-  TORCH_CHECK(window <= kIntMax && capacity >= window + sinks && capacity <= kIntMax,
-              "caches must hold the sinks and the window, and fewer than 2^31 tokens");
+  REQUIRE(key_cache.sizes() ==
+                  torch::IntArrayRef({slots, key.size(-2), capacity, key.size(-1)}) &&
+              value_cache.sizes() ==
+                  torch::IntArrayRef({slots, key.size(-2), capacity, value.size(-1)}),
+          "caches must have shape (slots, key heads, capacity, width)");
+  REQUIRE(window <= kIntMax && capacity >= window + sinks && capacity <= kIntMax,
+          "caches must hold the sinks and the window, and fewer than 2^31 tokens");
   for (const Tensor* cache : {&key_cache, &value_cache}) {
-    TORCH_CHECK(cache->device() == query.device(),
-                "caches must be on the CUDA device of the inputs");
-    TORCH_CHECK(cache->scalar_type() == query.scalar_type(),
-                "caches must have the dtype of the inputs");
-    TORCH_CHECK(cache->is_contiguous(), "caches must be contiguous");
-    at::assert_no_overlap(*cache, query);
-    at::assert_no_overlap(*cache, key);
-    at::assert_no_overlap(*cache, value);
+    REQUIRE(cache->scalar_type() == query.scalar_type(),
+            "caches must have the dtype of the inputs");
+    REQUIRE(cache->device() == query.device(), "all inputs and caches must be on the same device");
+    REQUIRE(cache->is_contiguous(), "caches must be contiguous");
+    REQUIRE(!overlap(*cache, query) && !overlap(*cache, key) && !overlap(*cache, value),
+            "caches must share no memory with the inputs");
   }
-  at::assert_no_overlap(key_cache, value_cache);
-  TORCH_CHECK(lengths.device() == query.device() && lengths.scalar_type() == torch::kInt32 &&
-                  lengths.dim() == 1 && lengths.size(0) == slots,
-              "lengths must be int32 with one entry per slot, on the CUDA device of the inputs");
+  REQUIRE(!overlap(key_cache, value_cache), "the caches must share no memory");
+  REQUIRE(lengths.dim() == 1 && lengths.size(0) == slots && lengths.scalar_type() == torch::kInt32,
+          "lengths must be an int32 tensor with one entry per slot");
+  REQUIRE(lengths.device() == query.device(), "all inputs and lengths must be on the same device");
+  check_device(query);
   const Guard guard(query.device());
-  const Call call = make_call(query, key, value, cu_seqlens, scale);
+  const Call call = make_call(query, key, value, cu_seqlens, factor);
   const Tensor output = new_output(call);
   if (query.numel() == 0) return output;
   const Tensor seen = lengths.contiguous();
@@ -413,41 +442,256 @@ Tensor window_attention_update_op(const Tensor& query, const Tensor& key, const 
   return output;
 }
 
+// ---------------------------------------------------------------------------
+// autograd
+// ---------------------------------------------------------------------------
+
+using torch::autograd::AutogradContext;
+using torch::autograd::variable_list;
+
+// the operators as the dispatcher has them, so that tracing sees them
+template <typename Signature>
+auto operator_handle(const char* name) {
+  return c10::Dispatcher::singleton().findSchemaOrThrow(name, "").template typed<Signature>();
+}
+Tensor call_decay(const Tensor& q, const Tensor& k, const Tensor& v, const OptionalTensor& cu,
+                  const Tensor& log_decay, Scale scale) {
+  static const auto handle =
+      operator_handle<decltype(decay_attention_op)>("rosa_soft::decay_attention");
+  return handle.call(q, k, v, cu, log_decay, scale);
+}
+Triple call_decay_vjp(const Tensor& q, const Tensor& k, const Tensor& v, const OptionalTensor& cu,
+                      const Tensor& log_decay, const Tensor& go, Scale scale, int64_t mask) {
+  static const auto handle =
+      operator_handle<decltype(decay_attention_vjp_op)>("rosa_soft::decay_attention_vjp");
+  return handle.call(q, k, v, cu, log_decay, go, scale, mask);
+}
+std::tuple<Tensor, Tensor> call_window(const Tensor& q, const Tensor& k, const Tensor& v,
+                                       const OptionalTensor& cu, int64_t window, int64_t sinks,
+                                       Scale scale, bool want_log_sum) {
+  static const auto handle =
+      operator_handle<decltype(window_attention_op)>("rosa_soft::window_attention");
+  return handle.call(q, k, v, cu, window, sinks, scale, want_log_sum);
+}
+Triple call_window_vjp(const Tensor& q, const Tensor& k, const Tensor& v, const OptionalTensor& cu,
+                       const Tensor& output, const Tensor& log_sum, const Tensor& go,
+                       int64_t window, int64_t sinks, Scale scale, int64_t mask) {
+  static const auto handle =
+      operator_handle<decltype(window_attention_vjp_op)>("rosa_soft::window_attention_vjp");
+  return handle.call(q, k, v, cu, output, log_sum, go, window, sinks, scale, mask);
+}
+
+int64_t gradient_mask_of(AutogradContext* ctx) {
+  int64_t mask = 0;
+  for (int i = 0; i < 3; ++i)  // query, key, value
+    if (ctx->needs_input_grad(i)) mask |= int64_t{1} << i;
+  return mask;
+}
+
+// The requested gradients in front of `others` empty ones.  They are differentiable once: with a
+// graph being made they lead to an error instead of nowhere.
+variable_list gradient_list(const Triple& gradients, int64_t mask, int others) {
+  variable_list list = {std::get<0>(gradients), std::get<1>(gradients), std::get<2>(gradients)};
+  for (int i = 0; i < 3; ++i)
+    if ((mask >> i & 1) == 0) list[i] = Tensor();
+  if (at::GradMode::is_enabled()) {
+    for (Tensor& gradient : list) {
+      if (!gradient.defined()) continue;
+      gradient.set_requires_grad(true);
+      const auto error = std::make_shared<torch::autograd::DelayedError>(
+          "trying to differentiate twice a mixer, whose gradients are differentiable once", 1);
+      gradient = (*error)({gradient})[0];
+    }
+  }
+  list.resize(3 + others);
+  return list;
+}
+
+struct DecayAttention : torch::autograd::Function<DecayAttention> {
+  static Tensor forward(AutogradContext* ctx, const Tensor& query, const Tensor& key,
+                        const Tensor& value, const OptionalTensor& cu_seqlens,
+                        const Tensor& log_decay, Scale scale) {
+    at::AutoDispatchBelowADInplaceOrView below;
+    ctx->save_for_backward({query, key, value, cu_seqlens.value_or(Tensor()), log_decay});
+    if (scale) ctx->saved_data["scale"] = *scale;
+    return call_decay(query, key, value, cu_seqlens, log_decay, scale);
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    const auto saved = ctx->get_saved_variables();
+    const OptionalTensor cu_seqlens = saved[3].defined() ? OptionalTensor(saved[3]) : std::nullopt;
+    const Scale scale = ctx->saved_data.count("scale")
+                            ? Scale(ctx->saved_data["scale"].toDouble()) : std::nullopt;
+    const int64_t mask = gradient_mask_of(ctx);
+    Triple gradients;
+    {
+      at::AutoDispatchBelowADInplaceOrView below;
+      gradients = call_decay_vjp(saved[0], saved[1], saved[2], cu_seqlens, saved[4], grads[0],
+                                 scale, mask);
+    }
+    return gradient_list(gradients, mask, 3);
+  }
+};
+
+struct WindowAttention : torch::autograd::Function<WindowAttention> {
+  static variable_list forward(AutogradContext* ctx, const Tensor& query, const Tensor& key,
+                               const Tensor& value, const OptionalTensor& cu_seqlens,
+                               int64_t window, int64_t sinks, Scale scale) {
+    at::AutoDispatchBelowADInplaceOrView below;
+    auto [output, log_sum] =
+        call_window(query, key, value, cu_seqlens, window, sinks, scale, true);
+    ctx->save_for_backward({query, key, value, cu_seqlens.value_or(Tensor()), output, log_sum});
+    ctx->mark_non_differentiable({log_sum});
+    ctx->saved_data["window"] = window;
+    ctx->saved_data["sinks"] = sinks;
+    if (scale) ctx->saved_data["scale"] = *scale;
+    return {output, log_sum};
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    const auto saved = ctx->get_saved_variables();
+    const OptionalTensor cu_seqlens = saved[3].defined() ? OptionalTensor(saved[3]) : std::nullopt;
+    const Scale scale = ctx->saved_data.count("scale")
+                            ? Scale(ctx->saved_data["scale"].toDouble()) : std::nullopt;
+    const int64_t mask = gradient_mask_of(ctx);
+    Triple gradients;
+    {
+      at::AutoDispatchBelowADInplaceOrView below;
+      gradients = call_window_vjp(saved[0], saved[1], saved[2], cu_seqlens, saved[4], saved[5],
+                                  grads[0], ctx->saved_data["window"].toInt(),
+                                  ctx->saved_data["sinks"].toInt(), scale, mask);
+    }
+    return gradient_list(gradients, mask, 4);
+  }
+};
+
+template <typename... Tensors>
+bool needs_backward(const Tensors&... tensors) {
+  return at::GradMode::is_enabled() && (tensors.requires_grad() || ...);
+}
+
+Tensor decay_attention_autograd(const Tensor& query, const Tensor& key, const Tensor& value,
+                                const OptionalTensor& cu_seqlens, const Tensor& log_decay,
+                                Scale scale) {
+  REQUIRE(!needs_backward(log_decay),
+          "log_decay is a constant of each head and takes no gradient: detach it");
+  if (!needs_backward(query, key, value)) {
+    at::AutoDispatchBelowADInplaceOrView below;
+    return call_decay(query, key, value, cu_seqlens, log_decay, scale);
+  }
+  refuse_capture("decay_attention", query);
+  return DecayAttention::apply(query, key, value, cu_seqlens, log_decay, scale);
+}
+
+std::tuple<Tensor, Tensor> window_attention_autograd(const Tensor& query, const Tensor& key,
+                                                     const Tensor& value,
+                                                     const OptionalTensor& cu_seqlens,
+                                                     int64_t window, int64_t sinks, Scale scale,
+                                                     bool want_log_sum) {
+  if (!needs_backward(query, key, value)) {
+    at::AutoDispatchBelowADInplaceOrView below;
+    return call_window(query, key, value, cu_seqlens, window, sinks, scale, want_log_sum);
+  }
+  refuse_capture("window_attention", query);
+  const auto results =
+      WindowAttention::apply(query, key, value, cu_seqlens, window, sinks, scale);
+  return {results[0], results[1]};
+}
+
+// Operators without a backward: whatever asks for one is refused, not cut off in silence.
+template <auto* kOperator, typename... Arguments>
+auto without_backward(Arguments... arguments) {
+  const auto asks = [](const auto& argument) {
+    if constexpr (std::is_same_v<std::decay_t<decltype(argument)>, Tensor>)
+      return argument.requires_grad();
+    else
+      return false;
+  };
+  TORCH_CHECK(!(at::GradMode::is_enabled() && (asks(arguments) || ...)),
+              "an update and the gradients of a mixer have no backward: call them under "
+              "torch.no_grad()");
+  at::AutoDispatchBelowADInplaceOrView below;
+  return (*kOperator)(std::forward<Arguments>(arguments)...);
+}
+
+Tensor call_decay_update(const Tensor& q, const Tensor& k, const Tensor& v,
+                         const OptionalTensor& cu, const Tensor& log_decay, Tensor state,
+                         Scale scale) {
+  static const auto handle =
+      operator_handle<decltype(decay_attention_update_op)>("rosa_soft::decay_attention_update");
+  return handle.call(q, k, v, cu, log_decay, state, scale);
+}
+Tensor call_decay_update_out(const Tensor& q, const Tensor& k, const Tensor& v,
+                             const OptionalTensor& cu, const Tensor& log_decay,
+                             const Tensor& state, Tensor state_out, Scale scale) {
+  static const auto handle = operator_handle<decltype(decay_attention_update_out_op)>(
+      "rosa_soft::decay_attention_update_out");
+  return handle.call(q, k, v, cu, log_decay, state, state_out, scale);
+}
+Tensor call_window_update(const Tensor& q, const Tensor& k, const Tensor& v, Tensor key_cache,
+                          Tensor value_cache, const Tensor& lengths, const OptionalTensor& cu,
+                          int64_t window, int64_t sinks, Scale scale) {
+  static const auto handle =
+      operator_handle<decltype(window_attention_update_op)>("rosa_soft::window_attention_update");
+  return handle.call(q, k, v, key_cache, value_cache, lengths, cu, window, sinks, scale);
+}
+
+template <auto* kOperator, typename Result, typename... Arguments>
+Result refuse_backward(Arguments... arguments) {
+  return without_backward<kOperator, Arguments...>(std::forward<Arguments>(arguments)...);
+}
+template <auto* kOperator, typename Result, typename... Arguments>
+constexpr auto refusing(Result (*)(Arguments...)) {
+  return &refuse_backward<kOperator, Result, Arguments...>;
+}
+
 }  // namespace
 
 TORCH_LIBRARY_FRAGMENT(rosa_soft, m) {
   m.def(
       "decay_attention(Tensor query, Tensor key, Tensor value, Tensor? cu_seqlens, "
-      "Tensor log_decay, float scale) -> Tensor output");
+      "Tensor log_decay, float? scale=None) -> Tensor output");
   m.def(
       "decay_attention_vjp(Tensor query, Tensor key, Tensor value, Tensor? cu_seqlens, "
-      "Tensor log_decay, Tensor grad_output, float scale, int gradient_mask) -> "
+      "Tensor log_decay, Tensor grad_output, float? scale, int gradient_mask) -> "
       "(Tensor grad_query, Tensor grad_key, Tensor grad_value)");
   m.def(
       "decay_attention_update(Tensor query, Tensor key, Tensor value, Tensor? cu_seqlens, "
-      "Tensor log_decay, Tensor(a!) state, float scale) -> Tensor output");
+      "Tensor log_decay, Tensor(a!) state, float? scale=None) -> Tensor output");
   m.def(
       "decay_attention_update_out(Tensor query, Tensor key, Tensor value, Tensor? cu_seqlens, "
-      "Tensor log_decay, Tensor state, Tensor(a!) state_out, float scale) -> Tensor output");
+      "Tensor log_decay, Tensor state, Tensor(a!) state_out, float? scale=None) -> Tensor output");
   m.def(
       "window_attention(Tensor query, Tensor key, Tensor value, Tensor? cu_seqlens, int window, "
-      "int sinks, float scale, bool want_log_sum) -> (Tensor output, Tensor log_sum)");
+      "int sinks, float? scale=None, bool want_log_sum=False) -> (Tensor output, Tensor log_sum)");
   m.def(
       "window_attention_vjp(Tensor query, Tensor key, Tensor value, Tensor? cu_seqlens, "
-      "Tensor output, Tensor log_sum, Tensor grad_output, int window, int sinks, float scale, "
+      "Tensor output, Tensor log_sum, Tensor grad_output, int window, int sinks, float? scale, "
       "int gradient_mask) -> (Tensor grad_query, Tensor grad_key, Tensor grad_value)");
   m.def(
       "window_attention_update(Tensor query, Tensor key, Tensor value, Tensor(a!) key_cache, "
       "Tensor(b!) value_cache, Tensor lengths, Tensor? cu_seqlens, int window, int sinks, "
-      "float scale) -> Tensor output");
+      "float? scale=None) -> Tensor output");
 }
 
-TORCH_LIBRARY_IMPL(rosa_soft, CUDA, m) {
-  m.impl("decay_attention", &decay_attention_op);
-  m.impl("decay_attention_vjp", &decay_attention_vjp_op);
-  m.impl("decay_attention_update", &decay_attention_update_op);
-  m.impl("decay_attention_update_out", &decay_attention_update_out_op);
-  m.impl("window_attention", &window_attention_op);
-  m.impl("window_attention_vjp", &window_attention_vjp_op);
+#define ROSA_MIXER_OPERATORS(m)                                           \
+  m.impl("decay_attention", &decay_attention_op);                         \
+  m.impl("decay_attention_vjp", &decay_attention_vjp_op);                 \
+  m.impl("decay_attention_update", &decay_attention_update_op);           \
+  m.impl("decay_attention_update_out", &decay_attention_update_out_op);   \
+  m.impl("window_attention", &window_attention_op);                       \
+  m.impl("window_attention_vjp", &window_attention_vjp_op);               \
   m.impl("window_attention_update", &window_attention_update_op);
+
+TORCH_LIBRARY_IMPL(rosa_soft, CUDA, m) { ROSA_MIXER_OPERATORS(m) }
+
+// host tensors meet the same checks, the last of which refuses them
+TORCH_LIBRARY_IMPL(rosa_soft, CPU, m) { ROSA_MIXER_OPERATORS(m) }
+
+TORCH_LIBRARY_IMPL(rosa_soft, Autograd, m) {
+  m.impl("decay_attention", &decay_attention_autograd);
+  m.impl("window_attention", &window_attention_autograd);
+  m.impl("decay_attention_vjp", refusing<&call_decay_vjp>(&call_decay_vjp));
+  m.impl("window_attention_vjp", refusing<&call_window_vjp>(&call_window_vjp));
+  m.impl("decay_attention_update", refusing<&call_decay_update>(&call_decay_update));
+  m.impl("decay_attention_update_out", refusing<&call_decay_update_out>(&call_decay_update_out));
+  m.impl("window_attention_update", refusing<&call_window_update>(&call_window_update));
 }

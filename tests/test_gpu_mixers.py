@@ -463,6 +463,52 @@ def test_invalid_offsets_give_nan_and_change_nothing(offsets):
     assert bool(torch.isnan(output).all()) and all(map(torch.equal, caches, kept))
 
 
+def test_tensors_of_two_devices_are_refused():
+    (q, k, v), _ = inputs_of(((2, 5), None, 2, 1, 8, 8), torch.float32, seed=145)
+    log_decay, state = rates(2), torch.zeros(2, 2, 8, 8, device=DEVICE)
+    caches = [torch.zeros(2, 1, 9, 8, device=DEVICE) for _ in range(2)]
+    lengths = torch.zeros(2, dtype=torch.int32, device=DEVICE)
+    packed, offsets = [t.flatten(0, 1) for t in (q, k, v)], offsets_of([4, 6])
+    for call in (lambda: mixers.decay_attention(q, k.cpu(), v, log_decay),
+                 lambda: mixers.decay_attention(q, k, v, log_decay.cpu()),
+                 lambda: mixers.decay_attention_varlen(*packed, offsets.cpu(), log_decay),
+                 lambda: mixers.decay_attention_update(q, k, v, log_decay, state.cpu()),
+                 lambda: mixers.window_attention(q, k, v.cpu(), window=3),
+                 lambda: mixers.window_attention_varlen(*packed, offsets.cpu(), window=3),
+                 lambda: mixers.window_attention_update(q, k, v, caches[0].cpu(), caches[1], lengths,
+                                                        window=9),
+                 lambda: mixers.window_attention_update(q, k, v, *caches, lengths.cpu(), window=9)):
+        with pytest.raises(ValueError, match="same device"):
+            call()
+
+
+def test_overlapping_states_and_caches_are_refused():
+    (q, k, v), _ = inputs_of(((1, 1), None, 2, 2, 8, 8), torch.float32, seed=146)
+    log_decay = rates(2)
+    both = torch.zeros(2 * 128 + 4, device=DEVICE)
+    with pytest.raises(ValueError, match="share no memory"):
+        mixers.decay_attention_update(q, k, v, log_decay, both[:128].view(1, 2, 8, 8),
+                                      state_out=both[4:132].view(1, 2, 8, 8))
+    cache = torch.zeros(1, 2, 9, 8, device=DEVICE)
+    lengths = torch.zeros(1, dtype=torch.int32, device=DEVICE)
+    with pytest.raises(ValueError, match="share no memory"):
+        mixers.window_attention_update(q, k, v, cache, cache, lengths, window=9)
+    with pytest.raises(ValueError, match="share no memory"):
+        mixers.window_attention_update(q, cache[:, :, :1].transpose(1, 2), v, cache,
+                                       torch.zeros_like(cache), lengths, window=9)
+
+
+@pytest.mark.parametrize("which", ["decay", "window"])
+def test_gradients_are_differentiable_once(which):
+    (q, k, v), _ = inputs_of(((1, 20), None, 2, 2, 8, 8), torch.float32, seed=147)
+    leaves = [t.requires_grad_() for t in (q, k, v)]
+    output = mixers.decay_attention(*leaves, rates(2)) if which == "decay" else \
+        mixers.window_attention(*leaves, window=5)
+    gradients = torch.autograd.grad(output.square().sum(), leaves, create_graph=True)
+    with pytest.raises(RuntimeError, match="differentiate twice"):
+        gradients[0].sum().backward()
+
+
 def test_updates_without_tokens():
     log_decay, state = rates(2), randn(150, 3, 2, 8, 8)
     other = torch.zeros_like(state)

@@ -16,12 +16,16 @@ def fake(*shape, dtype=torch.bfloat16, device="cuda"):
     return torch.empty(*shape, dtype=dtype, device=device)
 
 
-def arguments(**changes):
-    """A dense call that passes every check, under FakeTensorMode; ``changes`` replace parts."""
-    parts = dict(q=fake(2, 5, 4, 16), k=fake(2, 5, 2, 16), v=fake(2, 5, 2, 8),
-                 log_decay=fake(4, dtype=torch.float32), state=fake(2, 4, 16, 8, dtype=torch.float32),
-                 keys=fake(2, 2, 12, 16), values=fake(2, 2, 12, 8),
-                 lengths=fake(2, dtype=torch.int32), window=9, sinks=3)
+def host(*shape, dtype=torch.bfloat16):
+    return torch.zeros(*shape, dtype=dtype)
+
+
+def arguments(make=host, **changes):
+    """A dense call that passes every check but that of the device; ``changes`` replace parts."""
+    parts = dict(q=make(2, 5, 4, 16), k=make(2, 5, 2, 16), v=make(2, 5, 2, 8),
+                 log_decay=make(4, dtype=torch.float32), state=make(2, 4, 16, 8, dtype=torch.float32),
+                 keys=make(2, 2, 12, 16), values=make(2, 2, 12, 8),
+                 lengths=make(2, dtype=torch.int32), window=9, sinks=3)
     parts.update(changes)
     return parts
 
@@ -42,7 +46,7 @@ def calls(p):
 
 def test_calls_that_pass_give_outputs_of_the_right_shape():
     with FakeTensorMode():
-        for name, call in calls(arguments()).items():
+        for name, call in calls(arguments(fake)).items():
             output = call()
             assert output.shape == (2, 5, 4, 8) and output.dtype == torch.bfloat16, name
         packed = [fake(7, 4, 16), fake(7, 2, 16), fake(7, 2, 8)]
@@ -61,71 +65,69 @@ EVERY = ("decay", "decay_update", "window", "window_update")
 
 
 @pytest.mark.parametrize("names,changes,error,message", [
-    (EVERY, lambda: dict(q=fake(5, 4, 16)), ValueError, "must have shape"),
-    (EVERY, lambda: dict(k=fake(2, 6, 2, 16)), ValueError, "share their token dimensions"),
-    (EVERY, lambda: dict(v=fake(2, 5, 1, 8)), ValueError, "key and value head counts"),
-    (EVERY, lambda: dict(q=fake(2, 5, 3, 16)), ValueError, "divisible by key heads"),
-    (EVERY, lambda: dict(q=fake(2, 5, 4, 17)), ValueError, "query and key widths"),
-    (EVERY, lambda: dict(q=fake(2, 5, 4, 129), k=fake(2, 5, 2, 129)), ValueError, r"\[1, 128\]"),
-    (EVERY, lambda: dict(v=fake(2, 5, 2, 0)), ValueError, r"\[1, 128\]"),
-    (EVERY, lambda: dict(k=fake(2, 5, 2, 16, dtype=torch.float16)), ValueError, "same dtype"),
-    (EVERY, lambda: dict(k=fake(2, 5, 2, 16, device="cpu")), ValueError, "same device"),
-    (EVERY, lambda: {n: fake(2, 5, 2, 8, dtype=torch.float64) for n in "qkv"}, ValueError,
+    (EVERY, lambda: dict(q=host(5, 4, 16)), ValueError, "must have shape"),
+    (EVERY, lambda: dict(k=host(2, 6, 2, 16)), ValueError, "share their token dimensions"),
+    (EVERY, lambda: dict(v=host(2, 5, 1, 8)), ValueError, "key and value head counts"),
+    (EVERY, lambda: dict(q=host(2, 5, 3, 16)), ValueError, "divisible by key heads"),
+    (EVERY, lambda: dict(q=host(2, 5, 4, 17)), ValueError, "query and key widths"),
+    (EVERY, lambda: dict(q=host(2, 5, 4, 129), k=host(2, 5, 2, 129)), ValueError, r"\[1, 128\]"),
+    (EVERY, lambda: dict(v=host(2, 5, 2, 0)), ValueError, r"\[1, 128\]"),
+    (EVERY, lambda: dict(k=host(2, 5, 2, 16, dtype=torch.float16)), ValueError, "same dtype"),
+    (EVERY, lambda: {n: host(2, 5, 2, 8, dtype=torch.float64) for n in "qkv"}, ValueError,
      "float32, float16, and bfloat16"),
-    (EVERY, lambda: {n: fake(2, 5, 2, 8, device="cpu") for n in "qkv"}, ValueError,
-     "requires CUDA tensors"),
+    (EVERY, lambda: {}, ValueError, "require CUDA tensors"),
     (EVERY, lambda: dict(scale=0.0), ValueError, "positive normal"),
     (EVERY, lambda: dict(scale=math.inf), ValueError, "positive normal"),
     (EVERY, lambda: dict(scale=1e-40), ValueError, "positive normal"),
-    (("decay", "window"), lambda: dict(q=fake(2, 0, 4, 16), k=fake(2, 0, 2, 16), v=fake(2, 0, 2, 8)),
+    (("decay", "window"), lambda: dict(q=host(2, 0, 4, 16), k=host(2, 0, 2, 16), v=host(2, 0, 2, 8)),
      ValueError, "must be >= 1"),
     (("decay_update", "window_update"),
-     lambda: dict(q=fake(0, 5, 4, 16), k=fake(0, 5, 2, 16), v=fake(0, 5, 2, 8)), ValueError,
+     lambda: dict(q=host(0, 5, 4, 16), k=host(0, 5, 2, 16), v=host(0, 5, 2, 8)), ValueError,
      "at least one slot"),
-    (EVERY[:2], lambda: dict(log_decay=fake(2, dtype=torch.float32)), ValueError,
+    (EVERY[:2], lambda: dict(log_decay=host(2, dtype=torch.float32)), ValueError,
      "one entry per query head"),
-    (EVERY[:2], lambda: dict(log_decay=fake(4)), ValueError, "dtype float32"),
-    (EVERY[:2], lambda: dict(log_decay=fake(4, dtype=torch.float32, device="cpu")), ValueError,
-     "same device"),
-    (EVERY[:2], lambda: dict(log_decay=fake(4, dtype=torch.float32).requires_grad_()), ValueError,
+    (EVERY[:2], lambda: dict(log_decay=host(4)), ValueError, "dtype float32"),
+    (EVERY[:1], lambda: dict(log_decay=host(4, dtype=torch.float32).requires_grad_()), ValueError,
      "takes no gradient"),
-    (EVERY[1:2], lambda: dict(state=fake(2, 2, 16, 8, dtype=torch.float32)), ValueError, "shape"),
-    (EVERY[1:2], lambda: dict(state=fake(2, 4, 16, 8)), ValueError, "float32"),
-    (EVERY[1:2], lambda: dict(state=fake(2, 4, 8, 16, dtype=torch.float32).transpose(2, 3)),
+    (EVERY[1:2], lambda: dict(log_decay=host(4, dtype=torch.float32).requires_grad_()), RuntimeError,
+     "have no backward"),
+    (EVERY[1:2], lambda: dict(state=host(2, 2, 16, 8, dtype=torch.float32)), ValueError, "shape"),
+    (EVERY[1:2], lambda: dict(state=host(2, 4, 16, 8)), ValueError, "float32"),
+    (EVERY[1:2], lambda: dict(state=host(2, 4, 8, 16, dtype=torch.float32).transpose(2, 3)),
      ValueError, "contiguous"),
-    (EVERY[1:2], lambda: dict(state_out=fake(2, 4, 16, 9, dtype=torch.float32)), ValueError, "shape"),
+    (EVERY[1:2], lambda: dict(state_out=host(2, 4, 16, 9, dtype=torch.float32)), ValueError, "shape"),
     (EVERY[2:], lambda: dict(window=0), ValueError, "window must be >= 1"),
     (EVERY[2:], lambda: dict(window=True), TypeError, "window must be an integer"),
     (EVERY[2:], lambda: dict(window=2.5), TypeError, "window must be an integer"),
     (EVERY[2:], lambda: dict(sinks=-1), ValueError, "sinks"),
     (EVERY[2:], lambda: dict(sinks=65), ValueError, "sinks"),
-    (EVERY[3:], lambda: dict(keys=fake(2, 2, 11, 16), values=fake(2, 2, 11, 8)), ValueError,
+    (EVERY[3:], lambda: dict(keys=host(2, 2, 11, 16), values=host(2, 2, 11, 8)), ValueError,
      "hold the sinks and the window"),
-    (EVERY[3:], lambda: dict(values=fake(2, 2, 13, 8)), ValueError, "shape"),
-    (EVERY[3:], lambda: dict(keys=fake(2, 2, 12, 16, dtype=torch.float16)), ValueError, "dtype"),
-    (EVERY[3:], lambda: dict(keys=fake(2, 12, 2, 16).transpose(1, 2)), ValueError, "contiguous"),
-    (EVERY[3:], lambda: dict(lengths=fake(2, dtype=torch.int64)), ValueError, "lengths"),
-    (EVERY[3:], lambda: dict(lengths=fake(3, dtype=torch.int32)), ValueError, "lengths"),
-    (("decay_update", "window_update"), lambda: dict(q=fake(2, 5, 4, 16).requires_grad_()),
-     RuntimeError, "has no backward"),
+    (EVERY[3:], lambda: dict(values=host(2, 2, 13, 8)), ValueError, "shape"),
+    (EVERY[3:], lambda: dict(keys=host(2, 2, 12, 16, dtype=torch.float16)), ValueError, "dtype"),
+    (EVERY[3:], lambda: dict(keys=host(2, 12, 2, 16).transpose(1, 2)), ValueError, "contiguous"),
+    (EVERY[3:], lambda: dict(lengths=host(2, dtype=torch.int64)), ValueError, "lengths"),
+    (EVERY[3:], lambda: dict(lengths=host(3, dtype=torch.int32)), ValueError, "lengths"),
+    (("decay_update", "window_update"), lambda: dict(q=host(2, 5, 4, 16).requires_grad_()),
+     RuntimeError, "have no backward"),
 ])
 def test_refusals(names, changes, error, message):
-    with FakeTensorMode():
-        for name in names:
-            with pytest.raises(error, match=message):
-                calls(arguments(**changes()))[name]()
+    """Every check is made before the device is looked at: host tensors meet all of them."""
+
+    for name in names:
+        with pytest.raises(error, match=message):
+            calls(arguments(**changes()))[name]()
 
 
 def test_packed_refusals():
-    with FakeTensorMode():
-        packed = [fake(7, 4, 16), fake(7, 2, 16), fake(7, 2, 8)]
-        log_decay = fake(4, dtype=torch.float32)
-        for offsets, message in ((fake(3, dtype=torch.int64), "int32"), (fake(1, dtype=torch.int32), "one-dimensional"),
-                                 (fake(3, dtype=torch.int32, device="cpu"), "same device")):
-            for call in (lambda: mixers.decay_attention_varlen(*packed, offsets, log_decay),
-                         lambda: mixers.window_attention_varlen(*packed, offsets, window=2)):
-                with pytest.raises(ValueError, match=message):
-                    call()
+    packed = [host(7, 4, 16), host(7, 2, 16), host(7, 2, 8)]
+    log_decay = host(4, dtype=torch.float32)
+    for offsets, message in ((host(3, dtype=torch.int64), "int32"),
+                             (host(1, dtype=torch.int32), "one-dimensional")):
+        for call in (lambda: mixers.decay_attention_varlen(*packed, offsets, log_decay),
+                     lambda: mixers.window_attention_varlen(*packed, offsets, window=2)):
+            with pytest.raises(ValueError, match=message):
+                call()
 
 
 def test_signatures_and_schemas():

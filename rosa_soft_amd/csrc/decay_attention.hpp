@@ -59,10 +59,11 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2))) v
   constexpr int kWaveRows = kTiles / kWaveCols;
   constexpr int kSteps = WIDTH / 32;
 
-  __shared__ __attribute__((aligned(16))) T keys[kChunk * kPitch<T, WIDTH>];
-  __shared__ __attribute__((aligned(16))) T values[STATE_ONLY ? 16 : kChunk * kPitch<T, SLICE>];
-  __shared__ __attribute__((aligned(16))) ST weighted[TERMS * kChunk * kPitch<ST, SLICE>];
-  __shared__ __attribute__((aligned(16))) T state_rows[STATE_ONLY ? 16 : SLICE * kPitch<T, WIDTH>];
+  constexpr int kTerm = kTileElements<ST, kChunk, SLICE>;  // of the weighted values
+  __shared__ __attribute__((aligned(16))) Stored<T> keys[kTileElements<T, kChunk, WIDTH>];
+  __shared__ __attribute__((aligned(16))) Stored<T> values[STATE_ONLY ? 16 : kTileElements<T, kChunk, SLICE>];
+  __shared__ __attribute__((aligned(16))) Stored<ST> weighted[TERMS * kTerm];
+  __shared__ __attribute__((aligned(16))) Stored<T> state_rows[STATE_ONLY ? 16 : kTileElements<T, SLICE, WIDTH>];
   __shared__ float largest[4];
 
   const int64_t item = item_of_block(a.items);
@@ -222,17 +223,20 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2))) v
       float left[kElements];
 #pragma unroll
       for (int e = 0; e < kElements; ++e) left[e] = static_cast<float>(value_move.held[i][e]) * by;
+      if constexpr (sizeof(T) == 4) {
+        store_row<ST, kChunk, SLICE>(weighted, row, value_move.col_of(tid), left);
+      } else {
 #pragma unroll
-      for (int t = 0; t < TERMS; ++t) {
-        typedef ST Piece __attribute__((ext_vector_type(kElements)));
-        Piece term;
+        for (int t = 0; t < TERMS; ++t) {
+          typedef ST Piece __attribute__((ext_vector_type(kElements)));
+          Piece term;
 #pragma unroll
-        for (int e = 0; e < kElements; ++e) {
-          term[e] = static_cast<ST>(left[e]);
-          left[e] -= static_cast<float>(term[e]);
+          for (int e = 0; e < kElements; ++e) {
+            term[e] = static_cast<ST>(left[e]);
+            left[e] -= static_cast<float>(term[e]);
+          }
+          *reinterpret_cast<Piece*>(weighted + t * kTerm + row * kPitch<SLICE> + value_move.col_of(tid)) = term;
         }
-        *reinterpret_cast<Piece*>(weighted + (t * kChunk + row) * kPitch<ST, SLICE> +
-                                  value_move.col_of(tid)) = term;
       }
     }
     if constexpr (!STATE_ONLY) {
@@ -244,20 +248,19 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2))) v
       for (int i = 0; i < kWaveRows; ++i)
 #pragma unroll
         for (int j = 0; j < kWaveCols; ++j) {
-          Quad<T> rounded;
+          float rounded[4];
 #pragma unroll
-          for (int r = 0; r < 4; ++r) rounded[r] = static_cast<T>(state[i][j][r] * unit);
-          *reinterpret_cast<Quad<T>*>(state_rows +
-                                      ((col_tile + j) * 16 + column) * kPitch<T, WIDTH> +
-                                      (row_tile + i) * 16 + 4 * group) = rounded;
+          for (int r = 0; r < 4; ++r) rounded[r] = state[i][j][r] * unit;
+          store_row<T, SLICE, WIDTH>(state_rows, (col_tile + j) * 16 + column, (row_tile + i) * 16 + 4 * group,
+                                     rounded);
         }
     }
-    Frag<T> query[kSteps];
+    Operand<T> query[kSteps];
     if constexpr (!STATE_ONLY) {
 #pragma unroll
       for (int s = 0; s < kSteps; ++s) {
-        query[s] = next_query[s];
-        clear_operand<WHOLE>(query[s], s * 32 + 8 * group, p.key_width);
+        clear_operand<WHOLE>(next_query[s], s * 32 + 8 * group, p.key_width);
+        query[s] = as_operand<T>(next_query[s]);
       }
     }
     __syncthreads();
@@ -275,7 +278,7 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2))) v
         for (int s = 0; s < kSteps; ++s)
 #pragma unroll
           for (int t = 0; t < kColTiles; ++t)
-            out[t] = mma(row_operand<T, WIDTH>(state_rows, t * 16, s * 32, lane), query[s], out[t]);
+            out[t] = mma(row_operand<T, SLICE, WIDTH>(state_rows, t * 16, s * 32, lane), query[s], out[t]);
         f32x4 score[4];
         float step = 1.0f;  // lambda^16 for every tile further back
         const float tile_rate = power_of(rate, 16);
@@ -285,7 +288,7 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2))) v
           if (t <= wave) {
 #pragma unroll
             for (int s = 0; s < kSteps; ++s)
-              score[t] = mma(row_operand<T, WIDTH>(keys, t * 16, s * 32, lane), query[s], score[t]);
+              score[t] = mma(row_operand<T, kChunk, WIDTH>(keys, t * 16, s * 32, lane), query[s], score[t]);
             if (t == wave) {
 #pragma unroll
               for (int r = 0; r < 4; ++r)  // (a select, so that later keys never reach a token)
@@ -315,10 +318,10 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2))) v
 #pragma unroll
         for (int half = 0; half < 2; ++half) {
           if (2 * half <= wave) {
-            const Frag<T> scores = operand_of<T>(score[2 * half], score[2 * half + 1]);
+            const Operand<T> scores = operand_of<T>(score[2 * half], score[2 * half + 1]);
 #pragma unroll
             for (int t = 0; t < kColTiles; ++t)
-              out[t] = mma(column_operand<T, SLICE>(values, half * 32, t * 16, lane), scores, out[t]);
+              out[t] = mma(column_operand<T, kChunk, SLICE>(values, half * 32, t * 16, lane), scores, out[t]);
           }
         }
         ready_at = at;
@@ -339,16 +342,16 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2))) v
 #pragma unroll
     for (int half = 0; half < 2; ++half) {
       if (half * 32 >= fill) break;
-      Frag<ST> value[TERMS][kWaveCols];
+      Operand<ST> value[TERMS][kWaveCols];
 #pragma unroll
       for (int t = 0; t < TERMS; ++t)
 #pragma unroll
         for (int j = 0; j < kWaveCols; ++j)
-          value[t][j] = column_operand<ST, SLICE>(weighted + t * kChunk * kPitch<ST, SLICE>, half * 32,
+          value[t][j] = column_operand<ST, kChunk, SLICE>(weighted + t * kTerm, half * 32,
                                                   (col_tile + j) * 16, lane);
 #pragma unroll
       for (int i = 0; i < kWaveRows; ++i) {
-        const Frag<T> key = column_operand<T, WIDTH>(keys, half * 32, (row_tile + i) * 16, lane);
+        const Operand<T> key = column_operand<T, kChunk, WIDTH>(keys, half * 32, (row_tile + i) * 16, lane);
         if constexpr (std::is_same_v<T, _Float16>) {
           // a float16 is the sum of two bfloat16
           Frag<__bf16> high, low;

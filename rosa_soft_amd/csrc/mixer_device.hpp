@@ -4,9 +4,10 @@
 //
 // Everything is built from one product, D[16 x 16] += A[16 x 32] B[32 x 16] in float32.  Lane
 // l = 16 g + c of a wave holds A[c][8 g .. 8 g + 7], B[8 g .. 8 g + 7][c] and D[4 g + r][c],
-// r = 0..3.  For the 16-bit types that is v_mfma_f32_16x16x32; for float32 the same operands
-// are fed to eight v_mfma_f32_16x16x4 (the order of the 32 terms is free as long as A and B
-// agree), so that a kernel is written once for all three types.
+// r = 0..3.  For the 16-bit types that is v_mfma_f32_16x16x32 (16 cycles).  A float32 operand is
+// the sum of three bfloat16 ones, 2^-27 from it at most, and a product the six of their nine
+// products that reach 2^-24 of it: 96 cycles, where the eight v_mfma_f32_16x16x4 that take
+// float32 as it is need 256.  A kernel is written once for all three types.
 //
 // Two ways of reading an operand from a row-major tile exist.  Along a row (the summed index is
 // the column): 8 neighbouring elements.  Down a column (the summed index is the row): lanes of
@@ -39,10 +40,63 @@ __device__ __forceinline__ f32x4 mma(Frag<__bf16> a, Frag<__bf16> b, f32x4 c) {
 __device__ __forceinline__ f32x4 mma(Frag<_Float16> a, Frag<_Float16> b, f32x4 c) {
   return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
 }
-__device__ __forceinline__ f32x4 mma(Frag<float> a, Frag<float> b, f32x4 c) {
+
+struct SplitOperand {
+  Frag<__bf16> part[3];  // falling by 2^-8 or more
+};
+template <typename T> using Operand = std::conditional_t<sizeof(T) == 4, SplitOperand, Frag<T>>;
+// what tiles in LDS hold: one plane, or one for each part
+template <typename T> using Stored = std::conditional_t<sizeof(T) == 4, __bf16, T>;
+template <typename T> constexpr int kPlanes = sizeof(T) == 4 ? 3 : 1;
+
+__device__ __forceinline__ f32x4 mma(const SplitOperand& a, const SplitOperand& b, f32x4 c) {
 #pragma unroll
-  for (int e = 0; e < 8; ++e) c = __builtin_amdgcn_mfma_f32_16x16x4f32(a[e], b[e], c, 0, 0, 0);
+  for (int order = 2; order >= 0; --order)
+#pragma unroll
+    for (int i = 0; i <= order; ++i) c = mma(a.part[i], b.part[order - i], c);
   return c;
+}
+
+// N float32 as their parts
+template <int N>
+__device__ __forceinline__ void split(const float (&x)[N],
+                                      __bf16 __attribute__((ext_vector_type(N))) (&part)[3]) {
+#pragma unroll
+  for (int e = 0; e < N; ++e) {
+    float left = x[e];
+#pragma unroll
+    for (int p = 0; p < 3; ++p) {
+      part[p][e] = static_cast<__bf16>(left);
+      left -= static_cast<float>(part[p][e]);
+    }
+  }
+}
+
+// eight neighbouring elements as an operand
+template <typename T>
+__device__ __forceinline__ Operand<T> as_operand(Frag<T> x) {
+  if constexpr (sizeof(T) == 4) {
+    float values[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) values[e] = x[e];
+    SplitOperand out;
+    split<8>(values, out.part);
+    return out;
+  } else {
+    return x;
+  }
+}
+
+// c + the sums over the columns of an operand B, in every row
+template <typename T>
+__device__ __forceinline__ f32x4 add_sums(const Operand<T>& b, f32x4 c) {
+  if constexpr (sizeof(T) == 4) {
+#pragma unroll
+    for (int p = 2; p >= 0; --p) c = mma(Frag<__bf16>(static_cast<__bf16>(1.0f)), b.part[p], c);
+    return c;
+  } else {
+    return mma(Frag<T>(static_cast<T>(1.0f)), b, c);
+  }
 }
 
 __device__ __forceinline__ float exp2_of(float x) { return __builtin_amdgcn_exp2f(x); }
@@ -76,8 +130,9 @@ __device__ __forceinline__ float over_groups_sum(float x) {
 
 // Elements from one row of a tile to the next: 16 bytes more than the row, so that the 16 rows
 // that a row-wise operand reads start in 16 different groups of four banks.
-template <typename T, int WIDTH>
-constexpr int kPitch = WIDTH + 16 / static_cast<int>(sizeof(T));
+template <int WIDTH> constexpr int kPitch = WIDTH + 8;
+template <typename T, int ROWS, int WIDTH>
+constexpr int kTileElements = kPlanes<T> * ROWS * kPitch<WIDTH>;
 
 template <typename T>
 __device__ __forceinline__ Frag<T> load8(const T* p) {
@@ -85,49 +140,78 @@ __device__ __forceinline__ Frag<T> load8(const T* p) {
 }
 
 // operand whose summed index runs along the row: row `row0 + c`, columns col0 + 8 g ...
-template <typename T, int WIDTH>
-__device__ __forceinline__ Frag<T> row_operand(const T* tile, int row0, int col0, int lane) {
-  return load8(tile + (row0 + (lane & 15)) * kPitch<T, WIDTH> + col0 + 8 * (lane >> 4));
+template <typename T, int ROWS, int WIDTH>
+__device__ __forceinline__ Operand<T> row_operand(const Stored<T>* tile, int row0, int col0, int lane) {
+  const Stored<T>* at = tile + (row0 + (lane & 15)) * kPitch<WIDTH> + col0 + 8 * (lane >> 4);
+  if constexpr (sizeof(T) == 4) {
+    SplitOperand out;
+#pragma unroll
+    for (int p = 0; p < 3; ++p) out.part[p] = load8(at + p * ROWS * kPitch<WIDTH>);
+    return out;
+  } else {
+    return load8(at);
+  }
 }
 
 // operand whose summed index runs down the rows of the block [row0, row0 + 32): column col0 + c
-template <typename T, int WIDTH>
-__device__ __forceinline__ Frag<T> column_operand(const T* tile, int row0, int col0, int lane) {
-  Frag<T> out;
-  if constexpr (sizeof(T) == 2) {
-    // 16 lanes hand in four rows of 16 elements, 8 bytes each, and get a column each
-    const T* at = tile + (row0 + 4 * (lane >> 4) + ((lane & 15) >> 2)) * kPitch<T, WIDTH> + col0 +
-                  4 * (lane & 3);
+template <typename T, int ROWS, int WIDTH>
+__device__ __forceinline__ Operand<T> column_operand(const Stored<T>* tile, int row0, int col0, int lane) {
+  // 16 lanes hand in four rows of 16 elements, 8 bytes each, and get a column each
+  const Stored<T>* at = tile + (row0 + 4 * (lane >> 4) + ((lane & 15) >> 2)) * kPitch<WIDTH> + col0 +
+                        4 * (lane & 3);
+  const auto read = [](const Stored<T>* from) {
     typedef __attribute__((address_space(3))) s16x4 LdsQuad;
-    const s16x4 low = __builtin_amdgcn_ds_read_tr16_b64_v4i16((LdsQuad*)(at));
-    const s16x4 high =
-        __builtin_amdgcn_ds_read_tr16_b64_v4i16((LdsQuad*)(at + 16 * kPitch<T, WIDTH>));
+    const s16x4 low = __builtin_amdgcn_ds_read_tr16_b64_v4i16((LdsQuad*)(from));
+    const s16x4 high = __builtin_amdgcn_ds_read_tr16_b64_v4i16((LdsQuad*)(from + 16 * kPitch<WIDTH>));
     typedef short s16x8 __attribute__((ext_vector_type(8)));
     const s16x8 both = __builtin_shufflevector(low, high, 0, 1, 2, 3, 4, 5, 6, 7);
-    out = __builtin_bit_cast(Frag<T>, both);
-  } else {
-    const T* at = tile + (row0 + 4 * (lane >> 4)) * kPitch<T, WIDTH> + col0 + (lane & 15);
+    return __builtin_bit_cast(Frag<Stored<T>>, both);
+  };
+  if constexpr (sizeof(T) == 4) {
+    SplitOperand out;
 #pragma unroll
-    for (int e = 0; e < 8; ++e) out[e] = at[((e & 3) + 16 * (e >> 2)) * kPitch<T, WIDTH>];
+    for (int p = 0; p < 3; ++p) out.part[p] = read(at + p * ROWS * kPitch<WIDTH>);
+    return out;
+  } else {
+    return read(at);
   }
-  return out;
 }
 
-// LDS reads and products stay on their side of this point.  Left alone, the compiler puts every
-// read directly in front of its use and the wave waits for LDS each time; the kernels read the
-// operands of one batch of products ahead of the products of the batch before it.
-__device__ __forceinline__ void in_order() { __builtin_amdgcn_sched_barrier(0x476); }
+// N neighbouring values of a row of a tile
+template <typename T, int ROWS, int WIDTH, int N>
+__device__ __forceinline__ void store_row(Stored<T>* tile, int row, int col, const float (&values)[N]) {
+  typedef Stored<T> Part __attribute__((ext_vector_type(N)));
+  Stored<T>* at = tile + row * kPitch<WIDTH> + col;
+  if constexpr (sizeof(T) == 4) {
+    Part part[3];
+    split<N>(values, part);
+#pragma unroll
+    for (int p = 0; p < 3; ++p) *reinterpret_cast<Part*>(at + p * ROWS * kPitch<WIDTH>) = part[p];
+  } else {
+    Part rounded;
+#pragma unroll
+    for (int e = 0; e < N; ++e) rounded[e] = static_cast<T>(values[e]);
+    *reinterpret_cast<Part*>(at) = rounded;
+  }
+}
 
 // two results, rows [0, 16) and [16, 32) of the summed index, as the operand of the next product
 template <typename T>
-__device__ __forceinline__ Frag<T> operand_of(f32x4 low, f32x4 high) {
-  Frag<T> out;
+__device__ __forceinline__ Operand<T> operand_of(f32x4 low, f32x4 high) {
+  if constexpr (sizeof(T) == 4) {
+    const float values[8] = {low[0], low[1], low[2], low[3], high[0], high[1], high[2], high[3]};
+    SplitOperand out;
+    split<8>(values, out.part);
+    return out;
+  } else {
+    Frag<T> out;
 #pragma unroll
-  for (int r = 0; r < 4; ++r) {
-    out[r] = static_cast<T>(low[r]);
-    out[r + 4] = static_cast<T>(high[r]);
+    for (int r = 0; r < 4; ++r) {
+      out[r] = static_cast<T>(low[r]);
+      out[r + 4] = static_cast<T>(high[r]);
+    }
+    return out;
   }
-  return out;
 }
 
 // Rows of a head in memory: `stride` elements apart from `base` on, the last of them number `last`.
@@ -215,12 +299,18 @@ struct TileMove {
     return row < flip ? flip - 1 - row : row;
   }
 
-  __device__ __forceinline__ void store(T* tile, int width, int tid, int flip = 0) {
+  __device__ __forceinline__ void store(Stored<T>* tile, int width, int tid, int flip = 0) {
     clear_padding(width, tid);
 #pragma unroll
-    for (int i = 0; i < kPieces; ++i)
-      *reinterpret_cast<Piece*>(tile + walk_row(row_of(i, tid), flip) * kPitch<T, WIDTH> +
-                                col_of(tid)) = held[i];
+    for (int i = 0; i < kPieces; ++i) {
+      const int row = walk_row(row_of(i, tid), flip);
+      if constexpr (sizeof(T) == 4) {
+        const float values[4] = {held[i][0], held[i][1], held[i][2], held[i][3]};
+        store_row<T, ROWS, WIDTH, 4>(tile, row, col_of(tid), values);
+      } else {
+        *reinterpret_cast<Piece*>(tile + row * kPitch<WIDTH> + col_of(tid)) = held[i];
+      }
+    }
   }
 };
 

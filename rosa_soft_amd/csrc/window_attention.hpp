@@ -147,8 +147,8 @@ template <typename T, int WIDTH, int QUERIES, bool CACHED, bool WHOLE>
 __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(kWaves<T, WIDTH, WHOLE>))) void
 window_forward_kernel(WindowArgs<T> a) {
   constexpr int kSteps = WIDTH / 32, kRows = 64 * QUERIES, kCols = WIDTH / 16;
-  __shared__ __attribute__((aligned(16))) T keys[kKeys * kPitch<T, WIDTH>];
-  __shared__ __attribute__((aligned(16))) T values[kKeys * kPitch<T, WIDTH>];
+  __shared__ __attribute__((aligned(16))) Stored<T> keys[kTileElements<T, kKeys, WIDTH>];
+  __shared__ __attribute__((aligned(16))) Stored<T> values[kTileElements<T, kKeys, WIDTH>];
 
   const int64_t item = item_of_block(a.items);
   if (item >= a.items) return;
@@ -174,21 +174,22 @@ window_forward_kernel(WindowArgs<T> a) {
 
   // this wave's tokens, as the columns of operands
   const int wave_first = first + wave * 16 * QUERIES, wave_last = wave_first + 16 * QUERIES - 1;
-  Frag<T> query[QUERIES][kSteps];
+  Operand<T> query[QUERIES][kSteps];
   const Rows<T> query_rows = a.query.rows(run.batch, run.begin + first - past, head, last - first + 1);
 #pragma unroll
   for (int i = 0; i < QUERIES; ++i) {
     const int row = wave * 16 * QUERIES + i * 16 + column;
 #pragma unroll
     for (int s = 0; s < kSteps; ++s) {
-      query[i][s] = memory_operand<WHOLE>(query_rows, row, s * 32 + 8 * group, a.key_width);
-      clear_operand<WHOLE>(query[i][s], s * 32 + 8 * group, a.key_width);
+      Frag<T> part = memory_operand<WHOLE>(query_rows, row, s * 32 + 8 * group, a.key_width);
+      clear_operand<WHOLE>(part, s * 32 + 8 * group, a.key_width);
+      query[i][s] = as_operand<T>(part);
     }
   }
   f32x4 out[QUERIES][kCols];
   float most[QUERIES];
-  // The sums of the weights: for the 16-bit types a product with ones, which adds what is rounded
-  // and takes no vector instructions (every row of the result is the sum).
+  // The sums of the weights: a product with ones, which adds what is rounded and takes no vector
+  // instructions (every row of the result is the sum).
   f32x4 sum[QUERIES];
 #pragma unroll
   for (int i = 0; i < QUERIES; ++i) {
@@ -220,37 +221,18 @@ window_forward_kernel(WindowArgs<T> a) {
     if (!none) {
       const bool all = end - begin == kKeys && end - 1 <= wave_first && wave_last - begin < a.window;
       f32x4 score[QUERIES][4];
-      Frag<T> key[2][kSteps];
-      const auto read_keys = [&](int k) {
-#pragma unroll
-        for (int s = 0; s < kSteps; ++s)
-          key[k & 1][s] = row_operand<T, WIDTH>(keys, k * 16, s * 32, lane);
-      };
-      read_keys(0);
 #pragma unroll
       for (int k = 0; k < 4; ++k) {
-        if (k + 1 < 4) read_keys(k + 1);
-        in_order();
 #pragma unroll
         for (int i = 0; i < QUERIES; ++i) score[i][k] = f32x4(0.0f);
 #pragma unroll
-        for (int s = 0; s < kSteps; ++s)
+        for (int s = 0; s < kSteps; ++s) {
+          const Operand<T> key = row_operand<T, kKeys, WIDTH>(keys, k * 16, s * 32, lane);
 #pragma unroll
-          for (int i = 0; i < QUERIES; ++i) score[i][k] = mma(key[k & 1][s], query[i][s], score[i][k]);
-        in_order();
+          for (int i = 0; i < QUERIES; ++i) score[i][k] = mma(key, query[i][s], score[i][k]);
+        }
       }
-      // (the first values, for when the weights are there)
-      Frag<T> value[2][2][2];
-      const auto read_values = [&](int d) {
-#pragma unroll
-        for (int half = 0; half < 2; ++half)
-#pragma unroll
-          for (int e = 0; e < 2; ++e)
-            value[d / 2 & 1][half][e] = column_operand<T, WIDTH>(values, half * 32, (d + e) * 16, lane);
-      };
-      read_values(0);
-      in_order();
-      Frag<T> weights[QUERIES][2];
+      Operand<T> weights[QUERIES][2];
       if (!all) {
 #pragma unroll
         for (int i = 0; i < QUERIES; ++i) {
@@ -285,28 +267,21 @@ window_forward_kernel(WindowArgs<T> a) {
 #pragma unroll
           for (int r = 0; r < 4; ++r) {
             score[i][k][r] = exp2_of(score[i][k][r] * factor - base);
-            if constexpr (sizeof(T) == 4) sum[i][r] += score[i][k][r];
           }
 #pragma unroll
         for (int half = 0; half < 2; ++half) {
           weights[i][half] = operand_of<T>(score[i][2 * half], score[i][2 * half + 1]);
-          if constexpr (sizeof(T) == 2)
-            sum[i] = mma(Frag<T>(static_cast<T>(1.0f)), weights[i][half], sum[i]);
+          sum[i] = add_sums<T>(weights[i][half], sum[i]);
         }
       }
 #pragma unroll
-      for (int d = 0; d < kCols; d += 2) {
-        if (d + 2 < kCols) read_values(d + 2);
-        in_order();
+      for (int half = 0; half < 2; ++half)
 #pragma unroll
-        for (int half = 0; half < 2; ++half)
+        for (int d = 0; d < kCols; ++d) {
+          const Operand<T> value = column_operand<T, kKeys, WIDTH>(values, half * 32, d * 16, lane);
 #pragma unroll
-          for (int e = 0; e < 2; ++e)
-#pragma unroll
-            for (int i = 0; i < QUERIES; ++i)
-              out[i][d + e] = mma(value[d / 2 & 1][half][e], weights[i][half], out[i][d + e]);
-        in_order();
-      }
+          for (int i = 0; i < QUERIES; ++i) out[i][d] = mma(value, weights[i][half], out[i][d]);
+        }
     }
     __syncthreads();
   }
@@ -315,8 +290,7 @@ window_forward_kernel(WindowArgs<T> a) {
 #pragma unroll
   for (int i = 0; i < QUERIES; ++i) {
     const int t = wave_first + i * 16 + column;
-    float total = sum[i][0];
-    if constexpr (sizeof(T) == 4) total = over_groups_sum(sum[i][0] + sum[i][1] + sum[i][2] + sum[i][3]);
+    const float total = sum[i][0];
     if (t > last) continue;
     const int64_t token = run.first + t - past;
     T* to = a.out + (token * a.heads + head) * a.value_width;
@@ -333,8 +307,8 @@ template <typename T, int WIDTH, int QUERIES, bool WHOLE>
 __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(kWaves<T, WIDTH, WHOLE>))) void
 window_grad_query_kernel(WindowArgs<T> a) {
   constexpr int kSteps = WIDTH / 32, kRows = 64 * QUERIES, kCols = WIDTH / 16;
-  __shared__ __attribute__((aligned(16))) T keys[kKeys * kPitch<T, WIDTH>];
-  __shared__ __attribute__((aligned(16))) T values[kKeys * kPitch<T, WIDTH>];
+  __shared__ __attribute__((aligned(16))) Stored<T> keys[kTileElements<T, kKeys, WIDTH>];
+  __shared__ __attribute__((aligned(16))) Stored<T> values[kTileElements<T, kKeys, WIDTH>];
 
   const int64_t item = item_of_block(a.items);
   if (item >= a.items) return;
@@ -358,7 +332,7 @@ window_grad_query_kernel(WindowArgs<T> a) {
       history_of<false>(a, a.value, a.value_cache, a.value_width, run, kv_head, 0);
   const int wave_first = first + wave * 16 * QUERIES, wave_last = wave_first + 16 * QUERIES - 1;
 
-  Frag<T> query[QUERIES][kSteps], grad[QUERIES][kSteps];
+  Operand<T> query[QUERIES][kSteps], grad[QUERIES][kSteps];
   float log_sum[QUERIES], delta[QUERIES], unit[QUERIES];
   const int count = last - first + 1;
   const Rows<T> query_rows = a.query.rows(run.batch, run.begin + first, head, count);
@@ -372,14 +346,16 @@ window_grad_query_kernel(WindowArgs<T> a) {
     float dot = 0.0f;
 #pragma unroll
     for (int s = 0; s < kSteps; ++s) {
-      query[i][s] = memory_operand<WHOLE>(query_rows, row, s * 32 + 8 * group, a.key_width);
-      grad[i][s] = memory_operand<WHOLE>(grad_rows, row, s * 32 + 8 * group, a.value_width);
+      Frag<T> part = memory_operand<WHOLE>(query_rows, row, s * 32 + 8 * group, a.key_width);
+      Frag<T> grad_part = memory_operand<WHOLE>(grad_rows, row, s * 32 + 8 * group, a.value_width);
       Frag<T> out = memory_operand<WHOLE>(out_rows, row, s * 32 + 8 * group, a.value_width);
-      clear_operand<WHOLE>(query[i][s], s * 32 + 8 * group, a.key_width);
-      clear_operand<WHOLE>(grad[i][s], s * 32 + 8 * group, a.value_width);
+      clear_operand<WHOLE>(part, s * 32 + 8 * group, a.key_width);
+      clear_operand<WHOLE>(grad_part, s * 32 + 8 * group, a.value_width);
       clear_operand<WHOLE>(out, s * 32 + 8 * group, a.value_width);
 #pragma unroll
-      for (int e = 0; e < 8; ++e) dot += static_cast<float>(grad[i][s][e]) * static_cast<float>(out[e]);
+      for (int e = 0; e < 8; ++e) dot += static_cast<float>(grad_part[e]) * static_cast<float>(out[e]);
+      query[i][s] = as_operand<T>(part);
+      grad[i][s] = as_operand<T>(grad_part);
     }
     delta[i] = over_groups_sum(dot);
     const int64_t at = static_cast<int64_t>(head) * a.sequences.tokens + run.first + first + min(row, count - 1);
@@ -424,8 +400,8 @@ window_grad_query_kernel(WindowArgs<T> a) {
           for (int i = 0; i < QUERIES; ++i) score[i] = slope[i][k] = f32x4(0.0f);
 #pragma unroll
           for (int s = 0; s < kSteps; ++s) {
-            const Frag<T> key = row_operand<T, WIDTH>(keys, half * 32 + k * 16, s * 32, lane);
-            const Frag<T> value = row_operand<T, WIDTH>(values, half * 32 + k * 16, s * 32, lane);
+            const Operand<T> key = row_operand<T, kKeys, WIDTH>(keys, half * 32 + k * 16, s * 32, lane);
+            const Operand<T> value = row_operand<T, kKeys, WIDTH>(values, half * 32 + k * 16, s * 32, lane);
 #pragma unroll
             for (int i = 0; i < QUERIES; ++i) {
               score[i] = mma(key, query[i][s], score[i]);
@@ -447,7 +423,7 @@ window_grad_query_kernel(WindowArgs<T> a) {
             }
           }
         }
-        Frag<T> operand[QUERIES];
+        Operand<T> operand[QUERIES];
 #pragma unroll
         for (int i = 0; i < QUERIES; ++i) {
           if constexpr (kNarrow<T>) {
@@ -468,7 +444,7 @@ window_grad_query_kernel(WindowArgs<T> a) {
         }
 #pragma unroll
         for (int d = 0; d < kCols; ++d) {
-          const Frag<T> key = column_operand<T, WIDTH>(keys, half * 32, d * 16, lane);
+          const Operand<T> key = column_operand<T, kKeys, WIDTH>(keys, half * 32, d * 16, lane);
 #pragma unroll
           for (int i = 0; i < QUERIES; ++i) out[i][d] = mma(key, operand[i], out[i][d]);
         }
@@ -501,8 +477,8 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(WIDTH 
 window_grad_key_kernel(WindowArgs<T> a) {
   constexpr int kSteps = WIDTH / 32, kRows = 64 * KEYS, kCols = WIDTH / 16;
   constexpr int kQueries = sizeof(T) == 4 && WIDTH == 128 ? 32 : 64;  // (registers)
-  __shared__ __attribute__((aligned(16))) T queries[kQueries * kPitch<T, WIDTH>];
-  __shared__ __attribute__((aligned(16))) T grads[kQueries * kPitch<T, WIDTH>];
+  __shared__ __attribute__((aligned(16))) Stored<T> queries[kTileElements<T, kQueries, WIDTH>];
+  __shared__ __attribute__((aligned(16))) Stored<T> grads[kTileElements<T, kQueries, WIDTH>];
   __shared__ __attribute__((aligned(16))) float log_sums[kQueries], deltas[kQueries];
 
   const int64_t item = item_of_block(a.items);
@@ -530,17 +506,19 @@ window_grad_key_kernel(WindowArgs<T> a) {
   const int wave_first = first + wave * 16 * KEYS;
   const Rows<T> key_rows = a.key.rows(run.batch, run.begin + first, kv_head, behind - first);
   const Rows<T> value_rows = a.value.rows(run.batch, run.begin + first, kv_head, behind - first);
-  Frag<T> key[KEYS][kSteps], value[KEYS][kSteps];
+  Operand<T> key[KEYS][kSteps], value[KEYS][kSteps];
   f32x4 grad_key[KEYS][kCols], grad_value[KEYS][kCols];
 #pragma unroll
   for (int i = 0; i < KEYS; ++i) {
     const int row = wave * 16 * KEYS + i * 16 + column;
 #pragma unroll
     for (int step = 0; step < kSteps; ++step) {
-      key[i][step] = memory_operand<WHOLE>(key_rows, row, step * 32 + 8 * group, a.key_width);
-      value[i][step] = memory_operand<WHOLE>(value_rows, row, step * 32 + 8 * group, a.value_width);
-      clear_operand<WHOLE>(key[i][step], step * 32 + 8 * group, a.key_width);
-      clear_operand<WHOLE>(value[i][step], step * 32 + 8 * group, a.value_width);
+      Frag<T> part = memory_operand<WHOLE>(key_rows, row, step * 32 + 8 * group, a.key_width);
+      Frag<T> value_part = memory_operand<WHOLE>(value_rows, row, step * 32 + 8 * group, a.value_width);
+      clear_operand<WHOLE>(part, step * 32 + 8 * group, a.key_width);
+      clear_operand<WHOLE>(value_part, step * 32 + 8 * group, a.value_width);
+      key[i][step] = as_operand<T>(part);
+      value[i][step] = as_operand<T>(value_part);
     }
 #pragma unroll
     for (int d = 0; d < kCols; ++d) grad_key[i][d] = grad_value[i][d] = f32x4(0.0f);
@@ -609,8 +587,8 @@ window_grad_key_kernel(WindowArgs<T> a) {
           for (int i = 0; i < KEYS; ++i) weight[i][k] = slope[i][k] = f32x4(0.0f);
 #pragma unroll
           for (int s = 0; s < kSteps; ++s) {
-            const Frag<T> query = row_operand<T, WIDTH>(queries, row0, s * 32, lane);
-            const Frag<T> grad = row_operand<T, WIDTH>(grads, row0, s * 32, lane);
+            const Operand<T> query = row_operand<T, kQueries, WIDTH>(queries, row0, s * 32, lane);
+            const Operand<T> grad = row_operand<T, kQueries, WIDTH>(grads, row0, s * 32, lane);
 #pragma unroll
             for (int i = 0; i < KEYS; ++i) {
               weight[i][k] = mma(query, key[i][s], weight[i][k]);
@@ -644,7 +622,7 @@ window_grad_key_kernel(WindowArgs<T> a) {
               }
           }
         }
-        Frag<T> weights[KEYS], slopes[KEYS];
+        Operand<T> weights[KEYS], slopes[KEYS];
 #pragma unroll
         for (int i = 0; i < KEYS; ++i) {
           if constexpr (kNarrow<T>) {
@@ -666,8 +644,8 @@ window_grad_key_kernel(WindowArgs<T> a) {
         }
 #pragma unroll
         for (int d = 0; d < kCols; ++d) {
-          const Frag<T> grad = column_operand<T, WIDTH>(grads, half * 32, d * 16, lane);
-          const Frag<T> query = column_operand<T, WIDTH>(queries, half * 32, d * 16, lane);
+          const Operand<T> grad = column_operand<T, kQueries, WIDTH>(grads, half * 32, d * 16, lane);
+          const Operand<T> query = column_operand<T, kQueries, WIDTH>(queries, half * 32, d * 16, lane);
 #pragma unroll
           for (int i = 0; i < KEYS; ++i) {
             grad_value[i][d] = mma(grad, weights[i], grad_value[i][d]);
@@ -706,12 +684,12 @@ window_grad_sinks_kernel(WindowArgs<T> a) {
   constexpr int kSteps = WIDTH / 32, kCols = WIDTH / 16;
   constexpr int kRows = sizeof(T) == 4 ? 64 : 128, kTeams = kRows / 32;  // waves with tokens
   constexpr int kSumPitch = WIDTH + 4;
-  constexpr size_t kTileBytes = sizeof(T) * kRows * kPitch<T, WIDTH>;
+  constexpr size_t kTileBytes = sizeof(Stored<T>) * kTileElements<T, kRows, WIDTH>;
   static_assert(2 * kTileBytes >= sizeof(float) * kTeams * 2 * 16 * kSumPitch, "sums lie over the tiles");
   __shared__ __attribute__((aligned(16))) char shared[2 * kTileBytes];
   __shared__ __attribute__((aligned(16))) float log_sums[kRows], deltas[kRows];
-  T* queries = reinterpret_cast<T*>(shared);
-  T* grads = reinterpret_cast<T*>(shared + kTileBytes);
+  Stored<T>* queries = reinterpret_cast<Stored<T>*>(shared);
+  Stored<T>* grads = reinterpret_cast<Stored<T>*>(shared + kTileBytes);
 
   const int64_t item = item_of_block(a.items);
   if (item >= a.items) return;
@@ -729,16 +707,18 @@ window_grad_sinks_kernel(WindowArgs<T> a) {
   if (from >= to) return;  // (nor are its sums read)
 
   // these tokens see all sinks
-  Frag<T> key[kSteps], value[kSteps];
+  Operand<T> key[kSteps], value[kSteps];
   f32x4 grad_key[kCols], grad_value[kCols];
   const Rows<T> key_rows = a.key.rows(run.batch, run.begin + first, kv_head, a.sinks - first);
   const Rows<T> value_rows = a.value.rows(run.batch, run.begin + first, kv_head, a.sinks - first);
 #pragma unroll
   for (int step = 0; step < kSteps; ++step) {
-    key[step] = memory_operand<WHOLE>(key_rows, column, step * 32 + 8 * group, a.key_width);
-    value[step] = memory_operand<WHOLE>(value_rows, column, step * 32 + 8 * group, a.value_width);
-    clear_operand<WHOLE>(key[step], step * 32 + 8 * group, a.key_width);
-    clear_operand<WHOLE>(value[step], step * 32 + 8 * group, a.value_width);
+    Frag<T> part = memory_operand<WHOLE>(key_rows, column, step * 32 + 8 * group, a.key_width);
+    Frag<T> value_part = memory_operand<WHOLE>(value_rows, column, step * 32 + 8 * group, a.value_width);
+    clear_operand<WHOLE>(part, step * 32 + 8 * group, a.key_width);
+    clear_operand<WHOLE>(value_part, step * 32 + 8 * group, a.value_width);
+    key[step] = as_operand<T>(part);
+    value[step] = as_operand<T>(value_part);
   }
 #pragma unroll
   for (int d = 0; d < kCols; ++d) grad_key[d] = grad_value[d] = f32x4(0.0f);
@@ -768,8 +748,8 @@ window_grad_sinks_kernel(WindowArgs<T> a) {
       weight[k] = slope[k] = f32x4(0.0f);
 #pragma unroll
       for (int s = 0; s < kSteps; ++s) {
-        weight[k] = mma(row_operand<T, WIDTH>(queries, row0 + k * 16, s * 32, lane), key[s], weight[k]);
-        slope[k] = mma(row_operand<T, WIDTH>(grads, row0 + k * 16, s * 32, lane), value[s], slope[k]);
+        weight[k] = mma(row_operand<T, kRows, WIDTH>(queries, row0 + k * 16, s * 32, lane), key[s], weight[k]);
+        slope[k] = mma(row_operand<T, kRows, WIDTH>(grads, row0 + k * 16, s * 32, lane), value[s], slope[k]);
       }
       const int row = row0 + k * 16 + 4 * group;
       const f32x4 log_sum = *reinterpret_cast<const f32x4*>(log_sums + row);
@@ -793,11 +773,12 @@ window_grad_sinks_kernel(WindowArgs<T> a) {
       slope[0] *= unit;
       slope[1] *= unit;
     }
-    const Frag<T> weights = operand_of<T>(weight[0], weight[1]), slopes = operand_of<T>(slope[0], slope[1]);
+    const Operand<T> weights = operand_of<T>(weight[0], weight[1]);
+    const Operand<T> slopes = operand_of<T>(slope[0], slope[1]);
 #pragma unroll
     for (int d = 0; d < kCols; ++d) {
-      grad_value[d] = mma(column_operand<T, WIDTH>(grads, row0, d * 16, lane), weights, grad_value[d]);
-      grad_key[d] = mma(column_operand<T, WIDTH>(queries, row0, d * 16, lane), slopes, grad_key[d]);
+      grad_value[d] = mma(column_operand<T, kRows, WIDTH>(grads, row0, d * 16, lane), weights, grad_value[d]);
+      grad_key[d] = mma(column_operand<T, kRows, WIDTH>(queries, row0, d * 16, lane), slopes, grad_key[d]);
     }
   }
 
@@ -910,14 +891,14 @@ window_token_kernel(TokenArgs<T> args) {
   constexpr int kPieces = kTile * kPerRow / 64;
   typedef T Piece __attribute__((ext_vector_type(kElements)));
   const WindowArgs<T>& a = args.window;
-  constexpr size_t kTileBytes = sizeof(T) * kTile * kPitch<T, WIDTH>;
+  constexpr size_t kTileBytes = sizeof(Stored<T>) * kTileElements<T, kTile, WIDTH>;
   constexpr size_t kJoinBytes = sizeof(float) * 16 * (WIDTH + 4);
   __shared__ __attribute__((aligned(16))) char shared[4 * (kTileBytes > kJoinBytes ? kTileBytes : kJoinBytes)];
   __shared__ float tops[4][16], totals[4][16];
 
   const int tid = threadIdx.x, lane = tid & 63, group = lane >> 4, column = lane & 15;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  T* values = reinterpret_cast<T*>(shared) + wave * kTile * kPitch<T, WIDTH>;
+  Stored<T>* values = reinterpret_cast<Stored<T>*>(shared) + wave * kTileElements<T, kTile, WIDTH>;
   const int split = blockIdx.x % args.splits;
   const int head_block = blockIdx.x / args.splits % args.head_blocks;
   const int kv_head = blockIdx.x / args.splits / args.head_blocks % a.kv_heads;
@@ -945,11 +926,12 @@ window_token_kernel(TokenArgs<T> args) {
   // this column's member of the group of query heads (the last one again beyond it)
   const int head = kv_head * a.share + min(head_block * 16 + column, a.share - 1);
   const Rows<T> query_row = {a.query.row(slot, 0, head), 0, 0};
-  Frag<T> query[kSteps];
+  Operand<T> query[kSteps];
 #pragma unroll
   for (int s = 0; s < kSteps; ++s) {
-    query[s] = memory_operand<WHOLE>(query_row, 0, s * 32 + 8 * group, a.key_width);
-    clear_operand<WHOLE>(query[s], s * 32 + 8 * group, a.key_width);
+    Frag<T> part = memory_operand<WHOLE>(query_row, 0, s * 32 + 8 * group, a.key_width);
+    clear_operand<WHOLE>(part, s * 32 + 8 * group, a.key_width);
+    query[s] = as_operand<T>(part);
   }
   f32x4 out[kCols];
 #pragma unroll
@@ -989,15 +971,17 @@ window_token_kernel(TokenArgs<T> args) {
 #pragma unroll
       for (int s = 0; s < kSteps; ++s) {
         clear_operand<WHOLE>(key[k][s], s * 32 + 8 * group, a.key_width);
-        score[k] = mma(key[k][s], query[s], score[k]);
+        score[k] = mma(as_operand<T>(key[k][s]), query[s], score[k]);
       }
     }
     // (LDS accesses of one wave are carried out in order: its tile needs no barrier)
 #pragma unroll
     for (int i = 0; i < kPieces; ++i) {
       const int piece = i * 64 + lane;
-      *reinterpret_cast<Piece*>(values + piece / kPerRow * kPitch<T, WIDTH> +
-                                piece % kPerRow * kElements) = held[i];
+      float part[kElements];
+#pragma unroll
+      for (int e = 0; e < kElements; ++e) part[e] = static_cast<float>(held[i][e]);
+      store_row<T, kTile, WIDTH>(values, piece / kPerRow, piece % kPerRow * kElements, part);
     }
     asm volatile("" ::: "memory");
     if (tile + 4 < tile_end) fetch(tile + 4);
@@ -1026,10 +1010,10 @@ window_token_kernel(TokenArgs<T> args) {
         score[k][r] = exp2_of(score[k][r] * factor - base);
         sum += score[k][r];
       }
-    const Frag<T> weights = operand_of<T>(score[0], score[1]);
+    const Operand<T> weights = operand_of<T>(score[0], score[1]);
 #pragma unroll
     for (int d = 0; d < kCols; ++d)
-      out[d] = mma(column_operand<T, WIDTH>(values, 0, d * 16, lane), weights, out[d]);
+      out[d] = mma(column_operand<T, kTile, WIDTH>(values, 0, d * 16, lane), weights, out[d]);
     asm volatile("" ::: "memory");
   }
   sum = over_groups_sum(sum);
@@ -1140,10 +1124,11 @@ WindowArgs<T> window_args(const WindowCall& call) {
   return args;
 }
 
-// Tokens (in sixteens) of a wave.
-template <typename T, int WIDTH> constexpr int kForwardQueries = sizeof(T) == 4 && WIDTH == 128 ? 1 : 2;
-template <typename T, int WIDTH> constexpr int kGradQueries = sizeof(T) == 4 && WIDTH == 128 ? 1 : 2;
-template <typename T, int WIDTH> constexpr int kGradKeys = sizeof(T) == 4 && WIDTH == 128 ? 1 : 2;
+// Tokens or keys (in sixteens) of a wave: two, so that an operand read from LDS serves two products;
+// one where two would leave compute units idle (fewer than kFull blocks), and where two do not
+// fit the registers (float32, 128 columns).
+constexpr int64_t kFull = 512;
+template <typename T, int WIDTH> constexpr bool kPairs = !(sizeof(T) == 4 && WIDTH == 128);
 
 template <typename T>
 bool whole_inputs(const WindowCall& call) {
@@ -1155,13 +1140,21 @@ bool whole_inputs(const WindowCall& call) {
          aligned(call.output) && aligned(call.key_cache) && aligned(call.value_cache);
 }
 
-template <typename T, int WIDTH, bool CACHED, bool WHOLE>
+template <typename T, int WIDTH, int QUERIES, bool CACHED, bool WHOLE>
 void window_forward_launch(WindowArgs<T>& args, hipStream_t stream) {
-  constexpr int kQueries = kForwardQueries<T, WIDTH>;
-  args.slots = slots_of(args.sequences, 64 * kQueries);
+  args.slots = slots_of(args.sequences, 64 * QUERIES);
   args.items = args.slots * args.heads;
-  window_forward_kernel<T, WIDTH, kQueries, CACHED, WHOLE>
+  window_forward_kernel<T, WIDTH, QUERIES, CACHED, WHOLE>
       <<<dim3(static_cast<unsigned>(grid_of(args.items))), kThreads, 0, stream>>>(args);
+}
+
+template <typename T, int WIDTH, bool CACHED, bool WHOLE>
+void window_forward_rows(WindowArgs<T>& args, hipStream_t stream) {
+  if constexpr (kPairs<T, WIDTH>) {
+    if (slots_of(args.sequences, 128) * args.heads >= kFull)
+      return window_forward_launch<T, WIDTH, 2, CACHED, WHOLE>(args, stream);
+  }
+  window_forward_launch<T, WIDTH, 1, CACHED, WHOLE>(args, stream);
 }
 
 template <typename T, bool WHOLE>
@@ -1169,9 +1162,9 @@ void window_forward_width(const WindowCall& call) {
   WindowArgs<T> args = window_args<T>(call);
   const rosa_mixer_problem& p = *call.problem;
   switch (padded_width(p.D > p.Dv ? p.D : p.Dv)) {
-    case 32: return window_forward_launch<T, 32, false, WHOLE>(args, call.stream);
-    case 64: return window_forward_launch<T, 64, false, WHOLE>(args, call.stream);
-    default: return window_forward_launch<T, 128, false, WHOLE>(args, call.stream);
+    case 32: return window_forward_rows<T, 32, false, WHOLE>(args, call.stream);
+    case 64: return window_forward_rows<T, 64, false, WHOLE>(args, call.stream);
+    default: return window_forward_rows<T, 128, false, WHOLE>(args, call.stream);
   }
 }
 
@@ -1183,15 +1176,17 @@ void window_forward(const WindowCall& call) {
     window_forward_width<T, false>(call);
 }
 
-template <typename T, int WIDTH, bool WHOLE>
-void window_backward_launch(WindowArgs<T>& args, hipStream_t stream) {
-  constexpr int kQueries = kGradQueries<T, WIDTH>, kWaveKeys = kGradKeys<T, WIDTH>;
-  args.slots = slots_of(args.sequences, 64 * kQueries);
+template <typename T, int WIDTH, int QUERIES, bool WHOLE>
+void window_grad_query_launch(WindowArgs<T>& args, hipStream_t stream) {
+  args.slots = slots_of(args.sequences, 64 * QUERIES);
   args.items = args.slots * args.heads;
-  window_grad_query_kernel<T, WIDTH, kQueries, WHOLE>
+  window_grad_query_kernel<T, WIDTH, QUERIES, WHOLE>
       <<<dim3(static_cast<unsigned>(grid_of(args.items))), kThreads, 0, stream>>>(args);
-  if (args.grad_key == nullptr && args.grad_value == nullptr) return;
-  args.key_block = 64 * kWaveKeys;
+}
+
+template <typename T, int WIDTH, int KEYS, bool WHOLE>
+void window_grad_key_launch(WindowArgs<T>& args, hipStream_t stream) {
+  args.key_block = 64 * KEYS;
   if (args.sink_slots > 0) {
     args.items = args.sink_slots * args.heads * ((args.sinks + 15) / 16);
     window_grad_sinks_kernel<T, WIDTH, WHOLE>
@@ -1201,10 +1196,23 @@ void window_backward_launch(WindowArgs<T>& args, hipStream_t stream) {
         <<<dim3(static_cast<unsigned>((size + kThreads - 1) / kThreads * args.kv_heads * args.sequences.count)),
            kThreads, 0, stream>>>(args);
   }
-  args.slots = slots_of(args.sequences, 64 * kWaveKeys);
+  args.slots = slots_of(args.sequences, args.key_block);
   args.items = args.slots * args.kv_heads;
-  window_grad_key_kernel<T, WIDTH, kWaveKeys, WHOLE>
+  window_grad_key_kernel<T, WIDTH, KEYS, WHOLE>
       <<<dim3(static_cast<unsigned>(grid_of(args.items))), kThreads, 0, stream>>>(args);
+}
+
+template <typename T, int WIDTH, bool WHOLE>
+void window_backward_launch(WindowArgs<T>& args, hipStream_t stream) {
+  if (kPairs<T, WIDTH> && slots_of(args.sequences, 128) * args.heads >= kFull)
+    window_grad_query_launch<T, WIDTH, kPairs<T, WIDTH> ? 2 : 1, WHOLE>(args, stream);
+  else
+    window_grad_query_launch<T, WIDTH, 1, WHOLE>(args, stream);
+  if (args.grad_key == nullptr && args.grad_value == nullptr) return;
+  if (kPairs<T, WIDTH> && slots_of(args.sequences, 128) * args.kv_heads >= kFull / 4)
+    window_grad_key_launch<T, WIDTH, kPairs<T, WIDTH> ? 2 : 1, WHOLE>(args, stream);
+  else
+    window_grad_key_launch<T, WIDTH, 1, WHOLE>(args, stream);
 }
 
 template <typename T, bool WHOLE>
@@ -1254,7 +1262,7 @@ void window_update_launch(WindowArgs<T>& args, const WindowCall& call) {
           token.partial, args.out, plan.splits, p.Dv);
     return;
   }
-  window_forward_launch<T, WIDTH, true, WHOLE>(args, call.stream);
+  window_forward_rows<T, WIDTH, true, WHOLE>(args, call.stream);
   const int64_t blocks = slots_of(args.sequences, 64) * p.Hkv;
   window_append_kernel<T, WHOLE>
       <<<dim3(static_cast<unsigned>(blocks)), kThreads, 0, call.stream>>>(args, key_cache, value_cache);

@@ -235,7 +235,7 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2))) v
             term[e] = static_cast<ST>(left[e]);
             left[e] -= static_cast<float>(term[e]);
           }
-          *reinterpret_cast<Piece*>(weighted + t * kTerm + row * kPitch<SLICE> + value_move.col_of(tid)) = term;
+          *reinterpret_cast<Piece*>(weighted + t * kTerm + row * kPitch<ST, SLICE> + value_move.col_of(tid)) = term;
         }
       }
     }

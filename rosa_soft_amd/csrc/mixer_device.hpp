@@ -128,11 +128,13 @@ __device__ __forceinline__ float over_groups_sum(float x) {
 // tiles
 // ---------------------------------------------------------------------------
 
-// Elements from one row of a tile to the next: 16 bytes more than the row, so that the 16 rows
-// that a row-wise operand reads start in 16 different groups of four banks.
-template <int WIDTH> constexpr int kPitch = WIDTH + 8;
+// Elements from one row of a tile to the next: 32 bytes more than the row, so that eight rows lie
+// in eight different eighths of the 64 banks and both kinds of operand are read without bank
+// conflicts (16 bytes: half of the LDS time of every kernel was conflicts).  The three planes of
+// float32 tiles have room for 16.
+template <typename T, int WIDTH> constexpr int kPitch = WIDTH + (sizeof(T) == 4 ? 8 : 16);
 template <typename T, int ROWS, int WIDTH>
-constexpr int kTileElements = kPlanes<T> * ROWS * kPitch<WIDTH>;
+constexpr int kTileElements = kPlanes<T> * ROWS * kPitch<T, WIDTH>;
 
 template <typename T>
 __device__ __forceinline__ Frag<T> load8(const T* p) {
@@ -142,11 +144,11 @@ __device__ __forceinline__ Frag<T> load8(const T* p) {
 // operand whose summed index runs along the row: row `row0 + c`, columns col0 + 8 g ...
 template <typename T, int ROWS, int WIDTH>
 __device__ __forceinline__ Operand<T> row_operand(const Stored<T>* tile, int row0, int col0, int lane) {
-  const Stored<T>* at = tile + (row0 + (lane & 15)) * kPitch<WIDTH> + col0 + 8 * (lane >> 4);
+  const Stored<T>* at = tile + (row0 + (lane & 15)) * kPitch<T, WIDTH> + col0 + 8 * (lane >> 4);
   if constexpr (sizeof(T) == 4) {
     SplitOperand out;
 #pragma unroll
-    for (int p = 0; p < 3; ++p) out.part[p] = load8(at + p * ROWS * kPitch<WIDTH>);
+    for (int p = 0; p < 3; ++p) out.part[p] = load8(at + p * ROWS * kPitch<T, WIDTH>);
     return out;
   } else {
     return load8(at);
@@ -157,12 +159,12 @@ __device__ __forceinline__ Operand<T> row_operand(const Stored<T>* tile, int row
 template <typename T, int ROWS, int WIDTH>
 __device__ __forceinline__ Operand<T> column_operand(const Stored<T>* tile, int row0, int col0, int lane) {
   // 16 lanes hand in four rows of 16 elements, 8 bytes each, and get a column each
-  const Stored<T>* at = tile + (row0 + 4 * (lane >> 4) + ((lane & 15) >> 2)) * kPitch<WIDTH> + col0 +
+  const Stored<T>* at = tile + (row0 + 4 * (lane >> 4) + ((lane & 15) >> 2)) * kPitch<T, WIDTH> + col0 +
                         4 * (lane & 3);
   const auto read = [](const Stored<T>* from) {
     typedef __attribute__((address_space(3))) s16x4 LdsQuad;
     const s16x4 low = __builtin_amdgcn_ds_read_tr16_b64_v4i16((LdsQuad*)(from));
-    const s16x4 high = __builtin_amdgcn_ds_read_tr16_b64_v4i16((LdsQuad*)(from + 16 * kPitch<WIDTH>));
+    const s16x4 high = __builtin_amdgcn_ds_read_tr16_b64_v4i16((LdsQuad*)(from + 16 * kPitch<T, WIDTH>));
     typedef short s16x8 __attribute__((ext_vector_type(8)));
     const s16x8 both = __builtin_shufflevector(low, high, 0, 1, 2, 3, 4, 5, 6, 7);
     return __builtin_bit_cast(Frag<Stored<T>>, both);
@@ -170,7 +172,7 @@ __device__ __forceinline__ Operand<T> column_operand(const Stored<T>* tile, int 
   if constexpr (sizeof(T) == 4) {
     SplitOperand out;
 #pragma unroll
-    for (int p = 0; p < 3; ++p) out.part[p] = read(at + p * ROWS * kPitch<WIDTH>);
+    for (int p = 0; p < 3; ++p) out.part[p] = read(at + p * ROWS * kPitch<T, WIDTH>);
     return out;
   } else {
     return read(at);
@@ -181,12 +183,12 @@ __device__ __forceinline__ Operand<T> column_operand(const Stored<T>* tile, int 
 template <typename T, int ROWS, int WIDTH, int N>
 __device__ __forceinline__ void store_row(Stored<T>* tile, int row, int col, const float (&values)[N]) {
   typedef Stored<T> Part __attribute__((ext_vector_type(N)));
-  Stored<T>* at = tile + row * kPitch<WIDTH> + col;
+  Stored<T>* at = tile + row * kPitch<T, WIDTH> + col;
   if constexpr (sizeof(T) == 4) {
     Part part[3];
     split<N>(values, part);
 #pragma unroll
-    for (int p = 0; p < 3; ++p) *reinterpret_cast<Part*>(at + p * ROWS * kPitch<WIDTH>) = part[p];
+    for (int p = 0; p < 3; ++p) *reinterpret_cast<Part*>(at + p * ROWS * kPitch<T, WIDTH>) = part[p];
   } else {
     Part rounded;
 #pragma unroll
@@ -308,7 +310,7 @@ struct TileMove {
         const float values[4] = {held[i][0], held[i][1], held[i][2], held[i][3]};
         store_row<T, ROWS, WIDTH, 4>(tile, row, col_of(tid), values);
       } else {
-        *reinterpret_cast<Piece*>(tile + row * kPitch<WIDTH> + col_of(tid)) = held[i];
+        *reinterpret_cast<Piece*>(tile + row * kPitch<T, WIDTH> + col_of(tid)) = held[i];
       }
     }
   }

@@ -181,14 +181,10 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2))) v
   const auto store_ready = [&] {
     if (ready_at < 0 || ready_at + own >= stop) return;
     const int64_t row = ((run.first + token(ready_at + own) - run.begin) * a.heads + head) * p.value_width + col0;
-    const bool quads = WHOLE || p.value_width % 4 == 0;
-#pragma unroll
-    for (int t = 0; t < kColTiles; ++t) {
-      if (p.partial != nullptr)
-        store4(p.partial + row, t * 16 + 4 * group, ready[t], p.value_width - col0, quads);
-      else
-        store4(p.out + row, t * 16 + 4 * group, ready[t], p.value_width - col0, quads);
-    }
+    if (p.partial != nullptr)
+      store_tiles<WHOLE>(p.partial + row, ready, 1.0f, group, p.value_width - col0);
+    else
+      store_tiles<WHOLE>(p.out + row, ready, 1.0f, group, p.value_width - col0);
   };
 
   float unit = 1.0f;  // float16: brings the rounded state into range

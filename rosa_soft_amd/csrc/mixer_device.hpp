@@ -364,10 +364,58 @@ __device__ __forceinline__ void store4(T* row, int col, f32x4 value, int width, 
   }
 }
 
+// float16 has few exponents (see lift_of)
+template <typename T> constexpr bool kNarrow = std::is_same_v<T, _Float16>;
+
+// A result of TILES tiles of 16 columns, times `by`, to a row of an output.  Where rows are whole
+// 16-byte pieces of 16-bit elements, the lanes of a column exchange their quads of two neighbouring
+// tiles: each has a whole piece then, and a store fills 64 bytes of a row instead of 32.  The
+// products are rounded to float32 first in either form (left to itself the compiler makes one
+// float16 instruction of product and rounding in one of them, and strides would change results).
+template <bool WHOLE, typename T, int TILES>
+__device__ __forceinline__ void store_tiles(T* row, const f32x4 (&value)[TILES], float by, int group,
+                                            int width) {
+  f32x4 scaled[TILES];
+#pragma unroll
+  for (int t = 0; t < TILES; ++t)
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      float product = value[t][e] * by;
+      if constexpr (kNarrow<T>) asm("" : "+v"(product));
+      scaled[t][e] = product;
+    }
+  if constexpr (WHOLE && sizeof(T) == 2) {
+    static_assert(TILES % 2 == 0, "tiles are stored in pairs");
+    const int col = (group & 1) * 16 + (group >> 1) * 8;
+#pragma unroll
+    for (int t = 0; t < TILES; t += 2) {
+      typedef unsigned u32x2 __attribute__((ext_vector_type(2)));
+      typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
+      Quad<T> quad[2];
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) quad[h][e] = static_cast<T>(scaled[t + h][e]);
+      const u32x2 low = __builtin_bit_cast(u32x2, quad[0]), high = __builtin_bit_cast(u32x2, quad[1]);
+      u32x4 piece;
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        const auto swapped = __builtin_amdgcn_permlane16_swap(low[e], high[e], false, false);
+        piece[e] = swapped[0];
+        piece[2 + e] = swapped[1];
+      }
+      if (t * 16 + col < width) *reinterpret_cast<u32x4*>(row + t * 16 + col) = piece;
+    }
+  } else {
+#pragma unroll
+    for (int t = 0; t < TILES; ++t)
+      store4(row, t * 16 + 4 * group, scaled[t], width, WHOLE || width % 4 == 0);
+  }
+}
+
 // The power of two that brings a largest value into float16's upper range, [2^13, 2^14): float16
 // has few exponents, and what is rounded to it loses bits below 2^-14 and everything above 2^16.
 // The other types take values as they are.
-template <typename T> constexpr bool kNarrow = std::is_same_v<T, _Float16>;
 __device__ __forceinline__ float lift_of(float largest) {
   return largest > 0.0f && largest < __builtin_inff() ? exp2_of(13.0f - floorf(log2_of(largest)))
                                                       : 1.0f;

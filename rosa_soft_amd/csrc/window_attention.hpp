@@ -286,7 +286,6 @@ window_forward_kernel(WindowArgs<T> a) {
     __syncthreads();
   }
 
-  const bool quads = WHOLE || a.value_width % 4 == 0;
 #pragma unroll
   for (int i = 0; i < QUERIES; ++i) {
     const int t = wave_first + i * 16 + column;
@@ -295,8 +294,7 @@ window_forward_kernel(WindowArgs<T> a) {
     const int64_t token = run.first + t - past;
     T* to = a.out + (token * a.heads + head) * a.value_width;
     const float by = 1.0f / total;
-#pragma unroll
-    for (int d = 0; d < kCols; ++d) store4(to, d * 16 + 4 * group, out[i][d] * by, a.value_width, quads);
+    store_tiles<WHOLE>(to, out[i], by, group, a.value_width);
     if (a.log_sum != nullptr && group == 0)
       a.log_sum[static_cast<int64_t>(head) * a.sequences.tokens + token] = most[i] + log2_of(total) - kLift<T>;
   }
@@ -452,15 +450,13 @@ window_grad_query_kernel(WindowArgs<T> a) {
     }
     __syncthreads();
   }
-  const bool quads = WHOLE || a.key_width % 4 == 0;
 #pragma unroll
   for (int i = 0; i < QUERIES; ++i) {
     const int t = wave_first + i * 16 + column;
     if (t > last) continue;
     T* to = a.grad_query + ((run.first + t) * a.heads + head) * a.key_width;
     const float by = unit[i] == 0.0f ? a.scale : a.scale / unit[i];
-#pragma unroll
-    for (int d = 0; d < kCols; ++d) store4(to, d * 16 + 4 * group, out[i][d] * by, a.key_width, quads);
+    store_tiles<WHOLE>(to, out[i], by, group, a.key_width);
   }
 }
 
@@ -663,15 +659,11 @@ window_grad_key_kernel(WindowArgs<T> a) {
     if (s >= behind) continue;
     const float back = unit[i] == 0.0f ? 1.0f : 1.0f / unit[i];
     const int64_t row = (run.first + s) * a.kv_heads + kv_head;
-#pragma unroll
-    for (int d = 0; d < kCols; ++d) {
-      if (a.grad_key != nullptr)
-        store4(a.grad_key + row * a.key_width, d * 16 + 4 * group,
-               grad_key[i][d] * (a.scale * back * kUnlift<T>), a.key_width, WHOLE || a.key_width % 4 == 0);
-      if (a.grad_value != nullptr)
-        store4(a.grad_value + row * a.value_width, d * 16 + 4 * group, grad_value[i][d] * kUnlift<T>,
-               a.value_width, WHOLE || a.value_width % 4 == 0);
-    }
+    if (a.grad_key != nullptr)
+      store_tiles<WHOLE>(a.grad_key + row * a.key_width, grad_key[i], a.scale * back * kUnlift<T>, group,
+                         a.key_width);
+    if (a.grad_value != nullptr)
+      store_tiles<WHOLE>(a.grad_value + row * a.value_width, grad_value[i], kUnlift<T>, group, a.value_width);
   }
 }
 

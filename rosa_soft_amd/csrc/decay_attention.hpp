@@ -70,10 +70,12 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2))) v
   if (item >= a.items) return;
   const int tid = threadIdx.x, lane = tid & 63, group = lane >> 4, column = lane & 15;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  // Neighbours on one XCD, whose cache they share: the slices of a sequence, which read the same
+  // keys and queries, then the passes, which read the same four tensors.
   const int slice = static_cast<int>(item % a.slices);
-  const int64_t slot = item / a.slices % a.slots;
-  const int head = static_cast<int>(item / a.slices / a.slots % a.heads);
-  const int pass_index = static_cast<int>(item / a.slices / a.slots / a.heads);
+  const int pass_index = static_cast<int>(item / a.slices % a.passes);
+  const int64_t slot = item / a.slices / a.passes % a.slots;
+  const int head = static_cast<int>(item / a.slices / a.passes / a.slots);
   const DecayPass<T>& p = a.pass[pass_index];
   const int col0 = slice * SLICE;
   if (col0 >= p.value_width) return;
@@ -150,16 +152,18 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2))) v
   TileMove<T, kChunk, WIDTH, WHOLE> key_move;
   TileMove<T, kChunk, SLICE, WHOLE> value_move;
   Frag<T> next_query[kSteps];
+  const Rows<T> key_rows = p.key.rows(run.batch, run.begin, key_head, run.length),
+                value_rows = p.value.rows(run.batch, run.begin, value_head, run.length, col0);
+  Rows<T> query_rows{};
+  if constexpr (!STATE_ONLY) query_rows = p.query.rows(run.batch, run.begin, query_head, run.length);
   const auto fetch = [&](int at) {
     // the chunk's tokens as they lie in memory
     const int fill = min(kChunk, stop - at);
-    const int64_t first = run.begin + (p.reverse ? run.length - at - fill : at);
-    key_move.fetch(p.key.rows(run.batch, first, key_head, fill), p.key_width, tid);
-    Rows<T> values_here = p.value.rows(run.batch, first, value_head, fill);
-    values_here.base += col0;
-    value_move.fetch(values_here, p.value_width - col0, tid);
+    const int first = p.reverse ? run.length - at - fill : at;
+    key_move.fetch(rows_from(key_rows, first, fill), p.key_width, tid);
+    value_move.fetch(rows_from(value_rows, first, fill), p.value_width - col0, tid);
     if constexpr (!STATE_ONLY) {
-      const Rows<T> queries = p.query.rows(run.batch, first, query_head, fill);
+      const Rows<T> queries = rows_from(query_rows, first, fill);
       const int row = p.reverse ? max(fill - 1 - own, 0) : own;
 #pragma unroll
       for (int s = 0; s < kSteps; ++s)
@@ -255,7 +259,7 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2))) v
     if constexpr (!STATE_ONLY) {
 #pragma unroll
       for (int s = 0; s < kSteps; ++s) {
-        clear_operand<WHOLE>(next_query[s], s * 32 + 8 * group, p.key_width);
+        clear_operand<WHOLE>(next_query[s], s * 32, group, p.key_width);
         query[s] = as_operand<T>(next_query[s]);
       }
     }
@@ -518,11 +522,10 @@ __global__ __launch_bounds__(kThreads) void decay_token_kernel(DecayTokenArgs<T>
 
 template <typename T, int WIDTH, int TERMS, bool WHOLE>
 void decay_walk(DecayArgs<T>& args, const DecayPlan& plan, hipStream_t stream) {
-  constexpr int kSlice = WIDTH < 64 ? WIDTH : 64;
-  int widest = 0;
+  constexpr int kSlice = decay_slice(WIDTH);
+  args.slices = 0;
   for (int i = 0; i < args.passes; ++i)
-    widest = args.pass[i].value_width > widest ? args.pass[i].value_width : widest;
-  args.slices = (widest + kSlice - 1) / kSlice;
+    args.slices = std::max(args.slices, (args.pass[i].value_width + kSlice - 1) / kSlice);
   args.segment = plan.segment;
   args.slots = plan.slots;
   args.items = args.passes * plan.slots * args.heads * args.slices;
@@ -540,9 +543,8 @@ void decay_walk(DecayArgs<T>& args, const DecayPlan& plan, hipStream_t stream) {
 }
 
 template <typename T, int TERMS, bool WHOLE>
-void decay_walk_width(DecayArgs<T>& args, const DecayPlan& plan, const rosa_mixer_problem& p,
-                      hipStream_t stream) {
-  switch (padded_width(p.D > p.Dv ? p.D : p.Dv)) {
+void decay_walk_width(DecayArgs<T>& args, const DecayPlan& plan, hipStream_t stream) {
+  switch (plan.width) {
     case 32: return decay_walk<T, 32, TERMS, WHOLE>(args, plan, stream);
     case 64: return decay_walk<T, 64, TERMS, WHOLE>(args, plan, stream);
     default: return decay_walk<T, 128, TERMS, WHOLE>(args, plan, stream);
@@ -550,12 +552,11 @@ void decay_walk_width(DecayArgs<T>& args, const DecayPlan& plan, const rosa_mixe
 }
 
 template <typename T, int TERMS>
-void decay_walk_any(DecayArgs<T>& args, const DecayPlan& plan, const rosa_mixer_problem& p, bool whole,
-                    hipStream_t stream) {
+void decay_walk_any(DecayArgs<T>& args, const DecayPlan& plan, bool whole, hipStream_t stream) {
   if (whole)
-    decay_walk_width<T, TERMS, true>(args, plan, p, stream);
+    decay_walk_width<T, TERMS, true>(args, plan, stream);
   else
-    decay_walk_width<T, TERMS, false>(args, plan, p, stream);
+    decay_walk_width<T, TERMS, false>(args, plan, stream);
 }
 
 template <typename T>
@@ -595,7 +596,7 @@ void decay_forward(const DecayCall& call) {
   args.passes = 1;
   args.pass[0] = decay_forward_pass<T>(call);
   args.segment_states = reinterpret_cast<float*>(call.workspace);
-  decay_walk_any<T, kTrainTerms<T>>(args, plan, *call.problem, whole_inputs<T>(call), call.stream);
+  decay_walk_any<T, kTrainTerms<T>>(args, plan, whole_inputs<T>(call), call.stream);
 }
 
 template <typename T>
@@ -626,7 +627,7 @@ void decay_backward(const DecayCall& call) {
     args.pass[args.passes++] = {k, q, go, share, 1, 1, p.D, p.Dv,
                                 static_cast<T*>(call.grad_value), value_partial, true};
   }
-  decay_walk_any<T, kTrainTerms<T>>(args, plan, p, whole_inputs<T>(call), call.stream);
+  decay_walk_any<T, kTrainTerms<T>>(args, plan, whole_inputs<T>(call), call.stream);
   const int64_t rows = static_cast<int64_t>(p.N) * p.Hkv;
   const auto blocks = [&](int width) {
     return dim3(static_cast<unsigned>((rows * width + kThreads - 1) / kThreads));
@@ -666,7 +667,7 @@ void decay_update(const DecayCall& call) {
   args.segment_states = reinterpret_cast<float*>(call.workspace);
   args.state_in = call.state_in;
   args.state_out = call.state_out;
-  decay_walk_any<T, kUpdateTerms<T>>(args, plan, p, whole_inputs<T>(call), call.stream);
+  decay_walk_any<T, kUpdateTerms<T>>(args, plan, whole_inputs<T>(call), call.stream);
 }
 
 }  // namespace rosa_mixer

@@ -46,7 +46,9 @@ struct DecayCall {
 };
 
 // Work division, on the host alone.
+constexpr int decay_slice(int width) { return width < 64 ? width : 64; }  // value columns of a block
 struct DecayPlan {
+  int width;            // padded width of keys
   int segment;          // tokens of a segment; >= the longest sequence where there is but one
   bool segmented;
   int64_t slots;

@@ -224,6 +224,12 @@ struct Rows {
   int last;
 };
 
+// `count` of them from number `first` on
+template <typename T>
+__device__ __forceinline__ Rows<T> rows_from(const Rows<T>& rows, int first, int count) {
+  return {rows.base + first * rows.stride, rows.stride, count - 1};
+}
+
 // Where element `col` of a row lies.  WHOLE: the stride is below 2^24 bytes, so that a 32-bit
 // offset from a base that the whole block shares is enough: no 64-bit arithmetic per load.
 template <bool WHOLE, typename T>
@@ -281,18 +287,17 @@ struct TileMove {
   // Columns from `width` on become zeros here, not where the loads were issued: touching a loaded
   // register there would wait for it.
   __device__ __forceinline__ void clear_padding(int width, int tid) {
+    if (width >= WIDTH) return;  // (a branch of the whole block; selects would cost every full tile)
     const int col = col_of(tid);
-    if constexpr (WHOLE) {  // (all of a piece or nothing)
-      if (col >= width) {
 #pragma unroll
-        for (int i = 0; i < kPieces; ++i) held[i] = Piece(static_cast<T>(0.0f));
-      }
-    } else {
-#pragma unroll
-      for (int i = 0; i < kPieces; ++i)
+    for (int i = 0; i < kPieces; ++i) {
+      if constexpr (WHOLE) {  // all of a piece or nothing
+        held[i] = col < width ? held[i] : Piece(static_cast<T>(0.0f));
+      } else {
 #pragma unroll
         for (int e = 0; e < kElements; ++e)
           held[i][e] = col + e < width ? held[i][e] : static_cast<T>(0.0f);
+      }
     }
   }
 
@@ -339,12 +344,17 @@ __device__ __forceinline__ Frag<T> memory_operand(const Rows<T>& rows, int row, 
   return out;
 }
 
+// operand of columns [col0, col0 + 32)
 template <bool WHOLE, typename T>
-__device__ __forceinline__ void clear_operand(Frag<T>& operand, int col, int width) {
-  constexpr int kPiece = WHOLE ? 16 / static_cast<int>(sizeof(T)) : 1;  // all or nothing
+__device__ __forceinline__ void clear_operand(Frag<T>& operand, int col0, int group, int width) {
+  if (width >= col0 + 32) return;
+  const int col = col0 + 8 * group;
+  if constexpr (WHOLE && sizeof(T) == 2) {  // all or nothing
+    operand = col < width ? operand : Frag<T>(static_cast<T>(0.0f));
+  } else {
 #pragma unroll
-  for (int e = 0; e < 8; ++e)
-    operand[e] = col + e / kPiece * kPiece < width ? operand[e] : static_cast<T>(0.0f);
+    for (int e = 0; e < 8; ++e) operand[e] = col + e < width ? operand[e] : static_cast<T>(0.0f);
+  }
 }
 
 // four neighbouring elements of a contiguous output row; `quads`: rows are whole quads
@@ -445,8 +455,8 @@ struct View {
   }
   // `count` tokens from `token` on
   __device__ __forceinline__ Rows<std::remove_const_t<T>> rows(int64_t batch, int64_t token, int head,
-                                                               int count) const {
-    return {row(batch, token, head), token_stride, count - 1};
+                                                               int count, int col = 0) const {
+    return {row(batch, token, head) + col, token_stride, count - 1};
   }
 };
 

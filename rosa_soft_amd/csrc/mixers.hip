@@ -31,13 +31,17 @@ int64_t tile_slots(const rosa_mixer_problem& p, int64_t rows) {
 // is only summed (38 against 84 us at 2 x 4096 tokens, 32 heads of 128), the states' traffic and
 // the two more launches at 5 us a chunk.  Segments have at least two chunks.
 DecayPlan decay_plan(const rosa_mixer_problem& p, int passes) {
-  const int width = padded_width(std::max(p.D, p.Dv));
-  const int slices = width == 128 ? 2 : 1;
+  DecayPlan plan{};
+  // The backward passes have both widths in both places.  Forward, values are sliced anyway, and
+  // the narrower kernel would only make more slices of wide ones.
+  plan.width = padded_width(std::max(p.D, passes > 1 ? p.Dv : std::min(p.Dv, 64)));
+  const int slice = decay_slice(plan.width);
+  const auto slices = [slice](int columns) { return (columns + slice - 1) / slice; };
   const int64_t longest = p.cu_seqlens == nullptr ? p.T : p.N;
-  const int64_t walks = static_cast<int64_t>(p.H) * slices * passes;  // of every slot
+  // blocks of every slot; the queries' and keys' gradients have D columns
+  const int64_t walks = static_cast<int64_t>(p.H) * (slices(p.Dv) + (passes > 1 ? 2 * slices(p.D) : 0));
   const int64_t state = static_cast<int64_t>(passes) * p.H * p.D * p.Dv * 4;
   const int64_t chunks = (longest + kDecayChunk - 1) / kDecayChunk;
-  DecayPlan plan{};
   int64_t best_segment = chunks;
   double best = -1.0;
   for (int64_t cuts = 1; cuts <= std::min<int64_t>(chunks, 256); ++cuts) {

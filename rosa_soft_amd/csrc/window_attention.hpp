@@ -182,7 +182,7 @@ window_forward_kernel(WindowArgs<T> a) {
 #pragma unroll
     for (int s = 0; s < kSteps; ++s) {
       Frag<T> part = memory_operand<WHOLE>(query_rows, row, s * 32 + 8 * group, a.key_width);
-      clear_operand<WHOLE>(part, s * 32 + 8 * group, a.key_width);
+      clear_operand<WHOLE>(part, s * 32, group, a.key_width);
       query[i][s] = as_operand<T>(part);
     }
   }
@@ -347,9 +347,9 @@ window_grad_query_kernel(WindowArgs<T> a) {
       Frag<T> part = memory_operand<WHOLE>(query_rows, row, s * 32 + 8 * group, a.key_width);
       Frag<T> grad_part = memory_operand<WHOLE>(grad_rows, row, s * 32 + 8 * group, a.value_width);
       Frag<T> out = memory_operand<WHOLE>(out_rows, row, s * 32 + 8 * group, a.value_width);
-      clear_operand<WHOLE>(part, s * 32 + 8 * group, a.key_width);
-      clear_operand<WHOLE>(grad_part, s * 32 + 8 * group, a.value_width);
-      clear_operand<WHOLE>(out, s * 32 + 8 * group, a.value_width);
+      clear_operand<WHOLE>(part, s * 32, group, a.key_width);
+      clear_operand<WHOLE>(grad_part, s * 32, group, a.value_width);
+      clear_operand<WHOLE>(out, s * 32, group, a.value_width);
 #pragma unroll
       for (int e = 0; e < 8; ++e) dot += static_cast<float>(grad_part[e]) * static_cast<float>(out[e]);
       query[i][s] = as_operand<T>(part);
@@ -511,8 +511,8 @@ window_grad_key_kernel(WindowArgs<T> a) {
     for (int step = 0; step < kSteps; ++step) {
       Frag<T> part = memory_operand<WHOLE>(key_rows, row, step * 32 + 8 * group, a.key_width);
       Frag<T> value_part = memory_operand<WHOLE>(value_rows, row, step * 32 + 8 * group, a.value_width);
-      clear_operand<WHOLE>(part, step * 32 + 8 * group, a.key_width);
-      clear_operand<WHOLE>(value_part, step * 32 + 8 * group, a.value_width);
+      clear_operand<WHOLE>(part, step * 32, group, a.key_width);
+      clear_operand<WHOLE>(value_part, step * 32, group, a.value_width);
       key[i][step] = as_operand<T>(part);
       value[i][step] = as_operand<T>(value_part);
     }
@@ -707,8 +707,8 @@ window_grad_sinks_kernel(WindowArgs<T> a) {
   for (int step = 0; step < kSteps; ++step) {
     Frag<T> part = memory_operand<WHOLE>(key_rows, column, step * 32 + 8 * group, a.key_width);
     Frag<T> value_part = memory_operand<WHOLE>(value_rows, column, step * 32 + 8 * group, a.value_width);
-    clear_operand<WHOLE>(part, step * 32 + 8 * group, a.key_width);
-    clear_operand<WHOLE>(value_part, step * 32 + 8 * group, a.value_width);
+    clear_operand<WHOLE>(part, step * 32, group, a.key_width);
+    clear_operand<WHOLE>(value_part, step * 32, group, a.value_width);
     key[step] = as_operand<T>(part);
     value[step] = as_operand<T>(value_part);
   }
@@ -922,7 +922,7 @@ window_token_kernel(TokenArgs<T> args) {
 #pragma unroll
   for (int s = 0; s < kSteps; ++s) {
     Frag<T> part = memory_operand<WHOLE>(query_row, 0, s * 32 + 8 * group, a.key_width);
-    clear_operand<WHOLE>(part, s * 32 + 8 * group, a.key_width);
+    clear_operand<WHOLE>(part, s * 32, group, a.key_width);
     query[s] = as_operand<T>(part);
   }
   f32x4 out[kCols];
@@ -962,7 +962,7 @@ window_token_kernel(TokenArgs<T> args) {
       score[k] = f32x4(0.0f);
 #pragma unroll
       for (int s = 0; s < kSteps; ++s) {
-        clear_operand<WHOLE>(key[k][s], s * 32 + 8 * group, a.key_width);
+        clear_operand<WHOLE>(key[k][s], s * 32, group, a.key_width);
         score[k] = mma(as_operand<T>(key[k][s]), query[s], score[k]);
       }
     }

@@ -32,7 +32,7 @@ struct DecayPass {
 template <typename T>
 struct DecayArgs {
   DecayPass<T> pass[3];
-  int passes, heads, slices, segment;
+  int passes, heads, slices, segment;        // slices of all passes together
   int64_t slots, items;
   Sequences sequences;
   const float* log_decay;
@@ -72,13 +72,18 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2))) v
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   // Neighbours on one XCD, whose cache they share: the slices of a sequence, which read the same
   // keys and queries, then the passes, which read the same four tensors.
-  const int slice = static_cast<int>(item % a.slices);
-  const int pass_index = static_cast<int>(item / a.slices % a.passes);
-  const int64_t slot = item / a.slices / a.passes % a.slots;
-  const int head = static_cast<int>(item / a.slices / a.passes / a.slots);
+  // No item is empty for its pass alone: workgroups go round the shader engines of an XCD in turn,
+  // and empty ones in a regular pattern leave some engines twice the work of others.
+  int slice = static_cast<int>(item % a.slices), pass_index = 0;
+  for (; pass_index + 1 < a.passes; ++pass_index) {
+    const int slices = (a.pass[pass_index].value_width + SLICE - 1) / SLICE;
+    if (slice < slices) break;
+    slice -= slices;
+  }
+  const int64_t slot = item / a.slices % a.slots;
+  const int head = static_cast<int>(item / a.slices / a.slots);
   const DecayPass<T>& p = a.pass[pass_index];
   const int col0 = slice * SLICE;
-  if (col0 >= p.value_width) return;
 
   Run run;
   const Found found = find_run(a.sequences, slot, a.segment, tid, &run);
@@ -525,10 +530,10 @@ void decay_walk(DecayArgs<T>& args, const DecayPlan& plan, hipStream_t stream) {
   constexpr int kSlice = decay_slice(WIDTH);
   args.slices = 0;
   for (int i = 0; i < args.passes; ++i)
-    args.slices = std::max(args.slices, (args.pass[i].value_width + kSlice - 1) / kSlice);
+    args.slices += (args.pass[i].value_width + kSlice - 1) / kSlice;
   args.segment = plan.segment;
   args.slots = plan.slots;
-  args.items = args.passes * plan.slots * args.heads * args.slices;
+  args.items = plan.slots * args.heads * args.slices;
   const dim3 grid(static_cast<unsigned>(grid_of(args.items)));
   if (plan.segmented) {
     decay_chunks_kernel<T, WIDTH, kSlice, TERMS, true, WHOLE><<<grid, kThreads, 0, stream>>>(args);

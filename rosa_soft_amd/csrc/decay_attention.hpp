@@ -335,6 +335,10 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2))) v
           ready[t] = out[t];
           if constexpr (kNarrow<T>) ready[t] *= 1.0f / range;
         }
+        if constexpr (!WHOLE) {  // loads of single elements leave no registers to hold them back in
+          store_ready();
+          ready_at = -1;
+        }
       }
     }
 
@@ -435,10 +439,18 @@ __global__ __launch_bounds__(kThreads) void decay_join_kernel(DecayArgs<T> a, in
                     : a.state_in[(static_cast<int64_t>(sequence) * a.heads + head) * state_size + e];
   float* at = a.segment_states + ((pass_index * a.slots + slot) * a.heads + head) * state_size + e;
   const int64_t step = a.heads * state_size;
-  for (int s = 0; s < segments; ++s) {
-    const float own = s + 1 < segments ? at[s * step] : 0.0f;
-    at[s * step] = state;
-    state = decay * state + own;
+  constexpr int kAhead = 4;  // loads under way: a load behind each store took 16 us for 53 segments
+  for (int first = 0; first < segments; first += kAhead) {
+    float own[kAhead];
+#pragma unroll
+    for (int s = 0; s < kAhead; ++s)
+      own[s] = first + s + 1 < segments ? at[(first + s) * step] : 0.0f;
+#pragma unroll
+    for (int s = 0; s < kAhead; ++s) {
+      if (first + s >= segments) break;
+      at[(first + s) * step] = state;
+      state = decay * state + own[s];
+    }
   }
 }
 

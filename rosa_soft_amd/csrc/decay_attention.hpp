@@ -48,11 +48,20 @@ struct DecayArgs {
 template <typename T>
 using StateType = std::conditional_t<sizeof(T) == 4, float, __bf16>;
 
-// (two waves per SIMD: with one the accumulators would be kept apart from the other registers and
-// every use of them outside a product would be a move)
+template <typename T, int WIDTH, bool STATE_ONLY, bool WHOLE>
+constexpr int kDecayWaves = STATE_ONLY || sizeof(T) == 4 || !WHOLE ? 2 : 4;
+
+// Four waves take the outputs of 16 tokens each, four others the state, between the same barriers:
+// neither holds the registers of the other, and what one waits for the other fills.  Summing
+// states alone takes four waves.
+template <bool STATE_ONLY> constexpr int kDecayThreads = STATE_ONLY ? kThreads : 2 * kThreads;
+
 template <typename T, int WIDTH, int SLICE, int TERMS, bool STATE_ONLY, bool WHOLE>
-__global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2))) void decay_chunks_kernel(DecayArgs<T> a) {
+__global__ __launch_bounds__(kDecayThreads<STATE_ONLY>)
+    __attribute__((amdgpu_waves_per_eu(kDecayWaves<T, WIDTH, STATE_ONLY, WHOLE>))) void
+    decay_chunks_kernel(DecayArgs<T> a) {
   using ST = StateType<T>;
+  constexpr int kBlock = kDecayThreads<STATE_ONLY>;
   constexpr int kColTiles = SLICE / 16;
   constexpr int kTiles = WIDTH / 16 * kColTiles / 4;   // state tiles of a wave
   constexpr int kWaveCols = kTiles < kColTiles ? kTiles : kColTiles;
@@ -69,7 +78,8 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2))) v
   const int64_t item = item_of_block(a.items);
   if (item >= a.items) return;
   const int tid = threadIdx.x, lane = tid & 63, group = lane >> 4, column = lane & 15;
-  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int place = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int wave = place & 3;  // of those with the same task
   // Neighbours on one XCD, whose cache they share: the slices of a sequence, which read the same
   // keys and queries, then the passes, which read the same four tensors.
   // No item is empty for its pass alone: workgroups go round the shader engines of an XCD in turn,
@@ -86,7 +96,7 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2))) v
   const int col0 = slice * SLICE;
 
   Run run;
-  const Found found = find_run(a.sequences, slot, a.segment, tid, &run);
+  const Found found = find_run<kBlock>(a.sequences, slot, a.segment, tid, &run);
   const int64_t state_size = static_cast<int64_t>(p.key_width) * p.value_width;
   if (found != Found::kRun) {
     if constexpr (!STATE_ONLY) {
@@ -103,7 +113,7 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2))) v
       if (slice == 0 && a.state_out != a.state_in && kept >= 0 && kept < a.sequences.count &&
           (found == Found::kInvalid || run.tile == 0)) {
         const int64_t at = (kept * a.heads + head) * state_size;
-        for (int64_t e = tid; e < state_size; e += kThreads) a.state_out[at + e] = a.state_in[at + e];
+        for (int64_t e = tid; e < state_size; e += kBlock) a.state_out[at + e] = a.state_in[at + e];
       }
     }
     return;
@@ -113,67 +123,19 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2))) v
   if (STATE_ONLY && stop == run.length) return;                 // nothing follows this segment
   const float rate = a.log_decay[head] * 1.4426950408889634f;
 
-  // the walk's token i of this sequence
-  const auto token = [&](int i) { return run.begin + (p.reverse ? run.length - 1 - i : i); };
   const int query_head = head / p.query_share, key_head = head / p.key_share,
             value_head = head / p.value_share;
-
-  // state rows (key columns) and columns (value columns) of this wave's tiles
-  const int row_tile = wave * kTiles / kColTiles, col_tile = wave * kTiles % kColTiles;
-  f32x4 state[kWaveRows][kWaveCols];
-  {
-    const float* from = nullptr;
-    if (!STATE_ONLY && a.segment_states != nullptr)
-      from = a.segment_states + ((pass_index * a.slots + slot) * a.heads + head) * state_size;
-    else if (!STATE_ONLY && a.state_in != nullptr)
-      from = a.state_in + (static_cast<int64_t>(run.sequence) * a.heads + head) * state_size;
-#pragma unroll
-    for (int i = 0; i < kWaveRows; ++i)
-#pragma unroll
-      for (int j = 0; j < kWaveCols; ++j)
-#pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          const int row = (row_tile + i) * 16 + 4 * group + r, col = col0 + (col_tile + j) * 16 + column;
-          state[i][j][r] = from != nullptr && row < p.key_width && col < p.value_width
-                               ? from[static_cast<int64_t>(row) * p.value_width + col]
-                               : 0.0f;
-        }
-  }
-
-  // Weights of a token's scores, scale lambda^(i - j): of the tile of 16 keys that its own tile is,
-  // and of the tile before it, from which the ones before that are powers of lambda^16 away.
-  const int own = wave * 16 + column;
-  float diagonal[4], before[4];
-  if constexpr (!STATE_ONLY) {
-#pragma unroll
-    for (int r = 0; r < 4; ++r) {
-      const int apart = column - 4 * group - r;
-      diagonal[r] = apart >= 0 ? a.scale * power_of(rate, apart) : 0.0f;
-      before[r] = a.scale * power_of(rate, 16 + apart);
-    }
-  }
-  const float carry = a.scale * power_of(rate, own + 1);
-
-  TileMove<T, kChunk, WIDTH, WHOLE> key_move;
-  TileMove<T, kChunk, SLICE, WHOLE> value_move;
-  Frag<T> next_query[kSteps];
   const Rows<T> key_rows = p.key.rows(run.batch, run.begin, key_head, run.length),
                 value_rows = p.value.rows(run.batch, run.begin, value_head, run.length, col0);
-  Rows<T> query_rows{};
-  if constexpr (!STATE_ONLY) query_rows = p.query.rows(run.batch, run.begin, query_head, run.length);
+  TileMove<T, kChunk, WIDTH, WHOLE, kBlock> key_move;
+  TileMove<T, kChunk, SLICE, WHOLE, kBlock> value_move;
+  // the tokens of the chunk at `at` as they lie in memory
+  const auto fill_of = [&](int at) { return min(kChunk, stop - at); };
+  const auto first_of = [&](int at, int fill) { return p.reverse ? run.length - at - fill : at; };
   const auto fetch = [&](int at) {
-    // the chunk's tokens as they lie in memory
-    const int fill = min(kChunk, stop - at);
-    const int first = p.reverse ? run.length - at - fill : at;
+    const int fill = fill_of(at), first = first_of(at, fill);
     key_move.fetch(rows_from(key_rows, first, fill), p.key_width, tid);
     value_move.fetch(rows_from(value_rows, first, fill), p.value_width - col0, tid);
-    if constexpr (!STATE_ONLY) {
-      const Rows<T> queries = rows_from(query_rows, first, fill);
-      const int row = p.reverse ? max(fill - 1 - own, 0) : own;
-#pragma unroll
-      for (int s = 0; s < kSteps; ++s)
-        next_query[s] = memory_operand<WHOLE>(queries, row, s * 32 + 8 * group, p.key_width);
-    }
   };
   fetch(start);
   // what a row of values counts for in the state behind a whole chunk
@@ -183,42 +145,15 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2))) v
     whole_chunk[i] = power_of(
         rate, kChunk - 1 - value_move.walk_row(value_move.row_of(i, tid), p.reverse ? kChunk : 0));
 
-  // Outputs of a chunk are stored when the next one has begun: loads retire in order with the
-  // stores issued before them, and the wait for a chunk's tiles would be one for them as well.
-  f32x4 ready[kColTiles];
-  int ready_at = -1;
-  const auto store_ready = [&] {
-    if (ready_at < 0 || ready_at + own >= stop) return;
-    const int64_t row = ((run.first + token(ready_at + own) - run.begin) * a.heads + head) * p.value_width + col0;
-    if (p.partial != nullptr)
-      store_tiles<WHOLE>(p.partial + row, ready, 1.0f, group, p.value_width - col0);
-    else
-      store_tiles<WHOLE>(p.out + row, ready, 1.0f, group, p.value_width - col0);
-  };
-
-  float unit = 1.0f;  // float16: brings the rounded state into range
-  if constexpr (kNarrow<T> && !STATE_ONLY) {
-    float most = 0.0f;
-#pragma unroll
-    for (int i = 0; i < kWaveRows; ++i)
-#pragma unroll
-      for (int j = 0; j < kWaveCols; ++j)
-#pragma unroll
-        for (int r = 0; r < 4; ++r) most = fmaxf(most, fabsf(state[i][j][r]));
-    for (int apart = 1; apart < 64; apart *= 2) most = fmaxf(most, __shfl_xor(most, apart));
-    if (lane == 0) largest[wave] = most;
-    __syncthreads();
-  }
-
-  for (int at = start; at < stop; at += kChunk) {
-    const int fill = min(kChunk, stop - at);
-    // what this chunk reads goes to LDS: keys, values, weighted values, the state before it
+  // keys, values and weighted values of a chunk go to LDS
+  const auto store_tiles_of = [&](int fill) {
     const int flip = p.reverse ? fill : 0;
     key_move.store(keys, p.key_width, tid, flip);
     if constexpr (!STATE_ONLY)
       value_move.store(values, p.value_width - col0, tid, flip);
     else
       value_move.clear_padding(p.value_width - col0, tid);
+    if (!value_move.holds(tid)) return;
 #pragma unroll
     for (int i = 0; i < value_move.kPieces; ++i) {
       constexpr int kElements = value_move.kElements;
@@ -244,35 +179,70 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2))) v
         }
       }
     }
-    if constexpr (!STATE_ONLY) {
-      if constexpr (kNarrow<T>) {
-        const float most = fmaxf(fmaxf(largest[0], largest[1]), fmaxf(largest[2], largest[3]));
-        unit = lift_of(most);
-      }
+  };
+  // float16: brings the rounded state into range
+  const auto unit_of_state = [&] {
+    return lift_of(fmaxf(fmaxf(largest[0], largest[1]), fmaxf(largest[2], largest[3])));
+  };
+
+  if (!STATE_ONLY && place < 4) {
+    // Weights of a token's scores, scale lambda^(i - j): of the tile of 16 keys that its own tile
+    // is, and of the tile before it, from which the ones before that are powers of lambda^16 away.
+    const int own = wave * 16 + column;
+    float diagonal[4], before[4];
 #pragma unroll
-      for (int i = 0; i < kWaveRows; ++i)
-#pragma unroll
-        for (int j = 0; j < kWaveCols; ++j) {
-          float rounded[4];
-#pragma unroll
-          for (int r = 0; r < 4; ++r) rounded[r] = state[i][j][r] * unit;
-          store_row<T, SLICE, WIDTH>(state_rows, (col_tile + j) * 16 + column, (row_tile + i) * 16 + 4 * group,
-                                     rounded);
-        }
+    for (int r = 0; r < 4; ++r) {
+      const int apart = column - 4 * group - r;
+      diagonal[r] = apart >= 0 ? a.scale * power_of(rate, apart) : 0.0f;
+      before[r] = a.scale * power_of(rate, 16 + apart);
     }
-    Operand<T> query[kSteps];
-    if constexpr (!STATE_ONLY) {
+    const float carry = a.scale * power_of(rate, own + 1);
+    const float tile_rate = power_of(rate, 16);
+
+    const Rows<T> query_rows = p.query.rows(run.batch, run.begin, query_head, run.length);
+    Frag<T> next_query[kSteps];
+    const auto fetch_query = [&](int at) {
+      const int fill = fill_of(at);
+      const Rows<T> queries = rows_from(query_rows, first_of(at, fill), fill);
+      const int row = p.reverse ? max(fill - 1 - own, 0) : own;
+#pragma unroll
+      for (int s = 0; s < kSteps; ++s)
+        next_query[s] = memory_operand<WHOLE>(queries, row, s * 32 + 8 * group, p.key_width);
+    };
+    fetch_query(start);
+
+    // Outputs of a chunk are stored when the next one has begun: loads retire in order with the
+    // stores issued before them, and the wait for a chunk's tiles would be one for them as well.
+    f32x4 ready[kColTiles];
+    int ready_at = -1;
+    const auto store_ready = [&] {
+      const int i = ready_at + own;  // the walk's token
+      if (ready_at < 0 || i >= stop) return;
+      const int64_t row =
+          ((run.first + (p.reverse ? run.length - 1 - i : i)) * a.heads + head) * p.value_width + col0;
+      if (p.partial != nullptr)
+        store_tiles<WHOLE>(p.partial + row, ready, 1.0f, group, p.value_width - col0);
+      else
+        store_tiles<WHOLE>(p.out + row, ready, 1.0f, group, p.value_width - col0);
+    };
+    if constexpr (kNarrow<T>) __syncthreads();
+
+    for (int at = start; at < stop; at += kChunk) {
+      const int fill = fill_of(at);
+      store_tiles_of(fill);
+      const float unit = kNarrow<T> ? unit_of_state() : 1.0f;
+      Operand<T> query[kSteps];
 #pragma unroll
       for (int s = 0; s < kSteps; ++s) {
         clear_operand<WHOLE>(next_query[s], s * 32, group, p.key_width);
         query[s] = as_operand<T>(next_query[s]);
       }
-    }
-    __syncthreads();
-    if constexpr (!STATE_ONLY) store_ready();
-    if (at + kChunk < stop) fetch(at + kChunk);
-
-    if constexpr (!STATE_ONLY) {
+      __syncthreads();
+      store_ready();
+      if (at + kChunk < stop) {
+        fetch(at + kChunk);
+        fetch_query(at + kChunk);
+      }
       ready_at = -1;
       if (wave * 16 < fill) {
         // outputs transposed: rows are value columns, columns are this wave's 16 tokens
@@ -284,9 +254,9 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2))) v
 #pragma unroll
           for (int t = 0; t < kColTiles; ++t)
             out[t] = mma(row_operand<T, SLICE, WIDTH>(state_rows, t * 16, s * 32, lane), query[s], out[t]);
+        // (only tiles of earlier keys: with all four for every wave, and no branches, 7 % longer)
         f32x4 score[4];
         float step = 1.0f;  // lambda^16 for every tile further back
-        const float tile_rate = power_of(rate, 16);
 #pragma unroll
         for (int t = 3; t >= 0; --t) {
           score[t] = f32x4(0.0f);
@@ -340,50 +310,38 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2))) v
           ready_at = -1;
         }
       }
+      __syncthreads();
     }
+    store_ready();
+    return;
+  }
 
-    // the state behind the chunk
-    const float decay = power_of(rate, fill);
+  // state rows (key columns) and columns (value columns) of this wave's tiles
+  const int row_tile = wave * kTiles / kColTiles, col_tile = wave * kTiles % kColTiles;
+  f32x4 state[kWaveRows][kWaveCols];
+  const float* from = nullptr;
+  if (!STATE_ONLY && a.segment_states != nullptr)
+    from = a.segment_states + ((pass_index * a.slots + slot) * a.heads + head) * state_size;
+  else if (!STATE_ONLY && a.state_in != nullptr)
+    from = a.state_in + (static_cast<int64_t>(run.sequence) * a.heads + head) * state_size;
+#pragma unroll
+  for (int i = 0; i < kWaveRows; ++i)
+#pragma unroll
+    for (int j = 0; j < kWaveCols; ++j) state[i][j] = f32x4(0.0f);
+  if (from != nullptr) {
+    const int last_row = p.key_width - 1, last_col = p.value_width - 1;
 #pragma unroll
     for (int i = 0; i < kWaveRows; ++i)
 #pragma unroll
-      for (int j = 0; j < kWaveCols; ++j) state[i][j] *= decay;
+      for (int j = 0; j < kWaveCols; ++j)
 #pragma unroll
-    for (int half = 0; half < 2; ++half) {
-      if (half * 32 >= fill) break;
-      Operand<ST> value[TERMS][kWaveCols];
-#pragma unroll
-      for (int t = 0; t < TERMS; ++t)
-#pragma unroll
-        for (int j = 0; j < kWaveCols; ++j)
-          value[t][j] = column_operand<ST, kChunk, SLICE>(weighted + t * kTerm, half * 32,
-                                                  (col_tile + j) * 16, lane);
-#pragma unroll
-      for (int i = 0; i < kWaveRows; ++i) {
-        const Operand<T> key = column_operand<T, kChunk, WIDTH>(keys, half * 32, (row_tile + i) * 16, lane);
-        if constexpr (std::is_same_v<T, _Float16>) {
-          // a float16 is the sum of two bfloat16
-          Frag<__bf16> high, low;
-#pragma unroll
-          for (int e = 0; e < 8; ++e) {
-            high[e] = static_cast<__bf16>(static_cast<float>(key[e]));
-            low[e] = static_cast<__bf16>(static_cast<float>(key[e]) - static_cast<float>(high[e]));
-          }
-#pragma unroll
-          for (int t = 0; t < TERMS; ++t)
-#pragma unroll
-            for (int j = 0; j < kWaveCols; ++j) {
-              state[i][j] = mma(high, value[t][j], state[i][j]);
-              if (t == 0 || t + 1 < TERMS) state[i][j] = mma(low, value[t][j], state[i][j]);
-            }
-        } else {
-#pragma unroll
-          for (int t = 0; t < TERMS; ++t)
-#pragma unroll
-            for (int j = 0; j < kWaveCols; ++j) state[i][j] = mma(key, value[t][j], state[i][j]);
+        for (int r = 0; r < 4; ++r) {
+          const int row = (row_tile + i) * 16 + 4 * group + r, col = col0 + (col_tile + j) * 16 + column;
+          const float value = from[min(row, last_row) * p.value_width + min(col, last_col)];
+          state[i][j][r] = row <= last_row && col <= last_col ? value : 0.0f;
         }
-      }
-    }
+  }
+  const auto note_largest = [&] {
     if constexpr (kNarrow<T> && !STATE_ONLY) {
       float most = 0.0f;
 #pragma unroll
@@ -395,10 +353,72 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2))) v
       for (int apart = 1; apart < 64; apart *= 2) most = fmaxf(most, __shfl_xor(most, apart));
       if (lane == 0) largest[wave] = most;
     }
+  };
+  note_largest();
+  if constexpr (kNarrow<T> && !STATE_ONLY) __syncthreads();
+
+  for (int at = start; at < stop; at += kChunk) {
+    const int fill = fill_of(at);
+    store_tiles_of(fill);
+    if constexpr (!STATE_ONLY) {
+      const float unit = kNarrow<T> ? unit_of_state() : 1.0f;
+#pragma unroll
+      for (int i = 0; i < kWaveRows; ++i)
+#pragma unroll
+        for (int j = 0; j < kWaveCols; ++j) {
+          float rounded[4];
+#pragma unroll
+          for (int r = 0; r < 4; ++r) rounded[r] = state[i][j][r] * unit;
+          store_row<T, SLICE, WIDTH>(state_rows, (col_tile + j) * 16 + column, (row_tile + i) * 16 + 4 * group,
+                                     rounded);
+        }
+    }
+    __syncthreads();
+    if (at + kChunk < stop) fetch(at + kChunk);
+
+    // the state behind the chunk
+    const float decay = power_of(rate, fill);
+#pragma unroll
+    for (int i = 0; i < kWaveRows; ++i)
+#pragma unroll
+      for (int j = 0; j < kWaveCols; ++j) state[i][j] *= decay;
+#pragma unroll
+    for (int half = 0; half < 2; ++half) {
+      if (half * 32 >= fill) break;
+      // (a float16 key is the sum of two bfloat16)
+      constexpr bool kPair = std::is_same_v<T, _Float16>;
+      std::conditional_t<kPair, Frag<__bf16>, Operand<T>> key[kWaveRows], low[kPair ? kWaveRows : 1];
+#pragma unroll
+      for (int i = 0; i < kWaveRows; ++i) {
+        const Operand<T> read = column_operand<T, kChunk, WIDTH>(keys, half * 32, (row_tile + i) * 16, lane);
+        if constexpr (kPair) {
+#pragma unroll
+          for (int e = 0; e < 8; ++e) {
+            key[i][e] = static_cast<__bf16>(static_cast<float>(read[e]));
+            low[i][e] = static_cast<__bf16>(static_cast<float>(read[e]) - static_cast<float>(key[i][e]));
+          }
+        } else {
+          key[i] = read;
+        }
+      }
+#pragma unroll
+      for (int t = 0; t < TERMS; ++t)
+#pragma unroll
+        for (int j = 0; j < kWaveCols; ++j) {
+          const Operand<ST> value = column_operand<ST, kChunk, SLICE>(weighted + t * kTerm, half * 32,
+                                                                      (col_tile + j) * 16, lane);
+#pragma unroll
+          for (int i = 0; i < kWaveRows; ++i) {
+            state[i][j] = mma(key[i], value, state[i][j]);
+            if constexpr (kPair)
+              if (t == 0 || t + 1 < TERMS) state[i][j] = mma(low[i], value, state[i][j]);
+          }
+        }
+    }
+    note_largest();
     __syncthreads();
   }
 
-  if constexpr (!STATE_ONLY) store_ready();
   float* to = nullptr;
   if (STATE_ONLY)
     to = a.segment_states + ((pass_index * a.slots + slot) * a.heads + head) * state_size;
@@ -548,7 +568,8 @@ void decay_walk(DecayArgs<T>& args, const DecayPlan& plan, hipStream_t stream) {
   args.items = plan.slots * args.heads * args.slices;
   const dim3 grid(static_cast<unsigned>(grid_of(args.items)));
   if (plan.segmented) {
-    decay_chunks_kernel<T, WIDTH, kSlice, TERMS, true, WHOLE><<<grid, kThreads, 0, stream>>>(args);
+    decay_chunks_kernel<T, WIDTH, kSlice, TERMS, true, WHOLE>
+        <<<grid, kDecayThreads<true>, 0, stream>>>(args);
     const int64_t size = static_cast<int64_t>(args.pass[0].key_width) * args.pass[0].value_width;
     const dim3 join(static_cast<unsigned>((size + kThreads - 1) / kThreads * args.heads *
                                           args.passes * args.sequences.count));
@@ -556,7 +577,8 @@ void decay_walk(DecayArgs<T>& args, const DecayPlan& plan, hipStream_t stream) {
   } else {
     args.segment_states = nullptr;
   }
-  decay_chunks_kernel<T, WIDTH, kSlice, TERMS, false, WHOLE><<<grid, kThreads, 0, stream>>>(args);
+  decay_chunks_kernel<T, WIDTH, kSlice, TERMS, false, WHOLE>
+      <<<grid, kDecayThreads<false>, 0, stream>>>(args);
 }
 
 template <typename T, int TERMS, bool WHOLE>

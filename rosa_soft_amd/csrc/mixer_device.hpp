@@ -247,18 +247,19 @@ __device__ __forceinline__ const T* place_of(const Rows<T>& rows, int row, int c
 // A tile of ROWS x WIDTH on its way from memory to LDS through the registers of the block.  Rows
 // that do not exist are the last one again (a caller masks what comes of it), so that loads are
 // never predicated.  WHOLE: rows are whole 16-byte pieces at 16-byte addresses.
-template <typename T, int ROWS, int WIDTH, bool WHOLE>
+template <typename T, int ROWS, int WIDTH, bool WHOLE, int THREADS = kThreads>
 struct TileMove {
   static constexpr int kElements = 16 / static_cast<int>(sizeof(T));
   static constexpr int kPerRow = WIDTH / kElements;
-  static constexpr int kPieces = ROWS * kPerRow / kThreads;
-  static_assert(ROWS * kPerRow % kThreads == 0, "tiles are moved in whole pieces per thread");
+  static constexpr bool kSpare = ROWS * kPerRow < THREADS;  // threads without a piece
+  static constexpr int kPieces = kSpare ? 1 : ROWS * kPerRow / THREADS;
+  static_assert(kSpare || ROWS * kPerRow % THREADS == 0, "tiles are moved in whole pieces per thread");
   typedef T Piece __attribute__((ext_vector_type(kElements)));
 
   Piece held[kPieces];
 
   static __device__ __forceinline__ int row_of(int i, int tid) {
-    return i * (kThreads / kPerRow) + tid / kPerRow;
+    return i * (THREADS / kPerRow) + tid / kPerRow;
   }
   static __device__ __forceinline__ int col_of(int tid) { return tid % kPerRow * kElements; }
 
@@ -306,8 +307,11 @@ struct TileMove {
     return row < flip ? flip - 1 - row : row;
   }
 
+  static __device__ __forceinline__ bool holds(int tid) { return !kSpare || row_of(0, tid) < ROWS; }
+
   __device__ __forceinline__ void store(Stored<T>* tile, int width, int tid, int flip = 0) {
     clear_padding(width, tid);
+    if (!holds(tid)) return;
 #pragma unroll
     for (int i = 0; i < kPieces; ++i) {
       const int row = walk_row(row_of(i, tid), flip);
@@ -486,6 +490,7 @@ enum class Found { kRun, kNothing, kInvalid };
 
 // The run of a slot, for a whole block.  Offsets that do not start at zero, decrease or do not
 // end at the number of tokens make the call invalid.
+template <int THREADS = kThreads>
 __device__ __forceinline__ Found find_run(const Sequences& q, int64_t slot, int rows, int tid,
                                           Run* run) {
   if (q.offsets == nullptr) {
@@ -499,7 +504,7 @@ __device__ __forceinline__ Found find_run(const Sequences& q, int64_t slot, int 
     return Found::kRun;
   }
   int upto = 0, bad = 0;
-  for (int base = 0; base < q.count; base += kThreads) {
+  for (int base = 0; base < q.count; base += THREADS) {
     const int s = base + tid;
     bool below = false;
     if (s < q.count) {

@@ -27,11 +27,13 @@ int64_t tile_slots(const rosa_mixer_problem& p, int64_t rows) {
 // A sequence is walked by one block per head and slice of 64 value columns, chunk after chunk; where
 // that leaves compute units idle it is cut into segments, whose states are summed by a walk of
 // their own over keys and values and joined.  The number of segments is the one with the least
-// time by this count, in chunks of a block that has a compute unit to itself (2.8 us at a width of
-// 128): two blocks on one take 1.5 times as long, a chunk that is only summed takes half as long,
-// and the states' traffic and the two more launches take what they take.  At 2 x 4096 tokens and
-// 32 heads of 128, bfloat16, forward: 1 segment 185 us, 2 150, 4 113, 8 120; backward, with three
-// times the blocks: 1 segment 242 us, 2 260, 4 270.  Segments have at least two chunks.
+// time by this count, in chunks of a block that has a compute unit to itself (2.5 us at a width of
+// 128): two blocks on one take 1.65 times as long, a chunk that is only summed takes half as long,
+// a block's beginning and end take one and a half chunks, and the states' traffic and the two more
+// launches take what they take.  At 2 x 4096 tokens and 32 heads of 128, bfloat16, forward:
+// 1 segment 160 us, 2 145, 4 115, 8 126; backward, with three times the blocks: 1 segment 219 us,
+// 2 300, 4 290.  12 heads of 48 and 80, float16, 6728 tokens, forward: 1 segment 215 us, 7 66,
+// 18 46, 53 59.  Segments have at least two chunks.
 DecayPlan decay_plan(const rosa_mixer_problem& p, int passes) {
   DecayPlan plan{};
   // The backward passes have both widths in both places.  Forward, values are sliced anyway, and
@@ -46,7 +48,7 @@ DecayPlan decay_plan(const rosa_mixer_problem& p, int passes) {
   const int64_t chunks = (longest + kDecayChunk - 1) / kDecayChunk;
   const auto chunk_time = [](int64_t blocks) {  // of all blocks together
     const int64_t left = blocks % kBlocks;
-    return 1.5 * static_cast<double>(blocks / kBlocks) + (left == 0 ? 0.0 : left <= kBlocks / 2 ? 1.0 : 1.5);
+    return 1.65 * static_cast<double>(blocks / kBlocks) + (left == 0 ? 0.0 : left <= kBlocks / 2 ? 1.0 : 1.65);
   };
   int64_t best_segment = chunks;
   double best = -1.0;
@@ -58,11 +60,12 @@ DecayPlan decay_plan(const rosa_mixer_problem& p, int passes) {
     const int64_t filled = p.cu_seqlens == nullptr
                                ? slots
                                : std::max<int64_t>(1, p.N / (segment * kDecayChunk));
-    double cost = chunk_time(filled * walks) * segment;
+    const double length = static_cast<double>(segment) + 1.5;
+    double cost = chunk_time(filled * walks) * length;
     if (cuts > 1) {
       if (slots * state > kMostStateBytes) break;
       const double joined = 2.0 * static_cast<double>(filled * state) / 4.5e6 + 8.0;  // us
-      cost += 0.5 * chunk_time(filled * walks * (cuts - 1) / cuts) * segment + joined / 2.8;
+      cost += 0.5 * chunk_time(filled * walks * (cuts - 1) / cuts) * length + joined / 2.5;
     }
     if (best < 0.0 || cost < best) {
       best = cost;

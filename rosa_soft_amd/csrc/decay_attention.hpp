@@ -211,20 +211,6 @@ __global__ __launch_bounds__(kDecayThreads<STATE_ONLY>)
     };
     fetch_query(start);
 
-    // Outputs of a chunk are stored when the next one has begun: loads retire in order with the
-    // stores issued before them, and the wait for a chunk's tiles would be one for them as well.
-    f32x4 ready[kColTiles];
-    int ready_at = -1;
-    const auto store_ready = [&] {
-      const int i = ready_at + own;  // the walk's token
-      if (ready_at < 0 || i >= stop) return;
-      const int64_t row =
-          ((run.first + (p.reverse ? run.length - 1 - i : i)) * a.heads + head) * p.value_width + col0;
-      if (p.partial != nullptr)
-        store_tiles<WHOLE>(p.partial + row, ready, 1.0f, group, p.value_width - col0);
-      else
-        store_tiles<WHOLE>(p.out + row, ready, 1.0f, group, p.value_width - col0);
-    };
     if constexpr (kNarrow<T>) __syncthreads();
 
     for (int at = start; at < stop; at += kChunk) {
@@ -238,12 +224,10 @@ __global__ __launch_bounds__(kDecayThreads<STATE_ONLY>)
         query[s] = as_operand<T>(next_query[s]);
       }
       __syncthreads();
-      store_ready();
       if (at + kChunk < stop) {
         fetch(at + kChunk);
         fetch_query(at + kChunk);
       }
-      ready_at = -1;
       if (wave * 16 < fill) {
         // outputs transposed: rows are value columns, columns are this wave's 16 tokens
         f32x4 out[kColTiles];
@@ -299,20 +283,19 @@ __global__ __launch_bounds__(kDecayThreads<STATE_ONLY>)
               out[t] = mma(column_operand<T, kChunk, SLICE>(values, half * 32, t * 16, lane), scores, out[t]);
           }
         }
-        ready_at = at;
-#pragma unroll
-        for (int t = 0; t < kColTiles; ++t) {
-          ready[t] = out[t];
-          if constexpr (kNarrow<T>) ready[t] *= 1.0f / range;
-        }
-        if constexpr (!WHOLE) {  // loads of single elements leave no registers to hold them back in
-          store_ready();
-          ready_at = -1;
+        const int i = at + own;  // the walk's token
+        if (i < stop) {
+          const int64_t row =
+              ((run.first + (p.reverse ? run.length - 1 - i : i)) * a.heads + head) * p.value_width + col0;
+          // (streamed: prompts 93 -> 88 us; the window kernels, whose blocks share more, lose 1 %)
+          if (p.partial != nullptr)
+            store_tiles<WHOLE, true>(p.partial + row, out, 1.0f / range, group, p.value_width - col0);
+          else
+            store_tiles<WHOLE, true>(p.out + row, out, 1.0f / range, group, p.value_width - col0);
         }
       }
       __syncthreads();
     }
-    store_ready();
     return;
   }
 

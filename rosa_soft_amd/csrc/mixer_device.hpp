@@ -386,7 +386,8 @@ template <typename T> constexpr bool kNarrow = std::is_same_v<T, _Float16>;
 // tiles: each has a whole piece then, and a store fills 64 bytes of a row instead of 32.  The
 // products are rounded to float32 first in either form (left to itself the compiler makes one
 // float16 instruction of product and rounding in one of them, and strides would change results).
-template <bool WHOLE, typename T, int TILES>
+// STREAM: past the caches, which keeps what other blocks are about to read in them.
+template <bool WHOLE, bool STREAM, typename T, int TILES>
 __device__ __forceinline__ void store_tiles(T* row, const f32x4 (&value)[TILES], float by, int group,
                                             int width) {
   f32x4 scaled[TILES];
@@ -418,7 +419,13 @@ __device__ __forceinline__ void store_tiles(T* row, const f32x4 (&value)[TILES],
         piece[e] = swapped[0];
         piece[2 + e] = swapped[1];
       }
-      if (t * 16 + col < width) *reinterpret_cast<u32x4*>(row + t * 16 + col) = piece;
+      if (t * 16 + col < width) {
+        u32x4* to = reinterpret_cast<u32x4*>(row + t * 16 + col);
+        if constexpr (STREAM)
+          __builtin_nontemporal_store(piece, to);
+        else
+          *to = piece;
+      }
     }
   } else {
 #pragma unroll

@@ -294,7 +294,7 @@ window_forward_kernel(WindowArgs<T> a) {
     const int64_t token = run.first + t - past;
     T* to = a.out + (token * a.heads + head) * a.value_width;
     const float by = 1.0f / total;
-    store_tiles<WHOLE>(to, out[i], by, group, a.value_width);
+    store_tiles<WHOLE, false>(to, out[i], by, group, a.value_width);
     if (a.log_sum != nullptr && group == 0)
       a.log_sum[static_cast<int64_t>(head) * a.sequences.tokens + token] = most[i] + log2_of(total) - kLift<T>;
   }
@@ -456,7 +456,7 @@ window_grad_query_kernel(WindowArgs<T> a) {
     if (t > last) continue;
     T* to = a.grad_query + ((run.first + t) * a.heads + head) * a.key_width;
     const float by = unit[i] == 0.0f ? a.scale : a.scale / unit[i];
-    store_tiles<WHOLE>(to, out[i], by, group, a.key_width);
+    store_tiles<WHOLE, false>(to, out[i], by, group, a.key_width);
   }
 }
 
@@ -660,10 +660,10 @@ window_grad_key_kernel(WindowArgs<T> a) {
     const float back = unit[i] == 0.0f ? 1.0f : 1.0f / unit[i];
     const int64_t row = (run.first + s) * a.kv_heads + kv_head;
     if (a.grad_key != nullptr)
-      store_tiles<WHOLE>(a.grad_key + row * a.key_width, grad_key[i], a.scale * back * kUnlift<T>, group,
+      store_tiles<WHOLE, false>(a.grad_key + row * a.key_width, grad_key[i], a.scale * back * kUnlift<T>, group,
                          a.key_width);
     if (a.grad_value != nullptr)
-      store_tiles<WHOLE>(a.grad_value + row * a.value_width, grad_value[i], kUnlift<T>, group, a.value_width);
+      store_tiles<WHOLE, false>(a.grad_value + row * a.value_width, grad_value[i], kUnlift<T>, group, a.value_width);
   }
 }
 

@@ -586,11 +586,15 @@ View<const T> view_of(const rosa_mixer_tensor& t) {
 
 // rows of whole 16-byte pieces at 16-byte addresses, less than 2^24 bytes apart
 template <typename T>
+bool whole_stride(int64_t stride) {
+  return stride >= 0 && stride < (1 << 24) / static_cast<int64_t>(sizeof(T));
+}
+template <typename T>
 bool whole_pieces(const rosa_mixer_tensor& t, int width) {
   const int64_t piece = 16 / sizeof(T);
   return reinterpret_cast<uintptr_t>(t.data) % 16 == 0 && width % piece == 0 &&
          t.batch_stride % piece == 0 && t.token_stride % piece == 0 && t.head_stride % piece == 0 &&
-         t.token_stride >= 0 && t.token_stride < (1 << 24) / static_cast<int64_t>(sizeof(T));
+         whole_stride<T>(t.token_stride);
 }
 
 }  // namespace rosa_mixer

@@ -305,6 +305,8 @@ Tensor decay_attention_update_out_op(const Tensor& query, const Tensor& key, con
   }
   REQUIRE(state_out.const_data_ptr() == state.const_data_ptr() || !overlap(state_out, state),
           "state_out must be state or share no memory with it");
+  for (const Tensor* input : {&query, &key, &value, &log_decay})
+    REQUIRE(!overlap(state_out, *input), "states must share no memory with the inputs");
   check_device(query);
   const Guard guard(query.device());
   const Call call = make_call(query, key, value, cu_seqlens, factor);
@@ -596,6 +598,13 @@ std::tuple<Tensor, Tensor> window_attention_autograd(const Tensor& query, const 
   return {results[0], results[1]};
 }
 
+// A tensor that an operator changes (taken by value) has a new version for whoever saved it.
+template <typename Declared>
+void note_change(const std::decay_t<Declared>& argument) {
+  if constexpr (std::is_same_v<Declared, Tensor>)
+    if (!argument.is_inference()) torch::autograd::impl::bump_version(argument);
+}
+
 // Operators without a backward: whatever asks for one is refused, not cut off in silence.
 template <auto* kOperator, typename... Arguments>
 auto without_backward(Arguments... arguments) {
@@ -608,8 +617,12 @@ auto without_backward(Arguments... arguments) {
   TORCH_CHECK(!(at::GradMode::is_enabled() && (asks(arguments) || ...)),
               "an update and the gradients of a mixer have no backward: call them under "
               "torch.no_grad()");
-  at::AutoDispatchBelowADInplaceOrView below;
-  return (*kOperator)(std::forward<Arguments>(arguments)...);
+  const auto result = [&] {
+    at::AutoDispatchBelowADInplaceOrView below;
+    return (*kOperator)(arguments...);
+  }();
+  (note_change<Arguments>(arguments), ...);
+  return result;
 }
 
 Tensor call_decay_update(const Tensor& q, const Tensor& k, const Tensor& v,

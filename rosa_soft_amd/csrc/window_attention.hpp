@@ -1128,7 +1128,8 @@ bool whole_inputs(const WindowCall& call) {
   const auto aligned = [](const void* data) { return reinterpret_cast<uintptr_t>(data) % 16 == 0; };
   return whole_pieces<T>(*call.query, p.D) && whole_pieces<T>(*call.key, p.D) &&
          whole_pieces<T>(*call.value, p.Dv) &&
-         (call.grad_output == nullptr || whole_pieces<T>(*call.grad_output, p.Dv)) &&
+         (call.grad_output == nullptr || (whole_pieces<T>(*call.grad_output, p.Dv) &&
+                                          whole_stride<T>(static_cast<int64_t>(p.H) * p.Dv))) &&
          aligned(call.output) && aligned(call.key_cache) && aligned(call.value_cache);
 }
 

@@ -359,6 +359,23 @@ def test_strided_inputs_are_read_in_place(width, dtype):
             assert all(torch.equal(a, b) for a, b in zip(*results))
 
 
+def test_outputs_farther_apart_than_an_offset_of_24_bits():
+    """Tokens of 70000 heads are 17.9 MB of outputs apart; a gradient of the outputs that is
+    expanded has no such strides itself."""
+    heads, tokens = 70000, 20
+    q = randn(94, 1, tokens, heads, 8, dtype=torch.bfloat16)
+    k, v = randn(95, 1, tokens, 1, 8, dtype=torch.bfloat16), randn(96, 1, tokens, 1, 128, dtype=torch.bfloat16)
+    leaves = [t.requires_grad_() for t in (q, k, v)]
+    output = mixers.window_attention(*leaves, window=7)
+    grad = randn(97, 1, 1, 1, 128, dtype=torch.bfloat16).expand_as(output)
+    got, = torch.autograd.grad(output, (q,), grad)
+    few = [0, 1, 34999, heads - 1]
+    rows = [q.detach()[0, :, few], k.detach()[0], v.detach()[0]]
+    want, bounds, most = reference.window(*rows, 7, 0, grad_output=grad[0, :, few])
+    tolerances = window_tolerances(torch.bfloat16, bounds, most, 7, 128)
+    close(got[0, :, few], want[0], tolerances[0])
+
+
 def test_results_do_not_change_from_run_to_run():
     shape = (None, [700, 1, 900, 64], 8, 2, 64, 64)
     tensors, grad_output = inputs_of(shape, torch.bfloat16, seed=100)
@@ -507,6 +524,33 @@ def test_gradients_are_differentiable_once(which):
     gradients = torch.autograd.grad(output.square().sum(), leaves, create_graph=True)
     with pytest.raises(RuntimeError, match="differentiate twice"):
         gradients[0].sum().backward()
+
+
+def test_updates_are_seen_by_a_graph_that_keeps_what_they_change():
+    """A state, a cache that a graph has saved: its backward refuses to use what is there now."""
+    (q, k, v), _ = inputs_of(((2, 3), None, 2, 2, 8, 8), torch.float32, seed=148)
+    weight = torch.ones((), device=DEVICE, requires_grad=True)
+    state = torch.zeros(2, 2, 8, 8, device=DEVICE)
+    state_out = torch.zeros_like(state)
+    caches = [torch.zeros(2, 2, 9, 8, device=DEVICE) for _ in range(2)]
+    lengths = torch.zeros(2, dtype=torch.int32, device=DEVICE)
+    for changed, update in (
+        ([state], lambda: mixers.decay_attention_update(q, k, v, rates(2), state)),
+        ([state_out], lambda: mixers.decay_attention_update(q, k, v, rates(2), state,
+                                                            state_out=state_out)),
+        (caches, lambda: mixers.window_attention_update(q, k, v, *caches, lengths, window=9)),
+    ):
+        kept = [(weight * tensor).sum() for tensor in changed]
+        with torch.no_grad():
+            update()
+        for total in kept:
+            with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+                total.backward()
+    with torch.inference_mode():
+        state = torch.zeros(2, 2, 8, 8, device=DEVICE)
+        mixers.decay_attention_update(q, k, v, rates(2), state)
+    with torch.no_grad():  # and a state made in inference mode serves outside it
+        assert mixers.decay_attention_update(q, k, v, rates(2), state).shape == (2, 3, 2, 8)
 
 
 def test_updates_without_tokens():

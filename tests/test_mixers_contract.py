@@ -119,6 +119,23 @@ def test_refusals(names, changes, error, message):
             calls(arguments(**changes()))[name]()
 
 
+def test_states_share_no_memory_with_what_is_read():
+    """A block may store a state while another still reads its keys or rates."""
+    memory = torch.zeros(2 * 4 * 16 * 8 + 64)
+    state = memory[:1024].view(2, 4, 16, 8)
+    q, k, v = (torch.zeros(2, 1, 4, 16), torch.zeros(2, 1, 4, 16), torch.zeros(2, 1, 4, 8))
+    rates = torch.zeros(4)
+    inside = memory[512:640].view(2, 1, 4, 16)
+    for arguments in ((inside, k, v, rates), (q, inside, v, rates), (q, k, memory[960:1024].view(2, 1, 4, 8), rates),
+                      (q, k, v, memory[1020:1024])):
+        with pytest.raises(ValueError, match="share no memory"):
+            mixers.decay_attention_update(*arguments, state)
+        with pytest.raises(ValueError, match="share no memory"):
+            mixers.decay_attention_update(*arguments, torch.zeros_like(state), state_out=state)
+    with pytest.raises(ValueError, match="require CUDA tensors"):  # behind the state is none of it
+        mixers.decay_attention_update(q, k, v, memory[1024:1028], state)
+
+
 def test_packed_refusals():
     packed = [host(7, 4, 16), host(7, 2, 16), host(7, 2, 8)]
     log_decay = host(4, dtype=torch.float32)

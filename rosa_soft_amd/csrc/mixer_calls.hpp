@@ -59,8 +59,10 @@ DecayPlan decay_plan(const rosa_mixer_problem& p, int passes);
 
 struct WindowPlan {
   int64_t sink_slots;   // pieces of the tokens that see sinks beyond their window
-  size_t delta_bytes, sink_bytes, sink_part_bytes;
-  size_t bytes() const { return delta_bytes + sink_bytes + sink_part_bytes; }
+  int key_block;        // keys of a block of the keys' gradients
+  int key_parts;        // blocks that share the walk over the tokens that see them
+  size_t delta_bytes, sink_bytes, sink_part_bytes, key_sum_bytes;
+  size_t bytes() const { return delta_bytes + sink_bytes + sink_part_bytes + key_sum_bytes; }
 };
 WindowPlan window_plan(const rosa_mixer_problem& p, int window, int sinks);
 

@@ -51,6 +51,8 @@ struct WindowArgs {
   int64_t slots, sink_slots, items;
   int heads, kv_heads, share, key_width, value_width, window, sinks;
   int key_block;             // keys of a block of window_grad_key_kernel
+  int key_parts;             // blocks that share its walk
+  float *key_sums, *value_sums;  // [part][tokens][kv heads][width], where there is more than one
   float scale;
 };
 
@@ -481,16 +483,25 @@ window_grad_key_kernel(WindowArgs<T> a) {
   if (item >= a.items) return;
   const int tid = threadIdx.x, lane = tid & 63, group = lane >> 4, column = lane & 15;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int64_t slot = item % a.slots;
-  const int kv_head = static_cast<int>(item / a.slots);
+  const int part = static_cast<int>(item % a.key_parts);
+  const int64_t slot = item / a.key_parts % a.slots;
+  const int kv_head = static_cast<int>(item / a.key_parts / a.slots);
+  const int64_t rows_of_parts = static_cast<int64_t>(part) * a.sequences.tokens * a.kv_heads;
   Run run;
   const Found found = find_run(a.sequences, slot, kRows, tid, &run);
   if (found != Found::kRun) {
     if (found == Found::kInvalid) {
       const int64_t first = slot * kRows;
       const int64_t last = min(first + kRows, static_cast<int64_t>(a.sequences.tokens));
-      fill_nan(a.grad_key, first, last, a.kv_heads, kv_head, a.key_width, tid);
-      fill_nan(a.grad_value, first, last, a.kv_heads, kv_head, a.value_width, tid);
+      if (a.key_parts > 1) {  // (one part makes the sum NaN)
+        if (part == 0) {
+          fill_nan(a.key_sums, first, last, a.kv_heads, kv_head, a.key_width, tid);
+          fill_nan(a.value_sums, first, last, a.kv_heads, kv_head, a.value_width, tid);
+        }
+      } else {
+        fill_nan(a.grad_key, first, last, a.kv_heads, kv_head, a.key_width, tid);
+        fill_nan(a.grad_value, first, last, a.kv_heads, kv_head, a.value_width, tid);
+      }
     }
     return;
   }
@@ -522,7 +533,7 @@ window_grad_key_kernel(WindowArgs<T> a) {
   float unit[KEYS];
 #pragma unroll
   for (int i = 0; i < KEYS; ++i) unit[i] = kNarrow<T> ? 0.0f : 1.0f;
-  if (run.tile == 0 && a.sink_sums != nullptr && to < run.length) {
+  if (part == 0 && run.tile == 0 && a.sink_sums != nullptr && to < run.length) {
     const float* sinks = a.sink_sums + (static_cast<int64_t>(run.sequence) * a.kv_heads + kv_head) * a.sinks * sums;
 #pragma unroll
     for (int i = 0; i < KEYS; ++i) {
@@ -556,8 +567,11 @@ window_grad_key_kernel(WindowArgs<T> a) {
       next_delta = a.delta[at];
     }
   };
-  fetch(0);
-  for (int step = 0; step < walk * a.share; ++step) {
+  // this part's steps (the last parts of a short walk have none)
+  const int steps = (walk * a.share + a.key_parts - 1) / a.key_parts;
+  const int step_end = min(walk * a.share, (part + 1) * steps);
+  if (part * steps < step_end) fetch(part * steps);
+  for (int step = part * steps; step < step_end; ++step) {
     const int begin = first + step % walk * kQueries;
     query_move.store(queries, a.key_width, tid);
     grad_move.store(grads, a.value_width, tid);
@@ -566,7 +580,7 @@ window_grad_key_kernel(WindowArgs<T> a) {
       deltas[tid] = next_delta;
     }
     __syncthreads();
-    if (step + 1 < walk * a.share) fetch(step + 1);
+    if (step + 1 < step_end) fetch(step + 1);
     const int wave_last = min(wave_first + 16 * KEYS, behind) - 1;
     const bool none = idle || begin + kQueries - 1 < wave_first ||
                       (begin - wave_last >= a.window && wave_first >= a.sinks);
@@ -659,12 +673,31 @@ window_grad_key_kernel(WindowArgs<T> a) {
     if (s >= behind) continue;
     const float back = unit[i] == 0.0f ? 1.0f : 1.0f / unit[i];
     const int64_t row = (run.first + s) * a.kv_heads + kv_head;
+    const float key_by = a.scale * back * kUnlift<T>;
+    if (a.key_parts > 1) {
+      float* key_to = a.key_sums + (rows_of_parts + row) * a.key_width;
+      float* value_to = a.value_sums + (rows_of_parts + row) * a.value_width;
+      store_tiles<WHOLE, false>(key_to, grad_key[i], key_by, group, a.key_width);
+      store_tiles<WHOLE, false>(value_to, grad_value[i], kUnlift<T>, group, a.value_width);
+      continue;
+    }
     if (a.grad_key != nullptr)
-      store_tiles<WHOLE, false>(a.grad_key + row * a.key_width, grad_key[i], a.scale * back * kUnlift<T>, group,
-                         a.key_width);
+      store_tiles<WHOLE, false>(a.grad_key + row * a.key_width, grad_key[i], key_by, group, a.key_width);
     if (a.grad_value != nullptr)
-      store_tiles<WHOLE, false>(a.grad_value + row * a.value_width, grad_value[i], kUnlift<T>, group, a.value_width);
+      store_tiles<WHOLE, false>(a.grad_value + row * a.value_width, grad_value[i], kUnlift<T>, group,
+                                a.value_width);
   }
+}
+
+// The sum of the parts of a walk, in order.
+template <typename T>
+__global__ __launch_bounds__(kThreads) void window_join_keys_kernel(const float* parts, T* out, int count,
+                                                                    int64_t elements) {
+  const int64_t e = static_cast<int64_t>(blockIdx.x) * kThreads + threadIdx.x;
+  if (e >= elements) return;
+  float sum = 0.0f;
+  for (int part = 0; part < count; ++part) sum += parts[part * elements + e];
+  out[e] = static_cast<T>(sum);
 }
 
 // The gradients of the sinks from the tokens beyond the first block's walk: every block takes a
@@ -1116,9 +1149,9 @@ WindowArgs<T> window_args(const WindowCall& call) {
   return args;
 }
 
-// Tokens or keys (in sixteens) of a wave: two, so that an operand read from LDS serves two products;
-// one where two would leave compute units idle (fewer than kFull blocks), and where two do not
-// fit the registers (float32, 128 columns).
+// Tokens (in sixteens) of a wave: two, so that an operand read from LDS serves two products; one
+// where two would leave compute units idle (fewer than kFull blocks), and where two do not fit the
+// registers (float32, 128 columns).
 constexpr int64_t kFull = 512;
 template <typename T, int WIDTH> constexpr bool kPairs = !(sizeof(T) == 4 && WIDTH == 128);
 
@@ -1179,7 +1212,6 @@ void window_grad_query_launch(WindowArgs<T>& args, hipStream_t stream) {
 
 template <typename T, int WIDTH, int KEYS, bool WHOLE>
 void window_grad_key_launch(WindowArgs<T>& args, hipStream_t stream) {
-  args.key_block = 64 * KEYS;
   if (args.sink_slots > 0) {
     args.items = args.sink_slots * args.heads * ((args.sinks + 15) / 16);
     window_grad_sinks_kernel<T, WIDTH, WHOLE>
@@ -1190,9 +1222,18 @@ void window_grad_key_launch(WindowArgs<T>& args, hipStream_t stream) {
            kThreads, 0, stream>>>(args);
   }
   args.slots = slots_of(args.sequences, args.key_block);
-  args.items = args.slots * args.kv_heads;
+  args.items = args.slots * args.kv_heads * args.key_parts;
   window_grad_key_kernel<T, WIDTH, KEYS, WHOLE>
       <<<dim3(static_cast<unsigned>(grid_of(args.items))), kThreads, 0, stream>>>(args);
+  if (args.key_parts == 1) return;
+  const auto join = [&](const float* parts, T* out, int width) {
+    if (out == nullptr) return;
+    const int64_t elements = static_cast<int64_t>(args.sequences.tokens) * args.kv_heads * width;
+    window_join_keys_kernel<T><<<dim3(static_cast<unsigned>((elements + kThreads - 1) / kThreads)), kThreads,
+                                 0, stream>>>(parts, out, args.key_parts, elements);
+  };
+  join(args.key_sums, args.grad_key, args.key_width);
+  join(args.value_sums, args.grad_value, args.value_width);
 }
 
 template <typename T, int WIDTH, bool WHOLE>
@@ -1202,7 +1243,7 @@ void window_backward_launch(WindowArgs<T>& args, hipStream_t stream) {
   else
     window_grad_query_launch<T, WIDTH, 1, WHOLE>(args, stream);
   if (args.grad_key == nullptr && args.grad_value == nullptr) return;
-  if (kPairs<T, WIDTH> && slots_of(args.sequences, 128) * args.kv_heads >= kFull / 4)
+  if (kPairs<T, WIDTH> && args.key_block == 128)
     window_grad_key_launch<T, WIDTH, kPairs<T, WIDTH> ? 2 : 1, WHOLE>(args, stream);
   else
     window_grad_key_launch<T, WIDTH, 1, WHOLE>(args, stream);
@@ -1220,6 +1261,12 @@ void window_backward_width(const WindowCall& call) {
   args.grad_key = static_cast<T*>(call.grad_key);
   args.grad_value = static_cast<T*>(call.grad_value);
   args.sink_slots = plan.sink_slots;
+  args.key_block = plan.key_block;
+  args.key_parts = plan.key_parts;
+  if (plan.key_parts > 1) {
+    args.key_sums = reinterpret_cast<float*>(call.workspace + plan.bytes() - plan.key_sum_bytes);
+    args.value_sums = args.key_sums + static_cast<int64_t>(plan.key_parts) * p.N * p.Hkv * p.D;
+  }
   if (plan.sink_slots > 0) {
     args.sink_sums = reinterpret_cast<float*>(call.workspace + plan.delta_bytes);
     args.sink_parts = reinterpret_cast<float*>(call.workspace + plan.delta_bytes + plan.sink_bytes);

@@ -164,6 +164,40 @@ def test_sinks_of_long_sequences_collect_all_their_gradients(dtype):
         close(got, want, tolerance, i)
 
 
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("shape,masks", [
+    (((1, 1300), None, 8, 1, 32, 32), (2000, 0)),            # many parts, all causal
+    ((None, [700, 3, 900], 6, 1, 64, 48), (300, 4)),         # and sinks, which the first part has
+    (((1, 1600), None, 16, 1, 128, 128), (150, 0)),          # parts that end inside a head's walk
+    ((None, [1100, 60], 9, 1, 20, 36), (1000, 2)),           # a last part without steps
+])
+def test_few_key_heads_share_out_their_walks(shape, masks, dtype):
+    dense, lengths, H, Hkv, D, Dv = shape
+    tensors, grad_output = inputs_of(shape, dtype, seed=25)
+    leaves = [t.requires_grad_() for t in tensors]
+    cu = offsets_of(lengths or [dense[1]])
+    output = mixers.window_attention_varlen(*(t.view(-1, *t.shape[-2:]) for t in leaves), cu,
+                                            window=masks[0], sinks=masks[1])
+    gradients, again = (torch.autograd.grad(output, leaves, grad_output.view(output.shape),
+                                            retain_graph=True) for _ in range(2))
+    assert all(map(torch.equal, gradients, again))
+    lengths = lengths or [dense[1]]
+    parts = [reference.window(q, k, v, *masks, grad_output=go)
+             for q, k, v, go in zip(*(t.detach().view(-1, *t.shape[-2:]).split(lengths)
+                                      for t in (*leaves, grad_output)))]
+    for i, got in enumerate(gradients):
+        want, bound = (torch.cat([part[j][i] for part in parts]) for j in (0, 1))
+        tolerance, = window_tolerances(dtype, [bound], max(p[2] for p in parts), max(lengths) * H, D + Dv)
+        close(got.view(want.shape), want, tolerance, i)
+    bad = cu.clone()
+    bad[-1] += 1
+    for gradient in torch.autograd.grad(
+            mixers.window_attention_varlen(*(t.view(-1, *t.shape[-2:]) for t in leaves), bad,
+                                           window=masks[0], sinks=masks[1]), leaves,
+            grad_output.view(output.shape)):
+        assert bool(torch.isnan(gradient).all())
+
+
 # ---------------------------------------------------------------------------
 # serving
 # ---------------------------------------------------------------------------

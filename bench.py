@@ -378,12 +378,12 @@ PROFILE_SOURCE = re.compile(r"^bench-source: ([0-9a-f]{16})\s*$", re.MULTILINE)
 
 
 def kernel_source_digest() -> str:
-    """Digest of the HIP source and flags the library is built from; the counter summaries
-    under profiles/ carry the digest of what they measured."""
+    """Digest of the sources and flags the operator's kernels are built from; the counter
+    summaries under profiles/ carry the digest of what they measured."""
 
     from rosa_soft_amd import _build
 
-    return _build.source_digest()
+    return _build.operator_digest()
 
 
 def profile_figures(workload: str) -> dict:

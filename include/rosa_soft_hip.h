@@ -366,6 +366,12 @@ int rosa_hip_router_update(const rosa_router_update* update, void* stream);
  * [N, heads, width] in the problem's dtype and fully overwritten.  Sums, states and softmax
  * statistics are float32.  Results do not depend on the order in which blocks run.  Invalid device
  * offsets make every output and gradient NaN and leave states and caches as they were.
+ *
+ * The caller owns every buffer: outputs, gradients, states and caches share no memory with what a
+ * call reads (a state may be advanced in place), workspaces are 16-byte aligned and belong to one
+ * call at a time.  Nothing in a workspace is kept or has to be cleared.  Entry points return 0, 1
+ * (arguments), 2 (a NULL pointer), 3 (workspace too small) or 100 and more (HIP), with
+ * rosa_hip_last_error().
  */
 typedef struct rosa_mixer_problem {
   int dtype;

@@ -34,8 +34,10 @@ MIXER_SOURCE = os.path.join(HERE, "csrc", "mixers.hip")
 MIXER_INSTANCES_SOURCE = os.path.join(HERE, "csrc", "mixer_instances.hip")
 MIXER_TYPES = [("float", "float32"), ("_Float16", "float16"), ("__bf16", "bfloat16")]
 HIP_HEADERS = [os.path.join(HERE, "csrc", name)
-               for name in ("rosa_device_common.hpp", "rosa_vjp_bands.hpp", "mixer_calls.hpp",
-                            "mixer_device.hpp", "decay_attention.hpp", "window_attention.hpp")]
+               for name in ("rosa_device_common.hpp", "rosa_vjp_bands.hpp")]
+MIXER_HEADERS = [os.path.join(HERE, "csrc", name)
+                 for name in ("mixer_calls.hpp", "mixer_device.hpp", "decay_attention.hpp",
+                              "window_attention.hpp")]
 OBJECT_DIR = os.path.join(HERE, "build_objects")
 HIP_LIBRARY = os.path.join(HERE, "librosa_soft_hip.so")
 DISPATCH_SOURCES = [os.path.join(HERE, "csrc", name)
@@ -111,16 +113,28 @@ def kernel_resources(compiler_output: str) -> Dict[str, Dict[str, int]]:
 BUILD_RECORD = "__build__"
 
 
-def source_digest() -> str:
-    """First 16 hex digits of the SHA-256 of the HIP source and the compiler flags: what a
-    resource report or a counter summary must name to speak for the library in the tree."""
-
+def _digest(*sources: str) -> str:
     digest = hashlib.sha256()
-    for path in (HIP_SOURCE, INSTANCES_SOURCE, MIXER_SOURCE, MIXER_INSTANCES_SOURCE, *HIP_HEADERS):
+    for path in sources:
         with open(path, "rb") as handle:
             digest.update(handle.read())
     digest.update(" ".join(HIPCC_FLAGS).encode())
     return digest.hexdigest()[:16]
+
+
+def operator_digest() -> str:
+    """First 16 hex digits of the SHA-256 of the sources of the operator's own kernels and the
+    compiler flags: what a counter summary of its workloads must name to speak for the tree."""
+
+    return _digest(HIP_SOURCE, INSTANCES_SOURCE, *HIP_HEADERS)
+
+
+def source_digest() -> str:
+    """The same of all HIP sources, the mixers' too: what a resource report must name to speak
+    for the library in the tree."""
+
+    return _digest(HIP_SOURCE, INSTANCES_SOURCE, MIXER_SOURCE, MIXER_INSTANCES_SOURCE, *HIP_HEADERS,
+                   *MIXER_HEADERS)
 
 
 def build_hip_library() -> str:

@@ -5,7 +5,7 @@
 // A chunk of 64 tokens that starts from the state S is three products (i, j inside the chunk):
 //   o_i = scale (lambda^(i+1) q_i^T S + sum_{j<=i} lambda^(i-j) (q_i . k_j) v_j)
 //   S'  = lambda^64 S + sum_j lambda^(63-j) k_j v_j^T
-// so a block walks its sequence chunk by chunk with the state in the registers of its four
+// so a block walks its sequence chunk by chunk with the state in the registers of four of its
 // waves: one pass over the data, no state in memory.
 //
 // The gradients are the same operator on other operands, two of them from the last token to the
@@ -54,6 +54,15 @@ constexpr int kDecayWaves = STATE_ONLY || sizeof(T) == 4 || !WHOLE ? 2 : 4;
 // Four waves take the outputs of 16 tokens each, four others the state, between the same barriers:
 // neither holds the registers of the other, and what one waits for the other fills.  Summing
 // states alone takes four waves.
+//
+// Values are cut into slices of 64 columns, each with its part of the state (128 x 64 float32 are
+// 32 registers of four waves), rounded to the inputs' type once a chunk as the operand of the
+// queries' product.  Rounded so too: the scores; weighted values by TERMS.  Measured in bfloat16,
+// 2 x 4096 tokens, 32 heads of 128: 72 us forward (and 33 and 11 for the segments' states), 217 us
+// for the three passes of the backward, 805 MB in and out at 3.7 TB/s.  What bounds it: a chunk
+// takes a block 2.5 us alone on its compute unit and two of them 4.1, of which no part is more
+// than a sixth; left out one at a time, of 154 us (mean of both directions): loads 24, stores 21,
+// scores 14, the state's products 14, the queries' 10, weighted values 9, rounded state 8.
 template <bool STATE_ONLY> constexpr int kDecayThreads = STATE_ONLY ? kThreads : 2 * kThreads;
 
 template <typename T, int WIDTH, int SLICE, int TERMS, bool STATE_ONLY, bool WHOLE>
@@ -422,7 +431,8 @@ __global__ __launch_bounds__(kDecayThreads<STATE_ONLY>)
 }
 
 // What every segment starts from: the segments' own sums, in their place, become the states before
-// them.  One thread per element of a state, in the order of the segments.
+// them.  One thread per element of a state, in the order of the segments: 67 MB in and out in 11 us
+// (2 x 4096 tokens, 32 heads of 128, four segments).
 template <typename T>
 __global__ __launch_bounds__(kThreads) void decay_join_kernel(DecayArgs<T> a, int64_t state_size) {
   const int tid = threadIdx.x;
@@ -457,7 +467,8 @@ __global__ __launch_bounds__(kThreads) void decay_join_kernel(DecayArgs<T> a, in
   }
 }
 
-// Gradients of a head of keys or values shared by `share` query heads: their sum, in order.
+// Gradients of a head of keys or values shared by `share` query heads: their sum, in order.  (Bound
+// by the reads of the float32 parts.)
 template <typename T>
 __global__ __launch_bounds__(kThreads) void sum_shared_kernel(const float* partial, T* out,
                                                               int64_t rows, int share, int width) {
@@ -484,7 +495,8 @@ struct DecayTokenArgs {
   float scale;
 };
 
-// VEC neighbouring columns per thread, the rows dealt out to the threads that are left.
+// VEC neighbouring columns per thread, the rows dealt out to the threads that are left.  64 slots
+// with 32 states of 128 x 128: 268 MB in and out in 50 us, 5.4 TB/s.
 template <typename T, int VEC>
 __global__ __launch_bounds__(kThreads) void decay_token_kernel(DecayTokenArgs<T> a) {
   __shared__ float query[kMostWidth], key[kMostWidth];

@@ -161,6 +161,12 @@ int check_window(int window, int sinks) {
   return 0;
 }
 
+int check_aligned(const void* workspace) {
+  return reinterpret_cast<uintptr_t>(workspace) % 16 == 0
+             ? 0
+             : rosa_fail(1, "mixer workspaces must be 16-byte aligned");
+}
+
 int launched(const char* what) {
   const hipError_t status = hipGetLastError();
   return status == hipSuccess ? 0 : rosa_fail_hip(status, what);
@@ -209,6 +215,7 @@ int rosa_hip_decay_forward(const rosa_mixer_problem* problem, const rosa_mixer_t
   if (const int bad = check_tensors({query, key, value}, "decay_forward: NULL tensor")) return bad;
   if (!log_decay || !output || !workspace) return rosa_fail(2, "decay_forward: NULL pointer");
   if (workspace_bytes < decay_bytes(*problem, 0)) return rosa_fail(3, "decay_forward: workspace too small");
+  if (const int bad = check_aligned(workspace)) return bad;
   DecayCall call{};
   call.problem = problem;
   call.query = query;
@@ -233,6 +240,7 @@ int rosa_hip_decay_backward(const rosa_mixer_problem* problem, const rosa_mixer_
   if (!log_decay || !workspace) return rosa_fail(2, "decay_backward: NULL pointer");
   if (workspace_bytes < decay_bytes(*problem, 1)) return rosa_fail(3, "decay_backward: workspace too small");
   if (!grad_query && !grad_key && !grad_value) return 0;
+  if (const int bad = check_aligned(workspace)) return bad;
   DecayCall call{};
   call.problem = problem;
   call.query = query;
@@ -260,6 +268,7 @@ int rosa_hip_decay_update(const rosa_mixer_problem* problem, const rosa_mixer_te
   const size_t needed = decay_bytes(*problem, 2);
   if (needed > 0 && !workspace) return rosa_fail(2, "decay_update: NULL pointer");
   if (workspace_bytes < needed) return rosa_fail(3, "decay_update: workspace too small");
+  if (const int bad = check_aligned(workspace)) return bad;
   DecayCall call{};
   call.problem = problem;
   call.query = query;
@@ -320,6 +329,7 @@ int rosa_hip_window_backward(const rosa_mixer_problem* problem, int window, int 
   if (workspace_bytes < plan.bytes())
     return rosa_fail(3, "window_backward: workspace too small");
   if (!grad_query && !grad_key && !grad_value) return 0;
+  if (const int bad = check_aligned(workspace)) return bad;
   WindowCall call{};
   call.problem = problem;
   call.window = window;
@@ -354,6 +364,7 @@ int rosa_hip_window_update(const rosa_mixer_problem* problem, int window, int si
   const size_t needed = window_update_bytes(*problem, capacity);
   if (needed > 0 && !workspace) return rosa_fail(2, "window_update: NULL pointer");
   if (workspace_bytes < needed) return rosa_fail(3, "window_update: workspace too small");
+  if (const int bad = check_aligned(workspace)) return bad;
   WindowCall call{};
   call.problem = problem;
   call.window = window;

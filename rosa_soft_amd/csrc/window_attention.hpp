@@ -146,6 +146,15 @@ struct KeyTiles {
   __device__ __forceinline__ void next() { at = at < 0 ? window_begin : at + kKeys; }
 };
 
+// o (and the log-sums) of 64 QUERIES tokens of a query head, 16 QUERIES to a wave, over their key
+// tiles: keys and values go through registers to LDS while the tile before is worked on, queries
+// and sums stay in registers.  Weights are rounded to the inputs' type, as the operand of the
+// product with the values, and summed as rounded.  Measured in bfloat16, 2 x 4096 tokens, 32 heads
+// of 128 on 8, window 1024: 190 us, 635 TFLOP/s of visible pairs.  What bounds it: matrix and vector
+// instructions of the two waves of a SIMD, of the second mostly exponentials and rounding (left
+// out one at a time: scores 64 us, values' product 36, exponentials 17, loads 27).  One tile of
+// tokens per wave instead of two: 227 us.  Wave priorities around the products and keys read ahead
+// of them gained nothing.
 template <typename T, int WIDTH, int QUERIES, bool CACHED, bool WHOLE>
 __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(kWaves<T, WIDTH, WHOLE>))) void
 window_forward_kernel(WindowArgs<T> a) {
@@ -309,6 +318,8 @@ window_forward_kernel(WindowArgs<T> a) {
 // of the longest sequence) it would add half as much error again (dq and dk of 50 tokens in
 // bfloat16: 2.8e-3 of their norm instead of 2.4e-3), and a walk of its own sums delta over the
 // keys first (DELTA: 27 us of 150, forward included, at 6 x 520 tokens, 22 heads, window 40).
+// Slopes are rounded to the inputs' type, in float16 scaled to its upper range (follow_range).
+// Measured as above: 245 us, 740 TFLOP/s.
 constexpr int kExactSpan = 256;
 
 template <typename T, int WIDTH, int QUERIES, bool WHOLE, bool DELTA>
@@ -491,8 +502,11 @@ __device__ __forceinline__ int64_t walk_end(int first, int keys, int window) {
   return static_cast<int64_t>(first) + keys - 1 + window;
 }
 
-// dk and dv of the keys of a block, 16 KEYS to a wave, over the tokens that see them: scores have
-// the tokens down and the wave's keys across.
+// dk and dv of the keys of a block, 16 KEYS to a wave, over the tokens that see them and the query
+// heads that share them: scores have the tokens down and the wave's keys across.  Weights and slopes
+// are rounded to the inputs' type.  Measured as above: 390 us, 620 TFLOP/s, one wave per SIMD (of 128
+// columns, two key tiles take 377 registers): what bounds it is that nothing fills its waits.  One
+// key tile per wave instead: 432 us.
 template <typename T, int WIDTH, int KEYS, bool WHOLE>
 __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(WIDTH * sizeof(T) > 128 ? 1 : 2))) void
 window_grad_key_kernel(WindowArgs<T> a) {
@@ -725,7 +739,8 @@ __global__ __launch_bounds__(kThreads) void window_join_keys_kernel(const float*
 
 // The gradients of the sinks from the tokens beyond the first block's walk: every block takes a
 // piece of kSinkRows tokens of one query head and 16 sinks, every wave 32 tokens of a tile.  (One
-// block walking all of them would be the last to finish by far.)
+// block walking all of them would be the last to finish by far.)  Measured as above, 4 sinks:
+// 28 us, most of it the reads of q and dO (134 MB, 4.8 TB/s).
 template <typename T, int WIDTH, bool WHOLE>
 __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(1))) void
 window_grad_sinks_kernel(WindowArgs<T> a) {
@@ -884,7 +899,8 @@ __global__ __launch_bounds__(kThreads) void window_join_sinks_kernel(WindowArgs<
 // ---------------------------------------------------------------------------
 
 // The new tokens that a cache keeps, each on its row: the sinks and the newest `ring` others.
-// Blocks of 64 tokens of one head of keys.
+// Blocks of 64 tokens of one head of keys: 67 MB in and out in 11 us at 4 x 2048 tokens, 8 heads of
+// 128, bfloat16.
 template <typename T, bool WHOLE>
 __global__ __launch_bounds__(kThreads) void window_append_kernel(WindowArgs<T> a, T* key_cache,
                                                                  T* value_cache) {
@@ -922,7 +938,9 @@ __global__ __launch_bounds__(kThreads) void window_append_kernel(WindowArgs<T> a
 // One new token of every slot against its cache, which is shared out to the blocks of a head of
 // keys and, in tiles of 32 keys, to their waves: every wave has a softmax of its own over its
 // tiles, with the query heads of the group (up to 16) across; the waves are joined at the end and
-// the blocks by window_token_join_kernel.
+// the blocks by window_token_join_kernel.  Bound by the reads of the cache: 64 slots, 8 heads of
+// 128, window 4096, bfloat16: 1.07 GB in 175 us, 6.1 TB/s; 1 slot, 2 heads of 64, window 65536: 34 MB
+// in 10 us, of which the launch and the first loads are half, and 6 us for the join.
 template <typename T>
 struct TokenArgs {
   WindowArgs<T> window;

@@ -225,6 +225,17 @@ def test_c_entries_refuse_null_pointers_masks_and_small_workspaces():
     assert library.rosa_hip_decay_workspace_bytes(ctypes.byref(good), 3) == 0
 
 
+def test_c_entries_refuse_misaligned_workspaces():
+    library, good = cabi.load(), problem()
+    p, t = ctypes.byref(good), ctypes.byref(cabi.RosaMixerTensor(1, 0, 64, 64))
+    assert library.rosa_hip_decay_forward(p, t, t, t, 1, 1, 8, 1 << 40, None) == 1
+    assert library.rosa_hip_decay_backward(p, t, t, t, t, 1, 1, 1, 1, 8, 1 << 40, None) == 1
+    assert library.rosa_hip_decay_update(p, t, t, t, 1, 1, 1, 1, 8, 1 << 40, None) == 1
+    assert library.rosa_hip_window_backward(p, 10, 2, t, t, t, 1, 1, t, 1, 1, 1, 8, 1 << 40, None) == 1
+    assert library.rosa_hip_window_update(p, 10, 2, t, t, t, 1, 1, 12, 1, 1, 8, 1 << 40, None) == 1
+    assert b"16-byte aligned" in library.rosa_hip_last_error()
+
+
 def test_workspaces_of_extreme_shapes_stay_bounded():
     """States between segments take at most 2 GiB, however many short sequences a call has."""
     library = cabi.load()

@@ -25,6 +25,11 @@ template <typename T, int WIDTH, bool WHOLE>
 constexpr int kWaves = WIDTH == 128 && (sizeof(T) == 4 || !WHOLE) ? 1 : 2;
 constexpr float kLog2e = 1.4426950408889634f;
 
+// Tiles in LDS of the training kernels.  Two of 16 bits, in turn: a wave stores the next while
+// others work on the one before, and one barrier for a tile is enough (it lets no wave past that
+// has not finished the tile before last).  One of float32, whose three planes leave no room.
+template <typename T> constexpr int kBuffers = sizeof(T) == 2 ? 2 : 1;
+
 // Weights are formed as 2^kLift p and rounded so: float16 would lose bits of a weight below 2^-14,
 // which a long window's are.
 template <typename T> constexpr float kLift = kNarrow<T> ? 8.0f : 0.0f;
@@ -159,8 +164,9 @@ template <typename T, int WIDTH, int QUERIES, bool CACHED, bool WHOLE>
 __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(kWaves<T, WIDTH, WHOLE>))) void
 window_forward_kernel(WindowArgs<T> a) {
   constexpr int kSteps = WIDTH / 32, kRows = 64 * QUERIES, kCols = WIDTH / 16;
-  __shared__ __attribute__((aligned(16))) Stored<T> keys[kTileElements<T, kKeys, WIDTH>];
-  __shared__ __attribute__((aligned(16))) Stored<T> values[kTileElements<T, kKeys, WIDTH>];
+  constexpr int kTile = kTileElements<T, kKeys, WIDTH>;
+  __shared__ __attribute__((aligned(16))) Stored<T> key_tiles[kBuffers<T> * kTile];
+  __shared__ __attribute__((aligned(16))) Stored<T> value_tiles[kBuffers<T> * kTile];
 
   const int64_t item = item_of_block(a.items);
   if (item >= a.items) return;
@@ -220,9 +226,10 @@ window_forward_kernel(WindowArgs<T> a) {
     value_rows.fetch(value_move, begin, end, tid);
   };
   fetch();
-  while (tiles.more()) {
+  for (int side = 0; tiles.more(); side = kBuffers<T> - 1 - side) {
     const int begin = tiles.begin(), end = tiles.end();
     tiles.next();
+    Stored<T>*keys = key_tiles + side * kTile, *values = value_tiles + side * kTile;
     key_move.store(keys, a.key_width, tid);
     value_move.store(values, a.value_width, tid);
     __syncthreads();
@@ -295,7 +302,7 @@ window_forward_kernel(WindowArgs<T> a) {
           for (int i = 0; i < QUERIES; ++i) out[i][d] = mma(value, weights[i][half], out[i][d]);
         }
     }
-    __syncthreads();
+    if constexpr (kBuffers<T> == 1) __syncthreads();
   }
 
 #pragma unroll
@@ -326,8 +333,9 @@ template <typename T, int WIDTH, int QUERIES, bool WHOLE, bool DELTA>
 __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(kWaves<T, WIDTH, WHOLE>))) void
 window_grad_query_kernel(WindowArgs<T> a) {
   constexpr int kSteps = WIDTH / 32, kRows = 64 * QUERIES, kCols = WIDTH / 16;
-  __shared__ __attribute__((aligned(16))) Stored<T> keys[kTileElements<T, kKeys, WIDTH>];
-  __shared__ __attribute__((aligned(16))) Stored<T> values[kTileElements<T, kKeys, WIDTH>];
+  constexpr int kTile = kTileElements<T, kKeys, WIDTH>;
+  __shared__ __attribute__((aligned(16))) Stored<T> key_tiles[kBuffers<T> * kTile];
+  __shared__ __attribute__((aligned(16))) Stored<T> value_tiles[kBuffers<T> * kTile];
 
   const int64_t item = item_of_block(a.items);
   if (item >= a.items) return;
@@ -405,9 +413,10 @@ window_grad_query_kernel(WindowArgs<T> a) {
     value_rows.fetch(value_move, begin, end, tid);
   };
   fetch();
-  while (tiles.more()) {
+  for (int side = 0; tiles.more(); side = kBuffers<T> - 1 - side) {
     const int begin = tiles.begin(), end = tiles.end();
     tiles.next();
+    Stored<T>*keys = key_tiles + side * kTile, *values = value_tiles + side * kTile;
     key_move.store(keys, a.key_width, tid);
     value_move.store(values, a.value_width, tid);
     __syncthreads();
@@ -479,7 +488,7 @@ window_grad_query_kernel(WindowArgs<T> a) {
         }
       }
     }
-    __syncthreads();
+    if constexpr (kBuffers<T> == 1) __syncthreads();
   }
 #pragma unroll
   for (int i = 0; i < QUERIES; ++i) {
@@ -512,9 +521,10 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(WIDTH 
 window_grad_key_kernel(WindowArgs<T> a) {
   constexpr int kSteps = WIDTH / 32, kRows = 64 * KEYS, kCols = WIDTH / 16;
   constexpr int kQueries = sizeof(T) == 4 && WIDTH == 128 ? 32 : 64;  // (registers)
-  __shared__ __attribute__((aligned(16))) Stored<T> queries[kTileElements<T, kQueries, WIDTH>];
-  __shared__ __attribute__((aligned(16))) Stored<T> grads[kTileElements<T, kQueries, WIDTH>];
-  __shared__ __attribute__((aligned(16))) float log_sums[kQueries], deltas[kQueries];
+  constexpr int kTile = kTileElements<T, kQueries, WIDTH>;
+  __shared__ __attribute__((aligned(16))) Stored<T> query_tiles[kBuffers<T> * kTile];
+  __shared__ __attribute__((aligned(16))) Stored<T> grad_tiles[kBuffers<T> * kTile];
+  __shared__ __attribute__((aligned(16))) float tile_sums[kBuffers<T>][2][kQueries];
 
   const int64_t item = item_of_block(a.items);
   if (item >= a.items) return;
@@ -608,8 +618,10 @@ window_grad_key_kernel(WindowArgs<T> a) {
   const int steps = (walk * a.share + a.key_parts - 1) / a.key_parts;
   const int step_end = min(walk * a.share, (part + 1) * steps);
   if (part * steps < step_end) fetch(part * steps);
-  for (int step = part * steps; step < step_end; ++step) {
+  for (int step = part * steps, side = 0; step < step_end; ++step, side = kBuffers<T> - 1 - side) {
     const int begin = first + step % walk * kQueries;
+    Stored<T>*queries = query_tiles + side * kTile, *grads = grad_tiles + side * kTile;
+    float *log_sums = tile_sums[side][0], *deltas = tile_sums[side][1];
     query_move.store(queries, a.key_width, tid);
     grad_move.store(grads, a.value_width, tid);
     if (tid < kQueries) {
@@ -701,7 +713,7 @@ window_grad_key_kernel(WindowArgs<T> a) {
         }
       }
     }
-    __syncthreads();
+    if constexpr (kBuffers<T> == 1) __syncthreads();
   }
 
 #pragma unroll

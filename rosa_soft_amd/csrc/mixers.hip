@@ -92,17 +92,19 @@ WindowPlan window_plan(const rosa_mixer_problem& p, int window, int sinks) {
     plan.sink_part_bytes = aligned(static_cast<size_t>(plan.sink_slots) * p.H * size);
   }
   // Keys of a block: 128, so that an operand read from LDS serves two products, or 64 where that
-  // makes fewer than half a compute unit's worth of blocks for each and where 128 do not fit the
-  // registers (float32, 128 columns).  Few blocks with long walks have them shared out until
-  // there is one for every compute unit, or two of the smaller ones, as long as a part has eight
-  // tiles of tokens (4096 tokens, 8 query heads of 128 on one, window 1024, bfloat16: 4 parts).
+  // makes fewer than two blocks for each compute unit (240 blocks of 128 took 77 us where 448 of 64
+  // take 56, 336 took 47 us where 600 take 31; 512 take 390 us, 1024 of 64 402) and where 128 do not
+  // fit the registers (float32, 128 columns).  Few blocks with long walks have them shared out
+  // until there are two for each compute unit, or one of those float32 ones, as long as a part has
+  // eight tiles of tokens (4096 tokens, 8 query heads of 128 on one, window 1024, bfloat16: 59 us
+  // with 8 parts, 89 with 4).
   const int columns = padded_width(std::max(p.D, p.Dv));
   const bool pairs = p.dtype != ROSA_DTYPE_F32 || columns < 128;
-  plan.key_block = pairs && tile_slots(p, 128) * p.Hkv >= kBlocks / 4 ? 128 : 64;
+  plan.key_block = pairs && tile_slots(p, 128) * p.Hkv >= kBlocks ? 128 : 64;
   const int64_t blocks = tile_slots(p, plan.key_block) * p.Hkv;
   const int64_t walk = std::min<int64_t>(longest, static_cast<int64_t>(plan.key_block) + window);
   const int64_t tiles = (walk + 63) / 64 * (p.H / p.Hkv);
-  plan.key_parts = static_cast<int>(std::max<int64_t>(1, std::min((columns < 128 ? kBlocks : kBlocks / 2) / blocks, tiles / 8)));
+  plan.key_parts = static_cast<int>(std::max<int64_t>(1, std::min((pairs ? kBlocks : kBlocks / 2) / blocks, tiles / 8)));
   if (plan.key_parts > 1)
     plan.key_sum_bytes = aligned(static_cast<size_t>(plan.key_parts) * p.N * p.Hkv * (p.D + p.Dv) * 4);
   return plan;

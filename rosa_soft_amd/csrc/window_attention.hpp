@@ -515,9 +515,11 @@ __device__ __forceinline__ int64_t walk_end(int first, int keys, int window) {
 // heads that share them: scores have the tokens down and the wave's keys across.  Weights and slopes
 // are rounded to the inputs' type.  Measured as above: 390 us, 620 TFLOP/s, one wave per SIMD (of 128
 // columns, two key tiles take 377 registers): what bounds it is that nothing fills its waits.  One
-// key tile per wave instead: 432 us.
+// key tile per wave and two waves per SIMD instead: 402 us.
 template <typename T, int WIDTH, int KEYS, bool WHOLE>
-__global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(WIDTH * sizeof(T) > 128 ? 1 : 2))) void
+constexpr int kKeyWaves = WIDTH * sizeof(T) <= 128 || (sizeof(T) == 2 && KEYS == 1 && WHOLE) ? 2 : 1;
+template <typename T, int WIDTH, int KEYS, bool WHOLE>
+__global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(kKeyWaves<T, WIDTH, KEYS, WHOLE>))) void
 window_grad_key_kernel(WindowArgs<T> a) {
   constexpr int kSteps = WIDTH / 32, kRows = 64 * KEYS, kCols = WIDTH / 16;
   constexpr int kQueries = sizeof(T) == 4 && WIDTH == 128 ? 32 : 64;  // (registers)

@@ -1205,9 +1205,11 @@ WindowArgs<T> window_args(const WindowCall& call) {
 }
 
 // Tokens (in sixteens) of a wave: two, so that an operand read from LDS serves two products; one
-// where two would leave compute units idle (fewer than kFull blocks), and where two do not fit the
+// where two make fewer than kFull blocks, which two rounds of the chip's take (o and dq of 664
+// blocks of two: 26.5 and 32.6 us, of 1192 of one: 24.5 and 29.2; of 712: 43 and 64 us, of 1344: 44.6
+// and 62.6; of 2048: 195 and 250 us, of 4096 of one: 227 and 296), and where two do not fit the
 // registers (float32, 128 columns).
-constexpr int64_t kFull = 512;
+constexpr int64_t kFull = 1024;
 template <typename T, int WIDTH> constexpr bool kPairs = !(sizeof(T) == 4 && WIDTH == 128);
 
 template <typename T>

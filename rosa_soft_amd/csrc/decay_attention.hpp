@@ -58,11 +58,12 @@ constexpr int kDecayWaves = STATE_ONLY || sizeof(T) == 4 || !WHOLE ? 2 : 4;
 // Values are cut into slices of 64 columns, each with its part of the state (128 x 64 float32 are
 // 32 registers of four waves), rounded to the inputs' type once a chunk as the operand of the
 // queries' product.  Rounded so too: the scores; weighted values by TERMS.  Measured in bfloat16,
-// 2 x 4096 tokens, 32 heads of 128: 72 us forward (and 33 and 11 for the segments' states), 217 us
-// for the three passes of the backward, 805 MB in and out at 3.7 TB/s.  What bounds it: a chunk
-// takes a block 2.5 us alone on its compute unit and two of them 4.1, of which no part is more
-// than a sixth; left out one at a time, of 154 us (mean of both directions): loads 24, stores 21,
-// scores 14, the state's products 14, the queries' 10, weighted values 9, rounded state 8.
+// 2 x 4096 tokens, 32 heads of 128: 72 us forward, 309 MB in and out of HBM at 4.3 TB/s (and 32 and
+// 11 us for the segments' states), 213 us for the three passes of the backward, 763 MB at 3.6 TB/s;
+// a large copy reaches 4.9.  What bounds it besides: a chunk takes a block 2.5 us alone on its
+// compute unit and two of them 4.1, of which no part is more than a sixth; left out one at a
+// time, of 154 us (mean of both directions): loads 24, stores 21, scores 14, the state's products
+// 14, the queries' 10, weighted values 9, rounded state 8.
 template <bool STATE_ONLY> constexpr int kDecayThreads = STATE_ONLY ? kThreads : 2 * kThreads;
 
 template <typename T, int WIDTH, int SLICE, int TERMS, bool STATE_ONLY, bool WHOLE>

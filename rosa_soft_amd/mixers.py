@@ -22,7 +22,9 @@ states or caches, which are advanced in place.  They have no backward.
 
 Invalid device ``cu_seqlens`` cannot be seen without a synchronisation: they make every output and
 gradient NaN and leave states and caches as they were.  A row of values that is not finite makes
-the outputs NaN of every token that sees it, and may do so for up to 63 tokens before it.
+the outputs NaN of every token that sees it, and may do so for up to 63 tokens before it; a row of
+output gradients does the same to the gradients of what it sees.  States and caches share no
+memory with the inputs, and the updates count a version of them.
 """
 
 from __future__ import annotations

@@ -313,9 +313,9 @@ __global__ __launch_bounds__(kDecayThreads<STATE_ONLY>)
   const int row_tile = wave * kTiles / kColTiles, col_tile = wave * kTiles % kColTiles;
   f32x4 state[kWaveRows][kWaveCols];
   const float* from = nullptr;
-  if (!STATE_ONLY && a.segment_states != nullptr)
+  if (!STATE_ONLY && a.segment_states != nullptr && (run.tile > 0 || a.state_in != nullptr))
     from = a.segment_states + ((pass_index * a.slots + slot) * a.heads + head) * state_size;
-  else if (!STATE_ONLY && a.state_in != nullptr)
+  else if (!STATE_ONLY && a.segment_states == nullptr && a.state_in != nullptr)
     from = a.state_in + (static_cast<int64_t>(run.sequence) * a.heads + head) * state_size;
 #pragma unroll
   for (int i = 0; i < kWaveRows; ++i)
@@ -432,38 +432,42 @@ __global__ __launch_bounds__(kDecayThreads<STATE_ONLY>)
 }
 
 // What every segment starts from: the segments' own sums, in their place, become the states before
-// them.  One thread per element of a state, in the order of the segments: 67 MB in and out in 11 us
-// (2 x 4096 tokens, 32 heads of 128, four segments).
+// them, in the order of the segments; what a sequence starts from is only written where that is a
+// given state (it may be overwritten by the last segment while the first still reads it).
+// kPieceElements elements of a state to a block: 67 MB in and out in 11 us (2 x 4096 tokens, 32
+// heads of 128, four segments).  Offsets are only looked at as far as this block's accesses go; the
+// walk itself refuses the others.
+constexpr int kPieceElements = 4 * kThreads;
 template <typename T>
 __global__ __launch_bounds__(kThreads) void decay_join_kernel(DecayArgs<T> a, int64_t state_size) {
-  const int tid = threadIdx.x;
-  const int64_t pieces = (state_size + kThreads - 1) / kThreads, row = blockIdx.x / pieces;
+  const int64_t pieces = (state_size + kPieceElements - 1) / kPieceElements, row = blockIdx.x / pieces;
   const int head = static_cast<int>(row % a.heads);
   const int pass_index = static_cast<int>(row / a.heads % a.passes);
   const int sequence = static_cast<int>(row / a.heads / a.passes);
-  const Run run = run_of_sequence(a.sequences, sequence, tid);
-  if (run.length < 0) return;
+  const Run run = run_of_sequence(a.sequences, sequence);
+  const int segments = run.length < 0 ? 0 : (run.length + a.segment - 1) / a.segment;
+  if (segments < (a.state_in == nullptr ? 2 : 1)) return;
   const int64_t slot = first_slot(a.sequences, run, a.segment);
-  const int64_t e = blockIdx.x % pieces * kThreads + tid;
-  if (e >= state_size) return;
-  const int segments = (run.length + a.segment - 1) / a.segment;
   const float decay = power_of(a.log_decay[head] * 1.4426950408889634f, a.segment);
-  float state = a.state_in == nullptr
-                    ? 0.0f
-                    : a.state_in[(static_cast<int64_t>(sequence) * a.heads + head) * state_size + e];
-  float* at = a.segment_states + ((pass_index * a.slots + slot) * a.heads + head) * state_size + e;
   const int64_t step = a.heads * state_size;
   constexpr int kAhead = 4;  // loads under way: a load behind each store took 16 us for 53 segments
-  for (int first = 0; first < segments; first += kAhead) {
-    float own[kAhead];
+  const int64_t end = min((blockIdx.x % pieces + 1) * kPieceElements, state_size);
+  for (int64_t e = blockIdx.x % pieces * kPieceElements + threadIdx.x; e < end; e += kThreads) {
+    float state = a.state_in == nullptr
+                      ? 0.0f
+                      : a.state_in[(static_cast<int64_t>(sequence) * a.heads + head) * state_size + e];
+    float* at = a.segment_states + ((pass_index * a.slots + slot) * a.heads + head) * state_size + e;
+    for (int first = 0; first < segments; first += kAhead) {
+      float own[kAhead];
 #pragma unroll
-    for (int s = 0; s < kAhead; ++s)
-      own[s] = first + s + 1 < segments ? at[(first + s) * step] : 0.0f;
+      for (int s = 0; s < kAhead; ++s)
+        own[s] = first + s + 1 < segments ? at[(first + s) * step] : 0.0f;
 #pragma unroll
-    for (int s = 0; s < kAhead; ++s) {
-      if (first + s >= segments) break;
-      at[(first + s) * step] = state;
-      state = decay * state + own[s];
+      for (int s = 0; s < kAhead; ++s) {
+        if (first + s >= segments) break;
+        at[(first + s) * step] = state;
+        state = decay * state + own[s];
+      }
     }
   }
 }
@@ -567,7 +571,7 @@ void decay_walk(DecayArgs<T>& args, const DecayPlan& plan, hipStream_t stream) {
     decay_chunks_kernel<T, WIDTH, kSlice, TERMS, true, WHOLE>
         <<<grid, kDecayThreads<true>, 0, stream>>>(args);
     const int64_t size = static_cast<int64_t>(args.pass[0].key_width) * args.pass[0].value_width;
-    const dim3 join(static_cast<unsigned>((size + kThreads - 1) / kThreads * args.heads *
+    const dim3 join(static_cast<unsigned>((size + kPieceElements - 1) / kPieceElements * args.heads *
                                           args.passes * args.sequences.count));
     decay_join_kernel<T><<<join, kThreads, 0, stream>>>(args, size);
   } else {

@@ -510,16 +510,26 @@ __device__ __forceinline__ Found find_run(const Sequences& q, int64_t slot, int 
     run->first = static_cast<int64_t>(run->sequence) * q.length;
     return Found::kRun;
   }
+  // How many sequences begin at this slot or before it: with one a thread a count of the block, with
+  // more a sum, so that all loads are under way at once (16 rounds with a barrier each made 4096
+  // sequences of 16 tokens five times as long).
   int upto = 0, bad = 0;
-  for (int base = 0; base < q.count; base += THREADS) {
-    const int s = base + tid;
-    bool below = false;
-    if (s < q.count) {
-      const int begin = q.offsets[s], end = q.offsets[s + 1];
-      bad |= begin > end || (s == 0 && begin != 0) || (s == q.count - 1 && end != q.tokens);
-      below = static_cast<int64_t>(begin / rows) + s <= slot;
-    }
-    upto += __syncthreads_count(below);
+  const auto look_at = [&](int s) {
+    const int begin = q.offsets[s], end = q.offsets[s + 1];
+    bad |= begin > end || (s == 0 && begin != 0) || (s == q.count - 1 && end != q.tokens);
+    return static_cast<int64_t>(begin / rows) + s <= slot ? 1 : 0;
+  };
+  if (q.count <= THREADS) {
+    upto = __syncthreads_count(tid < q.count ? look_at(tid) : 0);
+  } else {
+    __shared__ int total;
+    if (tid == 0) total = 0;
+#pragma unroll 4
+    for (int s = tid; s < q.count; s += THREADS) upto += look_at(s);
+    __syncthreads();
+    atomicAdd(&total, upto);
+    __syncthreads();
+    upto = total;
   }
   if (__syncthreads_or(bad)) return Found::kInvalid;
   run->sequence = __builtin_amdgcn_readfirstlane(upto - 1);
@@ -532,16 +542,12 @@ __device__ __forceinline__ Found find_run(const Sequences& q, int64_t slot, int 
   return static_cast<int64_t>(run->tile) * rows < run->length ? Found::kRun : Found::kNothing;
 }
 
-// The whole of a sequence, for a whole block; of length -1 where the offsets are invalid.
-__device__ __forceinline__ Run run_of_sequence(const Sequences& q, int sequence, int tid) {
+// The whole of a sequence; of length -1 where its offsets do not lie among the tokens.
+__device__ __forceinline__ Run run_of_sequence(const Sequences& q, int sequence) {
   if (q.offsets == nullptr)
     return {sequence, q.length, 0, sequence, 0, static_cast<int64_t>(sequence) * q.length};
-  int bad = 0;
-  for (int s = tid; s < q.count; s += kThreads)
-    bad |= q.offsets[s] > q.offsets[s + 1] || (s == 0 && q.offsets[0] != 0) ||
-           (s == q.count - 1 && q.offsets[s + 1] != q.tokens);
-  const int begin = q.offsets[sequence], length = q.offsets[sequence + 1] - begin;
-  return {sequence, __syncthreads_or(bad) ? -1 : length, 0, 0, begin, begin};
+  const int begin = q.offsets[sequence], end = q.offsets[sequence + 1];
+  return {sequence, begin < 0 || end < begin || end > q.tokens ? -1 : end - begin, 0, 0, begin, begin};
 }
 
 // The slot of a sequence's first tile.

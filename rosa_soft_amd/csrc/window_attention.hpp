@@ -892,7 +892,7 @@ __global__ __launch_bounds__(kThreads) void window_join_sinks_kernel(WindowArgs<
   const int blocks = (size + kThreads - 1) / kThreads;
   const int sequence = static_cast<int>(blockIdx.x / blocks / a.kv_heads);
   const int kv_head = static_cast<int>(blockIdx.x / blocks % a.kv_heads);
-  const Run run = run_of_sequence(a.sequences, sequence, tid);
+  const Run run = run_of_sequence(a.sequences, sequence);
   if (run.length < 0) return;
   const int e = static_cast<int>(blockIdx.x % blocks) * kThreads + tid;
   if (e >= size) return;

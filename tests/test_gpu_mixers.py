@@ -393,6 +393,74 @@ def test_strided_inputs_are_read_in_place(width, dtype):
             assert all(torch.equal(a, b) for a, b in zip(*results))
 
 
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_more_sequences_than_threads(dtype):
+    """1100 sequences of 0 to 6 tokens: the search for a block's sequence takes several rounds."""
+    lengths = [(7 * i + i // 5) % 7 for i in range(1100)]
+    H, Hkv, D, Dv = 2, 1, 24, 40
+    tensors, grad_output = inputs_of((None, lengths, H, Hkv, D, Dv), dtype, seed=99)
+    log_decay, cu = rates(H), offsets_of(lengths)
+    parts = [[t.detach()[begin:end] for t in (*tensors, grad_output)]
+             for begin, end in zip(cu.tolist(), cu.tolist()[1:]) if end > begin]
+    leaves = [t.requires_grad_() for t in tensors]
+    output = mixers.decay_attention_varlen(*leaves, cu, log_decay)
+    got = [output.detach(), *torch.autograd.grad(output, leaves, grad_output)]
+    for i in range(4):
+        want, bound = (torch.cat([
+            reference.decay(*p[:3], log_decay, absolute=absolute)[0] if i == 0 else
+            reference.decay(*p[:3], log_decay, grad_output=p[3], absolute=absolute)[i - 1]
+            for p in parts]) for absolute in (False, True))
+        close(got[i], want, decay_tolerance(dtype, bound, 12, D + Dv), i)
+    output = mixers.window_attention_varlen(*leaves, cu, window=3, sinks=1)
+    got = [output.detach(), *torch.autograd.grad(output, leaves, grad_output)]
+    results = [(reference.window(*p[:3], 3, 1), reference.window(*p[:3], 3, 1, grad_output=p[3])) for p in parts]
+    most = max(forward[2] for forward, _ in results)
+    for i in range(4):
+        want, bound = (torch.cat([forward[j] if i == 0 else backward[j][i - 1]
+                                  for forward, backward in results]) for j in (0, 1))
+        tolerance, = window_tolerances(dtype, [bound], most, 12, D + Dv)
+        close(got[i], want, tolerance, i)
+    q, k, v = (t.detach() for t in leaves)
+    state, lengths_of = torch.zeros(len(lengths), H, D, Dv, device=DEVICE), torch.zeros(
+        len(lengths), dtype=torch.int32, device=DEVICE)
+    caches = [torch.zeros(len(lengths), Hkv, 4, w, dtype=dtype, device=DEVICE) for w in (D, Dv)]
+    assert torch.equal(mixers.window_attention_update(q, k, v, *caches, lengths_of, cu, window=3, sinks=1), got[0])
+    close(mixers.decay_attention_update(q, k, v, log_decay, state, cu),
+          *(torch.cat([f(reference.decay(*p[:3], log_decay, absolute=absolute)[0]) for p in parts])
+            for absolute, f in ((False, lambda x: x),
+                                (True, lambda x: decay_tolerance(dtype, x, 12, D + Dv)))))
+
+
+@pytest.mark.parametrize("which", ["decay", "window"])
+def test_a_sequence_of_more_than_two_billion_elements(which):
+    """The last tokens of 140000 with 128 heads of 128 lie beyond 32 bits in every tensor; they
+    depend on the tokens just before them alone."""
+    T, H, D, tail, before = 140000, 128, 128, 64, 400
+    generator = torch.Generator(device=DEVICE).manual_seed(98)
+    draw = lambda heads: torch.randn(1, T, heads, D, device=DEVICE, dtype=torch.bfloat16, generator=generator)
+    leaves = [draw(H).requires_grad_(), draw(1).requires_grad_(), draw(1).requires_grad_()]
+    log_decay = torch.full((H,), -0.3, device=DEVICE)
+    output = mixers.decay_attention(*leaves, log_decay) if which == "decay" else \
+        mixers.window_attention(*leaves, window=100)
+    grad = draw(H)
+    gradients = torch.autograd.grad(output, leaves, grad)
+    rows = [t.detach()[0, -before:] for t in leaves]
+    if which == "decay":
+        want = [reference.decay(*rows, log_decay)[0],
+                *reference.decay(*rows, log_decay, grad_output=grad[0, -before:])]
+        bound = [reference.decay(*rows, log_decay, absolute=True)[0],
+                 *reference.decay(*rows, log_decay, grad_output=grad[0, -before:], absolute=True)]
+        # (what the tokens before count for: e^(-0.3 * 336), 1e-44)
+        tolerances = [decay_tolerance(torch.bfloat16, b, before * H, 2 * D) for b in bound]
+    else:
+        out, b, most = reference.window(*rows, 100, 0)
+        grads, bounds, _ = reference.window(*rows, 100, 0, grad_output=grad[0, -before:])
+        want = [out, *grads]
+        tolerances = window_tolerances(torch.bfloat16, [b, *bounds], most, before * H, 2 * D)
+    for name, got, w, tolerance in zip(("output", "dq", "dk", "dv"), (output, *gradients), want, tolerances):
+        close(got.detach()[0, -tail:], w[-tail:], tolerance[-tail:], name)
+
+
 def test_outputs_farther_apart_than_an_offset_of_24_bits():
     """Tokens of 70000 heads are 17.9 MB of outputs apart; a gradient of the outputs that is
     expanded has no such strides itself."""

@@ -58,8 +58,8 @@ constexpr int kDecayWaves = STATE_ONLY || sizeof(T) == 4 || !WHOLE ? 2 : 4;
 // Values are cut into slices of 64 columns, each with its part of the state (128 x 64 float32 are
 // 32 registers of four waves), rounded to the inputs' type once a chunk as the operand of the
 // queries' product.  Rounded so too: the scores; weighted values by TERMS.  Measured in bfloat16,
-// 2 x 4096 tokens, 32 heads of 128: 72 us forward, 309 MB in and out of HBM at 4.3 TB/s (and 32 and
-// 11 us for the segments' states), 213 us for the three passes of the backward, 763 MB at 3.6 TB/s;
+// 2 x 4096 tokens, 32 heads of 128: 72 us forward, 303 MB in and out of HBM at 4.2 TB/s (and 31 and
+// 8 us for the segments' states), 210 us for the three passes of the backward, 761 MB at 3.6 TB/s;
 // a large copy reaches 4.9.  What bounds it besides: a chunk takes a block 2.5 us alone on its
 // compute unit and two of them 4.1, of which no part is more than a sixth; left out one at a
 // time, of 154 us (mean of both directions): loads 24, stores 21, scores 14, the state's products
@@ -434,7 +434,7 @@ __global__ __launch_bounds__(kDecayThreads<STATE_ONLY>)
 // What every segment starts from: the segments' own sums, in their place, become the states before
 // them, in the order of the segments; what a sequence starts from is only written where that is a
 // given state (it may be overwritten by the last segment while the first still reads it).
-// kPieceElements elements of a state to a block: 67 MB in and out in 11 us (2 x 4096 tokens, 32
+// kPieceElements elements of a state to a block: 30 MB in and out in 8 us (2 x 4096 tokens, 32
 // heads of 128, four segments).  Offsets are only looked at as far as this block's accesses go; the
 // walk itself refuses the others.
 constexpr int kPieceElements = 4 * kThreads;

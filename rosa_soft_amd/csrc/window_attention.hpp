@@ -754,7 +754,7 @@ __global__ __launch_bounds__(kThreads) void window_join_keys_kernel(const float*
 // The gradients of the sinks from the tokens beyond the first block's walk: every block takes a
 // piece of kSinkRows tokens of one query head and 16 sinks, every wave 32 tokens of a tile.  (One
 // block walking all of them would be the last to finish by far.)  Measured as above, 4 sinks:
-// 28 us, most of it the reads of q and dO (134 MB, 4.8 TB/s).
+// 28 us, most of it the reads of q and dO (98 MB, 3.5 TB/s).
 template <typename T, int WIDTH, bool WHOLE>
 __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(1))) void
 window_grad_sinks_kernel(WindowArgs<T> a) {

@@ -85,12 +85,6 @@ WindowPlan window_plan(const rosa_mixer_problem& p, int window, int sinks) {
   WindowPlan plan{};
   plan.delta_bytes = aligned(static_cast<size_t>(p.H) * p.N * 4);
   const int longest = p.cu_seqlens == nullptr ? p.T : p.N;
-  if (sinks > 0 && window < longest) {
-    const size_t size = static_cast<size_t>(sinks) * (p.D + p.Dv) * 4;
-    plan.sink_slots = tile_slots(p, kSinkRows);
-    plan.sink_bytes = aligned((p.cu_seqlens == nullptr ? p.B : p.S) * p.Hkv * size);
-    plan.sink_part_bytes = aligned(static_cast<size_t>(plan.sink_slots) * p.H * size);
-  }
   // Keys of a block: 128, so that an operand read from LDS serves two products, or 64 where that
   // makes fewer than two blocks for each compute unit (240 blocks of 128 took 77 us where 448 of 64
   // take 56, 336 took 47 us where 600 take 31; 512 take 390 us, 1024 of 64 402) and where 128 do not
@@ -101,6 +95,17 @@ WindowPlan window_plan(const rosa_mixer_problem& p, int window, int sinks) {
   const int columns = padded_width(std::max(p.D, p.Dv));
   const bool pairs = p.dtype != ROSA_DTYPE_F32 || columns < 128;
   plan.key_block = pairs && tile_slots(p, 128) * p.Hkv >= kBlocks ? 128 : 64;
+  // Tokens beyond the sinks' window are up to eight more steps of the first key block's walk, or have
+  // two kernels of their own: small calls wait for the host (256 tokens, 4 heads on 2, window 64:
+  // 51 and 85 us a pass with the kernels, 46 and 76 without, on a fast and a slow host).
+  const int64_t walked = std::min<int64_t>(longest, static_cast<int64_t>(plan.key_block) + window - 1);
+  const int64_t steps = (longest - walked + 63) / 64 * (p.H / p.Hkv) * (pairs ? 1 : 2);
+  if (sinks > 0 && steps > 8) {
+    const size_t size = static_cast<size_t>(sinks) * (p.D + p.Dv) * 4;
+    plan.sink_slots = tile_slots(p, kSinkRows);
+    plan.sink_bytes = aligned((p.cu_seqlens == nullptr ? p.B : p.S) * p.Hkv * size);
+    plan.sink_part_bytes = aligned(static_cast<size_t>(plan.sink_slots) * p.H * size);
+  }
   const int64_t blocks = tile_slots(p, plan.key_block) * p.Hkv;
   const int64_t walk = std::min<int64_t>(longest, static_cast<int64_t>(plan.key_block) + window);
   const int64_t tiles = (walk + 63) / 64 * (p.H / p.Hkv);

@@ -506,7 +506,8 @@ window_grad_query_kernel(WindowArgs<T> a) {
 }
 
 // The tokens from here on see the sinks beyond their window: the first block of keys of a sequence
-// walks the tokens before it, window_grad_sinks_kernel the others.
+// walks the tokens before it, window_grad_sinks_kernel the others, or that block all of them where
+// they are few.
 __device__ __forceinline__ int64_t walk_end(int first, int keys, int window) {
   return static_cast<int64_t>(first) + keys - 1 + window;
 }
@@ -556,7 +557,9 @@ window_grad_key_kernel(WindowArgs<T> a) {
   }
   // keys of the block; the tokens [first, to) walked for them
   const int first = run.tile * kRows, behind = min(first + kRows, run.length);
-  const int to = static_cast<int>(min<int64_t>(run.length, walk_end(first, kRows, a.window)));
+  const bool all_tokens = run.tile == 0 && a.sinks > 0 && a.sink_slots == 0;
+  const int to = all_tokens ? run.length
+                            : static_cast<int>(min<int64_t>(run.length, walk_end(first, kRows, a.window)));
   const int sums = a.key_width + a.value_width;
 
   const int wave_first = first + wave * 16 * KEYS;

@@ -280,7 +280,7 @@ __global__ __launch_bounds__(kDecayThreads<STATE_ONLY>)
           range = lift_of(over_groups_max(most));
 #pragma unroll
           for (int t = 0; t < 4; ++t) score[t] *= range;
-          carried *= range / unit;
+          carried = carried * range / unit;  // (range / unit may pass float32's range)
         }
 #pragma unroll
         for (int t = 0; t < kColTiles; ++t) out[t] *= carried;

@@ -436,10 +436,14 @@ __device__ __forceinline__ void store_tiles(T* row, const f32x4 (&value)[TILES],
 
 // The power of two that brings a largest value into float16's upper range, [2^13, 2^14): float16
 // has few exponents, and what is rounded to it loses bits below 2^-14 and everything above 2^16.
-// The other types take values as they are.
+// The other types take values as they are.  At most 2^60: what stays below 2^-47 then keeps steps
+// of 2^-84 and less, far below what a float16 result shows, and neither the factor (the logarithm of
+// a subnormal number is -inf) nor a sum times it passes float32's range.
+constexpr float kMostLift = 60.0f;
 __device__ __forceinline__ float lift_of(float largest) {
-  return largest > 0.0f && largest < __builtin_inff() ? exp2_of(13.0f - floorf(log2_of(largest)))
-                                                      : 1.0f;
+  return largest > 0.0f && largest < __builtin_inff()
+             ? exp2_of(fminf(13.0f - floorf(log2_of(largest)), kMostLift))
+             : 1.0f;
 }
 
 // A factor for a sum over many tiles: set by the first tile that is not zero, lowered when a later

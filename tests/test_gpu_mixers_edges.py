@@ -1,0 +1,118 @@
+"""The mixers where their arithmetic or their launches reach an end: factors that follow the data's
+range, rows that are not finite, outputs and scratch off 16 bytes, more blocks than one launch
+dimension holds.  Tolerances as in ``test_gpu_mixers``."""
+
+import pytest
+import torch
+
+from rosa_soft_amd import mixers
+from tests import mixer_reference as reference
+from tests.test_gpu_mixers import (DEVICE, close, decay_tolerance, offsets_of, randn, rates,
+                                   window_tolerances)
+from tests.mixer_reference import float32_slack
+
+pytestmark = pytest.mark.gpu
+
+# half a step of float16's smallest numbers, on the way to a product and on the way out
+SMALLEST = 2.0**-24
+
+
+# ---------------------------------------------------------------------------
+# float16: what is rounded is scaled by a power of two that follows the data
+# ---------------------------------------------------------------------------
+
+def decay_results(leaves, log_decay, grad):
+    output = mixers.decay_attention(*leaves, log_decay)
+    return [output.detach(), *torch.autograd.grad(output, leaves, grad)]
+
+
+def check_decay(tensors, log_decay, grad, what=""):
+    """One sequence, forward and backward, every element against the definition."""
+    leaves = [t.requires_grad_() for t in tensors]
+    got = decay_results(leaves, log_decay, grad)
+    rows, go = [t.detach()[0] for t in leaves], grad[0]
+    want, bound = ([reference.decay(*rows, log_decay, absolute=absolute)[0],
+                    *reference.decay(*rows, log_decay, grad_output=go, absolute=absolute)]
+                   for absolute in (False, True))
+    tokens, width = rows[0].shape[0], rows[0].shape[-1] + rows[2].shape[-1]
+    share = rows[0].shape[1] // rows[1].shape[1]
+    for name, g, w, b in zip(("output", "dq", "dk", "dv"), got, want, bound):
+        close(g[0], w, decay_tolerance(g.dtype, b, tokens * share, width) + SMALLEST, (what, name))
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("zeros", ["keys", "values", "gradients", "queries"])
+@pytest.mark.parametrize("spans", [((0, 1900),), ((90, 1800),), ((10, 70), (130, 700), (710, 1999))])
+def test_decayed_states_pass_through_every_exponent(zeros, spans, dtype):
+    """Over tokens that are exactly zero (padding, a loss that masks a prompt) states, and the
+    gradients' states, only decay, through every exponent down to zero."""
+    heads = 6
+    q, k, v = (randn(300 + i, 1, 2000, heads if i == 0 else 3, 32, dtype=dtype) for i in range(3))
+    grad = randn(303, 1, 2000, heads, 32, dtype=dtype)
+    for begin, end in spans:
+        dict(keys=k, values=v, gradients=grad, queries=q)[zeros][:, begin:end] = 0
+    # e^-0.02 passes 2^-128 after 4400 tokens, e^-5 after 18
+    check_decay([q, k, v], rates(heads, low=0.02, high=5.0), grad)
+
+
+@pytest.mark.parametrize("rate", [0.9, 1.1, 1.3, 1.35, 1.4, 1.45, 1.6, 3.0])
+def test_scores_that_are_nothing_but_a_far_key(rate):
+    """One key in 60 tokens: the scores behind it are powers of the rate alone, 2^-90 and less."""
+    q, k, v = (randn(310 + i, 1, 256, 2, 32, dtype=torch.float16) for i in range(3))
+    keep = torch.zeros(256, dtype=torch.bool, device=DEVICE)
+    keep[::60] = True
+    k[:, ~keep] = 0
+    check_decay([q, k, v], torch.full((2,), -rate, device=DEVICE),
+                randn(313, 1, 256, 2, 32, dtype=torch.float16), rate)
+
+
+@pytest.mark.parametrize("exponent", [-149, -140, -127, -120, -114, -100, -60, -20, 0])
+@pytest.mark.parametrize("zeros", [False, True])
+def test_updates_on_top_of_states_of_every_size(exponent, zeros):
+    log_decay = rates(2)
+    q, k, v = (randn(320 + i, 1, 70, 2, 32, dtype=torch.float16) for i in range(3))
+    if zeros:
+        k[:, :66] = 0
+    start = (randn(323, 1, 2, 32, 32).double() * 2.0**exponent).float()
+    state = start.clone()
+    output = mixers.decay_attention_update(q, k, v, log_decay, state)
+    rows = [t[0] for t in (q, k, v)]
+    want, last = reference.decay(*rows, log_decay, state=start[0])
+    bound, last_bound = reference.decay(*rows, log_decay, state=start[0], absolute=True)
+    close(output[0], want, decay_tolerance(torch.float16, bound, 70, 64) + SMALLEST)
+    # (2^-126: what float32 products may flush)
+    close(state[0], last, (float32_slack(70, 32) + 2.0**-23) * last_bound + 70 * 2.0**-126)
+
+
+def peaked(tokens, heads, low_keys, seed):
+    """Queries and keys along one direction: keys in ``low_keys`` score 56 to 100 nats, head by
+    head, below the others; values and output gradients as usual."""
+    scale = 32**-0.5
+    gap = torch.linspace(56.0, 100.0, heads, device=DEVICE)
+    q, k, v = (randn(seed + i, 1, tokens, heads, 32, scale=0.25) for i in range(3))
+    q[..., 0] = 16.0
+    k[..., 0] = (gap / (2 * scale * 16.0)) * torch.where(low_keys, -1.0, 1.0).view(1, -1, 1)
+    return [t.half() for t in (q, k, v)], randn(seed + 3, 1, tokens, heads, 32, dtype=torch.float16)
+
+
+@pytest.mark.parametrize("tokens,window,sinks", [
+    (100, 30, 1),      # the sink's own block walks the tokens beyond its window
+    (2000, 50, 1),     # kernels of their own
+    (1500, 300, 20),   # sums of dO . o from the output
+])
+@pytest.mark.parametrize("low", ["sinks", "blocks"])
+@pytest.mark.parametrize("small", [1.0, 2.0**-12])
+def test_slopes_of_keys_far_below_the_maximum(low, small, tokens, window, sinks):
+    position = torch.arange(tokens, device=DEVICE)
+    low_keys = position < sinks if low == "sinks" else position // 16 % 3 != 1
+    tensors, grad = peaked(tokens, 12, low_keys, seed=330)
+    grad = grad * small
+    leaves = [t.requires_grad_() for t in tensors]
+    output = mixers.window_attention(*leaves, window=window, sinks=sinks)
+    got = [output.detach(), *torch.autograd.grad(output, leaves, grad)]
+    rows = [t.detach()[0] for t in leaves]
+    out, bound, most = reference.window(*rows, window, sinks)
+    grads, bounds, _ = reference.window(*rows, window, sinks, grad_output=grad[0])
+    tolerances = window_tolerances(torch.float16, [bound, *bounds], most, tokens, 64)
+    for name, g, w, tolerance in zip(("output", "dq", "dk", "dv"), got, (out, *grads), tolerances):
+        close(g[0], w, tolerance + SMALLEST, name)

@@ -58,7 +58,9 @@ struct DecayPlan {
 DecayPlan decay_plan(const rosa_mixer_problem& p, int passes);
 
 struct WindowPlan {
-  int64_t sink_slots;   // pieces of the tokens that see sinks beyond their window
+  int64_t sink_slots;   // pieces of the tokens that see sinks beyond their window, or none
+  int sink_rows;        // tokens of a piece
+  int sink_far;         // sequences of no more tokens than this have no pieces
   int key_block;        // keys of a block of the keys' gradients
   int key_parts;        // blocks that share the walk over the tokens that see them
   size_t delta_bytes, sink_bytes, sink_part_bytes, key_sum_bytes;
@@ -72,7 +74,7 @@ struct TokenPlan {
 };
 TokenPlan token_plan(const rosa_mixer_problem& p, int64_t capacity);
 
-constexpr int kSinkRows = 256;    // tokens of a piece
+constexpr int kSinkRows = 256;    // tokens of a piece, where memory allows
 
 #define ROSA_MIXER_LAUNCHERS(NAME)                                     \
   void window_forward_##NAME(const WindowCall& call);                  \

@@ -12,7 +12,7 @@ namespace {
 constexpr int kDecayChunk = 64;
 // Blocks that a launch should have: two for each of 256 compute units.
 constexpr int64_t kBlocks = 512;
-// Most memory that the states between the segments of a call may take.
+// Most memory that the states between the segments of a call may take, and the sums of sinks.
 constexpr int64_t kMostStateBytes = int64_t{2} << 30;
 
 size_t aligned(size_t bytes) { return (bytes + 255) / 256 * 256; }
@@ -98,13 +98,29 @@ WindowPlan window_plan(const rosa_mixer_problem& p, int window, int sinks) {
   // Tokens beyond the sinks' window are up to eight more steps of the first key block's walk, or have
   // two kernels of their own: small calls wait for the host (256 tokens, 4 heads on 2, window 64:
   // 51 and 85 us a pass with the kernels, 46 and 76 without, on a fast and a slow host).
-  const int64_t walked = std::min<int64_t>(longest, static_cast<int64_t>(plan.key_block) + window - 1);
-  const int64_t steps = (longest - walked + 63) / 64 * (p.H / p.Hkv) * (pairs ? 1 : 2);
-  if (sinks > 0 && steps > 8) {
-    const size_t size = static_cast<size_t>(sinks) * (p.D + p.Dv) * 4;
-    plan.sink_slots = tile_slots(p, kSinkRows);
-    plan.sink_bytes = aligned((p.cu_seqlens == nullptr ? p.B : p.S) * p.Hkv * size);
-    plan.sink_part_bytes = aligned(static_cast<size_t>(plan.sink_slots) * p.H * size);
+  const int64_t share = p.H / p.Hkv, near = static_cast<int64_t>(plan.key_block) + window - 1;
+  int64_t far = near + 8 / (share * (pairs ? 1 : 2)) * 64;
+  plan.sink_far = 0x7fffffff;
+  if (sinks > 0 && longest > far) {
+    // A packed sequence with pieces begins more than `far` tokens behind the one before it, so that
+    // tokens alone bound their number (see sink_place).  Their sums take at most kMostStateBytes or
+    // as many bytes as the queries and output gradients in 16 bits: with many sinks and a short
+    // window pieces get longer, and what is shorter than a piece is left to the first key block.
+    const int64_t size = static_cast<int64_t>(sinks) * (p.D + p.Dv) * 4;
+    const int64_t most = std::max<int64_t>(kMostStateBytes, int64_t{2} * p.N * p.H * (p.D + p.Dv));
+    int64_t rows = kSinkRows, pieces, sums;
+    for (;; rows *= 2, far = std::max(far, rows)) {
+      pieces = p.cu_seqlens == nullptr ? tile_slots(p, rows) : p.N / rows + p.N / far + 1;
+      sums = p.cu_seqlens == nullptr ? p.B : p.N / far + 1;
+      if (longest <= far || (pieces * p.H + sums * p.Hkv) * size <= most) break;
+    }
+    if (longest > far) {
+      plan.sink_rows = static_cast<int>(rows);
+      plan.sink_far = static_cast<int>(far);
+      plan.sink_slots = tile_slots(p, rows);
+      plan.sink_bytes = aligned(sums * p.Hkv * size);
+      plan.sink_part_bytes = aligned(pieces * p.H * size);
+    }
   }
   const int64_t blocks = tile_slots(p, plan.key_block) * p.Hkv;
   const int64_t walk = std::min<int64_t>(longest, static_cast<int64_t>(plan.key_block) + window);

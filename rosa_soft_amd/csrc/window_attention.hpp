@@ -47,8 +47,9 @@ struct WindowArgs {
   T* out;
   float *log_sum, *delta;    // [heads][tokens]
   T *grad_query, *grad_key, *grad_value;
-  float* sink_sums;          // [sequence][kv head][sink][key_width + value_width]
-  float* sink_parts;         // [sink slot][head][sink][key_width + value_width]
+  float* sink_sums;          // [sequence: sink_place][kv head][sink][key_width + value_width]
+  float* sink_parts;         // [piece: sink_place][head][sink][key_width + value_width]
+  int sink_rows, sink_far;   // tokens of a piece; longer sequences than sink_far have pieces
   const T *key_cache, *value_cache;
   const int32_t* lengths;
   int64_t capacity;
@@ -507,9 +508,22 @@ window_grad_query_kernel(WindowArgs<T> a) {
 
 // The tokens from here on see the sinks beyond their window: the first block of keys of a sequence
 // walks the tokens before it, window_grad_sinks_kernel the others, or that block all of them where
-// they are few.
+// they are few (sequences of up to sink_far tokens).
 __device__ __forceinline__ int64_t walk_end(int first, int keys, int window) {
   return static_cast<int64_t>(first) + keys - 1 + window;
+}
+
+// Where the sums of a sequence's sinks lie, and its first piece.  Packed sequences go by where they
+// begin: of two with more than sink_far tokens the second begins more than sink_far behind the first,
+// and n tokens are at most n / sink_rows + 1 pieces, so that no two share a place.
+struct SinkPlace {
+  int64_t sums, piece;
+};
+template <typename T>
+__device__ __forceinline__ SinkPlace sink_place(const WindowArgs<T>& a, const Run& run) {
+  if (a.sequences.offsets == nullptr) return {run.sequence, first_slot(a.sequences, run, a.sink_rows)};
+  const int begin = static_cast<int>(run.begin);
+  return {begin / a.sink_far, static_cast<int64_t>(begin / a.sink_rows) + begin / a.sink_far};
 }
 
 // dk and dv of the keys of a block, 16 KEYS to a wave, over the tokens that see them and the query
@@ -557,7 +571,7 @@ window_grad_key_kernel(WindowArgs<T> a) {
   }
   // keys of the block; the tokens [first, to) walked for them
   const int first = run.tile * kRows, behind = min(first + kRows, run.length);
-  const bool all_tokens = run.tile == 0 && a.sinks > 0 && a.sink_slots == 0;
+  const bool all_tokens = run.tile == 0 && a.sinks > 0 && run.length <= a.sink_far;
   const int to = all_tokens ? run.length
                             : static_cast<int>(min<int64_t>(run.length, walk_end(first, kRows, a.window)));
   const int sums = a.key_width + a.value_width;
@@ -586,7 +600,7 @@ window_grad_key_kernel(WindowArgs<T> a) {
 #pragma unroll
   for (int i = 0; i < KEYS; ++i) unit[i] = kNarrow<T> ? 0.0f : 1.0f;
   if (part == 0 && run.tile == 0 && a.sink_sums != nullptr && to < run.length) {
-    const float* sinks = a.sink_sums + (static_cast<int64_t>(run.sequence) * a.kv_heads + kv_head) * a.sinks * sums;
+    const float* sinks = a.sink_sums + (sink_place(a, run).sums * a.kv_heads + kv_head) * a.sinks * sums;
 #pragma unroll
     for (int i = 0; i < KEYS; ++i) {
       const int s = wave_first + i * 16 + column;
@@ -755,7 +769,7 @@ __global__ __launch_bounds__(kThreads) void window_join_keys_kernel(const float*
 }
 
 // The gradients of the sinks from the tokens beyond the first block's walk: every block takes a
-// piece of kSinkRows tokens of one query head and 16 sinks, every wave 32 tokens of a tile.  (One
+// piece of sink_rows tokens of one query head and 16 sinks, every wave 32 tokens of a tile.  (One
 // block walking all of them would be the last to finish by far.)  Measured as above, 4 sinks:
 // 28 us, most of it the reads of q and dO (98 MB, 3.5 TB/s).
 template <typename T, int WIDTH, bool WHOLE>
@@ -780,10 +794,10 @@ window_grad_sinks_kernel(WindowArgs<T> a) {
   const int head = static_cast<int>(item / parts % a.heads), kv_head = head / a.share;
   const int64_t slot = item / parts / a.heads;
   Run run;
-  if (find_run(a.sequences, slot, kSinkRows, tid, &run) != Found::kRun) return;
-  const int from = static_cast<int>(
-      max<int64_t>(run.tile * kSinkRows, min<int64_t>(run.length, walk_end(0, a.key_block, a.window))));
-  const int to = min(run.length, (run.tile + 1) * kSinkRows);
+  if (find_run(a.sequences, slot, a.sink_rows, tid, &run) != Found::kRun) return;
+  if (run.length <= a.sink_far) return;  // (sink_far is no less than where the first block's walk ends)
+  const int from = max(run.tile * a.sink_rows, static_cast<int>(walk_end(0, a.key_block, a.window)));
+  const int to = run.tile * a.sink_rows + min(a.sink_rows, run.length - run.tile * a.sink_rows);
   if (from >= to) return;  // (nor are its sums read)
 
   // these tokens see all sinks
@@ -876,7 +890,8 @@ window_grad_sinks_kernel(WindowArgs<T> a) {
   }
   __syncthreads();
   const int columns = a.key_width + a.value_width, there = min(16, a.sinks - first);
-  float* piece = a.sink_parts + ((slot * a.heads + head) * a.sinks + first) * columns;
+  float* piece =
+      a.sink_parts + (((sink_place(a, run).piece + run.tile) * a.heads + head) * a.sinks + first) * columns;
   for (int e = tid; e < there * columns; e += kThreads) {
     const int s = e / columns, col = e % columns;
     const int at = col < a.key_width ? s * kSumPitch + col : (16 + s) * kSumPitch + col - a.key_width;
@@ -888,7 +903,7 @@ window_grad_sinks_kernel(WindowArgs<T> a) {
 }
 
 // The pieces of window_grad_sinks_kernel, and the query heads of a group, added up in their order:
-// [sequence][kv head][sink][key_width + value_width].
+// [sequence: sink_place][kv head][sink][key_width + value_width].
 template <typename T>
 __global__ __launch_bounds__(kThreads) void window_join_sinks_kernel(WindowArgs<T> a) {
   const int tid = threadIdx.x, size = a.sinks * (a.key_width + a.value_width);
@@ -896,19 +911,19 @@ __global__ __launch_bounds__(kThreads) void window_join_sinks_kernel(WindowArgs<
   const int sequence = static_cast<int>(blockIdx.x / blocks / a.kv_heads);
   const int kv_head = static_cast<int>(blockIdx.x / blocks % a.kv_heads);
   const Run run = run_of_sequence(a.sequences, sequence);
-  if (run.length < 0) return;
+  if (run.length <= a.sink_far) return;  // (of length -1: no offsets to rely on)
   const int e = static_cast<int>(blockIdx.x % blocks) * kThreads + tid;
   if (e >= size) return;
-  const int64_t begin = walk_end(0, a.key_block, a.window);
-  if (begin >= run.length) return;
-  const int first = static_cast<int>(begin) / kSinkRows, pieces = (run.length + kSinkRows - 1) / kSinkRows;
-  const int64_t slot = first_slot(a.sequences, run, kSinkRows) + first;
+  const int first = static_cast<int>(walk_end(0, a.key_block, a.window)) / a.sink_rows;
+  const int pieces = (run.length + a.sink_rows - 1) / a.sink_rows;
+  const SinkPlace place = sink_place(a, run);
+  const int64_t slot = place.piece + first;
   const float* part = a.sink_parts + (slot * a.heads + kv_head * a.share) * size + e;
   float sum = 0.0f;
 #pragma unroll 4
   for (int i = 0; i < (pieces - first) * a.share; ++i)
     sum += part[(static_cast<int64_t>(i / a.share) * a.heads + i % a.share) * size];
-  a.sink_sums[(static_cast<int64_t>(sequence) * a.kv_heads + kv_head) * size + e] = sum;
+  a.sink_sums[(place.sums * a.kv_heads + kv_head) * size + e] = sum;
 }
 
 // ---------------------------------------------------------------------------
@@ -1329,6 +1344,8 @@ void window_backward_width(const WindowCall& call) {
   args.grad_key = static_cast<T*>(call.grad_key);
   args.grad_value = static_cast<T*>(call.grad_value);
   args.sink_slots = plan.sink_slots;
+  args.sink_rows = plan.sink_rows;
+  args.sink_far = plan.sink_far;
   const int longest = p.cu_seqlens == nullptr ? p.T : p.N;
   args.exact_delta = sizeof(T) == 2 && std::min(call.window, longest / 2) <= kExactSpan;
   args.key_block = plan.key_block;

@@ -116,3 +116,53 @@ def test_slopes_of_keys_far_below_the_maximum(low, small, tokens, window, sinks)
     tolerances = window_tolerances(torch.float16, [bound, *bounds], most, tokens, 64)
     for name, g, w, tolerance in zip(("output", "dq", "dk", "dv"), got, (out, *grads), tolerances):
         close(g[0], w, tolerance + SMALLEST, name)
+
+
+# ---------------------------------------------------------------------------
+# the sinks' gradients by pieces of tokens
+# ---------------------------------------------------------------------------
+
+def check_window_sequences(tensors, grad, lengths, window, sinks, checked=None):
+    """A packed batch, forward and backward; sequences ``checked`` against the definition."""
+    leaves = [t.requires_grad_() for t in tensors]
+    output = mixers.window_attention_varlen(*leaves, offsets_of(lengths), window=window, sinks=sinks)
+    got = [output.detach(), *torch.autograd.grad(output, leaves, grad)]
+    parts = [[t.detach().split(lengths)[s] for t in (*leaves, grad)]
+             for s in (range(len(lengths)) if checked is None else checked)]
+    results = [t.split(lengths) for t in got]
+    share = leaves[0].shape[1] // leaves[1].shape[1]
+    width = leaves[0].shape[2] + leaves[2].shape[2]
+    # results below 2^-14 have steps of 2^-24 in float16, whatever their terms: rounding is off by
+    # 2^-25 where the tolerance, relative to the terms, may be less (the last key of a sequence has
+    # the one term p dO)
+    step = SMALLEST if leaves[0].dtype == torch.float16 else 0.0
+    for place, (q, k, v, go) in zip(range(len(lengths)) if checked is None else checked, parts):
+        if len(q) == 0:
+            continue
+        out, bound, most = reference.window(q, k, v, window, sinks)
+        grads, bounds, _ = reference.window(q, k, v, window, sinks, grad_output=go)
+        tolerances = window_tolerances(q.dtype, [bound, *bounds], most, len(q) * share, width)
+        for name, g, w, tolerance in zip(("output", "dq", "dk", "dv"), results, (out, *grads), tolerances):
+            close(g[place], w, tolerance + step, (place, len(q), name))
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("heads", [(8, 8), (8, 2), (9, 1)])
+def test_pieces_of_packed_sequences_keep_apart(heads, dtype):
+    """Sequences of one token more and less than the shortest with pieces (64 or 128 keys, a window
+    of 20, up to eight more steps of 64 tokens) beside long, short and empty ones; pieces of 256
+    tokens that begin and end everywhere."""
+    lengths = [84, 83, 1, 596, 595, 0, 660, 659, 84, 257, 1300, 511, 148, 147, 3, 276, 275, 700, 85]
+    tensors = [randn(340 + i, sum(lengths), heads[i > 0], 24, dtype=dtype) for i in range(3)]
+    grad = randn(343, sum(lengths), heads[0], 24, dtype=dtype)
+    check_window_sequences(tensors, grad, lengths, 20, 5)
+
+
+def test_pieces_get_longer_where_their_sums_would_take_too_much():
+    """16 heads on one, 64 sinks, a window of 8: sums of pieces of 256 tokens would take 4.8 GB,
+    those of 512 take half, and sequences of up to 512 tokens have none."""
+    lengths = [700, 90, 200, 1500, 513, 512, 64, 1, 1024, 400] * 43
+    tensors = [randn(350 + i, sum(lengths), 16 if i == 0 else 1, 128, dtype=torch.bfloat16) for i in range(3)]
+    grad = randn(353, sum(lengths), 16, 128, dtype=torch.bfloat16)
+    checked = [*range(10), 213, 218, *range(len(lengths) - 10, len(lengths))]
+    check_window_sequences(tensors, grad, lengths, 8, 64, checked)

@@ -249,6 +249,29 @@ def test_workspaces_of_extreme_shapes_stay_bounded():
     assert library.rosa_hip_decay_workspace_bytes(ctypes.byref(token), 2) == 256  # unused
 
 
+@pytest.mark.parametrize("fields", [
+    dict(S=8192, N=65536, H=32, Hkv=32),                       # many short sequences
+    dict(S=100_000, N=200_000, H=64, Hkv=64),
+    dict(S=100_000, N=200_000, H=64, Hkv=4),
+    dict(S=1, N=2**20, H=64, Hkv=8),                           # one that may be long
+    dict(B=512, T=2048, N=2**20, H=64, Hkv=8),
+    dict(B=2**15, T=40, N=40 * 2**15, H=16, Hkv=1),
+])
+@pytest.mark.parametrize("dtype", [0, 1, 2])
+@pytest.mark.parametrize("window,sinks", [(1, 64), (128, 16), (100, 64), (1024, 4)])
+def test_workspaces_of_sinks_stay_bounded(fields, dtype, window, sinks):
+    """The backward's sums of sinks go by tokens, not by sequences: 2 GiB, or the bytes of queries
+    and output gradients in 16 bits; the parts of shared walks take up to 512 blocks of keys."""
+    library = cabi.load()
+    packed = dict(B=0, T=0, cu_seqlens=1) if "S" in fields else {}
+    p = problem(**{**dict(D=128, Dv=128, dtype=dtype), **packed, **fields})
+    size = library.rosa_hip_window_workspace_bytes(ctypes.byref(p), window, sinks, 0)
+    delta = p.N * p.H * 4
+    sums = max(2 << 30, 2 * p.N * p.H * (p.D + p.Dv))
+    parts = 512 * 128 * (p.D + p.Dv) * 4
+    assert delta <= size <= delta + sums + parts + 4 * 256
+
+
 def test_the_definitions_agree_with_step_by_step_evaluation():
     """The 64-bit definitions the GPU tests use, against one token at a time."""
     generator = torch.Generator().manual_seed(0)

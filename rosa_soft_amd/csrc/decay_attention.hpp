@@ -645,7 +645,7 @@ void decay_backward(const DecayCall& call) {
   const DecayPlan plan = decay_plan(p, 3);
   DecayArgs<T> args = decay_args<T>(call);
   args.segment_states = reinterpret_cast<float*>(call.workspace);
-  float* partial = reinterpret_cast<float*>(call.workspace + plan.state_bytes);
+  char* partial = call.workspace + plan.state_bytes;
   const View<const T> q = view_of<T>(*call.query), k = view_of<T>(*call.key),
                       v = view_of<T>(*call.value), go = view_of<T>(*call.grad_output);
   float *key_partial = nullptr, *value_partial = nullptr;
@@ -654,15 +654,12 @@ void decay_backward(const DecayCall& call) {
     args.pass[args.passes++] = {go, v, k, 1, share, share, p.Dv, p.D,
                                 static_cast<T*>(call.grad_query), nullptr, false};
   if (call.grad_key) {
-    if (share > 1) {
-      key_partial = partial;
-      partial += static_cast<int64_t>(p.N) * p.H * p.D;
-    }
+    if (share > 1) key_partial = reinterpret_cast<float*>(partial);
     args.pass[args.passes++] = {v, go, q, share, 1, 1, p.Dv, p.D,
                                 static_cast<T*>(call.grad_key), key_partial, true};
   }
   if (call.grad_value) {
-    if (share > 1) value_partial = partial;
+    if (share > 1) value_partial = reinterpret_cast<float*>(partial + plan.key_partial_bytes);
     args.pass[args.passes++] = {k, q, go, share, 1, 1, p.D, p.Dv,
                                 static_cast<T*>(call.grad_value), value_partial, true};
   }

@@ -45,7 +45,9 @@ struct DecayCall {
   hipStream_t stream;
 };
 
-// Work division, on the host alone.
+// Work division, on the host alone.  Arrays in a workspace begin 256 bytes apart, whatever their
+// widths: kernels store four elements at once.
+constexpr size_t aligned(size_t bytes) { return (bytes + 255) / 256 * 256; }
 constexpr int decay_slice(int width) { return width < 64 ? width : 64; }  // value columns of a block
 struct DecayPlan {
   int width;            // padded width of keys
@@ -53,7 +55,7 @@ struct DecayPlan {
   bool segmented;
   int64_t slots;
   size_t state_bytes;   // incoming states of all segments, all passes
-  size_t partial_bytes; // one gradient of a shared head before the sum over its group
+  size_t key_partial_bytes, value_partial_bytes;  // gradients of shared heads before the sum over a group
 };
 DecayPlan decay_plan(const rosa_mixer_problem& p, int passes);
 
@@ -63,8 +65,10 @@ struct WindowPlan {
   int sink_far;         // sequences of no more tokens than this have no pieces
   int key_block;        // keys of a block of the keys' gradients
   int key_parts;        // blocks that share the walk over the tokens that see them
-  size_t delta_bytes, sink_bytes, sink_part_bytes, key_sum_bytes;
-  size_t bytes() const { return delta_bytes + sink_bytes + sink_part_bytes + key_sum_bytes; }
+  size_t delta_bytes, sink_bytes, sink_part_bytes, key_sum_bytes, value_sum_bytes;
+  size_t bytes() const {
+    return delta_bytes + sink_bytes + sink_part_bytes + key_sum_bytes + value_sum_bytes;
+  }
 };
 WindowPlan window_plan(const rosa_mixer_problem& p, int window, int sinks);
 

@@ -15,8 +15,6 @@ constexpr int64_t kBlocks = 512;
 // Most memory that the states between the segments of a call may take, and the sums of sinks.
 constexpr int64_t kMostStateBytes = int64_t{2} << 30;
 
-size_t aligned(size_t bytes) { return (bytes + 255) / 256 * 256; }
-
 int64_t tile_slots(const rosa_mixer_problem& p, int64_t rows) {
   return p.cu_seqlens == nullptr ? static_cast<int64_t>(p.B) * ((p.T + rows - 1) / rows)
                                  : static_cast<int64_t>(p.N) / rows + p.S;
@@ -76,8 +74,10 @@ DecayPlan decay_plan(const rosa_mixer_problem& p, int passes) {
   plan.segment = static_cast<int>(std::min<int64_t>(best_segment, 0x7fffffff / kDecayChunk)) * kDecayChunk;
   plan.slots = tile_slots(p, plan.segment);
   plan.state_bytes = plan.segmented ? aligned(static_cast<size_t>(plan.slots) * state) : 0;
-  if (passes > 1 && p.H > p.Hkv)
-    plan.partial_bytes = aligned(static_cast<size_t>(p.N) * p.H * (p.D + p.Dv) * 4);
+  if (passes > 1 && p.H > p.Hkv) {
+    plan.key_partial_bytes = aligned(static_cast<size_t>(p.N) * p.H * p.D * 4);
+    plan.value_partial_bytes = aligned(static_cast<size_t>(p.N) * p.H * p.Dv * 4);
+  }
   return plan;
 }
 
@@ -126,8 +126,11 @@ WindowPlan window_plan(const rosa_mixer_problem& p, int window, int sinks) {
   const int64_t walk = std::min<int64_t>(longest, static_cast<int64_t>(plan.key_block) + window);
   const int64_t tiles = (walk + 63) / 64 * (p.H / p.Hkv);
   plan.key_parts = static_cast<int>(std::max<int64_t>(1, std::min((pairs ? kBlocks : kBlocks / 2) / blocks, tiles / 8)));
-  if (plan.key_parts > 1)
-    plan.key_sum_bytes = aligned(static_cast<size_t>(plan.key_parts) * p.N * p.Hkv * (p.D + p.Dv) * 4);
+  if (plan.key_parts > 1) {
+    const size_t rows = static_cast<size_t>(plan.key_parts) * p.N * p.Hkv;
+    plan.key_sum_bytes = aligned(rows * p.D * 4);
+    plan.value_sum_bytes = aligned(rows * p.Dv * 4);
+  }
   return plan;
 }
 
@@ -206,7 +209,7 @@ bool is_token(const rosa_mixer_problem& p) { return p.cu_seqlens == nullptr && p
 size_t decay_bytes(const rosa_mixer_problem& p, int backward) {
   if (backward == 2 && is_token(p)) return 0;
   const DecayPlan plan = decay_plan(p, backward == 1 ? 3 : 1);
-  return plan.state_bytes + plan.partial_bytes;
+  return plan.state_bytes + plan.key_partial_bytes + plan.value_partial_bytes;
 }
 
 size_t window_update_bytes(const rosa_mixer_problem& p, int64_t capacity) {

@@ -1351,8 +1351,9 @@ void window_backward_width(const WindowCall& call) {
   args.key_block = plan.key_block;
   args.key_parts = plan.key_parts;
   if (plan.key_parts > 1) {
-    args.key_sums = reinterpret_cast<float*>(call.workspace + plan.bytes() - plan.key_sum_bytes);
-    args.value_sums = args.key_sums + static_cast<int64_t>(plan.key_parts) * p.N * p.Hkv * p.D;
+    char* sums = call.workspace + plan.delta_bytes + plan.sink_bytes + plan.sink_part_bytes;
+    args.key_sums = reinterpret_cast<float*>(sums);
+    args.value_sums = reinterpret_cast<float*>(sums + plan.key_sum_bytes);
   }
   if (plan.sink_slots > 0) {
     args.sink_sums = reinterpret_cast<float*>(call.workspace + plan.delta_bytes);

@@ -166,3 +166,19 @@ def test_pieces_get_longer_where_their_sums_would_take_too_much():
     grad = randn(353, sum(lengths), 16, 128, dtype=torch.bfloat16)
     checked = [*range(10), 213, 218, *range(len(lengths) - 10, len(lengths))]
     check_window_sequences(tensors, grad, lengths, 8, 64, checked)
+
+
+# ---------------------------------------------------------------------------
+# arrays off 16 bytes
+# ---------------------------------------------------------------------------
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("widths", [(7, 12), (5, 64), (33, 100), (1, 4)])
+def test_scratch_of_odd_widths(widths, dtype):
+    """Gradients of shared heads go through two float32 arrays, the second behind odd rows."""
+    D, Dv = widths
+    tensors = [randn(360, 1, 1301, 4, D, dtype=dtype), randn(361, 1, 1301, 1, D, dtype=dtype),
+               randn(362, 1, 1301, 1, Dv, dtype=dtype)]
+    grad = randn(363, 1, 1301, 4, Dv, dtype=dtype)
+    check_decay(tensors, rates(4), grad)
+    check_window_sequences([t.detach()[0] for t in tensors], grad[0], [1301], 1301, 0)

@@ -249,6 +249,19 @@ def test_workspaces_of_extreme_shapes_stay_bounded():
     assert library.rosa_hip_decay_workspace_bytes(ctypes.byref(token), 2) == 256  # unused
 
 
+def test_every_array_of_a_workspace_begins_on_its_own_256_bytes():
+    """Of odd widths too: kernels store four float32 at once, whose address has to be whole."""
+    library = cabi.load()
+    up = lambda size: (size + 255) // 256 * 256
+    p = problem(B=1, T=129, N=129, H=3, Hkv=1, D=7, Dv=12)
+    parts = up(129 * 3 * 7 * 4) + up(129 * 3 * 12 * 4)  # (one segment: no states)
+    assert library.rosa_hip_decay_workspace_bytes(ctypes.byref(p), 1) == parts
+    # 8192 tokens, 4 heads on 1: 128 blocks of 64 keys, whose walk of 8128 tokens is shared by four
+    p = problem(B=1, T=8191, N=8191, H=4, Hkv=1, D=7, Dv=11)
+    sums = up(4 * 8191 * 7 * 4) + up(4 * 8191 * 11 * 4)
+    assert library.rosa_hip_window_workspace_bytes(ctypes.byref(p), 8191, 0, 0) == up(4 * 8191 * 4) + sums
+
+
 @pytest.mark.parametrize("fields", [
     dict(S=8192, N=65536, H=32, Hkv=32),                       # many short sequences
     dict(S=100_000, N=200_000, H=64, Hkv=64),

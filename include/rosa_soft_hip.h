@@ -368,10 +368,11 @@ int rosa_hip_router_update(const rosa_router_update* update, void* stream);
  * offsets make every output and gradient NaN and leave states and caches as they were.
  *
  * The caller owns every buffer: outputs, gradients, states and caches share no memory with what a
- * call reads (a state may be advanced in place), workspaces are 16-byte aligned and belong to one
- * call at a time.  Nothing in a workspace is kept or has to be cleared.  Entry points return 0, 1
- * (arguments), 2 (a NULL pointer), 3 (workspace too small) or 100 and more (HIP), with
- * rosa_hip_last_error().
+ * call reads (a state may be advanced in place).  Tensors may lie at any address of their element
+ * type; where all inputs and outputs of a call lie at 16-byte ones, rows are moved in whole pieces.
+ * Workspaces are 16-byte aligned and belong to one call at a time; nothing in them is kept or has
+ * to be cleared.  Entry points return 0, 1 (arguments), 2 (a NULL pointer), 3 (workspace too small)
+ * or 100 and more (HIP), with rosa_hip_last_error().
  */
 typedef struct rosa_mixer_problem {
   int dtype;

@@ -599,11 +599,13 @@ void decay_walk_any(DecayArgs<T>& args, const DecayPlan& plan, bool whole, hipSt
 }
 
 template <typename T>
-bool whole_inputs(const DecayCall& call) {
+bool whole_rows(const DecayCall& call) {
   const rosa_mixer_problem& p = *call.problem;
   return whole_pieces<T>(*call.query, p.D) && whole_pieces<T>(*call.key, p.D) &&
          whole_pieces<T>(*call.value, p.Dv) &&
-         (call.grad_output == nullptr || whole_pieces<T>(*call.grad_output, p.Dv));
+         (call.grad_output == nullptr || whole_pieces<T>(*call.grad_output, p.Dv)) &&
+         whole_address(call.out) && whole_address(call.grad_query) && whole_address(call.grad_key) &&
+         whole_address(call.grad_value);
 }
 
 template <typename T>
@@ -635,7 +637,7 @@ void decay_forward(const DecayCall& call) {
   args.passes = 1;
   args.pass[0] = decay_forward_pass<T>(call);
   args.segment_states = reinterpret_cast<float*>(call.workspace);
-  decay_walk_any<T, kTrainTerms<T>>(args, plan, whole_inputs<T>(call), call.stream);
+  decay_walk_any<T, kTrainTerms<T>>(args, plan, whole_rows<T>(call), call.stream);
 }
 
 template <typename T>
@@ -663,7 +665,7 @@ void decay_backward(const DecayCall& call) {
     args.pass[args.passes++] = {k, q, go, share, 1, 1, p.D, p.Dv,
                                 static_cast<T*>(call.grad_value), value_partial, true};
   }
-  decay_walk_any<T, kTrainTerms<T>>(args, plan, whole_inputs<T>(call), call.stream);
+  decay_walk_any<T, kTrainTerms<T>>(args, plan, whole_rows<T>(call), call.stream);
   const int64_t rows = static_cast<int64_t>(p.N) * p.Hkv;
   const auto blocks = [&](int width) {
     return dim3(static_cast<unsigned>((rows * width + kThreads - 1) / kThreads));
@@ -703,7 +705,7 @@ void decay_update(const DecayCall& call) {
   args.segment_states = reinterpret_cast<float*>(call.workspace);
   args.state_in = call.state_in;
   args.state_out = call.state_out;
-  decay_walk_any<T, kUpdateTerms<T>>(args, plan, whole_inputs<T>(call), call.stream);
+  decay_walk_any<T, kUpdateTerms<T>>(args, plan, whole_rows<T>(call), call.stream);
 }
 
 }  // namespace rosa_mixer

@@ -361,7 +361,7 @@ __device__ __forceinline__ void clear_operand(Frag<T>& operand, int col0, int gr
   }
 }
 
-// four neighbouring elements of a contiguous output row; `quads`: rows are whole quads
+// four neighbouring elements of a contiguous output row; `quads`: it is whole quads at their addresses
 template <typename T>
 __device__ __forceinline__ void store4(T* row, int col, f32x4 value, int width, bool quads) {
   if (quads) {
@@ -428,9 +428,9 @@ __device__ __forceinline__ void store_tiles(T* row, const f32x4 (&value)[TILES],
       }
     }
   } else {
+    const bool quads = WHOLE || (width % 4 == 0 && reinterpret_cast<uintptr_t>(row) % sizeof(Quad<T>) == 0);
 #pragma unroll
-    for (int t = 0; t < TILES; ++t)
-      store4(row, t * 16 + 4 * group, scaled[t], width, WHOLE || width % 4 == 0);
+    for (int t = 0; t < TILES; ++t) store4(row, t * 16 + 4 * group, scaled[t], width, quads);
   }
 }
 
@@ -595,6 +595,7 @@ View<const T> view_of(const rosa_mixer_tensor& t) {
 }
 
 // rows of whole 16-byte pieces at 16-byte addresses, less than 2^24 bytes apart
+inline bool whole_address(const void* data) { return reinterpret_cast<uintptr_t>(data) % 16 == 0; }
 template <typename T>
 bool whole_stride(int64_t stride) {
   return stride >= 0 && stride < (1 << 24) / static_cast<int64_t>(sizeof(T));
@@ -602,7 +603,7 @@ bool whole_stride(int64_t stride) {
 template <typename T>
 bool whole_pieces(const rosa_mixer_tensor& t, int width) {
   const int64_t piece = 16 / sizeof(T);
-  return reinterpret_cast<uintptr_t>(t.data) % 16 == 0 && width % piece == 0 &&
+  return whole_address(t.data) && width % piece == 0 &&
          t.batch_stride % piece == 0 && t.token_stride % piece == 0 && t.head_stride % piece == 0 &&
          whole_stride<T>(t.token_stride);
 }

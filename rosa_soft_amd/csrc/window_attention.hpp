@@ -1231,14 +1231,15 @@ constexpr int64_t kFull = 1024;
 template <typename T, int WIDTH> constexpr bool kPairs = !(sizeof(T) == 4 && WIDTH == 128);
 
 template <typename T>
-bool whole_inputs(const WindowCall& call) {
+bool whole_rows(const WindowCall& call) {
   const rosa_mixer_problem& p = *call.problem;
-  const auto aligned = [](const void* data) { return reinterpret_cast<uintptr_t>(data) % 16 == 0; };
   return whole_pieces<T>(*call.query, p.D) && whole_pieces<T>(*call.key, p.D) &&
          whole_pieces<T>(*call.value, p.Dv) &&
          (call.grad_output == nullptr || (whole_pieces<T>(*call.grad_output, p.Dv) &&
                                           whole_stride<T>(static_cast<int64_t>(p.H) * p.Dv))) &&
-         aligned(call.output) && aligned(call.key_cache) && aligned(call.value_cache);
+         whole_address(call.output) && whole_address(call.key_cache) && whole_address(call.value_cache) &&
+         whole_address(call.out) && whole_address(call.grad_query) && whole_address(call.grad_key) &&
+         whole_address(call.grad_value);
 }
 
 template <typename T, int WIDTH, int QUERIES, bool CACHED, bool WHOLE>
@@ -1271,7 +1272,7 @@ void window_forward_width(const WindowCall& call) {
 
 template <typename T>
 void window_forward(const WindowCall& call) {
-  if (whole_inputs<T>(call))
+  if (whole_rows<T>(call))
     window_forward_width<T, true>(call);
   else
     window_forward_width<T, false>(call);
@@ -1368,7 +1369,7 @@ void window_backward_width(const WindowCall& call) {
 
 template <typename T>
 void window_backward(const WindowCall& call) {
-  if (whole_inputs<T>(call))
+  if (whole_rows<T>(call))
     window_backward_width<T, true>(call);
   else
     window_backward_width<T, false>(call);
@@ -1413,7 +1414,7 @@ void window_update_width(const WindowCall& call) {
 
 template <typename T>
 void window_update(const WindowCall& call) {
-  if (whole_inputs<T>(call))
+  if (whole_rows<T>(call))
     window_update_width<T, true>(call);
   else
     window_update_width<T, false>(call);

@@ -2,10 +2,12 @@
 range, rows that are not finite, outputs and scratch off 16 bytes, more blocks than one launch
 dimension holds.  Tolerances as in ``test_gpu_mixers``."""
 
+import ctypes
+
 import pytest
 import torch
 
-from rosa_soft_amd import mixers
+from rosa_soft_amd import cabi, mixers
 from tests import mixer_reference as reference
 from tests.test_gpu_mixers import (DEVICE, close, decay_tolerance, offsets_of, randn, rates,
                                    window_tolerances)
@@ -182,3 +184,63 @@ def test_scratch_of_odd_widths(widths, dtype):
     grad = randn(363, 1, 1301, 4, Dv, dtype=dtype)
     check_decay(tensors, rates(4), grad)
     check_window_sequences([t.detach()[0] for t in tensors], grad[0], [1301], 1301, 0)
+
+
+class Shifted:
+    """Memory for an output ``shift`` elements behind a 16-byte address, NaN around it."""
+
+    def __init__(self, like, shift):
+        self.shift, self.like = shift, like
+        self.memory = torch.full((like.numel() + 16,), float("nan"), dtype=like.dtype, device=DEVICE)
+
+    @property
+    def pointer(self):
+        return self.memory.data_ptr() + self.shift * self.memory.element_size()
+
+    def check(self, want):
+        inside = self.memory[self.shift:self.shift + want.numel()]
+        assert torch.equal(inside.view(want.shape), want)
+        outside = torch.cat([self.memory[:self.shift], self.memory[self.shift + want.numel():]])
+        assert bool(torch.isnan(outside).all())
+
+
+def described(tensor):
+    return ctypes.byref(cabi.RosaMixerTensor(tensor.data_ptr(), tensor.stride(0), *tensor.stride()[1:3]))
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("shift", [0, 1, 2, 3, 4, 6])
+@pytest.mark.parametrize("width", [64, 36])
+def test_c_entries_write_outputs_at_any_element(width, shift, dtype):
+    """Callers of the C interface choose where outputs and gradients lie."""
+    library = cabi.load()
+    q, k, v = (randn(370 + i, 2, 150, 4 if i == 0 else 2, width, dtype=dtype) for i in range(3))
+    grad = randn(373, 2, 150, 4, width, dtype=dtype)
+    log_decay, scale = rates(4), width**-0.5
+    code = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}[dtype]
+    problem = ctypes.byref(cabi.RosaMixerProblem(code, 2, 150, 300, 0, 4, 2, width, width, scale, None))
+    rows, go = [described(t) for t in (q, k, v)], described(grad)
+    stream = torch.cuda.current_stream().cuda_stream
+    workspace = torch.empty(1 << 24, dtype=torch.uint8, device=DEVICE)
+    space = (workspace.data_ptr(), workspace.numel(), stream)
+
+    leaves = [t.clone().requires_grad_() for t in (q, k, v)]
+    want = decay_results(leaves, log_decay, grad)
+    outs = [Shifted(t, shift) for t in want]
+    assert library.rosa_hip_decay_forward(problem, *rows, log_decay.data_ptr(), outs[0].pointer, *space) == 0
+    assert library.rosa_hip_decay_backward(problem, *rows, go, log_decay.data_ptr(),
+                                           *(o.pointer for o in outs[1:]), *space) == 0
+    for out, tensor in zip(outs, want):
+        out.check(tensor)
+
+    output, log_sum = torch.ops.rosa_soft.window_attention(*leaves, None, 40, 2, None, True)
+    want = [output.detach(), *torch.autograd.grad(output, leaves, grad)]
+    outs = [Shifted(t, shift) for t in want]
+    sums = torch.empty_like(log_sum)
+    assert library.rosa_hip_window_forward(problem, 40, 2, *rows, outs[0].pointer, sums.data_ptr(), stream) == 0
+    # (the forward's output is read where it was written)
+    assert library.rosa_hip_window_backward(problem, 40, 2, *rows, outs[0].pointer, sums.data_ptr(), go,
+                                            *(o.pointer for o in outs[1:]), *space) == 0
+    for out, tensor in zip(outs, want):
+        out.check(tensor)
+    assert torch.equal(sums, log_sum)

@@ -58,7 +58,7 @@ struct WindowArgs {
   int heads, kv_heads, share, key_width, value_width, window, sinks;
   int key_block;             // keys of a block of window_grad_key_kernel
   int key_parts;             // blocks that share its walk
-  bool exact_delta;          // delta is there already
+  bool exact_delta;          // delta of sequences whose tokens see few others is there already
   float *key_sums, *value_sums;  // [part][tokens][kv heads][width], where there is more than one
   float scale;
 };
@@ -323,12 +323,16 @@ window_forward_kernel(WindowArgs<T> a) {
 // dq, and the sums delta = dO . o = sum_s p_s dO . v_s that the gradients of keys need too.  The
 // walk of the forward pass.  Where tokens see many others delta is taken from the output, whose
 // rounding is small beside dO . v then.  Where they see kExactSpan or fewer (the window, or half
-// of the longest sequence) it would add half as much error again (dq and dk of 50 tokens in
+// of their sequence) it would add half as much error again (dq and dk of 50 tokens in
 // bfloat16: 2.8e-3 of their norm instead of 2.4e-3), and a walk of its own sums delta over the
 // keys first (DELTA: 27 us of 150, forward included, at 6 x 520 tokens, 22 heads, window 40).
+// Packed calls go by their mean length when that walk is launched, and sequence by sequence in it.
 // Slopes are rounded to the inputs' type, in float16 scaled to its upper range (follow_range).
 // Measured as above: 245 us, 740 TFLOP/s.
 constexpr int kExactSpan = 256;
+__host__ __device__ __forceinline__ bool few_seen(int window, int length) {
+  return window <= kExactSpan || length / 2 <= kExactSpan;
+}
 
 template <typename T, int WIDTH, int QUERIES, bool WHOLE, bool DELTA>
 __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(kWaves<T, WIDTH, WHOLE>))) void
@@ -354,6 +358,8 @@ window_grad_query_kernel(WindowArgs<T> a) {
                a.key_width, tid);
     return;
   }
+  const bool exact_delta = a.exact_delta && few_seen(a.window, run.length);
+  if (DELTA && !exact_delta) return;
   const int first = run.tile * kRows, last = min(first + kRows, run.length) - 1;
   const History<T, false> key_rows = history_of<false>(a, a.key, a.key_cache, a.key_width, run, kv_head, 0);
   const History<T, false> value_rows =
@@ -389,7 +395,7 @@ window_grad_query_kernel(WindowArgs<T> a) {
     log_sum[i] = a.log_sum[at];
     if constexpr (DELTA) {
       delta[i] = 0.0f;
-    } else if (a.exact_delta) {
+    } else if (exact_delta) {
       delta[i] = a.delta[at];
     } else {
       delta[i] = over_groups_sum(dot);
@@ -1347,8 +1353,7 @@ void window_backward_width(const WindowCall& call) {
   args.sink_slots = plan.sink_slots;
   args.sink_rows = plan.sink_rows;
   args.sink_far = plan.sink_far;
-  const int longest = p.cu_seqlens == nullptr ? p.T : p.N;
-  args.exact_delta = sizeof(T) == 2 && std::min(call.window, longest / 2) <= kExactSpan;
+  args.exact_delta = sizeof(T) == 2 && few_seen(call.window, p.cu_seqlens == nullptr ? p.T : p.N / p.S);
   args.key_block = plan.key_block;
   args.key_parts = plan.key_parts;
   if (plan.key_parts > 1) {

@@ -11,7 +11,7 @@ from rosa_soft_amd import cabi, mixers
 from tests import mixer_reference as reference
 from tests.test_gpu_mixers import (DEVICE, close, decay_tolerance, offsets_of, randn, rates,
                                    window_tolerances)
-from tests.mixer_reference import float32_slack
+from tests.mixer_reference import HALF_STEP, float32_slack
 
 pytestmark = pytest.mark.gpu
 
@@ -244,3 +244,34 @@ def test_c_entries_write_outputs_at_any_element(width, shift, dtype):
     for out, tensor in zip(outs, want):
         out.check(tensor)
     assert torch.equal(sums, log_sum)
+
+
+# ---------------------------------------------------------------------------
+# packed as dense
+# ---------------------------------------------------------------------------
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("lengths", [[32] * 64, [32] * 20 + [600] + [1, 400, 7, 513, 512] * 2])
+def test_packed_sequences_have_the_gradients_that_they_have_alone(lengths, dtype):
+    """Under a window that none of them fills: the sums dO . o are exact where a sequence is short,
+    whatever it is packed with, and come from the output where it is long."""
+    heads, masks = 2, dict(window=1024, sinks=0)
+    tensors = [randn(380 + i, sum(lengths), heads, 40, dtype=dtype) for i in range(3)]
+    grad = randn(383, sum(lengths), heads, 40, dtype=dtype)
+    leaves = [t.requires_grad_() for t in tensors]
+    output = mixers.window_attention_varlen(*leaves, offsets_of(lengths), **masks)
+    got = [t.split(lengths) for t in (output.detach(), *torch.autograd.grad(output, leaves, grad))]
+    for s in range(len(lengths)):
+        alone = [t.detach().split(lengths)[s].unsqueeze(0).clone().requires_grad_() for t in leaves]
+        output = mixers.window_attention(*alone, **masks)
+        want = [output.detach(), *torch.autograd.grad(output, alone, grad.split(lengths)[s].unsqueeze(0))]
+        for name, g, w in zip(("output", "dq"), got, want):
+            assert torch.equal(g[s], w[0]), (s, lengths[s], name)
+        # dk and dv are float32 sums over the tokens, in parts whose number goes by all tokens of a
+        # call: the order of a sum may differ, float32_slack of its terms, and with it the rounding
+        # of the result, half a step on either side
+        rows = [t.detach()[0] for t in alone]
+        _, bounds, _ = reference.window(*rows, *masks.values(), grad_output=grad.split(lengths)[s])
+        for g, w, bound in zip(got[2:], want[2:], bounds[1:]):
+            step = 2 * HALF_STEP[dtype] * w[0].double().abs() + (SMALLEST if dtype == torch.float16 else 0.0)
+            close(g[s], w[0].double(), step + float32_slack(lengths[s], 80) * bound, (s, lengths[s]))

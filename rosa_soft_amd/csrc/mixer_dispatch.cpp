@@ -570,9 +570,19 @@ bool needs_backward(const Tensors&... tensors) {
   return at::GradMode::is_enabled() && (tensors.requires_grad() || ...);
 }
 
+// There is no forward-mode derivative: a tangent is refused, not dropped.
+bool has_tangent(const Tensor& tensor) { return tensor._fw_grad(/*level=*/0).defined(); }
+template <typename... Tensors>
+void refuse_tangents(const Tensors&... tensors) {
+  TORCH_CHECK_NOT_IMPLEMENTED(
+      !(c10::AutogradState::get_tls_state().get_fw_grad_mode() && (has_tangent(tensors) || ...)),
+      "the mixers have no forward-mode derivative: their inputs must not be dual tensors");
+}
+
 Tensor decay_attention_autograd(const Tensor& query, const Tensor& key, const Tensor& value,
                                 const OptionalTensor& cu_seqlens, const Tensor& log_decay,
                                 Scale scale) {
+  refuse_tangents(query, key, value, log_decay);
   REQUIRE(!needs_backward(log_decay),
           "log_decay is a constant of each head and takes no gradient: detach it");
   if (!needs_backward(query, key, value)) {
@@ -588,6 +598,7 @@ std::tuple<Tensor, Tensor> window_attention_autograd(const Tensor& query, const 
                                                      const OptionalTensor& cu_seqlens,
                                                      int64_t window, int64_t sinks, Scale scale,
                                                      bool want_log_sum) {
+  refuse_tangents(query, key, value);
   if (!needs_backward(query, key, value)) {
     at::AutoDispatchBelowADInplaceOrView below;
     return call_window(query, key, value, cu_seqlens, window, sinks, scale, want_log_sum);
@@ -608,6 +619,10 @@ void note_change(const std::decay_t<Declared>& argument) {
 // Operators without a backward: whatever asks for one is refused, not cut off in silence.
 template <auto* kOperator, typename... Arguments>
 auto without_backward(Arguments... arguments) {
+  const auto look_at = [](const auto& argument) {
+    if constexpr (std::is_same_v<std::decay_t<decltype(argument)>, Tensor>) refuse_tangents(argument);
+  };
+  (look_at(arguments), ...);
   const auto asks = [](const auto& argument) {
     if constexpr (std::is_same_v<std::decay_t<decltype(argument)>, Tensor>)
       return argument.requires_grad();

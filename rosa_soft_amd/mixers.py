@@ -13,8 +13,8 @@ forms, ``(N, heads, width)`` with device ``cu_seqlens``; heads of keys and value
 groups of query heads; dtypes float32, float16 and bfloat16, head widths 1 to 128.  Inputs may be
 strided (the parts of a fused projection) as long as the elements of a head are neighbours;
 others are copied.  Gradients come in the dtype of their input, the same on every run, once
-differentiable, and like that of ``rosa_soft`` the backward cannot be recorded into a HIP graph;
-everything else can.
+differentiable and in reverse mode alone (dual tensors are refused), and like that of
+``rosa_soft`` the backward cannot be recorded into a HIP graph; everything else can.
 
 The ``_update`` forms serve slots, like ``RosaRuntime.update``: a chunk of one or more tokens per
 slot (or a packed chunk with ``cu_seqlens``, in which slots may bring none) on top of the slots'

@@ -119,6 +119,33 @@ def test_refusals(names, changes, error, message):
             calls(arguments(**changes()))[name]()
 
 
+@pytest.mark.parametrize("names,which", [
+    (EVERY, "q"), (EVERY, "k"), (EVERY, "v"), (EVERY[:2], "log_decay"), (EVERY[1:2], "state"),
+    (EVERY[3:], "keys"), (EVERY[3:], "values"),
+])
+def test_tangents_are_refused(names, which):
+    """Forward-mode derivatives do not exist: a dual input is an error, not an output without one."""
+    from torch.autograd import forward_ad
+
+    with FakeTensorMode():
+        for name in names:
+            with forward_ad.dual_level():
+                parts = arguments(fake)
+                parts[which] = forward_ad.make_dual(parts[which], torch.ones_like(parts[which]))
+                with pytest.raises(NotImplementedError, match="forward-mode"):
+                    calls(parts)[name]()
+            calls(arguments(fake))[name]()
+        with forward_ad.dual_level():
+            q, k, v = (fake(2, 5, 2, 8) for _ in range(3))
+            dual = forward_ad.make_dual(q, q)
+            for call in (
+                    lambda: torch.ops.rosa_soft.window_attention(dual, k, v, None, 3, 0),
+                    lambda: torch.ops.rosa_soft.decay_attention_vjp(
+                        q, k, v, None, fake(2, dtype=torch.float32), dual, None, 7)):
+                with pytest.raises(NotImplementedError, match="forward-mode"):
+                    call()
+
+
 def test_states_share_no_memory_with_what_is_read():
     """A block may store a state while another still reads its keys or rates."""
     memory = torch.zeros(2 * 4 * 16 * 8 + 64)

@@ -360,8 +360,8 @@ int rosa_hip_router_update(const rosa_router_update* update, void* stream);
  *            t - s < window or s < sinks (0 <= sinks <= 64).
  *
  * Layouts as for rosa_problem: dense (B sequences of T tokens, N = B T, S = 0, cu_seqlens NULL) or
- * packed (N tokens cut by cu_seqlens into S sequences, B = T = 0).  query [.., H, D], key
- * [.., Hkv, D], value [.., Hkv, Dv]; D and Dv in [1, 128].  Inputs are described by strides in
+ * packed (N tokens cut by cu_seqlens into S sequences, B = T = 0); T, or N packed, is below
+ * 2^31 - 1024.  query [.., H, D], key [.., Hkv, D], value [.., Hkv, Dv]; D and Dv in [1, 128].  Inputs are described by strides in
  * elements, with neighbouring elements inside a head; outputs and gradients are contiguous
  * [N, heads, width] in the problem's dtype and fully overwritten.  Sums, states and softmax
  * statistics are float32.  Results do not depend on the order in which blocks run.  Invalid device

@@ -129,7 +129,7 @@ __global__ __launch_bounds__(kDecayThreads<STATE_ONLY>)
     return;
   }
   const int start = run.tile * a.segment;                       // in the order of the walk
-  const int stop = min(start + a.segment, run.length);
+  const int stop = start + min(a.segment, run.length - start);
   if (STATE_ONLY && stop == run.length) return;                 // nothing follows this segment
   const float rate = a.log_decay[head] * 1.4426950408889634f;
 
@@ -445,7 +445,7 @@ __global__ __launch_bounds__(kThreads) void decay_join_kernel(DecayArgs<T> a, in
   const int pass_index = static_cast<int>(row / a.heads % a.passes);
   const int sequence = static_cast<int>(row / a.heads / a.passes);
   const Run run = run_of_sequence(a.sequences, sequence);
-  const int segments = run.length < 0 ? 0 : (run.length + a.segment - 1) / a.segment;
+  const int segments = tiles_of(run.length, a.segment);  // (of length -1: no offsets to rely on)
   if (segments < (a.state_in == nullptr ? 2 : 1)) return;
   const int64_t slot = first_slot(a.sequences, run, a.segment);
   const float decay = power_of(a.log_decay[head] * 1.4426950408889634f, a.segment);

@@ -17,6 +17,8 @@ constexpr int kWidths[] = {32, 64, 128};  // padded head widths that kernels exi
 constexpr int kMostWidth = 128;
 constexpr int kMostSinks = 64;
 constexpr int kMostSplits = 512;
+// Tokens of a call that is packed, or of a sequence: kernels count a tile and a window past the last.
+constexpr int kMostTokens = 0x7fffffff - 1024;
 
 constexpr int padded_width(int widest) { return widest <= 32 ? 32 : widest <= 64 ? 64 : 128; }
 

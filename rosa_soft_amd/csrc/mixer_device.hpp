@@ -492,8 +492,11 @@ struct Run {
 // leaves every sequence room for all its tiles (a sequence of n tokens has at most
 // (begin + n) / rows - begin / rows + 1 of them) and needs no table; dense sequences have a
 // fixed number of tiles each.
+__host__ __device__ __forceinline__ int tiles_of(int length, int rows) {
+  return length > 0 ? (length - 1) / rows + 1 : 0;  // (length + rows may pass 32 bits)
+}
 __host__ __device__ __forceinline__ int64_t slots_of(const Sequences& q, int rows) {
-  return q.offsets == nullptr ? static_cast<int64_t>(q.count) * ((q.length + rows - 1) / rows)
+  return q.offsets == nullptr ? static_cast<int64_t>(q.count) * tiles_of(q.length, rows)
                               : static_cast<int64_t>(q.tokens) / rows + q.count;
 }
 
@@ -505,7 +508,7 @@ template <int THREADS = kThreads>
 __device__ __forceinline__ Found find_run(const Sequences& q, int64_t slot, int rows, int tid,
                                           Run* run) {
   if (q.offsets == nullptr) {
-    const int tiles = (q.length + rows - 1) / rows;
+    const int tiles = tiles_of(q.length, rows);
     run->sequence = static_cast<int>(slot / tiles);
     run->tile = static_cast<int>(slot % tiles);
     run->length = q.length;
@@ -556,7 +559,7 @@ __device__ __forceinline__ Run run_of_sequence(const Sequences& q, int sequence)
 
 // The slot of a sequence's first tile.
 __device__ __forceinline__ int64_t first_slot(const Sequences& q, const Run& run, int rows) {
-  return q.offsets == nullptr ? static_cast<int64_t>(run.sequence) * ((q.length + rows - 1) / rows)
+  return q.offsets == nullptr ? static_cast<int64_t>(run.sequence) * tiles_of(q.length, rows)
                               : run.begin / rows + run.sequence;
 }
 

@@ -28,6 +28,7 @@ using OptionalTensor = std::optional<Tensor>;
 using Guard = c10::hip::HIPGuardMasqueradingAsCUDA;
 
 constexpr int64_t kIntMax = std::numeric_limits<int>::max();
+constexpr int64_t kMostTokens = kIntMax - 1024;  // of a sequence, or of a packed call
 constexpr int64_t kMostWidth = 128;
 constexpr int64_t kMostSinks = 64;
 
@@ -108,6 +109,7 @@ double check_call(const Tensor& query, const Tensor& key, const Tensor& value,
           "head widths must be in [1, 128]");
   REQUIRE(empty || tokens >= 1, "batch and sequence dimensions must be >= 1");
   REQUIRE(tokens <= kIntMax && tokens * heads <= kIntMax, "tokens times heads must fit in int32");
+  REQUIRE(query.size(rank - 3) <= kMostTokens, "a sequence must have at most 2^31 - 1025 tokens");
   REQUIRE(query.device() == key.device() && query.device() == value.device(),
           "all inputs must be on the same device");
   REQUIRE(query.scalar_type() == key.scalar_type() && query.scalar_type() == value.scalar_type(),

@@ -159,6 +159,8 @@ int check(const rosa_mixer_problem* p, bool update) {
     if (p->B < 1 || p->T < 1) return rosa_fail(1, "dense layout needs B >= 1 and T >= 1");
     if (static_cast<int64_t>(p->B) * p->T != p->N) return rosa_fail(1, "dense layout needs N = B * T");
   }
+  if ((p->cu_seqlens != nullptr ? p->N : p->T) > kMostTokens)
+    return rosa_fail(1, "a sequence must have at most 2^31 - 1025 tokens");
   if (p->H < 1 || p->Hkv < 1 || p->H % p->Hkv != 0)
     return rosa_fail(1, "query heads must be a positive multiple of key and value heads");
   if (p->D < 1 || p->D > kMostWidth || p->Dv < 1 || p->Dv > kMostWidth)

@@ -921,7 +921,7 @@ __global__ __launch_bounds__(kThreads) void window_join_sinks_kernel(WindowArgs<
   const int e = static_cast<int>(blockIdx.x % blocks) * kThreads + tid;
   if (e >= size) return;
   const int first = static_cast<int>(walk_end(0, a.key_block, a.window)) / a.sink_rows;
-  const int pieces = (run.length + a.sink_rows - 1) / a.sink_rows;
+  const int pieces = tiles_of(run.length, a.sink_rows);
   const SinkPlace place = sink_place(a, run);
   const int64_t slot = place.piece + first;
   const float* part = a.sink_parts + (slot * a.heads + kv_head * a.share) * size + e;

@@ -119,6 +119,25 @@ def test_refusals(names, changes, error, message):
             calls(arguments(**changes()))[name]()
 
 
+@pytest.mark.parametrize("tokens,refused", [(2**31 - 1025, False), (2**31 - 1024, True), (2**31 - 1, True)])
+def test_sequences_end_where_counts_past_their_last_tile_still_fit(tokens, refused):
+    """Kernels count up to a tile of tokens past the last one, in 32 bits."""
+    long = torch.zeros(1, 1, 1, 1).expand(1, tokens, 1, 1)
+    message = "at most 2\\^31 - 1025" if refused else "require CUDA tensors"
+    offsets = torch.tensor([0, 5], dtype=torch.int32)
+    for call in (lambda: mixers.decay_attention(long, long, long, torch.zeros(1)),
+                 lambda: mixers.window_attention(long, long, long, window=3),
+                 lambda: mixers.window_attention_varlen(long[0], long[0], long[0], offsets, window=3),
+                 lambda: mixers.decay_attention_update(long, long, long, torch.zeros(1), torch.zeros(1, 1, 1, 1))):
+        with pytest.raises(ValueError, match=message):
+            call()
+    library = cabi.load()
+    for fields in (dict(B=1, T=tokens), dict(B=0, T=0, S=3, cu_seqlens=1)):
+        p = ctypes.byref(problem(N=tokens, H=1, Hkv=1, D=1, Dv=1, **fields))
+        assert (library.rosa_hip_decay_workspace_bytes(p, 0) == 0) == refused
+        assert (library.rosa_hip_window_workspace_bytes(p, 10, 2, 0) == 0) == refused
+
+
 @pytest.mark.parametrize("names,which", [
     (EVERY, "q"), (EVERY, "k"), (EVERY, "v"), (EVERY[:2], "log_decay"), (EVERY[1:2], "state"),
     (EVERY[3:], "keys"), (EVERY[3:], "values"),

@@ -440,10 +440,13 @@ __global__ __launch_bounds__(kDecayThreads<STATE_ONLY>)
 constexpr int kPieceElements = 4 * kThreads;
 template <typename T>
 __global__ __launch_bounds__(kThreads) void decay_join_kernel(DecayArgs<T> a, int64_t state_size) {
-  const int64_t pieces = (state_size + kPieceElements - 1) / kPieceElements, row = blockIdx.x / pieces;
+  const uint32_t block = block_number();
+  const uint32_t pieces = static_cast<uint32_t>((state_size + kPieceElements - 1) / kPieceElements),
+                 row = block / pieces;
   const int head = static_cast<int>(row % a.heads);
   const int pass_index = static_cast<int>(row / a.heads % a.passes);
   const int sequence = static_cast<int>(row / a.heads / a.passes);
+  if (sequence >= a.sequences.count) return;
   const Run run = run_of_sequence(a.sequences, sequence);
   const int segments = tiles_of(run.length, a.segment);  // (of length -1: no offsets to rely on)
   if (segments < (a.state_in == nullptr ? 2 : 1)) return;
@@ -451,8 +454,9 @@ __global__ __launch_bounds__(kThreads) void decay_join_kernel(DecayArgs<T> a, in
   const float decay = power_of(a.log_decay[head] * 1.4426950408889634f, a.segment);
   const int64_t step = a.heads * state_size;
   constexpr int kAhead = 4;  // loads under way: a load behind each store took 16 us for 53 segments
-  const int64_t end = min((blockIdx.x % pieces + 1) * kPieceElements, state_size);
-  for (int64_t e = blockIdx.x % pieces * kPieceElements + threadIdx.x; e < end; e += kThreads) {
+  const int64_t begin = static_cast<int64_t>(block % pieces) * kPieceElements;
+  const int64_t end = min(begin + kPieceElements, state_size);
+  for (int64_t e = begin + threadIdx.x; e < end; e += kThreads) {
     float state = a.state_in == nullptr
                       ? 0.0f
                       : a.state_in[(static_cast<int64_t>(sequence) * a.heads + head) * state_size + e];
@@ -477,7 +481,7 @@ __global__ __launch_bounds__(kThreads) void decay_join_kernel(DecayArgs<T> a, in
 template <typename T>
 __global__ __launch_bounds__(kThreads) void sum_shared_kernel(const float* partial, T* out,
                                                               int64_t rows, int share, int width) {
-  const int64_t e = static_cast<int64_t>(blockIdx.x) * kThreads + threadIdx.x;
+  const int64_t e = static_cast<int64_t>(block_number()) * kThreads + threadIdx.x;
   if (e >= rows * width) return;
   const int64_t row = e / width, col = e % width;
   float sum = 0.0f;
@@ -496,7 +500,7 @@ struct DecayTokenArgs {
   const float* state_in;
   float* state_out;
   T* out;
-  int heads, share, key_width, value_width, slice;  // value columns of a block
+  int slots, heads, share, key_width, value_width, slice;  // value columns of a block
   float scale;
 };
 
@@ -508,8 +512,10 @@ __global__ __launch_bounds__(kThreads) void decay_token_kernel(DecayTokenArgs<T>
   __shared__ float sums[kThreads * VEC];
   const int tid = threadIdx.x;
   const int slices = (a.value_width + a.slice - 1) / a.slice;
-  const int col0 = blockIdx.x % slices * a.slice;
-  const int head = blockIdx.x / slices % a.heads, batch = blockIdx.x / slices / a.heads;
+  const uint32_t block = block_number();
+  const int col0 = block % slices * a.slice;
+  const int head = block / slices % a.heads, batch = block / slices / a.heads;
+  if (batch >= a.slots) return;
   const int columns = min(a.slice, a.value_width - col0);
   if (tid < a.key_width) {
     query[tid] = static_cast<float>(a.query.row(batch, 0, head)[tid]);
@@ -566,13 +572,13 @@ void decay_walk(DecayArgs<T>& args, const DecayPlan& plan, hipStream_t stream) {
   args.segment = plan.segment;
   args.slots = plan.slots;
   args.items = plan.slots * args.heads * args.slices;
-  const dim3 grid(static_cast<unsigned>(grid_of(args.items)));
+  const dim3 grid = grid_of_items(args.items);
   if (plan.segmented) {
     decay_chunks_kernel<T, WIDTH, kSlice, TERMS, true, WHOLE>
         <<<grid, kDecayThreads<true>, 0, stream>>>(args);
     const int64_t size = static_cast<int64_t>(args.pass[0].key_width) * args.pass[0].value_width;
-    const dim3 join(static_cast<unsigned>((size + kPieceElements - 1) / kPieceElements * args.heads *
-                                          args.passes * args.sequences.count));
+    const dim3 join = grid_of((size + kPieceElements - 1) / kPieceElements * args.heads * args.passes *
+                              args.sequences.count);
     decay_join_kernel<T><<<join, kThreads, 0, stream>>>(args, size);
   } else {
     args.segment_states = nullptr;
@@ -668,7 +674,7 @@ void decay_backward(const DecayCall& call) {
   decay_walk_any<T, kTrainTerms<T>>(args, plan, whole_rows<T>(call), call.stream);
   const int64_t rows = static_cast<int64_t>(p.N) * p.Hkv;
   const auto blocks = [&](int width) {
-    return dim3(static_cast<unsigned>((rows * width + kThreads - 1) / kThreads));
+    return grid_of((rows * width + kThreads - 1) / kThreads);
   };
   if (key_partial != nullptr)
     sum_shared_kernel<T><<<blocks(p.D), kThreads, 0, call.stream>>>(
@@ -684,14 +690,14 @@ void decay_update(const DecayCall& call) {
   if (p.cu_seqlens == nullptr && p.T == 1) {
     DecayTokenArgs<T> args{view_of<T>(*call.query), view_of<T>(*call.key), view_of<T>(*call.value),
                            call.log_decay, call.state_in, call.state_out,
-                           static_cast<T*>(call.out), p.H, p.H / p.Hkv, p.D, p.Dv, 0, p.scale};
+                           static_cast<T*>(call.out), p.B, p.H, p.H / p.Hkv, p.D, p.Dv, 0, p.scale};
     const bool quads = p.Dv % 4 == 0 && reinterpret_cast<uintptr_t>(call.state_in) % 16 == 0 &&
                        reinterpret_cast<uintptr_t>(call.state_out) % 16 == 0;
     // whole rows of a state per block, or narrower slices until there are blocks for the chip
     args.slice = padded_width(p.Dv);
     while (args.slice > 16 && static_cast<int64_t>(p.B) * p.H * (p.Dv / args.slice + 1) < 512)
       args.slice /= 2;
-    const dim3 grid(static_cast<unsigned>((p.Dv + args.slice - 1) / args.slice) * p.H * p.B);
+    const dim3 grid = grid_of(static_cast<int64_t>((p.Dv + args.slice - 1) / args.slice) * p.H * p.B);
     if (quads)
       decay_token_kernel<T, 4><<<grid, kThreads, 0, call.stream>>>(args);
     else

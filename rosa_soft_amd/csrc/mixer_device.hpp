@@ -563,14 +563,22 @@ __device__ __forceinline__ int64_t first_slot(const Sequences& q, const Run& run
                               : run.begin / rows + run.sequence;
 }
 
+// A launch has less than 2^32 threads in a dimension, and drops the others without an error: grids of
+// more blocks than a row holds go on in further rows (the decay's backward has 2^32 threads at 1.4
+// million sequences times heads of 128 columns).  Blocks behind the last item have nothing to do.
+constexpr int kGridRow = 1 << 22;
+inline dim3 grid_of(int64_t blocks) {
+  return blocks <= kGridRow ? dim3(static_cast<unsigned>(blocks))
+                            : dim3(kGridRow, static_cast<unsigned>((blocks + kGridRow - 1) / kGridRow));
+}
+__device__ __forceinline__ uint32_t block_number() { return blockIdx.y * kGridRow + blockIdx.x; }
+
 // Blocks are handed to the XCDs in turn; neighbouring work items, which share keys, values or
 // states, go to the same one: block b works on item (b mod 8) ceil(items / 8) + b / 8.
-__host__ __device__ __forceinline__ int64_t grid_of(int64_t items) {
-  return (items + kGroups - 1) / kGroups * kGroups;
-}
+inline dim3 grid_of_items(int64_t items) { return grid_of((items + kGroups - 1) / kGroups * kGroups); }
 __device__ __forceinline__ int64_t item_of_block(int64_t items) {
-  const int64_t block = blockIdx.x;
-  return block % kGroups * ((items + kGroups - 1) / kGroups) + block / kGroups;
+  const uint32_t block = block_number(), share = static_cast<uint32_t>((items + kGroups - 1) / kGroups);
+  return block / kGroups < share ? static_cast<int64_t>(block % kGroups) * share + block / kGroups : items;
 }
 
 // Rows [first, last) of a head of a contiguous [tokens, heads, width] tensor become NaN: what a

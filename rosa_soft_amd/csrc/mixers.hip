@@ -101,7 +101,9 @@ WindowPlan window_plan(const rosa_mixer_problem& p, int window, int sinks) {
   const int64_t share = p.H / p.Hkv, near = static_cast<int64_t>(plan.key_block) + window - 1;
   int64_t far = near + 8 / (share * (pairs ? 1 : 2)) * 64;
   plan.sink_far = 0x7fffffff;
-  if (sinks > 0 && longest > far) {
+  // (the join has up to 64 blocks for a sequence's head of keys, counted in 32 bits)
+  const int64_t sequences = p.cu_seqlens == nullptr ? p.B : p.S;
+  if (sinks > 0 && longest > far && sequences * p.Hkv <= (int64_t{1} << 25)) {
     // A packed sequence with pieces begins more than `far` tokens behind the one before it, so that
     // tokens alone bound their number (see sink_place).  Their sums take at most kMostStateBytes or
     // as many bytes as the queries and output gradients in 16 bits: with many sinks and a short
@@ -166,13 +168,13 @@ int check(const rosa_mixer_problem* p, bool update) {
   if (p->D < 1 || p->D > kMostWidth || p->Dv < 1 || p->Dv > kMostWidth)
     return rosa_fail(1, "head widths must be in [1, 128]");
   if (!(p->scale > 0.0f) || !std::isfinite(p->scale)) return rosa_fail(1, "scale must be finite and > 0");
-  // grids are one-dimensional; the finest division is 64 tokens (or a sequence) of a head, 16
-  // value columns of a state or a sixteenth of a group of heads
+  // Blocks are counted in 32 bits.  The finest division is 64 tokens (or a sequence) of a head, with
+  // two slices in each of three passes; of an update 16 value columns of a state.  (Joins of segments
+  // and of sinks are bounded by the memory of what they join, and by window_plan.)
   const int64_t sequences = p->cu_seqlens == nullptr ? p->B : p->S;
   const int64_t most = int64_t{0x7fffffff} - 8;
   if ((static_cast<int64_t>(p->N) / 64 + sequences) * p->H * 6 > most ||
-      (update && sequences * p->H * 8 > most) ||
-      sequences * p->H * 3 * ((static_cast<int64_t>(p->D) * p->Dv + 255) / 256) > most)
+      (update && sequences * p->H * 8 > most))
     return rosa_fail(1, "too many blocks: tokens and sequences times heads must be fewer");
   return 0;
 }

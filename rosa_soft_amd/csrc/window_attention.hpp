@@ -767,7 +767,7 @@ window_grad_key_kernel(WindowArgs<T> a) {
 template <typename T>
 __global__ __launch_bounds__(kThreads) void window_join_keys_kernel(const float* parts, T* out, int count,
                                                                     int64_t elements) {
-  const int64_t e = static_cast<int64_t>(blockIdx.x) * kThreads + threadIdx.x;
+  const int64_t e = static_cast<int64_t>(block_number()) * kThreads + threadIdx.x;
   if (e >= elements) return;
   float sum = 0.0f;
   for (int part = 0; part < count; ++part) sum += parts[part * elements + e];
@@ -914,11 +914,13 @@ template <typename T>
 __global__ __launch_bounds__(kThreads) void window_join_sinks_kernel(WindowArgs<T> a) {
   const int tid = threadIdx.x, size = a.sinks * (a.key_width + a.value_width);
   const int blocks = (size + kThreads - 1) / kThreads;
-  const int sequence = static_cast<int>(blockIdx.x / blocks / a.kv_heads);
-  const int kv_head = static_cast<int>(blockIdx.x / blocks % a.kv_heads);
+  const uint32_t block = block_number();
+  const int sequence = static_cast<int>(block / blocks / a.kv_heads);
+  const int kv_head = static_cast<int>(block / blocks % a.kv_heads);
+  if (sequence >= a.sequences.count) return;
   const Run run = run_of_sequence(a.sequences, sequence);
   if (run.length <= a.sink_far) return;  // (of length -1: no offsets to rely on)
-  const int e = static_cast<int>(blockIdx.x % blocks) * kThreads + tid;
+  const int e = static_cast<int>(block % blocks) * kThreads + tid;
   if (e >= size) return;
   const int first = static_cast<int>(walk_end(0, a.key_block, a.window)) / a.sink_rows;
   const int pieces = tiles_of(run.length, a.sink_rows);
@@ -943,8 +945,10 @@ template <typename T, bool WHOLE>
 __global__ __launch_bounds__(kThreads) void window_append_kernel(WindowArgs<T> a, T* key_cache,
                                                                  T* value_cache) {
   const int tid = threadIdx.x;
-  const int64_t slot = blockIdx.x / a.kv_heads;
-  const int kv_head = static_cast<int>(blockIdx.x % a.kv_heads);
+  const uint32_t block = block_number();
+  const int64_t slot = block / a.kv_heads;
+  const int kv_head = static_cast<int>(block % a.kv_heads);
+  if (slot >= slots_of(a.sequences, 64)) return;
   Run run;
   if (find_run(a.sequences, slot, 64, tid, &run) != Found::kRun) return;
   const int past = tokens_before<true>(a, run);
@@ -1003,10 +1007,12 @@ window_token_kernel(TokenArgs<T> args) {
   const int tid = threadIdx.x, lane = tid & 63, group = lane >> 4, column = lane & 15;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   Stored<T>* values = reinterpret_cast<Stored<T>*>(shared) + wave * kTileElements<T, kTile, WIDTH>;
-  const int split = blockIdx.x % args.splits;
-  const int head_block = blockIdx.x / args.splits % args.head_blocks;
-  const int kv_head = blockIdx.x / args.splits / args.head_blocks % a.kv_heads;
-  const int slot = blockIdx.x / args.splits / args.head_blocks / a.kv_heads;
+  const uint32_t block = block_number();
+  const int split = block % args.splits;
+  const int head_block = block / args.splits % args.head_blocks;
+  const int kv_head = block / args.splits / args.head_blocks % a.kv_heads;
+  const int slot = block / args.splits / args.head_blocks / a.kv_heads;
+  if (slot >= a.sequences.count) return;
   const Run run{slot, 1, 0, slot, 0, slot};
   const int past = tokens_before<true>(a, run);
   const History<T, true> key_rows = history_of<true>(a, a.key, a.key_cache, a.key_width, run, kv_head, past);
@@ -1253,7 +1259,7 @@ void window_forward_launch(WindowArgs<T>& args, hipStream_t stream) {
   args.slots = slots_of(args.sequences, 64 * QUERIES);
   args.items = args.slots * args.heads;
   window_forward_kernel<T, WIDTH, QUERIES, CACHED, WHOLE>
-      <<<dim3(static_cast<unsigned>(grid_of(args.items))), kThreads, 0, stream>>>(args);
+      <<<grid_of_items(args.items), kThreads, 0, stream>>>(args);
 }
 
 template <typename T, int WIDTH, bool CACHED, bool WHOLE>
@@ -1289,7 +1295,7 @@ void window_grad_query_launch(WindowArgs<T>& args, hipStream_t stream) {
   args.slots = slots_of(args.sequences, 64 * QUERIES);
   args.items = args.slots * args.heads;
   window_grad_query_kernel<T, WIDTH, QUERIES, WHOLE, DELTA>
-      <<<dim3(static_cast<unsigned>(grid_of(args.items))), kThreads, 0, stream>>>(args);
+      <<<grid_of_items(args.items), kThreads, 0, stream>>>(args);
 }
 
 template <typename T, int WIDTH, int KEYS, bool WHOLE>
@@ -1297,22 +1303,23 @@ void window_grad_key_launch(WindowArgs<T>& args, hipStream_t stream) {
   if (args.sink_slots > 0) {
     args.items = args.sink_slots * args.heads * ((args.sinks + 15) / 16);
     window_grad_sinks_kernel<T, WIDTH, WHOLE>
-        <<<dim3(static_cast<unsigned>(grid_of(args.items))), kThreads, 0, stream>>>(args);
+        <<<grid_of_items(args.items), kThreads, 0, stream>>>(args);
     const int size = args.sinks * (args.key_width + args.value_width);
     window_join_sinks_kernel<T>
-        <<<dim3(static_cast<unsigned>((size + kThreads - 1) / kThreads * args.kv_heads * args.sequences.count)),
+        <<<grid_of(static_cast<int64_t>((size + kThreads - 1) / kThreads) * args.kv_heads *
+                   args.sequences.count),
            kThreads, 0, stream>>>(args);
   }
   args.slots = slots_of(args.sequences, args.key_block);
   args.items = args.slots * args.kv_heads * args.key_parts;
   window_grad_key_kernel<T, WIDTH, KEYS, WHOLE>
-      <<<dim3(static_cast<unsigned>(grid_of(args.items))), kThreads, 0, stream>>>(args);
+      <<<grid_of_items(args.items), kThreads, 0, stream>>>(args);
   if (args.key_parts == 1) return;
   const auto join = [&](const float* parts, T* out, int width) {
     if (out == nullptr) return;
     const int64_t elements = static_cast<int64_t>(args.sequences.tokens) * args.kv_heads * width;
-    window_join_keys_kernel<T><<<dim3(static_cast<unsigned>((elements + kThreads - 1) / kThreads)), kThreads,
-                                 0, stream>>>(parts, out, args.key_parts, elements);
+    window_join_keys_kernel<T><<<grid_of((elements + kThreads - 1) / kThreads), kThreads, 0, stream>>>(
+        parts, out, args.key_parts, elements);
   };
   join(args.key_sums, args.grad_key, args.key_width);
   join(args.value_sums, args.grad_value, args.value_width);
@@ -1389,9 +1396,9 @@ void window_update_launch(WindowArgs<T>& args, const WindowCall& call) {
     const TokenPlan plan = token_plan(p, call.capacity);
     TokenArgs<T> token{args, key_cache, value_cache, plan.splits, plan.head_blocks,
                        reinterpret_cast<float*>(call.workspace)};
-    const unsigned blocks = static_cast<unsigned>(p.B) * p.Hkv * plan.head_blocks * plan.splits;
-    window_token_kernel<T, WIDTH, WHOLE><<<dim3(blocks), kThreads, 0, call.stream>>>(token);
-    if (plan.splits > 1)
+    const int64_t blocks = static_cast<int64_t>(p.B) * p.Hkv * plan.head_blocks * plan.splits;
+    window_token_kernel<T, WIDTH, WHOLE><<<grid_of(blocks), kThreads, 0, call.stream>>>(token);
+    if (plan.splits > 1)  // (of few slots)
       window_token_join_kernel<T><<<dim3(static_cast<unsigned>(p.B) * p.H), kThreads, 0, call.stream>>>(
           token.partial, args.out, plan.splits, p.Dv);
     return;
@@ -1399,7 +1406,7 @@ void window_update_launch(WindowArgs<T>& args, const WindowCall& call) {
   window_forward_rows<T, WIDTH, true, WHOLE>(args, call.stream);
   const int64_t blocks = slots_of(args.sequences, 64) * p.Hkv;
   window_append_kernel<T, WHOLE>
-      <<<dim3(static_cast<unsigned>(blocks)), kThreads, 0, call.stream>>>(args, key_cache, value_cache);
+      <<<grid_of(blocks), kThreads, 0, call.stream>>>(args, key_cache, value_cache);
 }
 
 template <typename T, bool WHOLE>

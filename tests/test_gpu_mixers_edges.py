@@ -275,3 +275,49 @@ def test_packed_sequences_have_the_gradients_that_they_have_alone(lengths, dtype
         for g, w, bound in zip(got[2:], want[2:], bounds[1:]):
             step = 2 * HALF_STEP[dtype] * w[0].double().abs() + (SMALLEST if dtype == torch.float16 else 0.0)
             close(g[s], w[0].double(), step + float32_slack(lengths[s], 80) * bound, (s, lengths[s]))
+
+
+# ---------------------------------------------------------------------------
+# more threads than one dimension of a launch has
+# ---------------------------------------------------------------------------
+
+def test_more_blocks_than_a_launch_dimension_holds():
+    """Sequences of one token, whose answers are one line each: o = scale (q . k) v for the decay,
+    o = v for the window, and dv = scale (q . k) dO, or dO.  2^32 threads are 4.2 million heads of
+    128 columns in the decay's forward, 1.4 million in its backward, 16.8 million in the window's."""
+    count, H, D = 66000, 64, 128
+    ones = dict(dtype=torch.bfloat16, device=DEVICE)
+    mark = (torch.arange(count, device=DEVICE) % 5 - 2).to(torch.bfloat16).view(count, 1, 1, 1)
+    q = mark.expand(count, 1, H, D).contiguous()
+    k, v = torch.ones(count, 1, 1, D, **ones), torch.full((count, 1, 1, D), 0.5, **ones)
+    log_decay = rates(H)
+    output = mixers.decay_attention(q, k, v, log_decay, scale=2.0**-7)
+    assert torch.equal(output, (mark * 0.5).expand_as(output))
+    del output
+    few = q[:24000].detach().requires_grad_(), k[:24000].clone().requires_grad_(), v[:24000].clone().requires_grad_()
+    output = mixers.decay_attention(*few, log_decay, scale=2.0**-7)
+    dq, dk, dv = torch.autograd.grad(output, few, torch.ones((), **ones).expand_as(output))
+    # sums of 64 heads and, in the products, of 128 columns: exact in float32 and in bfloat16
+    assert torch.equal(dq, torch.full_like(dq, 0.5))
+    assert torch.equal(dk, (32 * mark[:24000]).expand_as(dk))
+    assert torch.equal(dv, (64 * mark[:24000]).expand_as(dv))
+    del q, k, v, few, output, dq, dk, dv
+
+    count, H, D = 270000, 64, 4
+    mark = (torch.arange(count * H, device=DEVICE) % 251).to(torch.bfloat16).view(count, 1, H, 1)
+    v = mark.expand(count, 1, H, D).contiguous().requires_grad_()
+    q = torch.ones(count, 1, H, D, **ones)
+    for output in (mixers.window_attention(q, q, v, window=3, sinks=1),
+                   mixers.window_attention_varlen(q[:, 0], q[:, 0], v[:, 0], torch.arange(
+                       count + 1, dtype=torch.int32, device=DEVICE), window=3)):
+        assert torch.equal(output.view_as(v), v)
+        dv, = torch.autograd.grad(output, (v,), output.detach())
+        assert torch.equal(dv, v)
+    v = v.detach()
+    caches = [torch.zeros(count, H, 3, D, **ones) for _ in range(2)]
+    lengths = torch.zeros(count, dtype=torch.int32, device=DEVICE)
+    assert torch.equal(mixers.window_attention_update(q, q, v, *caches, lengths, window=3), v)
+    assert torch.equal(caches[1][:, :, 0], v[:, 0])
+    log_decay, state = rates(H), torch.zeros(count, H, D, D, device=DEVICE)
+    output = mixers.decay_attention_update(q, q, v, log_decay, state, scale=0.25)
+    assert torch.equal(output, v) and torch.equal(state[:, :, 1], v[:, 0].float())

@@ -186,9 +186,16 @@ def decay_attention_update(query: Tensor, key: Tensor, value: Tensor, log_decay:
 # attention with a sliding window and sinks
 # ---------------------------------------------------------------------------
 
+def _masks(window, sinks):
+    # (integers that the operators do not take at all are cut to ones that they refuse, or to an
+    # endless window)
+    if type(window) is int and type(sinks) is int and 0 <= window <= _INT64_MAX >= sinks >= 0:
+        return window, sinks
+    return _integer("window", window), _integer("sinks", sinks)
+
+
 def _window_attention(query, key, value, cu_seqlens, window, sinks, scale) -> Tensor:
-    if type(window) is not int or type(sinks) is not int or window > _INT64_MAX:
-        window, sinks = _integer("window", window), _integer("sinks", sinks)
+    window, sinks = _masks(window, sinks)
     return _window(query, key, value, cu_seqlens, window, sinks, _number("scale", scale))[0]
 
 
@@ -231,7 +238,6 @@ def window_attention_update(query: Tensor, key: Tensor, value: Tensor, key_cache
     ``lengths += T``.  Returns the outputs of the new tokens.
     """
 
-    if type(window) is not int or type(sinks) is not int or window > _INT64_MAX:
-        window, sinks = _integer("window", window), _integer("sinks", sinks)
+    window, sinks = _masks(window, sinks)
     return _window_update(query, key, value, key_cache, value_cache, lengths, cu_seqlens, window,
                           sinks, _number("scale", scale))

@@ -119,6 +119,18 @@ def test_refusals(names, changes, error, message):
             calls(arguments(**changes()))[name]()
 
 
+@pytest.mark.parametrize("masks,message", [
+    (dict(window=-2**70), "window must be >= 1"), (dict(sinks=2**70), "sinks must be in"),
+    (dict(sinks=-2**70), "sinks must be in"), (dict(window=2**63, sinks=2**63), "sinks must be in"),
+])
+def test_masks_of_more_than_64_bits(masks, message):
+    for name in EVERY[2:]:
+        with pytest.raises(ValueError, match=message):
+            calls(arguments(**masks))[name]()
+    with pytest.raises(ValueError, match="require CUDA tensors"):  # an endless window
+        calls(arguments(window=2**70))["window"]()
+
+
 @pytest.mark.parametrize("tokens,refused", [(2**31 - 1025, False), (2**31 - 1024, True), (2**31 - 1, True)])
 def test_sequences_end_where_counts_past_their_last_tile_still_fit(tokens, refused):
     """Kernels count up to a tile of tokens past the last one, in 32 bits."""

@@ -21,10 +21,16 @@ slot (or a packed chunk with ``cu_seqlens``, in which slots may bring none) on t
 states or caches, which are advanced in place.  They have no backward.
 
 Invalid device ``cu_seqlens`` cannot be seen without a synchronisation: they make every output and
-gradient NaN and leave states and caches as they were.  A row of values that is not finite makes
-the outputs NaN of every token that sees it, and may do so for up to 63 tokens before it; a row of
-output gradients does the same to the gradients of what it sees.  States and caches share no
-memory with the inputs, and the updates count a version of them.
+gradient NaN and leave states and caches as they were.  States and caches share no memory with the
+inputs, and the updates count a version of them.
+
+A row that is not finite makes NaN of every result that depends on it, and may do so to others near
+those, because masked weights of a tile are zeros that multiply its rows.  With ``decay_attention``
+these are results of up to 63 tokens before the row (values in outputs, keys in the gradients of
+queries) or behind it (queries and output gradients in those of keys and values).  With
+``window_attention`` they are up to 127 tokens away on either side, among outputs for values, among
+gradients for all inputs, and the gradients of a sequence's first 64 keys and values where there are
+sinks.  What is farther away, and other sequences, keep their results.
 """
 
 from __future__ import annotations

@@ -321,3 +321,69 @@ def test_more_blocks_than_a_launch_dimension_holds():
     log_decay, state = rates(H), torch.zeros(count, H, D, D, device=DEVICE)
     output = mixers.decay_attention_update(q, q, v, log_decay, state, scale=0.25)
     assert torch.equal(output, v) and torch.equal(state[:, :, 1], v[:, 0].float())
+
+
+# ---------------------------------------------------------------------------
+# rows that are not finite
+# ---------------------------------------------------------------------------
+
+def results_with(run, tensors, grad, spoiled=None, row=0, value=float("nan")):
+    """Output, dq, dk, dv with one row of one input replaced."""
+    tensors = [t.detach().clone() for t in (*tensors, grad)]
+    if spoiled is not None:
+        tensors["q k v go".split().index(spoiled)][row] = value
+    leaves = [t.requires_grad_() for t in tensors[:3]]
+    output = run(*leaves)
+    gradients = torch.autograd.grad(output, leaves, tensors[3])
+    return dict(zip(("output", "dq", "dk", "dv"), (output.detach(), *gradients)))
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("value", [float("nan"), float("inf")])
+def test_rows_that_are_not_finite_in_the_decay(value, dtype):
+    lengths, row = [300, 900, 200], 300 + 421
+    tensors = [randn(390 + i, sum(lengths), 4 if i == 0 else 2, 40, dtype=dtype) for i in range(3)]
+    grad, log_decay, cu = randn(393, sum(lengths), 4, 40, dtype=dtype), rates(4), offsets_of(lengths)
+    run = lambda *x: mixers.decay_attention_varlen(*x, cu, log_decay)
+    clean = results_with(run, tensors, grad)
+    own = (row, row + 1)
+    later, around_later = (row, 1200), (row - 63, 1200)
+    earlier, around_earlier = (300, row + 1), (300, row + 64)
+    reach = {"q": dict(output=own, dk=around_earlier, dv=earlier),
+             "k": dict(output=later, dq=around_later, dv=own),
+             "v": dict(output=around_later, dq=later, dk=own),
+             "go": dict(dq=own, dk=earlier, dv=around_earlier)}
+    for spoiled, reached in reach.items():
+        got = results_with(run, tensors, grad, spoiled, row, value)
+        for name, tensor in got.items():
+            begin, end = reached.get(name, (row, row))
+            for part in (slice(0, begin), slice(end, None)):
+                assert torch.equal(tensor[part], clean[name][part]), (spoiled, name)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("window,sinks,Hkv", [(40, 0, 4), (40, 5, 2), (300, 33, 1)])
+@pytest.mark.parametrize("value", [float("nan"), float("inf")])
+def test_rows_that_are_not_finite_in_the_window(value, window, sinks, Hkv, dtype):
+    lengths, row = [300, 2500, 200], 300 + 1203
+    tensors = [randn(395 + i, sum(lengths), 4 if i == 0 else Hkv, 40, dtype=dtype) for i in range(3)]
+    grad, cu = randn(398, sum(lengths), 4, 40, dtype=dtype), offsets_of(lengths)
+    run = lambda *x: mixers.window_attention_varlen(*x, cu, window=window, sinks=sinks)
+    clean = results_with(run, tensors, grad)
+    seen_by = (row, row + window)                        # the tokens that see the row
+    sees = (row - window + 1, row + 1)                   # what its token sees, but for the sinks
+    wide = lambda span: (span[0] - 127, span[1] + 127)
+    # whoever has a NaN output has NaN slopes, and hands them to what it sees
+    back = lambda span: (span[0] - window + 1 - 127, span[1] + 127)
+    own = (row, row + 1)
+    reach = {"q": dict(output=own, dq=own, dk=wide(sees), dv=wide(sees)),
+             "k": dict(output=seen_by, dq=wide(seen_by), dk=back(seen_by), dv=back(seen_by)),
+             "v": dict(output=wide(seen_by), dq=wide(seen_by), dk=back(wide(seen_by))),
+             "go": dict(dq=own, dk=wide(sees), dv=wide(sees))}
+    for spoiled, reached in reach.items():
+        got = results_with(run, tensors, grad, spoiled, row, value)
+        for name, tensor in got.items():
+            begin, end = reached.get(name, (row, row))
+            same = torch.equal(tensor[end:], clean[name][end:]) and torch.equal(tensor[:300], clean[name][:300])
+            first = 364 if sinks and name in ("dk", "dv") else 300
+            assert same and torch.equal(tensor[first:begin], clean[name][first:begin]), (spoiled, name)

@@ -29,9 +29,10 @@ int64_t tile_slots(const rosa_mixer_problem& p, int64_t rows) {
 // 128): two blocks on one take 1.65 times as long, a chunk that is only summed takes half as long,
 // a block's beginning and end take one and a half chunks, and the states' traffic and the two more
 // launches take what they take.  At 2 x 4096 tokens and 32 heads of 128, bfloat16, forward:
-// 1 segment 160 us, 2 145, 4 115, 8 126; backward, with three times the blocks: 1 segment 219 us,
-// 2 300, 4 290.  12 heads of 48 and 80, float16, 6728 tokens, forward: 1 segment 215 us, 7 66,
-// 18 46, 53 59.  Segments have at least two chunks.
+// 1 segment 128 us, 2 126, 4 113, 8 129; backward, with three times the blocks: 1 segment 205 us,
+// 2 266, 4 293.  12 heads of 48 and 80, float16, 6728 tokens, forward: 1 segment 179 us, 8 57,
+// 18 51, 53 81.  Four prompts of 2048 tokens, 32 heads of 128 with their states: 1 segment 89 us,
+// 2 127, 4 136.  Segments have at least two chunks.
 DecayPlan decay_plan(const rosa_mixer_problem& p, int passes) {
   DecayPlan plan{};
   // The backward passes have both widths in both places.  Forward, values are sliced anyway, and

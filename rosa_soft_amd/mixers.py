@@ -18,7 +18,8 @@ differentiable and in reverse mode alone (dual tensors are refused), and like th
 
 The ``_update`` forms serve slots, like ``RosaRuntime.update``: a chunk of one or more tokens per
 slot (or a packed chunk with ``cu_seqlens``, in which slots may bring none) on top of the slots'
-states or caches, which are advanced in place.  They have no backward.
+states or caches, which are advanced in place.  They have no backward.  One token for every slot is
+fastest dense: packed it runs as a chunk, whose blocks walk a slot's window alone.
 
 Invalid device ``cu_seqlens`` cannot be seen without a synchronisation: they make every output and
 gradient NaN and leave states and caches as they were.  States and caches share no memory with the

@@ -391,21 +391,21 @@ def _plain_selected(state):
 # ---------------------------------------------------------------------------
 
 def _own(state):
-    from rosa_soft_amd import mixers
+    from rosa_soft_amd import paged
 
     tables, lengths, offsets = state["tables"], state["lengths"], state["offsets"]
     if state["kind"] == "tables":
-        mixers.page_tables_release(tables, state["after"], lengths, state["pool"], page=state["page"])
-        rows = mixers.page_tables_update(tables, lengths, state["pool"], offsets,
-                                         tokens=state["tokens"], page=state["page"])
+        paged.page_tables_release(tables, state["after"], lengths, state["pool"], page=state["page"])
+        rows = paged.page_tables_update(tables, lengths, state["pool"], offsets,
+                                        tokens=state["tokens"], page=state["page"])
         return [rows, tables, state["pool"]]
     if state["kind"] == "paged":
-        output = mixers.paged_attention_update(*state["inputs"], *state["pages"], tables,
-                                               state["rows"], lengths, offsets)
+        output = paged.paged_attention_update(*state["inputs"], *state["pages"], tables,
+                                              state["rows"], lengths, offsets)
         return [output, *state["pages"]]
-    output = mixers.selected_attention_update(*state["inputs"], *state["pages"], state["bounds"],
-                                              tables, state["rows"], lengths, offsets,
-                                              count=state["count"])
+    output = paged.selected_attention_update(*state["inputs"], *state["pages"], state["bounds"],
+                                             tables, state["rows"], lengths, offsets,
+                                             count=state["count"])
     return [output, *state["pages"], state["bounds"]]
 
 

@@ -449,6 +449,74 @@ int rosa_hip_window_update(const rosa_mixer_problem* problem, int window, int si
                            size_t workspace_bytes, void* stream);
 
 /*
+ * The paged cache: keys and values of any number of slots on pages of one pool, so that a slot takes
+ * the memory of the tokens that it holds.
+ *
+ * Position p of slot s lies on row p mod page of the page tables[s][p / page] (int32 [slots, columns],
+ * device); a number outside [0, pages) is no page.  `pool` int32 [pages + 1] (device) holds the pages
+ * that no slot has: pool[0] is their number f, pool[1 .. f] a stack of them.  `page` is a power of
+ * two in [16, 256].  `lengths` int32 [slots] (device): the tokens that each slot has seen, which
+ * calls read and leave to the caller to advance; negative ones count as 0.  The new tokens are dense
+ * (`T` for each slot, cu_seqlens NULL) or `N` packed ones cut by cu_seqlens (int32 [slots + 1], device).
+ */
+typedef struct rosa_page_tables {
+  int32_t* tables;
+  const int32_t* lengths;
+  int32_t* pool;
+  int slots, columns, pages, page;
+} rosa_page_tables;
+
+/*
+ * Pages for the new tokens of every slot: columns [ceil(length / page), ceil((length + new) / page))
+ * (of those that there are) take pages from the top of the stack, in the order of slots and columns;
+ * where the pool has no more they take -1.  `rows` int64 [N], or [slots, T]: where each new token lies,
+ * tables[s][p / page] * page + p mod page, or -1 where it has no page.  Invalid offsets make every row
+ * -1 and change nothing.  At most 8192 slots.
+ */
+int rosa_hip_page_tables_update(const rosa_page_tables* tables, const int32_t* cu_seqlens, int T,
+                                int N, int64_t* rows, void* stream);
+
+/*
+ * The pages behind the first `keep` tokens (int32 [slots], device) of every slot's `lengths` go back
+ * to the pool, the first of them on top (after an update it is what was there before), and their
+ * entries become -1; numbers that are no page, and pages beyond the pool's size, are dropped.
+ */
+int rosa_hip_page_tables_release(const rosa_page_tables* tables, const int32_t* keep, void* stream);
+
+/*
+ * `rows` as above; `key_pages` [pages, Hkv, page, D] and `value_pages` [.., Dv] contiguous, of the
+ * problem's dtype; `key_bounds` [pages, Hkv, 2, D] (NULL: not kept), the least and the largest element of
+ * each column among the keys on a page.
+ */
+typedef struct rosa_paged_cache {
+  void *key_pages, *value_pages, *key_bounds;
+  const int32_t *tables, *lengths;
+  const int64_t* rows;
+  int columns, pages, page;
+} rosa_paged_cache;
+
+size_t rosa_hip_paged_workspace_bytes(const rosa_mixer_problem* problem,
+                                      const rosa_paged_cache* cache, int count);
+
+/*
+ * The new tokens of every slot (the problem's sequences) are put on their rows, and attend to the
+ * positions up to their own:
+ *   o_t = sum_s p_s v_s, p = softmax of scale q_t . k_s over the positions s <= t.
+ * With `count` > 0 (at most 1024; the bounds are needed) a token t sees, for each head of keys, the
+ * positions on its own page c = t / page and on the `count` pages j < c with the largest
+ *   max over the query heads of the group of  sum_d max(q_d low_jd, q_d high_jd),
+ * summed in 64 bits, ties to the lowest j; a sum that is not a number ranks first.  No key on a page
+ * that is left out has a larger product with a query than this bound.
+ * A token of which a visible position has no page has NaN as output.  Tokens without a row are not
+ * stored; they are seen in this call all the same, but not with `count` > 0.  Invalid offsets make every
+ * output NaN and leave the cache as it was.
+ */
+int rosa_hip_paged_update(const rosa_mixer_problem* problem, const rosa_paged_cache* cache, int count,
+                          const rosa_mixer_tensor* query, const rosa_mixer_tensor* key,
+                          const rosa_mixer_tensor* value, void* output, void* workspace,
+                          size_t workspace_bytes, void* stream);
+
+/*
  * Invalid device cu_seqlens values (not starting at 0, decreasing, or not ending
  * at N) cannot be seen by the host without a synchronisation.  The reference
  * aborts the process with a device assert (rosa_soft_kernels.cu:287-308); here no

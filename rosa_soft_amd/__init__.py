@@ -39,6 +39,12 @@ _OPERATORS = (
     "window_attention",
     "window_attention_vjp",
     "window_attention_update",
+    # rosa_soft_amd.paged
+    "page_tables_update",
+    "page_tables_release",
+    "paged_attention_update",
+    "paged_attention_update_bounds",
+    "selected_attention_update",
 )
 
 

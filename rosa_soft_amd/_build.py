@@ -32,16 +32,21 @@ TILE_FAMILIES = [(1, 8, 1), (1, 8, 2), (1, 16, 1), (1, 16, 2), (1, 32, 1), (1, 3
 # the mixers: checks and work division in one unit, kernels once per element type and operator
 MIXER_SOURCE = os.path.join(HERE, "csrc", "mixers.hip")
 MIXER_INSTANCES_SOURCE = os.path.join(HERE, "csrc", "mixer_instances.hip")
+# the paged cache: the same
+PAGED_SOURCE = os.path.join(HERE, "csrc", "paged.hip")
+PAGED_INSTANCES_SOURCE = os.path.join(HERE, "csrc", "paged_instances.hip")
 MIXER_TYPES = [("float", "float32"), ("_Float16", "float16"), ("__bf16", "bfloat16")]
 HIP_HEADERS = [os.path.join(HERE, "csrc", name)
                for name in ("rosa_device_common.hpp", "rosa_vjp_bands.hpp")]
 MIXER_HEADERS = [os.path.join(HERE, "csrc", name)
                  for name in ("mixer_calls.hpp", "mixer_device.hpp", "decay_attention.hpp",
-                              "window_attention.hpp")]
+                              "attention_device.hpp", "window_attention.hpp", "paged_calls.hpp",
+                              "paged_attention.hpp")]
 OBJECT_DIR = os.path.join(HERE, "build_objects")
 HIP_LIBRARY = os.path.join(HERE, "librosa_soft_hip.so")
 DISPATCH_SOURCES = [os.path.join(HERE, "csrc", name)
-                    for name in ("rosa_dispatch.cpp", "mixer_dispatch.cpp")]
+                    for name in ("rosa_dispatch.cpp", "mixer_dispatch.cpp",
+                                 "paged_dispatch.cpp")]
 # registers, spills, scratch and LDS of every kernel, as the compiler reported them
 RESOURCE_REPORT = os.path.join(HERE, "kernel_resources.json")
 
@@ -133,12 +138,12 @@ def source_digest() -> str:
     """The same of all HIP sources, the mixers' too: what a resource report must name to speak
     for the library in the tree."""
 
-    return _digest(HIP_SOURCE, INSTANCES_SOURCE, MIXER_SOURCE, MIXER_INSTANCES_SOURCE, *HIP_HEADERS,
-                   *MIXER_HEADERS)
+    return _digest(HIP_SOURCE, INSTANCES_SOURCE, MIXER_SOURCE, MIXER_INSTANCES_SOURCE, PAGED_SOURCE,
+                   PAGED_INSTANCES_SOURCE, *HIP_HEADERS, *MIXER_HEADERS)
 
 
 def build_hip_library() -> str:
-    """Compile the translation units (main, eight tile families, mixers) side by side, then link.
+    """Compile the translation units (main, eight tile families, mixers, paged cache) side by side, then link.
 
     One compiler process per translation unit; the families take one to two minutes each,
     which is also most of the build's wall time on eight cores."""
@@ -162,6 +167,13 @@ def build_hip_library() -> str:
                           f"-DROSA_MIXER_TYPE={element}", f"-DROSA_MIXER_NAME={name}",
                           f"-DROSA_MIXER_WINDOW={window}", "-c", MIXER_INSTANCES_SOURCE],
                          os.path.join(OBJECT_DIR, f"mixer_{operator}_{name}.o")))
+
+    jobs.append(([hipcc, *HIPCC_FLAGS, "-Rpass-analysis=kernel-resource-usage", "-c", PAGED_SOURCE],
+                 os.path.join(OBJECT_DIR, "paged.o")))
+    for element, name in MIXER_TYPES:
+        jobs.append(([hipcc, *HIPCC_FLAGS, "-Rpass-analysis=kernel-resource-usage",
+                      f"-DROSA_MIXER_TYPE={element}", f"-DROSA_MIXER_NAME={name}", "-c",
+                      PAGED_INSTANCES_SOURCE], os.path.join(OBJECT_DIR, f"paged_{name}.o")))
 
     def compile_one(job):
         command = [*job[0], "-o", job[1]]

@@ -55,6 +55,10 @@ EXPORTED_SYMBOLS = (
     "rosa_hip_window_forward",
     "rosa_hip_window_backward",
     "rosa_hip_window_update",
+    "rosa_hip_page_tables_update",
+    "rosa_hip_page_tables_release",
+    "rosa_hip_paged_workspace_bytes",
+    "rosa_hip_paged_update",
     "rosa_hip_read_offset_error",
     "rosa_hip_stage_timing",
     "rosa_hip_stage_count",
@@ -139,6 +143,36 @@ class RosaMixerTensor(ctypes.Structure):
         ("batch_stride", ctypes.c_int64),
         ("token_stride", ctypes.c_int64),
         ("head_stride", ctypes.c_int64),
+    ]
+
+
+class RosaPageTables(ctypes.Structure):
+    """``rosa_page_tables`` of ``include/rosa_soft_hip.h``."""
+
+    _fields_ = [
+        ("tables", ctypes.c_void_p),
+        ("lengths", ctypes.c_void_p),
+        ("pool", ctypes.c_void_p),
+        ("slots", ctypes.c_int),
+        ("columns", ctypes.c_int),
+        ("pages", ctypes.c_int),
+        ("page", ctypes.c_int),
+    ]
+
+
+class RosaPagedCache(ctypes.Structure):
+    """``rosa_paged_cache`` of ``include/rosa_soft_hip.h``."""
+
+    _fields_ = [
+        ("key_pages", ctypes.c_void_p),
+        ("value_pages", ctypes.c_void_p),
+        ("key_bounds", ctypes.c_void_p),
+        ("tables", ctypes.c_void_p),
+        ("lengths", ctypes.c_void_p),
+        ("rows", ctypes.c_void_p),
+        ("columns", ctypes.c_int),
+        ("pages", ctypes.c_int),
+        ("page", ctypes.c_int),
     ]
 
 
@@ -257,6 +291,17 @@ def load() -> ctypes.CDLL:
     library.rosa_hip_window_update.restype = ctypes.c_int
     library.rosa_hip_window_update.argtypes = [
         *masked, *[tensor_p] * 3, vp, vp, ctypes.c_int64, vp, vp, *sized,
+    ]
+    tables_p, cache_p = ctypes.POINTER(RosaPageTables), ctypes.POINTER(RosaPagedCache)
+    library.rosa_hip_page_tables_update.restype = ctypes.c_int
+    library.rosa_hip_page_tables_update.argtypes = [tables_p, vp, ctypes.c_int, ctypes.c_int, vp, vp]
+    library.rosa_hip_page_tables_release.restype = ctypes.c_int
+    library.rosa_hip_page_tables_release.argtypes = [tables_p, vp, vp]
+    library.rosa_hip_paged_workspace_bytes.restype = ctypes.c_size_t
+    library.rosa_hip_paged_workspace_bytes.argtypes = [mixer_p, cache_p, ctypes.c_int]
+    library.rosa_hip_paged_update.restype = ctypes.c_int
+    library.rosa_hip_paged_update.argtypes = [
+        mixer_p, cache_p, ctypes.c_int, *[tensor_p] * 3, vp, *sized,
     ]
     library.rosa_hip_read_offset_error.restype = ctypes.c_int
     library.rosa_hip_read_offset_error.argtypes = [vp, vp]

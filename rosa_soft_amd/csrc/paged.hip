@@ -1,0 +1,379 @@
+// C entry points of the paged cache: checks, work division and workspace in host arithmetic, and the
+// kernels that hand pages out and take them back.  The attention is in paged_attention.hpp, one
+// translation unit per element type.
+#include "paged_calls.hpp"
+#include "mixer_device.hpp"
+
+#include <algorithm>
+#include <cmath>
+
+namespace rosa_mixer {
+
+namespace {
+
+constexpr int kPortions = 512;                          // of a call: two blocks for a compute unit
+constexpr int64_t kMostScoreBytes = int64_t{1} << 28;   // of a slab of tokens
+constexpr int kTableThreads = 1024;
+// Tokens whose rows the block that hands out pages writes by itself; more have a launch of their own.
+constexpr int kFewRows = 16384;
+
+}  // namespace
+
+PagedPlan paged_plan(const rosa_mixer_problem& p, const rosa_paged_cache& cache, int count) {
+  PagedPlan plan{};
+  plan.width = padded_width(std::max(p.D, p.Dv));
+  const int share = p.H / p.Hkv;
+  const bool packed = p.cu_seqlens != nullptr;
+  const int64_t sequences = packed ? p.S : p.B;
+  const int64_t capacity = static_cast<int64_t>(cache.columns) * cache.page;
+  const int outs = plan.width + 4;
+  const auto finish = [&](PagedShare* s) {
+    if (s->parts > 0) {
+      s->part_bytes = aligned(static_cast<size_t>(s->parts) * p.Hkv * s->rows * outs * 4);
+      s->task_bytes = 256 + aligned(static_cast<size_t>(s->parts) * 32);
+    }
+  };
+  PagedShare& few = plan.few;
+  const bool two = p.dtype != ROSA_DTYPE_F32;  // two sixteens of rows of a wave fit its registers
+  if (count > 0) {
+    // tokens on their own, which see about as many keys each
+    few.used = true;
+    few.rows = share <= 16 || !two ? 16 : 32;
+    const int64_t tiles = static_cast<int64_t>(p.N) * ((share + few.rows - 1) / few.rows);
+    const int64_t walk = (std::min<int64_t>(count + 1, cache.columns) * cache.page + 31) / 32;
+    const int64_t blocks = tiles * p.Hkv;
+    few.target = static_cast<int>(
+        std::max<int64_t>(1, std::min((kPortions + blocks - 1) / blocks, walk / 8)));
+    few.items = tiles * few.target;
+    few.parts = few.target > 1 ? few.items : 0;
+    finish(&few);
+    plan.list_bytes = aligned(static_cast<size_t>(p.N) * p.Hkv * (count + 1) * 4);
+    plan.seen_bytes = aligned(static_cast<size_t>(p.N) * p.Hkv * 4);
+    const int64_t row = static_cast<int64_t>(p.Hkv) * cache.columns * 8;
+    plan.score_bytes = static_cast<size_t>(
+        row * std::min<int64_t>(p.N, std::max<int64_t>(1, kMostScoreBytes / row)));
+    return plan;
+  }
+  const int64_t rows = packed ? 0 : static_cast<int64_t>(p.T) * share;  // of a slot
+  const int64_t few_rows = packed ? share : rows;
+  few.used = few_rows <= 32;
+  few.rows = few_rows <= 16 || !two ? 16 : 32;
+  plan.most_few = !few.used ? 0 : few_rows <= 16 ? 16 : 32;
+  if (few.used) {
+    few.target = (2 * kPortions + p.Hkv - 1) / p.Hkv;
+    few.least = 8;
+    few.items = sequences * (plan.most_few / few.rows) + few.target;
+    few.parts = (capacity + 31) / 32 > few.least ? 2 * few.target : 0;
+    finish(&few);
+  }
+  PagedShare& many = plan.many;
+  many.used = packed || !few.used;
+  if (many.used) {
+    const bool pairs = p.dtype != ROSA_DTYPE_F32 || plan.width < 128;
+    const auto tiles_of_rows = [&](int64_t tile) {
+      return packed ? static_cast<int64_t>(p.N) * share / tile + sequences
+                    : sequences * ((rows + tile - 1) / tile);
+    };
+    many.rows = pairs && tiles_of_rows(128) * p.Hkv >= kPortions ? 128 : 64;
+    many.target = (kPortions + p.Hkv - 1) / p.Hkv;
+    many.least = 4;
+    many.items = tiles_of_rows(many.rows) + many.target;
+    many.parts = (capacity + 63) / 64 > many.least ? 2 * many.target : 0;
+    finish(&many);
+  }
+  return plan;
+}
+
+// ---------------------------------------------------------------------------
+// tables
+// ---------------------------------------------------------------------------
+
+namespace {
+
+struct TableArgs {
+  int32_t *tables, *pool;
+  const int32_t *lengths, *keep, *offsets;
+  int64_t* rows;
+  int slots, columns, pages, page_shift, T, N;
+  __device__ __forceinline__ int64_t held(int64_t tokens) const {  // columns of that many tokens
+    return min((tokens + (1 << page_shift) - 1) >> page_shift, static_cast<int64_t>(columns));
+  }
+  __device__ __forceinline__ int64_t length(int s) const { return max(lengths[s], 0); }
+  __device__ __forceinline__ int64_t row_at(int s, int64_t position) const {
+    const int64_t column = position >> page_shift;
+    const int id = column < columns ? tables[static_cast<int64_t>(s) * columns + column] : -1;
+    return id >= 0 && id < pages ? (static_cast<int64_t>(id) << page_shift) + (position & ((1 << page_shift) - 1))
+                                 : -1;
+  }
+};
+
+// Inclusive sum over the threads of a block, and its total.
+__device__ __forceinline__ int64_t scan_block(int64_t x, int tid, int64_t* ends, int64_t* total) {
+  const int lane = tid & 63, wave = tid >> 6;
+  for (int apart = 1; apart < 64; apart *= 2) {
+    const int64_t before = __shfl_up(static_cast<long long>(x), apart);
+    if (lane >= apart) x += before;
+  }
+  if (lane == 63) ends[wave] = x;
+  __syncthreads();
+  int64_t all = 0;
+  for (int w = 0; w < kTableThreads / 64; ++w) {
+    if (w < wave) x += ends[w];
+    all += ends[w];
+  }
+  __syncthreads();
+  *total = all;
+  return x;
+}
+
+// The last slot whose first item is `item` or one before it: the one that has it.
+__device__ __forceinline__ int slot_of_item(const int* first, int slots, int item) {
+  int low = 0, high = slots;
+  while (high - low > 1) {
+    const int middle = (low + high) / 2;
+    (first[middle] <= item ? low : high) = middle;
+  }
+  return low;
+}
+
+__device__ __forceinline__ int64_t row_of_token(const TableArgs& a, const int32_t* offsets, int token) {
+  if (offsets == nullptr) {
+    const int s = token / a.T;
+    return a.row_at(s, a.length(s) + token - s * a.T);
+  }
+  const int s = slot_of_item(offsets, a.slots, token);
+  return a.row_at(s, a.length(s) + token - offsets[s]);
+}
+
+// One block, since every page that is handed out depends on those before it: the items of a call (new
+// pages of slots, in order) are numbered by a sum over the slots, and every thread takes some of them.
+// Latency is all of it: 64 slots with 8 tokens each.
+__global__ __launch_bounds__(kTableThreads) void page_tables_update_kernel(TableArgs a, bool all_rows) {
+  extern __shared__ int first[];  // [slots] items, [slots + 1] tokens
+  __shared__ int64_t ends[kTableThreads / 64];
+  const int tid = threadIdx.x;
+  int* offsets = first + a.slots;
+  const int free = max(0, min(a.pool[0], a.pages));
+  int bad = 0;
+  if (a.offsets != nullptr) {
+    for (int s = tid; s < a.slots; s += kTableThreads) {
+      const int begin = a.offsets[s], end = a.offsets[s + 1];
+      bad |= begin > end || (s == 0 && begin != 0) || (s == a.slots - 1 && end != a.N);
+      offsets[s] = begin;
+    }
+    if (__syncthreads_or(bad)) {
+      if (all_rows)
+        for (int64_t n = tid; n < a.N; n += kTableThreads) a.rows[n] = -1;
+      return;
+    }
+  }
+  int64_t items = 0;
+  for (int base = 0; base < a.slots; base += kTableThreads) {
+    const int s = base + tid;
+    int64_t mine = 0, total;
+    if (s < a.slots) {
+      const int fresh = a.offsets == nullptr ? a.T : a.offsets[s + 1] - a.offsets[s];
+      mine = a.held(a.length(s) + fresh) - a.held(a.length(s));
+    }
+    const int64_t upto = items + scan_block(mine, tid, ends, &total);
+    if (s < a.slots) first[s] = static_cast<int>(upto - mine);
+    items += total;
+  }
+  __syncthreads();
+  for (int64_t k = tid; k < items; k += kTableThreads) {
+    const int s = slot_of_item(first, a.slots, static_cast<int>(k));
+    const int64_t column = a.held(a.length(s)) + k - first[s];
+    a.tables[static_cast<int64_t>(s) * a.columns + column] = k < free ? a.pool[free - k] : -1;
+  }
+  if (tid == 0) a.pool[0] = static_cast<int>(max(int64_t{0}, free - items));
+  if (!all_rows) return;
+  __syncthreads();
+  for (int64_t n = tid; n < a.N; n += kTableThreads)
+    a.rows[n] = row_of_token(a, a.offsets == nullptr ? nullptr : offsets, static_cast<int>(n));
+}
+
+// The rows of many tokens, once the tables are made.
+__global__ __launch_bounds__(kThreads) void page_rows_kernel(TableArgs a) {
+  int bad = 0;
+  if (a.offsets != nullptr) {
+    for (int s = threadIdx.x; s < a.slots; s += kThreads) {
+      const int begin = a.offsets[s], end = a.offsets[s + 1];
+      bad |= begin > end || (s == 0 && begin != 0) || (s == a.slots - 1 && end != a.N);
+    }
+    bad = __syncthreads_or(bad);
+  }
+  const int64_t n = static_cast<int64_t>(blockIdx.x) * kThreads + threadIdx.x;
+  if (n < a.N) a.rows[n] = bad ? -1 : row_of_token(a, a.offsets, static_cast<int>(n));
+}
+
+// The same backwards: from the last item to the first, each valid page goes on top of those before it.
+__global__ __launch_bounds__(kTableThreads) void page_tables_release_kernel(TableArgs a) {
+  extern __shared__ int first[];
+  __shared__ int64_t ends[kTableThreads / 64];
+  const int tid = threadIdx.x;
+  const auto kept = [&](int s) { return a.held(min(static_cast<int64_t>(max(a.keep[s], 0)), a.length(s))); };
+  int64_t top = max(0, min(a.pool[0], a.pages)), items = 0;
+  for (int base = 0; base < a.slots; base += kTableThreads) {
+    const int s = base + tid;
+    const int64_t mine = s < a.slots ? a.held(a.length(s)) - kept(s) : 0;
+    int64_t total;
+    const int64_t upto = items + scan_block(mine, tid, ends, &total);
+    if (s < a.slots) first[s] = static_cast<int>(upto - mine);
+    items += total;
+  }
+  __syncthreads();
+  for (int64_t base = items - 1; base >= 0; base -= kTableThreads) {
+    const int64_t k = base - tid;
+    int id = -1;
+    if (k >= 0) {
+      const int s = slot_of_item(first, a.slots, static_cast<int>(k));
+      int32_t* entry = a.tables + static_cast<int64_t>(s) * a.columns + kept(s) + k - first[s];
+      id = *entry;
+      *entry = -1;
+    }
+    const bool valid = id >= 0 && id < a.pages;
+    int64_t total;
+    const int64_t place = top + scan_block(valid ? 1 : 0, tid, ends, &total);
+    if (valid && place <= a.pages) a.pool[place] = id;
+    top += total;
+  }
+  if (tid == 0) a.pool[0] = static_cast<int>(min(top, static_cast<int64_t>(a.pages)));
+}
+
+int check_page(int page) {
+  return page >= 16 && page <= 256 && (page & (page - 1)) == 0
+             ? 0
+             : rosa_fail(1, "page must be a power of two in [16, 256]");
+}
+
+int check_tables(const rosa_page_tables* t) {
+  if (t == nullptr) return rosa_fail(1, "page tables are NULL");
+  if (t->slots < 1 || t->slots > kMostTableSlots) return rosa_fail(1, "page tables must have 1 to 8192 slots");
+  if (t->columns < 1 || t->pages < 1) return rosa_fail(1, "page tables need columns >= 1 and pages >= 1");
+  if (static_cast<int64_t>(t->slots) * t->columns > 0x7fffffff)
+    return rosa_fail(1, "page tables must have fewer than 2^31 entries");
+  if (const int bad = check_page(t->page)) return bad;
+  if (!t->tables || !t->lengths || !t->pool) return rosa_fail(2, "page tables: NULL pointer");
+  return 0;
+}
+
+TableArgs table_args(const rosa_page_tables& t) {
+  TableArgs args{};
+  args.tables = t.tables;
+  args.pool = t.pool;
+  args.lengths = t.lengths;
+  args.slots = t.slots;
+  args.columns = t.columns;
+  args.pages = t.pages;
+  args.page_shift = __builtin_ctz(static_cast<unsigned>(t.page));
+  return args;
+}
+
+int check_call(const rosa_mixer_problem* p, const rosa_paged_cache* c, int count) {
+  if (p == nullptr || c == nullptr) return rosa_fail(1, "paged update: problem or cache is NULL");
+  if (p->dtype < ROSA_DTYPE_F32 || p->dtype > ROSA_DTYPE_BF16) return rosa_fail(1, "unsupported dtype");
+  if (p->cu_seqlens != nullptr) {
+    if (p->S < 1 || p->N < 1) return rosa_fail(1, "packed layout needs S >= 1 and N >= 1");
+  } else {
+    if (p->B < 1 || p->T < 1) return rosa_fail(1, "dense layout needs B >= 1 and T >= 1");
+    if (static_cast<int64_t>(p->B) * p->T != p->N) return rosa_fail(1, "dense layout needs N = B * T");
+  }
+  if ((p->cu_seqlens != nullptr ? p->N : p->T) > kMostTokens)
+    return rosa_fail(1, "a sequence must have at most 2^31 - 1025 tokens");
+  if (p->H < 1 || p->Hkv < 1 || p->H % p->Hkv != 0)
+    return rosa_fail(1, "query heads must be a positive multiple of key and value heads");
+  if (p->D < 1 || p->D > kMostWidth || p->Dv < 1 || p->Dv > kMostWidth)
+    return rosa_fail(1, "head widths must be in [1, 128]");
+  if (!(p->scale > 0.0f) || !std::isfinite(p->scale)) return rosa_fail(1, "scale must be finite and > 0");
+  if (const int bad = check_page(c->page)) return bad;
+  if (c->columns < 1 || c->pages < 1) return rosa_fail(1, "paged update needs columns >= 1 and pages >= 1");
+  if (count < 0 || count > kMostCount) return rosa_fail(1, "count must be in [0, 1024]");
+  // Rows, blocks and portions are counted in 32 bits.
+  const int64_t sequences = p->cu_seqlens == nullptr ? p->B : p->S;
+  const int64_t most = int64_t{0x7fffffff} - 2048;
+  if (static_cast<int64_t>(p->N) * p->H > most || sequences * p->Hkv > most / 64)
+    return rosa_fail(1, "too many blocks: tokens and slots times heads must be fewer");
+  return 0;
+}
+
+int launched(const char* what) {
+  const hipError_t status = hipGetLastError();
+  return status == hipSuccess ? 0 : rosa_fail_hip(status, what);
+}
+
+}  // namespace
+
+}  // namespace rosa_mixer
+
+using namespace rosa_mixer;
+
+extern "C" {
+
+int rosa_hip_page_tables_update(const rosa_page_tables* tables, const int32_t* cu_seqlens, int T,
+                                int N, int64_t* rows, void* stream) {
+  if (const int bad = check_tables(tables)) return bad;
+  if (N < 0 || T < 0 || (cu_seqlens == nullptr && static_cast<int64_t>(tables->slots) * T != N))
+    return rosa_fail(1, "page_tables_update: needs N >= 0 tokens, slots * T of them if dense");
+  if (N == 0) return 0;
+  if (!rows) return rosa_fail(2, "page_tables_update: NULL pointer");
+  TableArgs args = table_args(*tables);
+  args.offsets = cu_seqlens;
+  args.rows = rows;
+  args.T = T;
+  args.N = N;
+  const bool all_rows = N <= kFewRows;
+  const auto on = static_cast<hipStream_t>(stream);
+  const size_t shared = static_cast<size_t>(tables->slots) * (cu_seqlens ? 8 : 4);
+  page_tables_update_kernel<<<1, kTableThreads, shared, on>>>(args, all_rows);
+  if (!all_rows) page_rows_kernel<<<(N - 1) / kThreads + 1, kThreads, 0, on>>>(args);
+  return launched("page_tables_update launch");
+}
+
+int rosa_hip_page_tables_release(const rosa_page_tables* tables, const int32_t* keep, void* stream) {
+  if (const int bad = check_tables(tables)) return bad;
+  if (!keep) return rosa_fail(2, "page_tables_release: NULL pointer");
+  TableArgs args = table_args(*tables);
+  args.keep = keep;
+  page_tables_release_kernel<<<1, kTableThreads, static_cast<size_t>(tables->slots) * 4,
+                               static_cast<hipStream_t>(stream)>>>(args);
+  return launched("page_tables_release launch");
+}
+
+size_t rosa_hip_paged_workspace_bytes(const rosa_mixer_problem* problem,
+                                      const rosa_paged_cache* cache, int count) {
+  if (check_call(problem, cache, count) != 0) return 0;
+  return std::max<size_t>(paged_plan(*problem, *cache, count).bytes(), 256);
+}
+
+int rosa_hip_paged_update(const rosa_mixer_problem* problem, const rosa_paged_cache* cache, int count,
+                          const rosa_mixer_tensor* query, const rosa_mixer_tensor* key,
+                          const rosa_mixer_tensor* value, void* output, void* workspace,
+                          size_t workspace_bytes, void* stream) {
+  if (const int bad = check_call(problem, cache, count)) return bad;
+  for (const rosa_mixer_tensor* t : {query, key, value})
+    if (t == nullptr || t->data == nullptr) return rosa_fail(2, "paged_update: NULL tensor");
+  if (!cache->key_pages || !cache->value_pages || !cache->tables || !cache->lengths || !cache->rows || !output)
+    return rosa_fail(2, "paged_update: NULL pointer");
+  if (count > 0 && !cache->key_bounds) return rosa_fail(2, "paged_update: selected pages need key_bounds");
+  const size_t needed = paged_plan(*problem, *cache, count).bytes();
+  if (needed > 0 && !workspace) return rosa_fail(2, "paged_update: NULL pointer");
+  if (workspace_bytes < needed) return rosa_fail(3, "paged_update: workspace too small");
+  if (reinterpret_cast<uintptr_t>(workspace) % 16 != 0)
+    return rosa_fail(1, "mixer workspaces must be 16-byte aligned");
+  PagedCall call{};
+  call.problem = problem;
+  call.cache = cache;
+  call.count = count;
+  call.query = query;
+  call.key = key;
+  call.value = value;
+  call.out = output;
+  call.workspace = static_cast<char*>(workspace);
+  call.stream = static_cast<hipStream_t>(stream);
+  (problem->dtype == ROSA_DTYPE_F32   ? paged_update_float32
+   : problem->dtype == ROSA_DTYPE_F16 ? paged_update_float16
+                                      : paged_update_bfloat16)(call);
+  return launched("paged_update launch");
+}
+
+}  // extern "C"

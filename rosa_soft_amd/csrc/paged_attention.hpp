@@ -1,0 +1,1353 @@
+// Attention of new tokens over a paged cache: position p of a slot lies on row p mod P of page
+// table[p / P], with P a power of two from 16 on, so that 16 neighbouring positions from a multiple of
+// 16 on are 16 neighbouring rows.
+//
+//   p = softmax_s(scale q_t . k_s) over s <= t (or those of them on selected pages),  o_t = sum_s p_s v_s
+//
+// The query heads of a group share keys and values: the rows of a slot are its (token, member of the
+// group) pairs, member fastest, whatever the number of either.  Slots of up to 16 or 32 rows (single
+// tokens, drafts) are bound by the reads of the cache and have paged_token_kernel, in which the waves
+// of a block share out keys; the others are bound by matrix products and have paged_chunk_kernel, in
+// which they share out rows and keys go through LDS.
+//
+// Neither the host nor a launch knows the slots' lengths.  Every block reads all of them and works out
+// by itself how the call is cut into portions of about the same number of keys, and which is its own
+// (portion_of); tiles that are cut leave partial sums to paged_join_kernel.
+#pragma once
+
+#include "attention_device.hpp"
+#include "paged_calls.hpp"
+
+#include <algorithm>
+
+namespace rosa_mixer {
+
+// A tile of rows whose keys are shared out to several portions.
+struct PagedTask {
+  int64_t first;              // token of the slot's first row
+  int row, rows, part, splits;
+};
+
+struct PagedDivision {
+  int target, least, most_few;
+  int64_t parts;              // of a head of keys: what two of them are apart in `partial`
+  float* partial;             // [kv head][part][row][width + 4]: outputs, maximum, sum
+  PagedTask* tasks;
+  int* task_count;
+};
+
+template <typename T>
+struct PagedArgs {
+  View<const T> query, key, value;
+  T* out;                     // [tokens][heads][value_width]
+  T *key_pages, *value_pages, *key_bounds;
+  const int32_t *tables, *lengths;
+  const int64_t* rows;
+  Sequences sequences;
+  int64_t pages;
+  int columns, page_shift;
+  int heads, kv_heads, share, key_width, value_width;
+  float scale;
+  bool fused;                 // single tokens, put on their rows by the kernel that attends
+  PagedDivision division;
+  // selected pages
+  double* scores;             // [token of the slab][kv head][column]
+  int32_t *lists, *seen;      // [token][kv head][count + 1], [token][kv head]
+  int count, list_splits;
+  int64_t slab_first, slab_tokens;
+
+  __device__ __forceinline__ int64_t capacity() const { return static_cast<int64_t>(columns) << page_shift; }
+  __device__ __forceinline__ bool is_page(int id) const { return id >= 0 && id < pages; }
+  // row of a page's head in the pools
+  __device__ __forceinline__ int64_t place(int id, int kv_head, int offset) const {
+    return ((static_cast<int64_t>(id) * kv_heads + kv_head) << page_shift) + offset;
+  }
+  // the row that a new token is put on, or -1
+  __device__ __forceinline__ int64_t row_of(int64_t token) const {
+    const int64_t row = rows[token];
+    return row >= 0 && row < pages << page_shift ? row : -1;
+  }
+};
+
+// ---------------------------------------------------------------------------
+// sharing out
+// ---------------------------------------------------------------------------
+
+struct SlotWork {
+  int begin, fresh, past, tiles, walk;  // first new token, new ones, earlier ones; tiles of rows, of keys
+};
+
+// ROWS, KEYS: of a tile.  FEW: slots of up to `most_few` rows, or the others.
+template <int ROWS, int KEYS, bool FEW, typename T>
+__device__ __forceinline__ SlotWork slot_work(const PagedArgs<T>& a, int s, int* bad) {
+  SlotWork w;
+  const Sequences& q = a.sequences;
+  if (q.offsets == nullptr) {
+    w.begin = 0;
+    w.fresh = q.length;
+  } else {
+    const int end = q.offsets[s + 1];
+    w.begin = q.offsets[s];
+    *bad |= w.begin > end || (s == 0 && w.begin != 0) || (s == q.count - 1 && end != q.tokens);
+    w.fresh = w.begin < 0 || end > q.tokens ? 0 : max(0, end - w.begin);
+  }
+  w.past = max(0, min(a.lengths[s], 0x7fffffff - 1024 - w.fresh));
+  const int rows = w.fresh * a.share;
+  w.tiles = w.fresh > 0 && (rows <= a.division.most_few) == FEW ? (rows - 1) / ROWS + 1 : 0;
+  const int64_t end = min(static_cast<int64_t>(w.past) + w.fresh, a.capacity());
+  w.walk = static_cast<int>((end + KEYS - 1) / KEYS);
+  return w;
+}
+
+struct Portion {
+  SlotWork work;
+  int slot, kv_head, tile, split, splits, part, task;
+};
+
+__device__ __forceinline__ int64_t over_wave_sum(int64_t x) {
+  for (int apart = 1; apart < 64; apart *= 2) x += __shfl_xor(static_cast<long long>(x), apart);
+  return x;
+}
+__device__ __forceinline__ int scan_wave(int x, int lane) {  // inclusive
+  for (int apart = 1; apart < 64; apart *= 2) {
+    const int before = __shfl_up(x, apart);
+    if (lane >= apart) x += before;
+  }
+  return x;
+}
+
+// Which head and which of its `total` portions a block works on; -1: none.  FEW: neighbouring blocks
+// have neighbouring heads, which lie side by side on a page.  Otherwise blocks of the same keys, which
+// are neighbours among a head's portions, go to the same XCD.
+template <bool FEW>
+__device__ __forceinline__ int64_t portion_number(int64_t total, int kv_heads, int* kv_head) {
+  const uint32_t block = block_number();
+  if constexpr (FEW) {
+    *kv_head = static_cast<int>(block % kv_heads);
+    const int64_t item = block / kv_heads;
+    return item < total ? item : -1;
+  } else {
+    const int64_t item = item_of_block(total * kv_heads);
+    if (item >= total * kv_heads) return -1;
+    *kv_head = static_cast<int>(item / total);
+    return item % total;
+  }
+}
+
+// Number `at` among the portions of a slot.
+template <bool FEW>
+__device__ __forceinline__ void place_portion(Portion* p, int at, int parts_before, int tasks_before) {
+  const int tiles = p->work.tiles;
+  if constexpr (FEW) {
+    p->split = at % p->splits;
+    p->tile = at / p->splits;
+  } else {  // late tiles, which see most, first
+    p->split = at / tiles;
+    p->tile = tiles - 1 - at % tiles;
+  }
+  p->part = parts_before + p->tile * p->splits + p->split;
+  p->task = tasks_before + p->tile;
+}
+
+// The portion of a block.  All portions of a call together have `all` = sum over its slots of (tiles of
+// rows) (tiles of keys); one has at most all / target of them, or `least`, so that a head of keys has
+// about `target` portions more than tiles of rows, however the slots' lengths differ.  Up to 64 slots
+// every wave looks at all of them by itself, a slot to a lane; beyond, the threads of the block have
+// neighbouring slots each.
+template <int ROWS, int KEYS, bool FEW, typename T>
+__device__ __forceinline__ Found portion_of(const PagedArgs<T>& a, int tid, Portion* p) {
+  const PagedDivision& d = a.division;
+  const int count = a.sequences.count, lane = tid & 63, wave = tid >> 6;
+  const auto portion_length = [&](int64_t all) {
+    return static_cast<int>(max(static_cast<int64_t>(d.least), (all + d.target - 1) / d.target));
+  };
+  const auto splits_of = [](const SlotWork& w, int length) {
+    return w.tiles > 0 ? (w.walk + length - 1) / length : 0;
+  };
+  const auto note_tasks = [&](int tasks) {
+    if (block_number() == 0 && tid == 0 && d.task_count != nullptr) *d.task_count = tasks;
+  };
+  if (count <= 64) {
+    int bad = 0;
+    SlotWork w{};
+    if (lane < count) w = slot_work<ROWS, KEYS, FEW>(a, lane, &bad);
+    if (__any(bad)) {
+      note_tasks(0);
+      return Found::kInvalid;
+    }
+    const int length = portion_length(over_wave_sum(static_cast<int64_t>(w.tiles) * w.walk));
+    const int splits = splits_of(w, length), items = w.tiles * splits;
+    const int upto = scan_wave(items, lane), total = __shfl(upto, 63);
+    const int parts = scan_wave(splits > 1 ? items : 0, lane);
+    const int tasks = scan_wave(splits > 1 ? w.tiles : 0, lane);
+    note_tasks(__shfl(tasks, 63));
+    const int64_t item = portion_number<FEW>(total, a.kv_heads, &p->kv_head);
+    if (item < 0) return Found::kNothing;
+    const int slot = __popcll(__ballot(upto <= item));
+    const auto of_slot = [&](int x) { return __builtin_amdgcn_readlane(x, slot); };
+    p->slot = slot;
+    p->work = {of_slot(w.begin), of_slot(w.fresh), of_slot(w.past), of_slot(w.tiles), of_slot(w.walk)};
+    p->splits = of_slot(splits);
+    const bool cut = p->splits > 1;
+    const int all = of_slot(items);
+    place_portion<FEW>(p, static_cast<int>(item) - (of_slot(upto) - all),
+                       of_slot(parts) - (cut ? all : 0), of_slot(tasks) - (cut ? p->work.tiles : 0));
+    return Found::kRun;
+  }
+  __shared__ int64_t sums[4];
+  __shared__ int ends[3][4];
+  __shared__ Portion found;
+  const int per = (count + kThreads - 1) / kThreads;
+  const int from = min(count, tid * per), to = min(count, from + per);
+  int bad = 0;
+  int64_t all = 0;
+  for (int s = from; s < to; ++s) {
+    const SlotWork w = slot_work<ROWS, KEYS, FEW>(a, s, &bad);
+    all += static_cast<int64_t>(w.tiles) * w.walk;
+  }
+  all = over_wave_sum(all);
+  if (lane == 0) sums[wave] = all;
+  if (__syncthreads_or(bad)) {
+    note_tasks(0);
+    return Found::kInvalid;
+  }
+  const int length = portion_length(sums[0] + sums[1] + sums[2] + sums[3]);
+  int mine[3] = {0, 0, 0};
+  for (int s = from; s < to; ++s) {
+    const SlotWork w = slot_work<ROWS, KEYS, FEW>(a, s, &bad);
+    const int splits = splits_of(w, length), items = w.tiles * splits;
+    mine[0] += items;
+    mine[1] += splits > 1 ? items : 0;
+    mine[2] += splits > 1 ? w.tiles : 0;
+  }
+  int before[3], total[3];
+#pragma unroll
+  for (int i = 0; i < 3; ++i) {
+    const int upto = scan_wave(mine[i], lane);
+    if (lane == 63) ends[i][wave] = upto;
+    before[i] = upto - mine[i];
+  }
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < 3; ++i) {
+    total[i] = 0;
+    for (int w = 0; w < 4; ++w) {
+      if (w == wave) before[i] += total[i];
+      total[i] += ends[i][w];
+    }
+  }
+  note_tasks(total[2]);
+  int kv_head = 0;
+  const int64_t item = portion_number<FEW>(total[0], a.kv_heads, &kv_head);
+  if (item < 0) return Found::kNothing;
+  if (item >= before[0] && item < before[0] + mine[0]) {
+    for (int s = from; s < to; ++s) {
+      const SlotWork w = slot_work<ROWS, KEYS, FEW>(a, s, &bad);
+      const int splits = splits_of(w, length), items = w.tiles * splits;
+      if (item < before[0] + items) {
+        Portion here;
+        here.work = w;
+        here.slot = s;
+        here.kv_head = kv_head;
+        here.splits = splits;
+        place_portion<FEW>(&here, static_cast<int>(item - before[0]), before[1], before[2]);
+        found = here;
+        break;
+      }
+      before[0] += items;
+      before[1] += splits > 1 ? items : 0;
+      before[2] += splits > 1 ? w.tiles : 0;
+    }
+  }
+  __syncthreads();
+  *p = found;
+  return Found::kRun;
+}
+
+// The slot of a new token.  (Offsets that decrease make it some slot.)
+template <typename T>
+__device__ __forceinline__ int slot_of_token(const PagedArgs<T>& a, int token, int lane) {
+  const Sequences& q = a.sequences;
+  if (q.offsets == nullptr) return token / q.length;
+  int slot = 0;
+  for (int s = 0; s < q.count; s += 64) {
+    const int upto = __popcll(__ballot(s + lane < q.count && q.offsets[s + lane + 1] <= token));
+    slot += upto;
+    if (upto < 64) break;
+  }
+  return min(slot, q.count - 1);
+}
+template <typename T>
+__device__ __forceinline__ int past_of(const PagedArgs<T>& a, int slot, int fresh) {
+  return max(0, min(a.lengths[slot], 0x7fffffff - 1024 - fresh));
+}
+template <typename T>
+__device__ __forceinline__ int position_of(const PagedArgs<T>& a, int token, int slot) {
+  const Sequences& q = a.sequences;
+  const int begin = q.offsets == nullptr ? slot * q.length : q.offsets[slot];
+  const int fresh = q.offsets == nullptr ? q.length : q.offsets[slot + 1] - begin;
+  return past_of(a, slot, max(0, min(fresh, q.tokens))) + max(0, token - begin);
+}
+
+template <typename T>
+__device__ __forceinline__ bool offsets_valid(const PagedArgs<T>& a, int tid) {
+  const Sequences& q = a.sequences;
+  if (q.offsets == nullptr) return true;
+  int bad = 0;
+  for (int s = tid; s < q.count; s += kThreads) {
+    const int begin = q.offsets[s], end = q.offsets[s + 1];
+    bad |= begin > end || (s == 0 && begin != 0) || (s == q.count - 1 && end != q.tokens);
+  }
+  return !__syncthreads_or(bad);
+}
+
+// ---------------------------------------------------------------------------
+// new tokens
+// ---------------------------------------------------------------------------
+
+// The least and the largest of what they are, or NaN where any of it is.
+__device__ __forceinline__ float lower_of(float a, float b) { return b < a || b != b ? b : a; }
+__device__ __forceinline__ float higher_of(float a, float b) { return b > a || b != b ? b : a; }
+
+// The new tokens on their rows, and the bounds of the pages that they lie on.  A block has one page of
+// one slot and head at a time: no other one changes its bounds.
+template <typename T, bool WHOLE>
+__global__ __launch_bounds__(kThreads) void paged_append_kernel(PagedArgs<T> a) {
+  __shared__ float lows[kMostWidth], highs[kMostWidth];
+  const int tid = threadIdx.x, page = 1 << a.page_shift;
+  const uint32_t block = block_number();
+  const int64_t slot64 = block / a.kv_heads;
+  const int kv_head = static_cast<int>(block % a.kv_heads);
+  if (slot64 >= a.sequences.count) return;
+  const int slot = static_cast<int>(slot64);
+  if (!offsets_valid(a, tid)) return;
+  const Run run = run_of_sequence(a.sequences, slot);
+  if (run.length < 1) return;
+  const int past = past_of(a, slot, run.length);
+  const T* keys = a.key.row(run.batch, run.begin, kv_head);
+  const T* values = a.value.row(run.batch, run.begin, kv_head);
+  constexpr int kElements = 16 / static_cast<int>(sizeof(T));
+  typedef T Piece __attribute__((ext_vector_type(kElements)));
+  for (int64_t number = blockIdx.z;; number += gridDim.z) {
+    const int64_t start = ((static_cast<int64_t>(past) >> a.page_shift) + number) << a.page_shift;
+    if (start >= static_cast<int64_t>(past) + run.length) break;
+    // new tokens [begin, end) of the slot
+    const int begin = static_cast<int>(max(start - past, int64_t{0}));
+    const int end = static_cast<int>(min(start + page - past, static_cast<int64_t>(run.length)));
+    const auto copy = [&](T* pages, int width, const T* from, int64_t stride) {
+      const int pieces = (width + kElements - 1) / kElements;
+      for (int e = tid; e < (end - begin) * pieces; e += kThreads) {
+        const int token = begin + e / pieces, col = e % pieces * kElements;
+        const int64_t row = a.row_of(run.first + token);
+        if (row < 0) continue;
+        const int id = static_cast<int>(row >> a.page_shift), offset = static_cast<int>(row & (page - 1));
+        T* to = pages + a.place(id, kv_head, offset) * width + col;
+        const T* source = from + token * stride + col;
+        if constexpr (WHOLE)
+          *reinterpret_cast<Piece*>(to) = *reinterpret_cast<const Piece*>(source);
+        else
+          for (int i = 0; i < kElements && col + i < width; ++i) to[i] = source[i];
+      }
+    };
+    copy(a.key_pages, a.key_width, keys, a.key.token_stride);
+    copy(a.value_pages, a.value_width, values, a.value.token_stride);
+    if (a.key_bounds == nullptr) continue;
+    const int64_t row = a.row_of(run.first + begin);
+    if (row < 0) continue;  // (the same for the whole block)
+    T* bounds = a.key_bounds + ((row >> a.page_shift) * a.kv_heads + kv_head) * 2 * a.key_width;
+    const int d = tid & (kMostWidth - 1), half = tid / kMostWidth;
+    float low = __builtin_inff(), high = -__builtin_inff();
+    if (d < a.key_width) {
+#pragma unroll 4
+      for (int token = begin + half; token < end; token += 2) {
+        const float x = static_cast<float>(keys[token * a.key.token_stride + d]);
+        low = lower_of(low, x);
+        high = higher_of(high, x);
+      }
+      if (half == 1) {
+        lows[d] = low;
+        highs[d] = high;
+      }
+    }
+    __syncthreads();
+    if (half == 0 && d < a.key_width) {
+      low = lower_of(low, lows[d]);
+      high = higher_of(high, highs[d]);
+      if (start < past) {
+        low = lower_of(low, static_cast<float>(bounds[d]));
+        high = higher_of(high, static_cast<float>(bounds[a.key_width + d]));
+      }
+      bounds[d] = static_cast<T>(low);
+      bounds[a.key_width + d] = static_cast<T>(high);
+    }
+    __syncthreads();
+  }
+}
+
+// ---------------------------------------------------------------------------
+// few rows
+// ---------------------------------------------------------------------------
+
+// A tile of 16 QUERIES rows of a slot and head of keys over a portion of its keys, in tiles of 32 that
+// the waves take in turn; every wave has a softmax of its own, and the waves are joined at the end.
+// Keys go from memory to the operands of the products, values through LDS, which transposes them.
+// With `lists` the keys are those of the pages in a token's list, one behind the other.
+template <typename T, int WIDTH, int QUERIES, bool WHOLE>
+__global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(kWaves<T, WIDTH, WHOLE>))) void
+paged_token_kernel(PagedArgs<T> a) {
+  constexpr int kSteps = WIDTH / 32, kCols = WIDTH / 16, kTile = 32, kRows = 16 * QUERIES;
+  constexpr int kElements = 16 / static_cast<int>(sizeof(T)), kPerRow = WIDTH / kElements;
+  constexpr int kPieces = kTile * kPerRow / 64, kPieceRows = 64 / kPerRow;
+  constexpr int kOuts = WIDTH + 4;
+  typedef T Piece __attribute__((ext_vector_type(kElements)));
+  constexpr size_t kTileBytes = sizeof(Stored<T>) * kTileElements<T, kTile, WIDTH>;
+  constexpr size_t kJoinBytes = sizeof(float) * kRows * kOuts;
+  __shared__ __attribute__((aligned(16))) char shared[4 * (kTileBytes > kJoinBytes ? kTileBytes : kJoinBytes)];
+  __shared__ float tops[4][kRows], totals[4][kRows];
+
+  const int tid = threadIdx.x, lane = tid & 63, group = lane >> 4, column = lane & 15;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  Stored<T>* tile_values = reinterpret_cast<Stored<T>*>(shared) + wave * kTileElements<T, kTile, WIDTH>;
+
+  // what the block works on: rows [row0, row0 + rows) of the tokens behind `first`
+  int kv_head, row0, rows, split, splits, part, task, past, last;
+  int64_t first, batch, begin;
+  const int32_t* table;
+  bool void_rows = false;  // nothing can be said of these tokens
+  if (a.lists != nullptr) {
+    const uint32_t block = block_number();
+    const int tiles = (a.share + kRows - 1) / kRows;
+    kv_head = static_cast<int>(block % a.kv_heads);
+    const int64_t item = block / a.kv_heads;
+    split = static_cast<int>(item % a.list_splits);
+    splits = a.list_splits;
+    const int tile = static_cast<int>(item / splits % tiles);
+    first = item / splits / tiles;
+    if (first >= a.sequences.tokens) return;
+    if (block == 0 && tid == 0 && splits > 1) *a.division.task_count = a.sequences.tokens * tiles;
+    task = static_cast<int>(first) * tiles + tile;
+    part = task * splits + split;
+    row0 = tile * kRows;
+    rows = min(kRows, a.share - row0);
+    const bool packed = a.sequences.offsets != nullptr;
+    batch = packed ? 0 : first / a.sequences.length;
+    begin = packed ? first : first % a.sequences.length;
+    const int64_t at = first * a.kv_heads + kv_head;
+    table = a.lists + at * (a.count + 1);
+    last = a.seen[at] - 1;
+    void_rows = last < 0;
+    past = last;
+  } else {
+    Portion p;
+    const Found found = portion_of<kRows, kTile, true>(a, tid, &p);
+    if (found != Found::kRun) return;  // (invalid offsets: paged_chunk_kernel says so)
+    kv_head = p.kv_head;
+    row0 = p.tile * kRows;
+    rows = min(kRows, p.work.fresh * a.share - row0);
+    split = p.split;
+    splits = p.splits;
+    part = p.part;
+    task = p.task;
+    past = p.work.past;
+    const bool packed = a.sequences.offsets != nullptr;
+    batch = packed ? 0 : p.slot;
+    begin = p.work.begin;
+    first = packed ? p.work.begin : static_cast<int64_t>(p.slot) * a.sequences.length;
+    table = a.tables + static_cast<int64_t>(p.slot) * a.columns;
+    last = static_cast<int>(min(static_cast<int64_t>(past) + (row0 + rows - 1) / a.share, a.capacity() - 1));
+  }
+  const bool single = a.lists != nullptr;
+  if (splits > 1 && split == 0 && kv_head == 0 && tid == 0)
+    a.division.tasks[task] = {first, row0, rows, part, splits};
+
+  const T* fresh_key = a.key.row(batch, begin, kv_head);
+  const T* fresh_value = a.value.row(batch, begin, kv_head);
+  // (in lists every key is on a page: no token sees one behind its own)
+  const int fresh_from = single ? 0x7fffffff : past;
+  if (a.fused && split == 0 && row0 == 0) {
+    const int64_t row = a.row_of(first);
+    if (row >= 0) {
+      const int id = static_cast<int>(row >> a.page_shift);
+      const int64_t to = a.place(id, kv_head, static_cast<int>(row & ((1 << a.page_shift) - 1)));
+      for (int d = tid; d < a.key_width; d += kThreads) a.key_pages[to * a.key_width + d] = fresh_key[d];
+      for (int d = tid; d < a.value_width; d += kThreads) a.value_pages[to * a.value_width + d] = fresh_value[d];
+      if (a.key_bounds != nullptr) {
+        T* bounds = a.key_bounds + (static_cast<int64_t>(id) * a.kv_heads + kv_head) * 2 * a.key_width;
+        const bool alone = (past & ((1 << a.page_shift) - 1)) == 0;
+        for (int d = tid; d < a.key_width; d += kThreads) {
+          const float x = static_cast<float>(fresh_key[d]);
+          bounds[d] = static_cast<T>(alone ? x : lower_of(x, static_cast<float>(bounds[d])));
+          T* high = bounds + a.key_width + d;
+          *high = static_cast<T>(alone ? x : higher_of(x, static_cast<float>(*high)));
+        }
+      }
+    }
+  }
+
+  const int tiles = last >> 5;  // number of the last one
+  const int share = (tiles + splits) / splits;
+  const int tile_end = void_rows ? 0 : min(tiles + 1, (split + 1) * share);
+  const int first_limit = single ? last : past + row0 / a.share;
+
+  // this wave's rows, as the columns of operands (the last one again beyond it)
+  Operand<T> query[QUERIES][kSteps];
+  int limit[QUERIES];
+#pragma unroll
+  for (int i = 0; i < QUERIES; ++i) {
+    const int row = row0 + min(i * 16 + column, rows - 1), token = row / a.share;
+    limit[i] = single ? last : past + token;
+    const Rows<T> query_row = {a.query.row(batch, begin + token, kv_head * a.share + row - token * a.share), 0, 0};
+#pragma unroll
+    for (int s = 0; s < kSteps; ++s) {
+      Frag<T> part_of_row = memory_operand<WHOLE>(query_row, 0, s * 32 + 8 * group, a.key_width);
+      clear_operand<WHOLE>(part_of_row, s * 32, group, a.key_width);
+      query[i][s] = as_operand<T>(part_of_row);
+    }
+  }
+  f32x4 out[QUERIES][kCols];
+  float most[QUERIES], sum[QUERIES];
+#pragma unroll
+  for (int i = 0; i < QUERIES; ++i) {
+    most[i] = -__builtin_inff();
+    sum[i] = 0.0f;
+#pragma unroll
+    for (int d = 0; d < kCols; ++d) out[i][d] = f32x4(0.0f);
+  }
+  const float factor = a.scale * kLog2e;
+
+  Frag<T> key[2][kSteps];
+  Piece held[kPieces];
+  // A half of a tile lies on one page.  Halves behind the last key are its half again, rows behind it
+  // its row: nothing that no token wrote is read.
+  const auto half_begin = [&](int tile, int h) { return min(tile * kTile + h * 16, last & ~15); };
+  const auto look_up = [&](int tile, int (&id)[2]) {
+#pragma unroll
+    for (int h = 0; h < 2; ++h)
+      id[h] = __builtin_amdgcn_readfirstlane(table[half_begin(tile, h) >> a.page_shift]);
+  };
+  const auto fetch = [&](int tile, const int (&id)[2]) {
+    int bad = 0;
+    const T *keys[2], *values[2];
+    int rows_left[2];
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const int at = half_begin(tile, h);
+      const bool there = a.is_page(id[h]);
+      bad |= there ? 0 : 1 << h;
+      const int64_t row = a.place(there ? id[h] : 0, kv_head, at & ((1 << a.page_shift) - 1));
+      keys[h] = a.key_pages + row * a.key_width;
+      values[h] = a.value_pages + row * a.value_width;
+      rows_left[h] = min(15, last - at);
+    }
+    // new tokens are taken from the inputs, whether they have a row or not
+    const bool ends = tile * kTile + kTile > fresh_from;
+    const auto source_of = [&](const T* row_zero, int h, int row, int width, const T* fresh, int64_t stride) {
+      const T* from = row_zero + row * width;
+      if (ends) {
+        const int token = half_begin(tile, h) + row - fresh_from;
+        if (token >= 0) from = fresh + token * stride;
+      }
+      return from;
+    };
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const Rows<T> source = {source_of(keys[h], h, min(column, rows_left[h]), a.key_width, fresh_key,
+                                        a.key.token_stride), 0, 0};
+#pragma unroll
+      for (int s = 0; s < kSteps; ++s)
+        key[h][s] = memory_operand<WHOLE>(source, 0, s * 32 + 8 * group, a.key_width);
+    }
+#pragma unroll
+    for (int i = 0; i < kPieces; ++i) {
+      const int h = i * kPieceRows / 16;
+      const int row = min(i * kPieceRows - 16 * h + lane / kPerRow, rows_left[h]);
+      const int col = lane % kPerRow * kElements;
+      const T* from = source_of(values[h], h, row, a.value_width, fresh_value, a.value.token_stride);
+      if constexpr (WHOLE) {
+        held[i] = *reinterpret_cast<const Piece*>(from + min(col, a.value_width - kElements));
+      } else {
+#pragma unroll
+        for (int e = 0; e < kElements; ++e) held[i][e] = from[min(col + e, a.value_width - 1)];
+      }
+    }
+    return bad;
+  };
+  int tile = split * share + wave, bad = 0, id[2] = {0, 0};
+  if (tile < tile_end) {
+    look_up(tile, id);
+    bad = fetch(tile, id);
+    look_up(tile + 4, id);
+  }
+  for (; tile < tile_end; tile += 4) {
+    f32x4 score[QUERIES][2];
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+#pragma unroll
+      for (int i = 0; i < QUERIES; ++i) score[i][k] = f32x4(0.0f);
+#pragma unroll
+      for (int s = 0; s < kSteps; ++s) {
+        clear_operand<WHOLE>(key[k][s], s * 32, group, a.key_width);
+        const Operand<T> operand = as_operand<T>(key[k][s]);
+#pragma unroll
+        for (int i = 0; i < QUERIES; ++i) score[i][k] = mma(operand, query[i][s], score[i][k]);
+      }
+    }
+    const int missing = bad;
+    if (missing != 0) {  // what is on no page makes NaN of the rows that see it, and nothing of others
+#pragma unroll
+      for (int i = 0; i < kPieces; ++i)
+        if (missing >> (i * kPieceRows / 16) & 1) held[i] = Piece(static_cast<T>(0.0f));
+    }
+    // (LDS accesses of one wave are carried out in order: its tile needs no barrier)
+#pragma unroll
+    for (int i = 0; i < kPieces; ++i) {
+      const int col = lane % kPerRow * kElements;
+      float part_of_row[kElements];
+#pragma unroll
+      for (int e = 0; e < kElements; ++e) part_of_row[e] = static_cast<float>(held[i][e]);
+      store_row<T, kTile, WIDTH>(tile_values, i * kPieceRows + lane / kPerRow, col, part_of_row);
+    }
+    asm volatile("" ::: "memory");
+    if (tile + 4 < tile_end) {
+      bad = fetch(tile + 4, id);
+      look_up(tile + 8, id);
+    }
+    if (missing != 0) {
+#pragma unroll
+      for (int k = 0; k < 2; ++k)
+        if (missing >> k & 1)
+#pragma unroll
+          for (int i = 0; i < QUERIES; ++i) score[i][k] = f32x4(__builtin_nanf(""));
+    }
+    Operand<T> weights[QUERIES];
+#pragma unroll
+    for (int i = 0; i < QUERIES; ++i) {
+      if (tile * kTile + kTile - 1 > first_limit) {
+#pragma unroll
+        for (int k = 0; k < 2; ++k)
+#pragma unroll
+          for (int r = 0; r < 4; ++r)
+            if (tile * kTile + k * 16 + 4 * group + r > min(limit[i], last)) score[i][k][r] = -__builtin_inff();
+      }
+      float here = -__builtin_inff();
+#pragma unroll
+      for (int k = 0; k < 2; ++k)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) here = fmaxf(here, score[i][k][r]);
+      here = over_groups_max(here) * factor;
+      if (__any(here > most[i])) {
+        const float larger = fmaxf(here, most[i]);
+        const float shrink = larger == -__builtin_inff() ? 1.0f : exp2_of(most[i] - larger);
+        sum[i] *= shrink;
+#pragma unroll
+        for (int d = 0; d < kCols; ++d) out[i][d] *= shrink;
+        most[i] = larger;
+      }
+      const float base = (most[i] == -__builtin_inff() ? 0.0f : most[i]) - kLift<T>;
+#pragma unroll
+      for (int k = 0; k < 2; ++k)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          score[i][k][r] = exp2_of(score[i][k][r] * factor - base);
+          sum[i] += score[i][k][r];
+        }
+      weights[i] = operand_of<T>(score[i][0], score[i][1]);
+    }
+#pragma unroll
+    for (int d = 0; d < kCols; ++d) {
+      const Operand<T> value = column_operand<T, kTile, WIDTH>(tile_values, 0, d * 16, lane);
+#pragma unroll
+      for (int i = 0; i < QUERIES; ++i) out[i][d] = mma(value, weights[i], out[i][d]);
+    }
+    asm volatile("" ::: "memory");
+  }
+
+  // the waves of the block
+  __syncthreads();
+  float* outs = reinterpret_cast<float*>(shared) + wave * kRows * kOuts;
+#pragma unroll
+  for (int i = 0; i < QUERIES; ++i) {
+    const float total = over_groups_sum(sum[i]);
+#pragma unroll
+    for (int d = 0; d < kCols; ++d)
+      *reinterpret_cast<f32x4*>(outs + (i * 16 + column) * kOuts + d * 16 + 4 * group) = out[i][d];
+    if (group == 0) {
+      // tokens behind the table have a key that is on no page
+      const bool lost = void_rows || (!single && limit[i] >= a.capacity());
+      tops[wave][i * 16 + column] = most[i];
+      totals[wave][i * 16 + column] = lost ? __builtin_nanf("") : total;
+    }
+  }
+  __syncthreads();
+  float* partial = a.division.partial + (static_cast<int64_t>(kv_head) * a.division.parts + part) * kRows * kOuts;
+  for (int e = tid; e < rows * a.value_width; e += kThreads) {
+    const int m = e / a.value_width, d = e % a.value_width;
+    const float top = fmaxf(fmaxf(tops[0][m], tops[1][m]), fmaxf(tops[2][m], tops[3][m]));
+    float total = 0.0f, value = 0.0f;
+#pragma unroll
+    for (int w = 0; w < 4; ++w) {
+      const float by = top == -__builtin_inff() ? 1.0f : exp2_of(tops[w][m] - top);
+      total += by * totals[w][m];
+      value += by * (reinterpret_cast<float*>(shared) + w * kRows * kOuts)[m * kOuts + d];
+    }
+    if (splits == 1) {
+      const int row = row0 + m, token = row / a.share;
+      const int64_t at = (first + token) * a.heads + kv_head * a.share + row - token * a.share;
+      a.out[at * a.value_width + d] = static_cast<T>(value / total);
+    } else {
+      float* to = partial + m * kOuts;
+      to[d] = value;
+      if (d == 0) {
+        to[WIDTH] = top;
+        to[WIDTH + 1] = total;
+      }
+    }
+  }
+}
+
+// ---------------------------------------------------------------------------
+// many rows
+// ---------------------------------------------------------------------------
+
+// 64 QUERIES rows of a slot and head of keys, 16 QUERIES to a wave, over a portion of its keys in tiles
+// of 64: keys and values go through registers to LDS while the tile before is worked on, queries and
+// sums stay in registers.  Weights are rounded to the inputs' type, as the operand of the product with
+// the values, and summed as rounded.
+template <typename T, int WIDTH, int QUERIES, bool WHOLE>
+__global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(kWaves<T, WIDTH, WHOLE>))) void
+paged_chunk_kernel(PagedArgs<T> a) {
+  constexpr int kSteps = WIDTH / 32, kRows = 64 * QUERIES, kCols = WIDTH / 16;
+  constexpr int kTile = kTileElements<T, kKeys, WIDTH>;
+  __shared__ __attribute__((aligned(16))) Stored<T> key_tiles[kBuffers<T> * kTile];
+  __shared__ __attribute__((aligned(16))) Stored<T> value_tiles[kBuffers<T> * kTile];
+
+  const int tid = threadIdx.x, lane = tid & 63, group = lane >> 4, column = lane & 15;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  Portion p;
+  const Found found = portion_of<kRows, kKeys, false>(a, tid, &p);
+  if (found != Found::kRun) {
+    if (found == Found::kInvalid) {
+      const int64_t elements = static_cast<int64_t>(a.sequences.tokens) * a.heads * a.value_width;
+      const int64_t blocks = static_cast<int64_t>(gridDim.x) * gridDim.y;
+      for (int64_t e = static_cast<int64_t>(blockIdx.y * gridDim.x + blockIdx.x) * kThreads + tid;
+           e < elements; e += blocks * kThreads)
+        a.out[e] = static_cast<T>(__builtin_nanf(""));
+    }
+    return;
+  }
+  const int kv_head = p.kv_head, past = p.work.past, row0 = p.tile * kRows;
+  const int rows = min(kRows, p.work.fresh * a.share - row0);
+  const bool packed = a.sequences.offsets != nullptr;
+  const int64_t batch = packed ? 0 : p.slot, begin_token = p.work.begin;
+  const int64_t first_token = packed ? p.work.begin : static_cast<int64_t>(p.slot) * a.sequences.length;
+  const int32_t* table = a.tables + static_cast<int64_t>(p.slot) * a.columns;
+  const int64_t capacity = a.capacity();
+  const int last = static_cast<int>(min(static_cast<int64_t>(past) + (row0 + rows - 1) / a.share, capacity - 1));
+  if (p.splits > 1 && p.split == 0 && kv_head == 0 && tid == 0)
+    a.division.tasks[p.task] = {first_token, row0, rows, p.part, p.splits};
+
+  // this wave's rows, as the columns of operands (the last one again beyond it)
+  const int wave_row = row0 + wave * 16 * QUERIES;
+  const int wave_first = past + min(wave_row, row0 + rows - 1) / a.share;
+  const int wave_last = past + min(wave_row + 16 * QUERIES, row0 + rows) / a.share;  // or one before
+  Operand<T> query[QUERIES][kSteps];
+  int limit[QUERIES];
+#pragma unroll
+  for (int i = 0; i < QUERIES; ++i) {
+    const int row = min(wave_row + i * 16 + column, row0 + rows - 1), token = row / a.share;
+    limit[i] = past + token;
+    const Rows<T> query_row = {
+        a.query.row(batch, begin_token + token, kv_head * a.share + row - token * a.share), 0, 0};
+#pragma unroll
+    for (int s = 0; s < kSteps; ++s) {
+      Frag<T> part = memory_operand<WHOLE>(query_row, 0, s * 32 + 8 * group, a.key_width);
+      clear_operand<WHOLE>(part, s * 32, group, a.key_width);
+      query[i][s] = as_operand<T>(part);
+    }
+  }
+  f32x4 out[QUERIES][kCols];
+  float most[QUERIES];
+  f32x4 sum[QUERIES];  // (a product with ones: every row of the result is the sum)
+#pragma unroll
+  for (int i = 0; i < QUERIES; ++i) {
+    most[i] = -__builtin_inff();
+    sum[i] = f32x4(0.0f);
+#pragma unroll
+    for (int d = 0; d < kCols; ++d) out[i][d] = f32x4(0.0f);
+  }
+  const float factor = a.scale * kLog2e;
+
+  // A quarter of a tile lies on one page, whose number a lane of the wave's first four holds.
+  // Quarters and rows behind the last key are the last one's again.
+  TileMove<T, kKeys, WIDTH, WHOLE> key_move, value_move;
+  const Rows<T> fresh_keys = a.key.rows(batch, begin_token, kv_head, p.work.fresh);
+  const Rows<T> fresh_values = a.value.rows(batch, begin_token, kv_head, p.work.fresh);
+  const auto look_up = [&](int tile) {
+    return table[min(tile * kKeys + 16 * (lane & 3), last & ~15) >> a.page_shift];
+  };
+  const auto missing_of = [&](int ids) {
+    return static_cast<int>(__ballot(lane < 4 && !a.is_page(ids)));
+  };
+  const auto fetch = [&](int tile, int ids) {
+    const int begin = tile * kKeys, left = min(kKeys - 1, last - begin);
+    ids = a.is_page(ids) ? ids : 0;
+    const auto row_at = [&](int row) {
+      row = min(row, left);
+      const int quarter = __builtin_amdgcn_readfirstlane(row >> 4);
+      const int id = __builtin_amdgcn_readlane(ids, quarter);
+      return a.place(id, kv_head, (begin + 16 * quarter) & ((1 << a.page_shift) - 1)) + (row & 15);
+    };
+    if (begin >= past) {  // new tokens are taken from the inputs, whether they have a row or not
+      key_move.fetch(rows_from(fresh_keys, begin - past, left + 1), a.key_width, tid);
+      value_move.fetch(rows_from(fresh_values, begin - past, left + 1), a.value_width, tid);
+    } else if (begin + left < past) {
+      key_move.fetch_from([&](int row, int col) { return a.key_pages + row_at(row) * a.key_width + col; },
+                          a.key_width, tid);
+      value_move.fetch_from([&](int row, int col) { return a.value_pages + row_at(row) * a.value_width + col; },
+                            a.value_width, tid);
+    } else {
+      const auto from = [&](const T* pages, int width, const Rows<T>& fresh, int row, int col) {
+        const T* held = pages + row_at(row) * width;
+        const int token = begin + min(row, left) - past;
+        return (token >= 0 ? fresh.base + token * fresh.stride : held) + col;
+      };
+      key_move.fetch_from([&](int row, int col) { return from(a.key_pages, a.key_width, fresh_keys, row, col); },
+                          a.key_width, tid);
+      value_move.fetch_from(
+          [&](int row, int col) { return from(a.value_pages, a.value_width, fresh_values, row, col); },
+          a.value_width, tid);
+    }
+  };
+  const int tiles = last / kKeys + 1, share = (tiles + p.splits - 1) / p.splits;
+  const int tile_end = min(tiles, (p.split + 1) * share);
+  int tile = p.split * share;
+  int ids = 0, next_missing = 0;
+  if (tile < tile_end) {
+    ids = look_up(tile);
+    next_missing = missing_of(ids);
+    fetch(tile, ids);
+    ids = look_up(tile + 1);
+  }
+  for (int side = 0; tile < tile_end; ++tile, side = kBuffers<T> - 1 - side) {
+    const int begin = tile * kKeys, missing = next_missing;
+    Stored<T>*keys = key_tiles + side * kTile, *values = value_tiles + side * kTile;
+    if (missing != 0) {  // what is on no page makes NaN of the rows that see it, and nothing of others
+#pragma unroll
+      for (int i = 0; i < value_move.kPieces; ++i)
+        if (missing >> (value_move.row_of(i, tid) >> 4) & 1)
+          value_move.held[i] = typename TileMove<T, kKeys, WIDTH, WHOLE>::Piece(static_cast<T>(0.0f));
+    }
+    key_move.store(keys, a.key_width, tid);
+    value_move.store(values, a.value_width, tid);
+    __syncthreads();
+    if (tile + 1 < tile_end) {
+      next_missing = missing_of(ids);
+      fetch(tile + 1, ids);
+      ids = look_up(tile + 2);
+    }
+    if (begin <= wave_last && wave_row < row0 + rows) {
+      f32x4 score[QUERIES][4];
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+#pragma unroll
+        for (int i = 0; i < QUERIES; ++i) score[i][k] = f32x4(0.0f);
+#pragma unroll
+        for (int s = 0; s < kSteps; ++s) {
+          const Operand<T> key = row_operand<T, kKeys, WIDTH>(keys, k * 16, s * 32, lane);
+#pragma unroll
+          for (int i = 0; i < QUERIES; ++i) score[i][k] = mma(key, query[i][s], score[i][k]);
+        }
+      }
+      if (missing != 0) {
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+          if (missing >> k & 1)
+#pragma unroll
+            for (int i = 0; i < QUERIES; ++i) score[i][k] = f32x4(__builtin_nanf(""));
+      }
+      if (begin + kKeys - 1 > min(wave_first, last)) {
+#pragma unroll
+        for (int i = 0; i < QUERIES; ++i) {
+          const int upto = min(limit[i], last) - begin - 4 * group;
+#pragma unroll
+          for (int k = 0; k < 4; ++k)
+#pragma unroll
+            for (int r = 0; r < 4; ++r)
+              score[i][k][r] = k * 16 + r <= upto ? score[i][k][r] : -__builtin_inff();
+        }
+      }
+      Operand<T> weights[QUERIES][2];
+#pragma unroll
+      for (int i = 0; i < QUERIES; ++i) {
+        float here = score[i][0][0];
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+#pragma unroll
+          for (int r = 0; r < 4; ++r) here = fmaxf(here, score[i][k][r]);
+        here = over_groups_max(here) * factor;
+        if (__any(here > most[i] + kSlack)) {
+          const float larger = fmaxf(here, most[i]);
+          const float shrink = larger == -__builtin_inff() ? 1.0f : exp2_of(most[i] - larger);
+          sum[i] *= shrink;
+#pragma unroll
+          for (int d = 0; d < kCols; ++d) out[i][d] *= shrink;
+          most[i] = larger;
+        }
+        const float base = (most[i] == -__builtin_inff() ? 0.0f : most[i]) - kLift<T>;
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+#pragma unroll
+          for (int r = 0; r < 4; ++r) score[i][k][r] = exp2_of(score[i][k][r] * factor - base);
+#pragma unroll
+        for (int half = 0; half < 2; ++half) {
+          weights[i][half] = operand_of<T>(score[i][2 * half], score[i][2 * half + 1]);
+          sum[i] = add_sums<T>(weights[i][half], sum[i]);
+        }
+      }
+#pragma unroll
+      for (int half = 0; half < 2; ++half)
+#pragma unroll
+        for (int d = 0; d < kCols; ++d) {
+          const Operand<T> value = column_operand<T, kKeys, WIDTH>(values, half * 32, d * 16, lane);
+#pragma unroll
+          for (int i = 0; i < QUERIES; ++i) out[i][d] = mma(value, weights[i][half], out[i][d]);
+        }
+    }
+    if constexpr (kBuffers<T> == 1) __syncthreads();
+  }
+
+#pragma unroll
+  for (int i = 0; i < QUERIES; ++i) {
+    const int row = wave_row + i * 16 + column;
+    if (row >= row0 + rows) continue;
+    // tokens behind the table have a key that is on no page
+    const float total = limit[i] >= capacity ? __builtin_nanf("") : sum[i][0];
+    const int token = row / a.share;
+    if (p.splits == 1) {
+      const int64_t at = (first_token + token) * a.heads + kv_head * a.share + row - token * a.share;
+      store_tiles<WHOLE, false>(a.out + at * a.value_width, out[i], 1.0f / total, group, a.value_width);
+    } else {
+      constexpr int kOuts = WIDTH + 4;
+      float* to = a.division.partial +
+                  ((static_cast<int64_t>(kv_head) * a.division.parts + p.part) * kRows + row - row0) * kOuts;
+#pragma unroll
+      for (int d = 0; d < kCols; ++d) *reinterpret_cast<f32x4*>(to + d * 16 + 4 * group) = out[i][d];
+      if (group == 0) {
+        to[WIDTH] = most[i];
+        to[WIDTH + 1] = total;
+      }
+    }
+  }
+}
+
+// ---------------------------------------------------------------------------
+// tiles that were cut
+// ---------------------------------------------------------------------------
+
+// The parts of a row.  BLOCK: a block has a row, whose parts its waves add up in turn, as of few rows
+// there are many; otherwise a wave has it.
+template <typename T, int WIDTH, bool BLOCK>
+__global__ __launch_bounds__(kThreads) void paged_join_kernel(PagedArgs<T> a, int tile_rows) {
+  constexpr int kOuts = WIDTH + 4;
+  __shared__ float weights[BLOCK ? kMostPortions : 1], sums[kThreads], tops[4], totals[4];
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const int64_t units = static_cast<int64_t>(*a.division.task_count) * a.kv_heads * tile_rows;
+  const int64_t apart = static_cast<int64_t>(tile_rows) * kOuts;
+  for (int64_t unit = BLOCK ? blockIdx.x : static_cast<int64_t>(blockIdx.x) * 4 + wave; unit < units;
+       unit += BLOCK ? gridDim.x : static_cast<int64_t>(gridDim.x) * 4) {
+    const PagedTask task = a.division.tasks[unit / tile_rows / a.kv_heads];
+    const int kv_head = static_cast<int>(unit / tile_rows % a.kv_heads), r = static_cast<int>(unit % tile_rows);
+    if (r >= task.rows) continue;
+    const float* parts = a.division.partial +
+                         ((static_cast<int64_t>(kv_head) * a.division.parts + task.part) * tile_rows + r) * kOuts;
+    const int row = task.row + r, token = row / a.share;
+    T* out = a.out + ((task.first + token) * a.heads + kv_head * a.share + row - token * a.share) * a.value_width;
+    float top = -__builtin_inff(), total = 0.0f;
+    if constexpr (BLOCK) {
+      for (int s = tid; s < task.splits; s += kThreads) {
+        weights[s] = parts[s * apart + WIDTH];
+        top = fmaxf(top, weights[s]);
+      }
+      for (int away = 1; away < 64; away *= 2) top = fmaxf(top, __shfl_xor(top, away));
+      if (lane == 0) tops[wave] = top;
+      __syncthreads();
+      top = fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3]));
+      for (int s = tid; s < task.splits; s += kThreads) {
+        const float by = top == -__builtin_inff() ? 1.0f : exp2_of(weights[s] - top);
+        weights[s] = by;
+        total += by * parts[s * apart + WIDTH + 1];
+      }
+      for (int away = 1; away < 64; away *= 2) total += __shfl_xor(total, away);
+      if (lane == 0) totals[wave] = total;
+      __syncthreads();
+      total = totals[0] + totals[1] + totals[2] + totals[3];
+      for (int col0 = 0; col0 < a.value_width; col0 += 64) {
+        const int col = col0 + lane;
+        float value = 0.0f;
+        if (col < a.value_width) {
+#pragma unroll 8
+          for (int s = wave; s < task.splits; s += 4) value += weights[s] * parts[s * apart + col];
+        }
+        sums[tid] = value;
+        __syncthreads();
+        if (wave == 0 && col < a.value_width)
+          out[col] = static_cast<T>((sums[lane] + sums[64 + lane] + sums[128 + lane] + sums[192 + lane]) / total);
+        __syncthreads();
+      }
+    } else {
+      for (int s = 0; s < task.splits; ++s) top = fmaxf(top, parts[s * apart + WIDTH]);
+      float value[2] = {0.0f, 0.0f};
+      for (int s = 0; s < task.splits; ++s) {
+        const float* part = parts + s * apart;
+        const float by = top == -__builtin_inff() ? 1.0f : exp2_of(part[WIDTH] - top);
+        total += by * part[WIDTH + 1];
+#pragma unroll
+        for (int c = 0; c < 2; ++c)
+          if (c * 64 < WIDTH) value[c] += by * part[min(c * 64 + lane, WIDTH - 1)];
+      }
+#pragma unroll
+      for (int c = 0; c < 2; ++c)
+        if (c * 64 + lane < a.value_width) out[c * 64 + lane] = static_cast<T>(value[c] / total);
+    }
+  }
+}
+
+// ---------------------------------------------------------------------------
+// selected pages
+// ---------------------------------------------------------------------------
+
+// The largest product that a key within a page's bounds can have with a query of the group, in 64 bits,
+// in which the products are exact: pages are ranked as their bounds rank, whatever the order of a sum.
+// A block has 64 pages of a token and head of keys at a time, a page to a lane and a quarter of the
+// columns to a wave.
+template <typename T, bool WHOLE>
+__global__ __launch_bounds__(kThreads) void paged_score_kernel(PagedArgs<T> a, int blocks_of_token) {
+  constexpr int kElements = 16 / static_cast<int>(sizeof(T)), kMembers = 4;
+  typedef T Piece __attribute__((ext_vector_type(kElements)));
+  __shared__ __attribute__((aligned(16))) float queries[kMembers][kMostWidth];
+  __shared__ double sums[4][kMembers][64];
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const uint32_t block = block_number();
+  const int64_t at = block / blocks_of_token;
+  const int64_t number = at / a.kv_heads;
+  const int kv_head = static_cast<int>(at % a.kv_heads);
+  if (number >= a.slab_tokens) return;
+  const int token = static_cast<int>(a.slab_first + number);
+  const int slot = slot_of_token(a, token, lane);
+  const int earlier = min(position_of(a, token, slot) >> a.page_shift, a.columns);
+  if (earlier <= a.count) return;  // all of them are selected
+  const bool packed = a.sequences.offsets != nullptr;
+  const int32_t* table = a.tables + static_cast<int64_t>(slot) * a.columns;
+  double* scores = a.scores + at * a.columns;
+  const int pieces = (a.key_width + kElements - 1) / kElements;
+  for (int base = static_cast<int>(block % blocks_of_token) * 64; base < earlier; base += blocks_of_token * 64) {
+    const int page = min(base + lane, earlier - 1), id = table[page];
+    const bool there = a.is_page(id);
+    const T* low = a.key_bounds + (static_cast<int64_t>(there ? id : 0) * a.kv_heads + kv_head) * 2 * a.key_width;
+    const T* high = low + a.key_width;
+    double best = -__builtin_inf();
+    for (int member0 = 0; member0 < a.share; member0 += kMembers) {
+      const int members = min(kMembers, a.share - member0);
+      __syncthreads();
+      for (int e = tid; e < kMembers * kMostWidth; e += kThreads) {
+        const int m = e / kMostWidth, d = e % kMostWidth;
+        const int head = kv_head * a.share + member0 + min(m, members - 1);
+        const T* query = packed ? a.query.row(0, token, head)
+                                : a.query.row(slot, token - slot * a.sequences.length, head);
+        queries[m][d] = d < a.key_width ? static_cast<float>(query[d]) : 0.0f;
+      }
+      __syncthreads();
+      double sum[kMembers] = {};
+      for (int piece = wave; piece < pieces; piece += 4) {
+        const int col = piece * kElements;
+        Piece lows, highs;
+        if constexpr (WHOLE) {
+          lows = *reinterpret_cast<const Piece*>(low + col);
+          highs = *reinterpret_cast<const Piece*>(high + col);
+        } else {
+#pragma unroll
+          for (int e = 0; e < kElements; ++e) {
+            lows[e] = col + e < a.key_width ? low[col + e] : static_cast<T>(0.0f);
+            highs[e] = col + e < a.key_width ? high[col + e] : static_cast<T>(0.0f);
+          }
+        }
+#pragma unroll
+        for (int e = 0; e < kElements; ++e) {
+          const float least = static_cast<float>(lows[e]), largest = static_cast<float>(highs[e]);
+#pragma unroll
+          for (int m = 0; m < kMembers; ++m) {
+            const float q = queries[m][col + e];
+            sum[m] = fma(static_cast<double>(q), static_cast<double>(q > 0.0f ? largest : least), sum[m]);
+          }
+        }
+      }
+#pragma unroll
+      for (int m = 0; m < kMembers; ++m) sums[wave][m][lane] = sum[m];
+      __syncthreads();
+      if (wave == 0) {
+#pragma unroll
+        for (int m = 0; m < kMembers; ++m) {
+          const double score = ((sums[0][m][lane] + sums[1][m][lane]) + sums[2][m][lane]) + sums[3][m][lane];
+          best = score > best || score != score ? score : best;
+        }
+      }
+    }
+    if (wave == 0 && base + lane < earlier) scores[page] = there ? best : __builtin_nan("");
+  }
+}
+
+// A score as a whole number that ranks alike; what is no number ranks first.
+__device__ __forceinline__ uint64_t rank_of(double score) {
+  if (score != score) return ~uint64_t{0};
+  const uint64_t bits = __builtin_bit_cast(uint64_t, score + 0.0);  // (no zero below zero)
+  return bits >> 63 ? ~bits : bits | uint64_t{1} << 63;
+}
+
+// The pages of a token and head of keys: the `count` with the largest scores, in the order of the
+// slot's table, and its own; and how many positions it sees on them.  A block finds the score of the
+// last one that is selected eight bits at a time, by counting.
+template <typename T>
+__global__ __launch_bounds__(kThreads) void paged_select_kernel(PagedArgs<T> a) {
+  __shared__ int counts[256], ends[4], equal_ends[4], chosen[2];
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const int64_t at = block_number(), number = at / a.kv_heads;
+  if (number >= a.slab_tokens) return;
+  const int token = static_cast<int>(a.slab_first + number);
+  const int64_t to = static_cast<int64_t>(token) * a.kv_heads + at % a.kv_heads;
+  int32_t* list = a.lists + to * (a.count + 1);
+  if (!offsets_valid(a, tid)) {
+    if (tid == 0) a.seen[to] = 0;
+    return;
+  }
+  const int slot = slot_of_token(a, token, lane), position = position_of(a, token, slot);
+  const int32_t* table = a.tables + static_cast<int64_t>(slot) * a.columns;
+  const int own = position >> a.page_shift, earlier = min(own, a.columns);
+  const int selected = min(earlier, a.count);
+  if (tid == 0) {
+    list[selected] = own < a.columns ? table[own] : -1;
+    a.seen[to] = (selected << a.page_shift) + (position & ((1 << a.page_shift) - 1)) + 1;
+  }
+  if (earlier <= a.count) {
+    for (int j = tid; j < earlier; j += kThreads) list[j] = table[j];
+    return;
+  }
+  const double* scores = a.scores + at * a.columns;
+  // those above `prefix` in the bits of `mask` are selected, and the first `need` of those equal to it
+  uint64_t prefix = 0, mask = 0;
+  int need = a.count;
+  for (int shift = 56; shift >= 0; shift -= 8) {
+    counts[tid] = 0;
+    __syncthreads();
+    for (int j = tid; j < earlier; j += kThreads) {
+      const uint64_t rank = rank_of(scores[j]);
+      if ((rank & mask) == prefix) atomicAdd(&counts[rank >> shift & 255], 1);
+    }
+    __syncthreads();
+    const int mine = counts[255 - tid], upto = scan_wave(mine, lane);
+    if (lane == 63) ends[wave] = upto;
+    __syncthreads();
+    int before = upto - mine;
+    for (int w = 0; w < wave; ++w) before += ends[w];
+    if (before < need && need <= before + mine) {
+      chosen[0] = 255 - tid;
+      chosen[1] = before;
+    }
+    __syncthreads();
+    const int digit = chosen[0];
+    need -= chosen[1];
+    prefix |= static_cast<uint64_t>(digit) << shift;
+    mask |= uint64_t{255} << shift;
+    const bool all = counts[digit] == need;
+    __syncthreads();
+    if (all) break;
+  }
+  int above = 0, equal = 0;  // of the pages so far
+  for (int base = 0; base < earlier; base += kThreads) {
+    const int j = base + tid;
+    const uint64_t rank = j < earlier ? rank_of(scores[j]) & mask : 0;
+    const bool more = j < earlier && rank > prefix, same = j < earlier && rank == prefix;
+    const uint64_t more_mask = __ballot(more), same_mask = __ballot(same);
+    if (lane == 0) {
+      ends[wave] = __popcll(more_mask);
+      equal_ends[wave] = __popcll(same_mask);
+    }
+    __syncthreads();
+    const uint64_t below = (uint64_t{1} << lane) - 1;
+    int above_me = above + __popcll(more_mask & below), equal_me = equal + __popcll(same_mask & below);
+    for (int w = 0; w < 4; ++w) {
+      if (w < wave) {
+        above_me += ends[w];
+        equal_me += equal_ends[w];
+      }
+      above += ends[w];
+      equal += equal_ends[w];
+    }
+    if (more || (same && equal_me < need)) list[above_me + min(equal_me, need)] = table[j];
+    __syncthreads();
+  }
+}
+
+// ---------------------------------------------------------------------------
+// launches
+// ---------------------------------------------------------------------------
+
+template <typename T>
+PagedArgs<T> paged_args(const PagedCall& call) {
+  const rosa_mixer_problem& p = *call.problem;
+  const rosa_paged_cache& c = *call.cache;
+  PagedArgs<T> args{};
+  args.query = view_of<T>(*call.query);
+  args.key = view_of<T>(*call.key);
+  args.value = view_of<T>(*call.value);
+  args.out = static_cast<T*>(call.out);
+  args.key_pages = static_cast<T*>(c.key_pages);
+  args.value_pages = static_cast<T*>(c.value_pages);
+  args.key_bounds = static_cast<T*>(c.key_bounds);
+  args.tables = c.tables;
+  args.lengths = c.lengths;
+  args.rows = c.rows;
+  args.sequences = sequences_of(p);
+  args.pages = c.pages;
+  args.columns = c.columns;
+  args.page_shift = __builtin_ctz(static_cast<unsigned>(c.page));
+  args.heads = p.H;
+  args.kv_heads = p.Hkv;
+  args.share = p.H / p.Hkv;
+  args.key_width = p.D;
+  args.value_width = p.Dv;
+  args.scale = p.scale;
+  args.count = call.count;
+  return args;
+}
+
+template <typename T>
+PagedDivision division_of(const PagedShare& share, int most_few, char* at) {
+  PagedDivision d{};
+  d.target = share.target;
+  d.least = share.least;
+  d.most_few = most_few;
+  d.parts = share.parts;
+  if (share.parts > 0) {
+    d.partial = reinterpret_cast<float*>(at);
+    d.task_count = reinterpret_cast<int*>(at + share.part_bytes);
+    d.tasks = reinterpret_cast<PagedTask*>(at + share.part_bytes + 256);
+  }
+  return d;
+}
+
+constexpr int kJoinBlocks = 2048;
+
+template <typename T, int WIDTH, bool WHOLE>
+void paged_token_launch(PagedArgs<T>& args, const PagedShare& share, hipStream_t stream) {
+  const dim3 grid = grid_of(share.items * args.kv_heads);
+  if constexpr (sizeof(T) == 2) {
+    if (share.rows == 32) paged_token_kernel<T, WIDTH, 2, WHOLE><<<grid, kThreads, 0, stream>>>(args);
+  }
+  if (share.rows == 16) paged_token_kernel<T, WIDTH, 1, WHOLE><<<grid, kThreads, 0, stream>>>(args);
+  if (share.parts == 0) return;
+  const int64_t rows = share.parts / 2 * args.kv_heads * share.rows;  // (a cut tile has two parts or more)
+  paged_join_kernel<T, WIDTH, true>
+      <<<dim3(static_cast<unsigned>(rows < kJoinBlocks ? rows : kJoinBlocks)), kThreads, 0, stream>>>(
+          args, share.rows);
+}
+
+template <typename T, int WIDTH, bool WHOLE>
+void paged_chunk_launch(PagedArgs<T>& args, const PagedShare& share, hipStream_t stream) {
+  const dim3 grid = grid_of_items(share.items * args.kv_heads);
+  if constexpr (kPairs<T, WIDTH>) {
+    if (share.rows == 128) paged_chunk_kernel<T, WIDTH, 2, WHOLE><<<grid, kThreads, 0, stream>>>(args);
+  }
+  if (share.rows == 64) paged_chunk_kernel<T, WIDTH, 1, WHOLE><<<grid, kThreads, 0, stream>>>(args);
+  if (share.parts == 0) return;
+  const int64_t waves = share.parts / 2 * args.kv_heads * share.rows;
+  paged_join_kernel<T, WIDTH, false>
+      <<<dim3(static_cast<unsigned>(waves / 4 < kJoinBlocks ? (waves + 3) / 4 : kJoinBlocks)), kThreads, 0,
+         stream>>>(args, share.rows);
+}
+
+template <typename T, bool WHOLE>
+void paged_append_launch(PagedArgs<T>& args, hipStream_t stream) {
+  const Sequences& q = args.sequences;
+  const int64_t most = q.offsets == nullptr ? q.length : q.tokens;  // of a slot
+  const int64_t touched = ((most - 1) >> args.page_shift) + 2;
+  dim3 grid = grid_of(static_cast<int64_t>(q.count) * args.kv_heads);
+  grid.z = static_cast<unsigned>(touched < 64 ? touched : 64);
+  paged_append_kernel<T, WHOLE><<<grid, kThreads, 0, stream>>>(args);
+}
+
+// Scores of a slab of tokens take at most this much memory, or one token's.
+template <typename T, bool WHOLE>
+void paged_select_launch(PagedArgs<T>& args, const PagedPlan& plan, hipStream_t stream) {
+  const int64_t row = static_cast<int64_t>(args.kv_heads) * args.columns * 8;
+  const int64_t slab = static_cast<int64_t>(plan.score_bytes) / row;
+  for (int64_t first = 0; first < args.sequences.tokens; first += slab) {
+    args.slab_first = first;
+    args.slab_tokens = std::min<int64_t>(slab, args.sequences.tokens - first);
+    const int64_t pairs = args.slab_tokens * args.kv_heads;
+    if (args.columns > args.count) {
+      const int64_t most = (args.columns + kScorePages - 1) / kScorePages;
+      const int blocks = static_cast<int>(std::max<int64_t>(1, std::min(most, 2048 / pairs)));
+      paged_score_kernel<T, WHOLE><<<grid_of(pairs * blocks), kThreads, 0, stream>>>(args, blocks);
+    }
+    paged_select_kernel<T><<<grid_of(pairs), kThreads, 0, stream>>>(args);
+  }
+}
+
+template <typename T, int WIDTH, bool WHOLE>
+void paged_update_launch(const PagedCall& call) {
+  const rosa_mixer_problem& p = *call.problem;
+  const PagedPlan plan = paged_plan(p, *call.cache, call.count);
+  PagedArgs<T> args = paged_args<T>(call);
+  char* at = call.workspace;
+  const PagedDivision few = division_of<T>(plan.few, plan.most_few, at);
+  at += plan.few.bytes();
+  const PagedDivision many = division_of<T>(plan.many, plan.most_few, at);
+  at += plan.many.bytes();
+  if (call.count > 0) {
+    paged_append_launch<T, WHOLE>(args, call.stream);
+    args.lists = reinterpret_cast<int32_t*>(at);
+    args.seen = reinterpret_cast<int32_t*>(at + plan.list_bytes);
+    args.scores = reinterpret_cast<double*>(at + plan.list_bytes + plan.seen_bytes);
+    paged_select_launch<T, WHOLE>(args, plan, call.stream);
+    args.division = few;
+    args.list_splits = plan.few.target;
+    return paged_token_launch<T, WIDTH, WHOLE>(args, plan.few, call.stream);
+  }
+  args.fused = p.cu_seqlens == nullptr && p.T == 1 && plan.few.used && !plan.many.used;
+  if (!args.fused) paged_append_launch<T, WHOLE>(args, call.stream);
+  if (plan.few.used) {
+    args.division = few;
+    paged_token_launch<T, WIDTH, WHOLE>(args, plan.few, call.stream);
+  }
+  if (plan.many.used) {
+    args.division = many;
+    paged_chunk_launch<T, WIDTH, WHOLE>(args, plan.many, call.stream);
+  }
+}
+
+template <typename T, bool WHOLE>
+void paged_update_width(const PagedCall& call) {
+  const rosa_mixer_problem& p = *call.problem;
+  switch (padded_width(p.D > p.Dv ? p.D : p.Dv)) {
+    case 32: return paged_update_launch<T, 32, WHOLE>(call);
+    case 64: return paged_update_launch<T, 64, WHOLE>(call);
+    default: return paged_update_launch<T, 128, WHOLE>(call);
+  }
+}
+
+template <typename T>
+void paged_update(const PagedCall& call) {
+  const rosa_mixer_problem& p = *call.problem;
+  const rosa_paged_cache& c = *call.cache;
+  const bool whole = whole_pieces<T>(*call.query, p.D) && whole_pieces<T>(*call.key, p.D) &&
+                     whole_pieces<T>(*call.value, p.Dv) && whole_address(call.out) &&
+                     whole_address(c.key_pages) && whole_address(c.value_pages) &&
+                     whole_address(c.key_bounds);
+  if (whole)
+    paged_update_width<T, true>(call);
+  else
+    paged_update_width<T, false>(call);
+}
+
+}  // namespace rosa_mixer

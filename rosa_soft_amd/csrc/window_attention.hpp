@@ -10,35 +10,10 @@
 // the weights are an operand of the product with the values as they stand.
 #pragma once
 
+#include "attention_device.hpp"
 #include "mixer_calls.hpp"
-#include "mixer_device.hpp"
 
 namespace rosa_mixer {
-
-constexpr int kKeys = 64;  // keys of a tile
-
-// Waves per SIMD that a kernel is compiled for: two, so that products of one overlap the softmax
-// of the other and accumulators share the registers that the rest can use directly; float32 tiles
-// of 128 columns leave room in LDS for one block, and moving 128 columns element by element takes
-// more registers.
-template <typename T, int WIDTH, bool WHOLE>
-constexpr int kWaves = WIDTH == 128 && (sizeof(T) == 4 || !WHOLE) ? 1 : 2;
-constexpr float kLog2e = 1.4426950408889634f;
-
-// Tiles in LDS of the training kernels.  Two of 16 bits, in turn: a wave stores the next while
-// others work on the one before, and one barrier for a tile is enough (it lets no wave past that
-// has not finished the tile before last).  One of float32, whose three planes leave no room.
-template <typename T> constexpr int kBuffers = sizeof(T) == 2 ? 2 : 1;
-
-// Weights are formed as 2^kLift p and rounded so: float16 would lose bits of a weight below 2^-14,
-// which a long window's are.
-template <typename T> constexpr float kLift = kNarrow<T> ? 8.0f : 0.0f;
-template <typename T> constexpr float kUnlift = kNarrow<T> ? 1.0f / 256.0f : 1.0f;
-
-// How far, in exponents of two, a score may pass the reference of its softmax before the sums so
-// far are scaled to a new one: weights up to 2^kSlack (with kLift below float16's largest) are as
-// exact, and most tiles leave the sums alone.
-constexpr float kSlack = 6.0f;
 
 template <typename T>
 struct WindowArgs {
@@ -1240,7 +1215,6 @@ WindowArgs<T> window_args(const WindowCall& call) {
 // and 62.6; of 2048: 195 and 250 us, of 4096 of one: 227 and 296), and where two do not fit the
 // registers (float32, 128 columns).
 constexpr int64_t kFull = 1024;
-template <typename T, int WIDTH> constexpr bool kPairs = !(sizeof(T) == 4 && WIDTH == 128);
 
 template <typename T>
 bool whole_rows(const WindowCall& call) {

@@ -11,13 +11,23 @@ namespace rosa_mixer {
 
 namespace {
 
-constexpr int kPortions = 512;                          // of a call: two blocks for a compute unit
+constexpr int64_t kBlocks = 512;                        // two for a compute unit
+constexpr int kFewRows = 16;                            // of a slot, that paged_token_kernel takes
 constexpr int64_t kMostScoreBytes = int64_t{1} << 28;   // of a slab of tokens
 constexpr int kTableThreads = 1024;
 // Tokens whose rows the block that hands out pages writes by itself; more have a launch of their own.
-constexpr int kFewRows = 16384;
+constexpr int kTokensOfBlock = 16384;
 
 }  // namespace
+
+// Portions of a call, beside one for each tile of rows, and from which part of a portion on a walk has
+// one more.  More share ragged slots out more evenly, and make more partial sums.  Few rows (reads bound
+// them; 64 slots of up to 9000 tokens, 8 heads of 128): 512 portions 296 us, 768 279, 1024 281, 2048 278;
+// two slots of up to 200000, 2 heads of 64: 43, 44, 46 and 50 us.  Many rows, dense (512 tokens behind
+// 60000, 32 heads on 8; 64 behind up to 8000 for each of 8 slots; one prompt of 2048): 512 portions, one
+// more from 3/8 on: 641, 76 and 69 us, from 7/8 on: 641, 98 and 68; 768: 694, 88 and 80.  Packed (a step of
+// 1 to 2047 tokens for 10 slots; 15 single ones and 1024): 139 and 281 us, 141 and 296, 116 and 247.
+constexpr int kFewPortions = 768, kManyPortions = 512, kPackedPortions = 768;
 
 PagedPlan paged_plan(const rosa_mixer_problem& p, const rosa_paged_cache& cache, int count) {
   PagedPlan plan{};
@@ -34,18 +44,19 @@ PagedPlan paged_plan(const rosa_mixer_problem& p, const rosa_paged_cache& cache,
     }
   };
   PagedShare& few = plan.few;
-  const bool two = p.dtype != ROSA_DTYPE_F32;  // two sixteens of rows of a wave fit its registers
+  few.rows = kFewRows;
   if (count > 0) {
-    // tokens on their own, which see about as many keys each
+    // Tokens on their own, which see about as many keys each: until there are two blocks for a compute
+    // unit or a wave has but two tiles.
     few.used = true;
-    few.rows = share <= 16 || !two ? 16 : 32;
     const int64_t tiles = static_cast<int64_t>(p.N) * ((share + few.rows - 1) / few.rows);
     const int64_t walk = (std::min<int64_t>(count + 1, cache.columns) * cache.page + 31) / 32;
     const int64_t blocks = tiles * p.Hkv;
     few.target = static_cast<int>(
-        std::max<int64_t>(1, std::min((kPortions + blocks - 1) / blocks, walk / 8)));
+        std::max<int64_t>(1, std::min((kBlocks + blocks - 1) / blocks, walk / 8)));
     few.items = tiles * few.target;
     few.parts = few.target > 1 ? few.items : 0;
+    few.unit_rows = std::min(few.rows, share);
     finish(&few);
     plan.list_bytes = aligned(static_cast<size_t>(p.N) * p.Hkv * (count + 1) * 4);
     plan.seen_bytes = aligned(static_cast<size_t>(p.N) * p.Hkv * 4);
@@ -54,30 +65,36 @@ PagedPlan paged_plan(const rosa_mixer_problem& p, const rosa_paged_cache& cache,
         row * std::min<int64_t>(p.N, std::max<int64_t>(1, kMostScoreBytes / row)));
     return plan;
   }
-  const int64_t rows = packed ? 0 : static_cast<int64_t>(p.T) * share;  // of a slot
-  const int64_t few_rows = packed ? share : rows;
-  few.used = few_rows <= 32;
-  few.rows = few_rows <= 16 || !two ? 16 : 32;
-  plan.most_few = !few.used ? 0 : few_rows <= 16 ? 16 : 32;
+  // A packed call's single tokens have the kernel for few rows beside the other one, unless prompts are
+  // most of the work: 63 single tokens behind up to 8000, 32 heads on 8, with 5 more tokens of another
+  // slot: 279 us with both, 305 with one; 15 with 1024 more: 269 and 280; 5 rows of single tokens and
+  // 1200 tokens of prompts: 126 and 116.  Of 20 rows (5 tokens, 4 heads on one) the other kernel is
+  // faster as well, 51 us and 62 in two sixteens for 16 slots of up to 4096 tokens.
+  const int64_t rows = packed ? share : static_cast<int64_t>(p.T) * share;  // of a slot, at least
+  few.used = rows <= kFewRows && !(packed && static_cast<int64_t>(p.N) * share >= 64 * sequences);
+  plan.most_few = few.used ? kFewRows : 0;
   if (few.used) {
-    few.target = (2 * kPortions + p.Hkv - 1) / p.Hkv;
-    few.least = 8;
-    few.items = sequences * (plan.most_few / few.rows) + few.target;
+    few.target = (kFewPortions + p.Hkv - 1) / p.Hkv;
+    few.least = 4;
+    few.round = 7;
+    few.unit_rows = packed ? few.rows : static_cast<int>(rows);
+    few.items = sequences + few.target;
     few.parts = (capacity + 31) / 32 > few.least ? 2 * few.target : 0;
     finish(&few);
   }
   PagedShare& many = plan.many;
   many.used = packed || !few.used;
   if (many.used) {
+    // 128 rows, so that an operand read from LDS serves two products, where a slot may have as many and
+    // they fit the registers (float32, 128 columns: they do not).
     const bool pairs = p.dtype != ROSA_DTYPE_F32 || plan.width < 128;
-    const auto tiles_of_rows = [&](int64_t tile) {
-      return packed ? static_cast<int64_t>(p.N) * share / tile + sequences
-                    : sequences * ((rows + tile - 1) / tile);
-    };
-    many.rows = pairs && tiles_of_rows(128) * p.Hkv >= kPortions ? 128 : 64;
-    many.target = (kPortions + p.Hkv - 1) / p.Hkv;
+    many.rows = pairs && (packed || rows > 64) ? 128 : 64;
+    const int64_t tiles = packed ? static_cast<int64_t>(p.N) * share / many.rows + sequences
+                                 : sequences * ((rows + many.rows - 1) / many.rows);
+    many.target = ((packed ? kPackedPortions : kManyPortions) + p.Hkv - 1) / p.Hkv;
     many.least = 4;
-    many.items = tiles_of_rows(many.rows) + many.target;
+    many.round = packed ? 7 : 3;
+    many.items = tiles + many.target;
     many.parts = (capacity + 63) / 64 > many.least ? 2 * many.target : 0;
     finish(&many);
   }
@@ -321,7 +338,7 @@ int rosa_hip_page_tables_update(const rosa_page_tables* tables, const int32_t* c
   args.rows = rows;
   args.T = T;
   args.N = N;
-  const bool all_rows = N <= kFewRows;
+  const bool all_rows = N <= kTokensOfBlock;
   const auto on = static_cast<hipStream_t>(stream);
   const size_t shared = static_cast<size_t>(tables->slots) * (cu_seqlens ? 8 : 4);
   page_tables_update_kernel<<<1, kTableThreads, shared, on>>>(args, all_rows);

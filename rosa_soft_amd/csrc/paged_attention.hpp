@@ -5,14 +5,14 @@
 //   p = softmax_s(scale q_t . k_s) over s <= t (or those of them on selected pages),  o_t = sum_s p_s v_s
 //
 // The query heads of a group share keys and values: the rows of a slot are its (token, member of the
-// group) pairs, member fastest, whatever the number of either.  Slots of up to 16 or 32 rows (single
-// tokens, drafts) are bound by the reads of the cache and have paged_token_kernel, in which the waves
+// group) pairs, member fastest, whatever the number of either.  Slots of up to 16 rows (single tokens,
+// short drafts) are bound by the reads of the cache and have paged_token_kernel, in which the waves
 // of a block share out keys; the others are bound by matrix products and have paged_chunk_kernel, in
 // which they share out rows and keys go through LDS.
 //
 // Neither the host nor a launch knows the slots' lengths.  Every block reads all of them and works out
 // by itself how the call is cut into portions of about the same number of keys, and which is its own
-// (portion_of); tiles that are cut leave partial sums to paged_join_kernel.
+// (portion_of); tiles that are cut leave partial sums to the paged_join kernels.
 #pragma once
 
 #include "attention_device.hpp"
@@ -29,7 +29,7 @@ struct PagedTask {
 };
 
 struct PagedDivision {
-  int target, least, most_few;
+  int target, least, most_few, round;
   int64_t parts;              // of a head of keys: what two of them are apart in `partial`
   float* partial;             // [kv head][part][row][width + 4]: outputs, maximum, sum
   PagedTask* tasks;
@@ -44,11 +44,10 @@ struct PagedArgs {
   const int32_t *tables, *lengths;
   const int64_t* rows;
   Sequences sequences;
-  int64_t pages;
-  int columns, page_shift;
+  int pages, columns, page_shift;
   int heads, kv_heads, share, key_width, value_width;
   float scale;
-  bool fused;                 // single tokens, put on their rows by the kernel that attends
+  bool fused;                 // the kernels that attend put new tokens on their rows
   PagedDivision division;
   // selected pages
   double* scores;             // [token of the slab][kv head][column]
@@ -57,7 +56,7 @@ struct PagedArgs {
   int64_t slab_first, slab_tokens;
 
   __device__ __forceinline__ int64_t capacity() const { return static_cast<int64_t>(columns) << page_shift; }
-  __device__ __forceinline__ bool is_page(int id) const { return id >= 0 && id < pages; }
+  __device__ __forceinline__ bool is_page(int id) const { return static_cast<uint32_t>(id) < static_cast<uint32_t>(pages); }
   // row of a page's head in the pools
   __device__ __forceinline__ int64_t place(int id, int kv_head, int offset) const {
     return ((static_cast<int64_t>(id) * kv_heads + kv_head) << page_shift) + offset;
@@ -65,7 +64,7 @@ struct PagedArgs {
   // the row that a new token is put on, or -1
   __device__ __forceinline__ int64_t row_of(int64_t token) const {
     const int64_t row = rows[token];
-    return row >= 0 && row < pages << page_shift ? row : -1;
+    return row >= 0 && row < static_cast<int64_t>(pages) << page_shift ? row : -1;
   }
 };
 
@@ -104,16 +103,29 @@ struct Portion {
   int slot, kv_head, tile, split, splits, part, task;
 };
 
-__device__ __forceinline__ int64_t over_wave_sum(int64_t x) {
-  for (int apart = 1; apart < 64; apart *= 2) x += __shfl_xor(static_cast<long long>(x), apart);
+// Inclusive sum over the lanes of a wave: within rows of 16 lanes, then the last lane of a row to the
+// next one, and that of the first half to the second.
+__device__ __forceinline__ int scan_wave(int x) {
+  x += __builtin_amdgcn_update_dpp(0, x, 0x111, 0xf, 0xf, true);  // from 1 lane before
+  x += __builtin_amdgcn_update_dpp(0, x, 0x112, 0xf, 0xf, true);  // 2
+  x += __builtin_amdgcn_update_dpp(0, x, 0x114, 0xf, 0xf, true);  // 4
+  x += __builtin_amdgcn_update_dpp(0, x, 0x118, 0xf, 0xf, true);  // 8
+  x += __builtin_amdgcn_update_dpp(0, x, 0x142, 0xa, 0xf, true);  // lane 15 of rows 0 and 2
+  x += __builtin_amdgcn_update_dpp(0, x, 0x143, 0xc, 0xf, true);  // lane 31
   return x;
 }
-__device__ __forceinline__ int scan_wave(int x, int lane) {  // inclusive
-  for (int apart = 1; apart < 64; apart *= 2) {
-    const int before = __shfl_up(x, apart);
-    if (lane >= apart) x += before;
-  }
+__device__ __forceinline__ float over_wave_float(float x) {
+  for (int away = 1; away < 64; away *= 2) x += __shfl_xor(x, away);
   return x;
+}
+// The sum over a wave of numbers below 2^62.
+__device__ __forceinline__ int64_t over_wave_sum(int64_t x) {
+  int64_t sum = 0;
+#pragma unroll
+  for (int shift = 0; shift < 64; shift += 24)  // (64 of 24 bits fit 32)
+    sum += static_cast<int64_t>(__builtin_amdgcn_readlane(scan_wave(static_cast<int>(x >> shift & 0xffffff)), 63))
+           << shift;
+  return sum;
 }
 
 // Which head and which of its `total` portions a block works on; -1: none.  FEW: neighbouring blocks
@@ -161,8 +173,8 @@ __device__ __forceinline__ Found portion_of(const PagedArgs<T>& a, int tid, Port
   const auto portion_length = [&](int64_t all) {
     return static_cast<int>(max(static_cast<int64_t>(d.least), (all + d.target - 1) / d.target));
   };
-  const auto splits_of = [](const SlotWork& w, int length) {
-    return w.tiles > 0 ? (w.walk + length - 1) / length : 0;
+  const auto splits_of = [&](const SlotWork& w, int length) {
+    return w.tiles > 0 ? max(1, (w.walk + length * d.round / 8) / length) : 0;
   };
   const auto note_tasks = [&](int tasks) {
     if (block_number() == 0 && tid == 0 && d.task_count != nullptr) *d.task_count = tasks;
@@ -177,10 +189,10 @@ __device__ __forceinline__ Found portion_of(const PagedArgs<T>& a, int tid, Port
     }
     const int length = portion_length(over_wave_sum(static_cast<int64_t>(w.tiles) * w.walk));
     const int splits = splits_of(w, length), items = w.tiles * splits;
-    const int upto = scan_wave(items, lane), total = __shfl(upto, 63);
-    const int parts = scan_wave(splits > 1 ? items : 0, lane);
-    const int tasks = scan_wave(splits > 1 ? w.tiles : 0, lane);
-    note_tasks(__shfl(tasks, 63));
+    const int upto = scan_wave(items), total = __builtin_amdgcn_readlane(upto, 63);
+    const int parts = scan_wave(splits > 1 ? items : 0);
+    const int tasks = scan_wave(splits > 1 ? w.tiles : 0);
+    note_tasks(__builtin_amdgcn_readlane(tasks, 63));
     const int64_t item = portion_number<FEW>(total, a.kv_heads, &p->kv_head);
     if (item < 0) return Found::kNothing;
     const int slot = __popcll(__ballot(upto <= item));
@@ -194,8 +206,9 @@ __device__ __forceinline__ Found portion_of(const PagedArgs<T>& a, int tid, Port
                        of_slot(parts) - (cut ? all : 0), of_slot(tasks) - (cut ? p->work.tiles : 0));
     return Found::kRun;
   }
-  __shared__ int64_t sums[4];
-  __shared__ int ends[3][4];
+  constexpr int kAll = kThreads / 64;
+  __shared__ int64_t sums[kAll];
+  __shared__ int ends[3][kAll];
   __shared__ Portion found;
   const int per = (count + kThreads - 1) / kThreads;
   const int from = min(count, tid * per), to = min(count, from + per);
@@ -211,7 +224,9 @@ __device__ __forceinline__ Found portion_of(const PagedArgs<T>& a, int tid, Port
     note_tasks(0);
     return Found::kInvalid;
   }
-  const int length = portion_length(sums[0] + sums[1] + sums[2] + sums[3]);
+  all = 0;
+  for (int w = 0; w < kAll; ++w) all += sums[w];
+  const int length = portion_length(all);
   int mine[3] = {0, 0, 0};
   for (int s = from; s < to; ++s) {
     const SlotWork w = slot_work<ROWS, KEYS, FEW>(a, s, &bad);
@@ -223,7 +238,7 @@ __device__ __forceinline__ Found portion_of(const PagedArgs<T>& a, int tid, Port
   int before[3], total[3];
 #pragma unroll
   for (int i = 0; i < 3; ++i) {
-    const int upto = scan_wave(mine[i], lane);
+    const int upto = scan_wave(mine[i]);
     if (lane == 63) ends[i][wave] = upto;
     before[i] = upto - mine[i];
   }
@@ -231,7 +246,7 @@ __device__ __forceinline__ Found portion_of(const PagedArgs<T>& a, int tid, Port
 #pragma unroll
   for (int i = 0; i < 3; ++i) {
     total[i] = 0;
-    for (int w = 0; w < 4; ++w) {
+    for (int w = 0; w < kAll; ++w) {
       if (w == wave) before[i] += total[i];
       total[i] += ends[i][w];
     }
@@ -289,12 +304,12 @@ __device__ __forceinline__ int position_of(const PagedArgs<T>& a, int token, int
   return past_of(a, slot, max(0, min(fresh, q.tokens))) + max(0, token - begin);
 }
 
-template <typename T>
+template <int THREADS = kThreads, typename T>
 __device__ __forceinline__ bool offsets_valid(const PagedArgs<T>& a, int tid) {
   const Sequences& q = a.sequences;
   if (q.offsets == nullptr) return true;
   int bad = 0;
-  for (int s = tid; s < q.count; s += kThreads) {
+  for (int s = tid; s < q.count; s += THREADS) {
     const int begin = q.offsets[s], end = q.offsets[s + 1];
     bad |= begin > end || (s == 0 && begin != 0) || (s == q.count - 1 && end != q.tokens);
   }
@@ -384,18 +399,46 @@ __global__ __launch_bounds__(kThreads) void paged_append_kernel(PagedArgs<T> a) 
   }
 }
 
+// The tokens whose first row is among [row0, row0 + rows) of a slot, on their rows.  (What a call reads
+// of the pages are earlier tokens: no other block waits for these.)
+template <bool WHOLE, typename T>
+__device__ __forceinline__ void put_tokens(const PagedArgs<T>& a, const T* keys, const T* values, int64_t first,
+                                           int kv_head, int row0, int rows, int tid) {
+  constexpr int kElements = 16 / static_cast<int>(sizeof(T));
+  typedef T Piece __attribute__((ext_vector_type(kElements)));
+  const int begin = (row0 + a.share - 1) / a.share, end = (row0 + rows + a.share - 1) / a.share;
+  const int key_pieces = (a.key_width + kElements - 1) / kElements;
+  const int pieces = key_pieces + (a.value_width + kElements - 1) / kElements;
+  for (int e = tid; e < (end - begin) * pieces; e += kThreads) {
+    const int token = begin + e / pieces, piece = e % pieces;
+    const int64_t row = a.row_of(first + token);
+    if (row < 0) continue;
+    const bool is_key = piece < key_pieces;
+    const int width = is_key ? a.key_width : a.value_width;
+    const int col = (is_key ? piece : piece - key_pieces) * kElements;
+    T* to = (is_key ? a.key_pages : a.value_pages) + col +
+            a.place(static_cast<int>(row >> a.page_shift), kv_head,
+                    static_cast<int>(row & ((1 << a.page_shift) - 1))) * width;
+    const T* from = is_key ? keys + token * a.key.token_stride : values + token * a.value.token_stride;
+    if constexpr (WHOLE)
+      *reinterpret_cast<Piece*>(to) = *reinterpret_cast<const Piece*>(from + col);
+    else
+      for (int i = 0; i < kElements && col + i < width; ++i) to[i] = from[col + i];
+  }
+}
+
 // ---------------------------------------------------------------------------
 // few rows
 // ---------------------------------------------------------------------------
 
-// A tile of 16 QUERIES rows of a slot and head of keys over a portion of its keys, in tiles of 32 that
+// A tile of 16 rows of a slot and head of keys over a portion of its keys, in tiles of 32 that
 // the waves take in turn; every wave has a softmax of its own, and the waves are joined at the end.
 // Keys go from memory to the operands of the products, values through LDS, which transposes them.
 // With `lists` the keys are those of the pages in a token's list, one behind the other.
-template <typename T, int WIDTH, int QUERIES, bool WHOLE>
+template <typename T, int WIDTH, bool WHOLE>
 __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(kWaves<T, WIDTH, WHOLE>))) void
 paged_token_kernel(PagedArgs<T> a) {
-  constexpr int kSteps = WIDTH / 32, kCols = WIDTH / 16, kTile = 32, kRows = 16 * QUERIES;
+  constexpr int kSteps = WIDTH / 32, kCols = WIDTH / 16, kTile = 32, kRows = 16;
   constexpr int kElements = 16 / static_cast<int>(sizeof(T)), kPerRow = WIDTH / kElements;
   constexpr int kPieces = kTile * kPerRow / 64, kPieceRows = 64 / kPerRow;
   constexpr int kOuts = WIDTH + 4;
@@ -464,21 +507,18 @@ paged_token_kernel(PagedArgs<T> a) {
   const T* fresh_value = a.value.row(batch, begin, kv_head);
   // (in lists every key is on a page: no token sees one behind its own)
   const int fresh_from = single ? 0x7fffffff : past;
-  if (a.fused && split == 0 && row0 == 0) {
-    const int64_t row = a.row_of(first);
-    if (row >= 0) {
-      const int id = static_cast<int>(row >> a.page_shift);
-      const int64_t to = a.place(id, kv_head, static_cast<int>(row & ((1 << a.page_shift) - 1)));
-      for (int d = tid; d < a.key_width; d += kThreads) a.key_pages[to * a.key_width + d] = fresh_key[d];
-      for (int d = tid; d < a.value_width; d += kThreads) a.value_pages[to * a.value_width + d] = fresh_value[d];
-      if (a.key_bounds != nullptr) {
-        T* bounds = a.key_bounds + (static_cast<int64_t>(id) * a.kv_heads + kv_head) * 2 * a.key_width;
+  if (a.fused && split == 0) {
+    put_tokens<WHOLE>(a, fresh_key, fresh_value, first, kv_head, row0, rows, tid);
+    if (a.key_bounds != nullptr && row0 == 0) {  // (of single tokens)
+      const int64_t row = a.row_of(first);
+      if (row >= 0) {
+        T* low = a.key_bounds + ((row >> a.page_shift) * a.kv_heads + kv_head) * 2 * a.key_width;
+        T* high = low + a.key_width;
         const bool alone = (past & ((1 << a.page_shift) - 1)) == 0;
         for (int d = tid; d < a.key_width; d += kThreads) {
           const float x = static_cast<float>(fresh_key[d]);
-          bounds[d] = static_cast<T>(alone ? x : lower_of(x, static_cast<float>(bounds[d])));
-          T* high = bounds + a.key_width + d;
-          *high = static_cast<T>(alone ? x : higher_of(x, static_cast<float>(*high)));
+          low[d] = static_cast<T>(alone ? x : lower_of(x, static_cast<float>(low[d])));
+          high[d] = static_cast<T>(alone ? x : higher_of(x, static_cast<float>(high[d])));
         }
       }
     }
@@ -490,29 +530,21 @@ paged_token_kernel(PagedArgs<T> a) {
   const int first_limit = single ? last : past + row0 / a.share;
 
   // this wave's rows, as the columns of operands (the last one again beyond it)
-  Operand<T> query[QUERIES][kSteps];
-  int limit[QUERIES];
+  Operand<T> query[kSteps];
+  const int my_row = row0 + min(column, rows - 1), my_token = my_row / a.share;
+  const int limit = single ? last : past + my_token;
+  const Rows<T> query_row = {
+      a.query.row(batch, begin + my_token, kv_head * a.share + my_row - my_token * a.share), 0, 0};
 #pragma unroll
-  for (int i = 0; i < QUERIES; ++i) {
-    const int row = row0 + min(i * 16 + column, rows - 1), token = row / a.share;
-    limit[i] = single ? last : past + token;
-    const Rows<T> query_row = {a.query.row(batch, begin + token, kv_head * a.share + row - token * a.share), 0, 0};
-#pragma unroll
-    for (int s = 0; s < kSteps; ++s) {
-      Frag<T> part_of_row = memory_operand<WHOLE>(query_row, 0, s * 32 + 8 * group, a.key_width);
-      clear_operand<WHOLE>(part_of_row, s * 32, group, a.key_width);
-      query[i][s] = as_operand<T>(part_of_row);
-    }
+  for (int s = 0; s < kSteps; ++s) {
+    Frag<T> part_of_row = memory_operand<WHOLE>(query_row, 0, s * 32 + 8 * group, a.key_width);
+    clear_operand<WHOLE>(part_of_row, s * 32, group, a.key_width);
+    query[s] = as_operand<T>(part_of_row);
   }
-  f32x4 out[QUERIES][kCols];
-  float most[QUERIES], sum[QUERIES];
+  f32x4 out[kCols];
 #pragma unroll
-  for (int i = 0; i < QUERIES; ++i) {
-    most[i] = -__builtin_inff();
-    sum[i] = 0.0f;
-#pragma unroll
-    for (int d = 0; d < kCols; ++d) out[i][d] = f32x4(0.0f);
-  }
+  for (int d = 0; d < kCols; ++d) out[d] = f32x4(0.0f);
+  float most = -__builtin_inff(), sum = 0.0f;
   const float factor = a.scale * kLog2e;
 
   Frag<T> key[2][kSteps];
@@ -539,15 +571,34 @@ paged_token_kernel(PagedArgs<T> a) {
       values[h] = a.value_pages + row * a.value_width;
       rows_left[h] = min(15, last - at);
     }
-    // new tokens are taken from the inputs, whether they have a row or not
-    const bool ends = tile * kTile + kTile > fresh_from;
-    const auto source_of = [&](const T* row_zero, int h, int row, int width, const T* fresh, int64_t stride) {
-      const T* from = row_zero + row * width;
-      if (ends) {
-        const int token = half_begin(tile, h) + row - fresh_from;
-        if (token >= 0) from = fresh + token * stride;
+    if (tile * kTile + kTile <= fresh_from) {
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const Rows<T> source = {keys[h], a.key_width, rows_left[h]};
+#pragma unroll
+        for (int s = 0; s < kSteps; ++s)
+          key[h][s] = memory_operand<WHOLE>(source, column, s * 32 + 8 * group, a.key_width);
       }
-      return from;
+#pragma unroll
+      for (int i = 0; i < kPieces; ++i) {
+        const int h = i * kPieceRows / 16, row = i * kPieceRows - 16 * h + lane / kPerRow;
+        const int col = lane % kPerRow * kElements;
+        const Rows<T> source = {values[h], a.value_width, rows_left[h]};
+        if constexpr (WHOLE) {
+          held[i] = *reinterpret_cast<const Piece*>(
+              place_of<WHOLE>(source, min(row, source.last), min(col, a.value_width - kElements)));
+        } else {
+          const T* from = place_of<WHOLE>(source, min(row, source.last), 0);
+#pragma unroll
+          for (int e = 0; e < kElements; ++e) held[i][e] = from[min(col + e, a.value_width - 1)];
+        }
+      }
+      return bad;
+    }
+    // new tokens are taken from the inputs, whether they have a row or not
+    const auto source_of = [&](const T* row_zero, int h, int row, int width, const T* fresh, int64_t stride) {
+      const int token = half_begin(tile, h) + row - fresh_from;
+      return token >= 0 ? fresh + token * stride : row_zero + row * width;
     };
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
@@ -579,17 +630,14 @@ paged_token_kernel(PagedArgs<T> a) {
     look_up(tile + 4, id);
   }
   for (; tile < tile_end; tile += 4) {
-    f32x4 score[QUERIES][2];
+    f32x4 score[2];
 #pragma unroll
     for (int k = 0; k < 2; ++k) {
-#pragma unroll
-      for (int i = 0; i < QUERIES; ++i) score[i][k] = f32x4(0.0f);
+      score[k] = f32x4(0.0f);
 #pragma unroll
       for (int s = 0; s < kSteps; ++s) {
         clear_operand<WHOLE>(key[k][s], s * 32, group, a.key_width);
-        const Operand<T> operand = as_operand<T>(key[k][s]);
-#pragma unroll
-        for (int i = 0; i < QUERIES; ++i) score[i][k] = mma(operand, query[i][s], score[i][k]);
+        score[k] = mma(as_operand<T>(key[k][s]), query[s], score[k]);
       }
     }
     const int missing = bad;
@@ -615,68 +663,56 @@ paged_token_kernel(PagedArgs<T> a) {
     if (missing != 0) {
 #pragma unroll
       for (int k = 0; k < 2; ++k)
-        if (missing >> k & 1)
-#pragma unroll
-          for (int i = 0; i < QUERIES; ++i) score[i][k] = f32x4(__builtin_nanf(""));
+        if (missing >> k & 1) score[k] = f32x4(__builtin_nanf(""));
     }
-    Operand<T> weights[QUERIES];
-#pragma unroll
-    for (int i = 0; i < QUERIES; ++i) {
-      if (tile * kTile + kTile - 1 > first_limit) {
-#pragma unroll
-        for (int k = 0; k < 2; ++k)
-#pragma unroll
-          for (int r = 0; r < 4; ++r)
-            if (tile * kTile + k * 16 + 4 * group + r > min(limit[i], last)) score[i][k][r] = -__builtin_inff();
-      }
-      float here = -__builtin_inff();
+    if (tile * kTile + kTile - 1 > first_limit) {
 #pragma unroll
       for (int k = 0; k < 2; ++k)
 #pragma unroll
-        for (int r = 0; r < 4; ++r) here = fmaxf(here, score[i][k][r]);
-      here = over_groups_max(here) * factor;
-      if (__any(here > most[i])) {
-        const float larger = fmaxf(here, most[i]);
-        const float shrink = larger == -__builtin_inff() ? 1.0f : exp2_of(most[i] - larger);
-        sum[i] *= shrink;
+        for (int r = 0; r < 4; ++r)
+          if (tile * kTile + k * 16 + 4 * group + r > min(limit, last)) score[k][r] = -__builtin_inff();
+    }
+    float here = -__builtin_inff();
 #pragma unroll
-        for (int d = 0; d < kCols; ++d) out[i][d] *= shrink;
-        most[i] = larger;
+    for (int k = 0; k < 2; ++k)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) here = fmaxf(here, score[k][r]);
+    here = over_groups_max(here) * factor;
+    if (__any(here > most)) {
+      const float larger = fmaxf(here, most);
+      const float shrink = larger == -__builtin_inff() ? 1.0f : exp2_of(most - larger);
+      sum *= shrink;
+#pragma unroll
+      for (int d = 0; d < kCols; ++d) out[d] *= shrink;
+      most = larger;
+    }
+    const float base = (most == -__builtin_inff() ? 0.0f : most) - kLift<T>;
+#pragma unroll
+    for (int k = 0; k < 2; ++k)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        score[k][r] = exp2_of(score[k][r] * factor - base);
+        sum += score[k][r];
       }
-      const float base = (most[i] == -__builtin_inff() ? 0.0f : most[i]) - kLift<T>;
+    const Operand<T> weights = operand_of<T>(score[0], score[1]);
 #pragma unroll
-      for (int k = 0; k < 2; ++k)
-#pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          score[i][k][r] = exp2_of(score[i][k][r] * factor - base);
-          sum[i] += score[i][k][r];
-        }
-      weights[i] = operand_of<T>(score[i][0], score[i][1]);
-    }
-#pragma unroll
-    for (int d = 0; d < kCols; ++d) {
-      const Operand<T> value = column_operand<T, kTile, WIDTH>(tile_values, 0, d * 16, lane);
-#pragma unroll
-      for (int i = 0; i < QUERIES; ++i) out[i][d] = mma(value, weights[i], out[i][d]);
-    }
+    for (int d = 0; d < kCols; ++d)
+      out[d] = mma(column_operand<T, kTile, WIDTH>(tile_values, 0, d * 16, lane), weights, out[d]);
     asm volatile("" ::: "memory");
   }
 
   // the waves of the block
   __syncthreads();
   float* outs = reinterpret_cast<float*>(shared) + wave * kRows * kOuts;
+  sum = over_groups_sum(sum);
 #pragma unroll
-  for (int i = 0; i < QUERIES; ++i) {
-    const float total = over_groups_sum(sum[i]);
-#pragma unroll
-    for (int d = 0; d < kCols; ++d)
-      *reinterpret_cast<f32x4*>(outs + (i * 16 + column) * kOuts + d * 16 + 4 * group) = out[i][d];
-    if (group == 0) {
-      // tokens behind the table have a key that is on no page
-      const bool lost = void_rows || (!single && limit[i] >= a.capacity());
-      tops[wave][i * 16 + column] = most[i];
-      totals[wave][i * 16 + column] = lost ? __builtin_nanf("") : total;
-    }
+  for (int d = 0; d < kCols; ++d)
+    *reinterpret_cast<f32x4*>(outs + column * kOuts + d * 16 + 4 * group) = out[d];
+  if (group == 0) {
+    // tokens behind the table have a key that is on no page
+    const bool lost = void_rows || (!single && limit >= a.capacity());
+    tops[wave][column] = most;
+    totals[wave][column] = lost ? __builtin_nanf("") : sum;
   }
   __syncthreads();
   float* partial = a.division.partial + (static_cast<int64_t>(kv_head) * a.division.parts + part) * kRows * kOuts;
@@ -710,14 +746,15 @@ paged_token_kernel(PagedArgs<T> a) {
 // ---------------------------------------------------------------------------
 
 // 64 QUERIES rows of a slot and head of keys, 16 QUERIES to a wave, over a portion of its keys in tiles
-// of 64: keys and values go through registers to LDS while the tile before is worked on, queries and
-// sums stay in registers.  Weights are rounded to the inputs' type, as the operand of the product with
-// the values, and summed as rounded.
-template <typename T, int WIDTH, int QUERIES, bool WHOLE>
+// of 64, which go through registers to LDS while the tile before is worked on; queries and sums stay in
+// registers.  USED: the columns that keys and values have at most (tiles have WIDTH).  Weights are
+// rounded to the inputs' type, as the operand of the product with the values, and summed as rounded.
+template <typename T, int WIDTH, int USED, int QUERIES, bool WHOLE>
 __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(kWaves<T, WIDTH, WHOLE>))) void
 paged_chunk_kernel(PagedArgs<T> a) {
-  constexpr int kSteps = WIDTH / 32, kRows = 64 * QUERIES, kCols = WIDTH / 16;
+  constexpr int kSteps = USED / 32, kRows = 64 * QUERIES, kCols = USED / 16;
   constexpr int kTile = kTileElements<T, kKeys, WIDTH>;
+  using Move = TileMove<T, kKeys, WIDTH, WHOLE>;
   __shared__ __attribute__((aligned(16))) Stored<T> key_tiles[kBuffers<T> * kTile];
   __shared__ __attribute__((aligned(16))) Stored<T> value_tiles[kBuffers<T> * kTile];
 
@@ -749,7 +786,8 @@ paged_chunk_kernel(PagedArgs<T> a) {
   // this wave's rows, as the columns of operands (the last one again beyond it)
   const int wave_row = row0 + wave * 16 * QUERIES;
   const int wave_first = past + min(wave_row, row0 + rows - 1) / a.share;
-  const int wave_last = past + min(wave_row + 16 * QUERIES, row0 + rows) / a.share;  // or one before
+  // no row of the wave sees a key from here on
+  const int wave_end = wave_row < row0 + rows ? past + (min(wave_row + 16 * QUERIES, row0 + rows) - 1) / a.share + 1 : 0;
   Operand<T> query[QUERIES][kSteps];
   int limit[QUERIES];
 #pragma unroll
@@ -779,73 +817,94 @@ paged_chunk_kernel(PagedArgs<T> a) {
 
   // A quarter of a tile lies on one page, whose number a lane of the wave's first four holds.
   // Quarters and rows behind the last key are the last one's again.
-  TileMove<T, kKeys, WIDTH, WHOLE> key_move, value_move;
+  Move key_move, value_move;
   const Rows<T> fresh_keys = a.key.rows(batch, begin_token, kv_head, p.work.fresh);
   const Rows<T> fresh_values = a.value.rows(batch, begin_token, kv_head, p.work.fresh);
+  const int page_mask = (1 << a.page_shift) - 1;
   const auto look_up = [&](int tile) {
     return table[min(tile * kKeys + 16 * (lane & 3), last & ~15) >> a.page_shift];
   };
   const auto missing_of = [&](int ids) {
     return static_cast<int>(__ballot(lane < 4 && !a.is_page(ids)));
   };
-  const auto fetch = [&](int tile, int ids) {
+  const auto fetch = [&](Move& move, const T* pages, int width, const Rows<T>& fresh, int tile, int ids) {
     const int begin = tile * kKeys, left = min(kKeys - 1, last - begin);
     ids = a.is_page(ids) ? ids : 0;
-    const auto row_at = [&](int row) {
-      row = min(row, left);
-      const int quarter = __builtin_amdgcn_readfirstlane(row >> 4);
-      const int id = __builtin_amdgcn_readlane(ids, quarter);
-      return a.place(id, kv_head, (begin + 16 * quarter) & ((1 << a.page_shift) - 1)) + (row & 15);
-    };
-    if (begin >= past) {  // new tokens are taken from the inputs, whether they have a row or not
-      key_move.fetch(rows_from(fresh_keys, begin - past, left + 1), a.key_width, tid);
-      value_move.fetch(rows_from(fresh_values, begin - past, left + 1), a.value_width, tid);
-    } else if (begin + left < past) {
-      key_move.fetch_from([&](int row, int col) { return a.key_pages + row_at(row) * a.key_width + col; },
-                          a.key_width, tid);
-      value_move.fetch_from([&](int row, int col) { return a.value_pages + row_at(row) * a.value_width + col; },
-                            a.value_width, tid);
-    } else {
-      const auto from = [&](const T* pages, int width, const Rows<T>& fresh, int row, int col) {
-        const T* held = pages + row_at(row) * width;
-        const int token = begin + min(row, left) - past;
-        return (token >= 0 ? fresh.base + token * fresh.stride : held) + col;
-      };
-      key_move.fetch_from([&](int row, int col) { return from(a.key_pages, a.key_width, fresh_keys, row, col); },
-                          a.key_width, tid);
-      value_move.fetch_from(
-          [&](int row, int col) { return from(a.value_pages, a.value_width, fresh_values, row, col); },
-          a.value_width, tid);
+    // new tokens are taken from the inputs, whether they have a row or not
+    const bool fresh_only = begin >= past, one_page = begin + left < past && a.page_shift >= 6;
+    if (fresh_only || one_page) {
+      const Rows<T> held = {pages + a.place(__builtin_amdgcn_readlane(ids, 0), kv_head, begin & page_mask) * width,
+                            width, left};
+      move.fetch(fresh_only ? rows_from(fresh, begin - past, left + 1) : held, width, tid);
+      return;
     }
+    if (WHOLE && begin + kKeys <= past && left == kKeys - 1) {
+      // (a base that the wave shares and an offset of 32 bits)
+      const uint32_t col = min(Move::col_of(tid), width - Move::kElements);
+#pragma unroll
+      for (int i = 0; i < Move::kPieces; ++i) {
+        const int quarter = (i * (kThreads / Move::kPerRow) + wave * (64 / Move::kPerRow)) >> 4;
+        const int id = __builtin_amdgcn_readlane(ids, quarter);
+        const T* base = pages + a.place(id, kv_head, (begin + 16 * quarter) & page_mask) * width;
+        const uint32_t offset = ((Move::row_of(i, tid) & 15) * static_cast<uint32_t>(width) + col) *
+                                static_cast<uint32_t>(sizeof(T));
+        move.held[i] = *reinterpret_cast<const typename Move::Piece*>(reinterpret_cast<const char*>(base) + offset);
+      }
+      return;
+    }
+    move.fetch_from(
+        [&](int row, int col) {
+          row = min(row, left);
+          const int quarter = __builtin_amdgcn_readfirstlane(row >> 4);
+          const int id = __builtin_amdgcn_readlane(ids, quarter);
+          const T* held = pages + (a.place(id, kv_head, (begin + 16 * quarter) & page_mask) + (row & 15)) * width;
+          const int token = begin + row - past;
+          return (token >= 0 ? fresh.base + token * fresh.stride : held) + col;
+        },
+        width, tid);
   };
+  const auto fetch_keys = [&](int tile, int ids) {
+    fetch(key_move, a.key_pages, a.key_width, fresh_keys, tile, ids);
+  };
+  const auto fetch_values = [&](int tile, int ids) {
+    fetch(value_move, a.value_pages, a.value_width, fresh_values, tile, ids);
+  };
+  // what is on no page makes NaN of the rows that see it, and nothing of others
+  const auto clear_missing = [&](int missing) {
+    if (missing == 0) return;
+#pragma unroll
+    for (int i = 0; i < Move::kPieces; ++i)
+      if (missing >> (Move::row_of(i, tid) >> 4) & 1)
+        value_move.held[i] = typename Move::Piece(static_cast<T>(0.0f));
+  };
+
   const int tiles = last / kKeys + 1, share = (tiles + p.splits - 1) / p.splits;
   const int tile_end = min(tiles, (p.split + 1) * share);
   int tile = p.split * share;
-  int ids = 0, next_missing = 0;
+  int ids = 0, missing = 0;  // (looked up a tile before their pages are)
   if (tile < tile_end) {
     ids = look_up(tile);
-    next_missing = missing_of(ids);
-    fetch(tile, ids);
+    missing = missing_of(ids);
+    fetch_keys(tile, ids);
+    fetch_values(tile, ids);
     ids = look_up(tile + 1);
   }
+  if (a.fused && p.split == 0)
+    put_tokens<WHOLE>(a, fresh_keys.base, fresh_values.base, first_token, kv_head, row0, rows, tid);
   for (int side = 0; tile < tile_end; ++tile, side = kBuffers<T> - 1 - side) {
-    const int begin = tile * kKeys, missing = next_missing;
+    const int begin = tile * kKeys, here_missing = missing;
     Stored<T>*keys = key_tiles + side * kTile, *values = value_tiles + side * kTile;
-    if (missing != 0) {  // what is on no page makes NaN of the rows that see it, and nothing of others
-#pragma unroll
-      for (int i = 0; i < value_move.kPieces; ++i)
-        if (missing >> (value_move.row_of(i, tid) >> 4) & 1)
-          value_move.held[i] = typename TileMove<T, kKeys, WIDTH, WHOLE>::Piece(static_cast<T>(0.0f));
-    }
+    clear_missing(missing);
     key_move.store(keys, a.key_width, tid);
     value_move.store(values, a.value_width, tid);
     __syncthreads();
     if (tile + 1 < tile_end) {
-      next_missing = missing_of(ids);
-      fetch(tile + 1, ids);
+      missing = missing_of(ids);
+      fetch_keys(tile + 1, ids);
+      fetch_values(tile + 1, ids);
       ids = look_up(tile + 2);
     }
-    if (begin <= wave_last && wave_row < row0 + rows) {
+    if (begin < wave_end) {
       f32x4 score[QUERIES][4];
 #pragma unroll
       for (int k = 0; k < 4; ++k) {
@@ -858,10 +917,20 @@ paged_chunk_kernel(PagedArgs<T> a) {
           for (int i = 0; i < QUERIES; ++i) score[i][k] = mma(key, query[i][s], score[i][k]);
         }
       }
-      if (missing != 0) {
+      if constexpr (sizeof(T) == 2) {
+        // operands are read from LDS some products ahead of their own
+        __builtin_amdgcn_sched_group_barrier(0x100, 6, 0);
+#pragma unroll
+        for (int j = 0; j < 4 * kSteps - 6; ++j) {
+          __builtin_amdgcn_sched_group_barrier(0x008, QUERIES, 0);
+          __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+        }
+        __builtin_amdgcn_sched_group_barrier(0x008, 6 * QUERIES, 0);
+      }
+      if (here_missing != 0) {
 #pragma unroll
         for (int k = 0; k < 4; ++k)
-          if (missing >> k & 1)
+          if (here_missing >> k & 1)
 #pragma unroll
             for (int i = 0; i < QUERIES; ++i) score[i][k] = f32x4(__builtin_nanf(""));
       }
@@ -912,6 +981,15 @@ paged_chunk_kernel(PagedArgs<T> a) {
 #pragma unroll
           for (int i = 0; i < QUERIES; ++i) out[i][d] = mma(value, weights[i][half], out[i][d]);
         }
+      if constexpr (sizeof(T) == 2) {
+        __builtin_amdgcn_sched_group_barrier(0x100, 8, 1);
+#pragma unroll
+        for (int j = 0; j < 2 * kCols - 4; ++j) {
+          __builtin_amdgcn_sched_group_barrier(0x008, QUERIES, 1);
+          __builtin_amdgcn_sched_group_barrier(0x100, 2, 1);
+        }
+        __builtin_amdgcn_sched_group_barrier(0x008, 6 * QUERIES, 1);
+      }
     }
     if constexpr (kBuffers<T> == 1) __syncthreads();
   }
@@ -944,71 +1022,106 @@ paged_chunk_kernel(PagedArgs<T> a) {
 // tiles that were cut
 // ---------------------------------------------------------------------------
 
-// The parts of a row.  BLOCK: a block has a row, whose parts its waves add up in turn, as of few rows
-// there are many; otherwise a wave has it.
-template <typename T, int WIDTH, bool BLOCK>
-__global__ __launch_bounds__(kThreads) void paged_join_kernel(PagedArgs<T> a, int tile_rows) {
-  constexpr int kOuts = WIDTH + 4;
-  __shared__ float weights[BLOCK ? kMostPortions : 1], sums[kThreads], tops[4], totals[4];
+// The parts of the first `unit_rows` rows of every tile.  Of few rows there may be many parts: a block
+// has a row, and its threads four columns of some parts each.
+template <typename T, int WIDTH>
+__global__ __launch_bounds__(kThreads) void paged_join_few_kernel(PagedArgs<T> a, int tile_rows, int unit_rows) {
+  constexpr int kOuts = WIDTH + 4, kLanes = WIDTH / 4, kTeams = kThreads / kLanes;
+  __shared__ __attribute__((aligned(16))) float sums[kTeams][WIDTH];
+  __shared__ float weights[kMostPortions], tops[4], totals[4];
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  const int64_t units = static_cast<int64_t>(*a.division.task_count) * a.kv_heads * tile_rows;
+  const int col = tid % kLanes * 4, team = tid / kLanes;
+  const int64_t units = static_cast<int64_t>(*a.division.task_count) * a.kv_heads * unit_rows;
   const int64_t apart = static_cast<int64_t>(tile_rows) * kOuts;
-  for (int64_t unit = BLOCK ? blockIdx.x : static_cast<int64_t>(blockIdx.x) * 4 + wave; unit < units;
-       unit += BLOCK ? gridDim.x : static_cast<int64_t>(gridDim.x) * 4) {
-    const PagedTask task = a.division.tasks[unit / tile_rows / a.kv_heads];
-    const int kv_head = static_cast<int>(unit / tile_rows % a.kv_heads), r = static_cast<int>(unit % tile_rows);
+  for (int64_t unit = blockIdx.x; unit < units; unit += gridDim.x) {
+    const PagedTask task = a.division.tasks[unit / unit_rows / a.kv_heads];
+    const int kv_head = static_cast<int>(unit / unit_rows % a.kv_heads), r = static_cast<int>(unit % unit_rows);
     if (r >= task.rows) continue;
     const float* parts = a.division.partial +
                          ((static_cast<int64_t>(kv_head) * a.division.parts + task.part) * tile_rows + r) * kOuts;
+    float top = -__builtin_inff(), total = 0.0f;
+    for (int s = tid; s < task.splits; s += kThreads) {
+      weights[s] = parts[s * apart + WIDTH];
+      top = fmaxf(top, weights[s]);
+    }
+    for (int away = 1; away < 64; away *= 2) top = fmaxf(top, __shfl_xor(top, away));
+    if (lane == 0) tops[wave] = top;
+    __syncthreads();
+    top = fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3]));
+    for (int s = tid; s < task.splits; s += kThreads) {
+      const float by = top == -__builtin_inff() ? 1.0f : exp2_of(weights[s] - top);
+      weights[s] = by;
+      total += by * parts[s * apart + WIDTH + 1];
+    }
+    total = over_wave_float(total);
+    if (lane == 0) totals[wave] = total;
+    __syncthreads();
+    f32x4 value = f32x4(0.0f);
+#pragma unroll 4
+    for (int s = team; s < task.splits; s += kTeams)
+      value += weights[s] * *reinterpret_cast<const f32x4*>(parts + s * apart + col);
+    *reinterpret_cast<f32x4*>(&sums[team][col]) = value;
+    __syncthreads();
+    if (tid < a.value_width) {
+      const int teams = min(kTeams, task.splits);
+      float all = sums[0][tid];
+      for (int t = 1; t < teams; ++t) all += sums[t][tid];
+      const int row = task.row + r, token = row / a.share;
+      const int64_t at = (task.first + token) * a.heads + kv_head * a.share + row - token * a.share;
+      a.out[at * a.value_width + tid] =
+          static_cast<T>(all / (totals[0] + totals[1] + totals[2] + totals[3]));
+    }
+    __syncthreads();
+  }
+}
+
+// Of many rows there are few parts each: a thread has four columns of a row, and takes four parts at
+// once, so that their loads are under way together.
+template <typename T, int WIDTH>
+__global__ __launch_bounds__(kThreads) void paged_join_many_kernel(PagedArgs<T> a, int tile_rows) {
+  constexpr int kOuts = WIDTH + 4, kAtOnce = 4, kLanes = WIDTH / 4, kTeams = kThreads / kLanes;
+  const int col = threadIdx.x % kLanes * 4, team = threadIdx.x / kLanes;
+  const int64_t units = static_cast<int64_t>(*a.division.task_count) * a.kv_heads * tile_rows;
+  const int64_t apart = static_cast<int64_t>(tile_rows) * kOuts;
+  for (int64_t unit = static_cast<int64_t>(blockIdx.x) * kTeams + team; unit < units;
+       unit += static_cast<int64_t>(gridDim.x) * kTeams) {
+    const int64_t tile = unit / tile_rows;
+    const PagedTask task = a.division.tasks[tile / a.kv_heads];
+    const int kv_head = static_cast<int>(tile % a.kv_heads), r = static_cast<int>(unit % tile_rows);
+    if (r >= task.rows) continue;
+    const float* parts = a.division.partial +
+                         ((static_cast<int64_t>(kv_head) * a.division.parts + task.part) * tile_rows + r) * kOuts;
+    float top = -__builtin_inff(), total = 0.0f;
+    f32x4 value = f32x4(0.0f);
+    for (int first = 0; first < task.splits; first += kAtOnce) {
+      float tops[kAtOnce], totals[kAtOnce];
+      f32x4 values[kAtOnce];
+#pragma unroll
+      for (int s = 0; s < kAtOnce; ++s) {
+        const float* part = parts + min(first + s, task.splits - 1) * apart;
+        tops[s] = part[WIDTH];
+        totals[s] = part[WIDTH + 1];
+        values[s] = *reinterpret_cast<const f32x4*>(part + col);
+      }
+      float larger = top;
+#pragma unroll
+      for (int s = 0; s < kAtOnce; ++s) larger = fmaxf(larger, tops[s]);
+      const float base = larger == -__builtin_inff() ? 0.0f : larger, shrink = exp2_of(top - base);
+      top = larger;
+      total *= shrink;
+      value *= shrink;
+#pragma unroll
+      for (int s = 0; s < kAtOnce; ++s)
+        if (first + s < task.splits) {
+          const float by = exp2_of(tops[s] - base);
+          total += by * totals[s];
+          value += by * values[s];
+        }
+    }
     const int row = task.row + r, token = row / a.share;
     T* out = a.out + ((task.first + token) * a.heads + kv_head * a.share + row - token * a.share) * a.value_width;
-    float top = -__builtin_inff(), total = 0.0f;
-    if constexpr (BLOCK) {
-      for (int s = tid; s < task.splits; s += kThreads) {
-        weights[s] = parts[s * apart + WIDTH];
-        top = fmaxf(top, weights[s]);
-      }
-      for (int away = 1; away < 64; away *= 2) top = fmaxf(top, __shfl_xor(top, away));
-      if (lane == 0) tops[wave] = top;
-      __syncthreads();
-      top = fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3]));
-      for (int s = tid; s < task.splits; s += kThreads) {
-        const float by = top == -__builtin_inff() ? 1.0f : exp2_of(weights[s] - top);
-        weights[s] = by;
-        total += by * parts[s * apart + WIDTH + 1];
-      }
-      for (int away = 1; away < 64; away *= 2) total += __shfl_xor(total, away);
-      if (lane == 0) totals[wave] = total;
-      __syncthreads();
-      total = totals[0] + totals[1] + totals[2] + totals[3];
-      for (int col0 = 0; col0 < a.value_width; col0 += 64) {
-        const int col = col0 + lane;
-        float value = 0.0f;
-        if (col < a.value_width) {
-#pragma unroll 8
-          for (int s = wave; s < task.splits; s += 4) value += weights[s] * parts[s * apart + col];
-        }
-        sums[tid] = value;
-        __syncthreads();
-        if (wave == 0 && col < a.value_width)
-          out[col] = static_cast<T>((sums[lane] + sums[64 + lane] + sums[128 + lane] + sums[192 + lane]) / total);
-        __syncthreads();
-      }
-    } else {
-      for (int s = 0; s < task.splits; ++s) top = fmaxf(top, parts[s * apart + WIDTH]);
-      float value[2] = {0.0f, 0.0f};
-      for (int s = 0; s < task.splits; ++s) {
-        const float* part = parts + s * apart;
-        const float by = top == -__builtin_inff() ? 1.0f : exp2_of(part[WIDTH] - top);
-        total += by * part[WIDTH + 1];
-#pragma unroll
-        for (int c = 0; c < 2; ++c)
-          if (c * 64 < WIDTH) value[c] += by * part[min(c * 64 + lane, WIDTH - 1)];
-      }
-#pragma unroll
-      for (int c = 0; c < 2; ++c)
-        if (c * 64 + lane < a.value_width) out[c * 64 + lane] = static_cast<T>(value[c] / total);
-    }
+    store4(out, col, value * (1.0f / total), a.value_width,
+           a.value_width % 4 == 0 && reinterpret_cast<uintptr_t>(out) % sizeof(Quad<T>) == 0);
   }
 }
 
@@ -1016,18 +1129,57 @@ __global__ __launch_bounds__(kThreads) void paged_join_kernel(PagedArgs<T> a, in
 // selected pages
 // ---------------------------------------------------------------------------
 
+// A single new token and the bounds of its page, which no token of the call has to know.
+template <typename T>
+__device__ __forceinline__ void put_single(const PagedArgs<T>& a, int64_t token, int slot, int kv_head, int past,
+                                           int tid) {
+  const int64_t row = a.row_of(token);
+  if (row < 0) return;
+  const int id = static_cast<int>(row >> a.page_shift), mask = (1 << a.page_shift) - 1;
+  const int64_t to = a.place(id, kv_head, static_cast<int>(row & mask));
+  const T* key = a.key.row(slot, 0, kv_head);
+  const T* value = a.value.row(slot, 0, kv_head);
+  T* low = a.key_bounds + (static_cast<int64_t>(id) * a.kv_heads + kv_head) * 2 * a.key_width;
+  T* high = low + a.key_width;
+  for (int d = tid; d < a.key_width; d += kThreads) {
+    const float x = static_cast<float>(key[d]);
+    const bool alone = (past & mask) == 0;
+    a.key_pages[to * a.key_width + d] = key[d];
+    low[d] = static_cast<T>(alone ? x : lower_of(x, static_cast<float>(low[d])));
+    high[d] = static_cast<T>(alone ? x : higher_of(x, static_cast<float>(high[d])));
+  }
+  for (int d = tid; d < a.value_width; d += kThreads) a.value_pages[to * a.value_width + d] = value[d];
+}
+
+// x of the lane that a pattern within 16 lanes names
+template <int PATTERN>
+__device__ __forceinline__ double from_lane(double x) {
+  const uint64_t bits = __builtin_bit_cast(uint64_t, x);
+  const uint32_t low = __builtin_amdgcn_update_dpp(0, static_cast<int>(bits), PATTERN, 0xf, 0xf, true);
+  const uint32_t high = __builtin_amdgcn_update_dpp(0, static_cast<int>(bits >> 32), PATTERN, 0xf, 0xf, true);
+  return __builtin_bit_cast(double, static_cast<uint64_t>(high) << 32 | low);
+}
+// The sum over groups of LANES lanes, 16 or 32 of them: within two, four, eight (mirrored, so that a
+// lane meets one of the other four), sixteen, and the next sixteen.
+template <int LANES>
+__device__ __forceinline__ double over_lanes_sum(double x) {
+  x += from_lane<0xb1>(x);
+  x += from_lane<0x4e>(x);
+  x += from_lane<0x141>(x);
+  x += from_lane<0x140>(x);
+  if constexpr (LANES == 32) x += __shfl_xor(x, 16);
+  return x;
+}
+
 // The largest product that a key within a page's bounds can have with a query of the group, in 64 bits,
 // in which the products are exact: pages are ranked as their bounds rank, whatever the order of a sum.
-// A block has 64 pages of a token and head of keys at a time, a page to a lane and a quarter of the
-// columns to a wave.
+// A lane has the queries' elements of its columns in registers for all pages; the lanes of a page add up.
 template <typename T, bool WHOLE>
 __global__ __launch_bounds__(kThreads) void paged_score_kernel(PagedArgs<T> a, int blocks_of_token) {
   constexpr int kElements = 16 / static_cast<int>(sizeof(T)), kMembers = 4;
+  constexpr int kLanes = kMostWidth / kElements, kPages = kThreads / kLanes, kTurns = 4;  // of a page; at once
   typedef T Piece __attribute__((ext_vector_type(kElements)));
-  __shared__ __attribute__((aligned(16))) float queries[kMembers][kMostWidth];
-  __shared__ double sums[4][kMembers][64];
   const int tid = threadIdx.x, lane = tid & 63;
-  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const uint32_t block = block_number();
   const int64_t at = block / blocks_of_token;
   const int64_t number = at / a.kv_heads;
@@ -1035,66 +1187,84 @@ __global__ __launch_bounds__(kThreads) void paged_score_kernel(PagedArgs<T> a, i
   if (number >= a.slab_tokens) return;
   const int token = static_cast<int>(a.slab_first + number);
   const int slot = slot_of_token(a, token, lane);
-  const int earlier = min(position_of(a, token, slot) >> a.page_shift, a.columns);
-  if (earlier <= a.count) return;  // all of them are selected
+  const int position = position_of(a, token, slot);
+  const int earlier = min(position >> a.page_shift, a.columns);
+  const bool puts = a.fused && block % blocks_of_token == 0;
+  if (earlier <= a.count) {  // all of them are selected
+    if (puts) put_single(a, token, slot, kv_head, position, tid);
+    return;
+  }
   const bool packed = a.sequences.offsets != nullptr;
   const int32_t* table = a.tables + static_cast<int64_t>(slot) * a.columns;
   double* scores = a.scores + at * a.columns;
-  const int pieces = (a.key_width + kElements - 1) / kElements;
-  for (int base = static_cast<int>(block % blocks_of_token) * 64; base < earlier; base += blocks_of_token * 64) {
-    const int page = min(base + lane, earlier - 1), id = table[page];
-    const bool there = a.is_page(id);
-    const T* low = a.key_bounds + (static_cast<int64_t>(there ? id : 0) * a.kv_heads + kv_head) * 2 * a.key_width;
-    const T* high = low + a.key_width;
-    double best = -__builtin_inf();
-    for (int member0 = 0; member0 < a.share; member0 += kMembers) {
-      const int members = min(kMembers, a.share - member0);
-      __syncthreads();
-      for (int e = tid; e < kMembers * kMostWidth; e += kThreads) {
-        const int m = e / kMostWidth, d = e % kMostWidth;
-        const int head = kv_head * a.share + member0 + min(m, members - 1);
-        const T* query = packed ? a.query.row(0, token, head)
-                                : a.query.row(slot, token - slot * a.sequences.length, head);
-        queries[m][d] = d < a.key_width ? static_cast<float>(query[d]) : 0.0f;
+  const int col = tid % kLanes * kElements;
+  // (lanes behind the last column have queries of zero and some other columns)
+  const int from = min(col, WHOLE ? a.key_width - kElements : a.key_width - 1);
+  for (int member0 = 0; member0 < a.share; member0 += kMembers) {
+    const int members = min(kMembers, a.share - member0);
+    double queries[kMembers][kElements];
+#pragma unroll
+    for (int m = 0; m < kMembers; ++m) {
+      const int head = kv_head * a.share + member0 + min(m, members - 1);
+      const T* query = packed ? a.query.row(0, token, head)
+                              : a.query.row(slot, token - slot * a.sequences.length, head);
+      Piece part;
+      if constexpr (WHOLE) {
+        part = *reinterpret_cast<const Piece*>(query + from);
+      } else {
+#pragma unroll
+        for (int e = 0; e < kElements; ++e) part[e] = query[min(col + e, a.key_width - 1)];
       }
-      __syncthreads();
-      double sum[kMembers] = {};
-      for (int piece = wave; piece < pieces; piece += 4) {
-        const int col = piece * kElements;
-        Piece lows, highs;
+#pragma unroll
+      for (int e = 0; e < kElements; ++e)
+        queries[m][e] = col + e < a.key_width ? static_cast<double>(static_cast<float>(part[e])) : 0.0;
+    }
+    const int step = blocks_of_token * kPages * kTurns;
+    for (int base = static_cast<int>(block % blocks_of_token) * kPages * kTurns; base < earlier; base += step) {
+      int id[kTurns];
+      Piece lows[kTurns], highs[kTurns];
+#pragma unroll
+      for (int i = 0; i < kTurns; ++i) id[i] = table[min(base + i * kPages + tid / kLanes, earlier - 1)];
+#pragma unroll
+      for (int i = 0; i < kTurns; ++i) {
+        const T* low = a.key_bounds +
+                       (static_cast<int64_t>(a.is_page(id[i]) ? id[i] : 0) * a.kv_heads + kv_head) * 2 * a.key_width;
+        const T* high = low + a.key_width;
         if constexpr (WHOLE) {
-          lows = *reinterpret_cast<const Piece*>(low + col);
-          highs = *reinterpret_cast<const Piece*>(high + col);
+          lows[i] = *reinterpret_cast<const Piece*>(low + from);
+          highs[i] = *reinterpret_cast<const Piece*>(high + from);
         } else {
 #pragma unroll
           for (int e = 0; e < kElements; ++e) {
-            lows[e] = col + e < a.key_width ? low[col + e] : static_cast<T>(0.0f);
-            highs[e] = col + e < a.key_width ? high[col + e] : static_cast<T>(0.0f);
-          }
-        }
-#pragma unroll
-        for (int e = 0; e < kElements; ++e) {
-          const float least = static_cast<float>(lows[e]), largest = static_cast<float>(highs[e]);
-#pragma unroll
-          for (int m = 0; m < kMembers; ++m) {
-            const float q = queries[m][col + e];
-            sum[m] = fma(static_cast<double>(q), static_cast<double>(q > 0.0f ? largest : least), sum[m]);
+            lows[i][e] = low[min(from + e, a.key_width - 1)];
+            highs[i][e] = high[min(from + e, a.key_width - 1)];
           }
         }
       }
 #pragma unroll
-      for (int m = 0; m < kMembers; ++m) sums[wave][m][lane] = sum[m];
-      __syncthreads();
-      if (wave == 0) {
+      for (int i = 0; i < kTurns; ++i) {
+        const int page = base + i * kPages + tid / kLanes;
+        if (base + i * kPages >= earlier) break;
+        double sum[kMembers] = {};
 #pragma unroll
-        for (int m = 0; m < kMembers; ++m) {
-          const double score = ((sums[0][m][lane] + sums[1][m][lane]) + sums[2][m][lane]) + sums[3][m][lane];
-          best = score > best || score != score ? score : best;
+        for (int e = 0; e < kElements; ++e) {
+          const double least = static_cast<float>(lows[i][e]), largest = static_cast<float>(highs[i][e]);
+#pragma unroll
+          for (int m = 0; m < kMembers; ++m)
+            sum[m] = fma(queries[m][e], queries[m][e] > 0.0 ? largest : least, sum[m]);
+        }
+#pragma unroll
+        for (int m = 0; m < kMembers; ++m) sum[m] = over_lanes_sum<kLanes>(sum[m]);
+        if (tid % kLanes == 0 && page < earlier) {
+          double best = member0 > 0 ? scores[page] : -__builtin_inf();
+#pragma unroll
+          for (int m = 0; m < kMembers; ++m) best = sum[m] > best || sum[m] != sum[m] ? sum[m] : best;
+          scores[page] = a.is_page(id[i]) ? best : __builtin_nan("");
         }
       }
     }
-    if (wave == 0 && base + lane < earlier) scores[page] = there ? best : __builtin_nan("");
   }
+  if (puts) put_single(a, token, slot, kv_head, position, tid);
 }
 
 // A score as a whole number that ranks alike; what is no number ranks first.
@@ -1106,17 +1276,20 @@ __device__ __forceinline__ uint64_t rank_of(double score) {
 
 // The pages of a token and head of keys: the `count` with the largest scores, in the order of the
 // slot's table, and its own; and how many positions it sees on them.  A block finds the score of the
-// last one that is selected eight bits at a time, by counting.
-template <typename T>
-__global__ __launch_bounds__(kThreads) void paged_select_kernel(PagedArgs<T> a) {
-  __shared__ int counts[256], ends[4], equal_ends[4], chosen[2];
+// last one that is selected eight bits at a time, by counting, of many pages from the first bit on in
+// which scores differ.
+template <typename T, int THREADS>
+__global__ __launch_bounds__(THREADS) void paged_select_kernel(PagedArgs<T> a) {
+  constexpr int kAll = THREADS / 64;
+  __shared__ int counts[256], ends[kAll], equal_ends[kAll], chosen[2];
+  __shared__ uint64_t lowest[kAll], highest[kAll];
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const int64_t at = block_number(), number = at / a.kv_heads;
   if (number >= a.slab_tokens) return;
   const int token = static_cast<int>(a.slab_first + number);
   const int64_t to = static_cast<int64_t>(token) * a.kv_heads + at % a.kv_heads;
   int32_t* list = a.lists + to * (a.count + 1);
-  if (!offsets_valid(a, tid)) {
+  if (!offsets_valid<THREADS>(a, tid)) {
     if (tid == 0) a.seen[to] = 0;
     return;
   }
@@ -1129,22 +1302,53 @@ __global__ __launch_bounds__(kThreads) void paged_select_kernel(PagedArgs<T> a) 
     a.seen[to] = (selected << a.page_shift) + (position & ((1 << a.page_shift) - 1)) + 1;
   }
   if (earlier <= a.count) {
-    for (int j = tid; j < earlier; j += kThreads) list[j] = table[j];
+    for (int j = tid; j < earlier; j += THREADS) list[j] = table[j];
     return;
   }
   const double* scores = a.scores + at * a.columns;
-  // those above `prefix` in the bits of `mask` are selected, and the first `need` of those equal to it
-  uint64_t prefix = 0, mask = 0;
-  int need = a.count;
-  for (int shift = 56; shift >= 0; shift -= 8) {
-    counts[tid] = 0;
-    __syncthreads();
-    for (int j = tid; j < earlier; j += kThreads) {
-      const uint64_t rank = rank_of(scores[j]);
-      if ((rank & mask) == prefix) atomicAdd(&counts[rank >> shift & 255], 1);
+  // the pages in turns of a block's threads, for all threads
+  const auto for_each = [&](auto&& visit) {
+    for (int base = 0; base < earlier; base += THREADS)
+      visit(base + tid, rank_of(scores[min(base + tid, earlier - 1)]));
+  };
+  // (of a few pages the first bits are not worth finding out)
+  uint64_t low = 0, high = ~uint64_t{0};
+  if (earlier > 1024) {
+    low = ~uint64_t{0};
+    high = 0;
+    for_each([&](int j, uint64_t rank) {
+      if (j < earlier) {
+        low = min(low, rank);
+        high = max(high, rank);
+      }
+    });
+    for (int away = 1; away < 64; away *= 2) {
+      low = min(low, static_cast<uint64_t>(__shfl_xor(static_cast<unsigned long long>(low), away)));
+      high = max(high, static_cast<uint64_t>(__shfl_xor(static_cast<unsigned long long>(high), away)));
+    }
+    if (lane == 0) {
+      lowest[wave] = low;
+      highest[wave] = high;
     }
     __syncthreads();
-    const int mine = counts[255 - tid], upto = scan_wave(mine, lane);
+    for (int w = 0; w < kAll; ++w) {
+      low = min(low, lowest[w]);
+      high = max(high, highest[w]);
+    }
+  }
+  // those above `prefix` in the bits of `mask` are selected, and the first `need` of those equal to it
+  int bits = low == high ? 0 : 64 - __clzll(low ^ high);  // that are not yet known
+  uint64_t mask = bits == 64 ? 0 : ~uint64_t{0} << bits, prefix = low & mask;
+  int need = a.count;
+  while (bits > 0) {
+    const int shift = max(bits - 8, 0), digits = (1 << (bits - shift)) - 1;
+    if (tid < 256) counts[tid] = 0;
+    __syncthreads();
+    for_each([&](int j, uint64_t rank) {
+      if (j < earlier && (rank & mask) == prefix) atomicAdd(&counts[rank >> shift & digits], 1);
+    });
+    __syncthreads();
+    const int mine = tid < 256 ? counts[255 - tid] : 0, upto = scan_wave(mine);
     if (lane == 63) ends[wave] = upto;
     __syncthreads();
     int before = upto - mine;
@@ -1157,15 +1361,15 @@ __global__ __launch_bounds__(kThreads) void paged_select_kernel(PagedArgs<T> a) 
     const int digit = chosen[0];
     need -= chosen[1];
     prefix |= static_cast<uint64_t>(digit) << shift;
-    mask |= uint64_t{255} << shift;
+    mask = ~uint64_t{0} << shift;
+    bits = shift;
     const bool all = counts[digit] == need;
     __syncthreads();
     if (all) break;
   }
   int above = 0, equal = 0;  // of the pages so far
-  for (int base = 0; base < earlier; base += kThreads) {
-    const int j = base + tid;
-    const uint64_t rank = j < earlier ? rank_of(scores[j]) & mask : 0;
+  for_each([&](int j, uint64_t rank) {
+    rank &= mask;
     const bool more = j < earlier && rank > prefix, same = j < earlier && rank == prefix;
     const uint64_t more_mask = __ballot(more), same_mask = __ballot(same);
     if (lane == 0) {
@@ -1175,7 +1379,7 @@ __global__ __launch_bounds__(kThreads) void paged_select_kernel(PagedArgs<T> a) 
     __syncthreads();
     const uint64_t below = (uint64_t{1} << lane) - 1;
     int above_me = above + __popcll(more_mask & below), equal_me = equal + __popcll(same_mask & below);
-    for (int w = 0; w < 4; ++w) {
+    for (int w = 0; w < kAll; ++w) {
       if (w < wave) {
         above_me += ends[w];
         equal_me += equal_ends[w];
@@ -1185,7 +1389,7 @@ __global__ __launch_bounds__(kThreads) void paged_select_kernel(PagedArgs<T> a) 
     }
     if (more || (same && equal_me < need)) list[above_me + min(equal_me, need)] = table[j];
     __syncthreads();
-  }
+  });
 }
 
 // ---------------------------------------------------------------------------
@@ -1227,6 +1431,7 @@ PagedDivision division_of(const PagedShare& share, int most_few, char* at) {
   d.target = share.target;
   d.least = share.least;
   d.most_few = most_few;
+  d.round = share.round;
   d.parts = share.parts;
   if (share.parts > 0) {
     d.partial = reinterpret_cast<float*>(at);
@@ -1236,34 +1441,46 @@ PagedDivision division_of(const PagedShare& share, int most_few, char* at) {
   return d;
 }
 
-constexpr int kJoinBlocks = 2048;
+// Blocks that go on to further work: a thousand more take the chip 4 us to begin, whatever they do.
+constexpr int64_t kJoinBlocks = 1024;
+constexpr int64_t kScoreBlocks = 1024;
 
 template <typename T, int WIDTH, bool WHOLE>
 void paged_token_launch(PagedArgs<T>& args, const PagedShare& share, hipStream_t stream) {
   const dim3 grid = grid_of(share.items * args.kv_heads);
-  if constexpr (sizeof(T) == 2) {
-    if (share.rows == 32) paged_token_kernel<T, WIDTH, 2, WHOLE><<<grid, kThreads, 0, stream>>>(args);
-  }
-  if (share.rows == 16) paged_token_kernel<T, WIDTH, 1, WHOLE><<<grid, kThreads, 0, stream>>>(args);
+  paged_token_kernel<T, WIDTH, WHOLE><<<grid, kThreads, 0, stream>>>(args);
   if (share.parts == 0) return;
-  const int64_t rows = share.parts / 2 * args.kv_heads * share.rows;  // (a cut tile has two parts or more)
-  paged_join_kernel<T, WIDTH, true>
-      <<<dim3(static_cast<unsigned>(rows < kJoinBlocks ? rows : kJoinBlocks)), kThreads, 0, stream>>>(
-          args, share.rows);
+  // (a cut tile has two parts or more)
+  const int64_t units = share.parts / 2 * args.kv_heads * share.unit_rows;
+  paged_join_few_kernel<T, WIDTH>
+      <<<dim3(static_cast<unsigned>(std::min<int64_t>(units, kJoinBlocks))), kThreads, 0, stream>>>(
+          args, share.rows, share.unit_rows);
+}
+
+template <typename T, int WIDTH, int USED, bool WHOLE>
+void paged_chunk_rows(PagedArgs<T>& args, const PagedShare& share, hipStream_t stream) {
+  const dim3 grid = grid_of_items(share.items * args.kv_heads);
+  if constexpr (kPairs<T, WIDTH>) {
+    if (share.rows == 128) paged_chunk_kernel<T, WIDTH, USED, 2, WHOLE><<<grid, kThreads, 0, stream>>>(args);
+  }
+  if (share.rows == 64) paged_chunk_kernel<T, WIDTH, USED, 1, WHOLE><<<grid, kThreads, 0, stream>>>(args);
 }
 
 template <typename T, int WIDTH, bool WHOLE>
 void paged_chunk_launch(PagedArgs<T>& args, const PagedShare& share, hipStream_t stream) {
-  const dim3 grid = grid_of_items(share.items * args.kv_heads);
-  if constexpr (kPairs<T, WIDTH>) {
-    if (share.rows == 128) paged_chunk_kernel<T, WIDTH, 2, WHOLE><<<grid, kThreads, 0, stream>>>(args);
+  // (columns that no head has are left out where that is a quarter of them)
+  if constexpr (WIDTH == 128) {
+    if (args.key_width <= 96 && args.value_width <= 96)
+      paged_chunk_rows<T, WIDTH, 96, WHOLE>(args, share, stream);
+    else
+      paged_chunk_rows<T, WIDTH, WIDTH, WHOLE>(args, share, stream);
+  } else {
+    paged_chunk_rows<T, WIDTH, WIDTH, WHOLE>(args, share, stream);
   }
-  if (share.rows == 64) paged_chunk_kernel<T, WIDTH, 1, WHOLE><<<grid, kThreads, 0, stream>>>(args);
   if (share.parts == 0) return;
-  const int64_t waves = share.parts / 2 * args.kv_heads * share.rows;
-  paged_join_kernel<T, WIDTH, false>
-      <<<dim3(static_cast<unsigned>(waves / 4 < kJoinBlocks ? (waves + 3) / 4 : kJoinBlocks)), kThreads, 0,
-         stream>>>(args, share.rows);
+  const int64_t blocks = share.parts / 2 * args.kv_heads * share.rows * (WIDTH / 4) / kThreads;
+  paged_join_many_kernel<T, WIDTH>
+      <<<dim3(static_cast<unsigned>(std::min<int64_t>(blocks, kJoinBlocks))), kThreads, 0, stream>>>(args, share.rows);
 }
 
 template <typename T, bool WHOLE>
@@ -1286,11 +1503,16 @@ void paged_select_launch(PagedArgs<T>& args, const PagedPlan& plan, hipStream_t 
     args.slab_tokens = std::min<int64_t>(slab, args.sequences.tokens - first);
     const int64_t pairs = args.slab_tokens * args.kv_heads;
     if (args.columns > args.count) {
-      const int64_t most = (args.columns + kScorePages - 1) / kScorePages;
-      const int blocks = static_cast<int>(std::max<int64_t>(1, std::min(most, 2048 / pairs)));
+      const int64_t at_once = 4 * kThreads / (kMostWidth * sizeof(T) / 16);
+      const int64_t most = (args.columns + at_once - 1) / at_once;
+      const int blocks = static_cast<int>(std::max<int64_t>(1, std::min(most, kScoreBlocks / pairs)));
       paged_score_kernel<T, WHOLE><<<grid_of(pairs * blocks), kThreads, 0, stream>>>(args, blocks);
     }
-    paged_select_kernel<T><<<grid_of(pairs), kThreads, 0, stream>>>(args);
+    // (few long lists: all the threads that a block can have)
+    if (pairs <= 256 && args.columns > 1024)
+      paged_select_kernel<T, 1024><<<grid_of(pairs), 1024, 0, stream>>>(args);
+    else
+      paged_select_kernel<T, kThreads><<<grid_of(pairs), kThreads, 0, stream>>>(args);
   }
 }
 
@@ -1305,16 +1527,20 @@ void paged_update_launch(const PagedCall& call) {
   const PagedDivision many = division_of<T>(plan.many, plan.most_few, at);
   at += plan.many.bytes();
   if (call.count > 0) {
-    paged_append_launch<T, WHOLE>(args, call.stream);
+    // (single tokens are put on their rows by the kernel of the scores, where it runs)
+    args.fused = p.cu_seqlens == nullptr && p.T == 1 && args.columns > args.count;
+    if (!args.fused) paged_append_launch<T, WHOLE>(args, call.stream);
     args.lists = reinterpret_cast<int32_t*>(at);
     args.seen = reinterpret_cast<int32_t*>(at + plan.list_bytes);
     args.scores = reinterpret_cast<double*>(at + plan.list_bytes + plan.seen_bytes);
     paged_select_launch<T, WHOLE>(args, plan, call.stream);
+    args.fused = false;
     args.division = few;
     args.list_splits = plan.few.target;
     return paged_token_launch<T, WIDTH, WHOLE>(args, plan.few, call.stream);
   }
-  args.fused = p.cu_seqlens == nullptr && p.T == 1 && plan.few.used && !plan.many.used;
+  // (bounds of a page that several tokens are put on have a kernel of their own)
+  args.fused = args.key_bounds == nullptr || (p.cu_seqlens == nullptr && p.T == 1 && !plan.many.used);
   if (!args.fused) paged_append_launch<T, WHOLE>(args, call.stream);
   if (plan.few.used) {
     args.division = few;

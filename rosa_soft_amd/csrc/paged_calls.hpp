@@ -11,14 +11,15 @@ constexpr int kMostPortions = 1024;
 // Slots of the tables that one call changes, at most: a prefix of each is kept in LDS.
 constexpr int kMostTableSlots = 8192;
 constexpr int kMostCount = 1024;  // selected pages of a token
-constexpr int kScorePages = 64;   // pages of a block of the scores
 
 // How the keys of one kernel's calls are shared out (see portion_of in paged_attention.hpp).
 struct PagedShare {
   bool used;
   int rows;              // of a tile: (token, member of the group) pairs
+  int unit_rows;         // of a tile that may be there
   int target;            // portions of a head of keys that a call is cut into, beside one for each tile
   int least;             // tiles of keys of a portion, at least
+  int round;             // eighths of a portion from which on a walk has one more
   int64_t items;         // portions of a head of keys, at most
   int64_t parts;         // portions of tiles that are cut, at most: those with partial sums
   size_t part_bytes, task_bytes;

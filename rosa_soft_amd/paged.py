@@ -27,9 +27,10 @@ pool, pages and bounds) shares no memory with what it reads, and gets a new vers
 depend on the order in which blocks run.
 
 Nothing that is on the device is looked at by the host: invalid ``cu_seqlens`` make every output NaN
-and change nothing, and numbers that are no page are never followed.  A page that holds something that
-is not finite may make NaN of every token that sees a part of it; tokens that see nothing of the 64
-positions around it, and other slots, keep their results.
+and change nothing, and numbers that are no page are never followed.  A key or value that is not finite
+makes NaN of every token that sees it, and may do so to new tokens up to 95 positions before it, because
+masked weights of a tile are zeros that multiply its rows; other tokens and slots keep their results.
+What no token was put on is never read.
 """
 
 from __future__ import annotations
@@ -160,7 +161,8 @@ def paged_attention_update(query: Tensor, key: Tensor, value: Tensor, key_pages:
 
     A new token whose row is negative (padding) is not stored; in this call it is seen like the others.
     A token that sees a position without a page has NaN as its output.
-    Slots may share pages as long as nobody writes to them; a page that is written belongs to one slot.
+    Slots may share pages as long as nobody writes to them; a page that is written belongs to one slot,
+    and no two tokens of a call to the same row.
     """
 
     scale = _number("scale", scale)

@@ -64,6 +64,7 @@ def check_tables(want, tables, pool):
 @pytest.mark.parametrize("slots,columns,pages,page,packed", [
     (1, 1, 1, 16, False), (1, 9, 40, 16, True), (3, 4, 20, 64, False), (5, 7, 12, 32, True),
     (70, 11, 300, 16, True), (70, 11, 900, 256, False), (1030, 5, 3000, 16, True), (8192, 3, 9000, 32, False),
+    (8192, 2, 20000, 16, True),
 ])
 def test_pages_come_and_go(slots, columns, pages, page, packed):
     """Steps of growth, rejected tokens and ended requests, with pools and tables that run out."""
@@ -256,6 +257,15 @@ def test_many_slots(slots, packed):
         server.check(server.step(fresh, as_packed), before, slots=range(0, slots, 7))
 
 
+@pytest.mark.parametrize("slots", [63, 130, 700])
+def test_selected_pages_of_many_packed_slots(slots):
+    lengths = [(s * 37) % 150 + 1 for s in range(slots)]
+    server = Server(350, [n + 5 for n in lengths], 4, 2, 32, 32, 16, torch.bfloat16)
+    for fresh, count in ((lengths, None), ([s % 3 for s in range(slots)], 2), ([1] * slots, 3)):
+        before = list(server.seen)
+        server.check(server.step(fresh, True, count), before, count, slots=range(0, slots, 13))
+
+
 @pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("widths,chunk", [((8, 1, 64, 64), 1), ((8, 2, 128, 128), 1), ((8, 2, 128, 128), 6),
                                           ((8, 2, 64, 64), 90), ((6, 2, 48, 80), 20)])
@@ -424,6 +434,28 @@ def test_tokens_without_a_row_are_not_stored(chunk):
         cut[:, chunk // 2:] = -1
         part = paged.paged_attention_update(*inputs, *caches, server.tables, cut, server.lengths)
         assert torch.equal(part[:, :chunk // 2], full[:, :chunk // 2])
+
+
+@pytest.mark.parametrize("chunk", [1, 6, 200])
+@pytest.mark.parametrize("what", [0, 1])
+def test_what_is_not_finite_stays_near(chunk, what):
+    """A key or value makes NaN of the tokens that see it, perhaps of those up to 95 positions before it,
+    and of no other."""
+    server = Server(1150, [500 + chunk, 400 + chunk], 4, 2, 64, 64, 16, torch.bfloat16, bounds=False)
+    server.step([500, 400], packed=True)
+    rows = paged.page_tables_update(server.tables, server.lengths, server.pool, tokens=chunk, page=16)
+    inputs = [torch.stack([stream[i][at:at + chunk] for stream, at in zip(server.streams, server.seen)])
+              for i in range(3)]
+    clean = paged.paged_attention_update(*inputs, *[c.clone() for c in server.caches], server.tables, rows,
+                                         server.lengths)
+    for token in {0, chunk // 2, chunk - 1}:
+        hurt = [t.clone() for t in inputs]
+        hurt[1 + what][0, token, :, 3] = math.nan if what == 0 else math.inf
+        output = paged.paged_attention_update(*hurt, *[c.clone() for c in server.caches], server.tables, rows,
+                                              server.lengths)
+        assert not bool(torch.isfinite(output[0, token:, :, 3]).any())
+        assert torch.equal(output[0, :max(0, token - 95)], clean[0, :max(0, token - 95)])
+        assert torch.equal(output[1], clean[1])
 
 
 def test_slots_share_pages_that_nobody_writes():

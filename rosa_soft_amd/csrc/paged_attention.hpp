@@ -170,8 +170,9 @@ template <int ROWS, int KEYS, bool FEW, typename T>
 __device__ __forceinline__ Found portion_of(const PagedArgs<T>& a, int tid, Portion* p) {
   const PagedDivision& d = a.division;
   const int count = a.sequences.count, lane = tid & 63, wave = tid >> 6;
+  // (no walk is as long as 2^27 tiles)
   const auto portion_length = [&](int64_t all) {
-    return static_cast<int>(max(static_cast<int64_t>(d.least), (all + d.target - 1) / d.target));
+    return static_cast<int>(min(max(static_cast<int64_t>(d.least), (all + d.target - 1) / d.target), int64_t{1} << 27));
   };
   const auto splits_of = [&](const SlotWork& w, int length) {
     return w.tiles > 0 ? max(1, (w.walk + length * d.round / 8) / length) : 0;
@@ -331,6 +332,8 @@ __device__ __forceinline__ float higher_of(float a, float b) { return b > a || b
 template <typename T, bool WHOLE>
 __global__ __launch_bounds__(kThreads) void paged_append_kernel(PagedArgs<T> a) {
   __shared__ float lows[kMostWidth], highs[kMostWidth];
+  __shared__ uint64_t stored[kThreads / 64];  // which tokens of the page have a row
+  __shared__ int number_of_page;
   const int tid = threadIdx.x, page = 1 << a.page_shift;
   const uint32_t block = block_number();
   const int64_t slot64 = block / a.kv_heads;
@@ -369,17 +372,23 @@ __global__ __launch_bounds__(kThreads) void paged_append_kernel(PagedArgs<T> a) 
     copy(a.key_pages, a.key_width, keys, a.key.token_stride);
     copy(a.value_pages, a.value_width, values, a.value.token_stride);
     if (a.key_bounds == nullptr) continue;
-    const int64_t row = a.row_of(run.first + begin);
-    if (row < 0) continue;  // (the same for the whole block)
-    T* bounds = a.key_bounds + ((row >> a.page_shift) * a.kv_heads + kv_head) * 2 * a.key_width;
+    // (padding is on no page, and has no part in its bounds; a page has at most as many as threads)
+    const int64_t row = tid < end - begin ? a.row_of(run.first + begin + tid) : -1;
+    const uint64_t put = __ballot(row >= 0);
+    if ((tid & 63) == 0) stored[tid >> 6] = put;
+    if (row >= 0) number_of_page = static_cast<int>(row >> a.page_shift);
+    if (!__syncthreads_or(row >= 0)) continue;
+    T* bounds = a.key_bounds + (static_cast<int64_t>(number_of_page) * a.kv_heads + kv_head) * 2 * a.key_width;
     const int d = tid & (kMostWidth - 1), half = tid / kMostWidth;
     float low = __builtin_inff(), high = -__builtin_inff();
     if (d < a.key_width) {
 #pragma unroll 4
       for (int token = begin + half; token < end; token += 2) {
         const float x = static_cast<float>(keys[token * a.key.token_stride + d]);
-        low = lower_of(low, x);
-        high = higher_of(high, x);
+        if (stored[(token - begin) >> 6] >> (token - begin & 63) & 1) {
+          low = lower_of(low, x);
+          high = higher_of(high, x);
+        }
       }
       if (half == 1) {
         lows[d] = low;
@@ -429,6 +438,25 @@ __device__ __forceinline__ void put_tokens(const PagedArgs<T>& a, const T* keys,
   }
 }
 
+// Clears 16 bytes of a value that are not all finite; whether they were not.  A weight of zero would make
+// NaN of them, in rows that do not see them as well: in tiles that not all rows see they are cleared, and
+// rows from their position on become NaN.  (Paid once a block, by the tiles on the diagonal.  Numbers
+// without their sign rank like whole ones: one comparison for all of them.)
+template <typename T, typename Piece>
+__device__ __forceinline__ bool clear_wild(Piece& piece) {
+  typedef uint32_t Words __attribute__((ext_vector_type(4)));
+  const Words words = __builtin_bit_cast(Words, piece);
+  uint32_t most = 0;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    most = max(most, words[i] & 0x7fffffff);
+    if constexpr (sizeof(T) == 2) most = max(most, words[i] << 16 & 0x7fffffff);
+  }
+  const bool wild = most >= (std::is_same_v<T, _Float16> ? 0x7c000000u : 0x7f800000u);
+  if (wild) piece = Piece(static_cast<T>(0.0f));
+  return wild;
+}
+
 // ---------------------------------------------------------------------------
 // few rows
 // ---------------------------------------------------------------------------
@@ -449,6 +477,7 @@ paged_token_kernel(PagedArgs<T> a) {
   constexpr size_t kJoinBytes = sizeof(float) * kRows * kOuts;
   __shared__ __attribute__((aligned(16))) char shared[4 * (kTileBytes > kJoinBytes ? kTileBytes : kJoinBytes)];
   __shared__ float tops[4][kRows], totals[4][kRows];
+  __shared__ int wild_from[4];  // position of a wave's first value that is not finite, where keys are masked
 
   const int tid = threadIdx.x, lane = tid & 63, group = lane >> 4, column = lane & 15;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -626,6 +655,7 @@ paged_token_kernel(PagedArgs<T> a) {
     return bad;
   };
   int tile = split * share + wave, bad = 0, id[2] = {0, 0};
+  if (lane == 0) wild_from[wave] = 0x7fffffff;
   if (tile < tile_end) {
     look_up(tile, id);
     bad = fetch(tile, id);
@@ -648,6 +678,12 @@ paged_token_kernel(PagedArgs<T> a) {
       for (int i = 0; i < kPieces; ++i)
         if (missing >> (i * kPieceRows / 16) & 1) held[i] = Piece(static_cast<T>(0.0f));
     }
+    const bool masked = tile * kTile + kTile - 1 > first_limit;
+    if (masked && first_limit < last) {
+#pragma unroll
+      for (int i = 0; i < kPieces; ++i)
+        if (clear_wild<T>(held[i])) atomicMin(&wild_from[wave], tile * kTile + i * kPieceRows + lane / kPerRow);
+    }
     // (LDS accesses of one wave are carried out in order: its tile needs no barrier)
 #pragma unroll
     for (int i = 0; i < kPieces; ++i) {
@@ -667,7 +703,7 @@ paged_token_kernel(PagedArgs<T> a) {
       for (int k = 0; k < 2; ++k)
         if (missing >> k & 1) score[k] = f32x4(__builtin_nanf(""));
     }
-    if (tile * kTile + kTile - 1 > first_limit) {
+    if (masked) {
 #pragma unroll
       for (int k = 0; k < 2; ++k)
 #pragma unroll
@@ -712,7 +748,7 @@ paged_token_kernel(PagedArgs<T> a) {
     *reinterpret_cast<f32x4*>(outs + column * kOuts + d * 16 + 4 * group) = out[d];
   if (group == 0) {
     // tokens behind the table have a key that is on no page
-    const bool lost = void_rows || (!single && limit >= a.capacity());
+    const bool lost = void_rows || (!single && limit >= a.capacity()) || limit >= wild_from[wave];
     tops[wave][column] = most;
     totals[wave][column] = lost ? __builtin_nanf("") : sum;
   }
@@ -759,6 +795,7 @@ paged_chunk_kernel(PagedArgs<T> a) {
   using Move = TileMove<T, kKeys, WIDTH, WHOLE>;
   __shared__ __attribute__((aligned(16))) Stored<T> key_tiles[kBuffers<T> * kTile];
   __shared__ __attribute__((aligned(16))) Stored<T> value_tiles[kBuffers<T> * kTile];
+  __shared__ int wild_from[4];  // position of a wave's first value that is not finite, where keys are masked
 
   const int tid = threadIdx.x, lane = tid & 63, group = lane >> 4, column = lane & 15;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -880,6 +917,10 @@ paged_chunk_kernel(PagedArgs<T> a) {
         value_move.held[i] = typename Move::Piece(static_cast<T>(0.0f));
   };
 
+  if (lane == 0) wild_from[wave] = 0x7fffffff;
+  int wild = 0x7fffffff;
+  const int first_limit = past + row0 / a.share;
+
   const int tiles = last / kKeys + 1, share = (tiles + p.splits - 1) / p.splits;
   const int tile_end = min(tiles, (p.split + 1) * share);
   int tile = p.split * share;
@@ -897,9 +938,17 @@ paged_chunk_kernel(PagedArgs<T> a) {
     const int begin = tile * kKeys, here_missing = missing;
     Stored<T>*keys = key_tiles + side * kTile, *values = value_tiles + side * kTile;
     clear_missing(missing);
+    const bool diagonal = begin + kKeys - 1 > first_limit && first_limit < last;
+    if (diagonal) {
+#pragma unroll
+      for (int i = 0; i < Move::kPieces; ++i)
+        if (clear_wild<T>(value_move.held[i])) atomicMin(&wild_from[wave], begin + Move::row_of(i, tid));
+    }
     key_move.store(keys, a.key_width, tid);
     value_move.store(values, a.value_width, tid);
     __syncthreads();
+    if (diagonal)
+      for (int w = 0; w < 4; ++w) wild = min(wild, wild_from[w]);
     if (tile + 1 < tile_end) {
       missing = missing_of(ids);
       fetch_keys(tile + 1, ids);
@@ -1001,7 +1050,7 @@ paged_chunk_kernel(PagedArgs<T> a) {
     const int row = wave_row + i * 16 + column;
     if (row >= row0 + rows) continue;
     // tokens behind the table have a key that is on no page
-    const float total = limit[i] >= capacity ? __builtin_nanf("") : sum[i][0];
+    const float total = limit[i] >= capacity || limit[i] >= wild ? __builtin_nanf("") : sum[i][0];
     const int token = row / a.share;
     if (p.splits == 1) {
       const int64_t at = (first_token + token) * a.heads + kv_head * a.share + row - token * a.share;
@@ -1200,7 +1249,7 @@ __global__ __launch_bounds__(kThreads) void paged_score_kernel(PagedArgs<T> a, i
   const int32_t* table = a.tables + static_cast<int64_t>(slot) * a.columns;
   double* scores = a.scores + at * a.columns;
   const int col = tid % kLanes * kElements;
-  // (lanes behind the last column have queries of zero and some other columns)
+  // (lanes behind the last column have queries of zero, some other bounds, and sums that are left out)
   const int from = min(col, WHOLE ? a.key_width - kElements : a.key_width - 1);
   for (int member0 = 0; member0 < a.share; member0 += kMembers) {
     const int members = min(kMembers, a.share - member0);
@@ -1238,8 +1287,9 @@ __global__ __launch_bounds__(kThreads) void paged_score_kernel(PagedArgs<T> a, i
         } else {
 #pragma unroll
           for (int e = 0; e < kElements; ++e) {
-            lows[i][e] = low[min(from + e, a.key_width - 1)];
-            highs[i][e] = high[min(from + e, a.key_width - 1)];
+            const bool there = from + e < a.key_width;
+            lows[i][e] = there ? low[from + e] : static_cast<T>(0.0f);
+            highs[i][e] = there ? high[from + e] : static_cast<T>(0.0f);
           }
         }
       }
@@ -1256,7 +1306,8 @@ __global__ __launch_bounds__(kThreads) void paged_score_kernel(PagedArgs<T> a, i
             sum[m] = fma(queries[m][e], queries[m][e] > 0.0 ? largest : least, sum[m]);
         }
 #pragma unroll
-        for (int m = 0; m < kMembers; ++m) sum[m] = over_lanes_sum<kLanes>(sum[m]);
+        for (int m = 0; m < kMembers; ++m)  // (zero times infinity is no number)
+          sum[m] = over_lanes_sum<kLanes>(col < a.key_width ? sum[m] : 0.0);
         if (tid % kLanes == 0 && page < earlier) {
           double best = member0 > 0 ? scores[page] : -__builtin_inf();
 #pragma unroll

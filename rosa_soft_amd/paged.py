@@ -27,10 +27,9 @@ pool, pages and bounds) shares no memory with what it reads, and gets a new vers
 depend on the order in which blocks run.
 
 Nothing that is on the device is looked at by the host: invalid ``cu_seqlens`` make every output NaN
-and change nothing, and numbers that are no page are never followed.  A key or value that is not finite
-makes NaN of every token that sees it, and may do so to new tokens up to 95 positions before it, because
-masked weights of a tile are zeros that multiply its rows; other tokens and slots keep their results.
-What no token was put on is never read.
+and change nothing, and numbers that are no page are never followed.  Tokens that see a key or a
+value that is not finite may have outputs that are not, in one column or in all; the others keep their
+results.  What no token was put on is never read.
 """
 
 from __future__ import annotations
@@ -159,7 +158,9 @@ def paged_attention_update(query: Tensor, key: Tensor, value: Tensor, key_pages:
     largest element of each column of the keys on a page are kept up to date, for
     ``selected_attention_update``.
 
-    A new token whose row is negative (padding) is not stored; in this call it is seen like the others.
+    A new token whose row is negative (padding) is not stored, and has no part in the bounds; in this
+    call the new tokens behind it see it like the others, so padding goes behind the real tokens.
+    Rejected tokens may leave the bounds of their page wider than its keys.
     A token that sees a position without a page has NaN as its output.
     Slots may share pages as long as nobody writes to them; a page that is written belongs to one slot,
     and no two tokens of a call to the same row.

@@ -436,26 +436,89 @@ def test_tokens_without_a_row_are_not_stored(chunk):
         assert torch.equal(part[:, :chunk // 2], full[:, :chunk // 2])
 
 
-@pytest.mark.parametrize("chunk", [1, 6, 200])
-@pytest.mark.parametrize("what", [0, 1])
-def test_what_is_not_finite_stays_near(chunk, what):
-    """A key or value makes NaN of the tokens that see it, perhaps of those up to 95 positions before it,
-    and of no other."""
-    server = Server(1150, [500 + chunk, 400 + chunk], 4, 2, 64, 64, 16, torch.bfloat16, bounds=False)
-    server.step([500, 400], packed=True)
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("widths", [(4, 2, 64, 64), (3, 1, 24, 33), (8, 1, 128, 128), (2, 1, 80, 96)])
+@pytest.mark.parametrize("chunk", [1, 2, 6, 30, 200])
+@pytest.mark.parametrize("past", [0, 500])
+def test_what_is_not_finite_stays_with_those_that_see_it(past, chunk, widths, dtype):
+    server = Server(1150, [past + chunk, past // 2 + chunk], *widths, 16, dtype, bounds=False)
+    if past:
+        server.step([past, past // 2], packed=True)
     rows = paged.page_tables_update(server.tables, server.lengths, server.pool, tokens=chunk, page=16)
     inputs = [torch.stack([stream[i][at:at + chunk] for stream, at in zip(server.streams, server.seen)])
               for i in range(3)]
-    clean = paged.paged_attention_update(*inputs, *[c.clone() for c in server.caches], server.tables, rows,
-                                         server.lengths)
-    for token in {0, chunk // 2, chunk - 1}:
-        hurt = [t.clone() for t in inputs]
-        hurt[1 + what][0, token, :, 3] = math.nan if what == 0 else math.inf
-        output = paged.paged_attention_update(*hurt, *[c.clone() for c in server.caches], server.tables, rows,
-                                              server.lengths)
-        assert not bool(torch.isfinite(output[0, token:, :, 3]).any())
-        assert torch.equal(output[0, :max(0, token - 95)], clean[0, :max(0, token - 95)])
-        assert torch.equal(output[1], clean[1])
+    where = server.tables, rows, server.lengths
+    clean = paged.paged_attention_update(*inputs, *[c.clone() for c in server.caches], *where)
+    for what, value in ((1, math.nan), (2, math.inf), (2, math.nan)):
+        for token in {0, chunk // 2, chunk - 1}:
+            hurt = [t.clone() for t in inputs]
+            hurt[what][0, token, 0, -1] = value
+            output = paged.paged_attention_update(*hurt, *[c.clone() for c in server.caches], *where)
+            group = widths[0] // widths[1]
+            assert not bool(torch.isfinite(output[0, token:, :group, -1]).any())
+            assert torch.equal(output[0, :token], clean[0, :token])
+            assert torch.equal(output[0, :, group:], clean[0, :, group:])
+            assert torch.equal(output[1], clean[1])
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("count", [None, 2])
+def test_padding_that_is_not_finite(count, dtype):
+    """A dense batch of prompts of several lengths, padded with what is no number: outputs, pages and
+    bounds are those of the real tokens, and so are those of the next step."""
+    lengths, most = [70, 33, 1, 48], 70
+    server = Server(1160, [n + 1 for n in lengths], 4, 2, 64, 64, 16, dtype)
+    padded = []
+    for i in range(3):
+        batch = torch.full((4, most, *server.streams[0][i].shape[1:]), math.nan, dtype=dtype, device=DEVICE)
+        for s, n in enumerate(lengths):
+            batch[s, :n] = server.streams[s][i][:n]
+        padded.append(batch)
+    packed_rows = paged.page_tables_update(server.tables, server.lengths, server.pool, offsets_of(lengths),
+                                           tokens=sum(lengths), page=16)
+    rows = torch.full((4, most), -1, dtype=torch.int64, device=DEVICE)
+    for s, part in enumerate(packed_rows.split(lengths)):
+        rows[s, :lengths[s]] = part
+    where = server.tables, rows, server.lengths
+    if count is None:
+        output = paged.paged_attention_update(*padded, *server.caches, *where, key_bounds=server.bounds)
+    else:
+        output = paged.selected_attention_update(*padded, *server.caches, server.bounds, *where, count=count)
+    server.lengths += i32(lengths)
+    server.seen = list(lengths)
+    server.check([output[s, :n] for s, n in enumerate(lengths)], [0] * 4, count)
+    server.check(server.step([1] * 4, False, count), lengths, count)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("width", [24, 33, 40, 128])
+@pytest.mark.parametrize("both", [False, True])
+def test_pages_with_a_key_that_is_not_finite(both, width, dtype):
+    """Minus infinity in a bound against queries above zero ranks last; who sees no such key is as ever."""
+    server = Server(1170, [101], 1, 1, width, width, 16, dtype)
+    for stream in (server.streams[0][0], server.streams[0][1]):
+        stream.abs_().add_(0.125)
+    if both:
+        server.streams[0][1][20, 0, -1] = -math.inf    # page 1, whose bounds from above stay finite
+    server.streams[0][1][32:48, 0, -1] = -math.inf  # page 2
+    server.step([100], True)
+    for count in (1, 4):
+        rows = paged.page_tables_update(server.tables, server.lengths, server.pool, tokens=1, page=16)
+        output = paged.selected_attention_update(
+            *(t[100:].unsqueeze(0) for t in server.streams[0]), *[c.clone() for c in server.caches],
+            server.bounds.clone(), server.tables, rows, server.lengths, count=count)
+        q, k, v = server.streams[0]
+        pages = reference.selected(q[100], k[:, 0], 16, count, 100)
+        kept = torch.cat([torch.arange(j * 16, min(101, j * 16 + 16), device=DEVICE) for j in pages])
+        assert 2 not in pages
+        if not bool(torch.isfinite(k[kept]).all()) and not bool(torch.isfinite(output).all()):
+            continue    # (a key that is seen may make the output what it is)
+        weights = torch.softmax(k[kept, 0].double() @ q[100, 0].double() * width ** -0.5, 0)
+        bound = (weights[:, None] * v[kept, 0].double().abs()).sum(0)
+        finite = torch.where(torch.isfinite(k[kept, 0]), k[kept, 0], 0).double()
+        most = float((finite.abs() @ q[100, 0].double().abs()).max()) * width ** -0.5
+        close(output[0, 0, 0], (weights[:, None] * v[kept, 0].double()).sum(0),
+              tolerance_of(dtype, bound, most, len(kept), 2 * width))
 
 
 def test_slots_share_pages_that_nobody_writes():

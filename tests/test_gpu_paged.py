@@ -291,6 +291,35 @@ def test_selected_pages(page, count, widths, dtype):
         server.check(server.step(fresh, packed, count), before, count)
 
 
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("widths", [(4, 2, 96, 96), (4, 1, 80, 96), (2, 2, 96, 64), (8, 2, 72, 100)])
+def test_widths_between_two_tiles(widths, dtype):
+    """Columns that no head has are left out of the products of many rows."""
+    server = Server(450, [2400, 300], *widths, 32, dtype)
+    server.step([2000, 100], packed=True)
+    for fresh, packed in (([150, 150], False), ([70, 0], True), ([1, 1], False), ([20, 20], False)):
+        before = list(server.seen)
+        server.check(server.step(fresh, packed), before)
+
+
+@pytest.mark.parametrize("fresh", [[1] * 15 + [6], [1] * 15 + [700], [0] * 15 + [1], [130] * 15 + [1]])
+def test_packed_single_tokens_beside_a_prompt(fresh):
+    """Slots of few rows have their own kernel, or the one of the prompts."""
+    totals = [(s * 331) % 3000 + 5 for s in range(16)]
+    server = Server(470, [a + b for a, b in zip(totals, fresh)], 8, 1, 64, 64, 16, torch.bfloat16)
+    server.step(totals, packed=True)
+    before = list(server.seen)
+    server.check(server.step(fresh, packed=True), before)
+
+
+def test_more_scores_than_are_kept_at_once():
+    """Tables so wide that the scores of a prompt are made in parts."""
+    server = Server(650, [800], 4, 2, 32, 32, 16, torch.float16, columns=70000)
+    server.step([500], packed=False)
+    before = list(server.seen)
+    server.check(server.step([300], packed=False, count=5), before, count=5)
+
+
 def test_selection_among_many_pages():
     """Thousands of scores, with a count from one to nearly all of them."""
     server = Server(600, [40000], 4, 1, 16, 16, 16, torch.bfloat16, columns=2600)
@@ -363,6 +392,26 @@ def test_missing_pages_make_nan_of_the_tokens_that_see_them(chunk, dtype):
             upto = visible.index(True)
             want, bound, most = reference.attention(inputs[0][0, :upto], k[:400 + upto], v[:400 + upto], 400)
             close(output[0, :upto], want, tolerance_of(dtype, bound, most, 500, 128))
+
+
+@pytest.mark.parametrize("chunk", [1, 4])
+def test_a_missing_page_among_those_to_select_from(chunk):
+    """It ranks first: its slot's tokens are NaN, and no others."""
+    server = Server(980, [400 + chunk] * 2, 4, 2, 64, 64, 16, torch.bfloat16)
+    server.step([400] * 2, packed=True)
+    for entry in (-1, server.pages, 2**31 - 1, -2**31):
+        tables = server.tables.clone()
+        rows = paged.page_tables_update(tables, server.lengths, server.pool.clone(), tokens=chunk, page=16)
+        inputs = [torch.stack([stream[i][400:] for stream in server.streams]) for i in range(3)]
+        results = []
+        for hurt in (False, True):
+            if hurt:
+                tables[0, 3] = entry
+            results.append(paged.selected_attention_update(
+                *inputs, *[c.clone() for c in server.caches], server.bounds.clone(), tables, rows,
+                server.lengths, count=2))
+        assert bool(torch.isnan(results[1][0]).all()) and torch.equal(results[0][1], results[1][1])
+        assert bool(torch.isfinite(results[0]).all())
 
 
 def test_tokens_behind_their_table_are_nan_and_lengths_without_sense_end():
@@ -669,6 +718,28 @@ def test_streams_and_graphs():
                 assert all(torch.equal(a, b) for a, b in zip(outputs, want))
                 assert torch.equal(recorded.tables, eager.tables) and torch.equal(recorded.pool, eager.pool)
                 assert torch.equal(recorded.bounds.nan_to_num(7.0), eager.bounds.nan_to_num(7.0))
+
+
+def test_two_servers_on_two_streams():
+    """Steps of two servers that run at once."""
+    totals, plans = [1500, 900, 40], [[700, 1, 30], [2, 5, 1], [1] * 3, [3] * 3, [1] * 3]
+    servers = [Server(seed, totals, 8, 2, 64, 64, 16, torch.bfloat16) for seed in (1710, 1750)]
+    streams = [torch.cuda.Stream() for _ in servers]
+    torch.cuda.synchronize()
+    outputs = [[], []]
+    for i, fresh in enumerate(plans):
+        for server, stream, kept in zip(servers, streams, outputs):
+            with torch.cuda.stream(stream):
+                kept.append((list(server.seen), fresh, server.step(fresh, len(set(fresh)) > 1, 4 if i > 2 else None)))
+    torch.cuda.synchronize()
+    for server, kept in zip(servers, outputs):
+        for i, (before, fresh, output) in enumerate(kept):
+            for s in range(3):
+                q, k, v = server.streams[s]
+                end = before[s] + fresh[s]
+                want, bound, most = reference.attention(q[before[s]:end], k[:end], v[:end], before[s], 16,
+                                                        4 if i > 2 else None)
+                close(output[s], want, tolerance_of(torch.bfloat16, bound, most, end, 128))
 
 
 def test_changed_tensors_get_new_versions():

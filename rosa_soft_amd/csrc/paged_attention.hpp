@@ -328,7 +328,10 @@ __device__ __forceinline__ float lower_of(float a, float b) { return b < a || b 
 __device__ __forceinline__ float higher_of(float a, float b) { return b > a || b != b ? b : a; }
 
 // The new tokens on their rows, and the bounds of the pages that they lie on.  A block has one page of
-// one slot and head at a time: no other one changes its bounds.
+// one slot and head at a time: no other one changes its bounds.  Only where several tokens bring bounds, or
+// are selected for in this call; otherwise the kernels that attend put tokens on their rows, which spares
+// a launch (64 slots' single tokens: 294 us before, 281 since).  Latency is all of it: 173 packed tokens
+// of 6 slots, 4 heads of 96 columns, 7.6 us.
 template <typename T, bool WHOLE>
 __global__ __launch_bounds__(kThreads) void paged_append_kernel(PagedArgs<T> a) {
   __shared__ float lows[kMostWidth], highs[kMostWidth];
@@ -465,6 +468,15 @@ __device__ __forceinline__ bool clear_wild(Piece& piece) {
 // the waves take in turn; every wave has a softmax of its own, and the waves are joined at the end.
 // Keys go from memory to the operands of the products, values through LDS, which transposes them.
 // With `lists` the keys are those of the pages in a token's list, one behind the other.
+//
+// Every key and value is read once for all members of the group, a tile ahead of its use, and reads are
+// what bounds it (a copy of 2 GiB moves 4.9 TB/s): 64 slots of up to 9000 tokens, 8 heads of 128, bf16,
+// 1.45 GB in 265 us, 5.5 TB/s; two slots of up to 200000, 2 heads of 64, fp16, 187 MB in 34 us; 33 pages
+// of 64 for each of 32 slots, 8 heads of 128, 277 MB in 45 us, 6.1 TB/s.  One slot of 512 tokens in
+// float32 takes 8.7 us: the way from the lengths to the table, the page and through the waves' softmaxes.
+// Waves have keys of their own because 16 rows are one operand: sharing rows out would leave three of
+// them without work.  Two sixteens of rows (drafts of 5 tokens, 4 heads on one) took 62 us, and the
+// kernel for many rows takes 49.
 template <typename T, int WIDTH, bool WHOLE>
 __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(kWaves<T, WIDTH, WHOLE>))) void
 paged_token_kernel(PagedArgs<T> a) {
@@ -787,6 +799,17 @@ paged_token_kernel(PagedArgs<T> a) {
 // of 64, which go through registers to LDS while the tile before is worked on; queries and sums stay in
 // registers.  USED: the columns that keys and values have at most (tiles have WIDTH).  Weights are
 // rounded to the inputs' type, as the operand of the product with the values, and summed as rounded.
+//
+// Four prompts of 2048 tokens behind up to 2500, 32 heads on 8 of 128 columns, bf16 (403 GFLOP): 430 to
+// 455 us, 890 TFLOP/s (a product of 8192 x 8192 x 8192 by the library: 1290).  LDS bounds it: a wave reads
+// all of both tiles, 32 KB, for its 32 rows; matrix pipes are busy for 38 % of the time, vector ones for
+// 43 %, two waves to a SIMD.  With operands read ahead of their products 476 us became 470.  Tried and not kept: the next half tile's scores
+// among the exponentials of this one, 588; eight waves for 256 rows in two teams, one with matrix
+// instructions while the other has vector ones, 497 to 669, as all eight read as much of LDS again.
+// Drafts of 5 tokens for 16 slots of up to 4096 (64 rows): 178 MB in 33 us, 5.4 TB/s.  Packed prompts of
+// 1 to 2047 tokens behind up to 3001 (12 heads on 4 of 80 columns, fp16, 38 GFLOP): 120 us, for portions
+// of unequal length (of 512 places for blocks the one that ends last has 1.4 times the mean) and columns
+// padded from 80 to 96.
 template <typename T, int WIDTH, int USED, int QUERIES, bool WHOLE>
 __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(kWaves<T, WIDTH, WHOLE>))) void
 paged_chunk_kernel(PagedArgs<T> a) {
@@ -1074,7 +1097,8 @@ paged_chunk_kernel(PagedArgs<T> a) {
 // ---------------------------------------------------------------------------
 
 // The parts of the first `unit_rows` rows of every tile.  Of few rows there may be many parts: a block
-// has a row, and its threads four columns of some parts each.
+// has a row, and its threads four columns of some parts each.  Four dependent reads of latency: 4 us for
+// one slot, 8 us for 64 slots with 2048 rows, of 20 MB of parts.
 template <typename T, int WIDTH>
 __global__ __launch_bounds__(kThreads) void paged_join_few_kernel(PagedArgs<T> a, int tile_rows, int unit_rows) {
   constexpr int kOuts = WIDTH + 4, kLanes = WIDTH / 4, kTeams = kThreads / kLanes;
@@ -1109,7 +1133,7 @@ __global__ __launch_bounds__(kThreads) void paged_join_few_kernel(PagedArgs<T> a
     __syncthreads();
     f32x4 value = f32x4(0.0f);
 #pragma unroll 4
-    for (int s = team; s < task.splits; s += kTeams)
+    for (int s = team; s < (col < a.value_width ? task.splits : 0); s += kTeams)
       value += weights[s] * *reinterpret_cast<const f32x4*>(parts + s * apart + col);
     *reinterpret_cast<f32x4*>(&sums[team][col]) = value;
     __syncthreads();
@@ -1127,7 +1151,8 @@ __global__ __launch_bounds__(kThreads) void paged_join_few_kernel(PagedArgs<T> a
 }
 
 // Of many rows there are few parts each: a thread has four columns of a row, and takes four parts at
-// once, so that their loads are under way together.
+// once, so that their loads are under way together: 6 us for 16 slots of 20 rows and 8 heads, 17 us for
+// 59 MB of parts of packed prompts, which come from memory (3.5 TB/s).
 template <typename T, int WIDTH>
 __global__ __launch_bounds__(kThreads) void paged_join_many_kernel(PagedArgs<T> a, int tile_rows) {
   constexpr int kOuts = WIDTH + 4, kAtOnce = 4, kLanes = WIDTH / 4, kTeams = kThreads / kLanes;
@@ -1139,7 +1164,7 @@ __global__ __launch_bounds__(kThreads) void paged_join_many_kernel(PagedArgs<T> 
     const int64_t tile = unit / tile_rows;
     const PagedTask task = a.division.tasks[tile / a.kv_heads];
     const int kv_head = static_cast<int>(tile % a.kv_heads), r = static_cast<int>(unit % tile_rows);
-    if (r >= task.rows) continue;
+    if (r >= task.rows || col >= a.value_width) continue;
     const float* parts = a.division.partial +
                          ((static_cast<int64_t>(kv_head) * a.division.parts + task.part) * tile_rows + r) * kOuts;
     float top = -__builtin_inff(), total = 0.0f;
@@ -1225,6 +1250,10 @@ __device__ __forceinline__ double over_lanes_sum(double x) {
 // The largest product that a key within a page's bounds can have with a query of the group, in 64 bits,
 // in which the products are exact: pages are ranked as their bounds rank, whatever the order of a sum.
 // A lane has the queries' elements of its columns in registers for all pages; the lanes of a page add up.
+// Vector instructions in 64 bits bound it, and the latency of a page's number and bounds, which four pages
+// at once hide: 32 slots of up to 256 pages, 32 heads on 8 of 128 columns, bf16, 15.5 us (one page at
+// once 19; a page to a lane with queries in LDS 13.5 to 19, and far slower for few pages; a lane for some
+// columns of all heads 26); two slots of 3125 pages 11 us; 173 packed tokens of up to 188 pages 19 us.
 template <typename T, bool WHOLE>
 __global__ __launch_bounds__(kThreads) void paged_score_kernel(PagedArgs<T> a, int blocks_of_token) {
   constexpr int kElements = 16 / static_cast<int>(sizeof(T)), kMembers = 4;
@@ -1330,7 +1359,8 @@ __device__ __forceinline__ uint64_t rank_of(double score) {
 // The pages of a token and head of keys: the `count` with the largest scores, in the order of the
 // slot's table, and its own; and how many positions it sees on them.  A block finds the score of the
 // last one that is selected eight bits at a time, by counting, of many pages from the first bit on in
-// which scores differ.
+// which scores differ.  Barriers bound it: 256 lists of up to 256 pages 6.5 us; 4 lists of 3125 pages, by
+// 1024 threads, 13 us.
 template <typename T, int THREADS>
 __global__ __launch_bounds__(THREADS) void paged_select_kernel(PagedArgs<T> a) {
   constexpr int kAll = THREADS / 64;

@@ -54,6 +54,7 @@ PagedPlan paged_plan(const rosa_mixer_problem& p, const rosa_paged_cache& cache,
     const int64_t blocks = tiles * p.Hkv;
     few.target = static_cast<int>(
         std::max<int64_t>(1, std::min((kBlocks + blocks - 1) / blocks, walk / 8)));
+    few.tiles = tiles;
     few.items = tiles * few.target;
     few.parts = few.target > 1 ? few.items : 0;
     few.unit_rows = std::min(few.rows, share);
@@ -78,6 +79,7 @@ PagedPlan paged_plan(const rosa_mixer_problem& p, const rosa_paged_cache& cache,
     few.least = 4;
     few.round = 7;
     few.unit_rows = packed ? few.rows : static_cast<int>(rows);
+    few.tiles = sequences;
     few.items = sequences + few.target;
     few.parts = (capacity + 31) / 32 > few.least ? 2 * few.target : 0;
     finish(&few);
@@ -94,6 +96,8 @@ PagedPlan paged_plan(const rosa_mixer_problem& p, const rosa_paged_cache& cache,
     many.target = ((packed ? kPackedPortions : kManyPortions) + p.Hkv - 1) / p.Hkv;
     many.least = 4;
     many.round = packed ? 7 : 3;
+    many.unit_rows = packed ? many.rows : static_cast<int>(std::min<int64_t>(many.rows, rows));
+    many.tiles = tiles;
     many.items = tiles + many.target;
     many.parts = (capacity + 63) / 64 > many.least ? 2 * many.target : 0;
     finish(&many);

@@ -801,9 +801,10 @@ paged_token_kernel(PagedArgs<T> a) {
 // rounded to the inputs' type, as the operand of the product with the values, and summed as rounded.
 //
 // Four prompts of 2048 tokens behind up to 2500, 32 heads on 8 of 128 columns, bf16 (403 GFLOP): 430 to
-// 455 us, 890 TFLOP/s (a product of 8192 x 8192 x 8192 by the library: 1290).  LDS bounds it: a wave reads
-// all of both tiles, 32 KB, for its 32 rows; matrix pipes are busy for 38 % of the time, vector ones for
-// 43 %, two waves to a SIMD.  With operands read ahead of their products 476 us became 470.  Tried and not kept: the next half tile's scores
+// 455 us, 890 TFLOP/s (a product of 8192 x 8192 x 8192 by the library: 1290).  No pipe is full: matrix ones are
+// busy for 39 % of the time, vector ones issue for 45 %, LDS works for 27 % (a wave reads all of both
+// tiles, 32 KB, for its 32 rows); the registers hold two waves to a SIMD, which wait for operands and for
+// one another's pipes.  With operands read ahead of their products 476 us became 470.  Tried and not kept: the next half tile's scores
 // among the exponentials of this one, 588; eight waves for 256 rows in two teams, one with matrix
 // instructions while the other has vector ones, 497 to 669, as all eight read as much of LDS again.
 // Drafts of 5 tokens for 16 slots of up to 4096 (64 rows): 178 MB in 33 us, 5.4 TB/s.  Packed prompts of
@@ -1098,7 +1099,7 @@ paged_chunk_kernel(PagedArgs<T> a) {
 
 // The parts of the first `unit_rows` rows of every tile.  Of few rows there may be many parts: a block
 // has a row, and its threads four columns of some parts each.  Four dependent reads of latency: 4 us for
-// one slot, 8 us for 64 slots with 2048 rows, of 20 MB of parts.
+// one slot, 8 us for 64 slots with 2048 rows, and for 32 rows of 380 parts each.
 template <typename T, int WIDTH>
 __global__ __launch_bounds__(kThreads) void paged_join_few_kernel(PagedArgs<T> a, int tile_rows, int unit_rows) {
   constexpr int kOuts = WIDTH + 4, kLanes = WIDTH / 4, kTeams = kThreads / kLanes;
@@ -1150,20 +1151,20 @@ __global__ __launch_bounds__(kThreads) void paged_join_few_kernel(PagedArgs<T> a
   }
 }
 
-// Of many rows there are few parts each: a thread has four columns of a row, and takes four parts at
-// once, so that their loads are under way together: 6 us for 16 slots of 20 rows and 8 heads, 17 us for
-// 59 MB of parts of packed prompts, which come from memory (3.5 TB/s).
+// The same of many rows.  There are few parts each: a thread has four columns of a row, and takes four parts at
+// once, so that their loads are under way together: 5 us for 16 slots of 20 rows and 8 heads, 17 us for
+// 51 MB of parts of packed prompts, which come from memory (3.4 TB/s).
 template <typename T, int WIDTH>
-__global__ __launch_bounds__(kThreads) void paged_join_many_kernel(PagedArgs<T> a, int tile_rows) {
+__global__ __launch_bounds__(kThreads) void paged_join_many_kernel(PagedArgs<T> a, int tile_rows, int unit_rows) {
   constexpr int kOuts = WIDTH + 4, kAtOnce = 4, kLanes = WIDTH / 4, kTeams = kThreads / kLanes;
   const int col = threadIdx.x % kLanes * 4, team = threadIdx.x / kLanes;
-  const int64_t units = static_cast<int64_t>(*a.division.task_count) * a.kv_heads * tile_rows;
+  const int64_t units = static_cast<int64_t>(*a.division.task_count) * a.kv_heads * unit_rows;
   const int64_t apart = static_cast<int64_t>(tile_rows) * kOuts;
   for (int64_t unit = static_cast<int64_t>(blockIdx.x) * kTeams + team; unit < units;
        unit += static_cast<int64_t>(gridDim.x) * kTeams) {
-    const int64_t tile = unit / tile_rows;
+    const int64_t tile = unit / unit_rows;
     const PagedTask task = a.division.tasks[tile / a.kv_heads];
-    const int kv_head = static_cast<int>(tile % a.kv_heads), r = static_cast<int>(unit % tile_rows);
+    const int kv_head = static_cast<int>(tile % a.kv_heads), r = static_cast<int>(unit % unit_rows);
     if (r >= task.rows || col >= a.value_width) continue;
     const float* parts = a.division.partial +
                          ((static_cast<int64_t>(kv_head) * a.division.parts + task.part) * tile_rows + r) * kOuts;
@@ -1251,11 +1252,15 @@ __device__ __forceinline__ double over_lanes_sum(double x) {
 // in which the products are exact: pages are ranked as their bounds rank, whatever the order of a sum.
 // A lane has the queries' elements of its columns in registers for all pages; the lanes of a page add up.
 // Vector instructions in 64 bits bound it, and the latency of a page's number and bounds, which four pages
-// at once hide: 32 slots of up to 256 pages, 32 heads on 8 of 128 columns, bf16, 15.5 us (one page at
+// at once hide: 32 slots of up to 256 pages, 32 heads on 8 of 128 columns, bf16, 15.2 us (one page at
 // once 19; a page to a lane with queries in LDS 13.5 to 19, and far slower for few pages; a lane for some
-// columns of all heads 26); two slots of 3125 pages 11 us; 173 packed tokens of up to 188 pages 19 us.
-template <typename T, bool WHOLE>
-__global__ __launch_bounds__(kThreads) void paged_score_kernel(PagedArgs<T> a, int blocks_of_token) {
+// columns of all heads 26; three waves to a SIMD 17.5); 173 packed tokens of up to 188 pages 17.5 us.
+// ONE: the group has at most four members, whose queries are loaded once.  More are loaded again for
+// every turn of pages, whose bounds and best scores stay in registers: two slots of 3125 pages, 16 heads
+// on 2, 9.6 us (11.8 with best scores in memory from one four to the next).
+template <typename T, bool WHOLE, bool ONE>
+__global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(ONE && WHOLE ? 4 : 2))) void
+paged_score_kernel(PagedArgs<T> a, int blocks_of_token) {
   constexpr int kElements = 16 / static_cast<int>(sizeof(T)), kMembers = 4;
   constexpr int kLanes = kMostWidth / kElements, kPages = kThreads / kLanes, kTurns = 4;  // of a page; at once
   typedef T Piece __attribute__((ext_vector_type(kElements)));
@@ -1280,9 +1285,9 @@ __global__ __launch_bounds__(kThreads) void paged_score_kernel(PagedArgs<T> a, i
   const int col = tid % kLanes * kElements;
   // (lanes behind the last column have queries of zero, some other bounds, and sums that are left out)
   const int from = min(col, WHOLE ? a.key_width - kElements : a.key_width - 1);
-  for (int member0 = 0; member0 < a.share; member0 += kMembers) {
+  double queries[kMembers][kElements];
+  const auto fetch_queries = [&](int member0) {
     const int members = min(kMembers, a.share - member0);
-    double queries[kMembers][kElements];
 #pragma unroll
     for (int m = 0; m < kMembers; ++m) {
       const int head = kv_head * a.share + member0 + min(m, members - 1);
@@ -1299,32 +1304,39 @@ __global__ __launch_bounds__(kThreads) void paged_score_kernel(PagedArgs<T> a, i
       for (int e = 0; e < kElements; ++e)
         queries[m][e] = col + e < a.key_width ? static_cast<double>(static_cast<float>(part[e])) : 0.0;
     }
-    const int step = blocks_of_token * kPages * kTurns;
-    for (int base = static_cast<int>(block % blocks_of_token) * kPages * kTurns; base < earlier; base += step) {
-      int id[kTurns];
-      Piece lows[kTurns], highs[kTurns];
+  };
+  const int step = blocks_of_token * kPages * kTurns;
+  const int start = static_cast<int>(block % blocks_of_token) * kPages * kTurns;
+  fetch_queries(0);
+  for (int base = start; base < earlier; base += step) {
+    int id[kTurns];
+    Piece lows[kTurns], highs[kTurns];
 #pragma unroll
-      for (int i = 0; i < kTurns; ++i) id[i] = table[min(base + i * kPages + tid / kLanes, earlier - 1)];
+    for (int i = 0; i < kTurns; ++i) id[i] = table[min(base + i * kPages + tid / kLanes, earlier - 1)];
 #pragma unroll
-      for (int i = 0; i < kTurns; ++i) {
-        const T* low = a.key_bounds +
-                       (static_cast<int64_t>(a.is_page(id[i]) ? id[i] : 0) * a.kv_heads + kv_head) * 2 * a.key_width;
-        const T* high = low + a.key_width;
-        if constexpr (WHOLE) {
-          lows[i] = *reinterpret_cast<const Piece*>(low + from);
-          highs[i] = *reinterpret_cast<const Piece*>(high + from);
-        } else {
+    for (int i = 0; i < kTurns; ++i) {
+      const T* low = a.key_bounds +
+                     (static_cast<int64_t>(a.is_page(id[i]) ? id[i] : 0) * a.kv_heads + kv_head) * 2 * a.key_width;
+      const T* high = low + a.key_width;
+      if constexpr (WHOLE) {
+        lows[i] = *reinterpret_cast<const Piece*>(low + from);
+        highs[i] = *reinterpret_cast<const Piece*>(high + from);
+      } else {
 #pragma unroll
-          for (int e = 0; e < kElements; ++e) {
-            const bool there = from + e < a.key_width;
-            lows[i][e] = there ? low[from + e] : static_cast<T>(0.0f);
-            highs[i][e] = there ? high[from + e] : static_cast<T>(0.0f);
-          }
+        for (int e = 0; e < kElements; ++e) {
+          const bool there = from + e < a.key_width;
+          lows[i][e] = there ? low[from + e] : static_cast<T>(0.0f);
+          highs[i][e] = there ? high[from + e] : static_cast<T>(0.0f);
         }
       }
+    }
+    double best[kTurns];
+#pragma unroll
+    for (int i = 0; i < kTurns; ++i) best[i] = -__builtin_inf();
+    for (int member0 = 0; member0 < (ONE ? 1 : a.share); member0 += kMembers) {
+      if (!ONE && (base > start || member0 > 0)) fetch_queries(member0);
 #pragma unroll
       for (int i = 0; i < kTurns; ++i) {
-        const int page = base + i * kPages + tid / kLanes;
         if (base + i * kPages >= earlier) break;
         double sum[kMembers] = {};
 #pragma unroll
@@ -1337,12 +1349,11 @@ __global__ __launch_bounds__(kThreads) void paged_score_kernel(PagedArgs<T> a, i
 #pragma unroll
         for (int m = 0; m < kMembers; ++m)  // (zero times infinity is no number)
           sum[m] = over_lanes_sum<kLanes>(col < a.key_width ? sum[m] : 0.0);
-        if (tid % kLanes == 0 && page < earlier) {
-          double best = member0 > 0 ? scores[page] : -__builtin_inf();
 #pragma unroll
-          for (int m = 0; m < kMembers; ++m) best = sum[m] > best || sum[m] != sum[m] ? sum[m] : best;
-          scores[page] = a.is_page(id[i]) ? best : __builtin_nan("");
-        }
+        for (int m = 0; m < kMembers; ++m) best[i] = sum[m] > best[i] || sum[m] != sum[m] ? sum[m] : best[i];
+        const int page = base + i * kPages + tid / kLanes;
+        if ((ONE || member0 + kMembers >= a.share) && tid % kLanes == 0 && page < earlier)
+          scores[page] = a.is_page(id[i]) ? best[i] : __builtin_nan("");
       }
     }
   }
@@ -1358,9 +1369,10 @@ __device__ __forceinline__ uint64_t rank_of(double score) {
 
 // The pages of a token and head of keys: the `count` with the largest scores, in the order of the
 // slot's table, and its own; and how many positions it sees on them.  A block finds the score of the
-// last one that is selected eight bits at a time, by counting, of many pages from the first bit on in
-// which scores differ.  Barriers bound it: 256 lists of up to 256 pages 6.5 us; 4 lists of 3125 pages, by
-// 1024 threads, 13 us.
+// last one that is selected eight bits at a time, by counting, from the first bit on in which scores
+// differ (before it all of them would count in one place), and keeps four scores a thread in registers.
+// Barriers bound it: 256 lists of up to 256 pages 6 us; 4 lists of 3125 pages, by 1024 threads, 11.7 us
+// (13.2 where every pass read the scores).
 template <typename T, int THREADS>
 __global__ __launch_bounds__(THREADS) void paged_select_kernel(PagedArgs<T> a) {
   constexpr int kAll = THREADS / 64;
@@ -1389,35 +1401,37 @@ __global__ __launch_bounds__(THREADS) void paged_select_kernel(PagedArgs<T> a) {
     return;
   }
   const double* scores = a.scores + at * a.columns;
-  // the pages in turns of a block's threads, for all threads
+  // the pages in turns of a block's threads, for all threads; a few turns stay in registers
+  constexpr int kHeld = 4;
+  uint64_t held[kHeld];
+#pragma unroll
+  for (int i = 0; i < kHeld; ++i) held[i] = rank_of(scores[min(i * THREADS + tid, earlier - 1)]);
   const auto for_each = [&](auto&& visit) {
-    for (int base = 0; base < earlier; base += THREADS)
+#pragma unroll
+    for (int i = 0; i < kHeld; ++i)
+      if (i * THREADS < earlier) visit(i * THREADS + tid, held[i]);
+    for (int base = kHeld * THREADS; base < earlier; base += THREADS)
       visit(base + tid, rank_of(scores[min(base + tid, earlier - 1)]));
   };
-  // (of a few pages the first bits are not worth finding out)
-  uint64_t low = 0, high = ~uint64_t{0};
-  if (earlier > 1024) {
-    low = ~uint64_t{0};
-    high = 0;
-    for_each([&](int j, uint64_t rank) {
-      if (j < earlier) {
-        low = min(low, rank);
-        high = max(high, rank);
-      }
-    });
-    for (int away = 1; away < 64; away *= 2) {
-      low = min(low, static_cast<uint64_t>(__shfl_xor(static_cast<unsigned long long>(low), away)));
-      high = max(high, static_cast<uint64_t>(__shfl_xor(static_cast<unsigned long long>(high), away)));
+  uint64_t low = ~uint64_t{0}, high = 0;
+  for_each([&](int j, uint64_t rank) {
+    if (j < earlier) {
+      low = min(low, rank);
+      high = max(high, rank);
     }
-    if (lane == 0) {
-      lowest[wave] = low;
-      highest[wave] = high;
-    }
-    __syncthreads();
-    for (int w = 0; w < kAll; ++w) {
-      low = min(low, lowest[w]);
-      high = max(high, highest[w]);
-    }
+  });
+  for (int away = 1; away < 64; away *= 2) {
+    low = min(low, static_cast<uint64_t>(__shfl_xor(static_cast<unsigned long long>(low), away)));
+    high = max(high, static_cast<uint64_t>(__shfl_xor(static_cast<unsigned long long>(high), away)));
+  }
+  if (lane == 0) {
+    lowest[wave] = low;
+    highest[wave] = high;
+  }
+  __syncthreads();
+  for (int w = 0; w < kAll; ++w) {
+    low = min(low, lowest[w]);
+    high = max(high, highest[w]);
   }
   // those above `prefix` in the bits of `mask` are selected, and the first `need` of those equal to it
   int bits = low == high ? 0 : 64 - __clzll(low ^ high);  // that are not yet known
@@ -1533,8 +1547,7 @@ void paged_token_launch(PagedArgs<T>& args, const PagedShare& share, hipStream_t
   const dim3 grid = grid_of(share.items * args.kv_heads);
   paged_token_kernel<T, WIDTH, WHOLE><<<grid, kThreads, 0, stream>>>(args);
   if (share.parts == 0) return;
-  // (a cut tile has two parts or more)
-  const int64_t units = share.parts / 2 * args.kv_heads * share.unit_rows;
+  const int64_t units = share.cut() * args.kv_heads * share.unit_rows;
   paged_join_few_kernel<T, WIDTH>
       <<<dim3(static_cast<unsigned>(std::min<int64_t>(units, kJoinBlocks))), kThreads, 0, stream>>>(
           args, share.rows, share.unit_rows);
@@ -1561,9 +1574,10 @@ void paged_chunk_launch(PagedArgs<T>& args, const PagedShare& share, hipStream_t
     paged_chunk_rows<T, WIDTH, WIDTH, WHOLE>(args, share, stream);
   }
   if (share.parts == 0) return;
-  const int64_t blocks = share.parts / 2 * args.kv_heads * share.rows * (WIDTH / 4) / kThreads;
+  const int64_t blocks = (share.cut() * args.kv_heads * share.unit_rows * (WIDTH / 4) - 1) / kThreads + 1;
   paged_join_many_kernel<T, WIDTH>
-      <<<dim3(static_cast<unsigned>(std::min<int64_t>(blocks, kJoinBlocks))), kThreads, 0, stream>>>(args, share.rows);
+      <<<dim3(static_cast<unsigned>(std::min<int64_t>(blocks, kJoinBlocks))), kThreads, 0, stream>>>(
+          args, share.rows, share.unit_rows);
 }
 
 template <typename T, bool WHOLE>
@@ -1589,7 +1603,10 @@ void paged_select_launch(PagedArgs<T>& args, const PagedPlan& plan, hipStream_t 
       const int64_t at_once = 4 * kThreads / (kMostWidth * sizeof(T) / 16);
       const int64_t most = (args.columns + at_once - 1) / at_once;
       const int blocks = static_cast<int>(std::max<int64_t>(1, std::min(most, kScoreBlocks / pairs)));
-      paged_score_kernel<T, WHOLE><<<grid_of(pairs * blocks), kThreads, 0, stream>>>(args, blocks);
+      if (args.share <= 4)
+        paged_score_kernel<T, WHOLE, true><<<grid_of(pairs * blocks), kThreads, 0, stream>>>(args, blocks);
+      else
+        paged_score_kernel<T, WHOLE, false><<<grid_of(pairs * blocks), kThreads, 0, stream>>>(args, blocks);
     }
     // (few long lists: all the threads that a block can have)
     if (pairs <= 256 && args.columns > 1024)

@@ -20,10 +20,13 @@ struct PagedShare {
   int target;            // portions of a head of keys that a call is cut into, beside one for each tile
   int least;             // tiles of keys of a portion, at least
   int round;             // eighths of a portion from which on a walk has one more
+  int64_t tiles;         // of rows, at most
   int64_t items;         // portions of a head of keys, at most
   int64_t parts;         // portions of tiles that are cut, at most: those with partial sums
   size_t part_bytes, task_bytes;
   size_t bytes() const { return part_bytes + task_bytes; }
+  // tiles that are cut, at most: each has two parts or more
+  int64_t cut() const { return parts / 2 < tiles ? parts / 2 : tiles; }
 };
 
 struct PagedPlan {

@@ -114,10 +114,6 @@ __device__ __forceinline__ int scan_wave(int x) {
   x += __builtin_amdgcn_update_dpp(0, x, 0x143, 0xc, 0xf, true);  // lane 31
   return x;
 }
-__device__ __forceinline__ float over_wave_float(float x) {
-  for (int away = 1; away < 64; away *= 2) x += __shfl_xor(x, away);
-  return x;
-}
 // The sum over a wave of numbers below 2^62.
 __device__ __forceinline__ int64_t over_wave_sum(int64_t x) {
   int64_t sum = 0;
@@ -1097,16 +1093,55 @@ paged_chunk_kernel(PagedArgs<T> a) {
 // tiles that were cut
 // ---------------------------------------------------------------------------
 
+// What a thread has of parts first, first + STEP, ... of a row: its four columns, relative to the maximum.
+struct PartSum {
+  f32x4 value;
+  float top, total;
+};
+// Four parts at once, so that their loads are under way together.  Columns from `used` on are left out.
+template <int STEP>
+__device__ __forceinline__ PartSum join_parts(const float* parts, int64_t apart, int first, int splits, int width,
+                                              int col, int used) {
+  constexpr int kAtOnce = 4;
+  PartSum sum = {f32x4(0.0f), -__builtin_inff(), 0.0f};
+  col = min(col, (used - 1) & ~3);
+  for (; first < splits; first += kAtOnce * STEP) {
+    float tops[kAtOnce], totals[kAtOnce];
+    f32x4 values[kAtOnce];
+#pragma unroll
+    for (int s = 0; s < kAtOnce; ++s) {
+      const float* part = parts + min(first + s * STEP, splits - 1) * apart;
+      tops[s] = part[width];
+      totals[s] = part[width + 1];
+      values[s] = *reinterpret_cast<const f32x4*>(part + col);
+    }
+    float larger = sum.top;
+#pragma unroll
+    for (int s = 0; s < kAtOnce; ++s) larger = fmaxf(larger, tops[s]);
+    const float base = larger == -__builtin_inff() ? 0.0f : larger, shrink = exp2_of(sum.top - base);
+    sum.top = larger;
+    sum.total *= shrink;
+    sum.value *= shrink;
+#pragma unroll
+    for (int s = 0; s < kAtOnce; ++s)
+      if (first + s * STEP < splits) {
+        const float by = exp2_of(tops[s] - base);
+        sum.total += by * totals[s];
+        sum.value += by * values[s];
+      }
+  }
+  return sum;
+}
+
 // The parts of the first `unit_rows` rows of every tile.  Of few rows there may be many parts: a block
-// has a row, and its threads four columns of some parts each.  Four dependent reads of latency: 4 us for
-// one slot, 8 us for 64 slots with 2048 rows, and for 32 rows of 380 parts each.
+// has a row, and its threads four columns of some parts each.  Latency: 3.4 us for one slot, 5.1 us for 64
+// slots with 2048 rows, 5.9 for 32 rows of 380 parts each (8.4 with the parts' maxima read before the rest).
 template <typename T, int WIDTH>
 __global__ __launch_bounds__(kThreads) void paged_join_few_kernel(PagedArgs<T> a, int tile_rows, int unit_rows) {
   constexpr int kOuts = WIDTH + 4, kLanes = WIDTH / 4, kTeams = kThreads / kLanes;
   __shared__ __attribute__((aligned(16))) float sums[kTeams][WIDTH];
-  __shared__ float weights[kMostPortions], tops[4], totals[4];
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  const int col = tid % kLanes * 4, team = tid / kLanes;
+  __shared__ float tops[kTeams], totals[kTeams];
+  const int tid = threadIdx.x, col = tid % kLanes * 4, team = tid / kLanes;
   const int64_t units = static_cast<int64_t>(*a.division.task_count) * a.kv_heads * unit_rows;
   const int64_t apart = static_cast<int64_t>(tile_rows) * kOuts;
   for (int64_t unit = blockIdx.x; unit < units; unit += gridDim.x) {
@@ -1115,48 +1150,35 @@ __global__ __launch_bounds__(kThreads) void paged_join_few_kernel(PagedArgs<T> a
     if (r >= task.rows) continue;
     const float* parts = a.division.partial +
                          ((static_cast<int64_t>(kv_head) * a.division.parts + task.part) * tile_rows + r) * kOuts;
-    float top = -__builtin_inff(), total = 0.0f;
-    for (int s = tid; s < task.splits; s += kThreads) {
-      weights[s] = parts[s * apart + WIDTH];
-      top = fmaxf(top, weights[s]);
+    const PartSum sum = join_parts<kTeams>(parts, apart, team, task.splits, WIDTH, col, a.value_width);
+    *reinterpret_cast<f32x4*>(&sums[team][col]) = sum.value;
+    if (col == 0) {
+      tops[team] = sum.top;
+      totals[team] = sum.total;
     }
-    for (int away = 1; away < 64; away *= 2) top = fmaxf(top, __shfl_xor(top, away));
-    if (lane == 0) tops[wave] = top;
-    __syncthreads();
-    top = fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3]));
-    for (int s = tid; s < task.splits; s += kThreads) {
-      const float by = top == -__builtin_inff() ? 1.0f : exp2_of(weights[s] - top);
-      weights[s] = by;
-      total += by * parts[s * apart + WIDTH + 1];
-    }
-    total = over_wave_float(total);
-    if (lane == 0) totals[wave] = total;
-    __syncthreads();
-    f32x4 value = f32x4(0.0f);
-#pragma unroll 4
-    for (int s = team; s < (col < a.value_width ? task.splits : 0); s += kTeams)
-      value += weights[s] * *reinterpret_cast<const f32x4*>(parts + s * apart + col);
-    *reinterpret_cast<f32x4*>(&sums[team][col]) = value;
     __syncthreads();
     if (tid < a.value_width) {
-      const int teams = min(kTeams, task.splits);
-      float all = sums[0][tid];
-      for (int t = 1; t < teams; ++t) all += sums[t][tid];
+      float top = tops[0], total = 0.0f, value = 0.0f;
+      for (int t = 1; t < kTeams; ++t) top = fmaxf(top, tops[t]);
+      const float base = top == -__builtin_inff() ? 0.0f : top;
+      for (int t = 0; t < kTeams; ++t) {
+        const float by = exp2_of(tops[t] - base);
+        total += by * totals[t];
+        value += by * sums[t][tid];
+      }
       const int row = task.row + r, token = row / a.share;
       const int64_t at = (task.first + token) * a.heads + kv_head * a.share + row - token * a.share;
-      a.out[at * a.value_width + tid] =
-          static_cast<T>(all / (totals[0] + totals[1] + totals[2] + totals[3]));
+      a.out[at * a.value_width + tid] = static_cast<T>(value / total);
     }
     __syncthreads();
   }
 }
 
-// The same of many rows.  There are few parts each: a thread has four columns of a row, and takes four parts at
-// once, so that their loads are under way together: 5 us for 16 slots of 20 rows and 8 heads, 17 us for
-// 51 MB of parts of packed prompts, which come from memory (3.4 TB/s).
+// The same of many rows, which have few parts each: a thread has four columns of a row.  5 us for 16
+// slots of 20 rows and 8 heads, 14 us for 51 MB of parts of packed prompts, which come from memory (4 TB/s).
 template <typename T, int WIDTH>
 __global__ __launch_bounds__(kThreads) void paged_join_many_kernel(PagedArgs<T> a, int tile_rows, int unit_rows) {
-  constexpr int kOuts = WIDTH + 4, kAtOnce = 4, kLanes = WIDTH / 4, kTeams = kThreads / kLanes;
+  constexpr int kOuts = WIDTH + 4, kLanes = WIDTH / 4, kTeams = kThreads / kLanes;
   const int col = threadIdx.x % kLanes * 4, team = threadIdx.x / kLanes;
   const int64_t units = static_cast<int64_t>(*a.division.task_count) * a.kv_heads * unit_rows;
   const int64_t apart = static_cast<int64_t>(tile_rows) * kOuts;
@@ -1168,36 +1190,10 @@ __global__ __launch_bounds__(kThreads) void paged_join_many_kernel(PagedArgs<T> 
     if (r >= task.rows || col >= a.value_width) continue;
     const float* parts = a.division.partial +
                          ((static_cast<int64_t>(kv_head) * a.division.parts + task.part) * tile_rows + r) * kOuts;
-    float top = -__builtin_inff(), total = 0.0f;
-    f32x4 value = f32x4(0.0f);
-    for (int first = 0; first < task.splits; first += kAtOnce) {
-      float tops[kAtOnce], totals[kAtOnce];
-      f32x4 values[kAtOnce];
-#pragma unroll
-      for (int s = 0; s < kAtOnce; ++s) {
-        const float* part = parts + min(first + s, task.splits - 1) * apart;
-        tops[s] = part[WIDTH];
-        totals[s] = part[WIDTH + 1];
-        values[s] = *reinterpret_cast<const f32x4*>(part + col);
-      }
-      float larger = top;
-#pragma unroll
-      for (int s = 0; s < kAtOnce; ++s) larger = fmaxf(larger, tops[s]);
-      const float base = larger == -__builtin_inff() ? 0.0f : larger, shrink = exp2_of(top - base);
-      top = larger;
-      total *= shrink;
-      value *= shrink;
-#pragma unroll
-      for (int s = 0; s < kAtOnce; ++s)
-        if (first + s < task.splits) {
-          const float by = exp2_of(tops[s] - base);
-          total += by * totals[s];
-          value += by * values[s];
-        }
-    }
+    const PartSum sum = join_parts<1>(parts, apart, 0, task.splits, WIDTH, col, a.value_width);
     const int row = task.row + r, token = row / a.share;
     T* out = a.out + ((task.first + token) * a.heads + kv_head * a.share + row - token * a.share) * a.value_width;
-    store4(out, col, value * (1.0f / total), a.value_width,
+    store4(out, col, sum.value * (1.0f / sum.total), a.value_width,
            a.value_width % 4 == 0 && reinterpret_cast<uintptr_t>(out) % sizeof(Quad<T>) == 0);
   }
 }
@@ -1538,8 +1534,9 @@ PagedDivision division_of(const PagedShare& share, int most_few, char* at) {
   return d;
 }
 
-// Blocks that go on to further work: a thousand more take the chip 4 us to begin, whatever they do.
-constexpr int64_t kJoinBlocks = 1024;
+// Blocks that go on to further work: a thousand more take the chip 4 us to begin, whatever they do.  Those
+// of a join are as many as it can hold at once (51 MB of parts: 1024 of them 17 us, 2048 14, 4096 14).
+constexpr int64_t kJoinBlocks = 2048;
 constexpr int64_t kScoreBlocks = 1024;
 
 template <typename T, int WIDTH, bool WHOLE>

@@ -6,8 +6,6 @@
 
 namespace rosa_mixer {
 
-// Splits of a walk, at most: the join keeps a weight of each in LDS.
-constexpr int kMostPortions = 1024;
 // Slots of the tables that one call changes, at most: a prefix of each is kept in LDS.
 constexpr int kMostTableSlots = 8192;
 constexpr int kMostCount = 1024;  // selected pages of a token

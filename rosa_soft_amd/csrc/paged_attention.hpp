@@ -1025,9 +1025,11 @@ paged_chunk_kernel(PagedArgs<T> a) {
 #pragma unroll
           for (int r = 0; r < 4; ++r) here = fmaxf(here, score[i][k][r]);
         here = over_groups_max(here) * factor;
-        if (__any(here > most[i] + kSlack)) {
-          const float larger = fmaxf(here, most[i]);
-          const float shrink = larger == -__builtin_inff() ? 1.0f : exp2_of(most[i] - larger);
+        // (every row by its own scores: what it does not see leaves its roundings as they are)
+        const bool passed = here > most[i] + kSlack;
+        if (__any(passed)) {
+          const float larger = passed ? here : most[i];
+          const float shrink = passed ? exp2_of(most[i] - larger) : 1.0f;
           sum[i] *= shrink;
 #pragma unroll
           for (int d = 0; d < kCols; ++d) out[i][d] *= shrink;

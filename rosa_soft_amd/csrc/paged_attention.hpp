@@ -440,7 +440,9 @@ __device__ __forceinline__ void put_tokens(const PagedArgs<T>& a, const T* keys,
 // Clears 16 bytes of a value that are not all finite; whether they were not.  A weight of zero would make
 // NaN of them, in rows that do not see them as well: in tiles that not all rows see they are cleared, and
 // rows from their position on become NaN.  (Paid once a block, by the tiles on the diagonal.  Numbers
-// without their sign rank like whole ones: one comparison for all of them.)
+// without their sign rank like whole ones: one comparison for all of them.)  The first of a float32's
+// three bfloat16 parts is infinite from 2^128 - 2^119 on, the middle between bfloat16's largest number
+// and 2^128, and the others are no numbers: float32 counts from there on.
 template <typename T, typename Piece>
 __device__ __forceinline__ bool clear_wild(Piece& piece) {
   typedef uint32_t Words __attribute__((ext_vector_type(4)));
@@ -451,7 +453,7 @@ __device__ __forceinline__ bool clear_wild(Piece& piece) {
     most = max(most, words[i] & 0x7fffffff);
     if constexpr (sizeof(T) == 2) most = max(most, words[i] << 16 & 0x7fffffff);
   }
-  const bool wild = most >= (std::is_same_v<T, _Float16> ? 0x7c000000u : 0x7f800000u);
+  const bool wild = most >= (std::is_same_v<T, _Float16> ? 0x7c000000u : sizeof(T) == 4 ? 0x7f7f8000u : 0x7f800000u);
   if (wild) piece = Piece(static_cast<T>(0.0f));
   return wild;
 }

@@ -28,8 +28,10 @@ depend on the order in which blocks run.
 
 Nothing that is on the device is looked at by the host: invalid ``cu_seqlens`` make every output NaN
 and change nothing, and numbers that are no page are never followed.  Tokens that see a key or a
-value that is not finite may have outputs that are not, in one column or in all; the others keep their
-results.  What no token was put on is never read.
+value that is not finite may have outputs that are not, in one column or in all; the others keep every
+bit of theirs.  In float32 a magnitude of ``2**128 - 2**119`` (3.396e38) or more counts as not finite,
+and in every type sums of weights times values that pass float32's range are.  What no token was put on
+is never read.
 """
 
 from __future__ import annotations

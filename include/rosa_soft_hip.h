@@ -479,7 +479,9 @@ int rosa_hip_page_tables_update(const rosa_page_tables* tables, const int32_t* c
 /*
  * The pages behind the first `keep` tokens (int32 [slots], device) of every slot's `lengths` go back
  * to the pool, the first of them on top (after an update it is what was there before), and their
- * entries become -1; numbers that are no page, and pages beyond the pool's size, are dropped.
+ * entries become -1; numbers that are no page, and pages beyond the pool's size, are dropped.  A page
+ * that the first `keep` tokens of any slot lie on stays with it, and one that several slots give back
+ * goes back once, with the last of them.
  */
 int rosa_hip_page_tables_release(const rosa_page_tables* tables, const int32_t* keep, void* stream);
 

@@ -133,6 +133,10 @@ def page_tables_release(tables: Tensor, lengths: Tensor, keep: Tensor, pool: Ten
     their pages lie on top of the stack, the first slot's first page uppermost, so that a release
     takes back an update.  Entries that are no page are passed over, and so are pages for which the
     pool has no place.  ``lengths`` is left to the caller.
+
+    A page in several tables goes back with the last of them: while the first ``keep`` tokens of any
+    slot lie on it (up to ``lengths``) it stays, and of several slots that give it back in one call the
+    last one does.  A prompt that is kept for later requests has a slot of its own that brings no tokens.
     """
 
     _tables_release(tables, lengths, keep, pool, _integer("page", page))
@@ -164,8 +168,9 @@ def paged_attention_update(query: Tensor, key: Tensor, value: Tensor, key_pages:
     call the new tokens behind it see it like the others, so padding goes behind the real tokens.
     Rejected tokens may leave the bounds of their page wider than its keys.
     A token that sees a position without a page has NaN as its output.
-    Slots may share pages as long as nobody writes to them; a page that is written belongs to one slot,
-    and no two tokens of a call to the same row.
+    Slots may share pages as long as nobody writes to them (a prompt in common: the tables begin with
+    the same numbers); a page that is written belongs to one slot, and no two tokens of a call to the
+    same row.
     """
 
     scale = _number("scale", scale)

@@ -6,7 +6,8 @@ import pytest
 import torch
 
 from rosa_soft_amd import paged
-from tests.test_gpu_paged import DEVICE, DTYPES, Server, i32, offsets_of
+from tests import paged_reference as reference
+from tests.test_gpu_paged import DEVICE, DTYPES, Server, check_tables, i32, offsets_of, shuffled
 
 pytestmark = pytest.mark.gpu
 
@@ -101,3 +102,143 @@ def test_the_largest_numbers_stay_with_those_that_see_them(past, chunk, widths, 
             assert torch.equal(output[0, :token], clean[0, :token])
             assert torch.equal(output[0, :, group:], clean[0, :, group:])
             assert torch.equal(output[1], clean[1])
+
+
+# ---------------------------------------------------------------------------
+# pages that several slots hold
+# ---------------------------------------------------------------------------
+
+def release(want, lengths, keep):
+    """A release of ``want``'s tables in which a page that a slot keeps stays with it, and a page that
+    several slots give back goes back once."""
+    columns = [(want.columns_of(min(max(k, 0), max(n, 0))), want.columns_of(n)) for n, k in zip(lengths, keep)]
+    kept = {entry for row, (begin, _) in zip(want.table, columns) for entry in row[:begin]}
+    for slot in reversed(range(len(want.table))):
+        begin, end = columns[slot]
+        for column in reversed(range(begin, end)):
+            entry, want.table[slot][column] = want.table[slot][column], -1
+            if 0 <= entry < want.pages and entry not in kept:
+                kept.add(entry)
+                if want.free < want.pages:
+                    want.stack[want.free:want.free + 1] = [entry]
+                want.free = min(want.free + 1, want.pages)
+
+
+def share(server, giver, taker, tokens):
+    """A prompt in common: the taker's table begins with the giver's pages."""
+    columns = tokens // server.page
+    assert tokens % server.page == 0 and server.seen[taker] == 0
+    server.tables[taker, :columns] = server.tables[giver, :columns]
+    server.lengths[taker], server.seen[taker] = tokens, tokens
+
+
+def free_pages(pool):
+    pool = pool.tolist()
+    return pool[1:1 + pool[0]]
+
+
+@pytest.mark.parametrize("ends", [0, 1])
+@pytest.mark.parametrize("keep", [0, 40])
+def test_a_page_that_another_slot_keeps_stays_with_it(ends, keep):
+    """One of two slots with a prompt in common ends, or goes back into it; a third takes the pages
+    on top of the stack; the other one's pages and outputs are as they were."""
+    page, prompt = 16, 96
+    stays = 1 - ends
+    server = Server(2100, [prompt + 30, prompt + 30, 400], 4, 2, 64, 64, page, torch.bfloat16,
+                    bounds=False)
+    server.streams[1] = [torch.cat([a[:prompt], b[prompt:]]) for a, b in zip(*server.streams[:2])]
+    server.step([prompt, 0, 0], packed=True)
+    share(server, 0, 1, prompt)
+    server.step([10, 20, 0], packed=True)
+    kept = [keep if s == ends else n for s, n in enumerate(server.seen)]
+    paged.page_tables_release(server.tables, server.lengths, i32(kept), server.pool, page=page)
+    server.seen[ends] = keep
+    server.lengths[ends] = keep
+    free = free_pages(server.pool)
+    held = server.tables[stays, :-(-server.seen[stays] // page)].tolist()
+    assert len(free) == len(set(free)) and not set(free) & set(held)
+    server.step([0, 0, min(400, len(free) * page)], packed=True)
+    before = list(server.seen)
+    fresh = [0, 0, 0]
+    fresh[stays] = min(10, page - before[stays] % page)
+    server.check(server.step(fresh, packed=True), before)
+    # and when all of them have ended every page is free, once
+    paged.page_tables_release(server.tables, server.lengths, i32([0] * 3), server.pool, page=page)
+    assert sorted(free_pages(server.pool)) == list(range(server.pages))
+    assert bool((server.tables == -1).all())
+
+
+def test_slots_with_a_prompt_in_common_end_at_once():
+    """Their pages go back once, in an order that does not depend on the run."""
+    page, slots = 16, 300
+    pools = []
+    for _ in range(3):
+        want = reference.Tables(slots, 20, 4000, page, order=shuffled(7, 4000))
+        tables, pool = want.tensors(DEVICE)
+        paged.page_tables_update(tables, i32([0] * slots), pool, offsets_of([160] + [0] * (slots - 1)),
+                                 tokens=160, page=page)
+        tables[1:, :10] = tables[:1, :10]
+        lengths = i32([160] * slots)
+        paged.page_tables_update(tables, lengths, pool, tokens=40, page=page)
+        paged.page_tables_release(tables, lengths + 40, lengths * 0, pool, page=page)
+        assert bool((tables == -1).all())
+        free = free_pages(pool)
+        assert sorted(free) == list(range(4000))
+        pools.append(free)
+    assert pools[0] == pools[1] == pools[2]
+
+
+@pytest.mark.parametrize("slots,columns,pages,page", [
+    (2, 3, 9, 16), (5, 40, 90, 32), (64, 70, 3000, 16), (300, 30, 5000, 16), (1500, 9, 4000, 64), (7, 3000, 9000, 16),
+    (40, 50, 300000, 16), (8192, 4, 140000, 16), (3, 2, 131073, 16),
+])
+def test_releases_of_shared_pages_are_those_of_lists(slots, columns, pages, page):
+    """Any page in any number of tables, what is kept and what goes at random."""
+    generator = torch.Generator().manual_seed(slots)
+    random = lambda high, count=slots: torch.randint(0, high + 1, (count,), generator=generator).tolist()
+    for step in range(4):
+        want = reference.Tables(slots, columns, pages, page, order=[], free=0)
+        few = (3, columns, pages - 1, pages - 1)[step]   # of which most slots have the same, or hardly any
+        spread = random(min(few, pages - 1), slots * columns)
+        if step == 3:   # and numbers that are no page
+            spread = [(n, -1, pages, -2**31, 2**31 - 1)[c] for n, c in zip(spread, random(4, slots * columns))]
+        want.table = [spread[s * columns:(s + 1) * columns] for s in range(slots)]
+        tables, pool = want.tensors(DEVICE)
+        lengths = random(columns * page + 40)
+        keep = [(0, n // 3, n, n + 9)[c] for n, c in zip(lengths, random(3))]
+        paged.page_tables_release(tables, i32(lengths), i32(keep), pool, page=page)
+        release(want, lengths, keep)
+        check_tables(want, tables, pool)
+
+
+def test_a_release_of_shared_pages_in_a_graph():
+    page, slots = 16, 5
+    build = lambda: reference.Tables(slots, 8, 60, page, order=shuffled(8, 60))
+    lengths = i32([100, 100, 50, 100, 0])
+    keep = i32([0, 100, 0, 32, 0])
+    want = build()
+    tables, pool = want.tensors(DEVICE)
+    saved = tables.clone(), pool.clone()
+
+    def step():
+        paged.page_tables_update(tables, lengths * 0, pool, offsets_of([100, 0, 0, 0, 0]), tokens=100, page=page)
+        tables[1:4] = tables[:1]
+        paged.page_tables_release(tables, lengths, keep, pool, page=page)
+
+    step()
+    result = tables.clone(), pool.clone()
+    graph = torch.cuda.CUDAGraph()
+    recorded = i32([0, 100, 100, 100, 100, 100])
+    tables.copy_(saved[0]), pool.copy_(saved[1])
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.graph(graph, stream=side):
+        paged.page_tables_update(tables, lengths * 0, pool, recorded, tokens=100, page=page)
+        tables[1:4] = tables[:1]
+        paged.page_tables_release(tables, lengths, keep, pool, page=page)
+    for _ in range(4):
+        tables.copy_(saved[0]), pool.copy_(saved[1])
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(tables, result[0]) and torch.equal(pool, result[1])
+    assert sorted(free_pages(pool) + tables[1, :7].tolist()) == list(range(60))

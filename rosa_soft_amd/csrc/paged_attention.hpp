@@ -1248,6 +1248,26 @@ __device__ __forceinline__ double over_lanes_sum(double x) {
   return x;
 }
 
+// Whether 16 bytes of numbers have infinity among them, or NaN: as whole numbers with a sign, of which
+// the largest is taken, they lie above all that is finite, and what is below zero below it.
+template <typename T, typename Piece>
+__device__ __forceinline__ bool reaches_infinity(const Piece& piece) {
+  if constexpr (sizeof(T) == 4) {
+    typedef int Words __attribute__((ext_vector_type(4)));
+    const Words words = __builtin_bit_cast(Words, piece);
+    return max(max(words[0], words[1]), max(words[2], words[3])) >= 0x7f800000;
+  } else {
+    typedef short Pair __attribute__((ext_vector_type(2)));
+    struct Pairs {
+      Pair of[4];
+    };
+    const Pairs pairs = __builtin_bit_cast(Pairs, piece);
+    const Pair most = __builtin_elementwise_max(__builtin_elementwise_max(pairs.of[0], pairs.of[1]),
+                                                __builtin_elementwise_max(pairs.of[2], pairs.of[3]));
+    return max(most[0], most[1]) >= (std::is_same_v<T, _Float16> ? 0x7c00 : 0x7f80);
+  }
+}
+
 // The largest product that a key within a page's bounds can have with a query of the group, in 64 bits,
 // in which the products are exact: pages are ranked as their bounds rank, whatever the order of a sum.
 // A lane has the queries' elements of its columns in registers for all pages; the lanes of a page add up.
@@ -1333,6 +1353,7 @@ paged_score_kernel(PagedArgs<T> a, int blocks_of_token) {
     double best[kTurns];
 #pragma unroll
     for (int i = 0; i < kTurns; ++i) best[i] = -__builtin_inf();
+    uint32_t no_number = 0;  // turns in which a sum is none after all
     for (int member0 = 0; member0 < (ONE ? 1 : a.share); member0 += kMembers) {
       if (!ONE && (base > start || member0 > 0)) fetch_queries(member0);
 #pragma unroll
@@ -1354,6 +1375,38 @@ paged_score_kernel(PagedArgs<T> a, int blocks_of_token) {
         const int page = base + i * kPages + tid / kLanes;
         if ((ONE || member0 + kMembers >= a.share) && tid % kLanes == 0 && page < earlier)
           scores[page] = a.is_page(id[i]) ? best[i] : __builtin_nan("");
+      }
+      // A query of zero took the lower bound, and is no number times the upper one either if that is
+      // infinite.  (Apart from the sums, and looked at last, so that nothing waits for it.)
+      bool infinite = false;
+#pragma unroll
+      for (int i = 0; i < kTurns; ++i) infinite |= reaches_infinity<T>(highs[i]);
+      if (__any(infinite))
+#pragma unroll
+        for (int i = 0; i < kTurns; ++i) {
+          // (converted in this branch: else all of them are held in registers for it)
+          typedef uint32_t Words __attribute__((ext_vector_type(4)));
+          Words words = __builtin_bit_cast(Words, highs[i]);
+          asm volatile("" : "+v"(words));
+          const Piece upper = __builtin_bit_cast(Piece, words);
+#pragma unroll
+          for (int e = 0; e < kElements; ++e) {
+            const double largest = static_cast<float>(upper[e]);
+#pragma unroll
+            for (int m = 0; m < kMembers; ++m) {
+              const double other = queries[m][e] * largest;
+              if (other != other) no_number |= 1u << i;
+            }
+          }
+        }
+    }
+    if (__any(no_number != 0)) {
+      const uint64_t lanes = ((uint64_t{1} << kLanes) - 1) << (lane & -kLanes);
+#pragma unroll
+      for (int i = 0; i < kTurns; ++i) {
+        const uint64_t those = __ballot(col < a.key_width && (no_number >> i & 1) != 0);
+        const int page = base + i * kPages + tid / kLanes;
+        if ((those & lanes) != 0 && tid % kLanes == 0 && page < earlier) scores[page] = __builtin_nan("");
       }
     }
   }

@@ -7,7 +7,8 @@ import torch
 
 from rosa_soft_amd import paged
 from tests import paged_reference as reference
-from tests.test_gpu_paged import DEVICE, DTYPES, Server, check_tables, i32, offsets_of, shuffled
+from tests.test_gpu_paged import (DEVICE, DTYPES, Server, check_tables, close, i32, offsets_of, randn,
+                                  shuffled, tolerance_of)
 
 pytestmark = pytest.mark.gpu
 
@@ -242,3 +243,33 @@ def test_a_release_of_shared_pages_in_a_graph():
         torch.cuda.synchronize()
         assert torch.equal(tables, result[0]) and torch.equal(pool, result[1])
     assert sorted(free_pages(pool) + tables[1, :7].tolist()) == list(range(60))
+
+
+# ---------------------------------------------------------------------------
+# bounds that are infinite
+# ---------------------------------------------------------------------------
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("width", [24, 33, 40, 128])
+@pytest.mark.parametrize("share", [1, 4, 6])
+@pytest.mark.parametrize("bound", [math.inf, -math.inf])
+def test_a_query_of_zero_and_an_infinite_bound_are_no_number(bound, share, width, dtype):
+    """Their product, whichever of the two bounds it is: the page ranks first, and makes NaN of the
+    token that sees it; the other heads' tokens have their own pages."""
+    server = Server(2200, [101], 2 * share, 2, width, width, 16, dtype)
+    for column in {0, width // 2, width - 1}:
+        server.caches = [torch.full_like(c, math.nan) for c in server.caches]
+        server.bounds = torch.full_like(server.bounds, math.nan)
+        server.tables, server.pool = reference.Tables(1, 8, server.pages, 16).tensors(DEVICE)
+        server.lengths, server.seen = i32([0]), [0]
+        q, k, v = server.streams[0] = [randn(2201 + i, 101, 2 * share if i == 0 else 2, width, dtype=dtype)
+                                       for i in range(3)]
+        k[35, 0, column] = bound             # on page 2
+        q[100, share - 1, column] = 0.0      # one member of the group
+        server.step([100], True)
+        output, = server.step([1], False, count=1)
+        pages = reference.selected(q[100, :share], k[:, 0], 16, 1, 100)
+        assert pages[0] == 2
+        assert bool(torch.isnan(output[0, share - 1]).all())
+        want, terms, most = reference.attention(q[100:, share:], k[:, 1:], v[:, 1:], 100, 16, 1)
+        close(output[:, share:], want, tolerance_of(dtype, terms, most, 101, 2 * width))

@@ -471,7 +471,9 @@ typedef struct rosa_page_tables {
  * (of those that there are) take pages from the top of the stack, in the order of slots and columns;
  * where the pool has no more they take -1.  `rows` int64 [N], or [slots, T]: where each new token lies,
  * tables[s][p / page] * page + p mod page, or -1 where it has no page.  Invalid offsets make every row
- * -1 and change nothing.  At most 8192 slots.
+ * -1 and change nothing.  At most 8192 slots.  What the columns held before is not looked at: of a step that ran
+ * out of pages, or whose tokens are not all kept, the rest is released before the next one, from
+ * lengths + new to lengths + kept.
  */
 int rosa_hip_page_tables_update(const rosa_page_tables* tables, const int32_t* cu_seqlens, int T,
                                 int N, int64_t* rows, void* stream);

@@ -118,6 +118,13 @@ def page_tables_update(tables: Tensor, lengths: Tensor, pool: Tensor,
     the device, and can be recorded into a graph; a server that must not run out of pages reads
     ``pool[0]`` before it admits a request.  Invalid ``cu_seqlens`` change nothing, and every row
     is -1.
+
+    Which columns are new follows from ``lengths`` alone, whatever they held before.  So of a step that
+    ran out of pages, or whose tokens are not all kept (padding, rejected drafts), the rest is given back
+    before the next one, ``page_tables_release(tables, lengths + new, lengths + kept, pool, page=page)``
+    with the tokens that it asked for and those that stay.  Otherwise the next step takes pages for the
+    same columns again and those that they had are lost, and columns that got none stay without once
+    ``lengths`` has passed them.
     """
 
     return _tables_update(tables, lengths, pool, cu_seqlens, _integer("tokens", tokens),

@@ -273,3 +273,45 @@ def test_a_query_of_zero_and_an_infinite_bound_are_no_number(bound, share, width
         assert bool(torch.isnan(output[0, share - 1]).all())
         want, terms, most = reference.attention(q[100:, share:], k[:, 1:], v[:, 1:], 100, 16, 1)
         close(output[:, share:], want, tolerance_of(dtype, terms, most, 101, 2 * width))
+
+
+# ---------------------------------------------------------------------------
+# steps that are undone
+# ---------------------------------------------------------------------------
+
+def test_a_step_that_ran_out_of_pages_is_undone_and_done_again():
+    page = 16
+    want = reference.Tables(3, 10, 12, page, order=shuffled(3, 12))
+    tables, pool = want.tensors(DEVICE)
+    lengths = [40, 70, 30]
+    paged.page_tables_update(tables, i32([0] * 3), pool, offsets_of(lengths), tokens=sum(lengths), page=page)
+    want.update([0] * 3, lengths)
+    rows = paged.page_tables_update(tables, i32(lengths), pool, tokens=30, page=page)
+    assert bool((rows == -1).any()) and pool[0].item() == 0
+    paged.page_tables_release(tables, i32(lengths) + 30, i32(lengths), pool, page=page)
+    check_tables(want, tables, pool)
+    # a request ends, and the step has room
+    paged.page_tables_release(tables, i32(lengths), i32([40, 0, 30]), pool, page=page)
+    want.release(lengths, [40, 0, 30])
+    rows = paged.page_tables_update(tables, i32([40, 0, 30]), pool, tokens=30, page=page)
+    assert rows.tolist() == want.update([40, 0, 30], [30] * 3)
+    assert bool((rows >= 0).all())
+    check_tables(want, tables, pool)
+
+
+def test_a_step_of_which_a_part_is_kept_loses_no_page():
+    """A dense step whose tokens are not all real: the rest's pages are given back before the next."""
+    page, slots, step = 16, 4, 40
+    want = reference.Tables(slots, 30, 60, page, order=shuffled(4, 60))
+    tables, pool = want.tensors(DEVICE)
+    lengths = [0] * slots
+    for real in ([40, 1, 0, 17], [3, 40, 16, 15], [0, 0, 40, 1]):
+        rows = paged.page_tables_update(tables, i32(lengths), pool, tokens=step, page=page)
+        assert rows.tolist() == want.update(lengths, [step] * slots)
+        upto, lengths = [n + step for n in lengths], [n + r for n, r in zip(lengths, real)]
+        paged.page_tables_release(tables, i32(upto), i32(lengths), pool, page=page)
+        want.release(upto, lengths)
+        check_tables(want, tables, pool)
+        held = [entry for row in tables.tolist() for entry in row if entry >= 0]
+        assert len(held) == sum(-(-n // page) for n in lengths)
+        assert sorted(held + free_pages(pool)) == list(range(60))

@@ -315,3 +315,25 @@ def test_a_step_of_which_a_part_is_kept_loses_no_page():
         held = [entry for row in tables.tolist() for entry in row if entry >= 0]
         assert len(held) == sum(-(-n // page) for n in lengths)
         assert sorted(held + free_pages(pool)) == list(range(60))
+
+
+# ---------------------------------------------------------------------------
+# many slots whose tiles are cut
+# ---------------------------------------------------------------------------
+
+MIXED = [(lambda s: 1, False), (lambda s: 3, False), (lambda s: 6, False), (lambda s: s % 2, True),
+         (lambda s: (0, 1, 5, 90)[s % 4], True), (lambda s: 0 if s % 10 else 70, True)]
+
+
+@pytest.mark.parametrize("widths", [(8, 2, 64, 64), (6, 2, 40, 33)])
+@pytest.mark.parametrize("slots", [64, 65, 130, 300])
+def test_long_and_short_caches_of_many_slots(slots, widths):
+    """Single tokens, drafts and packed mixes for slots of a few or thousands of tokens, among them
+    slots without new ones: every slot against the definition."""
+    lengths = [3000 + 7 * s if s % 10 == 0 else 0 if s % 10 == 3 else (s * 37) % 90 + 1 for s in range(slots)]
+    totals = [n + sum(fresh(s) for fresh, _ in MIXED) for s, n in enumerate(lengths)]
+    server = Server(2300, totals, *widths, 16, torch.bfloat16, columns=400, bounds=False)
+    server.step(lengths, packed=True)
+    for fresh, packed in MIXED:
+        before = list(server.seen)
+        server.check(server.step([fresh(s) for s in range(slots)], packed), before)

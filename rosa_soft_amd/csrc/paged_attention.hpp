@@ -276,20 +276,25 @@ __device__ __forceinline__ Found portion_of(const PagedArgs<T>& a, int tid, Port
   return Found::kRun;
 }
 
-// The slot of a new token, among 64 times as many with every look at them.  (Offsets that decrease make
-// it some slot.)
-template <typename T>
-__device__ __forceinline__ int slot_of_token(const PagedArgs<T>& a, int token, int lane) {
-  const Sequences& q = a.sequences;
-  if (q.offsets == nullptr) return token / q.length;
-  int slot = 0, left = q.count;  // it is one of [slot, slot + left)
+// The last of `count` slots that `begins` is true of, from slot 0 on, of which it is: among 64 times as many
+// with every look at them.
+template <typename Begins>
+__device__ __forceinline__ int last_slot(int count, int lane, Begins&& begins) {
+  int slot = 0, left = count;  // it is one of [slot, slot + left)
   while (left > 1) {
     const int step = (left + 63) / 64, end = (lane + 1) * step;
-    const int before = __popcll(__ballot(end < left && q.offsets[slot + end] <= token));
+    const int before = __popcll(__ballot(end < left && begins(slot + end)));
     slot += before * step;
     left = min(step, left - before * step);
   }
   return slot;
+}
+// The slot of a new token.  (Offsets that decrease make it some slot.)
+template <typename T>
+__device__ __forceinline__ int slot_of_token(const PagedArgs<T>& a, int token, int lane) {
+  const Sequences& q = a.sequences;
+  if (q.offsets == nullptr) return token / q.length;
+  return last_slot(q.count, lane, [&](int s) { return q.offsets[s] <= token; });
 }
 template <typename T>
 __device__ __forceinline__ int past_of(const PagedArgs<T>& a, int slot, int fresh) {
@@ -323,33 +328,57 @@ __device__ __forceinline__ bool offsets_valid(const PagedArgs<T>& a, int tid) {
 __device__ __forceinline__ float lower_of(float a, float b) { return b < a || b != b ? b : a; }
 __device__ __forceinline__ float higher_of(float a, float b) { return b > a || b != b ? b : a; }
 
+// Pages that a chunk touches for a head, at most: `each` of a slot, or in the order of packed slots, whose
+// pages begin at as many as the tokens before them fill whole, and two for each slot before.  (Blocks are
+// limited so that those of all heads are below 2^28.)
+__host__ __device__ __forceinline__ uint32_t pages_of_slot(int tokens, int page_shift) {
+  return static_cast<uint32_t>((tokens - 1) >> page_shift) + 2;
+}
+template <typename T>
+__host__ __device__ __forceinline__ uint32_t pages_touched(const PagedArgs<T>& a) {
+  const Sequences& q = a.sequences;
+  const auto count = static_cast<uint32_t>(q.count);
+  return q.offsets == nullptr ? count * pages_of_slot(q.length, a.page_shift)
+                              : static_cast<uint32_t>(q.tokens >> a.page_shift) + 2 * count;
+}
+
 // The new tokens on their rows, and the bounds of the pages that they lie on.  A block has one page of
-// one slot and head at a time: no other one changes its bounds.  Only where several tokens bring bounds, or
-// are selected for in this call; otherwise the kernels that attend put tokens on their rows, which spares
-// a launch (64 slots' single tokens: 294 us before, 281 since).  Latency is all of it: 173 packed tokens
-// of 6 slots, 4 heads of 96 columns, 7.6 us.
+// one slot and head at a time: no other one changes its bounds.  Only where bounds are kept, or pages
+// selected, of several tokens or packed ones: otherwise the kernels that attend (for groups of up to 16
+// members where there are bounds) or that score (for more columns than are selected) put tokens on
+// their rows, which spares a launch (64 slots' single tokens: 294 us before, 281 since).  Latency is all of
+// it: 173 packed tokens of 6 slots, 4 heads of 96 columns, 9.0 us.  Blocks by what is touched, which go on to
+// further pages: with a block for each slot, head and page that all tokens together may touch, 1024 packed
+// single tokens took 1350 us with their attention, 460 since.
 template <typename T, bool WHOLE>
 __global__ __launch_bounds__(kThreads) void paged_append_kernel(PagedArgs<T> a) {
   __shared__ float lows[kMostWidth], highs[kMostWidth];
   __shared__ uint64_t stored[kThreads / 64];  // which tokens of the page have a row
   __shared__ int number_of_page;
   const int tid = threadIdx.x, page = 1 << a.page_shift;
-  const uint32_t block = block_number();
-  const int64_t slot64 = block / a.kv_heads;
-  const int kv_head = static_cast<int>(block % a.kv_heads);
-  if (slot64 >= a.sequences.count) return;
-  const int slot = static_cast<int>(slot64);
   if (!offsets_valid(a, tid)) return;
-  const Run run = run_of_sequence(a.sequences, slot);
-  if (run.length < 1) return;
-  const int past = past_of(a, slot, run.length);
-  const T* keys = a.key.row(run.batch, run.begin, kv_head);
-  const T* values = a.value.row(run.batch, run.begin, kv_head);
   constexpr int kElements = 16 / static_cast<int>(sizeof(T));
   typedef T Piece __attribute__((ext_vector_type(kElements)));
-  for (int64_t number = blockIdx.z;; number += gridDim.z) {
+  const Sequences& q = a.sequences;
+  const uint32_t heads = static_cast<uint32_t>(a.kv_heads), items = pages_touched(a) * heads;
+  const uint32_t each = q.offsets == nullptr ? pages_of_slot(q.length, a.page_shift) : 1;
+  for (uint32_t at = blockIdx.x; at < items; at += gridDim.x) {
+    const uint32_t item = at / heads;
+    const int kv_head = static_cast<int>(at % heads);
+    const int slot = q.offsets == nullptr
+                         ? static_cast<int>(item / each)
+                         : last_slot(q.count, tid & 63, [&](int s) {
+                             return static_cast<uint32_t>(q.offsets[s] >> a.page_shift) + 2 * s <= item;
+                           });
+    const Run run = run_of_sequence(q, slot);
+    if (run.length < 1) continue;
+    // of a page among those that the slot's new tokens touch
+    const int64_t number = q.offsets == nullptr ? item % each : item - (run.begin >> a.page_shift) - 2 * slot;
+    const int past = past_of(a, slot, run.length);
+    const T* keys = a.key.row(run.batch, run.begin, kv_head);
+    const T* values = a.value.row(run.batch, run.begin, kv_head);
     const int64_t start = ((static_cast<int64_t>(past) >> a.page_shift) + number) << a.page_shift;
-    if (start >= static_cast<int64_t>(past) + run.length) break;
+    if (start >= static_cast<int64_t>(past) + run.length) continue;
     // new tokens [begin, end) of the slot
     const int begin = static_cast<int>(max(start - past, int64_t{0}));
     const int end = static_cast<int>(min(start + page - past, static_cast<int64_t>(run.length)));
@@ -370,7 +399,6 @@ __global__ __launch_bounds__(kThreads) void paged_append_kernel(PagedArgs<T> a) 
     };
     copy(a.key_pages, a.key_width, keys, a.key.token_stride);
     copy(a.value_pages, a.value_width, values, a.value.token_stride);
-    if (a.key_bounds == nullptr) continue;
     // (padding is on no page, and has no part in its bounds; a page has at most as many as threads)
     const int64_t row = tid < end - begin ? a.row_of(run.first + begin + tid) : -1;
     const uint64_t put = __ballot(row >= 0);
@@ -1594,6 +1622,8 @@ PagedDivision division_of(const PagedShare& share, int most_few, char* at) {
 // Blocks that go on to further work: a thousand more take the chip 4 us to begin, whatever they do.  Those
 // of a join are as many as it can hold at once (51 MB of parts: 1024 of them 17 us, 2048 14, 4096 14).
 constexpr int64_t kJoinBlocks = 2048;
+// And those that put tokens on their rows: each looks at all offsets once.
+constexpr int64_t kAppendBlocks = 2048;
 constexpr int64_t kScoreBlocks = 1024;
 
 template <typename T, int WIDTH, bool WHOLE>
@@ -1636,12 +1666,9 @@ void paged_chunk_launch(PagedArgs<T>& args, const PagedShare& share, hipStream_t
 
 template <typename T, bool WHOLE>
 void paged_append_launch(PagedArgs<T>& args, hipStream_t stream) {
-  const Sequences& q = args.sequences;
-  const int64_t most = q.offsets == nullptr ? q.length : q.tokens;  // of a slot
-  const int64_t touched = ((most - 1) >> args.page_shift) + 2;
-  dim3 grid = grid_of(static_cast<int64_t>(q.count) * args.kv_heads);
-  grid.z = static_cast<unsigned>(touched < 64 ? touched : 64);
-  paged_append_kernel<T, WHOLE><<<grid, kThreads, 0, stream>>>(args);
+  const int64_t items = static_cast<int64_t>(pages_touched(args)) * args.kv_heads;
+  paged_append_kernel<T, WHOLE>
+      <<<dim3(static_cast<unsigned>(std::min<int64_t>(items, kAppendBlocks))), kThreads, 0, stream>>>(args);
 }
 
 // Scores of a slab of tokens take at most this much memory, or one token's.

@@ -337,3 +337,24 @@ def test_long_and_short_caches_of_many_slots(slots, widths):
     for fresh, packed in MIXED:
         before = list(server.seen)
         server.check(server.step([fresh(s) for s in range(slots)], packed), before)
+
+
+@pytest.mark.parametrize("totals,steps", [
+    ([(s * 37) % 60 + 25 for s in range(2500)], [lambda s: s % 25, lambda s: 1, lambda s: 0 if s % 50 else 20]),
+    ([30000, 3, 20000], [lambda s: (29000, 0, 17)[s], lambda s: (5, 1, 19000)[s]]),
+])
+def test_bounds_of_many_pages_in_packed_calls(totals, steps):
+    """More pages that new tokens touch than blocks run at once."""
+    slots = len(totals)
+    server = Server(2400, totals, 4, 4, 32, 32, 16, torch.bfloat16)
+    for fresh in steps:
+        before = list(server.seen)
+        output = server.step([fresh(s) for s in range(slots)], packed=True)
+        if slots > 3:
+            server.check(output, before, slots=range(0, slots, 41))
+    for s in range(0, slots, 41 if slots > 3 else 1):
+        end, table = server.seen[s], server.tables[s, :-(-server.seen[s] // 16)].long()
+        for cache, stream in zip(server.caches, server.streams[s][1:]):
+            assert torch.equal(server.held(cache, s), stream[:end])
+        for g in range(4):
+            assert torch.equal(server.bounds[table, g], reference.bounds_of(server.streams[s][1][:end, g], 16))

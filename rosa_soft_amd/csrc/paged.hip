@@ -17,8 +17,8 @@ constexpr int64_t kMostScoreBytes = int64_t{1} << 28;   // of a slab of tokens
 constexpr int kTableThreads = 1024;
 // Tokens whose rows the block that hands out pages writes by itself; more have a launch of their own.
 constexpr int kTokensOfBlock = 16384;
-// Pages that a block can mark at a time, a bit of LDS each (16 KB): a larger pool is looked at in parts.
-constexpr int kMarkedPages = 1 << 17;
+// Pages that a block can mark at a time, a bit of LDS each (64 KB): a larger pool is looked at in parts.
+constexpr int kMarkedPages = 1 << 19;
 constexpr int kRun = 512;  // columns of a slot that a wave looks through at a time
 
 }  // namespace
@@ -239,6 +239,7 @@ struct Released {
   const TableArgs& a;
   const int* first;
   int64_t count;
+  bool all;  // no slot keeps any
   __device__ __forceinline__ int32_t* operator[](int64_t k) const {
     const int s = slot_of_item(first, a.slots, static_cast<int>(k));
     return a.tables + static_cast<int64_t>(s) * a.columns + a.kept(s) + k - first[s];
@@ -246,16 +247,21 @@ struct Released {
 };
 __device__ __forceinline__ Released released_entries(const TableArgs& a, int* first, int64_t* ends, int tid) {
   int64_t items = 0;
+  int keeps = 0;
   for (int base = 0; base < a.slots; base += kTableThreads) {
     const int s = base + tid;
-    const int64_t mine = s < a.slots ? a.held(a.length(s)) - a.kept(s) : 0;
-    int64_t total;
+    int64_t mine = 0, total;
+    if (s < a.slots) {
+      const int64_t kept = a.kept(s);
+      mine = a.held(a.length(s)) - kept;
+      keeps |= kept > 0;
+    }
     const int64_t upto = items + scan_block(mine, tid, ends, &total);
     if (s < a.slots) first[s] = static_cast<int>(upto - mine);
     items += total;
   }
-  __syncthreads();
-  return {a, first, items};
+  const bool some = __syncthreads_or(keeps);
+  return {a, first, items, !some};
 }
 
 // A bit for each page from `low` on.
@@ -281,15 +287,16 @@ __device__ __forceinline__ Marks no_marks(const TableArgs& a, uint32_t* words, i
 // A page may be in several tables (a prompt in common): ahead of a release, entries that it would take
 // from a slot become -1 where some slot keeps their page.  Every block marks the pages that are to go
 // back, looks for them among its share of the entries that stay, and has an entry dropped if it found
-// its page; blocks that read an entry which another one has dropped pass it over.  Latency again: 6.7 us
-// for 64 slots of up to 9000 tokens on pages of 16, of which eight each are taken back, 7.2 for 256 slots.
+// its page; blocks that read an entry which another one has dropped pass it over.  Latency again: 7.2 us
+// for 64 slots of up to 9000 tokens on pages of 16, of which eight each are taken back, 7.7 for 256 slots;
+// with the release 23 us for 512 slots of 20000 (8 without this look at 640000 entries).
 __global__ __launch_bounds__(kTableThreads) void page_tables_keep_kernel(TableArgs a) {
   extern __shared__ int first[];
   __shared__ int64_t ends[kTableThreads / 64];
   __shared__ uint32_t words[kMarkedPages / 32];
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const Released released = released_entries(a, first, ends, tid);
-  if (released.count == 0) return;
+  if (released.count == 0 || released.all) return;
   const int per = (a.columns + kRun - 1) / kRun;
   const int64_t runs = static_cast<int64_t>(a.slots) * per;
   for (int64_t low = 0; low < a.pages; low += kMarkedPages) {
@@ -348,8 +355,8 @@ __device__ __forceinline__ bool taken_before(const Marks& marks, int id, int* id
 
 // Numbering backwards: from the last entry to the first, each valid page goes on top of those before
 // it.  A page that several slots give back goes with the first of its entries in that order; the others
-// are passed over, those of pages beyond the first window in a look ahead of this one.  5.5 us for 64
-// slots with 8 tokens each.
+// are passed over, those of pages beyond the first window in a look ahead of this one.  5.7 us for 64
+// slots with 8 tokens each; each 1024 entries more take 3 us.
 __global__ __launch_bounds__(kTableThreads) void page_tables_release_kernel(TableArgs a) {
   extern __shared__ int first[];
   __shared__ int64_t ends[kTableThreads / 64];

@@ -141,9 +141,10 @@ def page_tables_release(tables: Tensor, lengths: Tensor, keep: Tensor, pool: Ten
     takes back an update.  Entries that are no page are passed over, and so are pages for which the
     pool has no place.  ``lengths`` is left to the caller.
 
-    A page in several tables goes back with the last of them: while the first ``keep`` tokens of any
-    slot lie on it (up to ``lengths``) it stays, and of several slots that give it back in one call the
-    last one does.  A prompt that is kept for later requests has a slot of its own that brings no tokens.
+    A page in several rows of ``tables`` goes back with the last of them: while the first ``keep`` tokens
+    of any slot lie on it (up to ``lengths``) it stays, and of several slots that give it back in one call
+    the last one does.  A prompt that is kept for later requests has a slot of its own that brings no
+    tokens.
     """
 
     _tables_release(tables, lengths, keep, pool, _integer("page", page))

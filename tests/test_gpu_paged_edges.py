@@ -192,6 +192,7 @@ def test_slots_with_a_prompt_in_common_end_at_once():
 @pytest.mark.parametrize("slots,columns,pages,page", [
     (2, 3, 9, 16), (5, 40, 90, 32), (64, 70, 3000, 16), (300, 30, 5000, 16), (1500, 9, 4000, 64), (7, 3000, 9000, 16),
     (40, 50, 300000, 16), (8192, 4, 140000, 16), (3, 2, 131073, 16),
+    (40, 50, 1200000, 16), (3, 2, 2**19 + 1, 16),
 ])
 def test_releases_of_shared_pages_are_those_of_lists(slots, columns, pages, page):
     """Any page in any number of tables, what is kept and what goes at random."""

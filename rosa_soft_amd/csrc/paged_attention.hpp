@@ -496,10 +496,15 @@ __device__ __forceinline__ bool clear_wild(Piece& piece) {
 // With `lists` the keys are those of the pages in a token's list, one behind the other.
 //
 // Every key and value is read once for all members of the group, a tile ahead of its use, and reads are
-// what bounds it (a copy of 2 GiB moves 4.9 TB/s): 64 slots of up to 9000 tokens, 8 heads of 128, bf16,
-// 1.45 GB in 265 us, 5.5 TB/s; two slots of up to 200000, 2 heads of 64, fp16, 187 MB in 34 us; 33 pages
-// of 64 for each of 32 slots, 8 heads of 128, 277 MB in 45 us, 6.1 TB/s.  One slot of 512 tokens in
-// float32 takes 8.7 us: the way from the lengths to the table, the page and through the waves' softmaxes.
+// what bounds it (2 GiB are read at 5.8 TB/s, copied at 4.9): 64 slots of up to 9000 tokens, 8 heads of
+// 128, bf16, 1395 MB in 264 us, 5.3 TB/s; two slots of up to 200000, 2 heads of 64, fp16, 197 MB in 34 us,
+// 5.9 TB/s; 33 pages of 64 for each of 32 slots, 8 heads of 128, 274 MB in 45 us, 6.1 TB/s.  In float32,
+// whose operands are split in registers, 64 slots of up to 4500 tokens take 386 us (3.6 TB/s, one wave to a
+// SIMD), of 9000 with 64 columns 303 (4.6 TB/s).  One slot of 512 tokens in float32 takes 8.6 us: the way
+// from the lengths to the table, the page and through the waves' softmaxes.
+// Weights are summed in float32 as they are, and rounded to the inputs' type as operands of the product with
+// the values: a result is off by half a step of them at most.  (paged_chunk_kernel sums them as rounded, a
+// product with ones: by a whole one at most, and by none where one weight is all.)
 // Waves have keys of their own because 16 rows are one operand: sharing rows out would leave three of
 // them without work.  Two sixteens of rows (drafts of 5 tokens, 4 heads on one) took 62 us, and the
 // kernel for many rows takes 49.
@@ -826,17 +831,21 @@ paged_token_kernel(PagedArgs<T> a) {
 // registers.  USED: the columns that keys and values have at most (tiles have WIDTH).  Weights are
 // rounded to the inputs' type, as the operand of the product with the values, and summed as rounded.
 //
-// Four prompts of 2048 tokens behind up to 2500, 32 heads on 8 of 128 columns, bf16 (403 GFLOP): 430 to
-// 455 us, 890 TFLOP/s (a product of 8192 x 8192 x 8192 by the library: 1290).  No pipe is full: matrix ones are
-// busy for 39 % of the time, vector ones issue for 45 %, LDS works for 27 % (a wave reads all of both
-// tiles, 32 KB, for its 32 rows); the registers hold two waves to a SIMD, which wait for operands and for
-// one another's pipes.  With operands read ahead of their products 476 us became 470.  Tried and not kept: the next half tile's scores
-// among the exponentials of this one, 588; eight waves for 256 rows in two teams, one with matrix
-// instructions while the other has vector ones, 497 to 669, as all eight read as much of LDS again.
-// Drafts of 5 tokens for 16 slots of up to 4096 (64 rows): 178 MB in 33 us, 5.4 TB/s.  Packed prompts of
-// 1 to 2047 tokens behind up to 3001 (12 heads on 4 of 80 columns, fp16, 38 GFLOP): 120 us, for portions
-// of unequal length (of 512 places for blocks the one that ends last has 1.4 times the mean) and columns
-// padded from 80 to 96.
+// Four prompts of 2048 tokens behind up to 2500, 32 heads on 8 of 128 columns, bf16 (399 GFLOP): 445 us on
+// a chip at work, 900 TFLOP/s (a product of 8192 x 8192 x 8192 by the library: 1400), 556 after it was idle
+// (1130).  No pipe is full: matrix ones are busy for 39 % of the time, vector ones issue for 45 %, LDS works
+// for 27 % (a wave reads all of both tiles, 32 KB, for its 32 rows); the registers hold two waves to a SIMD,
+// and waves wait for 32 % of their time.  With operands read ahead of their products 476 us became 470.
+// Tried and not kept: the next half tile's scores among the exponentials of this one, 588; eight waves for
+// 256 rows in two teams, one with matrix instructions while the other has vector ones, 497 to 669, as all
+// eight read as much of LDS again.
+// Drafts of 5 tokens for 16 slots of up to 4096 (64 rows): 181 MB in 33 us, 5.7 TB/s.  Packed prompts of
+// 1 to 2047 tokens behind up to 3001 (12 heads on 4 of 80 columns, fp16, 38 GFLOP): 120 us.  Portions
+// of unequal length (of 512 places for blocks the one that ends last has 1.4 times the mean), columns padded
+// from 80 to 96 and the prompts' distance from the library's rate make 70 of them; what the others are spent
+// on is not known.  In float32 drafts
+// take 136 us, prompts of 1024 tokens 112 TFLOP/s (176 with 64 columns); columns that are not whole pieces
+// of 16 bytes are moved one by one: 100 and 33 of them, 16 prompts of 200 tokens, 62 TFLOP/s.
 template <typename T, int WIDTH, int USED, int QUERIES, bool WHOLE>
 __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(kWaves<T, WIDTH, WHOLE>))) void
 paged_chunk_kernel(PagedArgs<T> a) {
@@ -1297,15 +1306,16 @@ __device__ __forceinline__ bool reaches_infinity(const Piece& piece) {
 }
 
 // The largest product that a key within a page's bounds can have with a query of the group, in 64 bits,
-// in which the products are exact: pages are ranked as their bounds rank, whatever the order of a sum.
+// in which the products are exact: pages are ranked as their bounds rank, to the rounding of a sum of 64 bits
+// (2^-53 of its largest part sum for each of up to 127 additions), whose order is the same in every run.
 // A lane has the queries' elements of its columns in registers for all pages; the lanes of a page add up.
 // Vector instructions in 64 bits bound it, and the latency of a page's number and bounds, which four pages
-// at once hide: 32 slots of up to 256 pages, 32 heads on 8 of 128 columns, bf16, 15.2 us (one page at
+// at once hide: 32 slots of up to 256 pages, 32 heads on 8 of 128 columns, bf16, 15.7 us (one page at
 // once 19; a page to a lane with queries in LDS 13.5 to 19, and far slower for few pages; a lane for some
-// columns of all heads 26; three waves to a SIMD 17.5); 173 packed tokens of up to 188 pages 17.5 us.
+// columns of all heads 26; three waves to a SIMD 17.5); 173 packed tokens of up to 188 pages 18.3 us.
 // ONE: the group has at most four members, whose queries are loaded once.  More are loaded again for
 // every turn of pages, whose bounds and best scores stay in registers: two slots of 3125 pages, 16 heads
-// on 2, 9.6 us (11.8 with best scores in memory from one four to the next).
+// on 2, 9.7 us (11.8 with best scores in memory from one four to the next).
 template <typename T, bool WHOLE, bool ONE>
 __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(ONE && WHOLE ? 4 : 2))) void
 paged_score_kernel(PagedArgs<T> a, int blocks_of_token) {

@@ -31,7 +31,8 @@ and change nothing, and numbers that are no page are never followed.  Tokens tha
 value that is not finite may have outputs that are not, in one column or in all; the others keep every
 bit of theirs.  In float32 a magnitude of ``2**128 - 2**119`` (3.396e38) or more counts as not finite,
 and in every type sums of weights times values that pass float32's range are.  What no token was put on
-is never read.
+is never read, but for padding among the queries of ``selected_attention_update``, whose outputs are
+unspecified.
 """
 
 from __future__ import annotations

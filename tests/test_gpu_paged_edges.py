@@ -359,3 +359,20 @@ def test_bounds_of_many_pages_in_packed_calls(totals, steps):
             assert torch.equal(server.held(cache, s), stream[:end])
         for g in range(4):
             assert torch.equal(server.bounds[table, g], reference.bounds_of(server.streams[s][1][:end, g], 16))
+
+
+def test_batches_of_calls_are_refused():
+    """``torch.vmap`` has no rule for operators that change their arguments."""
+    server = Server(2500, [40], 4, 2, 32, 32, 16, torch.bfloat16)
+    server.step([30], packed=False)
+    inputs = [randn(5 + i, 3, 1, 1, 4 if i == 0 else 2, 32, dtype=torch.bfloat16) for i in range(3)]
+    rows = torch.full((1, 1), -1, dtype=torch.int64, device=DEVICE)
+    before = [c.clone() for c in (*server.caches, server.bounds)]
+    where = server.tables, rows, server.lengths
+    for call in (lambda *x: paged.paged_attention_update(*x, *server.caches, *where),
+                 lambda *x: paged.paged_attention_update(*x, *server.caches, *where, key_bounds=server.bounds),
+                 lambda *x: paged.selected_attention_update(*x, *server.caches, server.bounds, *where, count=1)):
+        with pytest.raises(RuntimeError, match="[Bb]atching rule"):
+            torch.vmap(call)(*inputs)
+    for got, want in zip((*server.caches, server.bounds), before):
+        assert torch.equal(got.nan_to_num(7.0), want.nan_to_num(7.0))
